@@ -357,6 +357,79 @@ ODIE_API void odie_hashgrid32_destroy(void* handle);
 ODIE_API int odie_tile_topk_noalloc(const float* prediction, const uint8_t* target, int height, int width, int tile,
                    int k, double* scores, int64_t* chosen, uint8_t* selected, uint64_t stream);
 
+/* ------------------------------------------------------------------------
+ * Rows of routed experts (no reference counterpart).  `dtype` is the element
+ * type of every row: 0 fp16, 1 bf16, 2 fp32.  Rows are contiguous, of any
+ * width; `scratch` is caller-owned device memory of at least the bytes that
+ * the matching _scratch function returns (256-byte aligned; may be NULL for 0
+ * bytes), free for reuse in stream order.  Everything is asynchronous on
+ * `stream` and gives the same bits in every run.  -1 with odie_error() on
+ * invalid arguments.
+ *
+ * odie_sort_rows: n (row, choice) pairs ordered by key (int32 or int64:
+ * key_bytes 4 or 8), pairs of one key in their own order.  offsets
+ * i32[bins + 1]: the pairs with a smaller key; order i32[n]: the pair at each
+ * place, slot i32[n]: the place of each pair.  A key outside [0, bins) drops
+ * its pair: it stands behind the last group, its order is -1 and its slot
+ * ~place.
+ * odie_dispatch: sorted[n * choices][width] from rows[n][width]: the row of
+ * pair i = t * choices + j is weights[i] rows[t] (rows[t] without weights),
+ * zero for a dropped pair.
+ * odie_combine: out[n][width], row t = sum over j of weights[t][j] (1 without
+ * weights) times the row at slot[t][j], dropped pairs left out; fp32, in
+ * ascending j, rounded once.  Also the gradient of odie_dispatch.
+ * odie_combine_backward: d_sorted (as odie_dispatch of d_out; may be NULL) and
+ * d_weights f32[n][choices] = <row at slot, d_out[t]> (0 for a dropped pair;
+ * may be NULL).
+ * ------------------------------------------------------------------------ */
+ODIE_API int64_t odie_sort_rows_scratch(int64_t n, int bins);
+ODIE_API int odie_sort_rows(const void* keys, int key_bytes, int64_t n, int bins, int32_t* order, int32_t* slot,
+                   int32_t* offsets, void* scratch, uint64_t stream);
+ODIE_API int odie_dispatch(const void* rows, int64_t n, int choices, int64_t width, int dtype, const int32_t* slot,
+                   const float* weights, void* sorted, uint64_t stream);
+ODIE_API int odie_combine(const void* sorted, int64_t n, int choices, int64_t width, int dtype, const int32_t* slot,
+                   const float* weights, void* out, uint64_t stream);
+ODIE_API int odie_combine_backward(const void* d_out, const void* sorted, int64_t n, int choices, int64_t width, int dtype,
+                   const int32_t* slot, const float* weights, void* d_sorted, float* d_weights, uint64_t stream);
+
+/* ------------------------------------------------------------------------
+ * Linear layer of rows (no reference counterpart): y[rows][outputs] =
+ * residual + act(x W^T + b), x[rows][inputs], W[groups][outputs][inputs],
+ * b[groups][outputs] and residual[rows][outputs] (both may be NULL), all fp16
+ * (dtype 0) or bf16 (1); fp32 sums, one rounding.  offsets i32[groups + 1] on
+ * the device (NULL for one group of all rows; offsets[0] is taken as 0):
+ * group g is rows [offsets[g], offsets[g + 1]); rows behind the last group
+ * give zero rows.  activation: 0 none, 1 ReLU, 2 SiLU, 3 GELU (erf).  slope
+ * (may be NULL) u16[rows][outputs]: act'(x W^T + b) for the backward pass, as
+ * round(2^15 (act' + 1/4)), 65535 for NaN.
+ * odie_linear_backward: with dz = d_y act' (slope NULL: act' = 1), rounded to
+ * the rows' type for the products: d_x = dz W, d_weight = dz^T x, d_bias =
+ * sum of the unrounded dz over the group's rows and d_residual = d_y (each may
+ * be NULL); zero for rows behind the last group and for empty groups.
+ * x, weight, d_y and scratch start on 16-byte boundaries.
+ * ------------------------------------------------------------------------ */
+ODIE_API int64_t odie_linear_scratch(int64_t rows, int inputs, int outputs, int groups);
+ODIE_API int odie_linear(const void* x, const void* weight, const void* bias, const void* residual, int64_t rows, int inputs,
+                   int outputs, int groups, const int32_t* offsets, int dtype, int activation, void* y, uint16_t* slope,
+                   void* scratch, uint64_t stream);
+ODIE_API int64_t odie_linear_backward_scratch(int64_t rows, int inputs, int outputs, int groups);
+ODIE_API int odie_linear_backward(const void* d_y, const uint16_t* slope, const void* x, const void* weight, int64_t rows,
+                   int inputs, int outputs, int groups, const int32_t* offsets, int dtype, void* d_x, void* d_weight,
+                   void* d_bias, void* d_residual, void* scratch, uint64_t stream);
+
+/* ------------------------------------------------------------------------
+ * Learned rows by id (no reference counterpart): out[i] = scale
+ * table[ids[i]] (ids int32 or int64: id_bytes 4 or 8; an id outside
+ * [0, rows) gives a zero row), and the table's gradient: d_table[v] = scale
+ * times the fp32 sum of d_out over the positions of id v in a fixed order,
+ * zero for absent ids.  dtype as for the rows of routed experts.
+ * ------------------------------------------------------------------------ */
+ODIE_API int odie_embed(const void* ids, int id_bytes, int64_t n, const void* table, int64_t rows, int64_t width, int dtype,
+                   float scale, void* out, uint64_t stream);
+ODIE_API int64_t odie_embed_backward_scratch(int64_t n, int64_t rows, int64_t width);
+ODIE_API int odie_embed_backward(const void* ids, int id_bytes, int64_t n, const void* d_out, int64_t rows, int64_t width,
+                   int dtype, float scale, void* d_table, void* scratch, uint64_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -11,6 +11,7 @@ from pathlib import Path
 LIBRARY = Path(__file__).resolve().parent / 'libodie_b200.so'
 
 P, I32, I64, U64, B = C.c_void_p, C.c_int, C.c_int64, C.c_uint64, C.c_bool
+F32 = C.c_float
 
 
 class HashLevel(C.Structure):
@@ -71,6 +72,18 @@ SIGNATURES = {
     'odie_hashgrid32_profile': (I32, [P, I32]),
     'odie_hashgrid32_profile_report': (C.c_char_p, [P]),
     'odie_hashgrid32_destroy': (None, [P]),
+    'odie_sort_rows_scratch': (I64, [I64, I32]),
+    'odie_sort_rows': (I32, [P, I32, I64, I32, P, P, P, P, U64]),
+    'odie_dispatch': (I32, [P, I64, I32, I64, I32, P, P, P, U64]),
+    'odie_combine': (I32, [P, I64, I32, I64, I32, P, P, P, U64]),
+    'odie_combine_backward': (I32, [P, P, I64, I32, I64, I32, P, P, P, P, U64]),
+    'odie_linear_scratch': (I64, [I64, I32, I32, I32]),
+    'odie_linear': (I32, [P, P, P, P, I64, I32, I32, I32, P, I32, I32, P, P, P, U64]),
+    'odie_linear_backward_scratch': (I64, [I64, I32, I32, I32]),
+    'odie_linear_backward': (I32, [P, P, P, P, I64, I32, I32, I32, P, I32, P, P, P, P, P, U64]),
+    'odie_embed': (I32, [P, I32, I64, P, I64, I64, I32, F32, P, U64]),
+    'odie_embed_backward_scratch': (I64, [I64, I64, I64]),
+    'odie_embed_backward': (I32, [P, I32, I64, P, I64, I64, I32, F32, P, P, U64]),
 }
 
 

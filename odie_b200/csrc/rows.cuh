@@ -1,0 +1,105 @@
+// Rows of any width and type, loaded and stored a vector at a time (rows.cu, embed.cu, linear.cu).
+#pragma once
+#include <cuda_bf16.h>
+#include "common.cuh"
+
+namespace odie {
+
+// The element types of the row operators, as the C-ABI numbers them.
+enum RowType : int { ROW_F16 = 0, ROW_BF16 = 1, ROW_F32 = 2 };
+__host__ inline int row_type_size(int dtype) { return dtype == ROW_F32 ? 4 : 2; }
+
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float to_float(float v) { return v; }
+template <typename T>
+__device__ __forceinline__ T from_float(float v);
+template <>
+__device__ __forceinline__ __half from_float<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+template <>
+__device__ __forceinline__ float from_float<float>(float v) { return v; }
+
+template <int BYTES>
+struct Raw;
+template <>
+struct Raw<16> { using type = uint4; };
+template <>
+struct Raw<4> { using type = uint32_t; };
+template <>
+struct Raw<2> { using type = uint16_t; };
+
+// BYTES / sizeof(T) consecutive elements, moved by one load or store.
+template <typename T, int BYTES>
+struct alignas(BYTES) Pack {
+    static constexpr int N = BYTES / int(sizeof(T));
+    T v[N];
+    __device__ __forceinline__ static Pack load(const T* p) {
+        Pack r;
+        *reinterpret_cast<typename Raw<BYTES>::type*>(&r) = __ldg(reinterpret_cast<const typename Raw<BYTES>::type*>(p));
+        return r;
+    }
+    __device__ __forceinline__ static Pack zero() {
+        Pack r;
+        *reinterpret_cast<typename Raw<BYTES>::type*>(&r) = typename Raw<BYTES>::type{};
+        return r;
+    }
+    __device__ __forceinline__ void store(T* p) const {
+        *reinterpret_cast<typename Raw<BYTES>::type*>(p) = *reinterpret_cast<const typename Raw<BYTES>::type*>(this);
+    }
+};
+
+// The widest vector that every row of these buffers starts on: 16 bytes, 4 bytes or one element.
+inline int row_vector(int64_t width, int dtype, const void* a, const void* b = nullptr, const void* c = nullptr) {
+    const int size = row_type_size(dtype);
+    const uintptr_t bits = uintptr_t(a) | uintptr_t(b) | uintptr_t(c) | uintptr_t(width * size);
+    return bits % 16 == 0 ? 16 : bits % 4 == 0 ? 4 : size;
+}
+
+// Calls f(T{}, std::integral_constant<int, BYTES>) for the type and vector width at run time.
+template <typename F>
+void with_row_type(int dtype, int vector, F&& f) {
+    if (dtype == ROW_F32) {
+        if (vector == 16) f(float{}, std::integral_constant<int, 16>{});
+        else f(float{}, std::integral_constant<int, 4>{});
+    } else if (dtype == ROW_BF16) {
+        if (vector == 16) f(__nv_bfloat16{}, std::integral_constant<int, 16>{});
+        else if (vector == 4) f(__nv_bfloat16{}, std::integral_constant<int, 4>{});
+        else f(__nv_bfloat16{}, std::integral_constant<int, 2>{});
+    } else {
+        if (vector == 16) f(__half{}, std::integral_constant<int, 16>{});
+        else if (vector == 4) f(__half{}, std::integral_constant<int, 4>{});
+        else f(__half{}, std::integral_constant<int, 2>{});
+    }
+}
+
+// Threads of a 256-thread block that share one row of `vectors` vectors: the smallest power of two that gives
+// every thread at most four of them (four independent loads in flight), at least 1 and at most 256.
+inline int row_lanes(int64_t vectors) {
+    int lanes = 1;
+    while (lanes < 256 && int64_t(lanes) * 4 < vectors) lanes *= 2;
+    return lanes;
+}
+
+// Sorted (key, index) pairs: sort_pairs (sort.cu).  keys: int32 or int64 (key_bytes 4 or 8), anything outside
+// [0, bins) counts as `bins`.  Writes order[p] = index of the p-th pair by (key, index), and where non-null
+// sorted[p] = its key and slot[i] = its place; for keys outside the range order is -1 and slot ~place.
+// offsets (may be null): i32[bins + 1], the number of pairs with a smaller key.
+struct SortArgs {
+    const void* keys = nullptr;
+    int key_bytes = 4;
+    int64_t n = 0;
+    int bins = 0;
+    int* order = nullptr;
+    uint32_t* sorted = nullptr;
+    int* slot = nullptr;
+    int* offsets = nullptr;
+    void* scratch = nullptr;
+};
+int64_t sort_scratch_bytes(int64_t n, int bins);
+void launch_sort(const SortArgs& a, cudaStream_t stream);
+
+inline void check_row_type(int dtype) { ODIE_REQUIRE(dtype >= 0 && dtype <= 2, "element type must be 0 (fp16), 1 (bf16) or 2 (fp32)"); }
+
+}  // namespace odie
