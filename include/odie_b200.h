@@ -416,6 +416,9 @@ ODIE_API int64_t odie_linear_backward_scratch(int64_t rows, int inputs, int outp
 ODIE_API int odie_linear_backward(const void* d_y, const uint16_t* slope, const void* x, const void* weight, int64_t rows,
                    int inputs, int outputs, int groups, const int32_t* offsets, int dtype, void* d_x, void* d_weight,
                    void* d_bias, void* d_residual, void* scratch, uint64_t stream);
+/* *status (device int32) = 0, or 2 once a bounded wait of the linear kernels on this
+ * device has run out (their results are then incomplete). */
+ODIE_API int odie_linear_status(int32_t* status, uint64_t stream);
 
 /* ------------------------------------------------------------------------
  * Learned rows by id (no reference counterpart): out[i] = scale

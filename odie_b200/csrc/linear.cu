@@ -6,8 +6,15 @@
 // Rows of no group (behind the last offset) give zero rows of y and d x and add to no gradient.  Training keeps
 // act'(z) as a 16-bit fixed-point code (15 fraction bits above -1/4): act' lies in (-0.13, 1.13) for every
 // activation here, so the code is within 2^-16 of it, closer than a 16-bit float of it or of z would be.
+//
+// The three products are one tensor-core kernel (gemm_kernel) with another operand order each; see there.  dz is
+// rounded to the rows' type, because the tensor cores take 16-bit operands; the bias gradient sums it unrounded.
 #include "rows.cuh"
 #include "odie_b200.h"
+#include "tc.cuh"
+#include <cuda.h>
+#include <cudaTypedefs.h>
+#include <algorithm>
 #include <type_traits>
 
 namespace odie {
@@ -15,14 +22,19 @@ namespace {
 
 enum Activation : int { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3 };
 
-// 0xffff is kept for NaN.
-__device__ __forceinline__ uint16_t slope_code(float d) {
-    return d == d ? uint16_t(min(65534.0f, max(0.0f, rintf(fmaf(d, 32768.0f, 8192.0f))))) : uint16_t(0xffff);
-}
-__device__ __forceinline__ float slope_value(uint16_t c) {
-    return c == 0xffff ? __int_as_float(0x7fffffff) : fmaf(float(c), 1.0f / 32768.0f, -0.25f);
+// The slope's code, as the low bits of 2^23 + code (one fused multiply-add rounds to nearest; act' in (-1/4, 7/4)
+// needs no clamp).  A NaN slope is the canonical NaN, whose low 16 bits are 0xffff.
+__device__ __forceinline__ uint32_t slope_bits(float d) { return __float_as_uint(fmaf(d, 32768.0f, 8388608.0f + 8192.0f)); }
+__device__ __forceinline__ float slope_value(uint32_t c) {  // c: 16 bits
+    const float d = fmaf(__uint_as_float(0x4b000000u | c), 1.0f / 32768.0f, -256.25f);  // exact
+    return c == 0xffffu ? __int_as_float(0x7fffffff) : d;
 }
 
+// act(z), with act'(z) in slope.
+//   SiLU  p = 1 / (1 + e^-z): z p and p + z p (1 - p).
+//   GELU  z P(z) and P(z) + z e^(-z^2/2) / sqrt(2 pi), P the normal distribution function by Abramowitz and
+//         Stegun 7.1.26: erfc(u) = (a1 t + .. + a5 t^5) e^(-u^2), t = 1 / (1 + 0.3275911 u), u = |z| / sqrt 2, off
+//         by at most 1.5e-7 absolutely; it shares the slope's exponential.
 template <int ACT>
 __device__ __forceinline__ float activate(float z, float& slope) {
     if (ACT == ACT_RELU) {
@@ -30,13 +42,18 @@ __device__ __forceinline__ float activate(float z, float& slope) {
         return z > 0.0f || z != z ? z : 0.0f;
     }
     if (ACT == ACT_SILU) {
-        const float p = 1.0f / (1.0f + __expf(-z));
-        slope = p * (1.0f + z * (1.0f - p));
-        return z * p;
+        const float p = __fdividef(1.0f, 1.0f + __expf(-z));
+        const float a = z * p;
+        slope = fmaf(a, 1.0f - p, p);
+        return a;
     }
     if (ACT == ACT_GELU) {
-        const float p = 0.5f * (1.0f + erff(z * 0.70710678118654752f));
-        slope = p + z * __expf(-0.5f * z * z) * 0.39894228040143268f;
+        const float e = __expf(-0.5f * z * z);
+        const float t = __fdividef(1.0f, fmaf(fabsf(z), 0.3275911f * 0.70710678118654752f, 1.0f));
+        const float q = 0.5f * t * e *
+                        fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+        const float p = z < 0.0f ? q : 1.0f - q;
+        slope = fmaf(z * 0.39894228040143268f, e, p);
         return z * p;
     }
     slope = 1.0f;
@@ -44,132 +61,710 @@ __device__ __forceinline__ float activate(float z, float& slope) {
 }
 
 // Rows [begin, end) of group g: offsets clamped to [0, rows], so no offset reads or writes out of range.
+__device__ __forceinline__ long long clamp_offset(long long offset, long long rows) { return min(rows, max(0ll, offset)); }
 __device__ __forceinline__ void group_rows(const int* offsets, int g, long long rows, long long& begin, long long& end) {
     if (!offsets) {
         begin = 0;
         end = rows;
         return;
     }
-    begin = g == 0 ? 0 : min(rows, max(0ll, (long long)offsets[g]));
-    end = max(begin, min(rows, max(0ll, (long long)offsets[g + 1])));
+    begin = g == 0 ? 0 : clamp_offset(offsets[g], rows);
+    end = max(begin, clamp_offset(offsets[g + 1], rows));
 }
 
-// C[m][n] = sum_k A(m, k) B(n, k) with element strides.
-struct Product {
-    const void* a;
-    const void* b;
-    long long a_m, a_k, b_n, b_k, b_group, c_group;
-    long long rows;     // of all groups
-    int m, n, k;        // of dW: m = outputs, n = inputs; of y, dX: m unused
+// ---------------------------------------------------------------- the tensor-core product
+//
+// C = A B^T over tiles of 128 CG x BN, K in blocks of 64, by CG CTAs of an SM pair (CG = 2: tcgen05 cta_group::2,
+// each CTA holding its 128 rows of A and half of B's rows; 256 x 256 tiles, twice the arithmetic per byte of
+// shared memory) or one (CG = 1: 128 x 128 and 128 x 64 tiles for fewer rows or columns).
+//
+//   FWD  A = x [rows][inputs] (K-major), B = W_g [outputs][inputs] (K-major), K = inputs
+//   DX   A = dz [rows][outputs] (K-major), B = W_g read along its columns (MN-major), K = outputs
+//   DW   A = dz, B = x read along their columns (both MN-major), K = the group's rows; C = d W_g
+//
+// One warp loads (TMA, 128-byte swizzle, STAGES blocks in flight), one thread multiplies into one of two TMEM
+// accumulators, eight warps take the other one to global memory with bias, activation, residual and slope, so
+// that the epilogue of one tile runs beside the products of the next.  Persistent: CTA (pair) i takes tiles i,
+// i + grid, ...  Rows of other groups that a tile loads are never stored (FWD, DX); for DW, whose sum runs over
+// the rows, each group has its own tensor maps that end at the group's last row, and the hardware reads zeros
+// behind it.
+enum Mode : int { FWD = 0, DX = 1, DW = 2 };
+
+constexpr int BK = 64;
+constexpr int GEMM_THREADS = 384, EPILOGUE_WARP = 4, EPILOGUE_WARPS = 8;
+constexpr uint32_t WAIT_LIMIT = 1u << 22;
+constexpr int STAGING = 2048;  // bytes per epilogue warp: 32 rows x 32 columns of 16 bits
+
+struct GemmArgs {
     int groups;
-    const int* offsets;
-    bool reduce_rows;   // k runs over the group's rows (dW)
+    const int* offsets;  // null: one group of all rows
+    long long rows;
+    int m;               // DW: outputs (rows of d W)
+    int n;               // columns of C
+    int k;               // FWD, DX: length of the sum
+    int chunk;           // DW: rows per unit of work (a multiple of BK)
+    void* out;
+    const void* bias;
+    const void* residual;
+    uint16_t* slope;
+    int activation;
+    float* partial;      // DW with several units per tile: [unit][m][n] sums, joined by join_kernel
+    const CUtensorMap* group_maps;  // DW with offsets: [groups][2]
+    int* error;
 };
 
-template <typename T, typename Out>
-__global__ void __launch_bounds__(256) product_kernel(Product p, Out out) {
-    __shared__ float as[16][65], bs[16][65];
-    const T* a = static_cast<const T*>(p.a);
-    const T* b = static_cast<const T*>(p.b);
-    const int g = blockIdx.z, tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    long long begin, end;
-    if (g < p.groups) group_rows(p.offsets, g, p.rows, begin, end);
-    else {  // the rows of no group
-        long long from;
-        group_rows(p.offsets, p.groups - 1, p.rows, from, begin);
-        end = p.rows;
+template <int CG, int BN>
+struct Shape {
+    static constexpr int TM = 128 * CG;
+    static constexpr int B_ROWS = BN / CG;  // per CTA
+    static constexpr int A_BYTES = 128 * 128, B_BYTES = B_ROWS * 128, STAGE = A_BYTES + B_BYTES;
+    static constexpr int STAGES = 6;
+    static constexpr int COLUMNS = 2 * BN;  // TMEM: two accumulators
+    static constexpr int HEAD = 1024;       // barriers, TMEM address
+    static int bytes(int groups) {
+        return 1024 + STAGES * STAGE + EPILOGUE_WARPS * (STAGING + 128) + HEAD + (2 * (groups + 2)) * 4;
     }
-    const bool nothing = g >= p.groups;
-    const long long m_count = p.reduce_rows ? p.m : end - begin, k_count = nothing ? 0 : p.reduce_rows ? end - begin : p.k;
-    const long long m_base = p.reduce_rows ? 0 : begin, k_base = p.reduce_rows ? begin : 0;
-    const int n0 = blockIdx.x * 64;
-    if (!nothing) b += p.reduce_rows ? 0 : g * p.b_group;
-    for (long long m0 = (long long)blockIdx.y * 64; m0 < m_count; m0 += (long long)gridDim.y * 64) {
-        float acc[4][4] = {};
-        for (long long k0 = 0; k0 < k_count; k0 += 16) {
-            for (int i = threadIdx.x; i < 1024; i += 256) {
-                const int kk = i & 15, r = i >> 4;
-                as[kk][r] = m0 + r < m_count && k0 + kk < k_count
-                                ? to_float(a[(m_base + m0 + r) * p.a_m + (k_base + k0 + kk) * p.a_k]) : 0.0f;
-                bs[kk][r] = n0 + r < p.n && k0 + kk < k_count
-                                ? to_float(b[(long long)(n0 + r) * p.b_n + (k_base + k0 + kk) * p.b_k]) : 0.0f;
-            }
-            __syncthreads();
+};
+
+struct Tile {
+    int g;
+    int m0, n0;          // first row (FWD, DX: global row; DW: output) of the tile and first column
+    int m_end;           // rows from here on are not stored
+    int k0, k_blocks;    // DW: first row of the sum; blocks of 64
+    int unit;            // DW: index of the partial sum
+    bool zero;           // nothing to sum: zeros are stored
+};
+
+template <int MODE, int CG, int BN>
+__device__ __forceinline__ Tile tile_at(const GemmArgs& p, const int* begin, const int* first, int t) {
+    constexpr int TM = 128 * CG;
+    constexpr int BAND = 16;  // row tiles walked together, so that a W tile serves them from L2
+    Tile tile;
+    const int nt = (p.n + BN - 1) / BN;
+    int key = t, inside = 0;
+    if (MODE == DW) {
+        const int per = nt * ((p.m + TM - 1) / TM);
+        key = t / per;
+        inside = t % per;
+    }
+    int lo = 0, hi = p.groups;  // first[lo] <= key < first[hi + 1]
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (first[mid] <= key) lo = mid;
+        else hi = mid - 1;
+    }
+    tile.g = lo;
+    const int from = begin[lo], to = lo < p.groups ? begin[lo + 1] : int(p.rows);
+    int local = key - first[lo];
+    tile.unit = key;
+    if (MODE == DW) {
+        tile.k0 = from + local * p.chunk;
+        const int rows = max(0, min(to - tile.k0, p.chunk));
+        tile.k_blocks = (rows + BK - 1) / BK;
+        tile.zero = rows == 0;
+        tile.n0 = (inside % nt) * BN;
+        tile.m0 = (inside / nt) * TM;
+        tile.m_end = p.m;
+    } else {
+        const int mt = (to - from + TM - 1) / TM;
+        const int band = local / (BAND * nt), height = min(BAND, mt - band * BAND);
+        local -= band * BAND * nt;
+        tile.m0 = from + (band * BAND + local % height) * TM;
+        tile.n0 = (local / height) * BN;
+        tile.m_end = to;
+        tile.k0 = 0;
+        tile.k_blocks = (p.k + BK - 1) / BK;
+        tile.zero = lo == p.groups;
+    }
+    return tile;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
+    uint32_t r;
+    if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack_pair(uint32_t v) {
+    if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&v));
+    else return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+
+// The staging tile of an epilogue warp: 32 rows of 64 bytes, the 16-byte units of a row permuted so that both a
+// thread per row and four threads per row meet no bank twice.
+__device__ __forceinline__ uint4* staged(char* base, int row, int unit) {
+    return reinterpret_cast<uint4*>(base + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4));
+}
+
+// 32 rows x 32 columns of a row-major 16-bit matrix between global memory and registers: thread (lane) holds the
+// 16-byte unit lane % 4 of rows lane / 4 + 8 i.
+struct Window {
+    long long ld;
+    int rows, columns;  // inside the matrix
+    bool wide;          // 16-byte accesses
+};
+__device__ __forceinline__ void window_load(const uint16_t* at, const Window& w, int lane, uint4 (&v)[4]) {
 #pragma unroll
-            for (int kk = 0; kk < 16; ++kk)
+    for (int i = 0; i < 4; ++i) {
+        const int r = lane / 4 + 8 * i, c = (lane & 3) * 8;
+        v[i] = make_uint4(0, 0, 0, 0);
+        if (r >= w.rows || c >= w.columns) continue;
+        const uint16_t* from = at + r * w.ld + c;
+        if (w.wide && c + 8 <= w.columns) {
+            v[i] = __ldg(reinterpret_cast<const uint4*>(from));
+        } else {
+            uint16_t e[8];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(as[kk][ty * 4 + i], bs[kk][tx * 4 + j], acc[i][j]);
-            __syncthreads();
+            for (int j = 0; j < 8; ++j) e[j] = c + j < w.columns ? from[j] : uint16_t(0);
+            v[i] = make_uint4(e[0] | uint32_t(e[1]) << 16, e[2] | uint32_t(e[3]) << 16, e[4] | uint32_t(e[5]) << 16,
+                              e[6] | uint32_t(e[7]) << 16);
         }
+    }
+}
+__device__ __forceinline__ void window_store(uint16_t* at, const Window& w, int lane, const char* staging) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+    for (int i = 0; i < 4; ++i) {
+        const int r = lane / 4 + 8 * i, c = (lane & 3) * 8;
+        if (r >= w.rows || c >= w.columns) continue;
+        const uint4 v = *staged(const_cast<char*>(staging), r, lane & 3);
+        uint16_t* to = at + r * w.ld + c;
+        if (w.wide && c + 8 <= w.columns) {
+            *reinterpret_cast<uint4*>(to) = v;
+        } else {
+            const uint32_t e[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (m0 + ty * 4 + i < m_count && n0 + tx * 4 + j < p.n)
-                    out(g, m_base + m0 + ty * 4 + i, n0 + tx * 4 + j, acc[i][j], nothing);
+            for (int j = 0; j < 8; ++j)
+                if (c + j < w.columns) to[j] = uint16_t(e[j / 2] >> (16 * (j & 1)));
+        }
     }
 }
 
 template <typename T, int ACT>
-struct ForwardOut {
-    const T* bias;
-    const T* residual;
-    T* y;
-    uint16_t* slope;
-    long long n;
-    __device__ void operator()(int g, long long m, int c, float acc, bool nothing) const {
-        float s = 0.0f, v = 0.0f;
-        if (!nothing) {
-            v = activate<ACT>(acc + (bias ? to_float(bias[g * n + c]) : 0.0f), s);
-            if (residual) v += to_float(residual[m * n + c]);
+__device__ __forceinline__ void finish(float (&v)[32], uint32_t (&codes)[16], const float* bias) {
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+        const float4 b = *reinterpret_cast<const float4*>(bias + i);
+        float s[4];
+        v[i] = activate<ACT>(v[i] + b.x, s[0]);
+        v[i + 1] = activate<ACT>(v[i + 1] + b.y, s[1]);
+        v[i + 2] = activate<ACT>(v[i + 2] + b.z, s[2]);
+        v[i + 3] = activate<ACT>(v[i + 3] + b.w, s[3]);
+        codes[i / 2] = __byte_perm(slope_bits(s[0]), slope_bits(s[1]), 0x5410);
+        codes[i / 2 + 1] = __byte_perm(slope_bits(s[2]), slope_bits(s[3]), 0x5410);
+    }
+}
+
+template <typename T, int MODE, int CG, int BN>
+__global__ void __launch_bounds__(GEMM_THREADS, 1)
+    gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GemmArgs p) {
+    using S = Shape<CG, BN>;
+    constexpr int STAGES = S::STAGES;
+    extern __shared__ char raw[];
+    char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) / 1024 * 1024);
+    char* stages = smem;
+    char* staging = stages + STAGES * S::STAGE;
+    float* biases = reinterpret_cast<float*>(staging + EPILOGUE_WARPS * STAGING);
+    uint64_t* full = reinterpret_cast<uint64_t*>(staging + EPILOGUE_WARPS * (STAGING + 128));
+    uint64_t* empty = full + STAGES;
+    uint64_t* done = empty + STAGES;     // [2] accumulator summed
+    uint64_t* drained = done + 2;        // [2] accumulator read out
+    uint64_t* drain = drained + 2;
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drain + 1);
+    int* begin = reinterpret_cast<int*>(reinterpret_cast<char*>(full) + S::HEAD);  // [groups + 2] first row of each group
+    int* first = begin + p.groups + 2;                                            // [groups + 2] first unit
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = CG == 2 ? tc::cluster_rank() : 0;
+    const int nt = (p.n + BN - 1) / BN;
+
+    if (warp == 0 && lane == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            tc::bar_init(full + s, 1);
+            tc::bar_init(empty + s, 1);
         }
-        y[m * n + c] = from_float<T>(v);
-        if (slope) slope[m * n + c] = slope_code(s);
+        for (int a = 0; a < 2; ++a) {
+            tc::bar_init(done + a, 1);
+            tc::bar_init(drained + a, EPILOGUE_WARPS * CG);
+        }
+        tc::bar_init(drain, 1);
+        tc::fence_bar_init();
     }
-};
-template <typename T>
-struct PlainOut {
-    T* c;
-    long long ld, group;
-    __device__ void operator()(int g, long long m, int n, float acc, bool) const { c[g * group + m * ld + n] = from_float<T>(acc); }
-};
-
-template <typename T>
-__global__ void __launch_bounds__(256) dz_kernel(const T* d_y, const uint16_t* slope, T* dz, T* d_residual, long long rows, int n,
-                                                 const int* offsets, int groups) {
-    long long from, live;
-    group_rows(offsets, groups - 1, rows, from, live);
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < rows * n; i += (long long)gridDim.x * 256) {
-        dz[i] = from_float<T>(to_float(d_y[i]) * (slope ? slope_value(slope[i]) : 1.0f));
-        if (d_residual) d_residual[i] = i < live * n ? d_y[i] : from_float<T>(0.0f);
+    if (warp == 2) tc::tmem_alloc_group<CG>(tmem_at, S::COLUMNS);
+    if (warp == 3) {  // the groups' rows and units
+        int units = 0;
+        for (int g0 = 0; g0 <= p.groups; g0 += 32) {
+            const int g = g0 + lane;
+            int count = 0;
+            if (g <= p.groups) {
+                long long from = 0, to = 0;
+                if (g < p.groups) {
+                    group_rows(p.offsets, g, p.rows, from, to);
+                } else {  // the rows of no group
+                    long long b;
+                    group_rows(p.offsets, p.groups - 1, p.rows, b, from);
+                    to = p.rows;
+                }
+                begin[g] = int(from);
+                if (MODE == DW) count = g == p.groups ? 0 : max(1, int((to - from + p.chunk - 1) / p.chunk));
+                else count = int((to - from + S::TM - 1) / S::TM) * nt;
+            }
+            int sum = count;
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) {
+                const int other = __shfl_up_sync(0xffffffffu, sum, d);
+                if (lane >= d) sum += other;
+            }
+            if (g <= p.groups) first[g] = units + sum - count;
+            units += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (lane == 0) first[p.groups + 1] = units;
     }
-}
-
-template <typename T>
-__global__ void __launch_bounds__(256) bias_kernel(const T* d_y, const uint16_t* slope, T* d_bias, long long rows, int n,
-                                                   const int* offsets) {
-    const int g = blockIdx.y, c = blockIdx.x * 32 + (threadIdx.x & 31);
-    __shared__ float part[8][32];
-    long long begin, end;
-    group_rows(offsets, g, rows, begin, end);
-    float sum = 0.0f;
-    if (c < n)
-        for (long long r = begin + (threadIdx.x >> 5); r < end; r += 8)
-            sum += to_float(d_y[r * n + c]) * (slope ? slope_value(slope[r * n + c]) : 1.0f);
-    part[threadIdx.x >> 5][threadIdx.x & 31] = sum;
+    tc::fence_before_sync();
     __syncthreads();
-    if (threadIdx.x < 32 && c < n) {
-        sum = 0.0f;
-        for (int i = 0; i < 8; ++i) sum += part[i][threadIdx.x];
-        d_bias[(long long)g * n + c] = from_float<T>(sum);
+    if (CG == 2) tc::cluster_sync();
+    tc::fence_after_sync();
+    const uint32_t tmem = *tmem_at;
+    const int units = first[p.groups + 1];
+    const int tiles = MODE == DW ? units * nt * ((p.m + S::TM - 1) / S::TM) : units;
+    const int start = int(blockIdx.x) / CG, step = int(gridDim.x) / CG;
+    bool fine = true;
+
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t issued = 0;
+            for (int t = start; t < tiles && fine; t += step) {
+                const Tile tile = tile_at<MODE, CG, BN>(p, begin, first, t);
+                if (tile.zero) continue;
+                const void* ma = &map_a;
+                const void* mb = &map_b;
+                if (MODE == DW && p.group_maps) {
+                    ma = p.group_maps + 2 * tile.g;
+                    mb = p.group_maps + 2 * tile.g + 1;
+                    asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(ma) : "memory");
+                    asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(mb) : "memory");
+                }
+                for (int kb = 0; kb < tile.k_blocks; ++kb, ++issued) {
+                    const int s = issued % STAGES;
+                    fine = tc::bar_wait_cluster(empty + s, ((issued / STAGES) & 1) ^ 1, WAIT_LIMIT);
+                    if (!fine) break;
+                    const uint32_t bar = CG == 2 ? tc::leader_address(full + s) : tc::smem_u32(full + s);
+                    if (rank == 0) tc::bar_expect(full + s, S::STAGE * CG);
+                    char* a = stages + s * S::STAGE;
+                    char* b = a + S::A_BYTES;
+                    const int k = kb * BK, m = tile.m0 + int(rank) * 128, n = tile.n0 + int(rank) * S::B_ROWS;
+                    if (MODE == DW) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) tc::tma_load_2d<CG>(a + i * 8192, ma, m + 64 * i, tile.k0 + k, bar);
+#pragma unroll
+                        for (int i = 0; i < S::B_ROWS / 64; ++i)
+                            tc::tma_load_2d<CG>(b + i * 8192, mb, n + 64 * i, tile.k0 + k, bar);
+                    } else {
+                        tc::tma_load_2d<CG>(a, ma, k, m, bar);
+                        if (MODE == FWD) {
+                            tc::tma_load_3d<CG>(b, mb, k, n, tile.g, bar);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < S::B_ROWS / 64; ++i)
+                                tc::tma_load_3d<CG>(b + i * 8192, mb, n + 64 * i, k, tile.g, bar);
+                        }
+                    }
+                }
+            }
+            // every stage read out: no arrival is on its way when the CTA ends, and no copy (had a wait run out,
+            // the leader waits for its pair's copies here, with a limit)
+            for (uint32_t i = 0; i < STAGES && i < issued; ++i) {
+                const uint32_t last = issued - 1 - i;
+                if (fine) fine = tc::bar_wait_cluster(empty + last % STAGES, (last / STAGES) & 1, WAIT_LIMIT);
+                else if (rank == 0) tc::bar_wait(full + last % STAGES, (last / STAGES) & 1, WAIT_LIMIT);
+            }
+            if (!fine) atomicExch(p.error, 2);
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            constexpr int A_MN = MODE == DW, B_MN = MODE != FWD;
+            constexpr uint32_t ID = std::is_same<T, __half>::value ? tc::idesc(S::TM, BN, A_MN, B_MN) : tc::idesc_bf16(S::TM, BN, A_MN, B_MN);
+            constexpr uint64_t A_STEP = (A_MN ? 2048 : 32) >> 4, B_STEP = (B_MN ? 2048 : 32) >> 4;
+            uint32_t used = 0, summed = 0;
+            for (int t = start; t < tiles && fine; t += step) {
+                const Tile tile = tile_at<MODE, CG, BN>(p, begin, first, t);
+                if (tile.zero) continue;
+                const int acc = summed & 1;
+                fine = tc::bar_wait_cluster(drained + acc, ((summed >> 1) & 1) ^ 1, WAIT_LIMIT);
+                if (!fine) break;
+                tc::fence_after_sync();
+                for (int kb = 0; kb < tile.k_blocks; ++kb, ++used) {
+                    const int s = used % STAGES;
+                    fine = tc::bar_wait_cluster(full + s, (used / STAGES) & 1, WAIT_LIMIT);
+                    if (!fine) break;
+                    tc::fence_after_sync();
+                    const uint32_t a = tc::smem_u32(stages + s * S::STAGE);
+                    const uint64_t da = tc::sdesc_swizzled(a, A_MN ? 8192 : 16);
+                    const uint64_t db = tc::sdesc_swizzled(a + S::A_BYTES, B_MN ? 8192 : 16);
+#pragma unroll
+                    for (int i = 0; i < BK / 16; ++i)
+                        tc::mma_group<CG>(tmem + acc * BN, da + i * A_STEP, db + i * B_STEP, ID, kb > 0 || i > 0);
+                    tc::commit_group<CG>(empty + s);
+                }
+                if (!fine) break;
+                tc::commit_group<CG>(done + acc);
+                ++summed;
+            }
+            if (!fine) {
+                atomicExch(p.error, 2);
+                tc::commit_group<CG>(drain);
+                tc::bar_wait(drain, 0, WAIT_LIMIT);
+            }
+        }
+    } else if (warp >= EPILOGUE_WARP) {
+        const int quadrant = warp & 3, half = (warp - EPILOGUE_WARP) >> 2;
+        char* stage = staging + (warp - EPILOGUE_WARP) * STAGING;
+        float* bias = biases + (warp - EPILOGUE_WARP) * 32;
+        const uint32_t lanes = tmem + (uint32_t(quadrant * 32) << 16);
+        const bool wide = p.n % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.slope)) % 16 == 0;
+        const bool wide_residual = p.n % 8 == 0 && reinterpret_cast<uintptr_t>(p.residual) % 16 == 0;
+        uint32_t summed = 0;
+        for (int t = start; t < tiles && fine; t += step) {
+            const Tile tile = tile_at<MODE, CG, BN>(p, begin, first, t);
+            const int acc = summed & 1;
+            const int row = tile.m0 + int(rank) * 128 + quadrant * 32;
+            const uint16_t* residual = nullptr;
+            if (MODE == FWD && p.residual && !tile.zero) residual = static_cast<const uint16_t*>(p.residual) + (long long)row * p.n;
+            Window w{p.n, min(32, tile.m_end - row), 0, wide};
+            Window wr{p.n, w.rows, 0, wide_residual};
+            uint4 r[4];
+            if (residual) {  // the first window's residual travels while the sum is awaited
+                wr.columns = p.n - (tile.n0 + half * 32);
+                window_load(residual + tile.n0 + half * 32, wr, lane, r);
+            }
+            if (!tile.zero) {
+                fine = __all_sync(0xffffffffu, tc::bar_wait_cluster(done + acc, (summed >> 1) & 1, WAIT_LIMIT));
+                if (!fine) break;
+                tc::fence_after_sync();
+            }
+#pragma unroll 1
+            for (int c = half; c < BN / 32; c += 2) {
+                const int column = tile.n0 + c * 32;
+                w.columns = p.n - column;
+                if (w.columns <= 0) break;
+                float v[32];
+                uint32_t codes[16];
+                if (tile.zero) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) v[i] = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) codes[i] = 0;
+                } else {
+                    tc::tmem_ld32(lanes + acc * BN + c * 32, v);
+                }
+                if (MODE == DW && p.partial) {
+                    if (lane < w.rows) {
+                        float* to = p.partial + ((long long)tile.unit * p.m + row + lane) * p.n + column;
+                        if (p.n % 4 == 0) {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4)
+                                if (i < w.columns) *reinterpret_cast<float4*>(to + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i)
+                                if (i < w.columns) to[i] = v[i];
+                        }
+                    }
+                    continue;
+                }
+                if (MODE == FWD && !tile.zero) {
+                    bias[lane] = p.bias && lane < w.columns
+                                     ? to_float(static_cast<const T*>(p.bias)[(long long)tile.g * p.n + column + lane]) : 0.0f;
+                    if (residual) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) *staged(stage, lane / 4 + 8 * i, lane & 3) = r[i];
+                    }
+                    __syncwarp();
+                    if (p.activation == ACT_RELU) finish<T, ACT_RELU>(v, codes, bias);
+                    else if (p.activation == ACT_SILU) finish<T, ACT_SILU>(v, codes, bias);
+                    else if (p.activation == ACT_GELU) finish<T, ACT_GELU>(v, codes, bias);
+                    else finish<T, ACT_NONE>(v, codes, bias);
+                    if (residual) {
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            const uint4 q = *staged(stage, lane, u);
+                            const uint32_t e[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float2 f = unpack_pair<T>(e[i]);
+                                v[u * 8 + i * 2] += f.x;
+                                v[u * 8 + i * 2 + 1] += f.y;
+                            }
+                        }
+                        if (c + 2 < BN / 32) {
+                            wr.columns = p.n - (column + 64);
+                            window_load(residual + column + 64, wr, lane, r);
+                        }
+                    }
+                    __syncwarp();
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    *staged(stage, lane, u) = make_uint4(pack_pair<T>(v[u * 8], v[u * 8 + 1]), pack_pair<T>(v[u * 8 + 2], v[u * 8 + 3]),
+                                                         pack_pair<T>(v[u * 8 + 4], v[u * 8 + 5]), pack_pair<T>(v[u * 8 + 6], v[u * 8 + 7]));
+                __syncwarp();
+                const long long group = MODE == DW ? (long long)tile.g * p.m * p.n : 0;
+                window_store(static_cast<uint16_t*>(p.out) + group + (long long)row * p.n + column, w, lane, stage);
+                __syncwarp();
+                if (MODE == FWD && p.slope) {
+#pragma unroll
+                    for (int u = 0; u < 4; ++u)
+                        *staged(stage, lane, u) = make_uint4(codes[u * 4], codes[u * 4 + 1], codes[u * 4 + 2], codes[u * 4 + 3]);
+                    __syncwarp();
+                    window_store(p.slope + (long long)row * p.n + column, w, lane, stage);
+                    __syncwarp();
+                }
+            }
+            if (!tile.zero) {
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) tc::bar_arrive_cluster(CG == 2 ? tc::leader_address(drained + acc) : tc::smem_u32(drained + acc));
+                ++summed;
+            }
+        }
+        if (!fine && lane == 0) atomicExch(p.error, 2);
+    }
+    __syncwarp();
+    tc::fence_before_sync();
+    __syncthreads();
+    if (CG == 2) tc::cluster_sync();
+    tc::fence_after_sync();
+    if (warp == 2) tc::tmem_dealloc_group<CG>(tmem, S::COLUMNS);
+}
+
+// Tensor maps of dz and x that end at each group's last row.
+__global__ void __launch_bounds__(32) group_maps_kernel(const __grid_constant__ CUtensorMap a, const __grid_constant__ CUtensorMap b,
+                                                        const int* offsets, long long rows, CUtensorMap* maps) {
+    __shared__ alignas(128) uint32_t map[32];
+    const int g = blockIdx.x >> 1;
+    const CUtensorMap& from = blockIdx.x & 1 ? b : a;
+    map[threadIdx.x] = reinterpret_cast<const uint32_t*>(&from)[threadIdx.x];
+    __syncwarp();
+    if (threadIdx.x == 0) {
+        long long begin, end;
+        group_rows(offsets, g, rows, begin, end);
+        asm volatile("tensormap.replace.tile.global_dim.shared::cta.b1024.b32 [%0], 1, %1;" ::"r"(tc::smem_u32(map)),
+                     "r"(int(max(1ll, end)))
+                     : "memory");
+    }
+    __syncwarp();
+    asm volatile("tensormap.cp_fenceproxy.global.shared::cta.tensormap::generic.release.gpu.sync.aligned [%0], [%1], 128;" ::"l"(
+                     maps + blockIdx.x),
+                 "r"(tc::smem_u32(map))
+                 : "memory");
+}
+
+// d W from the units' sums, in unit order.
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(const float* partial, T* out, const int* offsets, int groups, long long rows, int chunk,
+                                                   long long size) {
+    const int g = blockIdx.y;
+    long long unit = 0, begin, end;
+    for (int i = 0; i < g; ++i) {
+        group_rows(offsets, i, rows, begin, end);
+        unit += max(1ll, (end - begin + chunk - 1) / chunk);
+    }
+    group_rows(offsets, g, rows, begin, end);
+    const int count = int(max(1ll, (end - begin + chunk - 1) / chunk));
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < size; i += (long long)gridDim.x * 256) {
+        float sum = 0.0f;
+#pragma unroll 8
+        for (int u = 0; u < count; ++u) sum += partial[(unit + u) * size + i];
+        out[g * size + i] = from_float<T>(sum);
     }
 }
+
+// ---------------------------------------------------------------- dz and the bias gradient
+struct DzArgs {
+    const void* d_y;
+    const uint16_t* slope;  // null: 1
+    void* dz;               // null: not wanted
+    void* d_residual;
+    float* partial;         // [row blocks][n] sums of dz, or null
+    void* d_bias;
+    long long rows;
+    int n;
+    long long ld;           // of dz
+    int block_rows;         // rows per block
+    int groups;
+    const int* offsets;
+    bool wide;
+};
+
+template <typename T>
+__device__ __forceinline__ void dz_load(const DzArgs& a, long long row, int column, float (&v)[8], uint4& raw) {
+    const uint16_t* from = static_cast<const uint16_t*>(a.d_y) + row * a.n + column;
+    uint4 s = make_uint4(0, 0, 0, 0);
+    if (a.wide) {
+        raw = __ldg(reinterpret_cast<const uint4*>(from));
+        if (a.slope) s = __ldg(reinterpret_cast<const uint4*>(a.slope + row * a.n + column));
+    } else {
+        uint16_t e[8], f[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            e[j] = column + j < a.n ? from[j] : uint16_t(0);
+            f[j] = a.slope && column + j < a.n ? a.slope[row * a.n + column + j] : uint16_t(0);
+        }
+        raw = make_uint4(e[0] | uint32_t(e[1]) << 16, e[2] | uint32_t(e[3]) << 16, e[4] | uint32_t(e[5]) << 16,
+                         e[6] | uint32_t(e[7]) << 16);
+        s = make_uint4(f[0] | uint32_t(f[1]) << 16, f[2] | uint32_t(f[3]) << 16, f[4] | uint32_t(f[5]) << 16,
+                       f[6] | uint32_t(f[7]) << 16);
+    }
+    const uint32_t y[4] = {raw.x, raw.y, raw.z, raw.w}, c[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack_pair<T>(y[i]);
+        v[2 * i] = a.slope ? f.x * slope_value(c[i] & 0xffffu) : f.x;
+        v[2 * i + 1] = a.slope ? f.y * slope_value(c[i] >> 16) : f.y;
+    }
+}
+
+// A block: block_rows rows x 8 columns per thread of `lanes` threads.  Column sums: each thread over its rows,
+// then over the block's threads in order.
+template <typename T>
+__global__ void __launch_bounds__(256) dz_kernel(DzArgs a, int lanes_log2) {
+    __shared__ float sums[256][9];
+    const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1), line = threadIdx.x >> lanes_log2, lines = 256 >> lanes_log2;
+    const int column = (blockIdx.y * lanes + lane) * 8;
+    const long long from = (long long)blockIdx.x * a.block_rows, to = min(a.rows, from + a.block_rows);
+    long long b, live;
+    group_rows(a.offsets, a.groups - 1, a.rows, b, live);
+    float sum[8] = {};
+    if (column < a.n) {
+#pragma unroll 4
+        for (long long row = from + line; row < to; row += lines) {
+            float v[8];
+            uint4 raw;
+            dz_load<T>(a, row, column, v, raw);
+            if (a.dz)
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.dz) + row * a.ld + column) =
+                    make_uint4(pack_pair<T>(v[0], v[1]), pack_pair<T>(v[2], v[3]), pack_pair<T>(v[4], v[5]), pack_pair<T>(v[6], v[7]));
+            if (a.d_residual) {
+                const bool on = row < live;
+                if (a.wide) {
+                    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.d_residual) + row * a.n + column) = on ? raw : make_uint4(0, 0, 0, 0);
+                } else {
+                    const uint32_t e[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (column + j < a.n)
+                            static_cast<uint16_t*>(a.d_residual)[row * a.n + column + j] = on ? uint16_t(e[j / 2] >> (16 * (j & 1))) : uint16_t(0);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] += v[i];
+        }
+    }
+    if (!a.partial) return;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sums[threadIdx.x][i] = sum[i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < lanes * 8; i += 256) {
+        const int c = i >> 3, e = i & 7, at = (blockIdx.y * lanes + c) * 8 + e;
+        if (at >= a.n) continue;
+        float total = 0.0f;
+        for (int l = 0; l < lines; ++l) total += sums[l * lanes + c][e];
+        a.partial[(long long)blockIdx.x * a.n + at] = total;
+    }
+}
+
+// d b_g: the whole row blocks inside the group from their sums, the rows before and behind them from d y.
+template <typename T>
+__global__ void __launch_bounds__(256) bias_kernel(DzArgs a) {
+    __shared__ float part[8][33];
+    const int g = blockIdx.y, lane = threadIdx.x & 31, line = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
+    long long begin, end;
+    group_rows(a.offsets, g, a.rows, begin, end);
+    const long long r = a.block_rows;
+    long long block = (begin + r - 1) / r;
+    // the last block may be short: it is whole if the group reaches the last row
+    long long last = end == a.rows ? (a.rows + r - 1) / r : end / r;
+    const long long head = min(end, block * r), tail = max(head, min(end, last * r));
+    float sum = 0.0f;
+    if (c < a.n) {
+        const T* d_y = static_cast<const T*>(a.d_y);
+        auto rows = [&](long long from, long long to) {
+#pragma unroll 4
+            for (long long row = from + line; row < to; row += 8) {
+                const float v = to_float(d_y[row * a.n + c]);
+                sum += a.slope ? v * slope_value(a.slope[row * a.n + c]) : v;
+            }
+        };
+        rows(begin, head);
+#pragma unroll 4
+        for (long long i = block + line; i < last; i += 8) sum += a.partial[i * a.n + c];
+        rows(tail, end);
+    }
+    part[line][lane] = sum;
+    __syncthreads();
+    if (line == 0 && c < a.n) {
+        sum = 0.0f;
+        for (int i = 0; i < 8; ++i) sum += part[i][lane];
+        static_cast<T*>(a.d_bias)[(long long)g * a.n + c] = from_float<T>(sum);
+    }
+}
+
+// Rows whose length is no multiple of 16 bytes, copied to ones that are: TMA reads no others.
+__global__ void __launch_bounds__(256) pad_kernel(const uint16_t* from, uint16_t* to, long long rows, int width, int ld) {
+    const long long count = rows * (ld / 8);
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < count; i += (long long)gridDim.x * 256) {
+        const long long row = i / (ld / 8);
+        const int c = int(i % (ld / 8)) * 8;
+        uint16_t e[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) e[j] = c + j < width ? from[row * width + c + j] : uint16_t(0);
+        *reinterpret_cast<uint4*>(to + row * ld + c) = make_uint4(e[0] | uint32_t(e[1]) << 16, e[2] | uint32_t(e[3]) << 16,
+                                                                  e[4] | uint32_t(e[5]) << 16, e[6] | uint32_t(e[7]) << 16);
+    }
+}
+
+// ---------------------------------------------------------------- host
+__device__ int linear_error;
+
+int* error_word() {
+    int* p;
+    ODIE_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&p), linear_error));
+    return p;
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+    static const PFN_cuTensorMapEncodeTiled_v12000 found = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult status;
+        ODIE_CUDA(cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &f, 12000, cudaEnableDefault, &status));
+        ODIE_REQUIRE(f && status == cudaDriverEntryPointSuccess, "the driver has no cuTensorMapEncodeTiled");
+        return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+    }();
+    return found;
+}
+
+// A row-major [depth][rows][width] matrix of 16-bit elements with rows of ld elements; boxes of 64 columns x box_rows.
+CUtensorMap tensor_map(const void* base, bool bf16, int64_t width, int64_t rows, int64_t depth, int64_t ld, int box_rows) {
+    CUtensorMap map;
+    const cuuint64_t dims[3] = {cuuint64_t(width), cuuint64_t(rows), cuuint64_t(std::max<int64_t>(1, depth))};
+    const cuuint64_t strides[2] = {cuuint64_t(ld * 2), cuuint64_t(rows * ld * 2)};
+    const cuuint32_t box[3] = {64, cuuint32_t(box_rows), 1}, unit[3] = {1, 1, 1};
+    ODIE_REQUIRE(uintptr_t(base) % 16 == 0, "x, weight, d_y and scratch must start on 16-byte boundaries");
+    const CUresult status = encoder()(&map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, depth ? 3 : 2,
+                                      const_cast<void*>(base), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    ODIE_REQUIRE(status == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with " + std::to_string(int(status)));
+    return map;
+}
+
+int64_t aligned(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 void check_linear(int64_t rows, int inputs, int outputs, int groups, const int32_t* offsets, int dtype, int activation) {
     ODIE_REQUIRE(dtype == ROW_F16 || dtype == ROW_BF16, "linear takes fp16 (0) or bf16 (1)");
-    ODIE_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31), "0 to 2^31 - 1 rows");
+    ODIE_REQUIRE(rows >= 0 && rows < (int64_t(1) << 31) - 256, "0 to 2^31 - 257 rows");
     ODIE_REQUIRE(inputs >= 1 && outputs >= 1 && inputs <= (1 << 20) && outputs <= (1 << 20), "1 to 2^20 inputs and outputs");
     ODIE_REQUIRE(groups >= 1 && groups <= 1024, "1 to 1024 groups");
     ODIE_REQUIRE(offsets || groups == 1, "more than one group needs offsets");
@@ -182,8 +777,123 @@ void with_linear_type(int dtype, F&& f) {
     else f(__half{});
 }
 
-dim3 product_grid(int64_t m, int64_t n, int groups) {
-    return dim3(unsigned((n + 63) / 64), unsigned(std::min<int64_t>(65535, (m + 63) / 64)), unsigned(groups));
+constexpr int SMS = 148;  // of a B200: the sizes of scratch must not depend on the device that asks
+
+// Tiles of 256 x 256 by SM pairs where they fill the machine, else 128 x 128, or 128 x 64 for 64 columns or fewer.
+struct Config {
+    int cg, bn;
+};
+Config tile_config(int64_t m, int n, int64_t others) {
+    if (n <= 64) return {1, 64};
+    if (ceil_div(m, 256) * ceil_div(n, 256) * others >= SMS / 2) return {2, 256};
+    return {1, 128};
+}
+template <typename F>
+void with_config(Config c, F&& f) {
+    if (c.cg == 2) f(std::integral_constant<int, 2>{}, std::integral_constant<int, 256>{});
+    else if (c.bn == 128) f(std::integral_constant<int, 1>{}, std::integral_constant<int, 128>{});
+    else f(std::integral_constant<int, 1>{}, std::integral_constant<int, 64>{});
+}
+
+template <typename T, int MODE, int CG, int BN>
+void launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmArgs& p, int64_t tiles, cudaStream_t stream) {
+    ODIE_REQUIRE(tiles < (int64_t(1) << 30), "too many rows and columns for one launch");
+    using S = Shape<CG, BN>;
+    const auto kernel = gemm_kernel<T, MODE, CG, BN>;
+    ODIE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes(1024)));
+    const int pairs = int(std::min<int64_t>(tiles, sm_count() / CG));
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(unsigned(pairs * CG));
+    config.blockDim = dim3(GEMM_THREADS);
+    config.dynamicSmemBytes = size_t(S::bytes(p.groups));
+    config.stream = stream;
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = CG;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    config.attrs = &cluster;
+    config.numAttrs = 1;
+    ODIE_CUDA(cudaLaunchKernelEx(&config, kernel, a, b, p));
+    note_launch();
+}
+
+void launch_pad(const void* from, void* to, int64_t rows, int width, cudaStream_t stream) {
+    const int ld = int(round8(width));
+    const int64_t blocks = std::min<int64_t>(ceil_div(rows * (ld / 8), 256), 32 * sm_count());
+    pad_kernel<<<unsigned(blocks), 256, 0, stream>>>(static_cast<const uint16_t*>(from), static_cast<uint16_t*>(to), rows, width, ld);
+    ODIE_CUDA(cudaGetLastError());
+    note_launch();
+}
+
+// Caller-owned scratch, handed out in 256-byte steps.
+struct Scratch {
+    char* at;
+    int64_t used = 0;
+    void* take(int64_t bytes) {
+        char* p = at ? at + used : nullptr;
+        used += aligned(bytes);
+        return p;
+    }
+};
+
+// ---- the pieces of scratch, in order; the size functions walk the same list
+struct ForwardScratch {
+    void *x, *weight;
+    int64_t bytes;
+    ForwardScratch(void* base, int64_t rows, int inputs, int outputs, int groups) {
+        Scratch s{static_cast<char*>(base)};
+        const bool pad = inputs % 8 != 0;
+        x = pad ? s.take(rows * round8(inputs) * 2) : nullptr;
+        weight = pad ? s.take(int64_t(groups) * outputs * round8(inputs) * 2) : nullptr;
+        bytes = s.used;
+    }
+};
+
+// DW: the rows of a unit of work.  Where there are fewer tiles than SMs, the rows are cut so that about two units
+// fall to each.
+struct WeightUnits {
+    Config config;
+    int64_t tiles;  // of one group
+    int64_t chunk, units;
+    bool split;
+    WeightUnits(int64_t rows, int inputs, int outputs, int groups) {
+        config = tile_config(outputs, inputs, groups);
+        tiles = ceil_div(outputs, 128 * config.cg) * ceil_div(inputs, config.bn);
+        const int64_t wanted = 2 * SMS / config.cg, have = tiles * groups;
+        chunk = std::max<int64_t>(BK, ceil_div(rows, BK) * BK);
+        split = have < wanted / 2 && rows > 4 * BK;
+        if (split) chunk = std::max<int64_t>(4 * BK, ceil_div(ceil_div(rows * tiles, wanted), BK) * BK);
+        units = split ? ceil_div(rows, chunk) + groups : groups;  // at most
+    }
+};
+
+int dz_block_rows(int64_t rows, int groups) {
+    // at most about 512 sums for one group; for several, short blocks, since the rows at a group's ends are read twice
+    const int64_t r = groups == 1 ? ceil_div(rows, 512) : ceil_div(rows, int64_t(groups) * 16);
+    return int(std::max<int64_t>(64, ceil_div(r, 64) * 64));
+}
+
+struct BackwardScratch {
+    void *dz, *x, *weight, *maps;
+    float *bias, *partial;
+    int64_t bytes;
+    BackwardScratch(void* base, int64_t rows, int inputs, int outputs, int groups) {
+        Scratch s{static_cast<char*>(base)};
+        const bool pad = inputs % 8 != 0;
+        dz = s.take(rows * round8(outputs) * 2);
+        x = pad ? s.take(rows * round8(inputs) * 2) : nullptr;
+        weight = pad ? s.take(int64_t(groups) * outputs * round8(inputs) * 2) : nullptr;
+        maps = s.take(int64_t(groups) * 2 * sizeof(CUtensorMap));
+        bias = static_cast<float*>(s.take(ceil_div(rows, dz_block_rows(rows, groups)) * outputs * 4));
+        const WeightUnits u(rows, inputs, outputs, groups);
+        partial = static_cast<float*>(u.split ? s.take(u.units * outputs * int64_t(inputs) * 4) : nullptr);
+        bytes = s.used;
+    }
+};
+
+bool sizes_fit(int64_t rows, int inputs, int outputs, int groups) {
+    return rows >= 0 && rows < (int64_t(1) << 31) && inputs >= 1 && outputs >= 1 && inputs <= (1 << 20) && outputs <= (1 << 20) &&
+           groups >= 1 && groups <= 1024;
 }
 
 }  // namespace
@@ -191,7 +901,10 @@ dim3 product_grid(int64_t m, int64_t n, int groups) {
 
 using namespace odie;
 
-extern "C" int64_t odie_linear_scratch(int64_t rows, int inputs, int outputs, int groups) { return 0; }
+extern "C" int64_t odie_linear_scratch(int64_t rows, int inputs, int outputs, int groups) {
+    if (!sizes_fit(rows, inputs, outputs, groups)) return 0;
+    return ForwardScratch(nullptr, rows, inputs, outputs, groups).bytes;
+}
 
 extern "C" int odie_linear(const void* x, const void* weight, const void* bias, const void* residual, int64_t rows, int inputs,
                            int outputs, int groups, const int32_t* offsets, int dtype, int activation, void* y,
@@ -201,26 +914,42 @@ extern "C" int odie_linear(const void* x, const void* weight, const void* bias, 
         if (rows == 0) return;
         ODIE_REQUIRE(x && weight && y, "x, weight and y are required");
         const cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_handle);
-        Product p{x, weight, inputs, 1, inputs, 1, int64_t(outputs) * inputs, 0, rows, 0, outputs, inputs, groups, offsets, false};
+        const ForwardScratch s(scratch, rows, inputs, outputs, groups);
+        ODIE_REQUIRE(scratch || s.bytes == 0, "scratch is required");
+        const int64_t ld = round8(inputs);
+        if (s.x) {
+            launch_pad(x, s.x, rows, inputs, stream);
+            launch_pad(weight, s.weight, int64_t(groups) * outputs, inputs, stream);
+            x = s.x;
+            weight = s.weight;
+        }
+        GemmArgs p{};
+        p.groups = groups;
+        p.offsets = offsets;
+        p.rows = rows;
+        p.n = outputs;
+        p.k = inputs;
+        p.out = y;
+        p.bias = bias;
+        p.residual = residual;
+        p.slope = slope;
+        p.activation = activation;
+        p.error = error_word();
+        const bool bf16 = dtype == ROW_BF16;
         with_linear_type(dtype, [&](auto type) {
-            using T = decltype(type);
-            auto go = [&](auto act) {
-                ForwardOut<T, decltype(act)::value> out{static_cast<const T*>(bias), static_cast<const T*>(residual),
-                                                       static_cast<T*>(y), slope, outputs};
-                product_kernel<T><<<product_grid(rows, outputs, groups + (offsets ? 1 : 0)), 256, 0, stream>>>(p, out);
-            };
-            if (activation == ACT_RELU) go(std::integral_constant<int, ACT_RELU>{});
-            else if (activation == ACT_SILU) go(std::integral_constant<int, ACT_SILU>{});
-            else if (activation == ACT_GELU) go(std::integral_constant<int, ACT_GELU>{});
-            else go(std::integral_constant<int, ACT_NONE>{});
+            with_config(tile_config(ceil_div(rows, groups), outputs, groups), [&](auto cg, auto bn) {
+                constexpr int CG = decltype(cg)::value, BN = decltype(bn)::value;
+                launch_gemm<decltype(type), FWD, CG, BN>(tensor_map(x, bf16, inputs, rows, 0, ld, 128),
+                                                         tensor_map(weight, bf16, inputs, outputs, groups, ld, BN / CG), p,
+                                                         (ceil_div(rows, 128 * CG) + groups + 1) * ceil_div(outputs, BN), stream);
+            });
         });
-        ODIE_CUDA(cudaGetLastError());
-        note_launch();
     });
 }
 
 extern "C" int64_t odie_linear_backward_scratch(int64_t rows, int inputs, int outputs, int groups) {
-    return rows * outputs * 2;
+    if (!sizes_fit(rows, inputs, outputs, groups)) return 0;
+    return BackwardScratch(nullptr, rows, inputs, outputs, groups).bytes;
 }
 
 extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, const void* x, const void* weight, int64_t rows,
@@ -229,33 +958,96 @@ extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, cons
     return guarded([&] {
         check_linear(rows, inputs, outputs, groups, offsets, dtype, ACT_NONE);
         const cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_handle);
-        const int64_t weights = int64_t(groups) * outputs * inputs;
         if (rows == 0) {
-            if (d_weight) ODIE_CUDA(cudaMemsetAsync(d_weight, 0, size_t(weights) * 2, stream));
+            if (d_weight) ODIE_CUDA(cudaMemsetAsync(d_weight, 0, size_t(groups) * outputs * inputs * 2, stream));
             if (d_bias) ODIE_CUDA(cudaMemsetAsync(d_bias, 0, size_t(groups) * outputs * 2, stream));
             return;
         }
         ODIE_REQUIRE(d_y && (x || !d_weight) && (weight || !d_x) && scratch, "d_y, x, weight and scratch are required");
+        const BackwardScratch s(scratch, rows, inputs, outputs, groups);
+        const bool bf16 = dtype == ROW_BF16;
+        const int64_t ld_x = round8(inputs), ld_z = round8(outputs);
+        const bool products = d_x || d_weight;
+        const bool as_is = !slope && outputs % 8 == 0;  // dz is d_y
+        const void* dz = as_is ? d_y : s.dz;
         with_linear_type(dtype, [&](auto type) {
             using T = decltype(type);
-            T* dz = static_cast<T*>(scratch);
-            dz_kernel<T><<<1184, 256, 0, stream>>>(static_cast<const T*>(d_y), slope, dz, static_cast<T*>(d_residual), rows, outputs,
-                                                   offsets, groups);
-            if (d_bias)
-                bias_kernel<T><<<dim3((outputs + 31) / 32, groups), 256, 0, stream>>>(static_cast<const T*>(d_y), slope,
-                                                                                     static_cast<T*>(d_bias), rows, outputs, offsets);
+            if ((products && !as_is) || d_bias || d_residual) {
+                DzArgs a{};
+                a.d_y = d_y;
+                a.slope = slope;
+                a.dz = products && !as_is ? s.dz : nullptr;
+                a.d_residual = d_residual;
+                a.partial = d_bias ? s.bias : nullptr;
+                a.d_bias = d_bias;
+                a.rows = rows;
+                a.n = outputs;
+                a.ld = ld_z;
+                a.block_rows = dz_block_rows(rows, groups);
+                a.groups = groups;
+                a.offsets = offsets;
+                a.wide = outputs % 8 == 0 && (uintptr_t(d_y) | uintptr_t(slope) | uintptr_t(d_residual)) % 16 == 0;
+                int log2 = 0;
+                while (log2 < 5 && (8 << log2) < outputs) ++log2;
+                dz_kernel<T><<<dim3(unsigned(ceil_div(rows, a.block_rows)), unsigned(ceil_div(outputs, 8 << log2))), 256, 0, stream>>>(a, log2);
+                ODIE_CUDA(cudaGetLastError());
+                note_launch();
+                if (d_bias) {
+                    bias_kernel<T><<<dim3(unsigned(ceil_div(outputs, 32)), unsigned(groups)), 256, 0, stream>>>(a);
+                    ODIE_CUDA(cudaGetLastError());
+                    note_launch();
+                }
+            }
+            GemmArgs p{};
+            p.groups = groups;
+            p.offsets = offsets;
+            p.rows = rows;
+            p.n = inputs;
+            p.error = error_word();
             if (d_x) {
-                Product p{dz, weight, outputs, 1, 1, inputs, int64_t(outputs) * inputs, 0, rows, 0, inputs, outputs, groups, offsets, false};
-                product_kernel<T><<<product_grid(rows, inputs, groups + (offsets ? 1 : 0)), 256, 0, stream>>>(
-                    p, PlainOut<T>{static_cast<T*>(d_x), inputs, 0});
+                if (s.weight) launch_pad(weight, s.weight, int64_t(groups) * outputs, inputs, stream);
+                p.k = outputs;
+                p.out = d_x;
+                with_config(tile_config(ceil_div(rows, groups), inputs, groups), [&](auto cg, auto bn) {
+                    constexpr int CG = decltype(cg)::value, BN = decltype(bn)::value;
+                    launch_gemm<T, DX, CG, BN>(tensor_map(dz, bf16, outputs, rows, 0, ld_z, 128),
+                                               tensor_map(s.weight ? s.weight : weight, bf16, inputs, outputs, groups, ld_x, 64), p,
+                                               (ceil_div(rows, 128 * CG) + groups + 1) * ceil_div(inputs, BN), stream);
+                });
             }
             if (d_weight) {
-                Product p{dz, x, 1, outputs, 1, inputs, 0, int64_t(outputs) * inputs, rows, outputs, inputs, 0, groups, offsets, true};
-                product_kernel<T><<<product_grid(outputs, inputs, groups), 256, 0, stream>>>(
-                    p, PlainOut<T>{static_cast<T*>(d_weight), inputs, int64_t(outputs) * inputs});
+                if (s.x) launch_pad(x, s.x, rows, inputs, stream);
+                const WeightUnits u(rows, inputs, outputs, groups);
+                const CUtensorMap a = tensor_map(dz, bf16, outputs, rows, 0, ld_z, 64);
+                const CUtensorMap b = tensor_map(s.x ? s.x : x, bf16, inputs, rows, 0, ld_x, 64);
+                p.m = outputs;
+                p.chunk = int(u.chunk);
+                p.out = d_weight;
+                p.partial = u.split ? s.partial : nullptr;
+                if (offsets) {
+                    group_maps_kernel<<<unsigned(2 * groups), 32, 0, stream>>>(a, b, offsets, rows, static_cast<CUtensorMap*>(s.maps));
+                    ODIE_CUDA(cudaGetLastError());
+                    note_launch();
+                    p.group_maps = static_cast<const CUtensorMap*>(s.maps);
+                }
+                with_config(u.config, [&](auto cg, auto bn) {
+                    launch_gemm<T, DW, decltype(cg)::value, decltype(bn)::value>(a, b, p, u.units * u.tiles, stream);
+                });
+                if (u.split) {
+                    const int64_t size = int64_t(outputs) * inputs;
+                    join_kernel<T><<<dim3(unsigned(std::min<int64_t>(ceil_div(size, 256), 1024)), unsigned(groups)), 256, 0, stream>>>(
+                        s.partial, static_cast<T*>(d_weight), offsets, groups, rows, int(u.chunk), size);
+                    ODIE_CUDA(cudaGetLastError());
+                    note_launch();
+                }
             }
         });
-        ODIE_CUDA(cudaGetLastError());
-        note_launch(1 + (d_bias ? 1 : 0) + (d_x ? 1 : 0) + (d_weight ? 1 : 0));
+    });
+}
+
+extern "C" int odie_linear_status(int32_t* status, uint64_t stream) {
+    return guarded([&] {
+        ODIE_REQUIRE(status, "status is required");
+        ODIE_CUDA(cudaMemcpyAsync(status, error_word(), sizeof(int), cudaMemcpyDeviceToDevice, reinterpret_cast<cudaStream_t>(stream)));
     });
 }

@@ -44,6 +44,35 @@ __host__ __device__ constexpr uint32_t idesc(int M, int N, int a_mn_major, int b
            (uint32_t(M >> 4) << 24);
 }
 
+// Matrices in the 128-byte swizzled layout a TMA load with SWIZZLE_128B leaves: lines of 128 bytes (64 16-bit
+// elements), 8 lines to a swizzle atom of 1024 bytes, atoms on 1024-byte boundaries.
+// K-major (a line holds 64 values of K of one row): 8-row groups 1024 bytes apart; K-step s (16 values) starts
+// 32 s bytes further.
+// MN-major (a line holds 64 rows at one value of K): 8-value groups of K 1024 bytes apart, the next 64 rows `lbo`
+// bytes further; K-step s starts 2048 s bytes further.
+__device__ __forceinline__ uint64_t sdesc_swizzled(uint32_t address, uint32_t lbo) {
+    return sdesc(address, lbo, 1024u) | (uint64_t(2) << 61);
+}
+// Instruction descriptor of kind::f16 with bf16 operands.
+__host__ __device__ constexpr uint32_t idesc_bf16(int M, int N, int a_mn_major, int b_mn_major) {
+    return idesc(M, N, a_mn_major, b_mn_major) | (1u << 7) | (1u << 10);
+}
+
+// D[tmem] (+)= A * B, issued by one thread; CG CTAs (a pair's leader issues for both).
+template <int CG>
+__device__ __forceinline__ void mma_group(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+            "l"(a), "l"(b), "r"(id), "r"(accumulate));
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+            "l"(a), "l"(b), "r"(id), "r"(accumulate));
+}
+
 // D[tmem] (+)= A * B, issued by one thread.
 __device__ __forceinline__ void mma(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
     const uint32_t mask = 0;
@@ -79,6 +108,22 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, uint32_
     return false;
 }
 
+// The same, also ordered after what other CTAs of the cluster did before they arrived.
+__device__ __forceinline__ bool bar_wait_cluster(uint64_t* bar, uint32_t parity, uint32_t limit) {
+    const uint32_t address = smem_u32(bar);
+    for (uint32_t i = 0; i < limit; ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, "
+            "p;\n\t}\n"
+            : "=r"(done)
+            : "r"(address), "r"(parity)
+            : "memory");
+        if (done) return true;
+    }
+    return false;
+}
+
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 __device__ __forceinline__ void fence_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void fence_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
@@ -94,6 +139,92 @@ __device__ __forceinline__ void tmem_relinquish() {
 }
 __device__ __forceinline__ void tmem_dealloc(uint32_t base, uint32_t columns) {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(base), "r"(columns) : "memory");
+}
+
+// The same for a group of CG CTAs, and for a pair the arrival at the barrier in both CTAs.
+template <int CG>
+__device__ __forceinline__ void commit_group(uint64_t* bar) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(
+                smem_u32(bar)),
+            "h"(uint16_t(3))
+            : "memory");
+    else
+        commit(bar);
+}
+template <int CG>
+__device__ __forceinline__ void tmem_alloc_group(uint32_t* dst, uint32_t columns) {
+    if constexpr (CG == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(dst)), "r"(columns)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+    } else {
+        tmem_alloc(dst, columns);
+        tmem_relinquish();
+    }
+}
+template <int CG>
+__device__ __forceinline__ void tmem_dealloc_group(uint32_t base, uint32_t columns) {
+    if constexpr (CG == 2)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(base), "r"(columns) : "memory");
+    else
+        tmem_dealloc(base, columns);
+}
+
+// Cluster helpers: this CTA's rank, the shared::cluster address of CTA 0's copy of a shared variable, and the
+// barrier over all threads of the cluster.
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t leader_address(const void* p) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(smem_u32(p)));
+    return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void bar_arrive_cluster(uint32_t address) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(address) : "memory");
+}
+__device__ __forceinline__ void bar_expect(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+
+// TMA loads of one box into this CTA's shared memory, their bytes counted at `bar` (a shared::cluster address:
+// for a pair the leader's barrier).  No multicast.
+template <int CG>
+__device__ __forceinline__ void tma_load_2d(void* dst, const void* map, int x, int y, uint32_t bar) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(
+                smem_u32(dst)),
+            "l"(map), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n" ::"r"(
+                smem_u32(dst)),
+            "l"(map), "r"(x), "r"(y), "r"(bar)
+            : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void tma_load_3d(void* dst, const void* map, int x, int y, int z, uint32_t bar) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(
+                smem_u32(dst)),
+            "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(
+                smem_u32(dst)),
+            "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+            : "memory");
 }
 
 // 16 consecutive fp32 columns of this thread's TMEM lane (32x32b shape, warp-collective).

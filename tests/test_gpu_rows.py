@@ -301,6 +301,14 @@ def test_linear_gradient_against_differences(cuda, activation):
     assert abs(got - slope) <= allowed
 
 
+def test_linear_waits_never_run_out(cuda):
+    import odie_b200._lib as _lib
+    status = torch.full((1,), -1, dtype=torch.int32, device=cuda)
+    check_linear(linear_case(700, 520, 776, torch.bfloat16, 'gelu'), 'gelu')
+    _lib.check(_lib.library().odie_linear_status(status.data_ptr(), _lib.stream_handle()), 'odie_linear_status')
+    assert status.item() == 0
+
+
 def test_linear_refusals(cuda):
     from odie_b200.experts import linear
     x, w = torch.zeros(4, 8, device=cuda).half(), torch.zeros(16, 8, device=cuda).half()
