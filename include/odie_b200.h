@@ -370,11 +370,11 @@ ODIE_API int odie_tile_topk_noalloc(const float* prediction, const uint8_t* targ
  * key_bytes 4 or 8), pairs of one key in their own order.  offsets
  * i32[bins + 1]: the pairs with a smaller key; order i32[n]: the pair at each
  * place, slot i32[n]: the place of each pair.  A key outside [0, bins) drops
- * its pair: it stands behind the last group, its order is -1 and its slot
+ * its pair: it stands behind the last group, its order is ~pair and its slot
  * ~place.
  * odie_dispatch: sorted[n * choices][width] from rows[n][width]: the row of
- * pair i = t * choices + j is weights[i] rows[t] (rows[t] without weights),
- * zero for a dropped pair.
+ * pair i = t * choices + j stands at its place: weights[i] rows[t] (rows[t]
+ * without weights), zero for a dropped pair.
  * odie_combine: out[n][width], row t = sum over j of weights[t][j] (1 without
  * weights) times the row at slot[t][j], dropped pairs left out; fp32, in
  * ascending j, rounded once.  Also the gradient of odie_dispatch.
@@ -385,12 +385,12 @@ ODIE_API int odie_tile_topk_noalloc(const float* prediction, const uint8_t* targ
 ODIE_API int64_t odie_sort_rows_scratch(int64_t n, int bins);
 ODIE_API int odie_sort_rows(const void* keys, int key_bytes, int64_t n, int bins, int32_t* order, int32_t* slot,
                    int32_t* offsets, void* scratch, uint64_t stream);
-ODIE_API int odie_dispatch(const void* rows, int64_t n, int choices, int64_t width, int dtype, const int32_t* slot,
+ODIE_API int odie_dispatch(const void* rows, int64_t n, int choices, int64_t width, int dtype, const int32_t* order,
                    const float* weights, void* sorted, uint64_t stream);
 ODIE_API int odie_combine(const void* sorted, int64_t n, int choices, int64_t width, int dtype, const int32_t* slot,
                    const float* weights, void* out, uint64_t stream);
 ODIE_API int odie_combine_backward(const void* d_out, const void* sorted, int64_t n, int choices, int64_t width, int dtype,
-                   const int32_t* slot, const float* weights, void* d_sorted, float* d_weights, uint64_t stream);
+                   const int32_t* order, const float* weights, void* d_sorted, float* d_weights, uint64_t stream);
 
 /* ------------------------------------------------------------------------
  * Linear layer of rows (no reference counterpart): y[rows][outputs] =

@@ -4,9 +4,10 @@
 //   dispatch   sorted[slot] = w x[t]             (w = 1 without weights), zero rows for dropped choices
 //   combine    out[t] = sum_j w[t, j] sorted[slot[t, j]], an fp32 chain in ascending j, rounded once
 //   backward   d sorted[slot] = w d out[t], d w[t, j] = <sorted[slot], d out[t]> in fp32
-// The gradient of dispatch is combine without weights.  All are bound by the bytes of the rows: every kernel
-// walks the unsorted side in order, so that a row is read once however many choices it has, and moves whole
-// rows of the sorted side in 16-byte vectors.
+// The gradient of dispatch is combine without weights.  All are bound by the bytes of the rows.  Each kernel walks
+// the side that it writes, so that writes are whole lines in order and only reads are scattered (by row; the
+// unsorted rows that are read once per choice come from L2).  Scattered writes of 64-byte rows took half as long
+// again: 47 us against 31 for 2^20 rows of 32 fp16.
 #include "rows.cuh"
 #include "odie_b200.h"
 #include <type_traits>
@@ -14,150 +15,188 @@
 namespace odie {
 namespace {
 
-constexpr int THREADS = 256;
-
 struct RowArgs {
-    long long n;        // unsorted rows
+    RowShape shape;     // of the side that the kernel walks
+    long long places;   // rows of the sorted side, and (row, choice) pairs
     int choices;
     long long width;    // elements of a row
-    int lanes_log2;     // threads per row
-    const int* slot;    // [n][choices]; negative: dropped, ~slot is its place
+    const int* order;   // [places] pair at each place; negative: dropped, ~order is the pair
+    const int* slot;    // [rows][choices] place of each pair; negative: dropped, ~slot is its place
     const float* weights;
 };
 
-template <typename T, int BYTES>
-__global__ void __launch_bounds__(THREADS) dispatch_kernel(RowArgs a, const T* __restrict__ rows, T* __restrict__ sorted) {
+// Walks the sorted rows: they are written in order, and row order[p] / choices is fetched for each.
+template <typename T, int BYTES, bool NARROW>
+__global__ void __launch_bounds__(ROW_THREADS) dispatch_kernel(RowArgs a, const T* __restrict__ rows, T* __restrict__ sorted) {
     using P = Pack<T, BYTES>;
-    const int lanes = 1 << a.lanes_log2, lane = threadIdx.x & (lanes - 1);
-    const long long t = ((long long)blockIdx.x * THREADS + threadIdx.x) >> a.lanes_log2;
-    if (t >= a.n) return;
-    const long long vectors = a.width / P::N, places = a.n * a.choices;
-    const T* from = rows + t * a.width;
-    for (long long c = lane; c < vectors; c += lanes) {
-        const P v = P::load(from + c * P::N);
-        for (int j = 0; j < a.choices; ++j) {
-            const int s = __ldg(a.slot + t * a.choices + j);
-            const long long place = s < 0 ? ~s : s;
-            if (place >= places) continue;
-            P o = v;
-            if (s < 0) {
-                o = P::zero();
-            } else if (a.weights) {
-                const float w = __ldg(a.weights + t * a.choices + j);
+    constexpr int ITEMS = 4;
+    const RowWalk<NARROW, ITEMS> walk(a.shape);
+    long long row[ITEMS];
+    float w[ITEMS];
+    bool kept[ITEMS];
 #pragma unroll
-                for (int i = 0; i < P::N; ++i) o.v[i] = from_float<T>(w * to_float(v.v[i]));
+    for (int q = 0; q < ITEMS; ++q) {
+        const int i = walk.row_of(q) < walk.rows ? __ldg(a.order + walk.row_of(q)) : -1;
+        kept[q] = i >= 0 && i < a.places;
+        row[q] = kept[q] ? i / a.choices : 0;
+        w[q] = kept[q] && a.weights ? __ldg(a.weights + i) : 1.0f;
+    }
+    for (long long c = walk.lane; c < walk.vectors; c += walk.stride()) {
+        P v[ITEMS];
+#pragma unroll
+        for (int q = 0; q < ITEMS; ++q)
+            v[q] = P::load(rows + row[q] * a.width + (walk.vector_of(c, q) < walk.vectors ? walk.vector_of(c, q) : 0) * P::N);
+#pragma unroll
+        for (int q = 0; q < ITEMS; ++q) {
+            P o = kept[q] ? v[q] : P::zero();
+            if (a.weights && kept[q]) {
+#pragma unroll
+                for (int i = 0; i < P::N; ++i) o.v[i] = from_float<T>(w[q] * to_float(v[q].v[i]));
             }
-            o.store(sorted + place * a.width + c * P::N);
+            if (walk.on(c, q)) o.store(sorted + walk.row_of(q) * a.width + walk.vector_of(c, q) * P::N);
         }
     }
 }
 
-template <typename T, int BYTES>
-__global__ void __launch_bounds__(THREADS) combine_kernel(RowArgs a, const T* __restrict__ sorted, T* __restrict__ out) {
+// BATCH choices of ITEMS vectors are loaded together (dropped ones as the first row, and left out of the sum): one
+// choice takes four vectors, two take two, and more take four choices of one.
+template <typename T, int BYTES, bool NARROW, int BATCH>
+__global__ void __launch_bounds__(ROW_THREADS) combine_kernel(RowArgs a, const T* __restrict__ sorted, T* __restrict__ out) {
     using P = Pack<T, BYTES>;
-    constexpr int BATCH = 4;  // choices whose rows are loaded together
-    const int lanes = 1 << a.lanes_log2, lane = threadIdx.x & (lanes - 1);
-    const long long t = ((long long)blockIdx.x * THREADS + threadIdx.x) >> a.lanes_log2;
-    if (t >= a.n) return;
-    const long long vectors = a.width / P::N, places = a.n * a.choices;
-    for (long long c = lane; c < vectors; c += lanes) {
-        float sum[P::N] = {};
+    constexpr int ITEMS = 4 / BATCH;
+    const RowWalk<NARROW, ITEMS> walk(a.shape);
+    for (long long c = walk.lane; c < walk.vectors; c += walk.stride()) {
+        float sum[ITEMS][P::N];
+#pragma unroll
+        for (int q = 0; q < ITEMS; ++q)
+#pragma unroll
+            for (int i = 0; i < P::N; ++i) sum[q][i] = 0.0f;
         for (int j0 = 0; j0 < a.choices; j0 += BATCH) {
-            P v[BATCH];
-            float w[BATCH];
-            bool on[BATCH];
+            P v[ITEMS][BATCH];
+            float w[ITEMS][BATCH];
+            bool on[ITEMS][BATCH];
+            int s[ITEMS][BATCH];
 #pragma unroll
-            for (int b = 0; b < BATCH; ++b) {
-                const int j = j0 + b;
-                const int s = j < a.choices ? __ldg(a.slot + t * a.choices + j) : -1;
-                on[b] = s >= 0 && s < places;
-                if (on[b]) {
-                    v[b] = P::load(sorted + s * a.width + c * P::N);
-                    w[b] = a.weights ? __ldg(a.weights + t * a.choices + j) : 1.0f;
+            for (int q = 0; q < ITEMS; ++q)
+#pragma unroll
+                for (int b = 0; b < BATCH; ++b) {
+                    const bool inside = walk.on(c, q) && j0 + b < a.choices;
+                    const long long pair = inside ? walk.row_of(q) * a.choices + j0 + b : 0;
+                    s[q][b] = __ldg(a.slot + pair);
+                    w[q][b] = a.weights ? __ldg(a.weights + pair) : 1.0f;
+                    on[q][b] = inside && s[q][b] >= 0 && s[q][b] < a.places;
                 }
-            }
 #pragma unroll
-            for (int b = 0; b < BATCH; ++b)
-                if (on[b]) {
+            for (int q = 0; q < ITEMS; ++q)
 #pragma unroll
-                    for (int i = 0; i < P::N; ++i) sum[i] = fmaf(w[b], to_float(v[b].v[i]), sum[i]);
+                for (int b = 0; b < BATCH; ++b) {
+                    const long long place = on[q][b] ? s[q][b] : 0, at = walk.vector_of(c, q);
+                    v[q][b] = P::load(sorted + place * a.width + (at < walk.vectors ? at : 0) * P::N);
                 }
+#pragma unroll
+            for (int q = 0; q < ITEMS; ++q)
+#pragma unroll
+                for (int b = 0; b < BATCH; ++b)
+#pragma unroll
+                    for (int i = 0; i < P::N; ++i) {
+                        const float next = fmaf(w[q][b], to_float(v[q][b].v[i]), sum[q][i]);
+                        sum[q][i] = on[q][b] ? next : sum[q][i];
+                    }
         }
-        P o;
 #pragma unroll
-        for (int i = 0; i < P::N; ++i) o.v[i] = from_float<T>(sum[i]);
-        o.store(out + t * a.width + c * P::N);
+        for (int q = 0; q < ITEMS; ++q) {
+            P o;
+#pragma unroll
+            for (int i = 0; i < P::N; ++i) o.v[i] = from_float<T>(sum[q][i]);
+            if (walk.on(c, q)) o.store(out + walk.row_of(q) * a.width + walk.vector_of(c, q) * P::N);
+        }
     }
 }
 
-// A row's threads per (row, choice).  The dot product's partial sums are joined in a fixed tree.
-template <typename T, int BYTES>
-__global__ void __launch_bounds__(THREADS) combine_backward_kernel(RowArgs a, const T* __restrict__ d_out,
-                                                                   const T* __restrict__ sorted, T* __restrict__ d_sorted,
-                                                                   float* __restrict__ d_weights) {
+// Walks the sorted rows.  The dot product's partial sums are joined in a fixed tree.
+template <typename T, int BYTES, bool NARROW>
+__global__ void __launch_bounds__(ROW_THREADS) combine_backward_kernel(RowArgs a, const T* __restrict__ d_out,
+                                                                       const T* __restrict__ sorted, T* __restrict__ d_sorted,
+                                                                       float* __restrict__ d_weights) {
     using P = Pack<T, BYTES>;
-    __shared__ float partial[THREADS / 32];
-    const int lanes = 1 << a.lanes_log2, lane = threadIdx.x & (lanes - 1);
-    const long long pair = ((long long)blockIdx.x * THREADS + threadIdx.x) >> a.lanes_log2;
-    const long long places = a.n * a.choices, vectors = a.width / P::N;
-    const bool live = pair < places;
-    const int s = live ? __ldg(a.slot + pair) : 0;
-    const long long place = s < 0 ? ~s : s;
-    const bool inside = live && place < places;
-    float dot = 0.0f;
-    if (inside) {
-        const long long t = pair / a.choices;
-        const float w = a.weights ? __ldg(a.weights + pair) : 1.0f;
-        for (long long c = lane; c < vectors; c += lanes) {
-            P o = P::zero();
-            if (s >= 0) {
-                const P g = P::load(d_out + t * a.width + c * P::N);
+    constexpr int ITEMS = 2;
+    __shared__ float partial[ROW_THREADS / 32];
+    const RowWalk<NARROW, ITEMS> walk(a.shape);
+    long long place[ITEMS], row[ITEMS], pair[ITEMS];
+    float w[ITEMS], dot[ITEMS];
+    bool kept[ITEMS];
 #pragma unroll
-                for (int i = 0; i < P::N; ++i) o.v[i] = from_float<T>(w * to_float(g.v[i]));
-                if (d_weights) {
-                    const P y = P::load(sorted + place * a.width + c * P::N);
-                    float part = 0.0f;
+    for (int q = 0; q < ITEMS; ++q) {
+        place[q] = walk.row_of(q) < walk.rows ? walk.row_of(q) : 0;
+        const int i = __ldg(a.order + place[q]);
+        pair[q] = i < 0 ? ~i : i;
+        kept[q] = i >= 0 && i < a.places;
+        row[q] = kept[q] ? i / a.choices : 0;
+        w[q] = kept[q] && a.weights ? __ldg(a.weights + i) : 1.0f;
+        dot[q] = 0.0f;
+    }
+    for (long long c = walk.lane; c < walk.vectors; c += walk.stride()) {
+        P g[ITEMS], y[ITEMS];
 #pragma unroll
-                    for (int i = 0; i < P::N; ++i) part = fmaf(to_float(y.v[i]), to_float(g.v[i]), part);
-                    dot += part;
-                }
+        for (int q = 0; q < ITEMS; ++q) {
+            const long long at = (walk.vector_of(c, q) < walk.vectors ? walk.vector_of(c, q) : 0) * P::N;
+            g[q] = P::load(d_out + row[q] * a.width + at);
+            if (d_weights) y[q] = P::load(sorted + place[q] * a.width + at);
+        }
+#pragma unroll
+        for (int q = 0; q < ITEMS; ++q) {
+            const bool on = walk.on(c, q);
+            if (d_weights) {
+                float part = 0.0f;
+#pragma unroll
+                for (int i = 0; i < P::N; ++i) part = fmaf(to_float(y[q].v[i]), to_float(g[q].v[i]), part);
+                const int to = NARROW ? q : 0;
+                dot[to] = kept[q] && on ? dot[to] + part : dot[to];
             }
-            if (d_sorted) o.store(d_sorted + place * a.width + c * P::N);
+            if (d_sorted && on) {
+                P o = P::zero();
+                if (kept[q]) {
+#pragma unroll
+                    for (int i = 0; i < P::N; ++i) o.v[i] = from_float<T>(w[q] * to_float(g[q].v[i]));
+                }
+                o.store(d_sorted + place[q] * a.width + walk.vector_of(c, q) * P::N);
+            }
         }
     }
     if (!d_weights) return;
 #pragma unroll
-    for (int d = 16; d > 0; d /= 2)
-        if (d < lanes) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-    if (lanes > 32) {
-        if ((threadIdx.x & 31) == 0) partial[threadIdx.x >> 5] = dot;
-        __syncthreads();
-        if (lane == 0) {
-            dot = 0.0f;
-            for (int w = 0; w < lanes / 32; ++w) dot += partial[(threadIdx.x >> 5) + w];
+    for (int q = 0; q < (NARROW ? ITEMS : 1); ++q) {
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) {
+            const float other = __shfl_xor_sync(0xffffffffu, dot[q], d);
+            if (d < walk.lanes) dot[q] += other;
         }
+        if (!NARROW && walk.lanes > 32) {
+            if ((threadIdx.x & 31) == 0) partial[threadIdx.x >> 5] = dot[q];
+            __syncthreads();
+            if (walk.lane == 0) {
+                dot[q] = 0.0f;
+                for (int i = 0; i < walk.lanes / 32; ++i) dot[q] += partial[(threadIdx.x >> 5) + i];
+            }
+        }
+        if (walk.lane == 0 && walk.row_of(q) < walk.rows && pair[q] < a.places) d_weights[pair[q]] = kept[q] ? dot[q] : 0.0f;
     }
-    if (live && lane == 0) d_weights[pair] = inside && s >= 0 ? dot : 0.0f;
 }
 
-RowArgs row_args(int64_t n, int choices, int64_t width, int dtype, const int32_t* slot, const float* weights, int vector) {
-    RowArgs a{n, choices, width, 0, slot, weights};
-    const int lanes = row_lanes(width * row_type_size(dtype) / vector);
-    while ((1 << a.lanes_log2) < lanes) ++a.lanes_log2;
-    return a;
-}
-
-void check_rows(int64_t n, int choices, int64_t width, int dtype, const int32_t* slot) {
+void check_rows(int64_t n, int choices, int64_t width, int dtype, const int32_t* order, const char* name) {
     check_row_type(dtype);
     ODIE_REQUIRE(n >= 0 && choices >= 1 && n < (int64_t(1) << 31) / choices, "0 to 2^31 - 1 (row, choice) pairs");
     ODIE_REQUIRE(width >= 1 && width <= (int64_t(1) << 31), "rows have 1 to 2^31 elements");
-    ODIE_REQUIRE(n == 0 || slot, "slot is required");
+    ODIE_REQUIRE(n == 0 || order, std::string(name) + " is required");
 }
 
-unsigned row_blocks(int64_t rows, const RowArgs& a) {
-    const int64_t blocks = ((rows << a.lanes_log2) + THREADS - 1) / THREADS;
-    ODIE_REQUIRE(blocks < (int64_t(1) << 31), "too many rows for one launch");
-    return unsigned(blocks);
+// f(T{}, integral_constant<int, BYTES>, bool_constant<NARROW>)
+template <typename F>
+void with_rows(int dtype, int vector, bool narrow, F&& f) {
+    with_row_type(dtype, vector, [&](auto type, auto bytes) {
+        if (narrow) f(type, bytes, std::true_type{});
+        else f(type, bytes, std::false_type{});
+    });
 }
 
 }  // namespace
@@ -165,18 +204,19 @@ unsigned row_blocks(int64_t rows, const RowArgs& a) {
 
 using namespace odie;
 
-extern "C" int odie_dispatch(const void* rows, int64_t n, int choices, int64_t width, int dtype, const int32_t* slot,
+extern "C" int odie_dispatch(const void* rows, int64_t n, int choices, int64_t width, int dtype, const int32_t* order,
                              const float* weights, void* sorted, uint64_t stream) {
     return guarded([&] {
-        check_rows(n, choices, width, dtype, slot);
+        check_rows(n, choices, width, dtype, order, "order");
         if (n == 0) return;
         ODIE_REQUIRE(rows && sorted, "rows and sorted are required");
         const int vector = row_vector(width, dtype, rows, sorted);
-        const RowArgs a = row_args(n, choices, width, dtype, slot, weights, vector);
-        with_row_type(dtype, vector, [&](auto type, auto bytes) {
+        const RowArgs a{row_shape(n * choices, width * row_type_size(dtype) / vector), n * choices, choices, width, order, nullptr, weights};
+        with_rows(dtype, vector, a.shape.narrow, [&](auto type, auto bytes, auto narrow) {
             using T = decltype(type);
-            dispatch_kernel<T, decltype(bytes)::value><<<row_blocks(n, a), THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-                a, static_cast<const T*>(rows), static_cast<T*>(sorted));
+            dispatch_kernel<T, decltype(bytes)::value, decltype(narrow)::value>
+                <<<row_blocks(a.shape, 4), ROW_THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+                    a, static_cast<const T*>(rows), static_cast<T*>(sorted));
         });
         ODIE_CUDA(cudaGetLastError());
         note_launch();
@@ -186,15 +226,21 @@ extern "C" int odie_dispatch(const void* rows, int64_t n, int choices, int64_t w
 extern "C" int odie_combine(const void* sorted, int64_t n, int choices, int64_t width, int dtype, const int32_t* slot,
                             const float* weights, void* out, uint64_t stream) {
     return guarded([&] {
-        check_rows(n, choices, width, dtype, slot);
+        check_rows(n, choices, width, dtype, slot, "slot");
         if (n == 0) return;
         ODIE_REQUIRE(sorted && out, "sorted and out are required");
         const int vector = row_vector(width, dtype, sorted, out);
-        const RowArgs a = row_args(n, choices, width, dtype, slot, weights, vector);
-        with_row_type(dtype, vector, [&](auto type, auto bytes) {
+        const RowArgs a{row_shape(n, width * row_type_size(dtype) / vector), n * choices, choices, width, nullptr, slot, weights};
+        with_rows(dtype, vector, a.shape.narrow, [&](auto type, auto bytes, auto narrow) {
             using T = decltype(type);
-            combine_kernel<T, decltype(bytes)::value><<<row_blocks(n, a), THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-                a, static_cast<const T*>(sorted), static_cast<T*>(out));
+            auto go = [&](auto batch) {
+                combine_kernel<T, decltype(bytes)::value, decltype(narrow)::value, decltype(batch)::value>
+                    <<<row_blocks(a.shape, 4 / decltype(batch)::value), ROW_THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+                        a, static_cast<const T*>(sorted), static_cast<T*>(out));
+            };
+            if (choices == 1) go(std::integral_constant<int, 1>{});
+            else if (choices == 2) go(std::integral_constant<int, 2>{});
+            else go(std::integral_constant<int, 4>{});
         });
         ODIE_CUDA(cudaGetLastError());
         note_launch();
@@ -202,18 +248,18 @@ extern "C" int odie_combine(const void* sorted, int64_t n, int choices, int64_t 
 }
 
 extern "C" int odie_combine_backward(const void* d_out, const void* sorted, int64_t n, int choices, int64_t width, int dtype,
-                                     const int32_t* slot, const float* weights, void* d_sorted, float* d_weights,
+                                     const int32_t* order, const float* weights, void* d_sorted, float* d_weights,
                                      uint64_t stream) {
     return guarded([&] {
-        check_rows(n, choices, width, dtype, slot);
+        check_rows(n, choices, width, dtype, order, "order");
         if (n == 0 || (!d_sorted && !d_weights)) return;
         ODIE_REQUIRE(d_out && (sorted || !d_weights), "d_out is required, and sorted for the weights' gradient");
         const int vector = row_vector(width, dtype, d_out, d_weights ? sorted : d_out, d_sorted);
-        const RowArgs a = row_args(n, choices, width, dtype, slot, weights, vector);
-        with_row_type(dtype, vector, [&](auto type, auto bytes) {
+        const RowArgs a{row_shape(n * choices, width * row_type_size(dtype) / vector), n * choices, choices, width, order, nullptr, weights};
+        with_rows(dtype, vector, a.shape.narrow, [&](auto type, auto bytes, auto narrow) {
             using T = decltype(type);
-            combine_backward_kernel<T, decltype(bytes)::value>
-                <<<row_blocks(n * choices, a), THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+            combine_backward_kernel<T, decltype(bytes)::value, decltype(narrow)::value>
+                <<<row_blocks(a.shape, 2), ROW_THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
                     a, static_cast<const T*>(d_out), static_cast<const T*>(sorted), static_cast<T*>(d_sorted), d_weights);
         });
         ODIE_CUDA(cudaGetLastError());

@@ -15,40 +15,46 @@
 namespace odie {
 namespace {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = ROW_THREADS;
 constexpr int CHUNK = 64, BATCH = 8;  // BATCH rows are loaded together
 
 struct EmbedArgs {
+    RowShape shape;   // of the result
     const void* ids;
     int id_bytes;
-    long long n;
     long long rows;   // of the table
     long long width;
-    int lanes_log2;
     float scale;
 };
 
-__device__ __forceinline__ long long read_id(const EmbedArgs& a, long long i) {
-    return a.id_bytes == 8 ? reinterpret_cast<const long long*>(a.ids)[i]
-                           : (long long)reinterpret_cast<const int*>(a.ids)[i];
-}
-
-template <typename T, int BYTES>
+template <typename T, int BYTES, bool NARROW>
 __global__ void __launch_bounds__(THREADS) embed_kernel(EmbedArgs a, const T* __restrict__ table, T* __restrict__ out) {
     using P = Pack<T, BYTES>;
-    const int lanes = 1 << a.lanes_log2, lane = threadIdx.x & (lanes - 1);
-    const long long i = ((long long)blockIdx.x * THREADS + threadIdx.x) >> a.lanes_log2;
-    if (i >= a.n) return;
-    const long long id = read_id(a, i), vectors = a.width / P::N;
-    const bool inside = id >= 0 && id < a.rows;
-    for (long long c = lane; c < vectors; c += lanes) {
-        P o = P::zero();
-        if (inside) {
-            o = P::load(table + id * a.width + c * P::N);
+    constexpr int ITEMS = 4;
+    const RowWalk<NARROW, ITEMS> walk(a.shape);
+    long long id[ITEMS];
+    bool inside[ITEMS];
 #pragma unroll
-            for (int e = 0; e < P::N; ++e) o.v[e] = from_float<T>(a.scale * to_float(o.v[e]));
+    for (int q = 0; q < ITEMS; ++q) {
+        const long long i = walk.row_of(q) < walk.rows ? walk.row_of(q) : 0;
+        id[q] = a.id_bytes == 8 ? __ldg(static_cast<const long long*>(a.ids) + i) : (long long)__ldg(static_cast<const int*>(a.ids) + i);
+        inside[q] = id[q] >= 0 && id[q] < a.rows;
+        if (!inside[q]) id[q] = 0;
+    }
+    for (long long c = walk.lane; c < walk.vectors; c += walk.stride()) {
+        P v[ITEMS];
+#pragma unroll
+        for (int q = 0; q < ITEMS; ++q)
+            v[q] = P::load(table + id[q] * a.width + (walk.vector_of(c, q) < walk.vectors ? walk.vector_of(c, q) : 0) * P::N);
+#pragma unroll
+        for (int q = 0; q < ITEMS; ++q) {
+            P o = P::zero();
+            if (inside[q]) {
+#pragma unroll
+                for (int e = 0; e < P::N; ++e) o.v[e] = from_float<T>(a.scale * to_float(v[q].v[e]));
+            }
+            if (walk.on(c, q)) o.store(out + walk.row_of(q) * a.width + walk.vector_of(c, q) * P::N);
         }
-        o.store(out + i * a.width + c * P::N);
     }
 }
 
@@ -185,13 +191,14 @@ extern "C" int odie_embed(const void* ids, int id_bytes, int64_t n, const void* 
         if (n == 0) return;
         ODIE_REQUIRE(ids && table && out, "ids, table and out are required");
         const int vector = row_vector(width, dtype, table, out);
-        const EmbedArgs a{ids, id_bytes, n, rows, width, log2_of(row_lanes(width * row_type_size(dtype) / vector)), scale};
-        const int64_t blocks = ((n << a.lanes_log2) + THREADS - 1) / THREADS;
-        ODIE_REQUIRE(blocks < (int64_t(1) << 31), "too many rows for one launch");
+        const EmbedArgs a{row_shape(n, width * row_type_size(dtype) / vector), ids, id_bytes, rows, width, scale};
         with_row_type(dtype, vector, [&](auto type, auto bytes) {
             using T = decltype(type);
-            embed_kernel<T, decltype(bytes)::value><<<unsigned(blocks), THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
-                a, static_cast<const T*>(table), static_cast<T*>(out));
+            constexpr int B = decltype(bytes)::value;
+            const cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+            const unsigned blocks = row_blocks(a.shape, 4);
+            if (a.shape.narrow) embed_kernel<T, B, true><<<blocks, THREADS, 0, s>>>(a, static_cast<const T*>(table), static_cast<T*>(out));
+            else embed_kernel<T, B, false><<<blocks, THREADS, 0, s>>>(a, static_cast<const T*>(table), static_cast<T*>(out));
         });
         ODIE_CUDA(cudaGetLastError());
         note_launch();

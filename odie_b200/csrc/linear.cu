@@ -22,41 +22,97 @@ namespace {
 
 enum Activation : int { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3 };
 
+// Pairs of fp32 values: sm_100 multiplies and adds two per instruction.
+struct Pair {
+    unsigned long long v;
+};
+__device__ __forceinline__ Pair pair(float a, float b) {
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 both(Pair p) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p.v));
+    return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return d;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
+__device__ __forceinline__ Pair same(float a) { return pair(a, a); }
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float inverse_approx(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
 // The slope's code, as the low bits of 2^23 + code (one fused multiply-add rounds to nearest; act' in (-1/4, 7/4)
 // needs no clamp).  A NaN slope is the canonical NaN, whose low 16 bits are 0xffff.
-__device__ __forceinline__ uint32_t slope_bits(float d) { return __float_as_uint(fmaf(d, 32768.0f, 8388608.0f + 8192.0f)); }
+__device__ __forceinline__ uint32_t slope_codes(Pair slope) {
+    const float2 c = both(fma2(slope, same(32768.0f), same(8388608.0f + 8192.0f)));
+    return __byte_perm(__float_as_uint(c.x), __float_as_uint(c.y), 0x5410);
+}
 __device__ __forceinline__ float slope_value(uint32_t c) {  // c: 16 bits
     const float d = fmaf(__uint_as_float(0x4b000000u | c), 1.0f / 32768.0f, -256.25f);  // exact
     return c == 0xffffu ? __int_as_float(0x7fffffff) : d;
 }
 
-// act(z), with act'(z) in slope.
+// act(z), with act'(z) in slope, of two values.
 //   SiLU  p = 1 / (1 + e^-z): z p and p + z p (1 - p).
 //   GELU  z P(z) and P(z) + z e^(-z^2/2) / sqrt(2 pi), P the normal distribution function by Abramowitz and
 //         Stegun 7.1.26: erfc(u) = (a1 t + .. + a5 t^5) e^(-u^2), t = 1 / (1 + 0.3275911 u), u = |z| / sqrt 2, off
 //         by at most 1.5e-7 absolutely; it shares the slope's exponential.
+// Written in pairs, and with one instruction each for exponential and inverse: the epilogue shares the SM with
+// nothing else, but at 45 instructions per element it took twice the products' time for 1024 inputs.
 template <int ACT>
-__device__ __forceinline__ float activate(float z, float& slope) {
+__device__ __forceinline__ Pair activate(Pair z, Pair& slope) {
+    constexpr float LOG2E = 1.4426950408889634f;
+    const float2 s = both(z);
     if (ACT == ACT_RELU) {
-        slope = z > 0.0f ? 1.0f : z != z ? z : 0.0f;
-        return z > 0.0f || z != z ? z : 0.0f;
+        slope = pair(s.x > 0.0f ? 1.0f : s.x != s.x ? s.x : 0.0f, s.y > 0.0f ? 1.0f : s.y != s.y ? s.y : 0.0f);
+        return pair(s.x > 0.0f || s.x != s.x ? s.x : 0.0f, s.y > 0.0f || s.y != s.y ? s.y : 0.0f);
     }
     if (ACT == ACT_SILU) {
-        const float p = __fdividef(1.0f, 1.0f + __expf(-z));
-        const float a = z * p;
-        slope = fmaf(a, 1.0f - p, p);
+        const float2 x = both(mul2(z, same(-LOG2E)));
+        const float2 d = both(add2(pair(exp2_approx(x.x), exp2_approx(x.y)), same(1.0f)));
+        const Pair p = pair(inverse_approx(d.x), inverse_approx(d.y));
+        const Pair a = mul2(z, p);
+        slope = fma2(a, fma2(p, same(-1.0f), same(1.0f)), p);
         return a;
     }
     if (ACT == ACT_GELU) {
-        const float e = __expf(-0.5f * z * z);
-        const float t = __fdividef(1.0f, fmaf(fabsf(z), 0.3275911f * 0.70710678118654752f, 1.0f));
-        const float q = 0.5f * t * e *
-                        fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-        const float p = z < 0.0f ? q : 1.0f - q;
-        slope = fmaf(z * 0.39894228040143268f, e, p);
-        return z * p;
+        const float2 x = both(mul2(mul2(z, z), same(-0.5f * LOG2E)));
+        const Pair e = pair(exp2_approx(x.x), exp2_approx(x.y));
+        const float2 d = both(fma2(pair(fabsf(s.x), fabsf(s.y)), same(0.3275911f * 0.70710678118654752f), same(1.0f)));
+        const Pair t = pair(inverse_approx(d.x), inverse_approx(d.y));
+        Pair q = fma2(t, same(0.5f * 1.061405429f), same(0.5f * -1.453152027f));
+        q = fma2(t, q, same(0.5f * 1.421413741f));
+        q = fma2(t, q, same(0.5f * -0.284496736f));
+        q = fma2(t, q, same(0.5f * 0.254829592f));
+        q = mul2(mul2(q, t), e);  // P(-|z|)
+        const float2 below = both(q), above = both(fma2(q, same(-1.0f), same(1.0f)));
+        const Pair p = pair(s.x < 0.0f ? below.x : above.x, s.y < 0.0f ? below.y : above.y);
+        slope = fma2(mul2(z, same(0.39894228040143268f)), e, p);
+        return mul2(z, p);
     }
-    slope = 1.0f;
+    slope = same(1.0f);
     return z;
 }
 
@@ -94,6 +150,7 @@ constexpr int BK = 64;
 constexpr int GEMM_THREADS = 384, EPILOGUE_WARP = 4, EPILOGUE_WARPS = 8;
 constexpr uint32_t WAIT_LIMIT = 1u << 22;
 constexpr int STAGING = 2048;  // bytes per epilogue warp: 32 rows x 32 columns of 16 bits
+constexpr int BIAS = 128;      // fp32 values per epilogue warp
 
 struct GemmArgs {
     int groups;
@@ -122,7 +179,7 @@ struct Shape {
     static constexpr int COLUMNS = 2 * BN;  // TMEM: two accumulators
     static constexpr int HEAD = 1024;       // barriers, TMEM address
     static int bytes(int groups) {
-        return 1024 + STAGES * STAGE + EPILOGUE_WARPS * (STAGING + 128) + HEAD + (2 * (groups + 2)) * 4;
+        return 1024 + STAGES * STAGE + EPILOGUE_WARPS * (STAGING + BIAS * 4) + HEAD + (2 * (groups + 2)) * 4;
     }
 };
 
@@ -198,61 +255,60 @@ __device__ __forceinline__ uint4* staged(char* base, int row, int unit) {
     return reinterpret_cast<uint4*>(base + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4));
 }
 
-// 32 rows x 32 columns of a row-major 16-bit matrix between global memory and registers: thread (lane) holds the
-// 16-byte unit lane % 4 of rows lane / 4 + 8 i.
+// 32 rows x 32 columns of a row-major 16-bit matrix, moved between global memory and the staging tile.  Where every
+// row starts on a 16-byte boundary, thread (lane) moves the 16-byte unit lane % 4 of rows lane / 4 + 8 i, else the
+// element `lane` of every row.
 struct Window {
-    long long ld;
+    int ld;
     int rows, columns;  // inside the matrix
     bool wide;          // 16-byte accesses
 };
 __device__ __forceinline__ void window_load(const uint16_t* at, const Window& w, int lane, uint4 (&v)[4]) {
+    const int r = lane / 4, c = (lane & 3) * 8;
+    const uint16_t* from = at + (long long)r * w.ld + c;
+    if (c + 8 <= w.columns) {  // wide rows: columns are a multiple of 8
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = lane / 4 + 8 * i, c = (lane & 3) * 8;
-        v[i] = make_uint4(0, 0, 0, 0);
-        if (r >= w.rows || c >= w.columns) continue;
-        const uint16_t* from = at + r * w.ld + c;
-        if (w.wide && c + 8 <= w.columns) {
-            v[i] = __ldg(reinterpret_cast<const uint4*>(from));
-        } else {
-            uint16_t e[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) e[j] = c + j < w.columns ? from[j] : uint16_t(0);
-            v[i] = make_uint4(e[0] | uint32_t(e[1]) << 16, e[2] | uint32_t(e[3]) << 16, e[4] | uint32_t(e[5]) << 16,
-                              e[6] | uint32_t(e[7]) << 16);
-        }
+        for (int i = 0; i < 4; ++i)
+            v[i] = r + 8 * i < w.rows ? __ldg(reinterpret_cast<const uint4*>(from + (long long)(8 * i) * w.ld)) : make_uint4(0, 0, 0, 0);
     }
 }
-__device__ __forceinline__ void window_store(uint16_t* at, const Window& w, int lane, const char* staging) {
+__device__ __forceinline__ uint16_t* staged_element(char* base, int row, int c) {
+    return reinterpret_cast<uint16_t*>(staged(base, row, c >> 3)) + (c & 7);
+}
+__device__ __forceinline__ void window_fetch(const uint16_t* at, const Window& w, int lane, char* staging) {
+    if (lane < w.columns) {
+#pragma unroll 8
+        for (int r = 0; r < w.rows; ++r) *staged_element(staging, r, lane) = at[(long long)r * w.ld + lane];
+    }
+}
+__device__ __forceinline__ void window_store(uint16_t* at, const Window& w, int lane, char* staging) {
+    if (w.wide) {
+        const int r = lane / 4, c = (lane & 3) * 8;
+        uint16_t* to = at + (long long)r * w.ld + c;
+        if (c + 8 <= w.columns) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = lane / 4 + 8 * i, c = (lane & 3) * 8;
-        if (r >= w.rows || c >= w.columns) continue;
-        const uint4 v = *staged(const_cast<char*>(staging), r, lane & 3);
-        uint16_t* to = at + r * w.ld + c;
-        if (w.wide && c + 8 <= w.columns) {
-            *reinterpret_cast<uint4*>(to) = v;
-        } else {
-            const uint32_t e[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (c + j < w.columns) to[j] = uint16_t(e[j / 2] >> (16 * (j & 1)));
+            for (int i = 0; i < 4; ++i)
+                if (r + 8 * i < w.rows) *reinterpret_cast<uint4*>(to + (long long)(8 * i) * w.ld) = *staged(staging, r + 8 * i, lane & 3);
         }
+    } else if (lane < w.columns) {
+#pragma unroll 8
+        for (int r = 0; r < w.rows; ++r) at[(long long)r * w.ld + lane] = *staged_element(staging, r, lane);
     }
 }
 
-template <typename T, int ACT>
+template <int ACT>
 __device__ __forceinline__ void finish(float (&v)[32], uint32_t (&codes)[16], const float* bias) {
 #pragma unroll
     for (int i = 0; i < 32; i += 4) {
         const float4 b = *reinterpret_cast<const float4*>(bias + i);
-        float s[4];
-        v[i] = activate<ACT>(v[i] + b.x, s[0]);
-        v[i + 1] = activate<ACT>(v[i + 1] + b.y, s[1]);
-        v[i + 2] = activate<ACT>(v[i + 2] + b.z, s[2]);
-        v[i + 3] = activate<ACT>(v[i + 3] + b.w, s[3]);
-        codes[i / 2] = __byte_perm(slope_bits(s[0]), slope_bits(s[1]), 0x5410);
-        codes[i / 2 + 1] = __byte_perm(slope_bits(s[2]), slope_bits(s[3]), 0x5410);
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+            Pair slope;
+            const float2 y = both(activate<ACT>(add2(pair(v[i + j], v[i + j + 1]), j ? pair(b.z, b.w) : pair(b.x, b.y)), slope));
+            v[i + j] = y.x;
+            v[i + j + 1] = y.y;
+            codes[(i + j) / 2] = slope_codes(slope);
+        }
     }
 }
 
@@ -266,7 +322,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
     char* stages = smem;
     char* staging = stages + STAGES * S::STAGE;
     float* biases = reinterpret_cast<float*>(staging + EPILOGUE_WARPS * STAGING);
-    uint64_t* full = reinterpret_cast<uint64_t*>(staging + EPILOGUE_WARPS * (STAGING + 128));
+    uint64_t* full = reinterpret_cast<uint64_t*>(staging + EPILOGUE_WARPS * (STAGING + BIAS * 4));
     uint64_t* empty = full + STAGES;
     uint64_t* done = empty + STAGES;     // [2] accumulator summed
     uint64_t* drained = done + 2;        // [2] accumulator read out
@@ -419,8 +475,9 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
         }
     } else if (warp >= EPILOGUE_WARP) {
         const int quadrant = warp & 3, half = (warp - EPILOGUE_WARP) >> 2;
+        constexpr int WINDOWS = BN / 64;  // of 32 columns for each warp: columns 32 (half + 2 j)
         char* stage = staging + (warp - EPILOGUE_WARP) * STAGING;
-        float* bias = biases + (warp - EPILOGUE_WARP) * 32;
+        float* bias = biases + (warp - EPILOGUE_WARP) * BIAS;
         const uint32_t lanes = tmem + (uint32_t(quadrant * 32) << 16);
         const bool wide = p.n % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.slope)) % 16 == 0;
         const bool wide_residual = p.n % 8 == 0 && reinterpret_cast<uintptr_t>(p.residual) % 16 == 0;
@@ -428,15 +485,20 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
         for (int t = start; t < tiles && fine; t += step) {
             const Tile tile = tile_at<MODE, CG, BN>(p, begin, first, t);
             const int acc = summed & 1;
-            const int row = tile.m0 + int(rank) * 128 + quadrant * 32;
-            const uint16_t* residual = nullptr;
-            if (MODE == FWD && p.residual && !tile.zero) residual = static_cast<const uint16_t*>(p.residual) + (long long)row * p.n;
-            Window w{p.n, min(32, tile.m_end - row), 0, wide};
-            Window wr{p.n, w.rows, 0, wide_residual};
+            const int row = tile.m0 + int(rank) * 128 + quadrant * 32, column0 = tile.n0 + half * 32;
+            const long long at = (MODE == DW ? (long long)tile.g * p.m * p.n : 0) + (long long)row * p.n + column0;
+            const uint16_t* residual = MODE == FWD && p.residual && !tile.zero ? static_cast<const uint16_t*>(p.residual) + at : nullptr;
+            Window w{p.n, min(32, tile.m_end - row), p.n - column0, wide};
+            Window wr{p.n, w.rows, w.columns, wide_residual};
             uint4 r[4];
-            if (residual) {  // the first window's residual travels while the sum is awaited
-                wr.columns = p.n - (tile.n0 + half * 32);
-                window_load(residual + tile.n0 + half * 32, wr, lane, r);
+            if (MODE == FWD && !tile.zero) {  // what does not need the sum is read while it is awaited
+                if (residual && wr.wide) window_load(residual, wr, lane, r);
+#pragma unroll
+                for (int j = 0; j < WINDOWS; ++j)
+                    bias[j * 32 + lane] = p.bias && j * 64 + lane < w.columns
+                                              ? to_float(static_cast<const T*>(p.bias)[(long long)tile.g * p.n + column0 + j * 64 + lane])
+                                              : 0.0f;
+                __syncwarp();
             }
             if (!tile.zero) {
                 fine = __all_sync(0xffffffffu, tc::bar_wait_cluster(done + acc, (summed >> 1) & 1, WAIT_LIMIT));
@@ -444,9 +506,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
                 tc::fence_after_sync();
             }
 #pragma unroll 1
-            for (int c = half; c < BN / 32; c += 2) {
-                const int column = tile.n0 + c * 32;
-                w.columns = p.n - column;
+            for (int j = 0; j < WINDOWS; ++j) {
                 if (w.columns <= 0) break;
                 float v[32];
                 uint32_t codes[16];
@@ -456,11 +516,11 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) codes[i] = 0;
                 } else {
-                    tc::tmem_ld32(lanes + acc * BN + c * 32, v);
+                    tc::tmem_ld32(lanes + acc * BN + (half + 2 * j) * 32, v);
                 }
                 if (MODE == DW && p.partial) {
                     if (lane < w.rows) {
-                        float* to = p.partial + ((long long)tile.unit * p.m + row + lane) * p.n + column;
+                        float* to = p.partial + ((long long)tile.unit * p.m + row + lane) * p.n + column0 + j * 64;
                         if (p.n % 4 == 0) {
 #pragma unroll
                             for (int i = 0; i < 32; i += 4)
@@ -471,20 +531,26 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
                                 if (i < w.columns) to[i] = v[i];
                         }
                     }
+                    w.columns -= 64;
                     continue;
                 }
                 if (MODE == FWD && !tile.zero) {
-                    bias[lane] = p.bias && lane < w.columns
-                                     ? to_float(static_cast<const T*>(p.bias)[(long long)tile.g * p.n + column + lane]) : 0.0f;
                     if (residual) {
+                        if (wr.wide) {
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) *staged(stage, lane / 4 + 8 * i, lane & 3) = r[i];
+                            for (int i = 0; i < 4; ++i) *staged(stage, lane / 4 + 8 * i, lane & 3) = r[i];
+                            wr.columns -= 64;
+                            if (j + 1 < WINDOWS && wr.columns > 0) window_load(residual + (j + 1) * 64, wr, lane, r);
+                        } else {
+                            window_fetch(residual + j * 64, wr, lane, stage);
+                            wr.columns -= 64;
+                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
-                    if (p.activation == ACT_RELU) finish<T, ACT_RELU>(v, codes, bias);
-                    else if (p.activation == ACT_SILU) finish<T, ACT_SILU>(v, codes, bias);
-                    else if (p.activation == ACT_GELU) finish<T, ACT_GELU>(v, codes, bias);
-                    else finish<T, ACT_NONE>(v, codes, bias);
+                    if (p.activation == ACT_RELU) finish<ACT_RELU>(v, codes, bias + j * 32);
+                    else if (p.activation == ACT_SILU) finish<ACT_SILU>(v, codes, bias + j * 32);
+                    else if (p.activation == ACT_GELU) finish<ACT_GELU>(v, codes, bias + j * 32);
+                    else finish<ACT_NONE>(v, codes, bias + j * 32);
                     if (residual) {
 #pragma unroll
                         for (int u = 0; u < 4; ++u) {
@@ -497,29 +563,25 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
                                 v[u * 8 + i * 2 + 1] += f.y;
                             }
                         }
-                        if (c + 2 < BN / 32) {
-                            wr.columns = p.n - (column + 64);
-                            window_load(residual + column + 64, wr, lane, r);
-                        }
+                        __syncwarp();
                     }
-                    __syncwarp();
                 }
 #pragma unroll
                 for (int u = 0; u < 4; ++u)
                     *staged(stage, lane, u) = make_uint4(pack_pair<T>(v[u * 8], v[u * 8 + 1]), pack_pair<T>(v[u * 8 + 2], v[u * 8 + 3]),
                                                          pack_pair<T>(v[u * 8 + 4], v[u * 8 + 5]), pack_pair<T>(v[u * 8 + 6], v[u * 8 + 7]));
                 __syncwarp();
-                const long long group = MODE == DW ? (long long)tile.g * p.m * p.n : 0;
-                window_store(static_cast<uint16_t*>(p.out) + group + (long long)row * p.n + column, w, lane, stage);
+                window_store(static_cast<uint16_t*>(p.out) + at + j * 64, w, lane, stage);
                 __syncwarp();
                 if (MODE == FWD && p.slope) {
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
                         *staged(stage, lane, u) = make_uint4(codes[u * 4], codes[u * 4 + 1], codes[u * 4 + 2], codes[u * 4 + 3]);
                     __syncwarp();
-                    window_store(p.slope + (long long)row * p.n + column, w, lane, stage);
+                    window_store(p.slope + at + j * 64, w, lane, stage);
                     __syncwarp();
                 }
+                w.columns -= 64;
             }
             if (!tile.zero) {
                 tc::fence_before_sync();
@@ -560,23 +622,36 @@ __global__ void __launch_bounds__(32) group_maps_kernel(const __grid_constant__ 
                  : "memory");
 }
 
-// d W from the units' sums, in unit order.
+// d W from the units' sums: a block per 32 elements, each warp over its share of the units, the shares in order.
 template <typename T>
-__global__ void __launch_bounds__(256) join_kernel(const float* partial, T* out, const int* offsets, int groups, long long rows, int chunk,
+__global__ void __launch_bounds__(256) join_kernel(const float* partial, T* out, const int* offsets, long long rows, int chunk,
                                                    long long size) {
-    const int g = blockIdx.y;
+    __shared__ float part[8][33];
+    const int g = blockIdx.y, lane = threadIdx.x & 31, line = threadIdx.x >> 5;
     long long unit = 0, begin, end;
     for (int i = 0; i < g; ++i) {
         group_rows(offsets, i, rows, begin, end);
         unit += max(1ll, (end - begin + chunk - 1) / chunk);
     }
     group_rows(offsets, g, rows, begin, end);
-    const int count = int(max(1ll, (end - begin + chunk - 1) / chunk));
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < size; i += (long long)gridDim.x * 256) {
+    const int count = int(max(1ll, (end - begin + chunk - 1) / chunk)), share = (count + 7) / 8;
+    const int from = min(count, line * share), to = min(count, from + share);
+    for (long long i0 = (long long)blockIdx.x * 32; i0 < size; i0 += (long long)gridDim.x * 32) {
+        const long long i = i0 + lane;
         float sum = 0.0f;
+        if (i < size) {
 #pragma unroll 8
-        for (int u = 0; u < count; ++u) sum += partial[(unit + u) * size + i];
-        out[g * size + i] = from_float<T>(sum);
+            for (int u = from; u < to; ++u) sum += partial[(unit + u) * size + i];
+        }
+        part[line][lane] = sum;
+        __syncthreads();
+        if (line == 0 && i < size) {
+            sum = part[0][lane];
+#pragma unroll
+            for (int w = 1; w < 8; ++w) sum += part[w][lane];
+            out[g * size + i] = from_float<T>(sum);
+        }
+        __syncthreads();
     }
 }
 
@@ -1035,8 +1110,8 @@ extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, cons
                 });
                 if (u.split) {
                     const int64_t size = int64_t(outputs) * inputs;
-                    join_kernel<T><<<dim3(unsigned(std::min<int64_t>(ceil_div(size, 256), 1024)), unsigned(groups)), 256, 0, stream>>>(
-                        s.partial, static_cast<T*>(d_weight), offsets, groups, rows, int(u.chunk), size);
+                    join_kernel<T><<<dim3(unsigned(std::min<int64_t>(ceil_div(size, 32), 4096)), unsigned(groups)), 256, 0, stream>>>(
+                        s.partial, static_cast<T*>(d_weight), offsets, rows, int(u.chunk), size);
                     ODIE_CUDA(cudaGetLastError());
                     note_launch();
                 }

@@ -74,17 +74,53 @@ void with_row_type(int dtype, int vector, F&& f) {
     }
 }
 
-// Threads of a 256-thread block that share one row of `vectors` vectors: the smallest power of two that gives
-// every thread at most four of them (four independent loads in flight), at least 1 and at most 256.
-inline int row_lanes(int64_t vectors) {
-    int lanes = 1;
-    while (lanes < 256 && int64_t(lanes) * 4 < vectors) lanes *= 2;
-    return lanes;
+// How the 256 threads of a block share rows of `vectors` vectors, so that each has several independent loads in
+// flight and neighbours read neighbouring vectors.  Narrow rows (at most 32 vectors): 2^lanes_log2 threads hold
+// one vector each of a row, and a thread takes ITEMS rows.  Wide rows: 32 to 256 threads walk a row together,
+// ITEMS vectors at a time.  item<ITEMS>(q, ..) is the thread's q-th (row, vector) of a step.
+constexpr int ROW_THREADS = 256;
+struct RowShape {
+    long long rows;
+    long long vectors;
+    int lanes_log2;
+    bool narrow;
+};
+inline RowShape row_shape(int64_t rows, int64_t vectors) {
+    RowShape s{rows, vectors, 0, vectors <= 32};
+    if (s.narrow) {
+        while ((1 << s.lanes_log2) < vectors) ++s.lanes_log2;
+    } else {
+        s.lanes_log2 = 5;
+        while (s.lanes_log2 < 8 && (int64_t(4) << s.lanes_log2) < vectors) ++s.lanes_log2;
+    }
+    return s;
 }
+inline unsigned row_blocks(const RowShape& s, int items) {
+    const int64_t per = (ROW_THREADS >> s.lanes_log2) * int64_t(s.narrow ? items : 1);
+    const int64_t blocks = (s.rows + per - 1) / per;
+    ODIE_REQUIRE(blocks < (int64_t(1) << 31), "too many rows for one launch");
+    return unsigned(blocks);
+}
+template <bool NARROW, int ITEMS>
+struct RowWalk {
+    long long row, vectors, rows;
+    int lane, lanes, step;
+    __device__ __forceinline__ explicit RowWalk(const RowShape& s) : vectors(s.vectors), rows(s.rows) {
+        lanes = 1 << s.lanes_log2;
+        lane = threadIdx.x & (lanes - 1);
+        step = ROW_THREADS >> s.lanes_log2;
+        row = (long long)blockIdx.x * (step * (NARROW ? ITEMS : 1)) + (threadIdx.x >> s.lanes_log2);
+    }
+    __device__ __forceinline__ long long row_of(int q) const { return NARROW ? row + q * step : row; }
+    __device__ __forceinline__ long long vector_of(long long c, int q) const { return NARROW ? c : c + q * lanes; }
+    __device__ __forceinline__ bool on(long long c, int q) const { return row_of(q) < rows && vector_of(c, q) < vectors; }
+    __device__ __forceinline__ int stride() const { return NARROW ? lanes : lanes * ITEMS; }
+};
 
 // Sorted (key, index) pairs: sort_pairs (sort.cu).  keys: int32 or int64 (key_bytes 4 or 8), anything outside
 // [0, bins) counts as `bins`.  Writes order[p] = index of the p-th pair by (key, index), and where non-null
-// sorted[p] = its key and slot[i] = its place; for keys outside the range order is -1 and slot ~place.
+// sorted[p] = its key and slot[i] = its place; for keys outside the range order is ~index and
+// slot ~place.
 // offsets (may be null): i32[bins + 1], the number of pairs with a smaller key.
 struct SortArgs {
     const void* keys = nullptr;

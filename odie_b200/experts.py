@@ -10,7 +10,6 @@ is the MLP of `model.Head` with one set of weights per expert, built from them.
 
 There is no CPU path: tensors that are not on a CUDA device are refused.
 """
-from contextlib import nullcontext
 import math
 from typing import NamedTuple
 
@@ -31,7 +30,7 @@ class RowOrder(NamedTuple):
 
     Pair i = row * choices + choice.  order int32 [pairs]: the pair at each place; slot int32 [rows, choices]: the
     place of each pair; offsets int32 [bins + 1]: the first place of each expert, the last one the count of pairs
-    that have an expert.  Dropped pairs stand behind: their order is -1 and their slot ~place."""
+    that have an expert.  Dropped pairs stand behind: their order is ~pair and their slot ~place."""
     order: torch.Tensor
     slot: torch.Tensor
     offsets: torch.Tensor
@@ -45,18 +44,24 @@ class RowOrder(NamedTuple):
         return self.slot.shape[1]
 
 
-def _on(device):
-    """The device's context: the library launches on the current device."""
-    return nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _stream(index):
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _call(name, device, *arguments):
-    with _on(device):
-        _lib.check(getattr(_lib.library(), name)(*arguments, torch.cuda.current_stream(device).cuda_stream), name)
+    """One library call on the device's current stream (the library launches on the current device)."""
+    index = device.index
+    if index == torch.cuda.current_device():
+        status = getattr(_lib.library(), name)(*arguments, _stream(index))
+    else:
+        with torch.cuda.device(device):
+            status = getattr(_lib.library(), name)(*arguments, _stream(index))
+    _lib.check(status, name)
 
 
 def _scratch(device, count, *sizes):
-    return torch.empty(getattr(_lib.library(), count)(*sizes), dtype=torch.uint8, device=device)
+    size = getattr(_lib.library(), count)(*sizes)
+    return torch.empty(size, dtype=torch.uint8, device=device) if size else None
 
 
 def _need(condition, message):
@@ -64,19 +69,25 @@ def _need(condition, message):
         raise ValueError(message)
 
 
-def _check_rows(x, name, dims=2):
-    _need(isinstance(x, torch.Tensor) and x.is_cuda and x.dtype in ROW_TYPES and x.dim() == dims and x.shape[-1] > 0,
-          f'{name} must be a CUDA fp16, bf16 or fp32 tensor of {dims} dimensions with at least one column')
+def _check_rows(x, name):
+    if not (isinstance(x, torch.Tensor) and x.is_cuda and x.dtype in ROW_TYPES and x.dim() == 2 and x.shape[1] > 0):
+        raise ValueError(f'{name} must be a CUDA fp16, bf16 or fp32 tensor [rows, width] with at least one column')
 
 
 def _check_ids(ids, name):
-    _need(isinstance(ids, torch.Tensor) and ids.is_cuda and ids.dtype in (torch.int32, torch.int64),
-          f'{name} must be a CUDA int32 or int64 tensor')
+    if not (isinstance(ids, torch.Tensor) and ids.is_cuda and ids.dtype in (torch.int32, torch.int64)):
+        raise ValueError(f'{name} must be a CUDA int32 or int64 tensor')
 
 
 def _same_device(x, **others):
+    device = x.device
     for name, t in others.items():
-        _need(t is None or t.device == x.device, f'{name} is on {t.device if t is not None else None}, not {x.device}')
+        if t is not None and t.device != device:
+            raise ValueError(f'{name} is on {t.device}, not {device}')
+
+
+def _needs_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
 # ---------------------------------------------------------------- order
@@ -92,20 +103,21 @@ def sort_rows(expert, bins):
     n, device = rows * choices, expert.device
     _need(n < 2 ** 31 - 4096, 'too many (row, choice) pairs')
     expert = expert.detach().contiguous()
-    order = torch.empty(n, dtype=torch.int32, device=device)
-    slot = torch.empty((rows, choices), dtype=torch.int32, device=device)
-    offsets = torch.empty(bins + 1, dtype=torch.int32, device=device)
+    order, slot, offsets = torch.empty(2 * n + bins + 1, dtype=torch.int32, device=device).split((n, n, bins + 1))
     scratch = _scratch(device, 'odie_sort_rows_scratch', n, bins)
     _call('odie_sort_rows', device, expert.data_ptr(), expert.element_size(), n, bins, order.data_ptr(),
-          slot.data_ptr(), offsets.data_ptr(), scratch.data_ptr())
-    return RowOrder(order, slot, offsets)
+          slot.data_ptr(), offsets.data_ptr(), _lib.ptr(scratch))
+    return RowOrder(order, slot.view(rows, choices), offsets)
 
 
 def _check_order(order):
-    _need(isinstance(order, RowOrder), 'order must be the RowOrder of sort_rows')
-    slot = order.slot
-    _need(slot.is_cuda and slot.dtype == torch.int32 and slot.dim() == 2 and slot.is_contiguous(),
-          'order.slot must be a contiguous CUDA int32 tensor [rows, choices]')
+    if not isinstance(order, RowOrder):
+        raise ValueError('order must be the RowOrder of sort_rows')
+    order_, slot = order.order, order.slot
+    if not (slot.is_cuda and slot.dtype == torch.int32 and slot.dim() == 2 and slot.is_contiguous()
+            and order_.device == slot.device and order_.dtype == torch.int32 and order_.shape == (slot.numel(),)
+            and order_.is_contiguous()):
+        raise ValueError('order must hold contiguous CUDA int32 tensors: order [rows * choices] and slot [rows, choices]')
 
 
 def _check_weights(weights, order):
@@ -119,62 +131,62 @@ def _check_weights(weights, order):
     return weights.float().reshape(shape)  # differentiable: the gradient takes the weights' own type and shape
 
 
-def _dispatch(x, slot, weights):
-    n, choices = slot.shape
+def _dispatch(x, order, weights):
+    n, choices = order.slot.shape
     out = torch.empty((n * choices, x.shape[1]), dtype=x.dtype, device=x.device)
-    _call('odie_dispatch', x.device, x.data_ptr(), n, choices, x.shape[1], ROW_TYPES[x.dtype], slot.data_ptr(),
+    _call('odie_dispatch', x.device, x.data_ptr(), n, choices, x.shape[1], ROW_TYPES[x.dtype], order.order.data_ptr(),
           _lib.ptr(weights), out.data_ptr())
     return out
 
 
-def _combine(rows, slot, weights):
-    n, choices = slot.shape
+def _combine(rows, order, weights):
+    n, choices = order.slot.shape
     out = torch.empty((n, rows.shape[1]), dtype=rows.dtype, device=rows.device)
     _call('odie_combine', rows.device, rows.data_ptr(), n, choices, rows.shape[1], ROW_TYPES[rows.dtype],
-          slot.data_ptr(), _lib.ptr(weights), out.data_ptr())
+          order.slot.data_ptr(), _lib.ptr(weights), out.data_ptr())
     return out
 
 
-def _combine_backward(d_out, rows, slot, weights, need_rows, need_weights):
-    n, choices = slot.shape
+def _combine_backward(d_out, rows, order, weights, need_rows, need_weights):
+    n, choices = order.slot.shape
     width = d_out.shape[1]
     d_rows = torch.empty((n * choices, width), dtype=d_out.dtype, device=d_out.device) if need_rows else None
     d_weights = torch.empty((n, choices), dtype=torch.float32, device=d_out.device) if need_weights else None
     _call('odie_combine_backward', d_out.device, d_out.data_ptr(), _lib.ptr(rows), n, choices, width,
-          ROW_TYPES[d_out.dtype], slot.data_ptr(), _lib.ptr(weights), _lib.ptr(d_rows), _lib.ptr(d_weights))
+          ROW_TYPES[d_out.dtype], order.order.data_ptr(), _lib.ptr(weights), _lib.ptr(d_rows), _lib.ptr(d_weights))
     return d_rows, d_weights
 
 
 class _Dispatch(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, slot, weights):
-        ctx.save_for_backward(x if ctx.needs_input_grad[2] else None, slot, weights)
-        return _dispatch(x, slot, weights)
+    def forward(ctx, x, weights, order, slot):
+        ctx.save_for_backward(x if ctx.needs_input_grad[1] else None, weights, order, slot)
+        return _dispatch(x, RowOrder(order, slot, None), weights)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_rows):
-        x, slot, weights = ctx.saved_tensors
-        d_rows = d_rows.contiguous()
-        d_x = _combine(d_rows, slot, weights) if ctx.needs_input_grad[0] else None
+        x, weights, order, slot = ctx.saved_tensors
+        order, d_rows = RowOrder(order, slot, None), d_rows.contiguous()
+        d_x = _combine(d_rows, order, weights) if ctx.needs_input_grad[0] else None
         # d weights[t, j] = <x[t], d_rows[slot]>: the same product as combine's, the rows' roles exchanged
-        d_weights = _combine_backward(x, d_rows, slot, None, False, True)[1] if ctx.needs_input_grad[2] else None
-        return d_x, None, d_weights
+        d_weights = _combine_backward(x, d_rows, order, None, False, True)[1] if ctx.needs_input_grad[1] else None
+        return d_x, d_weights, None, None
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, rows, slot, weights):
-        ctx.save_for_backward(rows if ctx.needs_input_grad[2] else None, slot, weights)
-        return _combine(rows, slot, weights)
+    def forward(ctx, rows, weights, order, slot):
+        ctx.save_for_backward(rows if ctx.needs_input_grad[1] else None, weights, order, slot)
+        return _combine(rows, RowOrder(order, slot, None), weights)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_out):
-        rows, slot, weights = ctx.saved_tensors
-        d_rows, d_weights = _combine_backward(d_out.contiguous(), rows, slot, weights, ctx.needs_input_grad[0],
-                                              ctx.needs_input_grad[2])
-        return d_rows, None, d_weights
+        rows, weights, order, slot = ctx.saved_tensors
+        d_rows, d_weights = _combine_backward(d_out.contiguous(), rows, RowOrder(order, slot, None), weights,
+                                              ctx.needs_input_grad[0], ctx.needs_input_grad[1])
+        return d_rows, d_weights, None, None
 
 
 def dispatch(x, order, weights=None):
@@ -185,7 +197,10 @@ def dispatch(x, order, weights=None):
     _need(x.shape[0] == order.rows, f'x has {x.shape[0]} rows, the order {order.rows}')
     weights = _check_weights(weights, order)
     _same_device(x, order=order.slot, weights=weights)
-    return _Dispatch.apply(x.contiguous(), order.slot, weights)
+    x = x.contiguous()
+    if _needs_grad(x, weights):
+        return _Dispatch.apply(x, weights, order.order, order.slot)
+    return _dispatch(x, order, weights)
 
 
 def combine(rows, order, weights=None):
@@ -197,7 +212,10 @@ def combine(rows, order, weights=None):
           f'rows has {rows.shape[0]} rows, the order {order.rows} x {order.choices}')
     weights = _check_weights(weights, order)
     _same_device(rows, order=order.slot, weights=weights)
-    return _Combine.apply(rows.contiguous(), order.slot, weights)
+    rows = rows.contiguous()
+    if _needs_grad(rows, weights):
+        return _Combine.apply(rows, weights, order.order, order.slot)
+    return _combine(rows, order, weights)
 
 
 # ---------------------------------------------------------------- linear
@@ -217,7 +235,7 @@ def _linear(x, weight, bias, residual, offsets, activation, training):
     scratch = _scratch(x.device, 'odie_linear_scratch', rows, inputs, outputs, groups)
     _call('odie_linear', x.device, x.data_ptr(), weight.data_ptr(), _lib.ptr(bias), _lib.ptr(residual), rows, inputs,
           outputs, groups, _lib.ptr(offsets), ROW_TYPES[x.dtype], activation, y.data_ptr(), _lib.ptr(slope),
-          scratch.data_ptr())
+          _lib.ptr(scratch))
     return y, slope
 
 
@@ -252,7 +270,7 @@ class _Linear(torch.autograd.Function):
             _call('odie_linear_backward', d_y.device, d_y.data_ptr(), _lib.ptr(slope), _lib.ptr(x), _lib.ptr(weight),
                   rows, inputs, outputs, groups, _lib.ptr(offsets), ROW_TYPES[d_y.dtype], _lib.ptr(d_x),
                   _lib.ptr(d_weight), _lib.ptr(d_bias), None if offsets is None else _lib.ptr(d_residual),
-                  scratch.data_ptr())
+                  _lib.ptr(scratch))
         return d_x, d_weight, d_bias, d_residual if need[3] else None, None, None
 
 
@@ -263,34 +281,40 @@ def linear(x, weight, bias=None, residual=None, activation='none', offsets=None)
     RowOrder; non-decreasing from 0): x [rows, inputs], weight [experts, outputs, inputs], bias [experts, outputs];
     rows [offsets[e], offsets[e + 1]) take expert e's layer, rows behind the last offset give zero rows (without
     the residual).  residual: broadcastable to the result.  activation: 'none', 'relu', 'silu' or 'gelu' (erf)."""
-    _need(isinstance(x, torch.Tensor) and x.is_cuda and x.dtype in (torch.float16, torch.bfloat16) and x.dim() >= 1
-          and x.shape[-1] > 0, 'x must be a CUDA fp16 or bf16 tensor with at least one column')
-    _need(activation in ACTIVATIONS, f'activation must be one of {", ".join(ACTIVATIONS)}')
-    _need(isinstance(weight, torch.Tensor) and weight.dim() == (2 if offsets is None else 3)
-          and weight.shape[-1] == x.shape[-1] and weight.numel() > 0,
-          f'weight must be {"[outputs" if offsets is None else "[experts, outputs"}, {x.shape[-1]}]')
-    _need(bias is None or tuple(bias.shape) == tuple(weight.shape[:-1]), f'bias must be {tuple(weight.shape[:-1])}')
+    if not (isinstance(x, torch.Tensor) and x.is_cuda and x.dtype in (torch.float16, torch.bfloat16) and x.dim() >= 1
+            and x.shape[-1] > 0):
+        raise ValueError('x must be a CUDA fp16 or bf16 tensor with at least one column')
+    if activation not in ACTIVATIONS:
+        raise ValueError(f'activation must be one of {", ".join(ACTIVATIONS)}')
+    if not (isinstance(weight, torch.Tensor) and weight.dim() == (2 if offsets is None else 3)
+            and weight.shape[-1] == x.shape[-1] and weight.numel() > 0):
+        raise ValueError(f'weight must be {"[outputs" if offsets is None else "[experts, outputs"}, {x.shape[-1]}]')
+    if bias is not None and bias.shape != weight.shape[:-1]:
+        raise ValueError(f'bias must be {tuple(weight.shape[:-1])}')
     for name, t in (('weight', weight), ('bias', bias), ('residual', residual)):
-        _need(t is None or t.dtype == x.dtype, f'{name} must have the type of x, {x.dtype}')
+        if t is not None and t.dtype != x.dtype:
+            raise ValueError(f'{name} must have the type of x, {x.dtype}')
     if offsets is not None:
         _need(x.dim() == 2, 'x must be [rows, inputs] with offsets')
         _need(weight.shape[0] <= 1024, 'at most 1024 experts')
-        _need(isinstance(offsets, torch.Tensor) and offsets.is_cuda and offsets.dtype == torch.int32
-              and tuple(offsets.shape) == (weight.shape[0] + 1,), f'offsets must be CUDA int32 [{weight.shape[0] + 1}]')
+        if not (isinstance(offsets, torch.Tensor) and offsets.is_cuda and offsets.dtype == torch.int32
+                and offsets.shape == (weight.shape[0] + 1,)):
+            raise ValueError(f'offsets must be CUDA int32 [{weight.shape[0] + 1}]')
         offsets = offsets.contiguous()
     _same_device(x, weight=weight, bias=bias, residual=residual, offsets=offsets)
-    outputs = weight.shape[-2]
-    lead = x.shape[:-1]
-    flat = x.reshape(math.prod(lead), x.shape[-1])
+    outputs, lead = weight.shape[-2], x.shape[:-1]
+    flat = x if x.dim() == 2 else x.reshape(math.prod(lead), x.shape[-1])
     if residual is not None:
-        residual = residual.expand(*lead, outputs).reshape(flat.shape[0], outputs)
-    tensors = [t for t in (flat, weight, bias, residual) if t is not None]
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        if residual.shape != (*lead, outputs):
+            residual = residual.expand(*lead, outputs)
+        if residual.dim() != 2:
+            residual = residual.reshape(flat.shape[0], outputs)
+    if _needs_grad(flat, weight, bias, residual):
         y = _Linear.apply(flat, weight, bias, residual, offsets, ACTIVATIONS[activation])
     else:
         bias, residual = (None if t is None else t.contiguous() for t in (bias, residual))
         y, _ = _linear(_aligned(flat), _aligned(weight), bias, residual, offsets, ACTIVATIONS[activation], False)
-    return y.reshape(*lead, outputs)
+    return y if x.dim() == 2 else y.reshape(*lead, outputs)
 
 
 # ---------------------------------------------------------------- learned rows by id
@@ -317,7 +341,7 @@ class _Embed(torch.autograd.Function):
         d_table = torch.empty((rows, width), dtype=d_out.dtype, device=d_out.device)
         scratch = _scratch(d_out.device, 'odie_embed_backward_scratch', ids.numel(), rows, width)
         _call('odie_embed_backward', d_out.device, ids.data_ptr(), ids.element_size(), ids.numel(), d_out.data_ptr(),
-              rows, width, ROW_TYPES[d_out.dtype], ctx.scale, d_table.data_ptr(), scratch.data_ptr())
+              rows, width, ROW_TYPES[d_out.dtype], ctx.scale, d_table.data_ptr(), _lib.ptr(scratch))
         return None, d_table, None
 
 
@@ -329,8 +353,9 @@ def embed(ids, table, scale=1.0):
     _need(1 <= table.shape[0] < 1 << 30, 'the table must have 1 to 2^30 - 1 rows')
     _need(ids.numel() < 2 ** 31 - 4096, 'too many ids')
     _same_device(table, ids=ids)
-    out = _Embed.apply(ids.detach().contiguous(), table.contiguous(), float(scale))
-    return out.view(*ids.shape, table.shape[1])
+    flat, table = ids.contiguous(), table.contiguous()
+    out = _Embed.apply(flat, table, float(scale)) if _needs_grad(table) else _embed(flat, table, float(scale))
+    return out if ids.dim() == 1 else out.view(*ids.shape, table.shape[1])
 
 
 # ---------------------------------------------------------------- a model of them

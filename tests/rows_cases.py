@@ -45,7 +45,7 @@ def plain_order(expert, bins):
     for k, _ in kept:
         counts[k + 1] += 1
     offsets = torch.tensor(counts).cumsum(0)
-    return torch.tensor([i for _, i in kept] + [-1] * len(gone)), torch.tensor(slot).reshape(expert.shape), offsets
+    return torch.tensor([i for _, i in kept] + [~i for i in gone]), torch.tensor(slot).reshape(expert.shape), offsets
 
 
 def activated(z, name):
