@@ -386,11 +386,12 @@ ODIE_API int64_t odie_sort_rows_scratch(int64_t n, int bins);
 ODIE_API int odie_sort_rows(const void* keys, int key_bytes, int64_t n, int bins, int32_t* order, int32_t* slot,
                    int32_t* offsets, void* scratch, uint64_t stream);
 ODIE_API int odie_dispatch(const void* rows, int64_t n, int choices, int64_t width, int dtype, const int32_t* order,
-                   const float* weights, void* sorted, uint64_t stream);
+                   const int32_t* slot, const float* weights, void* sorted, uint64_t stream);
 ODIE_API int odie_combine(const void* sorted, int64_t n, int choices, int64_t width, int dtype, const int32_t* slot,
                    const float* weights, void* out, uint64_t stream);
 ODIE_API int odie_combine_backward(const void* d_out, const void* sorted, int64_t n, int choices, int64_t width, int dtype,
-                   const int32_t* order, const float* weights, void* d_sorted, float* d_weights, uint64_t stream);
+                   const int32_t* order, const int32_t* slot, const float* weights, void* d_sorted, float* d_weights,
+                   uint64_t stream);
 
 /* ------------------------------------------------------------------------
  * Linear layer of rows (no reference counterpart): y[rows][outputs] =

@@ -74,9 +74,9 @@ SIGNATURES = {
     'odie_hashgrid32_destroy': (None, [P]),
     'odie_sort_rows_scratch': (I64, [I64, I32]),
     'odie_sort_rows': (I32, [P, I32, I64, I32, P, P, P, P, U64]),
-    'odie_dispatch': (I32, [P, I64, I32, I64, I32, P, P, P, U64]),
+    'odie_dispatch': (I32, [P, I64, I32, I64, I32, P, P, P, P, U64]),
     'odie_combine': (I32, [P, I64, I32, I64, I32, P, P, P, U64]),
-    'odie_combine_backward': (I32, [P, P, I64, I32, I64, I32, P, P, P, P, U64]),
+    'odie_combine_backward': (I32, [P, P, I64, I32, I64, I32, P, P, P, P, P, U64]),
     'odie_linear_scratch': (I64, [I64, I32, I32, I32]),
     'odie_linear': (I32, [P, P, P, P, I64, I32, I32, I32, P, I32, I32, P, P, P, U64]),
     'odie_linear_backward_scratch': (I64, [I64, I32, I32, I32]),

@@ -4,10 +4,10 @@
 //   dispatch   sorted[slot] = w x[t]             (w = 1 without weights), zero rows for dropped choices
 //   combine    out[t] = sum_j w[t, j] sorted[slot[t, j]], an fp32 chain in ascending j, rounded once
 //   backward   d sorted[slot] = w d out[t], d w[t, j] = <sorted[slot], d out[t]> in fp32
-// The gradient of dispatch is combine without weights.  All are bound by the bytes of the rows.  Each kernel walks
-// the side that it writes, so that writes are whole lines in order and only reads are scattered (by row; the
-// unsorted rows that are read once per choice come from L2).  Scattered writes of 64-byte rows took half as long
-// again: 47 us against 31 for 2^20 rows of 32 fp16.
+// The gradient of dispatch is combine without weights.  All are bound by the bytes of the rows.  Kernels walk the
+// side that they write, so that writes are whole lines in order and only reads are scattered (writes of 64-byte rows
+// to their places took half as long again: 47 us against 31 for 2^20 rows of 32 fp16), but for wide rows with several
+// choices, whose places are whole lines anyway.
 #include "rows.cuh"
 #include "odie_b200.h"
 #include <type_traits>
@@ -54,6 +54,32 @@ __global__ void __launch_bounds__(ROW_THREADS) dispatch_kernel(RowArgs a, const 
                 for (int i = 0; i < P::N; ++i) o.v[i] = from_float<T>(w[q] * to_float(v[q].v[i]));
             }
             if (walk.on(c, q)) o.store(sorted + walk.row_of(q) * a.width + walk.vector_of(c, q) * P::N);
+        }
+    }
+}
+
+// Wide rows with several choices: walks the unsorted rows, so that each is read once however many choices it has.
+// (Walking the sorted side, rows were evicted from L2 between their choices: 16384 rows of 4 KB, four choices each,
+// took 82 us against 54.)
+template <typename T, int BYTES>
+__global__ void __launch_bounds__(ROW_THREADS) dispatch_rows_kernel(RowArgs a, const T* __restrict__ rows, T* __restrict__ sorted) {
+    using P = Pack<T, BYTES>;
+    const RowWalk<false, 1> walk(a.shape);
+    if (walk.row >= walk.rows) return;
+    const long long pair = walk.row * a.choices;
+    for (long long c = walk.lane; c < walk.vectors; c += walk.lanes) {
+        const P v = P::load(rows + walk.row * a.width + c * P::N);
+#pragma unroll 4
+        for (int j = 0; j < a.choices; ++j) {
+            const int s = __ldg(a.slot + pair + j);
+            const long long place = s < 0 ? ~s : s;
+            P o = s < 0 ? P::zero() : v;
+            if (s >= 0 && a.weights) {
+                const float w = __ldg(a.weights + pair + j);
+#pragma unroll
+                for (int i = 0; i < P::N; ++i) o.v[i] = from_float<T>(w * to_float(v.v[i]));
+            }
+            if (place < a.places) o.store(sorted + place * a.width + c * P::N);
         }
     }
 }
@@ -183,11 +209,93 @@ __global__ void __launch_bounds__(ROW_THREADS) combine_backward_kernel(RowArgs a
     }
 }
 
+// The same for wide rows with several choices, walking the unsorted rows: d out is read once for up to four choices.
+template <typename T, int BYTES>
+__global__ void __launch_bounds__(ROW_THREADS) combine_backward_rows_kernel(RowArgs a, const T* __restrict__ d_out,
+                                                                            const T* __restrict__ sorted, T* __restrict__ d_sorted,
+                                                                            float* __restrict__ d_weights) {
+    using P = Pack<T, BYTES>;
+    constexpr int BATCH = 4;
+    __shared__ float partial[BATCH][ROW_THREADS / 32];
+    const RowWalk<false, 1> walk(a.shape);
+    const bool live = walk.row < walk.rows;
+    const long long row = live ? walk.row : 0;
+    for (int j0 = 0; j0 < a.choices; j0 += BATCH) {
+        long long place[BATCH];
+        float w[BATCH], dot[BATCH];
+        bool kept[BATCH], on[BATCH];
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {
+            const bool inside = live && j0 + b < a.choices;
+            const long long pair = row * a.choices + (inside ? j0 + b : 0);
+            const int s = __ldg(a.slot + pair);
+            place[b] = s < 0 ? ~s : s;
+            on[b] = inside && place[b] < a.places;
+            kept[b] = on[b] && s >= 0;
+            if (!on[b]) place[b] = 0;
+            w[b] = a.weights ? __ldg(a.weights + pair) : 1.0f;
+            dot[b] = 0.0f;
+        }
+        for (long long c = walk.lane; c < walk.vectors; c += walk.lanes) {
+            const P g = P::load(d_out + row * a.width + c * P::N);
+            P y[BATCH];
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b)
+                if (d_weights) y[b] = P::load(sorted + place[b] * a.width + c * P::N);
+#pragma unroll
+            for (int b = 0; b < BATCH; ++b) {
+                if (d_weights) {
+                    float part = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < P::N; ++i) part = fmaf(to_float(y[b].v[i]), to_float(g.v[i]), part);
+                    dot[b] = kept[b] ? dot[b] + part : 0.0f;
+                }
+                if (d_sorted && on[b]) {
+                    P o = P::zero();
+                    if (kept[b]) {
+#pragma unroll
+                        for (int i = 0; i < P::N; ++i) o.v[i] = from_float<T>(w[b] * to_float(g.v[i]));
+                    }
+                    o.store(d_sorted + place[b] * a.width + c * P::N);
+                }
+            }
+        }
+        if (!d_weights) continue;
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b) {
+#pragma unroll
+            for (int d = 16; d > 0; d /= 2) dot[b] += __shfl_xor_sync(0xffffffffu, dot[b], d);
+            if ((threadIdx.x & 31) == 0) partial[b][threadIdx.x >> 5] = dot[b];
+        }
+        __syncthreads();
+        if (walk.lane < BATCH && live && j0 + walk.lane < a.choices) {
+            float total = 0.0f;
+            for (int i = 0; i < walk.lanes / 32; ++i) total += partial[walk.lane][(threadIdx.x >> 5) + i];
+            d_weights[row * a.choices + j0 + walk.lane] = total;
+        }
+        __syncthreads();
+    }
+}
+
 void check_rows(int64_t n, int choices, int64_t width, int dtype, const int32_t* order, const char* name) {
     check_row_type(dtype);
     ODIE_REQUIRE(n >= 0 && choices >= 1 && n < (int64_t(1) << 31) / choices, "0 to 2^31 - 1 (row, choice) pairs");
     ODIE_REQUIRE(width >= 1 && width <= (int64_t(1) << 31), "rows have 1 to 2^31 elements");
     ODIE_REQUIRE(n == 0 || order, std::string(name) + " is required");
+}
+
+// The walk of a kernel that writes the sorted side: by rows (slot) for wide rows with several choices, by places
+// (order) for the others.
+RowArgs sorted_args(int64_t n, int choices, int64_t width, int dtype, int vector, const int32_t* order, const int32_t* slot,
+                    const float* weights) {
+    const int64_t vectors = width * row_type_size(dtype) / vector;
+    RowArgs a{row_shape(n * choices, vectors), n * choices, choices, width, order, nullptr, weights};
+    if (!a.shape.narrow && choices > 1) {
+        a.shape = row_shape(n, vectors);
+        a.order = nullptr;
+        a.slot = slot;
+    }
+    return a;
 }
 
 // f(T{}, integral_constant<int, BYTES>, bool_constant<NARROW>)
@@ -205,14 +313,22 @@ void with_rows(int dtype, int vector, bool narrow, F&& f) {
 using namespace odie;
 
 extern "C" int odie_dispatch(const void* rows, int64_t n, int choices, int64_t width, int dtype, const int32_t* order,
-                             const float* weights, void* sorted, uint64_t stream) {
+                             const int32_t* slot, const float* weights, void* sorted, uint64_t stream) {
     return guarded([&] {
         check_rows(n, choices, width, dtype, order, "order");
+        ODIE_REQUIRE(n == 0 || slot, "slot is required");
         if (n == 0) return;
         ODIE_REQUIRE(rows && sorted, "rows and sorted are required");
         const int vector = row_vector(width, dtype, rows, sorted);
-        const RowArgs a{row_shape(n * choices, width * row_type_size(dtype) / vector), n * choices, choices, width, order, nullptr, weights};
-        with_rows(dtype, vector, a.shape.narrow, [&](auto type, auto bytes, auto narrow) {
+        const RowArgs a = sorted_args(n, choices, width, dtype, vector, order, slot, weights);
+        if (a.slot) {
+            with_row_type(dtype, vector, [&](auto type, auto bytes) {
+                using T = decltype(type);
+                dispatch_rows_kernel<T, decltype(bytes)::value>
+                    <<<row_blocks(a.shape, 1), ROW_THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+                        a, static_cast<const T*>(rows), static_cast<T*>(sorted));
+            });
+        } else with_rows(dtype, vector, a.shape.narrow, [&](auto type, auto bytes, auto narrow) {
             using T = decltype(type);
             dispatch_kernel<T, decltype(bytes)::value, decltype(narrow)::value>
                 <<<row_blocks(a.shape, 4), ROW_THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
@@ -248,15 +364,23 @@ extern "C" int odie_combine(const void* sorted, int64_t n, int choices, int64_t 
 }
 
 extern "C" int odie_combine_backward(const void* d_out, const void* sorted, int64_t n, int choices, int64_t width, int dtype,
-                                     const int32_t* order, const float* weights, void* d_sorted, float* d_weights,
-                                     uint64_t stream) {
+                                     const int32_t* order, const int32_t* slot, const float* weights, void* d_sorted,
+                                     float* d_weights, uint64_t stream) {
     return guarded([&] {
         check_rows(n, choices, width, dtype, order, "order");
+        ODIE_REQUIRE(n == 0 || slot, "slot is required");
         if (n == 0 || (!d_sorted && !d_weights)) return;
         ODIE_REQUIRE(d_out && (sorted || !d_weights), "d_out is required, and sorted for the weights' gradient");
         const int vector = row_vector(width, dtype, d_out, d_weights ? sorted : d_out, d_sorted);
-        const RowArgs a{row_shape(n * choices, width * row_type_size(dtype) / vector), n * choices, choices, width, order, nullptr, weights};
-        with_rows(dtype, vector, a.shape.narrow, [&](auto type, auto bytes, auto narrow) {
+        const RowArgs a = sorted_args(n, choices, width, dtype, vector, order, slot, weights);
+        if (a.slot) {
+            with_row_type(dtype, vector, [&](auto type, auto bytes) {
+                using T = decltype(type);
+                combine_backward_rows_kernel<T, decltype(bytes)::value>
+                    <<<row_blocks(a.shape, 1), ROW_THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+                        a, static_cast<const T*>(d_out), static_cast<const T*>(sorted), static_cast<T*>(d_sorted), d_weights);
+            });
+        } else with_rows(dtype, vector, a.shape.narrow, [&](auto type, auto bytes, auto narrow) {
             using T = decltype(type);
             combine_backward_kernel<T, decltype(bytes)::value, decltype(narrow)::value>
                 <<<row_blocks(a.shape, 2), ROW_THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(

@@ -139,7 +139,7 @@ __device__ __forceinline__ void group_rows(const int* offsets, int g, long long 
 //   DW   A = dz, B = x read along their columns (both MN-major), K = the group's rows; C = d W_g
 //
 // One warp loads (TMA, 128-byte swizzle, STAGES blocks in flight), one thread multiplies into one of two TMEM
-// accumulators, eight warps take the other one to global memory with bias, activation, residual and slope, so
+// accumulators, eight or sixteen warps take the other one to global memory with bias, activation, residual and slope, so
 // that the epilogue of one tile runs beside the products of the next.  Persistent: CTA (pair) i takes tiles i,
 // i + grid, ...  Rows of other groups that a tile loads are never stored (FWD, DX); for DW, whose sum runs over
 // the rows, each group has its own tensor maps that end at the group's last row, and the hardware reads zeros
@@ -147,10 +147,9 @@ __device__ __forceinline__ void group_rows(const int* offsets, int g, long long 
 enum Mode : int { FWD = 0, DX = 1, DW = 2 };
 
 constexpr int BK = 64;
-constexpr int GEMM_THREADS = 384, EPILOGUE_WARP = 4, EPILOGUE_WARPS = 8;
+constexpr int EPILOGUE_WARP = 4;  // the first one
 constexpr uint32_t WAIT_LIMIT = 1u << 22;
 constexpr int STAGING = 2048;  // bytes per epilogue warp: 32 rows x 32 columns of 16 bits
-constexpr int BIAS = 128;      // fp32 values per epilogue warp
 
 struct GemmArgs {
     int groups;
@@ -175,11 +174,16 @@ struct Shape {
     static constexpr int TM = 128 * CG;
     static constexpr int B_ROWS = BN / CG;  // per CTA
     static constexpr int A_BYTES = 128 * 128, B_BYTES = B_ROWS * 128, STAGE = A_BYTES + B_BYTES;
-    static constexpr int STAGES = 6;
+    static constexpr int STAGES = BN == 64 ? 6 : 5;
+    static constexpr int EPILOGUE_WARPS = BN == 64 ? 8 : 16;
+    static constexpr int THREADS = (EPILOGUE_WARP + EPILOGUE_WARPS) * 32;
+    static constexpr int GROUPS = EPILOGUE_WARPS / 4;      // of 32 columns, each to the four warps of a TMEM quadrant set
+    static constexpr int WINDOWS = BN / 32 / GROUPS;       // per warp and tile: columns 32 (group + GROUPS j)
+    static constexpr int WARP_BYTES = STAGING + WINDOWS * 128;  // staging tile and bias of an epilogue warp
     static constexpr int COLUMNS = 2 * BN;  // TMEM: two accumulators
     static constexpr int HEAD = 1024;       // barriers, TMEM address
     static int bytes(int groups) {
-        return 1024 + STAGES * STAGE + EPILOGUE_WARPS * (STAGING + BIAS * 4) + HEAD + (2 * (groups + 2)) * 4;
+        return 1024 + STAGES * STAGE + EPILOGUE_WARPS * WARP_BYTES + HEAD + (2 * (groups + 2)) * 4;
     }
 };
 
@@ -313,7 +317,7 @@ __device__ __forceinline__ void finish(float (&v)[32], uint32_t (&codes)[16], co
 }
 
 template <typename T, int MODE, int CG, int BN>
-__global__ void __launch_bounds__(GEMM_THREADS, 1)
+__global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GemmArgs p) {
     using S = Shape<CG, BN>;
     constexpr int STAGES = S::STAGES;
@@ -321,8 +325,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
     char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) / 1024 * 1024);
     char* stages = smem;
     char* staging = stages + STAGES * S::STAGE;
-    float* biases = reinterpret_cast<float*>(staging + EPILOGUE_WARPS * STAGING);
-    uint64_t* full = reinterpret_cast<uint64_t*>(staging + EPILOGUE_WARPS * (STAGING + BIAS * 4));
+    uint64_t* full = reinterpret_cast<uint64_t*>(staging + S::EPILOGUE_WARPS * S::WARP_BYTES);
     uint64_t* empty = full + STAGES;
     uint64_t* done = empty + STAGES;     // [2] accumulator summed
     uint64_t* drained = done + 2;        // [2] accumulator read out
@@ -342,7 +345,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
         }
         for (int a = 0; a < 2; ++a) {
             tc::bar_init(done + a, 1);
-            tc::bar_init(drained + a, EPILOGUE_WARPS * CG);
+            tc::bar_init(drained + a, S::EPILOGUE_WARPS * CG);
         }
         tc::bar_init(drain, 1);
         tc::fence_bar_init();
@@ -474,10 +477,10 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
             }
         }
     } else if (warp >= EPILOGUE_WARP) {
-        const int quadrant = warp & 3, half = (warp - EPILOGUE_WARP) >> 2;
-        constexpr int WINDOWS = BN / 64;  // of 32 columns for each warp: columns 32 (half + 2 j)
+        constexpr int WINDOWS = S::WINDOWS, STRIDE = 32 * S::GROUPS;
+        const int quadrant = warp & 3, group = (warp - EPILOGUE_WARP) >> 2;
         char* stage = staging + (warp - EPILOGUE_WARP) * STAGING;
-        float* bias = biases + (warp - EPILOGUE_WARP) * BIAS;
+        float* bias = reinterpret_cast<float*>(staging + S::EPILOGUE_WARPS * STAGING) + (warp - EPILOGUE_WARP) * WINDOWS * 32;
         const uint32_t lanes = tmem + (uint32_t(quadrant * 32) << 16);
         const bool wide = p.n % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.slope)) % 16 == 0;
         const bool wide_residual = p.n % 8 == 0 && reinterpret_cast<uintptr_t>(p.residual) % 16 == 0;
@@ -485,7 +488,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
         for (int t = start; t < tiles && fine; t += step) {
             const Tile tile = tile_at<MODE, CG, BN>(p, begin, first, t);
             const int acc = summed & 1;
-            const int row = tile.m0 + int(rank) * 128 + quadrant * 32, column0 = tile.n0 + half * 32;
+            const int row = tile.m0 + int(rank) * 128 + quadrant * 32, column0 = tile.n0 + group * 32;
             const long long at = (MODE == DW ? (long long)tile.g * p.m * p.n : 0) + (long long)row * p.n + column0;
             const uint16_t* residual = MODE == FWD && p.residual && !tile.zero ? static_cast<const uint16_t*>(p.residual) + at : nullptr;
             Window w{p.n, min(32, tile.m_end - row), p.n - column0, wide};
@@ -495,8 +498,8 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
                 if (residual && wr.wide) window_load(residual, wr, lane, r);
 #pragma unroll
                 for (int j = 0; j < WINDOWS; ++j)
-                    bias[j * 32 + lane] = p.bias && j * 64 + lane < w.columns
-                                              ? to_float(static_cast<const T*>(p.bias)[(long long)tile.g * p.n + column0 + j * 64 + lane])
+                    bias[j * 32 + lane] = p.bias && j * STRIDE + lane < w.columns
+                                              ? to_float(static_cast<const T*>(p.bias)[(long long)tile.g * p.n + column0 + j * STRIDE + lane])
                                               : 0.0f;
                 __syncwarp();
             }
@@ -507,7 +510,8 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
             }
 #pragma unroll 1
             for (int j = 0; j < WINDOWS; ++j) {
-                if (w.columns <= 0) break;
+                const bool last = j + 1 == WINDOWS || w.columns <= STRIDE;  // of this warp's windows inside the matrix
+                if (w.columns <= 0 && j > 0) break;
                 float v[32];
                 uint32_t codes[16];
                 if (tile.zero) {
@@ -516,11 +520,17 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
 #pragma unroll
                     for (int i = 0; i < 16; ++i) codes[i] = 0;
                 } else {
-                    tc::tmem_ld32(lanes + acc * BN + (half + 2 * j) * 32, v);
+                    tc::tmem_ld32(lanes + acc * BN + group * 32 + j * STRIDE, v);
+                    if (last) {  // the accumulator is free as soon as it is in registers
+                        tc::fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0)
+                            tc::bar_arrive_cluster(CG == 2 ? tc::leader_address(drained + acc) : tc::smem_u32(drained + acc));
+                    }
                 }
                 if (MODE == DW && p.partial) {
                     if (lane < w.rows) {
-                        float* to = p.partial + ((long long)tile.unit * p.m + row + lane) * p.n + column0 + j * 64;
+                        float* to = p.partial + ((long long)tile.unit * p.m + row + lane) * p.n + column0 + j * STRIDE;
                         if (p.n % 4 == 0) {
 #pragma unroll
                             for (int i = 0; i < 32; i += 4)
@@ -531,7 +541,7 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
                                 if (i < w.columns) to[i] = v[i];
                         }
                     }
-                    w.columns -= 64;
+                    w.columns -= STRIDE;
                     continue;
                 }
                 if (MODE == FWD && !tile.zero) {
@@ -539,11 +549,11 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
                         if (wr.wide) {
 #pragma unroll
                             for (int i = 0; i < 4; ++i) *staged(stage, lane / 4 + 8 * i, lane & 3) = r[i];
-                            wr.columns -= 64;
-                            if (j + 1 < WINDOWS && wr.columns > 0) window_load(residual + (j + 1) * 64, wr, lane, r);
+                            wr.columns -= STRIDE;
+                            if (j + 1 < WINDOWS && wr.columns > 0) window_load(residual + (j + 1) * STRIDE, wr, lane, r);
                         } else {
-                            window_fetch(residual + j * 64, wr, lane, stage);
-                            wr.columns -= 64;
+                            window_fetch(residual + j * STRIDE, wr, lane, stage);
+                            wr.columns -= STRIDE;
                         }
                         __syncwarp();
                     }
@@ -571,24 +581,19 @@ __global__ void __launch_bounds__(GEMM_THREADS, 1)
                     *staged(stage, lane, u) = make_uint4(pack_pair<T>(v[u * 8], v[u * 8 + 1]), pack_pair<T>(v[u * 8 + 2], v[u * 8 + 3]),
                                                          pack_pair<T>(v[u * 8 + 4], v[u * 8 + 5]), pack_pair<T>(v[u * 8 + 6], v[u * 8 + 7]));
                 __syncwarp();
-                window_store(static_cast<uint16_t*>(p.out) + at + j * 64, w, lane, stage);
+                window_store(static_cast<uint16_t*>(p.out) + at + j * STRIDE, w, lane, stage);
                 __syncwarp();
                 if (MODE == FWD && p.slope) {
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
                         *staged(stage, lane, u) = make_uint4(codes[u * 4], codes[u * 4 + 1], codes[u * 4 + 2], codes[u * 4 + 3]);
                     __syncwarp();
-                    window_store(p.slope + at + j * 64, w, lane, stage);
+                    window_store(p.slope + at + j * STRIDE, w, lane, stage);
                     __syncwarp();
                 }
-                w.columns -= 64;
+                w.columns -= STRIDE;
             }
-            if (!tile.zero) {
-                tc::fence_before_sync();
-                __syncwarp();
-                if (lane == 0) tc::bar_arrive_cluster(CG == 2 ? tc::leader_address(drained + acc) : tc::smem_u32(drained + acc));
-                ++summed;
-            }
+            if (!tile.zero) ++summed;
         }
         if (!fine && lane == 0) atomicExch(p.error, 2);
     }
@@ -879,7 +884,7 @@ void launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmArgs& p, 
     const int pairs = int(std::min<int64_t>(tiles, sm_count() / CG));
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(unsigned(pairs * CG));
-    config.blockDim = dim3(GEMM_THREADS);
+    config.blockDim = dim3(S::THREADS);
     config.dynamicSmemBytes = size_t(S::bytes(p.groups));
     config.stream = stream;
     cudaLaunchAttribute cluster{};

@@ -187,8 +187,9 @@ __device__ __forceinline__ uint32_t leader_address(const void* p) {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
+// Orders nothing but what tcgen05 fences order: a release would wait for the warp's stores to global memory.
 __device__ __forceinline__ void bar_arrive_cluster(uint32_t address) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(address) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(address) : "memory");
 }
 __device__ __forceinline__ void bar_expect(uint64_t* bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");

@@ -135,7 +135,7 @@ def _dispatch(x, order, weights):
     n, choices = order.slot.shape
     out = torch.empty((n * choices, x.shape[1]), dtype=x.dtype, device=x.device)
     _call('odie_dispatch', x.device, x.data_ptr(), n, choices, x.shape[1], ROW_TYPES[x.dtype], order.order.data_ptr(),
-          _lib.ptr(weights), out.data_ptr())
+          order.slot.data_ptr(), _lib.ptr(weights), out.data_ptr())
     return out
 
 
@@ -153,7 +153,8 @@ def _combine_backward(d_out, rows, order, weights, need_rows, need_weights):
     d_rows = torch.empty((n * choices, width), dtype=d_out.dtype, device=d_out.device) if need_rows else None
     d_weights = torch.empty((n, choices), dtype=torch.float32, device=d_out.device) if need_weights else None
     _call('odie_combine_backward', d_out.device, d_out.data_ptr(), _lib.ptr(rows), n, choices, width,
-          ROW_TYPES[d_out.dtype], order.order.data_ptr(), _lib.ptr(weights), _lib.ptr(d_rows), _lib.ptr(d_weights))
+          ROW_TYPES[d_out.dtype], order.order.data_ptr(), order.slot.data_ptr(), _lib.ptr(weights), _lib.ptr(d_rows),
+          _lib.ptr(d_weights))
     return d_rows, d_weights
 
 

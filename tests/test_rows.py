@@ -48,19 +48,22 @@ def test_sort_rows_refuses(lib, change, message):
     (dict(n=-1), 'pairs'), (dict(choices=0), 'pairs'), (dict(n=2 ** 30, choices=2), 'pairs'), (dict(width=0), 'elements'),
     (dict(dtype=3), 'element type'), (dict(dtype=-1), 'element type'), (dict(slot=None), 'is required'), (dict(rows=None), 'required'),
     (dict(out=None), 'required')])
-@pytest.mark.parametrize('name', ['odie_dispatch', 'odie_combine'])
-def test_dispatch_and_combine_refuse(lib, name, change, message):
+def test_dispatch_and_combine_refuse(lib, change, message):
     a = dict(rows=SOME, n=8, choices=2, width=8, dtype=0, slot=SOME, weights=None, out=SOME, stream=0)
     a.update(change)
-    assert getattr(lib, name)(*a.values()) == -1
+    assert lib.odie_combine(*a.values()) == -1
+    assert message in _lib.error()
+    a = dict(rows=SOME, n=8, choices=2, width=8, dtype=0, order=SOME, slot=SOME, weights=None, out=SOME, stream=0)
+    a.update(change)
+    assert lib.odie_dispatch(*a.values()) == -1
     assert message in _lib.error()
 
 
 @pytest.mark.parametrize('change, message', [
-    (dict(width=0), 'elements'), (dict(dtype=5), 'element type'), (dict(order=None), 'order'), (dict(d_out=None), 'required'),
+    (dict(width=0), 'elements'), (dict(dtype=5), 'element type'), (dict(order=None), 'order'), (dict(slot=None), 'slot'), (dict(d_out=None), 'required'),
     (dict(rows=None), 'required')])
 def test_combine_backward_refuses(lib, change, message):
-    a = dict(d_out=SOME, rows=SOME, n=8, choices=2, width=8, dtype=0, order=SOME, weights=None, d_rows=SOME, d_weights=SOME,
+    a = dict(d_out=SOME, rows=SOME, n=8, choices=2, width=8, dtype=0, order=SOME, slot=SOME, weights=None, d_rows=SOME, d_weights=SOME,
              stream=0)
     a.update(change)
     assert lib.odie_combine_backward(*a.values()) == -1
