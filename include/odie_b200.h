@@ -403,7 +403,8 @@ ODIE_API int odie_combine_backward(const void* d_out, const void* sorted, int64_
  * give zero rows.  activation: 0 none, 1 ReLU, 2 SiLU, 3 GELU (erf).  slope
  * (may be NULL) u16[rows][outputs]: act'(x W^T + b) for the backward pass, as
  * round(2^15 (act' + 1/4)), 65535 for NaN.
- * odie_linear_backward: with dz = d_y act' (slope NULL: act' = 1), rounded to
+ * odie_linear_backward: with dz = d_y act' (slope NULL: act' = 1; or, for a
+ * ReLU without residual, relu_y = its y, whose sign is act'), rounded to
  * the rows' type for the products: d_x = dz W, d_weight = dz^T x, d_bias =
  * sum of the unrounded dz over the group's rows and d_residual = d_y (each may
  * be NULL); zero for rows behind the last group and for empty groups.
@@ -414,8 +415,8 @@ ODIE_API int odie_linear(const void* x, const void* weight, const void* bias, co
                    int outputs, int groups, const int32_t* offsets, int dtype, int activation, void* y, uint16_t* slope,
                    void* scratch, uint64_t stream);
 ODIE_API int64_t odie_linear_backward_scratch(int64_t rows, int inputs, int outputs, int groups);
-ODIE_API int odie_linear_backward(const void* d_y, const uint16_t* slope, const void* x, const void* weight, int64_t rows,
-                   int inputs, int outputs, int groups, const int32_t* offsets, int dtype, void* d_x, void* d_weight,
+ODIE_API int odie_linear_backward(const void* d_y, const uint16_t* slope, const void* relu_y, const void* x, const void* weight,
+                   int64_t rows, int inputs, int outputs, int groups, const int32_t* offsets, int dtype, void* d_x, void* d_weight,
                    void* d_bias, void* d_residual, void* scratch, uint64_t stream);
 /* *status (device int32) = 0, or 2 once a bounded wait of the linear kernels on this
  * device has run out (their results are then incomplete). */

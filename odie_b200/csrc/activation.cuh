@@ -1,0 +1,138 @@
+// Activations of the linear layers with their slopes, two values at a time (linear.cu, thin.cu).
+#pragma once
+#include "rows.cuh"
+#include <type_traits>
+
+namespace odie {
+
+enum Activation : int { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3 };
+
+// Pairs of fp32 values: sm_100 multiplies and adds two per instruction.
+struct Pair {
+    unsigned long long v;
+};
+__device__ __forceinline__ Pair pair(float a, float b) {
+    Pair r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 both(Pair p) {
+    float2 r;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p.v));
+    return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return d;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
+__device__ __forceinline__ Pair same(float a) { return pair(a, a); }
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float inverse_approx(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// The slope's code, as the low bits of 2^23 + code (one fused multiply-add rounds to nearest; act' in (-1/4, 7/4)
+// needs no clamp).  A NaN slope is the canonical NaN, whose low 16 bits are 0xffff.
+__device__ __forceinline__ uint32_t slope_codes(Pair slope) {
+    const float2 c = both(fma2(slope, same(32768.0f), same(8388608.0f + 8192.0f)));
+    return __byte_perm(__float_as_uint(c.x), __float_as_uint(c.y), 0x5410);
+}
+__device__ __forceinline__ float slope_value(uint32_t c) {  // c: 16 bits
+    const float d = fmaf(__uint_as_float(0x4b000000u | c), 1.0f / 32768.0f, -256.25f);  // exact
+    return c == 0xffffu ? __int_as_float(0x7fffffff) : d;
+}
+
+// The slope of a ReLU by its output (NaN where that is NaN).
+__device__ __forceinline__ float sign_slope(float y) { return y > 0.0f ? 1.0f : y; }
+
+// act(z), with act'(z) in slope, of two values.
+//   SiLU  p = 1 / (1 + e^-z): z p and p + z p (1 - p).
+//   GELU  z P(z) and P(z) + z e^(-z^2/2) / sqrt(2 pi), P the normal distribution function by Abramowitz and
+//         Stegun 7.1.26: erfc(u) = (a1 t + .. + a5 t^5) e^(-u^2), t = 1 / (1 + 0.3275911 u), u = |z| / sqrt 2, off
+//         by at most 1.5e-7 absolutely; it shares the slope's exponential.
+// Written in pairs, and with one instruction each for exponential and inverse: the epilogue shares the SM with
+// nothing else, but at 45 instructions per element it took twice the products' time for 1024 inputs.
+template <int ACT>
+__device__ __forceinline__ Pair activate(Pair z, Pair& slope) {
+    constexpr float LOG2E = 1.4426950408889634f;
+    const float2 s = both(z);
+    if (ACT == ACT_RELU) {
+        const Pair r = pair(max_nan(s.x, 0.0f), max_nan(s.y, 0.0f));
+        slope = pair(s.x > 0.0f ? 1.0f : both(r).x, s.y > 0.0f ? 1.0f : both(r).y);  // 0 or NaN where z is not positive
+        return r;
+    }
+    if (ACT == ACT_SILU) {
+        const float2 x = both(mul2(z, same(-LOG2E)));
+        const float2 d = both(add2(pair(exp2_approx(x.x), exp2_approx(x.y)), same(1.0f)));
+        const Pair p = pair(inverse_approx(d.x), inverse_approx(d.y));
+        const Pair a = mul2(z, p);
+        slope = fma2(a, fma2(p, same(-1.0f), same(1.0f)), p);
+        return a;
+    }
+    if (ACT == ACT_GELU) {
+        const float2 x = both(mul2(mul2(z, z), same(-0.5f * LOG2E)));
+        const Pair e = pair(exp2_approx(x.x), exp2_approx(x.y));
+        const float2 d = both(fma2(pair(fabsf(s.x), fabsf(s.y)), same(0.3275911f * 0.70710678118654752f), same(1.0f)));
+        const Pair t = pair(inverse_approx(d.x), inverse_approx(d.y));
+        Pair q = fma2(t, same(0.5f * 1.061405429f), same(0.5f * -1.453152027f));
+        q = fma2(t, q, same(0.5f * 1.421413741f));
+        q = fma2(t, q, same(0.5f * -0.284496736f));
+        q = fma2(t, q, same(0.5f * 0.254829592f));
+        q = mul2(mul2(q, t), e);  // P(-|z|)
+        const float2 below = both(q), above = both(fma2(q, same(-1.0f), same(1.0f)));
+        const Pair p = pair(s.x < 0.0f ? below.x : above.x, s.y < 0.0f ? below.y : above.y);
+        slope = fma2(mul2(z, same(0.39894228040143268f)), e, p);
+        return mul2(z, p);
+    }
+    slope = same(1.0f);
+    return z;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
+    uint32_t r;
+    if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack_pair(uint32_t v) {
+    if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&v));
+    else return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+
+// Rows [begin, end) of group g: offsets clamped to [0, rows], so no offset reads or writes out of range.
+__device__ __forceinline__ long long clamp_offset(long long offset, long long rows) { return min(rows, max(0ll, offset)); }
+__device__ __forceinline__ void group_rows(const int* offsets, int g, long long rows, long long& begin, long long& end) {
+    if (!offsets) {
+        begin = 0;
+        end = rows;
+        return;
+    }
+    begin = g == 0 ? 0 : clamp_offset(offsets[g], rows);
+    end = max(begin, clamp_offset(offsets[g + 1], rows));
+}
+
+}  // namespace odie

@@ -5,128 +5,22 @@
 //
 // Rows of no group (behind the last offset) give zero rows of y and d x and add to no gradient.  Training keeps
 // act'(z) as a 16-bit fixed-point code (15 fraction bits above -1/4): act' lies in (-0.13, 1.13) for every
-// activation here, so the code is within 2^-16 of it, closer than a 16-bit float of it or of z would be.
+// activation here, so the code is within 2^-16 of it, closer than a 16-bit float of it or of z would be.  A ReLU
+// without residual keeps nothing: its output's sign is its slope.
 //
 // The three products are one tensor-core kernel (gemm_kernel) with another operand order each; see there.  dz is
 // rounded to the rows' type, because the tensor cores take 16-bit operands; the bias gradient sums it unrounded.
-#include "rows.cuh"
+#include "thin.cuh"
 #include "odie_b200.h"
 #include "tc.cuh"
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <algorithm>
+#include <initializer_list>
 #include <type_traits>
 
 namespace odie {
 namespace {
-
-enum Activation : int { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3 };
-
-// Pairs of fp32 values: sm_100 multiplies and adds two per instruction.
-struct Pair {
-    unsigned long long v;
-};
-__device__ __forceinline__ Pair pair(float a, float b) {
-    Pair r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float2 both(Pair p) {
-    float2 r;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p.v));
-    return r;
-}
-__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
-    Pair d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return d;
-}
-__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
-    Pair d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-    return d;
-}
-__device__ __forceinline__ Pair add2(Pair a, Pair b) {
-    Pair d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-    return d;
-}
-__device__ __forceinline__ Pair same(float a) { return pair(a, a); }
-__device__ __forceinline__ float exp2_approx(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-__device__ __forceinline__ float inverse_approx(float x) {
-    float r;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-
-// The slope's code, as the low bits of 2^23 + code (one fused multiply-add rounds to nearest; act' in (-1/4, 7/4)
-// needs no clamp).  A NaN slope is the canonical NaN, whose low 16 bits are 0xffff.
-__device__ __forceinline__ uint32_t slope_codes(Pair slope) {
-    const float2 c = both(fma2(slope, same(32768.0f), same(8388608.0f + 8192.0f)));
-    return __byte_perm(__float_as_uint(c.x), __float_as_uint(c.y), 0x5410);
-}
-__device__ __forceinline__ float slope_value(uint32_t c) {  // c: 16 bits
-    const float d = fmaf(__uint_as_float(0x4b000000u | c), 1.0f / 32768.0f, -256.25f);  // exact
-    return c == 0xffffu ? __int_as_float(0x7fffffff) : d;
-}
-
-// act(z), with act'(z) in slope, of two values.
-//   SiLU  p = 1 / (1 + e^-z): z p and p + z p (1 - p).
-//   GELU  z P(z) and P(z) + z e^(-z^2/2) / sqrt(2 pi), P the normal distribution function by Abramowitz and
-//         Stegun 7.1.26: erfc(u) = (a1 t + .. + a5 t^5) e^(-u^2), t = 1 / (1 + 0.3275911 u), u = |z| / sqrt 2, off
-//         by at most 1.5e-7 absolutely; it shares the slope's exponential.
-// Written in pairs, and with one instruction each for exponential and inverse: the epilogue shares the SM with
-// nothing else, but at 45 instructions per element it took twice the products' time for 1024 inputs.
-template <int ACT>
-__device__ __forceinline__ Pair activate(Pair z, Pair& slope) {
-    constexpr float LOG2E = 1.4426950408889634f;
-    const float2 s = both(z);
-    if (ACT == ACT_RELU) {
-        slope = pair(s.x > 0.0f ? 1.0f : s.x != s.x ? s.x : 0.0f, s.y > 0.0f ? 1.0f : s.y != s.y ? s.y : 0.0f);
-        return pair(s.x > 0.0f || s.x != s.x ? s.x : 0.0f, s.y > 0.0f || s.y != s.y ? s.y : 0.0f);
-    }
-    if (ACT == ACT_SILU) {
-        const float2 x = both(mul2(z, same(-LOG2E)));
-        const float2 d = both(add2(pair(exp2_approx(x.x), exp2_approx(x.y)), same(1.0f)));
-        const Pair p = pair(inverse_approx(d.x), inverse_approx(d.y));
-        const Pair a = mul2(z, p);
-        slope = fma2(a, fma2(p, same(-1.0f), same(1.0f)), p);
-        return a;
-    }
-    if (ACT == ACT_GELU) {
-        const float2 x = both(mul2(mul2(z, z), same(-0.5f * LOG2E)));
-        const Pair e = pair(exp2_approx(x.x), exp2_approx(x.y));
-        const float2 d = both(fma2(pair(fabsf(s.x), fabsf(s.y)), same(0.3275911f * 0.70710678118654752f), same(1.0f)));
-        const Pair t = pair(inverse_approx(d.x), inverse_approx(d.y));
-        Pair q = fma2(t, same(0.5f * 1.061405429f), same(0.5f * -1.453152027f));
-        q = fma2(t, q, same(0.5f * 1.421413741f));
-        q = fma2(t, q, same(0.5f * -0.284496736f));
-        q = fma2(t, q, same(0.5f * 0.254829592f));
-        q = mul2(mul2(q, t), e);  // P(-|z|)
-        const float2 below = both(q), above = both(fma2(q, same(-1.0f), same(1.0f)));
-        const Pair p = pair(s.x < 0.0f ? below.x : above.x, s.y < 0.0f ? below.y : above.y);
-        slope = fma2(mul2(z, same(0.39894228040143268f)), e, p);
-        return mul2(z, p);
-    }
-    slope = same(1.0f);
-    return z;
-}
-
-// Rows [begin, end) of group g: offsets clamped to [0, rows], so no offset reads or writes out of range.
-__device__ __forceinline__ long long clamp_offset(long long offset, long long rows) { return min(rows, max(0ll, offset)); }
-__device__ __forceinline__ void group_rows(const int* offsets, int g, long long rows, long long& begin, long long& end) {
-    if (!offsets) {
-        begin = 0;
-        end = rows;
-        return;
-    }
-    begin = g == 0 ? 0 : clamp_offset(offsets[g], rows);
-    end = max(begin, clamp_offset(offsets[g + 1], rows));
-}
 
 // ---------------------------------------------------------------- the tensor-core product
 //
@@ -138,8 +32,8 @@ __device__ __forceinline__ void group_rows(const int* offsets, int g, long long 
 //   DX   A = dz [rows][outputs] (K-major), B = W_g read along its columns (MN-major), K = outputs
 //   DW   A = dz, B = x read along their columns (both MN-major), K = the group's rows; C = d W_g
 //
-// One warp loads (TMA, 128-byte swizzle, STAGES blocks in flight), one thread multiplies into one of two TMEM
-// accumulators, eight or sixteen warps take the other one to global memory with bias, activation, residual and slope, so
+// One warp loads (TMA, 128-byte swizzle, STAGES blocks in flight), one thread multiplies into one of two (or four) TMEM
+// accumulators, sixteen warps take the other one to global memory with bias, activation, residual and slope, so
 // that the epilogue of one tile runs beside the products of the next.  Persistent: CTA (pair) i takes tiles i,
 // i + grid, ...  Rows of other groups that a tile loads are never stored (FWD, DX); for DW, whose sum runs over
 // the rows, each group has its own tensor maps that end at the group's last row, and the hardware reads zeros
@@ -175,12 +69,14 @@ struct Shape {
     static constexpr int B_ROWS = BN / CG;  // per CTA
     static constexpr int A_BYTES = 128 * 128, B_BYTES = B_ROWS * 128, STAGE = A_BYTES + B_BYTES;
     static constexpr int STAGES = BN == 64 ? 6 : 5;
-    static constexpr int EPILOGUE_WARPS = BN == 64 ? 8 : 16;
-    static constexpr int THREADS = (EPILOGUE_WARP + EPILOGUE_WARPS) * 32;
-    static constexpr int GROUPS = EPILOGUE_WARPS / 4;      // of 32 columns, each to the four warps of a TMEM quadrant set
-    static constexpr int WINDOWS = BN / 32 / GROUPS;       // per warp and tile: columns 32 (group + GROUPS j)
+    // Sixteen epilogue warps, four per set of 32 TMEM columns (GROUPS) of a tile; the short tiles of 64 columns are
+    // handed out to four such sets in turn (SETS), each with an accumulator of its own.
+    static constexpr int EPILOGUE_WARPS = 16, THREADS = (EPILOGUE_WARP + EPILOGUE_WARPS) * 32;
+    static constexpr int SETS = BN == 64 ? 4 : 1, GROUPS = EPILOGUE_WARPS / 4 / SETS;
+    static constexpr int WINDOWS = BN / 32 / GROUPS;            // per warp and tile: columns 32 (group + GROUPS j)
+    static constexpr int ACCUMULATORS = SETS == 1 ? 2 : SETS;
     static constexpr int WARP_BYTES = STAGING + WINDOWS * 128;  // staging tile and bias of an epilogue warp
-    static constexpr int COLUMNS = 2 * BN;  // TMEM: two accumulators
+    static constexpr int COLUMNS = ACCUMULATORS * BN;  // of TMEM
     static constexpr int HEAD = 1024;       // barriers, TMEM address
     static int bytes(int groups) {
         return 1024 + STAGES * STAGE + EPILOGUE_WARPS * WARP_BYTES + HEAD + (2 * (groups + 2)) * 4;
@@ -238,19 +134,6 @@ __device__ __forceinline__ Tile tile_at(const GemmArgs& p, const int* begin, con
         tile.zero = lo == p.groups;
     }
     return tile;
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
-    uint32_t r;
-    if constexpr (std::is_same<T, __half>::value) asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-    else asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
-    return r;
-}
-template <typename T>
-__device__ __forceinline__ float2 unpack_pair(uint32_t v) {
-    if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&v));
-    else return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
 
 // The staging tile of an epilogue warp: 32 rows of 64 bytes, the 16-byte units of a row permuted so that both a
@@ -327,9 +210,9 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
     char* staging = stages + STAGES * S::STAGE;
     uint64_t* full = reinterpret_cast<uint64_t*>(staging + S::EPILOGUE_WARPS * S::WARP_BYTES);
     uint64_t* empty = full + STAGES;
-    uint64_t* done = empty + STAGES;     // [2] accumulator summed
-    uint64_t* drained = done + 2;        // [2] accumulator read out
-    uint64_t* drain = drained + 2;
+    uint64_t* done = empty + STAGES;                  // per accumulator: summed
+    uint64_t* drained = done + S::ACCUMULATORS;       // per accumulator: read out
+    uint64_t* drain = drained + S::ACCUMULATORS;
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drain + 1);
     int* begin = reinterpret_cast<int*>(reinterpret_cast<char*>(full) + S::HEAD);  // [groups + 2] first row of each group
     int* first = begin + p.groups + 2;                                            // [groups + 2] first unit
@@ -343,9 +226,9 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
             tc::bar_init(full + s, 1);
             tc::bar_init(empty + s, 1);
         }
-        for (int a = 0; a < 2; ++a) {
+        for (int a = 0; a < S::ACCUMULATORS; ++a) {
             tc::bar_init(done + a, 1);
-            tc::bar_init(drained + a, S::EPILOGUE_WARPS * CG);
+            tc::bar_init(drained + a, S::EPILOGUE_WARPS / S::SETS * CG);
         }
         tc::bar_init(drain, 1);
         tc::fence_bar_init();
@@ -448,12 +331,11 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
             uint32_t used = 0, summed = 0;
             for (int t = start; t < tiles && fine; t += step) {
                 const Tile tile = tile_at<MODE, CG, BN>(p, begin, first, t);
-                if (tile.zero) continue;
-                const int acc = summed & 1;
-                fine = tc::bar_wait_cluster(drained + acc, ((summed >> 1) & 1) ^ 1, WAIT_LIMIT);
+                const int acc = summed % S::ACCUMULATORS;
+                fine = tc::bar_wait_cluster(drained + acc, ((summed / S::ACCUMULATORS) & 1) ^ 1, WAIT_LIMIT);
                 if (!fine) break;
                 tc::fence_after_sync();
-                for (int kb = 0; kb < tile.k_blocks; ++kb, ++used) {
+                for (int kb = 0; kb < tile.k_blocks && !tile.zero; ++kb, ++used) {
                     const int s = used % STAGES;
                     fine = tc::bar_wait_cluster(full + s, (used / STAGES) & 1, WAIT_LIMIT);
                     if (!fine) break;
@@ -478,16 +360,18 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
         }
     } else if (warp >= EPILOGUE_WARP) {
         constexpr int WINDOWS = S::WINDOWS, STRIDE = 32 * S::GROUPS;
-        const int quadrant = warp & 3, group = (warp - EPILOGUE_WARP) >> 2;
+        const int quadrant = warp & 3, group = ((warp - EPILOGUE_WARP) >> 2) % S::GROUPS;
+        const int set = ((warp - EPILOGUE_WARP) >> 2) / S::GROUPS;
         char* stage = staging + (warp - EPILOGUE_WARP) * STAGING;
         float* bias = reinterpret_cast<float*>(staging + S::EPILOGUE_WARPS * STAGING) + (warp - EPILOGUE_WARP) * WINDOWS * 32;
         const uint32_t lanes = tmem + (uint32_t(quadrant * 32) << 16);
         const bool wide = p.n % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.slope)) % 16 == 0;
         const bool wide_residual = p.n % 8 == 0 && reinterpret_cast<uintptr_t>(p.residual) % 16 == 0;
-        uint32_t summed = 0;
-        for (int t = start; t < tiles && fine; t += step) {
+        int bias_g = -1, bias_n0 = -1;  // whose bias is held
+        uint32_t summed = set;
+        for (int t = start + set * step; t < tiles && fine; t += S::SETS * step, summed += S::SETS) {
             const Tile tile = tile_at<MODE, CG, BN>(p, begin, first, t);
-            const int acc = summed & 1;
+            const int acc = summed % S::ACCUMULATORS;
             const int row = tile.m0 + int(rank) * 128 + quadrant * 32, column0 = tile.n0 + group * 32;
             const long long at = (MODE == DW ? (long long)tile.g * p.m * p.n : 0) + (long long)row * p.n + column0;
             const uint16_t* residual = MODE == FWD && p.residual && !tile.zero ? static_cast<const uint16_t*>(p.residual) + at : nullptr;
@@ -496,18 +380,20 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
             uint4 r[4];
             if (MODE == FWD && !tile.zero) {  // what does not need the sum is read while it is awaited
                 if (residual && wr.wide) window_load(residual, wr, lane, r);
+                if (tile.g != bias_g || tile.n0 != bias_n0) {
+                    bias_g = tile.g;
+                    bias_n0 = tile.n0;
 #pragma unroll
-                for (int j = 0; j < WINDOWS; ++j)
-                    bias[j * 32 + lane] = p.bias && j * STRIDE + lane < w.columns
+                    for (int j = 0; j < WINDOWS; ++j)
+                        bias[j * 32 + lane] = p.bias && j * STRIDE + lane < w.columns
                                               ? to_float(static_cast<const T*>(p.bias)[(long long)tile.g * p.n + column0 + j * STRIDE + lane])
                                               : 0.0f;
-                __syncwarp();
+                    __syncwarp();
+                }
             }
-            if (!tile.zero) {
-                fine = __all_sync(0xffffffffu, tc::bar_wait_cluster(done + acc, (summed >> 1) & 1, WAIT_LIMIT));
-                if (!fine) break;
-                tc::fence_after_sync();
-            }
+            fine = __all_sync(0xffffffffu, tc::bar_wait_cluster(done + acc, (summed / S::ACCUMULATORS) & 1, WAIT_LIMIT));
+            if (!fine) break;
+            tc::fence_after_sync();
 #pragma unroll 1
             for (int j = 0; j < WINDOWS; ++j) {
                 const bool last = j + 1 == WINDOWS || w.columns <= STRIDE;  // of this warp's windows inside the matrix
@@ -521,12 +407,11 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
                     for (int i = 0; i < 16; ++i) codes[i] = 0;
                 } else {
                     tc::tmem_ld32(lanes + acc * BN + group * 32 + j * STRIDE, v);
-                    if (last) {  // the accumulator is free as soon as it is in registers
-                        tc::fence_before_sync();
-                        __syncwarp();
-                        if (lane == 0)
-                            tc::bar_arrive_cluster(CG == 2 ? tc::leader_address(drained + acc) : tc::smem_u32(drained + acc));
-                    }
+                }
+                if (last) {  // the accumulator is free as soon as it is in registers
+                    tc::fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) tc::bar_arrive_cluster(CG == 2 ? tc::leader_address(drained + acc) : tc::smem_u32(drained + acc));
                 }
                 if (MODE == DW && p.partial) {
                     if (lane < w.rows) {
@@ -593,7 +478,6 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
                 }
                 w.columns -= STRIDE;
             }
-            if (!tile.zero) ++summed;
         }
         if (!fine && lane == 0) atomicExch(p.error, 2);
     }
@@ -628,9 +512,10 @@ __global__ void __launch_bounds__(32) group_maps_kernel(const __grid_constant__ 
 }
 
 // d W from the units' sums: a block per 32 elements, each warp over its share of the units, the shares in order.
+// A unit holds `size` sums of d W and `bias` sums of d b (either may be unwanted: null).
 template <typename T>
-__global__ void __launch_bounds__(256) join_kernel(const float* partial, T* out, const int* offsets, long long rows, int chunk,
-                                                   long long size) {
+__global__ void __launch_bounds__(256) join_kernel(const float* partial, T* d_weight, T* d_bias, const int* offsets, long long rows,
+                                                   int chunk, long long size, int bias) {
     __shared__ float part[8][33];
     const int g = blockIdx.y, lane = threadIdx.x & 31, line = threadIdx.x >> 5;
     long long unit = 0, begin, end;
@@ -640,21 +525,23 @@ __global__ void __launch_bounds__(256) join_kernel(const float* partial, T* out,
     }
     group_rows(offsets, g, rows, begin, end);
     const int count = int(max(1ll, (end - begin + chunk - 1) / chunk)), share = (count + 7) / 8;
-    const int from = min(count, line * share), to = min(count, from + share);
-    for (long long i0 = (long long)blockIdx.x * 32; i0 < size; i0 += (long long)gridDim.x * 32) {
+    const int from = min(count, line * share), last = min(count, from + share);
+    const long long all = size + bias;
+    for (long long i0 = (long long)blockIdx.x * 32; i0 < all; i0 += (long long)gridDim.x * 32) {
         const long long i = i0 + lane;
+        T* to = i < size ? (d_weight ? d_weight + g * size + i : nullptr) : i < all && d_bias ? d_bias + (long long)g * bias + (i - size) : nullptr;
         float sum = 0.0f;
-        if (i < size) {
+        if (to) {
 #pragma unroll 8
-            for (int u = from; u < to; ++u) sum += partial[(unit + u) * size + i];
+            for (int u = from; u < last; ++u) sum += partial[(unit + u) * all + i];
         }
         part[line][lane] = sum;
         __syncthreads();
-        if (line == 0 && i < size) {
+        if (line == 0 && to) {
             sum = part[0][lane];
 #pragma unroll
             for (int w = 1; w < 8; ++w) sum += part[w][lane];
-            out[g * size + i] = from_float<T>(sum);
+            *to = from_float<T>(sum);
         }
         __syncthreads();
     }
@@ -663,11 +550,12 @@ __global__ void __launch_bounds__(256) join_kernel(const float* partial, T* out,
 // ---------------------------------------------------------------- dz and the bias gradient
 struct DzArgs {
     const void* d_y;
-    const uint16_t* slope;  // null: 1
+    const uint16_t* slope;  // codes; null: 1
+    const void* y;          // instead of codes: the output of a ReLU, whose slope is its sign
     void* dz;               // null: not wanted
     void* d_residual;
-    float* partial;         // [row blocks][n] sums of dz, or null
-    void* d_bias;
+    void* d_bias;           // null: not wanted
+    float* partial;         // [row blocks][n] sums of dz; null: one block holds all rows and writes d_bias itself
     long long rows;
     int n;
     long long ld;           // of dz
@@ -680,16 +568,17 @@ struct DzArgs {
 template <typename T>
 __device__ __forceinline__ void dz_load(const DzArgs& a, long long row, int column, float (&v)[8], uint4& raw) {
     const uint16_t* from = static_cast<const uint16_t*>(a.d_y) + row * a.n + column;
+    const uint16_t* slope = a.slope ? a.slope : static_cast<const uint16_t*>(a.y);
     uint4 s = make_uint4(0, 0, 0, 0);
     if (a.wide) {
         raw = __ldg(reinterpret_cast<const uint4*>(from));
-        if (a.slope) s = __ldg(reinterpret_cast<const uint4*>(a.slope + row * a.n + column));
+        if (slope) s = __ldg(reinterpret_cast<const uint4*>(slope + row * a.n + column));
     } else {
         uint16_t e[8], f[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             e[j] = column + j < a.n ? from[j] : uint16_t(0);
-            f[j] = a.slope && column + j < a.n ? a.slope[row * a.n + column + j] : uint16_t(0);
+            f[j] = slope && column + j < a.n ? slope[row * a.n + column + j] : uint16_t(0);
         }
         raw = make_uint4(e[0] | uint32_t(e[1]) << 16, e[2] | uint32_t(e[3]) << 16, e[4] | uint32_t(e[5]) << 16,
                          e[6] | uint32_t(e[7]) << 16);
@@ -700,8 +589,16 @@ __device__ __forceinline__ void dz_load(const DzArgs& a, long long row, int colu
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float2 f = unpack_pair<T>(y[i]);
-        v[2 * i] = a.slope ? f.x * slope_value(c[i] & 0xffffu) : f.x;
-        v[2 * i + 1] = a.slope ? f.y * slope_value(c[i] >> 16) : f.y;
+        v[2 * i] = f.x;
+        v[2 * i + 1] = f.y;
+        if (a.slope) {
+            v[2 * i] *= slope_value(c[i] & 0xffffu);
+            v[2 * i + 1] *= slope_value(c[i] >> 16);
+        } else if (a.y) {
+            const float2 o = unpack_pair<T>(c[i]);
+            v[2 * i] *= sign_slope(o.x);
+            v[2 * i + 1] *= sign_slope(o.y);
+        }
     }
 }
 
@@ -741,7 +638,7 @@ __global__ void __launch_bounds__(256) dz_kernel(DzArgs a, int lanes_log2) {
             for (int i = 0; i < 8; ++i) sum[i] += v[i];
         }
     }
-    if (!a.partial) return;
+    if (!a.d_bias) return;
 #pragma unroll
     for (int i = 0; i < 8; ++i) sums[threadIdx.x][i] = sum[i];
     __syncthreads();
@@ -750,7 +647,8 @@ __global__ void __launch_bounds__(256) dz_kernel(DzArgs a, int lanes_log2) {
         if (at >= a.n) continue;
         float total = 0.0f;
         for (int l = 0; l < lines; ++l) total += sums[l * lanes + c][e];
-        a.partial[(long long)blockIdx.x * a.n + at] = total;
+        if (a.partial) a.partial[(long long)blockIdx.x * a.n + at] = total;
+        else static_cast<T*>(a.d_bias)[at] = from_float<T>(total);
     }
 }
 
@@ -773,7 +671,8 @@ __global__ void __launch_bounds__(256) bias_kernel(DzArgs a) {
 #pragma unroll 4
             for (long long row = from + line; row < to; row += 8) {
                 const float v = to_float(d_y[row * a.n + c]);
-                sum += a.slope ? v * slope_value(a.slope[row * a.n + c]) : v;
+                sum += a.slope ? v * slope_value(a.slope[row * a.n + c])
+                       : a.y ? v * sign_slope(to_float(static_cast<const T*>(a.y)[row * a.n + c])) : v;
             }
         };
         rows(begin, head);
@@ -790,18 +689,93 @@ __global__ void __launch_bounds__(256) bias_kernel(DzArgs a) {
     }
 }
 
-// Rows whose length is no multiple of 16 bytes, copied to ones that are: TMA reads no others.
-__global__ void __launch_bounds__(256) pad_kernel(const uint16_t* from, uint16_t* to, long long rows, int width, int ld) {
-    const long long count = rows * (ld / 8);
+// Rows whose length is no multiple of 16 bytes, copied to ones that are, zeros behind: TMA reads no others.  Two
+// matrices of one width in one launch.
+__global__ void __launch_bounds__(256) pad_kernel(const uint16_t* from0, uint16_t* to0, long long rows0, const uint16_t* from1,
+                                                  uint16_t* to1, long long rows1, int width, int ld) {
+    const int units = ld / 8;
+    const long long count = (rows0 + rows1) * units;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < count; i += (long long)gridDim.x * 256) {
-        const long long row = i / (ld / 8);
-        const int c = int(i % (ld / 8)) * 8;
+        long long row = i / units;
+        const int c = int(i % units) * 8;
+        const uint16_t* from = row < rows0 ? from0 : from1;
+        uint16_t* to = row < rows0 ? to0 : to1;
+        if (row >= rows0) row -= rows0;
         uint16_t e[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) e[j] = c + j < width ? from[row * width + c + j] : uint16_t(0);
         *reinterpret_cast<uint4*>(to + row * ld + c) = make_uint4(e[0] | uint32_t(e[1]) << 16, e[2] | uint32_t(e[3]) << 16,
                                                                   e[4] | uint32_t(e[5]) << 16, e[6] | uint32_t(e[7]) << 16);
     }
+}
+
+// ---------------------------------------------------------------- a few rows
+// Up to eight rows: y is bound by the bytes of W, which every warp reads straight into registers, one row of W (one
+// output) per warp and U vectors in flight per lane; x comes from L1.  (The tensor-core tiles, 128 rows each, took
+// 26 us for one row of 4096 x 4096 bf16: 32 CTAs cannot draw the memory's rate.)
+struct FewArgs {
+    const void* x;
+    const void* weight;
+    const void* bias;
+    const void* residual;
+    void* y;
+    uint16_t* slope;
+    int rows, inputs, outputs;
+    int activation;
+};
+
+constexpr int FEW_ROWS = 8, FEW_THREADS = 128;
+
+template <typename T, int BYTES, int M>
+__global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(FewArgs a) {
+    using P = Pack<T, BYTES>;
+    constexpr int U = M <= 2 ? 16 : 8;
+    const int lane = threadIdx.x & 31, n = blockIdx.x * (FEW_THREADS / 32) + (threadIdx.x >> 5);
+    if (n >= a.outputs) return;
+    const T* w = static_cast<const T*>(a.weight) + (long long)n * a.inputs;
+    const T* x = static_cast<const T*>(a.x);
+    float sum[M];
+#pragma unroll
+    for (int m = 0; m < M; ++m) sum[m] = 0.0f;
+    for (int k0 = lane * P::N; k0 < a.inputs; k0 += 32 * P::N * U) {
+        P v[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = k0 + u * 32 * P::N;
+            v[u] = k < a.inputs ? P::load_once(w + k) : P::zero();
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = k0 + u * 32 * P::N;
+            if (k >= a.inputs) break;
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+                const P q = P::load(x + (long long)min(m, a.rows - 1) * a.inputs + k);
+#pragma unroll
+                for (int e = 0; e < P::N; ++e) sum[m] = fmaf(to_float(v[u].v[e]), to_float(q.v[e]), sum[m]);
+            }
+        }
+    }
+    float mine = 0.0f;
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) sum[m] += __shfl_xor_sync(0xffffffffu, sum[m], d);
+        if (lane == m) mine = sum[m];
+    }
+    if (lane >= min(M, a.rows)) return;
+    const long long at = (long long)lane * a.outputs + n;
+    if (a.bias) mine += to_float(static_cast<const T*>(a.bias)[n]);
+    Pair slope;
+    Pair z = same(mine);
+    if (a.activation == ACT_RELU) z = activate<ACT_RELU>(z, slope);
+    else if (a.activation == ACT_SILU) z = activate<ACT_SILU>(z, slope);
+    else if (a.activation == ACT_GELU) z = activate<ACT_GELU>(z, slope);
+    else z = activate<ACT_NONE>(z, slope);
+    float v = both(z).x;
+    if (a.residual) v += to_float(static_cast<const T*>(a.residual)[at]);
+    static_cast<T*>(a.y)[at] = from_float<T>(v);
+    if (a.slope) a.slope[at] = uint16_t(slope_codes(slope));
 }
 
 // ---------------------------------------------------------------- host
@@ -897,10 +871,38 @@ void launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmArgs& p, 
     note_launch();
 }
 
-void launch_pad(const void* from, void* to, int64_t rows, int width, cudaStream_t stream) {
+void launch_pad(const void* from0, void* to0, int64_t rows0, const void* from1, void* to1, int64_t rows1, int width, cudaStream_t stream) {
     const int ld = int(round8(width));
-    const int64_t blocks = std::min<int64_t>(ceil_div(rows * (ld / 8), 256), 32 * sm_count());
-    pad_kernel<<<unsigned(blocks), 256, 0, stream>>>(static_cast<const uint16_t*>(from), static_cast<uint16_t*>(to), rows, width, ld);
+    const int64_t blocks = std::min<int64_t>(ceil_div((rows0 + rows1) * (ld / 8), 256), 32 * sm_count());
+    pad_kernel<<<unsigned(blocks), 256, 0, stream>>>(static_cast<const uint16_t*>(from0), static_cast<uint16_t*>(to0), rows0,
+                                                     static_cast<const uint16_t*>(from1), static_cast<uint16_t*>(to1), rows1, width, ld);
+    ODIE_CUDA(cudaGetLastError());
+    note_launch();
+}
+
+template <typename T>
+void launch_few_rows(const FewArgs& a, cudaStream_t stream) {
+    const unsigned blocks = unsigned(ceil_div(a.outputs, FEW_THREADS / 32));
+    const int vector = row_vector(a.inputs, ROW_F16, a.x, a.weight);
+    auto go = [&](auto bytes) {
+        constexpr int B = decltype(bytes)::value;
+        if (a.rows == 1) few_rows_kernel<T, B, 1><<<blocks, FEW_THREADS, 0, stream>>>(a);
+        else if (a.rows == 2) few_rows_kernel<T, B, 2><<<blocks, FEW_THREADS, 0, stream>>>(a);
+        else if (a.rows <= 4) few_rows_kernel<T, B, 4><<<blocks, FEW_THREADS, 0, stream>>>(a);
+        else few_rows_kernel<T, B, 8><<<blocks, FEW_THREADS, 0, stream>>>(a);
+    };
+    if (vector == 16) go(std::integral_constant<int, 16>{});
+    else if (vector == 4) go(std::integral_constant<int, 4>{});
+    else go(std::integral_constant<int, 2>{});
+    ODIE_CUDA(cudaGetLastError());
+    note_launch();
+}
+
+template <typename T>
+void launch_join(const float* partial, void* d_weight, void* d_bias, const int* offsets, int groups, int64_t rows, int64_t chunk,
+                 int64_t size, int bias, cudaStream_t stream) {
+    join_kernel<T><<<dim3(unsigned(std::min<int64_t>(ceil_div(size + bias, 32), 4096)), unsigned(groups)), 256, 0, stream>>>(
+        partial, static_cast<T*>(d_weight), static_cast<T*>(d_bias), offsets, rows, int(chunk), size, bias);
     ODIE_CUDA(cudaGetLastError());
     note_launch();
 }
@@ -915,6 +917,12 @@ struct Scratch {
         return p;
     }
 };
+
+bool on_16_bytes(std::initializer_list<const void*> pointers) {
+    uintptr_t bits = 0;
+    for (const void* p : pointers) bits |= uintptr_t(p);
+    return bits % 16 == 0;
+}
 
 // ---- the pieces of scratch, in order; the size functions walk the same list
 struct ForwardScratch {
@@ -941,12 +949,14 @@ struct WeightUnits {
         tiles = ceil_div(outputs, 128 * config.cg) * ceil_div(inputs, config.bn);
         const int64_t wanted = 2 * SMS / config.cg, have = tiles * groups;
         chunk = std::max<int64_t>(BK, ceil_div(rows, BK) * BK);
-        split = have < wanted / 2 && rows > 4 * BK;
-        if (split) chunk = std::max<int64_t>(4 * BK, ceil_div(ceil_div(rows * tiles, wanted), BK) * BK);
+        split = have < wanted / 2 && rows > 32 * BK;  // a second kernel joins the sums: 2048 rows are walked sooner
+        if (split) chunk = std::max<int64_t>(8 * BK, ceil_div(ceil_div(rows * tiles, wanted), BK) * BK);
         units = split ? ceil_div(rows, chunk) + groups : groups;  // at most
     }
 };
 
+// One group of up to 4096 rows: a block sums all rows of its columns, and no second kernel is needed.
+bool dz_direct(int64_t rows, const int32_t* offsets) { return rows <= 4096 && !offsets; }
 int dz_block_rows(int64_t rows, int groups) {
     // at most about 512 sums for one group; for several, short blocks, since the rows at a group's ends are read twice
     const int64_t r = groups == 1 ? ceil_div(rows, 512) : ceil_div(rows, int64_t(groups) * 16);
@@ -955,7 +965,7 @@ int dz_block_rows(int64_t rows, int groups) {
 
 struct BackwardScratch {
     void *dz, *x, *weight, *maps;
-    float *bias, *partial;
+    float *bias, *partial, *thin;
     int64_t bytes;
     BackwardScratch(void* base, int64_t rows, int inputs, int outputs, int groups) {
         Scratch s{static_cast<char*>(base)};
@@ -968,6 +978,9 @@ struct BackwardScratch {
         const WeightUnits u(rows, inputs, outputs, groups);
         partial = static_cast<float*>(u.split ? s.take(u.units * outputs * int64_t(inputs) * 4) : nullptr);
         bytes = s.used;
+        thin = static_cast<float*>(base);  // thin layers need nothing else
+        if (thin_sizes(inputs, outputs))
+            bytes = std::max(bytes, aligned(thin_units(rows, groups, thin_chunk(rows, true)) * (int64_t(outputs) * inputs + outputs) * 4));
     }
 };
 
@@ -994,12 +1007,34 @@ extern "C" int odie_linear(const void* x, const void* weight, const void* bias, 
         if (rows == 0) return;
         ODIE_REQUIRE(x && weight && y, "x, weight and y are required");
         const cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_handle);
+        if (rows <= FEW_ROWS && !offsets) {
+            const FewArgs a{x, weight, bias, residual, y, slope, int(rows), inputs, outputs, activation};
+            with_linear_type(dtype, [&](auto type) { launch_few_rows<decltype(type)>(a, stream); });
+            return;
+        }
+        if (thin_sizes(inputs, outputs) && on_16_bytes({x, weight, residual, y, slope})) {
+            ThinArgs a{};
+            a.rows = rows;
+            a.inputs = inputs;
+            a.outputs = outputs;
+            a.groups = groups;
+            a.offsets = offsets;
+            a.chunk = thin_chunk(rows, false);
+            a.x = x;
+            a.weight = weight;
+            a.bias = bias;
+            a.residual = residual;
+            a.y = y;
+            a.slope = slope;
+            a.activation = activation;
+            with_linear_type(dtype, [&](auto type) { launch_thin_forward<decltype(type)>(a, stream); });
+            return;
+        }
         const ForwardScratch s(scratch, rows, inputs, outputs, groups);
         ODIE_REQUIRE(scratch || s.bytes == 0, "scratch is required");
         const int64_t ld = round8(inputs);
         if (s.x) {
-            launch_pad(x, s.x, rows, inputs, stream);
-            launch_pad(weight, s.weight, int64_t(groups) * outputs, inputs, stream);
+            launch_pad(x, s.x, rows, weight, s.weight, int64_t(groups) * outputs, inputs, stream);
             x = s.x;
             weight = s.weight;
         }
@@ -1032,7 +1067,7 @@ extern "C" int64_t odie_linear_backward_scratch(int64_t rows, int inputs, int ou
     return BackwardScratch(nullptr, rows, inputs, outputs, groups).bytes;
 }
 
-extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, const void* x, const void* weight, int64_t rows,
+extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, const void* relu_y, const void* x, const void* weight, int64_t rows,
                                     int inputs, int outputs, int groups, const int32_t* offsets, int dtype, void* d_x,
                                     void* d_weight, void* d_bias, void* d_residual, void* scratch, uint64_t stream_handle) {
     return guarded([&] {
@@ -1044,11 +1079,39 @@ extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, cons
             return;
         }
         ODIE_REQUIRE(d_y && (x || !d_weight) && (weight || !d_x) && scratch, "d_y, x, weight and scratch are required");
+        ODIE_REQUIRE(!slope || !relu_y, "slope and relu_y exclude each other");
         const BackwardScratch s(scratch, rows, inputs, outputs, groups);
+        if (thin_sizes(inputs, outputs) && on_16_bytes({d_y, slope, relu_y, x, weight, d_x, d_residual})) {
+            ThinArgs a{};
+            a.rows = rows;
+            a.inputs = inputs;
+            a.outputs = outputs;
+            a.groups = groups;
+            a.offsets = offsets;
+            a.chunk = thin_chunk(rows, true);
+            a.x = x;
+            a.weight = weight;
+            a.d_y = d_y;
+            a.code = slope;
+            a.relu_y = relu_y;
+            a.d_x = d_x;
+            a.d_weight = d_weight;
+            a.d_bias = d_bias;
+            a.d_residual = d_residual;
+            const bool join = rows > a.chunk && (d_weight || d_bias);
+            a.partial = join ? s.thin : nullptr;
+            with_linear_type(dtype, [&](auto type) {
+                using T = decltype(type);
+                launch_thin_backward<T>(a, stream);
+                if (join)
+                    launch_join<T>(s.thin, d_weight, d_bias, offsets, groups, rows, a.chunk, int64_t(outputs) * inputs, outputs, stream);
+            });
+            return;
+        }
         const bool bf16 = dtype == ROW_BF16;
         const int64_t ld_x = round8(inputs), ld_z = round8(outputs);
         const bool products = d_x || d_weight;
-        const bool as_is = !slope && outputs % 8 == 0;  // dz is d_y
+        const bool as_is = !slope && !relu_y && outputs % 8 == 0;  // dz is d_y
         const void* dz = as_is ? d_y : s.dz;
         with_linear_type(dtype, [&](auto type) {
             using T = decltype(type);
@@ -1056,28 +1119,32 @@ extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, cons
                 DzArgs a{};
                 a.d_y = d_y;
                 a.slope = slope;
+                a.y = relu_y;
                 a.dz = products && !as_is ? s.dz : nullptr;
                 a.d_residual = d_residual;
-                a.partial = d_bias ? s.bias : nullptr;
+                const bool direct = dz_direct(rows, offsets);
+                a.partial = direct ? nullptr : s.bias;
                 a.d_bias = d_bias;
                 a.rows = rows;
                 a.n = outputs;
                 a.ld = ld_z;
-                a.block_rows = dz_block_rows(rows, groups);
+                a.block_rows = direct ? int(rows) : dz_block_rows(rows, groups);
                 a.groups = groups;
                 a.offsets = offsets;
-                a.wide = outputs % 8 == 0 && (uintptr_t(d_y) | uintptr_t(slope) | uintptr_t(d_residual)) % 16 == 0;
+                a.wide = outputs % 8 == 0 && (uintptr_t(d_y) | uintptr_t(slope) | uintptr_t(relu_y) | uintptr_t(d_residual)) % 16 == 0;
                 int log2 = 0;
-                while (log2 < 5 && (8 << log2) < outputs) ++log2;
+                while (log2 < (direct ? 1 : 5) && (8 << log2) < outputs) ++log2;  // direct: 16 columns and 128 rows at a time
                 dz_kernel<T><<<dim3(unsigned(ceil_div(rows, a.block_rows)), unsigned(ceil_div(outputs, 8 << log2))), 256, 0, stream>>>(a, log2);
                 ODIE_CUDA(cudaGetLastError());
                 note_launch();
-                if (d_bias) {
+                if (d_bias && !direct) {
                     bias_kernel<T><<<dim3(unsigned(ceil_div(outputs, 32)), unsigned(groups)), 256, 0, stream>>>(a);
                     ODIE_CUDA(cudaGetLastError());
                     note_launch();
                 }
             }
+            if (s.x && products)
+                launch_pad(x, s.x, d_weight ? rows : 0, weight, s.weight, d_x ? int64_t(groups) * outputs : 0, inputs, stream);
             GemmArgs p{};
             p.groups = groups;
             p.offsets = offsets;
@@ -1085,7 +1152,6 @@ extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, cons
             p.n = inputs;
             p.error = error_word();
             if (d_x) {
-                if (s.weight) launch_pad(weight, s.weight, int64_t(groups) * outputs, inputs, stream);
                 p.k = outputs;
                 p.out = d_x;
                 with_config(tile_config(ceil_div(rows, groups), inputs, groups), [&](auto cg, auto bn) {
@@ -1096,7 +1162,6 @@ extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, cons
                 });
             }
             if (d_weight) {
-                if (s.x) launch_pad(x, s.x, rows, inputs, stream);
                 const WeightUnits u(rows, inputs, outputs, groups);
                 const CUtensorMap a = tensor_map(dz, bf16, outputs, rows, 0, ld_z, 64);
                 const CUtensorMap b = tensor_map(s.x ? s.x : x, bf16, inputs, rows, 0, ld_x, 64);
@@ -1115,10 +1180,7 @@ extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, cons
                 });
                 if (u.split) {
                     const int64_t size = int64_t(outputs) * inputs;
-                    join_kernel<T><<<dim3(unsigned(std::min<int64_t>(ceil_div(size, 32), 4096)), unsigned(groups)), 256, 0, stream>>>(
-                        s.partial, static_cast<T*>(d_weight), offsets, rows, int(u.chunk), size);
-                    ODIE_CUDA(cudaGetLastError());
-                    note_launch();
+                    launch_join<T>(s.partial, d_weight, nullptr, offsets, groups, rows, u.chunk, int64_t(outputs) * inputs, 0, stream);
                 }
             }
         });

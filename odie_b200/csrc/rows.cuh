@@ -40,6 +40,17 @@ struct alignas(BYTES) Pack {
         *reinterpret_cast<typename Raw<BYTES>::type*>(&r) = __ldg(reinterpret_cast<const typename Raw<BYTES>::type*>(p));
         return r;
     }
+    // Read once: not kept in L1, whose lines are for what is read again.
+    __device__ __forceinline__ static Pack load_once(const T* p) {
+        Pack r;
+        if constexpr (BYTES == 16) {
+            uint4& v = *reinterpret_cast<uint4*>(&r);
+            asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+            return r;
+        } else {
+            return load(p);
+        }
+    }
     __device__ __forceinline__ static Pack zero() {
         Pack r;
         *reinterpret_cast<typename Raw<BYTES>::type*>(&r) = typename Raw<BYTES>::type{};

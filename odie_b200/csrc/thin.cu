@@ -1,0 +1,399 @@
+// Linear layers of up to 64 inputs and outputs: forward, and the whole backward pass (dz, d x, d W, d b) in one kernel.
+//
+// Bound by the bytes of the rows (64 to 128 bytes each), not by arithmetic: 2^20 rows of 32 -> 64 fp16 are 192 MB
+// forward against 4.3 GFLOP.  So a warp keeps its 16 rows in registers from the 16-byte loads to the 16-byte stores
+// and multiplies them with mma.sync fragments.  (The tensor-core tiles of linear.cu, whose rows pass through shared
+// memory, TMEM and a staging tile, took 102 us forward and 205 us in four kernels backward.)
+//
+// The fragments' order of columns is chosen so that no data is exchanged.  Lane (g, c) = (lane / 4, lane % 4) loads
+// the 8 columns 8 c .. 8 c + 7 of rows g and g + 8 for each 32-column block: word i (columns 8 c + 2 i, + 1) is what
+// m16n8k16 wants of row g for K-step i / 2, first (i even) or second (i odd) half, if K is counted in this order;
+// W is read in the same order.  Column n' of output tile j stands for column 8 (n' / 2) + 2 j + n' % 2, so a lane
+// ends with the 8 columns 8 c .. 8 c + 7 of the result.  d W = dz^T x needs dz and x by columns: movmatrix turns
+// each 8 x 8 tile, in the same order of columns.
+#include "thin.cuh"
+#include "odie_b200.h"
+#include <algorithm>
+
+namespace odie {
+namespace {
+
+constexpr int THREADS = 128, WARPS = 4;
+
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    if constexpr (std::is_same<T, __half>::value)
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+            : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t turned(uint32_t v) {
+    uint32_t r;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// The rows of a unit of work: chunk rows of a group, or of the rows of no group (g = groups).  Found by one warp.
+struct Unit {
+    int g;
+    int index;          // among all units
+    long long from, to;
+};
+template <bool EVERY_GROUP>  // a group without rows has a unit too
+__device__ __forceinline__ Unit unit_at(const ThinArgs& a, int unit) {
+    const int lane = threadIdx.x & 31;
+    Unit u{-1, unit, 0, 0};
+    int before = 0;
+    for (int g0 = 0; g0 <= a.groups && u.g < 0; g0 += 32) {
+        const int g = g0 + lane;
+        long long from = 0, to = 0;
+        if (g < a.groups) {
+            group_rows(a.offsets, g, a.rows, from, to);
+        } else if (g == a.groups) {
+            long long b;
+            group_rows(a.offsets, a.groups - 1, a.rows, b, from);
+            to = a.rows;
+        }
+        int count = int((to - from + a.chunk - 1) / a.chunk);
+        if (EVERY_GROUP && g < a.groups) count = max(1, count);
+        int sum = count;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int other = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d) sum += other;
+        }
+        const int first = before + sum - count;
+        const uint32_t found = __ballot_sync(0xffffffffu, unit >= first && unit < first + count);
+        if (found) {
+            const int at = __ffs(found) - 1;
+            u.g = g0 + at;
+            from = __shfl_sync(0xffffffffu, from, at) + (long long)(unit - __shfl_sync(0xffffffffu, first, at)) * a.chunk;
+            to = __shfl_sync(0xffffffffu, to, at);
+            u.from = from;
+            u.to = min(to, from + a.chunk);
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return u;
+}
+
+__device__ __forceinline__ uint4 load_row(const void* base, long long row, int width, int column, bool on) {
+    return on ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + row * width + column)) : make_uint4(0, 0, 0, 0);
+}
+
+// KB, NB: blocks of 32 inputs and outputs.
+template <typename T, int KB, int NB>
+__global__ void __launch_bounds__(THREADS) thin_forward_kernel(ThinArgs a) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+    const Unit u = unit_at<false>(a, blockIdx.x);
+    if (u.g < 0) return;
+    if (u.g == a.groups) {  // rows of no group
+        for (long long row = u.from + warp * 8 + g; row < u.to; row += WARPS * 8) {
+            for (int nb = 0; nb < NB; ++nb) {
+                const int column = nb * 32 + c * 8;
+                if (column >= a.outputs) continue;
+                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.y) + row * a.outputs + column) = make_uint4(0, 0, 0, 0);
+                if (a.slope) *reinterpret_cast<uint4*>(a.slope + row * a.outputs + column) = make_uint4(0, 0, 0, 0);
+            }
+        }
+        return;
+    }
+    uint4 w[NB][4][KB];
+    float bias[NB][8];
+    const uint16_t* weight = static_cast<const uint16_t*>(a.weight) + (long long)u.g * a.outputs * a.inputs;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                const int n = nb * 32 + (g >> 1) * 8 + j * 2 + (g & 1), k = kb * 32 + c * 8;
+                w[nb][j][kb] = load_row(weight, n, a.inputs, k, n < a.outputs && k < a.inputs);
+            }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int n = nb * 32 + c * 8 + e;
+            bias[nb][e] = a.bias && n < a.outputs ? to_float(static_cast<const T*>(a.bias)[(long long)u.g * a.outputs + n]) : 0.0f;
+        }
+    }
+    for (long long r0 = u.from + warp * 16; r0 < u.to; r0 += WARPS * 16) {
+        uint4 x[KB][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                const long long row = r0 + g + 8 * h;
+                x[kb][h] = load_row(a.x, row, a.inputs, kb * 32 + c * 8, row < u.to && kb * 32 + c * 8 < a.inputs);
+            }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const int column = nb * 32 + c * 8;
+            const bool inside = column < a.outputs;
+            uint4 r[2];
+            if (a.residual) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) r[h] = load_row(a.residual, r0 + g + 8 * h, a.outputs, column, inside && r0 + g + 8 * h < u.to);
+            }
+            float d[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) d[j][i] = bias[nb][j * 2 + (i & 1)];
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                    for (int s = 0; s < 2; ++s)
+                        mma16816<T>(d[j], word(x[kb][0], 2 * s), word(x[kb][1], 2 * s), word(x[kb][0], 2 * s + 1), word(x[kb][1], 2 * s + 1),
+                                    word(w[nb][j][kb], 2 * s), word(w[nb][j][kb], 2 * s + 1));
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                uint32_t y[4], codes[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    Pair slope, z = pair(d[j][2 * h], d[j][2 * h + 1]);
+                    if (a.activation == ACT_RELU) z = activate<ACT_RELU>(z, slope);
+                    else if (a.activation == ACT_SILU) z = activate<ACT_SILU>(z, slope);
+                    else if (a.activation == ACT_GELU) z = activate<ACT_GELU>(z, slope);
+                    else z = activate<ACT_NONE>(z, slope);
+                    if (a.residual) {
+                        const float2 f = unpack_pair<T>(word(r[h], j));
+                        z = add2(z, pair(f.x, f.y));
+                    }
+                    y[j] = pack_pair<T>(both(z).x, both(z).y);
+                    codes[j] = slope_codes(slope);
+                }
+                const long long row = r0 + g + 8 * h;
+                if (row < u.to && inside) {
+                    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.y) + row * a.outputs + column) = make_uint4(y[0], y[1], y[2], y[3]);
+                    if (a.slope) *reinterpret_cast<uint4*>(a.slope + row * a.outputs + column) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+                }
+            }
+        }
+    }
+}
+
+template <typename T, int KB, int NB>
+__global__ void __launch_bounds__(THREADS, KB * NB == 4 ? 2 : 3) thin_backward_kernel(ThinArgs a) {
+    // W by its rows' order for d x: [K-step of 16 outputs][8-column tile of inputs][lane]
+    __shared__ uint2 turned_w[NB * 2][KB * 4][32];
+    __shared__ float sums[NB * 32][KB * 32 + 1];
+    __shared__ float bias_sums[NB * 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+    const Unit u = unit_at<true>(a, blockIdx.x);
+    if (u.g < 0) return;
+    if (u.g == a.groups) {  // rows of no group
+        for (long long row = u.from + warp * 8 + g; row < u.to; row += WARPS * 8) {
+            for (int kb = 0; kb < KB; ++kb)
+                if (a.d_x && kb * 32 + c * 8 < a.inputs)
+                    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.d_x) + row * a.inputs + kb * 32 + c * 8) = make_uint4(0, 0, 0, 0);
+            for (int nb = 0; nb < NB; ++nb)
+                if (a.d_residual && nb * 32 + c * 8 < a.outputs)
+                    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.d_residual) + row * a.outputs + nb * 32 + c * 8) = make_uint4(0, 0, 0, 0);
+        }
+        return;
+    }
+    const bool sum_weights = a.d_weight || a.d_bias;
+    if (a.d_x) {
+        const uint16_t* weight = static_cast<const uint16_t*>(a.weight) + (long long)u.g * a.outputs * a.inputs;
+        for (int i = warp; i < NB * 2 * KB * 4; i += WARPS) {
+            const int step = i / (KB * 4), tile = i % (KB * 4), nb = step / 2, s = step % 2, kb = tile / 4, j = tile % 4;
+            const int n = nb * 32 + c * 8 + s * 4, k = kb * 32 + (g >> 1) * 8 + j * 2 + (g & 1);
+            uint32_t e[4];
+#pragma unroll
+            for (int q = 0; q < 4; ++q) e[q] = n + q < a.outputs && k < a.inputs ? weight[(n + q) * a.inputs + k] : 0;
+            turned_w[step][tile][lane] = make_uint2(e[0] | e[1] << 16, e[2] | e[3] << 16);
+        }
+    }
+    for (int i = threadIdx.x; i < NB * 32 * (KB * 32 + 1); i += THREADS) (&sums[0][0])[i] = 0.0f;
+    for (int i = threadIdx.x; i < NB * 32; i += THREADS) bias_sums[i] = 0.0f;
+    __syncthreads();
+    float dw[NB * 2][KB * 4][4], db[NB][8];
+#pragma unroll
+    for (int m = 0; m < NB * 2; ++m)
+#pragma unroll
+        for (int n = 0; n < KB * 4; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dw[m][n][i] = 0.0f;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) db[nb][e] = 0.0f;
+    const void* kept = a.code ? static_cast<const void*>(a.code) : a.relu_y;
+    for (long long r0 = u.from + warp * 16; r0 < u.to; r0 += WARPS * 16) {
+        uint4 z[NB][2], s[NB][2], x[KB][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const long long row = r0 + g + 8 * h;
+            const bool on = row < u.to;
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                const int column = nb * 32 + c * 8;
+                z[nb][h] = load_row(a.d_y, row, a.outputs, column, on && column < a.outputs);
+                s[nb][h] = load_row(kept, row, a.outputs, column, kept && on && column < a.outputs);
+            }
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                const int column = kb * 32 + c * 8;
+                x[kb][h] = load_row(a.x, row, a.inputs, column, a.d_weight && on && column < a.inputs);
+            }
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const long long row = r0 + g + 8 * h;
+                if (a.d_residual && row < u.to && nb * 32 + c * 8 < a.outputs)
+                    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.d_residual) + row * a.outputs + nb * 32 + c * 8) = z[nb][h];
+                uint32_t q[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float2 f = unpack_pair<T>(word(z[nb][h], i));
+                    const uint32_t k = word(s[nb][h], i);
+                    if (a.code) {
+                        f.x *= slope_value(k & 0xffffu);
+                        f.y *= slope_value(k >> 16);
+                    } else if (a.relu_y) {
+                        const float2 o = unpack_pair<T>(k);
+                        f.x *= sign_slope(o.x);
+                        f.y *= sign_slope(o.y);
+                    }
+                    db[nb][2 * i] += f.x;
+                    db[nb][2 * i + 1] += f.y;
+                    q[i] = pack_pair<T>(f.x, f.y);
+                }
+                z[nb][h] = make_uint4(q[0], q[1], q[2], q[3]);
+            }
+        if (a.d_x) {
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                float d[4][4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) d[j][i] = 0.0f;
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                        for (int t = 0; t < 2; ++t) {
+                            const uint2 b = turned_w[nb * 2 + t][kb * 4 + j][lane];
+                            mma16816<T>(d[j], word(z[nb][0], 2 * t), word(z[nb][1], 2 * t), word(z[nb][0], 2 * t + 1), word(z[nb][1], 2 * t + 1),
+                                        b.x, b.y);
+                        }
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const long long row = r0 + g + 8 * h;
+                    const int column = kb * 32 + c * 8;
+                    if (row < u.to && column < a.inputs)
+                        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.d_x) + row * a.inputs + column) =
+                            make_uint4(pack_pair<T>(d[0][2 * h], d[0][2 * h + 1]), pack_pair<T>(d[1][2 * h], d[1][2 * h + 1]),
+                                       pack_pair<T>(d[2][2 * h], d[2][2 * h + 1]), pack_pair<T>(d[3][2 * h], d[3][2 * h + 1]));
+                }
+            }
+        }
+        if (a.d_weight) {
+            uint32_t xt[KB][4][2];
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) xt[kb][i][h] = turned(word(x[kb][h], i));
+#pragma unroll
+            for (int m = 0; m < NB * 2; ++m) {
+                const int nb = m / 2, p = m % 2;
+                const uint32_t a0 = turned(word(z[nb][0], 2 * p)), a1 = turned(word(z[nb][0], 2 * p + 1));
+                const uint32_t a2 = turned(word(z[nb][1], 2 * p)), a3 = turned(word(z[nb][1], 2 * p + 1));
+#pragma unroll
+                for (int n = 0; n < KB * 4; ++n) mma16816<T>(dw[m][n], a0, a1, a2, a3, xt[n / 4][n % 4][0], xt[n / 4][n % 4][1]);
+            }
+        }
+    }
+    if (!sum_weights) return;
+    // the block's sums: the warps' in order
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int d = 4; d < 32; d *= 2) db[nb][e] += __shfl_xor_sync(0xffffffffu, db[nb][e], d);
+    for (int w = 0; w < WARPS; ++w) {
+        if (warp == w) {
+#pragma unroll
+            for (int m = 0; m < NB * 2; ++m)
+#pragma unroll
+                for (int n = 0; n < KB * 4; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int out = (m / 2) * 32 + (g >> 1) * 8 + (2 * (m % 2) + (i >> 1)) * 2 + (g & 1);
+                        sums[out][(n / 4) * 32 + c * 8 + (n % 4) * 2 + (i & 1)] += dw[m][n][i];
+                    }
+            if (g == 0) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) bias_sums[nb * 32 + c * 8 + e] += db[nb][e];
+            }
+        }
+        __syncthreads();
+    }
+    const int size = a.outputs * a.inputs;
+    if (a.partial) {
+        float* to = a.partial + (long long)u.index * (size + a.outputs);
+        if (a.d_weight)
+            for (int i = threadIdx.x; i < size; i += THREADS) to[i] = sums[i / a.inputs][i % a.inputs];
+        for (int i = threadIdx.x; i < a.outputs; i += THREADS) to[size + i] = bias_sums[i];
+    } else {
+        if (a.d_weight)
+            for (int i = threadIdx.x; i < size; i += THREADS)
+                static_cast<T*>(a.d_weight)[(long long)u.g * size + i] = from_float<T>(sums[i / a.inputs][i % a.inputs]);
+        if (a.d_bias)
+            for (int i = threadIdx.x; i < a.outputs; i += THREADS)
+                static_cast<T*>(a.d_bias)[(long long)u.g * a.outputs + i] = from_float<T>(bias_sums[i]);
+    }
+}
+
+template <typename F>
+void with_blocks(int inputs, int outputs, F&& f) {
+    auto second = [&](auto kb) {
+        if (outputs <= 32) f(kb, std::integral_constant<int, 1>{});
+        else f(kb, std::integral_constant<int, 2>{});
+    };
+    if (inputs <= 32) second(std::integral_constant<int, 1>{});
+    else second(std::integral_constant<int, 2>{});
+}
+
+}  // namespace
+
+template <typename T>
+void launch_thin_forward(const ThinArgs& a, cudaStream_t stream) {
+    with_blocks(a.inputs, a.outputs, [&](auto kb, auto nb) {
+        thin_forward_kernel<T, decltype(kb)::value, decltype(nb)::value>
+            <<<unsigned(thin_units(a.rows, a.groups, a.chunk)), THREADS, 0, stream>>>(a);
+    });
+    ODIE_CUDA(cudaGetLastError());
+    note_launch();
+}
+
+template <typename T>
+void launch_thin_backward(const ThinArgs& a, cudaStream_t stream) {
+    with_blocks(a.inputs, a.outputs, [&](auto kb, auto nb) {
+        thin_backward_kernel<T, decltype(kb)::value, decltype(nb)::value>
+            <<<unsigned(thin_units(a.rows, a.groups, a.chunk)), THREADS, 0, stream>>>(a);
+    });
+    ODIE_CUDA(cudaGetLastError());
+    note_launch();
+}
+
+template void launch_thin_forward<__half>(const ThinArgs&, cudaStream_t);
+template void launch_thin_forward<__nv_bfloat16>(const ThinArgs&, cudaStream_t);
+template void launch_thin_backward<__half>(const ThinArgs&, cudaStream_t);
+template void launch_thin_backward<__nv_bfloat16>(const ThinArgs&, cudaStream_t);
+
+}  // namespace odie

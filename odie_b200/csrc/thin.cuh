@@ -1,0 +1,47 @@
+// Thin linear layers (thin.cu): up to 64 inputs and outputs, multiples of 8, the sizes of this library's own heads.
+#pragma once
+#include "activation.cuh"
+#include <algorithm>
+
+namespace odie {
+
+struct ThinArgs {
+    long long rows;
+    int inputs, outputs, groups;
+    const int* offsets;     // null: one group of all rows
+    int chunk;              // rows per block, a multiple of 64
+    const void* x;
+    const void* weight;
+    // forward
+    const void* bias;
+    const void* residual;
+    void* y;
+    uint16_t* slope;
+    int activation;
+    // backward
+    const void* d_y;
+    const uint16_t* code;   // of the slope, or
+    const void* relu_y;     // a ReLU's output, or neither
+    void* d_x;              // each null where not wanted
+    void* d_weight;
+    void* d_bias;
+    void* d_residual;
+    float* partial;         // [unit][outputs * inputs + outputs] sums of several units per group; null: one unit each
+};
+
+inline bool thin_sizes(int inputs, int outputs) { return inputs <= 64 && outputs <= 64 && inputs % 8 == 0 && outputs % 8 == 0; }
+// Rows per block: about two blocks per SM and warp slot for few rows, at most 512 (forward) or 1024 (backward, whose
+// blocks each leave a sum of the weights' gradient).
+inline int thin_chunk(int64_t rows, bool backward) {
+    const int64_t most = backward ? 1024 : 512, share = (rows + 591) / 592;
+    return int(std::max<int64_t>(64, std::min(most, (share + 63) / 64 * 64)));
+}
+// Units of work (blocks) at most: every group has at least one, and rows of no group their own.
+inline int64_t thin_units(int64_t rows, int groups, int chunk) { return (rows + chunk - 1) / chunk + groups + 1; }
+
+template <typename T>
+void launch_thin_forward(const ThinArgs& a, cudaStream_t stream);
+template <typename T>
+void launch_thin_backward(const ThinArgs& a, cudaStream_t stream);
+
+}  // namespace odie

@@ -246,15 +246,18 @@ class _Linear(torch.autograd.Function):
         x, weight = _aligned(x), _aligned(weight)
         bias, residual = (None if t is None else t.contiguous() for t in (bias, residual))
         need = ctx.needs_input_grad
-        y, slope = _linear(x, weight, bias, residual, offsets, activation, any(need[:3]))
-        ctx.save_for_backward(x if need[1] else None, weight if need[0] else None, slope, offsets)
+        # a ReLU's slope is the sign of its output, unless a residual hides it
+        sign = activation == ACTIVATIONS['relu'] and residual is None
+        y, slope = _linear(x, weight, bias, residual, offsets, activation, any(need[:3]) and not sign)
+        ctx.save_for_backward(x if need[1] else None, weight if need[0] else None, slope,
+                              y if sign and any(need[:3]) else None, offsets)
         ctx.sizes = (x.shape, weight.shape)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, d_y):
-        x, weight, slope, offsets = ctx.saved_tensors
+        x, weight, slope, relu_y, offsets = ctx.saved_tensors
         (rows, inputs), shape = ctx.sizes
         groups, outputs = (shape[0] if len(shape) == 3 else 1), shape[-2]
         need = ctx.needs_input_grad
@@ -268,8 +271,8 @@ class _Linear(torch.autograd.Function):
         d_residual = d_y if offsets is None else empty(need[3], rows, outputs)
         if any(need[:3]) or (need[3] and offsets is not None):
             scratch = _scratch(d_y.device, 'odie_linear_backward_scratch', rows, inputs, outputs, groups)
-            _call('odie_linear_backward', d_y.device, d_y.data_ptr(), _lib.ptr(slope), _lib.ptr(x), _lib.ptr(weight),
-                  rows, inputs, outputs, groups, _lib.ptr(offsets), ROW_TYPES[d_y.dtype], _lib.ptr(d_x),
+            _call('odie_linear_backward', d_y.device, d_y.data_ptr(), _lib.ptr(slope), _lib.ptr(relu_y), _lib.ptr(x),
+                  _lib.ptr(weight), rows, inputs, outputs, groups, _lib.ptr(offsets), ROW_TYPES[d_y.dtype], _lib.ptr(d_x),
                   _lib.ptr(d_weight), _lib.ptr(d_bias), None if offsets is None else _lib.ptr(d_residual),
                   _lib.ptr(scratch))
         return d_x, d_weight, d_bias, d_residual if need[3] else None, None, None

@@ -20,7 +20,8 @@ def normal(g, *shape, dtype=torch.float32, std=1.0):
 
 # ---------------------------------------------------------------- order
 SORTS = [(0, 1, 4), (1, 1, 1), (31, 1, 3), (4096, 1, 5), (4097, 1, 5), (257, 3, 64), (1000, 8, 1023), (3000, 2, 1024),
-         (20000, 1, 1), (12345, 2, 200), (9000, 1, 70000), (5, 1, 70000), (50000, 1, (1 << 20) + 3)]
+         (20000, 1, 1), (12345, 2, 200), (9000, 1, 70000), (5, 1, 70000), (50000, 1, (1 << 20) + 3),
+         (16384, 1, 511), (16385, 1, 512), (8192, 2, 1 << 19), (4096, 1, 300), (70000, 1, 5)]
 
 
 @pytest.mark.parametrize('rows, choices, bins', SORTS)
@@ -143,7 +144,9 @@ def test_unaligned_and_strided_rows(cuda):
 
 # ---------------------------------------------------------------- linear
 LINEARS = [(1, 1, 1), (1, 64, 128), (2, 7, 3), (3, 256, 260), (8, 136, 24), (17, 40, 1000), (5, 333, 515), (127, 64, 64),
-           (128, 32, 64), (129, 256, 256), (300, 1000, 72), (1000, 72, 264), (257, 2048, 128), (640, 520, 776)]
+           (128, 32, 64), (129, 256, 256), (300, 1000, 72), (1000, 72, 264), (257, 2048, 128), (640, 520, 776), (5000, 200, 48), (2500, 1030, 31),
+           # up to 64 inputs and outputs: the layers that stay in registers
+           (9, 8, 8), (200, 24, 32), (333, 64, 40), (3000, 40, 64), (5000, 64, 64), (1111, 32, 8)]
 
 
 def linear_case(rows, inputs, outputs, dtype, activation, groups=None, seed=0, bias=True, residual=True):
@@ -190,7 +193,7 @@ GROUPS = [[0], [1], [5, 0, 3], [127, 128, 129], [0, 0, 300], [64, 1, 0, 63, 200]
 
 
 @pytest.mark.parametrize('sizes', GROUPS)
-@pytest.mark.parametrize('inputs, outputs', [(64, 128), (96, 40), (37, 21), (264, 520)])
+@pytest.mark.parametrize('inputs, outputs', [(64, 128), (96, 40), (37, 21), (264, 520), (32, 64), (64, 40)])
 @pytest.mark.parametrize('dtype, activation', [(torch.float16, 'relu'), (torch.bfloat16, 'gelu'), (torch.bfloat16, 'none')])
 @pytest.mark.parametrize('tail', [0, 19])
 def test_linear_groups(cuda, sizes, inputs, outputs, dtype, activation, tail):
@@ -300,6 +303,25 @@ def test_linear_gradient_against_differences(cuda, activation):
     bounds = [plain['d_' + n][1] for n in ('x', 'weight', 'bias', 'residual')]
     allowed = sum((b * d.abs()).sum().item() for b, d in zip(bounds, along)) + 1e-6 * abs(slope) + 1e-6
     assert abs(got - slope) <= allowed
+
+
+@pytest.mark.parametrize('rows, inputs, outputs', [(40, 32, 64), (40, 64, 128), (5, 64, 64)])
+@pytest.mark.parametrize('wanted', ['x', 'weight', 'bias', 'residual'])
+def test_linear_single_gradients(cuda, rows, inputs, outputs, wanted):
+    """Each gradient by itself, the others not asked for, has the bits of the whole backward pass."""
+    from odie_b200.experts import linear
+    case = linear_case(rows, inputs, outputs, torch.bfloat16, 'silu')
+    offsets = torch.tensor([0, rows - 3], dtype=torch.int32, device=cuda)
+    for grouped in (False, True):
+        named = dict(zip(('x', 'weight', 'bias', 'residual'), (t.detach() for t in case[:4])))
+        if grouped:
+            named.update(weight=named['weight'][None], bias=named['bias'][None])
+        more = dict(activation='silu', offsets=offsets if grouped else None)
+        every = {k: v.clone().requires_grad_() for k, v in named.items()}
+        want = torch.autograd.grad(linear(**every, **more), every[wanted], case[4])[0]
+        one = {k: v.clone().requires_grad_(k == wanted) for k, v in named.items()}
+        got = torch.autograd.grad(linear(**one, **more), one[wanted], case[4])[0]
+        assert torch.equal(got, want)
 
 
 def test_linear_waits_never_run_out(cuda):
