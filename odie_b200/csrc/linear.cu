@@ -711,7 +711,7 @@ __global__ void __launch_bounds__(256) pad_kernel(const uint16_t* from0, uint16_
 
 // ---------------------------------------------------------------- a few rows
 // Up to eight rows: y is bound by the bytes of W, which every warp reads straight into registers, one row of W (one
-// output) per warp and U vectors in flight per lane; x comes from L1.  (The tensor-core tiles, 128 rows each, took
+// output) per warp and U vectors in flight per lane; x comes through shared memory meanwhile.  (The tensor-core tiles, 128 rows each, took
 // 26 us for one row of 4096 x 4096 bf16: 32 CTAs cannot draw the memory's rate.)
 struct FewArgs {
     const void* x;
@@ -729,33 +729,42 @@ constexpr int FEW_ROWS = 8, FEW_THREADS = 128;
 template <typename T, int BYTES, int M>
 __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(FewArgs a) {
     using P = Pack<T, BYTES>;
-    constexpr int U = M <= 2 ? 16 : 8;
+    constexpr int U = M <= 2 ? 16 : 8, CHUNK = 32 * P::N * U;  // values of K at a time
+    __shared__ alignas(16) T xs[M][CHUNK];
     const int lane = threadIdx.x & 31, n = blockIdx.x * (FEW_THREADS / 32) + (threadIdx.x >> 5);
-    if (n >= a.outputs) return;
-    const T* w = static_cast<const T*>(a.weight) + (long long)n * a.inputs;
+    const T* w = static_cast<const T*>(a.weight) + (long long)min(n, a.outputs - 1) * a.inputs;
     const T* x = static_cast<const T*>(a.x);
     float sum[M];
 #pragma unroll
     for (int m = 0; m < M; ++m) sum[m] = 0.0f;
-    for (int k0 = lane * P::N; k0 < a.inputs; k0 += 32 * P::N * U) {
+    for (int c0 = 0; c0 < a.inputs; c0 += CHUNK) {
         P v[U];
 #pragma unroll
         for (int u = 0; u < U; ++u) {
-            const int k = k0 + u * 32 * P::N;
+            const int k = c0 + (u * 32 + lane) * P::N;
             v[u] = k < a.inputs ? P::load_once(w + k) : P::zero();
         }
+        const int count = min(CHUNK, a.inputs - c0) / P::N;
+        if (c0 > 0) __syncthreads();
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int k = k0 + u * 32 * P::N;
-            if (k >= a.inputs) break;
+        for (int m = 0; m < M; ++m)
+#pragma unroll 4
+            for (int i = threadIdx.x; i < CHUNK / P::N; i += FEW_THREADS) {
+                const P q = i < count ? P::load(x + (long long)min(m, a.rows - 1) * a.inputs + c0 + i * P::N) : P::zero();
+                q.store(&xs[m][i * P::N]);
+            }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int m = 0; m < M; ++m) {
-                const P q = P::load(x + (long long)min(m, a.rows - 1) * a.inputs + k);
+                P q;
+                *reinterpret_cast<typename Raw<BYTES>::type*>(&q) = *reinterpret_cast<const typename Raw<BYTES>::type*>(&xs[m][(u * 32 + lane) * P::N]);
 #pragma unroll
                 for (int e = 0; e < P::N; ++e) sum[m] = fmaf(to_float(v[u].v[e]), to_float(q.v[e]), sum[m]);
             }
-        }
     }
+    if (n >= a.outputs) return;
     float mine = 0.0f;
 #pragma unroll
     for (int m = 0; m < M; ++m) {

@@ -19,6 +19,7 @@ namespace odie {
 namespace {
 
 constexpr int THREADS = 128, WARPS = 4;
+constexpr int FORWARD_STAGES = 4, BACKWARD_STAGES = 3;  // steps of 16 rows per warp, one in work, the others on their way
 
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -82,13 +83,26 @@ __device__ __forceinline__ Unit unit_at(const ThinArgs& a, int unit) {
     return u;
 }
 
+// Copies ahead: a lane's own 16-byte words, in shared memory slots that only it reads, so that rows are on their way
+// without holding registers.  A copy that is off writes zeros.
+__device__ __forceinline__ void copy_ahead(uint4* slot, const void* base, long long row, int width, int column, bool on) {
+    const uint16_t* from = static_cast<const uint16_t*>(base) + (on ? row * width + column : 0);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(uint32_t(__cvta_generic_to_shared(slot))), "l"(from), "r"(on ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
 __device__ __forceinline__ uint4 load_row(const void* base, long long row, int width, int column, bool on) {
     return on ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + row * width + column)) : make_uint4(0, 0, 0, 0);
 }
 
 // KB, NB: blocks of 32 inputs and outputs.
 template <typename T, int KB, int NB>
-__global__ void __launch_bounds__(THREADS) thin_forward_kernel(ThinArgs a) {
+__global__ void __launch_bounds__(THREADS, 4) thin_forward_kernel(ThinArgs a) {
+    constexpr int VECTORS = KB * 2 + NB * 2;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
     const Unit u = unit_at<false>(a, blockIdx.x);
     if (u.g < 0) return;
@@ -121,15 +135,36 @@ __global__ void __launch_bounds__(THREADS) thin_forward_kernel(ThinArgs a) {
             bias[nb][e] = a.bias && n < a.outputs ? to_float(static_cast<const T*>(a.bias)[(long long)u.g * a.outputs + n]) : 0.0f;
         }
     }
-    for (long long r0 = u.from + warp * 16; r0 < u.to; r0 += WARPS * 16) {
+    extern __shared__ uint4 slots[];
+    uint4* mine = slots + warp * (FORWARD_STAGES * VECTORS * 32) + lane;
+    auto ahead = [&](int step) {
+        const long long r0 = u.from + warp * 16 + (long long)step * WARPS * 16;
+        uint4* to = mine + step % FORWARD_STAGES * (VECTORS * 32);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const long long row = r0 + g + 8 * h;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+                copy_ahead(to + (kb * 2 + h) * 32, a.x, row, a.inputs, kb * 32 + c * 8, row < u.to && kb * 32 + c * 8 < a.inputs);
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+                if (a.residual)
+                    copy_ahead(to + (KB * 2 + nb * 2 + h) * 32, a.residual, row, a.outputs, nb * 32 + c * 8,
+                               row < u.to && nb * 32 + c * 8 < a.outputs);
+        }
+        copies_end();
+    };
+    for (int s = 0; s < FORWARD_STAGES - 1; ++s) ahead(s);
+    int step = 0;
+    for (long long r0 = u.from + warp * 16; r0 < u.to; r0 += WARPS * 16, ++step) {
+        ahead(step + FORWARD_STAGES - 1);
+        copies_wait<FORWARD_STAGES - 1>();
+        const uint4* now = mine + step % FORWARD_STAGES * (VECTORS * 32);
         uint4 x[KB][2];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-                const long long row = r0 + g + 8 * h;
-                x[kb][h] = load_row(a.x, row, a.inputs, kb * 32 + c * 8, row < u.to && kb * 32 + c * 8 < a.inputs);
-            }
+            for (int kb = 0; kb < KB; ++kb) x[kb][h] = now[(kb * 2 + h) * 32];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             const int column = nb * 32 + c * 8;
@@ -137,7 +172,7 @@ __global__ void __launch_bounds__(THREADS) thin_forward_kernel(ThinArgs a) {
             uint4 r[2];
             if (a.residual) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) r[h] = load_row(a.residual, r0 + g + 8 * h, a.outputs, column, inside && r0 + g + 8 * h < u.to);
+                for (int h = 0; h < 2; ++h) r[h] = now[(KB * 2 + nb * 2 + h) * 32];
             }
             float d[4][4];
 #pragma unroll
@@ -180,6 +215,8 @@ __global__ void __launch_bounds__(THREADS) thin_forward_kernel(ThinArgs a) {
 
 template <typename T, int KB, int NB>
 __global__ void __launch_bounds__(THREADS, KB * NB == 4 ? 2 : 3) thin_backward_kernel(ThinArgs a) {
+    constexpr int VECTORS = NB * 4 + KB * 2;
+    extern __shared__ uint4 slots[];
     // W by its rows' order for d x: [K-step of 16 outputs][8-column tile of inputs][lane]
     __shared__ uint2 turned_w[NB * 2][KB * 4][32];
     __shared__ float sums[NB * 32][KB * 32 + 1];
@@ -225,8 +262,10 @@ __global__ void __launch_bounds__(THREADS, KB * NB == 4 ? 2 : 3) thin_backward_k
 #pragma unroll
         for (int e = 0; e < 8; ++e) db[nb][e] = 0.0f;
     const void* kept = a.code ? static_cast<const void*>(a.code) : a.relu_y;
-    for (long long r0 = u.from + warp * 16; r0 < u.to; r0 += WARPS * 16) {
-        uint4 z[NB][2], s[NB][2], x[KB][2];
+    uint4* mine = slots + warp * (BACKWARD_STAGES * VECTORS * 32) + lane;
+    auto ahead = [&](int step) {
+        const long long r0 = u.from + warp * 16 + (long long)step * WARPS * 16;
+        uint4* to = mine + step % BACKWARD_STAGES * (VECTORS * 32);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             const long long row = r0 + g + 8 * h;
@@ -234,14 +273,33 @@ __global__ void __launch_bounds__(THREADS, KB * NB == 4 ? 2 : 3) thin_backward_k
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 const int column = nb * 32 + c * 8;
-                z[nb][h] = load_row(a.d_y, row, a.outputs, column, on && column < a.outputs);
-                s[nb][h] = load_row(kept, row, a.outputs, column, kept && on && column < a.outputs);
+                copy_ahead(to + (nb * 2 + h) * 32, a.d_y, row, a.outputs, column, on && column < a.outputs);
+                if (kept) copy_ahead(to + (NB * 2 + nb * 2 + h) * 32, kept, row, a.outputs, column, on && column < a.outputs);
             }
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
                 const int column = kb * 32 + c * 8;
-                x[kb][h] = load_row(a.x, row, a.inputs, column, a.d_weight && on && column < a.inputs);
+                if (a.d_weight) copy_ahead(to + (NB * 4 + kb * 2 + h) * 32, a.x, row, a.inputs, column, on && column < a.inputs);
             }
+        }
+        copies_end();
+    };
+    for (int s = 0; s < BACKWARD_STAGES - 1; ++s) ahead(s);
+    int step = 0;
+    for (long long r0 = u.from + warp * 16; r0 < u.to; r0 += WARPS * 16, ++step) {
+        ahead(step + BACKWARD_STAGES - 1);
+        copies_wait<BACKWARD_STAGES - 1>();
+        const uint4* now = mine + step % BACKWARD_STAGES * (VECTORS * 32);
+        uint4 z[NB][2], s[NB][2], x[KB][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                z[nb][h] = now[(nb * 2 + h) * 32];
+                s[nb][h] = kept ? now[(NB * 2 + nb * 2 + h) * 32] : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) x[kb][h] = a.d_weight ? now[(NB * 4 + kb * 2 + h) * 32] : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
@@ -374,8 +432,10 @@ void with_blocks(int inputs, int outputs, F&& f) {
 template <typename T>
 void launch_thin_forward(const ThinArgs& a, cudaStream_t stream) {
     with_blocks(a.inputs, a.outputs, [&](auto kb, auto nb) {
-        thin_forward_kernel<T, decltype(kb)::value, decltype(nb)::value>
-            <<<unsigned(thin_units(a.rows, a.groups, a.chunk)), THREADS, 0, stream>>>(a);
+        constexpr int KB = decltype(kb)::value, NB = decltype(nb)::value;
+        constexpr int BYTES = WARPS * FORWARD_STAGES * (KB * 2 + NB * 2) * 512;
+        ODIE_CUDA(cudaFuncSetAttribute(thin_forward_kernel<T, KB, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES));
+        thin_forward_kernel<T, KB, NB><<<unsigned(thin_units(a.rows, a.groups, a.chunk)), THREADS, BYTES, stream>>>(a);
     });
     ODIE_CUDA(cudaGetLastError());
     note_launch();
@@ -384,8 +444,10 @@ void launch_thin_forward(const ThinArgs& a, cudaStream_t stream) {
 template <typename T>
 void launch_thin_backward(const ThinArgs& a, cudaStream_t stream) {
     with_blocks(a.inputs, a.outputs, [&](auto kb, auto nb) {
-        thin_backward_kernel<T, decltype(kb)::value, decltype(nb)::value>
-            <<<unsigned(thin_units(a.rows, a.groups, a.chunk)), THREADS, 0, stream>>>(a);
+        constexpr int KB = decltype(kb)::value, NB = decltype(nb)::value;
+        constexpr int BYTES = WARPS * BACKWARD_STAGES * (NB * 4 + KB * 2) * 512;
+        ODIE_CUDA(cudaFuncSetAttribute(thin_backward_kernel<T, KB, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES));
+        thin_backward_kernel<T, KB, NB><<<unsigned(thin_units(a.rows, a.groups, a.chunk)), THREADS, BYTES, stream>>>(a);
     });
     ODIE_CUDA(cudaGetLastError());
     note_launch();

@@ -30,11 +30,11 @@ struct ThinArgs {
 };
 
 inline bool thin_sizes(int inputs, int outputs) { return inputs <= 64 && outputs <= 64 && inputs % 8 == 0 && outputs % 8 == 0; }
-// Rows per block: about two blocks per SM and warp slot for few rows, at most 512 (forward) or 1024 (backward, whose
-// blocks each leave a sum of the weights' gradient).
+// Rows per block: as many blocks as fit the SMs at once (four or three per SM), so that W is read and sums are
+// written as seldom as that allows.
 inline int thin_chunk(int64_t rows, bool backward) {
-    const int64_t most = backward ? 1024 : 512, share = (rows + 591) / 592;
-    return int(std::max<int64_t>(64, std::min(most, (share + 63) / 64 * 64)));
+    const int64_t blocks = 148 * (backward ? 3 : 4), share = (rows + blocks - 1) / blocks;
+    return int(std::max<int64_t>(64, (share + 63) / 64 * 64));
 }
 // Units of work (blocks) at most: every group has at least one, and rows of no group their own.
 inline int64_t thin_units(int64_t rows, int groups, int chunk) { return (rows + chunk - 1) / chunk + groups + 1; }
