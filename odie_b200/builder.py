@@ -1,4 +1,4 @@
-"""Build the sm_100a shared library libodie_b200.so in-tree with nvcc.
+"""Build the sm_100a shared library libodie_b200.so in-tree with nvcc, and _torch_ops.so, the torch functions over it.
 
 The library is the product's compute path: every CUDA kernel plus the C-ABI
 declared in include/odie_b200.h.  It is built next to this file so that it
@@ -15,6 +15,7 @@ SOURCES = ['encode.cu', 'step.cu', 'mlp_tc.cu', 'router.cu', 'probe.cu', 'layout
            'synth.cu', 'hashgrid32.cu', 'sort.cu', 'dispatch.cu', 'embed.cu', 'thin.cu', 'linear.cu',
            'runtime.cu']
 LIBRARY = PACKAGE / 'libodie_b200.so'
+TORCH_OPS = PACKAGE / '_torch_ops.so'  # a Python extension module: odie_b200._torch_ops
 ARCH = ['-gencode', 'arch=compute_100a,code=sm_100a']
 FLAGS = ['-O3', '-std=c++17', '-lineinfo', '--expt-relaxed-constexpr', '-Xcompiler', '-fPIC',
          '-Xcompiler', '-fvisibility=hidden', '-diag-suppress', '177']
@@ -28,13 +29,45 @@ def stale():
     if not LIBRARY.exists():
         return True
     built = LIBRARY.stat().st_mtime
-    inputs = list((PACKAGE / 'csrc').glob('*')) + [ROOT / 'include' / 'odie_b200.h', Path(__file__)]
+    inputs = [p for p in (PACKAGE / 'csrc').glob('*') if p.suffix != '.cpp'] + [ROOT / 'include' / 'odie_b200.h', Path(__file__)]
     return any(p.stat().st_mtime > built for p in inputs)
 
 
+def torch_ops_stale():
+    if not TORCH_OPS.exists():
+        return True
+    built = TORCH_OPS.stat().st_mtime
+    return any(p.stat().st_mtime > built for p in (PACKAGE / 'csrc' / 'torch_ops.cpp', ROOT / 'include' / 'odie_b200.h',
+                                                   Path(__file__)))
+
+
+def build_torch_ops():
+    """g++ on csrc/torch_ops.cpp against this interpreter's torch; the library beside it is found by its folder."""
+    import sysconfig
+    import torch
+    from torch.utils import cpp_extension
+    include = [*cpp_extension.include_paths(), sysconfig.get_paths()['include'],
+               str(Path(os.environ.get('CUDA_HOME', '/usr/local/cuda')) / 'include'), str(ROOT / 'include')]
+    libs = Path(torch.__file__).parent / 'lib'
+    tmp = TORCH_OPS.with_suffix('.so.tmp')
+    command = ['g++', '-O2', '-std=c++17', '-shared', '-fPIC', '-fvisibility=hidden', '-DTORCH_EXTENSION_NAME=_torch_ops',
+               f'-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}',
+               *[flag for path in include for flag in ('-isystem', path)], str(PACKAGE / 'csrc' / 'torch_ops.cpp'), '-o', str(tmp),
+               f'-L{libs}', '-lc10', '-lc10_cuda', '-ltorch', '-ltorch_cpu', '-ltorch_cuda', '-ltorch_python', f'-L{PACKAGE}',
+               '-lodie_b200', '-Wl,-rpath,$ORIGIN', f'-Wl,-rpath,{libs}']
+    subprocess.run(command, check=True)
+    os.replace(tmp, TORCH_OPS)
+
+
 def build(force=False, verbose=False):
-    if not force and not stale():
-        return LIBRARY
+    if force or stale():
+        build_library(verbose)
+    if force or torch_ops_stale():
+        build_torch_ops()
+    return LIBRARY
+
+
+def build_library(verbose=False):
     build_dir = PACKAGE / '_build'
     build_dir.mkdir(exist_ok=True)
     objects = []
@@ -49,7 +82,6 @@ def build(force=False, verbose=False):
     tmp = LIBRARY.with_suffix('.so.tmp')
     subprocess.run([nvcc(), '-shared', *ARCH, *objects, '-o', str(tmp), '-lcudart'], check=True)
     os.replace(tmp, LIBRARY)
-    return LIBRARY
 
 
 if __name__ == '__main__':
