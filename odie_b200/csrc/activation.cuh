@@ -67,21 +67,22 @@ __device__ __forceinline__ float slope_value(uint32_t c) {  // c: 16 bits
 // The slope of a ReLU by its output (NaN where that is NaN).
 __device__ __forceinline__ float sign_slope(float y) { return y > 0.0f ? 1.0f : y; }
 
-// act(z), with act'(z) in slope, of two values.
+// act(z) (with ADD: added + act(z), its last product and the sum one fused step, so that kernels that do and do not
+// keep the slope give the same bits), with act'(z) in slope, of two values.
 //   SiLU  p = 1 / (1 + e^-z): z p and p + z p (1 - p).
 //   GELU  z P(z) and P(z) + z e^(-z^2/2) / sqrt(2 pi), P the normal distribution function by Abramowitz and
 //         Stegun 7.1.26: erfc(u) = (a1 t + .. + a5 t^5) e^(-u^2), t = 1 / (1 + 0.3275911 u), u = |z| / sqrt 2, off
 //         by at most 1.5e-7 absolutely; it shares the slope's exponential.
 // Written in pairs, and with one instruction each for exponential and inverse: the epilogue shares the SM with
 // nothing else, but at 45 instructions per element it took twice the products' time for 1024 inputs.
-template <int ACT>
-__device__ __forceinline__ Pair activate(Pair z, Pair& slope) {
+template <int ACT, bool ADD = false>
+__device__ __forceinline__ Pair activate(Pair z, Pair& slope, Pair added = Pair{}) {
     constexpr float LOG2E = 1.4426950408889634f;
     const float2 s = both(z);
     if (ACT == ACT_RELU) {
         const Pair r = pair(max_nan(s.x, 0.0f), max_nan(s.y, 0.0f));
         slope = pair(s.x > 0.0f ? 1.0f : both(r).x, s.y > 0.0f ? 1.0f : both(r).y);  // 0 or NaN where z is not positive
-        return r;
+        return ADD ? add2(r, added) : r;
     }
     if (ACT == ACT_SILU) {
         const float2 x = both(mul2(z, same(-LOG2E)));
@@ -89,7 +90,7 @@ __device__ __forceinline__ Pair activate(Pair z, Pair& slope) {
         const Pair p = pair(inverse_approx(d.x), inverse_approx(d.y));
         const Pair a = mul2(z, p);
         slope = fma2(a, fma2(p, same(-1.0f), same(1.0f)), p);
-        return a;
+        return ADD ? fma2(z, p, added) : a;
     }
     if (ACT == ACT_GELU) {
         const float2 x = both(mul2(mul2(z, z), same(-0.5f * LOG2E)));
@@ -104,10 +105,10 @@ __device__ __forceinline__ Pair activate(Pair z, Pair& slope) {
         const float2 below = both(q), above = both(fma2(q, same(-1.0f), same(1.0f)));
         const Pair p = pair(s.x < 0.0f ? below.x : above.x, s.y < 0.0f ? below.y : above.y);
         slope = fma2(mul2(z, same(0.39894228040143268f)), e, p);
-        return mul2(z, p);
+        return ADD ? fma2(z, p, added) : mul2(z, p);
     }
     slope = same(1.0f);
-    return z;
+    return ADD ? add2(z, added) : z;
 }
 
 template <typename T>
@@ -133,6 +134,50 @@ __device__ __forceinline__ void group_rows(const int* offsets, int g, long long 
     }
     begin = g == 0 ? 0 : clamp_offset(offsets[g], rows);
     end = max(begin, clamp_offset(offsets[g + 1], rows));
+}
+
+// The rows of a unit of work: chunk rows of a group, or of the rows of no group (g = groups).  Found by one warp.
+struct Unit {
+    int g;
+    int index;          // among all units
+    long long from, to;
+};
+template <bool EVERY_GROUP>  // a group without rows has a unit too
+__device__ __forceinline__ Unit unit_at(const int* offsets, int groups, long long rows, long long chunk, int unit) {
+    const int lane = threadIdx.x & 31;
+    Unit u{-1, unit, 0, 0};
+    int before = 0;
+    for (int g0 = 0; g0 <= groups && u.g < 0; g0 += 32) {
+        const int g = g0 + lane;
+        long long from = 0, to = 0;
+        if (g < groups) {
+            group_rows(offsets, g, rows, from, to);
+        } else if (g == groups) {
+            long long b;
+            group_rows(offsets, groups - 1, rows, b, from);
+            to = rows;
+        }
+        int count = int((to - from + chunk - 1) / chunk);
+        if (EVERY_GROUP && g < groups) count = max(1, count);
+        int sum = count;
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            const int other = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d) sum += other;
+        }
+        const int first = before + sum - count;
+        const uint32_t found = __ballot_sync(0xffffffffu, unit >= first && unit < first + count);
+        if (found) {
+            const int at = __ffs(found) - 1;
+            u.g = g0 + at;
+            from = __shfl_sync(0xffffffffu, from, at) + (long long)(unit - __shfl_sync(0xffffffffu, first, at)) * chunk;
+            to = __shfl_sync(0xffffffffu, to, at);
+            u.from = from;
+            u.to = min(to, from + chunk);
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return u;
 }
 
 }  // namespace odie

@@ -58,28 +58,38 @@ __global__ void __launch_bounds__(ROW_THREADS) dispatch_kernel(RowArgs a, const 
     }
 }
 
+// Vectors of a row that a thread takes together where they are 16 bytes (1) or fewer (4: as many bytes in flight).
+template <int BYTES>
+constexpr int SCALE = BYTES == 16 ? 1 : 4;
+
 // Wide rows with several choices: walks the unsorted rows, so that each is read once however many choices it has.
 // (Walking the sorted side, rows were evicted from L2 between their choices: 16384 rows of 4 KB, four choices each,
 // took 82 us against 54.)
 template <typename T, int BYTES>
 __global__ void __launch_bounds__(ROW_THREADS) dispatch_rows_kernel(RowArgs a, const T* __restrict__ rows, T* __restrict__ sorted) {
     using P = Pack<T, BYTES>;
-    const RowWalk<false, 1> walk(a.shape);
+    constexpr int ITEMS = SCALE<BYTES>;
+    const RowWalk<false, ITEMS> walk(a.shape);
     if (walk.row >= walk.rows) return;
     const long long pair = walk.row * a.choices;
-    for (long long c = walk.lane; c < walk.vectors; c += walk.lanes) {
-        const P v = P::load(rows + walk.row * a.width + c * P::N);
+    for (long long c = walk.lane; c < walk.vectors; c += walk.stride()) {
+        P v[ITEMS];
+#pragma unroll
+        for (int q = 0; q < ITEMS; ++q) v[q] = P::load(rows + walk.row * a.width + (walk.on(c, q) ? walk.vector_of(c, q) : 0) * P::N);
 #pragma unroll 4
         for (int j = 0; j < a.choices; ++j) {
             const int s = __ldg(a.slot + pair + j);
             const long long place = s < 0 ? ~s : s;
-            P o = s < 0 ? P::zero() : v;
-            if (s >= 0 && a.weights) {
-                const float w = __ldg(a.weights + pair + j);
+            const float w = s >= 0 && a.weights ? __ldg(a.weights + pair + j) : 1.0f;
 #pragma unroll
-                for (int i = 0; i < P::N; ++i) o.v[i] = from_float<T>(w * to_float(v.v[i]));
+            for (int q = 0; q < ITEMS; ++q) {
+                P o = s < 0 ? P::zero() : v[q];
+                if (s >= 0 && a.weights) {
+#pragma unroll
+                    for (int i = 0; i < P::N; ++i) o.v[i] = from_float<T>(w * to_float(v[q].v[i]));
+                }
+                if (place < a.places && walk.on(c, q)) o.store(sorted + place * a.width + walk.vector_of(c, q) * P::N);
             }
-            if (place < a.places) o.store(sorted + place * a.width + c * P::N);
         }
     }
 }
@@ -89,7 +99,7 @@ __global__ void __launch_bounds__(ROW_THREADS) dispatch_rows_kernel(RowArgs a, c
 template <typename T, int BYTES, bool NARROW, int BATCH>
 __global__ void __launch_bounds__(ROW_THREADS) combine_kernel(RowArgs a, const T* __restrict__ sorted, T* __restrict__ out) {
     using P = Pack<T, BYTES>;
-    constexpr int ITEMS = 4 / BATCH;
+    constexpr int ITEMS = 4 / BATCH * SCALE<BYTES>, ROWS = NARROW ? ITEMS : 1;
     const RowWalk<NARROW, ITEMS> walk(a.shape);
     for (long long c = walk.lane; c < walk.vectors; c += walk.stride()) {
         float sum[ITEMS][P::N];
@@ -99,25 +109,26 @@ __global__ void __launch_bounds__(ROW_THREADS) combine_kernel(RowArgs a, const T
             for (int i = 0; i < P::N; ++i) sum[q][i] = 0.0f;
         for (int j0 = 0; j0 < a.choices; j0 += BATCH) {
             P v[ITEMS][BATCH];
-            float w[ITEMS][BATCH];
-            bool on[ITEMS][BATCH];
-            int s[ITEMS][BATCH];
+            float w[ROWS][BATCH];
+            bool on[ROWS][BATCH];
+            long long place[ROWS][BATCH];
 #pragma unroll
-            for (int q = 0; q < ITEMS; ++q)
+            for (int q = 0; q < ROWS; ++q)
 #pragma unroll
                 for (int b = 0; b < BATCH; ++b) {
-                    const bool inside = walk.on(c, q) && j0 + b < a.choices;
+                    const bool inside = walk.row_of(q) < walk.rows && j0 + b < a.choices;
                     const long long pair = inside ? walk.row_of(q) * a.choices + j0 + b : 0;
-                    s[q][b] = __ldg(a.slot + pair);
+                    const int s = __ldg(a.slot + pair);
                     w[q][b] = a.weights ? __ldg(a.weights + pair) : 1.0f;
-                    on[q][b] = inside && s[q][b] >= 0 && s[q][b] < a.places;
+                    on[q][b] = inside && s >= 0 && s < a.places;
+                    place[q][b] = on[q][b] ? s : 0;
                 }
 #pragma unroll
             for (int q = 0; q < ITEMS; ++q)
 #pragma unroll
                 for (int b = 0; b < BATCH; ++b) {
-                    const long long place = on[q][b] ? s[q][b] : 0, at = walk.vector_of(c, q);
-                    v[q][b] = P::load(sorted + place * a.width + (at < walk.vectors ? at : 0) * P::N);
+                    const long long at = walk.vector_of(c, q);
+                    v[q][b] = P::load(sorted + place[NARROW ? q : 0][b] * a.width + (at < walk.vectors ? at : 0) * P::N);
                 }
 #pragma unroll
             for (int q = 0; q < ITEMS; ++q)
@@ -125,8 +136,8 @@ __global__ void __launch_bounds__(ROW_THREADS) combine_kernel(RowArgs a, const T
                 for (int b = 0; b < BATCH; ++b)
 #pragma unroll
                     for (int i = 0; i < P::N; ++i) {
-                        const float next = fmaf(w[q][b], to_float(v[q][b].v[i]), sum[q][i]);
-                        sum[q][i] = on[q][b] ? next : sum[q][i];
+                        const float next = fmaf(w[NARROW ? q : 0][b], to_float(v[q][b].v[i]), sum[q][i]);
+                        sum[q][i] = on[NARROW ? q : 0][b] ? next : sum[q][i];
                     }
         }
 #pragma unroll
@@ -215,9 +226,9 @@ __global__ void __launch_bounds__(ROW_THREADS) combine_backward_rows_kernel(RowA
                                                                             const T* __restrict__ sorted, T* __restrict__ d_sorted,
                                                                             float* __restrict__ d_weights) {
     using P = Pack<T, BYTES>;
-    constexpr int BATCH = 4;
+    constexpr int BATCH = 4, ITEMS = SCALE<BYTES>;
     __shared__ float partial[BATCH][ROW_THREADS / 32];
-    const RowWalk<false, 1> walk(a.shape);
+    const RowWalk<false, ITEMS> walk(a.shape);
     const bool live = walk.row < walk.rows;
     const long long row = live ? walk.row : 0;
     for (int j0 = 0; j0 < a.choices; j0 += BATCH) {
@@ -236,27 +247,35 @@ __global__ void __launch_bounds__(ROW_THREADS) combine_backward_rows_kernel(RowA
             w[b] = a.weights ? __ldg(a.weights + pair) : 1.0f;
             dot[b] = 0.0f;
         }
-        for (long long c = walk.lane; c < walk.vectors; c += walk.lanes) {
-            const P g = P::load(d_out + row * a.width + c * P::N);
-            P y[BATCH];
+        for (long long c = walk.lane; c < walk.vectors; c += walk.stride()) {
+            P g[ITEMS], y[ITEMS][BATCH];
 #pragma unroll
-            for (int b = 0; b < BATCH; ++b)
-                if (d_weights) y[b] = P::load(sorted + place[b] * a.width + c * P::N);
+            for (int q = 0; q < ITEMS; ++q) {
+                const long long at = (walk.vector_of(c, q) < walk.vectors ? walk.vector_of(c, q) : 0) * P::N;
+                g[q] = P::load(d_out + row * a.width + at);
 #pragma unroll
-            for (int b = 0; b < BATCH; ++b) {
-                if (d_weights) {
-                    float part = 0.0f;
+                for (int b = 0; b < BATCH; ++b)
+                    if (d_weights) y[q][b] = P::load(sorted + place[b] * a.width + at);
+            }
 #pragma unroll
-                    for (int i = 0; i < P::N; ++i) part = fmaf(to_float(y[b].v[i]), to_float(g.v[i]), part);
-                    dot[b] = kept[b] ? dot[b] + part : 0.0f;
-                }
-                if (d_sorted && on[b]) {
-                    P o = P::zero();
-                    if (kept[b]) {
+            for (int q = 0; q < ITEMS; ++q) {
+                if (walk.vector_of(c, q) >= walk.vectors) continue;
 #pragma unroll
-                        for (int i = 0; i < P::N; ++i) o.v[i] = from_float<T>(w[b] * to_float(g.v[i]));
+                for (int b = 0; b < BATCH; ++b) {
+                    if (d_weights) {
+                        float part = 0.0f;
+#pragma unroll
+                        for (int i = 0; i < P::N; ++i) part = fmaf(to_float(y[q][b].v[i]), to_float(g[q].v[i]), part);
+                        dot[b] = kept[b] ? dot[b] + part : 0.0f;
                     }
-                    o.store(d_sorted + place[b] * a.width + c * P::N);
+                    if (d_sorted && on[b]) {
+                        P o = P::zero();
+                        if (kept[b]) {
+#pragma unroll
+                            for (int i = 0; i < P::N; ++i) o.v[i] = from_float<T>(w[b] * to_float(g[q].v[i]));
+                        }
+                        o.store(d_sorted + place[b] * a.width + walk.vector_of(c, q) * P::N);
+                    }
                 }
             }
         }
@@ -351,7 +370,7 @@ extern "C" int odie_combine(const void* sorted, int64_t n, int choices, int64_t 
             using T = decltype(type);
             auto go = [&](auto batch) {
                 combine_kernel<T, decltype(bytes)::value, decltype(narrow)::value, decltype(batch)::value>
-                    <<<row_blocks(a.shape, 4 / decltype(batch)::value), ROW_THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+                    <<<row_blocks(a.shape, 4 / decltype(batch)::value * SCALE<decltype(bytes)::value>), ROW_THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
                         a, static_cast<const T*>(sorted), static_cast<T*>(out));
             };
             if (choices == 1) go(std::integral_constant<int, 1>{});

@@ -10,13 +10,14 @@
 // Bound by the bytes of d out and d table.
 #include "rows.cuh"
 #include "odie_b200.h"
+#include <algorithm>
 #include <type_traits>
 
 namespace odie {
 namespace {
 
 constexpr int THREADS = ROW_THREADS;
-constexpr int CHUNK = 64, BATCH = 8;  // BATCH rows are loaded together
+constexpr int CHUNK = 64, BATCH = 4;  // BATCH rows are loaded together, the next ones' positions with them
 
 struct EmbedArgs {
     RowShape shape;   // of the result
@@ -70,7 +71,7 @@ struct GradArgs {
 
 // One unit: CHUNK sorted positions x one vector per thread of `lanes` columns.
 template <typename T, int BYTES>
-__global__ void __launch_bounds__(THREADS) embed_chunk_kernel(GradArgs a, const T* __restrict__ d_out, T* __restrict__ d_table) {
+__global__ void __launch_bounds__(THREADS, 4) embed_chunk_kernel(GradArgs a, const T* __restrict__ d_out, T* __restrict__ d_table) {
     using P = Pack<T, BYTES>;
     const int lanes = 1 << a.lanes_log2, lane = threadIdx.x & (lanes - 1);
     const long long chunk = ((long long)blockIdx.x * THREADS + threadIdx.x) >> a.lanes_log2;
@@ -100,22 +101,34 @@ __global__ void __launch_bounds__(THREADS) embed_chunk_kernel(GradArgs a, const 
             o.store(d_table + (long long)current * a.width + c * P::N);
         }
     };
+    uint32_t key[BATCH];
+    int at[BATCH];
+    auto positions = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < BATCH; ++i) {
+            const long long p = min(begin + b + i, a.n - 1);
+            key[i] = b + i < count ? __ldg(a.sorted + p) : outside;
+            at[i] = __ldg(a.order + p);
+        }
+    };
+    positions(0);
     for (int b = 0; b < count && !done; b += BATCH) {
-        uint32_t key[BATCH];
+        uint32_t now[BATCH];
         P v[BATCH];
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
-            key[i] = b + i < count ? a.sorted[begin + b + i] : outside;
-            if (key[i] < outside) v[i] = P::load(d_out + (long long)a.order[begin + b + i] * a.width + c * P::N);
+            now[i] = key[i];
+            v[i] = P::load(d_out + (long long)(now[i] < outside ? at[i] : 0) * a.width + c * P::N);
         }
+        positions(b + BATCH);
 #pragma unroll
         for (int i = 0; i < BATCH; ++i) {
             if (b + i >= count || done) continue;
-            if (key[i] != current) {
+            if (now[i] != current) {
                 flush(false);
                 if (marks) a.runs[current].y = int(begin + b + i);
                 open = false;
-                current = key[i];
+                current = now[i];
                 if (current >= outside) {
                     done = true;
                     continue;
@@ -134,33 +147,41 @@ __global__ void __launch_bounds__(THREADS) embed_chunk_kernel(GradArgs a, const 
     if (marks && !crosses) a.runs[current].y = int(begin + count);
 }
 
-// One unit: one table row x `lanes` columns of vectors.
+// A block: `span` table rows, whose runs are read together, x one vector per thread.  (With a row per thread the wait
+// for its run alone took 33 us for 65536 rows of 2 KB, most of them zero.)
+constexpr int MAX_SPAN = 128;
 template <typename T, int BYTES>
-__global__ void __launch_bounds__(THREADS) embed_join_kernel(GradArgs a, T* __restrict__ d_table) {
+__global__ void __launch_bounds__(THREADS) embed_join_kernel(GradArgs a, T* __restrict__ d_table, int span) {
     using P = Pack<T, BYTES>;
-    const int lanes = 1 << a.lanes_log2, lane = threadIdx.x & (lanes - 1);
-    const long long v = ((long long)blockIdx.x * THREADS + threadIdx.x) >> a.lanes_log2;
+    __shared__ int2 runs[MAX_SPAN];
+    const long long v0 = (long long)blockIdx.x * span;
+    const int count = int(min((long long)span, a.rows - v0));
+    if (threadIdx.x < count) runs[threadIdx.x] = a.runs[v0 + threadIdx.x];
+    __syncthreads();
+    const int lanes = 1 << a.lanes_log2, lane = threadIdx.x & (lanes - 1), step = THREADS >> a.lanes_log2;
     const long long c = (long long)blockIdx.y * lanes + lane;
-    if (v >= a.rows || c * P::N >= a.width) return;
-    const int2 run = a.runs[v];
-    P o = P::zero();
-    if (run.y > run.x) {
-        const long long first = run.x / CHUNK, last = (run.y - 1) / CHUNK;
-        if (first == last) return;  // written by its chunk
-        float sum[P::N];
-        const float* from = a.partial + (first * 2 + 1) * a.width + c * P::N;
+    if (c * P::N >= a.width) return;
+    for (int q = threadIdx.x >> a.lanes_log2; q < count; q += step) {
+        const int2 run = runs[q];
+        P o = P::zero();
+        if (run.y > run.x) {
+            const long long first = run.x / CHUNK, last = (run.y - 1) / CHUNK;
+            if (first == last) continue;  // written by its chunk
+            float sum[P::N];
+            const float* from = a.partial + (first * 2 + 1) * a.width + c * P::N;
 #pragma unroll
-        for (int e = 0; e < P::N; ++e) sum[e] = from[e];
+            for (int e = 0; e < P::N; ++e) sum[e] = from[e];
 #pragma unroll 4
-        for (long long k = first + 1; k <= last; ++k) {
-            const float* more = a.partial + k * 2 * a.width + c * P::N;
+            for (long long k = first + 1; k <= last; ++k) {
+                const float* more = a.partial + k * 2 * a.width + c * P::N;
 #pragma unroll
-            for (int e = 0; e < P::N; ++e) sum[e] += more[e];
+                for (int e = 0; e < P::N; ++e) sum[e] += more[e];
+            }
+#pragma unroll
+            for (int e = 0; e < P::N; ++e) o.v[e] = from_float<T>(a.scale * sum[e]);
         }
-#pragma unroll
-        for (int e = 0; e < P::N; ++e) o.v[e] = from_float<T>(a.scale * sum[e]);
+        o.store(d_table + (v0 + q) * a.width + c * P::N);
     }
-    o.store(d_table + v * a.width + c * P::N);
 }
 
 int log2_of(int lanes) {
@@ -255,16 +276,17 @@ extern "C" int odie_embed_backward(const void* ids, int id_bytes, int64_t n, con
         g.lanes_log2 = log2_of(lanes);
         const int64_t columns = (vectors + lanes - 1) / lanes;
         const int64_t chunk_blocks = ((chunks << g.lanes_log2) + THREADS - 1) / THREADS;
-        const int64_t row_blocks = ((rows << g.lanes_log2) + THREADS - 1) / THREADS;
-        ODIE_REQUIRE(columns <= 65535 && chunk_blocks < (int64_t(1) << 31) && row_blocks < (int64_t(1) << 31),
+        const int64_t step = THREADS >> g.lanes_log2;
+        const int64_t span = std::max<int64_t>(1, std::min<int64_t>({MAX_SPAN, 16 * step, rows / (148 * 8)})), join_blocks = (rows + span - 1) / span;
+        ODIE_REQUIRE(columns <= 65535 && chunk_blocks < (int64_t(1) << 31) && join_blocks < (int64_t(1) << 31),
                      "too many rows or columns for one launch");
         with_row_type(dtype, vector, [&](auto type, auto bytes) {
             using T = decltype(type);
             constexpr int B = decltype(bytes)::value;
             embed_chunk_kernel<T, B><<<dim3(unsigned(chunk_blocks), unsigned(columns)), THREADS, 0, stream>>>(
                 g, static_cast<const T*>(d_out), static_cast<T*>(d_table));
-            embed_join_kernel<T, B><<<dim3(unsigned(row_blocks), unsigned(columns)), THREADS, 0, stream>>>(
-                g, static_cast<T*>(d_table));
+            embed_join_kernel<T, B><<<dim3(unsigned(join_blocks), unsigned(columns)), THREADS, 0, stream>>>(
+                g, static_cast<T*>(d_table), int(span));
         });
         ODIE_CUDA(cudaGetLastError());
         note_launch(2);

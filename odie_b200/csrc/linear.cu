@@ -518,11 +518,13 @@ __global__ void __launch_bounds__(256) join_kernel(const float* partial, T* d_we
                                                    int chunk, long long size, int bias) {
     __shared__ float part[8][33];
     const int g = blockIdx.y, lane = threadIdx.x & 31, line = threadIdx.x >> 5;
-    long long unit = 0, begin, end;
-    for (int i = 0; i < g; ++i) {
+    long long begin, end;
+    int before = 0;  // units of earlier groups
+    for (int i = lane; i < g; i += 32) {
         group_rows(offsets, i, rows, begin, end);
-        unit += max(1ll, (end - begin + chunk - 1) / chunk);
+        before += int(max(1ll, (end - begin + chunk - 1) / chunk));
     }
+    const long long unit = __reduce_add_sync(0xffffffffu, before);
     group_rows(offsets, g, rows, begin, end);
     const int count = int(max(1ll, (end - begin + chunk - 1) / chunk)), share = (count + 7) / 8;
     const int from = min(count, line * share), last = min(count, from + share);
@@ -553,139 +555,97 @@ struct DzArgs {
     const uint16_t* slope;  // codes; null: 1
     const void* y;          // instead of codes: the output of a ReLU, whose slope is its sign
     void* dz;               // null: not wanted
-    void* d_residual;
+    void* d_residual;       // null: not wanted
     void* d_bias;           // null: not wanted
-    float* partial;         // [row blocks][n] sums of dz; null: one block holds all rows and writes d_bias itself
+    float* partial;         // [unit][n] sums of dz, joined by join_kernel; null: one unit, which writes d_bias itself
     long long rows;
     int n;
     long long ld;           // of dz
-    int block_rows;         // rows per block
+    int chunk;              // rows per unit
     int groups;
     const int* offsets;
-    bool wide;
 };
 
 template <typename T>
-__device__ __forceinline__ void dz_load(const DzArgs& a, long long row, int column, float (&v)[8], uint4& raw) {
-    const uint16_t* from = static_cast<const uint16_t*>(a.d_y) + row * a.n + column;
-    const uint16_t* slope = a.slope ? a.slope : static_cast<const uint16_t*>(a.y);
-    uint4 s = make_uint4(0, 0, 0, 0);
-    if (a.wide) {
-        raw = __ldg(reinterpret_cast<const uint4*>(from));
-        if (slope) s = __ldg(reinterpret_cast<const uint4*>(slope + row * a.n + column));
-    } else {
-        uint16_t e[8], f[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            e[j] = column + j < a.n ? from[j] : uint16_t(0);
-            f[j] = slope && column + j < a.n ? slope[row * a.n + column + j] : uint16_t(0);
-        }
-        raw = make_uint4(e[0] | uint32_t(e[1]) << 16, e[2] | uint32_t(e[3]) << 16, e[4] | uint32_t(e[5]) << 16,
-                         e[6] | uint32_t(e[7]) << 16);
-        s = make_uint4(f[0] | uint32_t(f[1]) << 16, f[2] | uint32_t(f[3]) << 16, f[4] | uint32_t(f[5]) << 16,
-                       f[6] | uint32_t(f[7]) << 16);
+__device__ __forceinline__ float2 dz_pair(const DzArgs& a, uint32_t d_y, uint32_t kept) {
+    float2 f = unpack_pair<T>(d_y);
+    if (a.slope) {
+        f.x *= slope_value(kept & 0xffffu);
+        f.y *= slope_value(kept >> 16);
+    } else if (a.y) {
+        const float2 o = unpack_pair<T>(kept);
+        f.x *= sign_slope(o.x);
+        f.y *= sign_slope(o.y);
     }
-    const uint32_t y[4] = {raw.x, raw.y, raw.z, raw.w}, c[4] = {s.x, s.y, s.z, s.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = unpack_pair<T>(y[i]);
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
-        if (a.slope) {
-            v[2 * i] *= slope_value(c[i] & 0xffffu);
-            v[2 * i + 1] *= slope_value(c[i] >> 16);
-        } else if (a.y) {
-            const float2 o = unpack_pair<T>(c[i]);
-            v[2 * i] *= sign_slope(o.x);
-            v[2 * i + 1] *= sign_slope(o.y);
-        }
-    }
+    return f;
 }
 
-// A block: block_rows rows x 8 columns per thread of `lanes` threads.  Column sums: each thread over its rows,
-// then over the block's threads in order.
-template <typename T>
-__global__ void __launch_bounds__(256) dz_kernel(DzArgs a, int lanes_log2) {
-    __shared__ float sums[256][9];
-    const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1), line = threadIdx.x >> lanes_log2, lines = 256 >> lanes_log2;
-    const int column = (blockIdx.y * lanes + lane) * 8;
-    const long long from = (long long)blockIdx.x * a.block_rows, to = min(a.rows, from + a.block_rows);
-    long long b, live;
-    group_rows(a.offsets, a.groups - 1, a.rows, b, live);
-    float sum[8] = {};
+// A block: one unit of rows (of one group, or of none) x COLUMNS columns per thread of `lanes` threads: eight, or one
+// where rows do not start on 16-byte boundaries.  Column sums: each thread over its rows, the lanes of a warp in a
+// tree, the warps in order.
+template <typename T, int COLUMNS, int THREADS>
+__global__ void __launch_bounds__(THREADS) dz_kernel(DzArgs a, int lanes_log2) {
+    constexpr int WARPS = THREADS / 32;
+    __shared__ float sums[WARPS][32 * COLUMNS];
+    const Unit u = unit_at<true>(a.offsets, a.groups, a.rows, a.chunk, blockIdx.x);
+    if (u.g < 0) return;
+    const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1), line = threadIdx.x >> lanes_log2, lines = THREADS >> lanes_log2;
+    const int column = (blockIdx.y * lanes + lane) * COLUMNS;
+    const bool live = u.g < a.groups;
+    const void* kept = a.slope ? static_cast<const void*>(a.slope) : a.y;
+    float sum[COLUMNS];
+#pragma unroll
+    for (int i = 0; i < COLUMNS; ++i) sum[i] = 0.0f;
     if (column < a.n) {
 #pragma unroll 4
-        for (long long row = from + line; row < to; row += lines) {
-            float v[8];
-            uint4 raw;
-            dz_load<T>(a, row, column, v, raw);
-            if (a.dz)
-                *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.dz) + row * a.ld + column) =
-                    make_uint4(pack_pair<T>(v[0], v[1]), pack_pair<T>(v[2], v[3]), pack_pair<T>(v[4], v[5]), pack_pair<T>(v[6], v[7]));
-            if (a.d_residual) {
-                const bool on = row < live;
-                if (a.wide) {
-                    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.d_residual) + row * a.n + column) = on ? raw : make_uint4(0, 0, 0, 0);
-                } else {
-                    const uint32_t e[4] = {raw.x, raw.y, raw.z, raw.w};
+        for (long long row = u.from + line; row < u.to; row += lines) {
+            const long long at = row * a.n + column;
+            if constexpr (COLUMNS == 8) {
+                const uint4 d = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.d_y) + at));
+                const uint4 k = kept ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(kept) + at)) : make_uint4(0, 0, 0, 0);
+                const uint32_t ds[4] = {d.x, d.y, d.z, d.w}, ks[4] = {k.x, k.y, k.z, k.w};
+                uint32_t z[4];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (column + j < a.n)
-                            static_cast<uint16_t*>(a.d_residual)[row * a.n + column + j] = on ? uint16_t(e[j / 2] >> (16 * (j & 1))) : uint16_t(0);
+                for (int i = 0; i < 4; ++i) {
+                    const float2 f = dz_pair<T>(a, ds[i], ks[i]);
+                    z[i] = pack_pair<T>(f.x, f.y);
+                    sum[2 * i] += f.x;
+                    sum[2 * i + 1] += f.y;
                 }
+                if (a.dz) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.dz) + row * a.ld + column) = make_uint4(z[0], z[1], z[2], z[3]);
+                if (a.d_residual)
+                    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.d_residual) + at) = live ? d : make_uint4(0, 0, 0, 0);
+            } else {
+                const uint16_t d = static_cast<const uint16_t*>(a.d_y)[at];
+                const float f = dz_pair<T>(a, d, kept ? static_cast<const uint16_t*>(kept)[at] : 0).x;
+                if (a.dz) static_cast<T*>(a.dz)[row * a.ld + column] = from_float<T>(f);
+                if (a.d_residual) static_cast<uint16_t*>(a.d_residual)[at] = live ? d : uint16_t(0);
+                sum[0] += f;
             }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sum[i] += v[i];
         }
     }
-    if (!a.d_bias) return;
+    if (!a.d_bias || !live) return;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sums[threadIdx.x][i] = sum[i];
+    for (int i = 0; i < COLUMNS; ++i) {
+#pragma unroll
+        for (int d = 16; d > 0; d /= 2) {
+            const float other = __shfl_xor_sync(0xffffffffu, sum[i], d);
+            if (d >= lanes) sum[i] += other;
+        }
+    }
+    if ((threadIdx.x & 31) < lanes) {
+#pragma unroll
+        for (int i = 0; i < COLUMNS; ++i) sums[threadIdx.x >> 5][(threadIdx.x & 31) * COLUMNS + i] = sum[i];
+    }
     __syncthreads();
-    for (int i = threadIdx.x; i < lanes * 8; i += 256) {
-        const int c = i >> 3, e = i & 7, at = (blockIdx.y * lanes + c) * 8 + e;
+    for (int i = threadIdx.x; i < lanes * COLUMNS; i += THREADS) {
+        const int at = blockIdx.y * lanes * COLUMNS + i;
         if (at >= a.n) continue;
         float total = 0.0f;
-        for (int l = 0; l < lines; ++l) total += sums[l * lanes + c][e];
-        if (a.partial) a.partial[(long long)blockIdx.x * a.n + at] = total;
-        else static_cast<T*>(a.d_bias)[at] = from_float<T>(total);
-    }
-}
-
-// d b_g: the whole row blocks inside the group from their sums, the rows before and behind them from d y.
-template <typename T>
-__global__ void __launch_bounds__(256) bias_kernel(DzArgs a) {
-    __shared__ float part[8][33];
-    const int g = blockIdx.y, lane = threadIdx.x & 31, line = threadIdx.x >> 5, c = blockIdx.x * 32 + lane;
-    long long begin, end;
-    group_rows(a.offsets, g, a.rows, begin, end);
-    const long long r = a.block_rows;
-    long long block = (begin + r - 1) / r;
-    // the last block may be short: it is whole if the group reaches the last row
-    long long last = end == a.rows ? (a.rows + r - 1) / r : end / r;
-    const long long head = min(end, block * r), tail = max(head, min(end, last * r));
-    float sum = 0.0f;
-    if (c < a.n) {
-        const T* d_y = static_cast<const T*>(a.d_y);
-        auto rows = [&](long long from, long long to) {
-#pragma unroll 4
-            for (long long row = from + line; row < to; row += 8) {
-                const float v = to_float(d_y[row * a.n + c]);
-                sum += a.slope ? v * slope_value(a.slope[row * a.n + c])
-                       : a.y ? v * sign_slope(to_float(static_cast<const T*>(a.y)[row * a.n + c])) : v;
-            }
-        };
-        rows(begin, head);
-#pragma unroll 4
-        for (long long i = block + line; i < last; i += 8) sum += a.partial[i * a.n + c];
-        rows(tail, end);
-    }
-    part[line][lane] = sum;
-    __syncthreads();
-    if (line == 0 && c < a.n) {
-        sum = 0.0f;
-        for (int i = 0; i < 8; ++i) sum += part[i][lane];
-        static_cast<T*>(a.d_bias)[(long long)g * a.n + c] = from_float<T>(sum);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) total += sums[w][i];
+        if (a.partial) a.partial[(long long)u.index * a.n + at] = total;
+        else static_cast<T*>(a.d_bias)[(long long)u.g * a.n + at] = from_float<T>(total);
     }
 }
 
@@ -775,14 +735,13 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(FewArgs a) {
     if (lane >= min(M, a.rows)) return;
     const long long at = (long long)lane * a.outputs + n;
     if (a.bias) mine += to_float(static_cast<const T*>(a.bias)[n]);
-    Pair slope;
-    Pair z = same(mine);
-    if (a.activation == ACT_RELU) z = activate<ACT_RELU>(z, slope);
-    else if (a.activation == ACT_SILU) z = activate<ACT_SILU>(z, slope);
-    else if (a.activation == ACT_GELU) z = activate<ACT_GELU>(z, slope);
-    else z = activate<ACT_NONE>(z, slope);
-    float v = both(z).x;
-    if (a.residual) v += to_float(static_cast<const T*>(a.residual)[at]);
+    const Pair z = same(mine), added = same(a.residual ? to_float(static_cast<const T*>(a.residual)[at]) : 0.0f);
+    Pair slope, y;
+    if (a.activation == ACT_RELU) y = activate<ACT_RELU, true>(z, slope, added);
+    else if (a.activation == ACT_SILU) y = activate<ACT_SILU, true>(z, slope, added);
+    else if (a.activation == ACT_GELU) y = activate<ACT_GELU, true>(z, slope, added);
+    else y = activate<ACT_NONE, true>(z, slope, added);
+    const float v = both(y).x;
     static_cast<T*>(a.y)[at] = from_float<T>(v);
     if (a.slope) a.slope[at] = uint16_t(slope_codes(slope));
 }
@@ -964,12 +923,30 @@ struct WeightUnits {
     }
 };
 
-// One group of up to 4096 rows: a block sums all rows of its columns, and no second kernel is needed.
-bool dz_direct(int64_t rows, const int32_t* offsets) { return rows <= 4096 && !offsets; }
-int dz_block_rows(int64_t rows, int groups) {
-    // at most about 512 sums for one group; for several, short blocks, since the rows at a group's ends are read twice
-    const int64_t r = groups == 1 ? ceil_div(rows, 512) : ceil_div(rows, int64_t(groups) * 16);
-    return int(std::max<int64_t>(64, ceil_div(r, 64) * 64));
+// Rows per unit of dz.  One group of up to 4096 rows is one unit, in blocks of 1024 threads: no second kernel joins
+// its sums.  Else 64 to 1024 rows, so that a group's sums are few and the blocks many.
+bool dz_single(int64_t rows, int groups) { return rows <= 4096 && groups == 1; }
+int64_t dz_chunk(int64_t rows, int groups) {
+    if (dz_single(rows, groups)) return std::max<int64_t>(1, rows);
+    return std::max<int64_t>(64, std::min<int64_t>(1024, ceil_div(ceil_div(rows, int64_t(16) * groups), 64) * 64));
+}
+int64_t dz_units(int64_t rows, int groups) { return ceil_div(rows, dz_chunk(rows, groups)) + groups + 1; }
+
+template <typename T>
+void launch_dz(const DzArgs& a, cudaStream_t stream) {
+    const bool wide = a.n % 8 == 0 && (uintptr_t(a.d_y) | uintptr_t(a.slope) | uintptr_t(a.y) | uintptr_t(a.d_residual)) % 16 == 0;
+    const bool single = dz_single(a.rows, a.groups);
+    const int columns = wide ? 8 : 1;
+    int log2 = 0;
+    while (log2 < (single && wide ? 1 : 5) && (columns << log2) < a.n) ++log2;
+    const dim3 grid(unsigned(dz_units(a.rows, a.groups)), unsigned(ceil_div(a.n, columns << log2)));
+    ODIE_REQUIRE(grid.y <= 65535, "too many outputs for one launch");
+    if (single && wide) dz_kernel<T, 8, 1024><<<grid, 1024, 0, stream>>>(a, log2);
+    else if (single) dz_kernel<T, 1, 1024><<<grid, 1024, 0, stream>>>(a, log2);
+    else if (wide) dz_kernel<T, 8, 256><<<grid, 256, 0, stream>>>(a, log2);
+    else dz_kernel<T, 1, 256><<<grid, 256, 0, stream>>>(a, log2);
+    ODIE_CUDA(cudaGetLastError());
+    note_launch();
 }
 
 struct BackwardScratch {
@@ -983,7 +960,7 @@ struct BackwardScratch {
         x = pad ? s.take(rows * round8(inputs) * 2) : nullptr;
         weight = pad ? s.take(int64_t(groups) * outputs * round8(inputs) * 2) : nullptr;
         maps = s.take(int64_t(groups) * 2 * sizeof(CUtensorMap));
-        bias = static_cast<float*>(s.take(ceil_div(rows, dz_block_rows(rows, groups)) * outputs * 4));
+        bias = static_cast<float*>(s.take(dz_units(rows, groups) * outputs * 4));
         const WeightUnits u(rows, inputs, outputs, groups);
         partial = static_cast<float*>(u.split ? s.take(u.units * outputs * int64_t(inputs) * 4) : nullptr);
         bytes = s.used;
@@ -1131,26 +1108,17 @@ extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, cons
                 a.y = relu_y;
                 a.dz = products && !as_is ? s.dz : nullptr;
                 a.d_residual = d_residual;
-                const bool direct = dz_direct(rows, offsets);
-                a.partial = direct ? nullptr : s.bias;
+                const bool join = d_bias && rows > dz_chunk(rows, groups);
+                a.partial = join ? s.bias : nullptr;
                 a.d_bias = d_bias;
                 a.rows = rows;
                 a.n = outputs;
                 a.ld = ld_z;
-                a.block_rows = direct ? int(rows) : dz_block_rows(rows, groups);
+                a.chunk = int(dz_chunk(rows, groups));
                 a.groups = groups;
                 a.offsets = offsets;
-                a.wide = outputs % 8 == 0 && (uintptr_t(d_y) | uintptr_t(slope) | uintptr_t(relu_y) | uintptr_t(d_residual)) % 16 == 0;
-                int log2 = 0;
-                while (log2 < (direct ? 1 : 5) && (8 << log2) < outputs) ++log2;  // direct: 16 columns and 128 rows at a time
-                dz_kernel<T><<<dim3(unsigned(ceil_div(rows, a.block_rows)), unsigned(ceil_div(outputs, 8 << log2))), 256, 0, stream>>>(a, log2);
-                ODIE_CUDA(cudaGetLastError());
-                note_launch();
-                if (d_bias && !direct) {
-                    bias_kernel<T><<<dim3(unsigned(ceil_div(outputs, 32)), unsigned(groups)), 256, 0, stream>>>(a);
-                    ODIE_CUDA(cudaGetLastError());
-                    note_launch();
-                }
+                launch_dz<T>(a, stream);
+                if (join) launch_join<T>(s.bias, nullptr, d_bias, offsets, groups, rows, a.chunk, 0, outputs, stream);
             }
             if (s.x && products)
                 launch_pad(x, s.x, d_weight ? rows : 0, weight, s.weight, d_x ? int64_t(groups) * outputs : 0, inputs, stream);

@@ -39,50 +39,6 @@ __device__ __forceinline__ uint32_t turned(uint32_t v) {
 }
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
-// The rows of a unit of work: chunk rows of a group, or of the rows of no group (g = groups).  Found by one warp.
-struct Unit {
-    int g;
-    int index;          // among all units
-    long long from, to;
-};
-template <bool EVERY_GROUP>  // a group without rows has a unit too
-__device__ __forceinline__ Unit unit_at(const ThinArgs& a, int unit) {
-    const int lane = threadIdx.x & 31;
-    Unit u{-1, unit, 0, 0};
-    int before = 0;
-    for (int g0 = 0; g0 <= a.groups && u.g < 0; g0 += 32) {
-        const int g = g0 + lane;
-        long long from = 0, to = 0;
-        if (g < a.groups) {
-            group_rows(a.offsets, g, a.rows, from, to);
-        } else if (g == a.groups) {
-            long long b;
-            group_rows(a.offsets, a.groups - 1, a.rows, b, from);
-            to = a.rows;
-        }
-        int count = int((to - from + a.chunk - 1) / a.chunk);
-        if (EVERY_GROUP && g < a.groups) count = max(1, count);
-        int sum = count;
-#pragma unroll
-        for (int d = 1; d < 32; d *= 2) {
-            const int other = __shfl_up_sync(0xffffffffu, sum, d);
-            if (lane >= d) sum += other;
-        }
-        const int first = before + sum - count;
-        const uint32_t found = __ballot_sync(0xffffffffu, unit >= first && unit < first + count);
-        if (found) {
-            const int at = __ffs(found) - 1;
-            u.g = g0 + at;
-            from = __shfl_sync(0xffffffffu, from, at) + (long long)(unit - __shfl_sync(0xffffffffu, first, at)) * a.chunk;
-            to = __shfl_sync(0xffffffffu, to, at);
-            u.from = from;
-            u.to = min(to, from + a.chunk);
-        }
-        before += __shfl_sync(0xffffffffu, sum, 31);
-    }
-    return u;
-}
-
 // Copies ahead: a lane's own 16-byte words, in shared memory slots that only it reads, so that rows are on their way
 // without holding registers.  A copy that is off writes zeros.
 __device__ __forceinline__ void copy_ahead(uint4* slot, const void* base, long long row, int width, int column, bool on) {
@@ -100,11 +56,11 @@ __device__ __forceinline__ uint4 load_row(const void* base, long long row, int w
 }
 
 // KB, NB: blocks of 32 inputs and outputs.
-template <typename T, int KB, int NB>
+template <typename T, int KB, int NB, int ACT>
 __global__ void __launch_bounds__(THREADS, 4) thin_forward_kernel(ThinArgs a) {
     constexpr int VECTORS = KB * 2 + NB * 2;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
-    const Unit u = unit_at<false>(a, blockIdx.x);
+    const Unit u = unit_at<false>(a.offsets, a.groups, a.rows, a.chunk, blockIdx.x);
     if (u.g < 0) return;
     if (u.g == a.groups) {  // rows of no group
         for (long long row = u.from + warp * 8 + g; row < u.to; row += WARPS * 8) {
@@ -191,17 +147,10 @@ __global__ void __launch_bounds__(THREADS, 4) thin_forward_kernel(ThinArgs a) {
                 uint32_t y[4], codes[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    Pair slope, z = pair(d[j][2 * h], d[j][2 * h + 1]);
-                    if (a.activation == ACT_RELU) z = activate<ACT_RELU>(z, slope);
-                    else if (a.activation == ACT_SILU) z = activate<ACT_SILU>(z, slope);
-                    else if (a.activation == ACT_GELU) z = activate<ACT_GELU>(z, slope);
-                    else z = activate<ACT_NONE>(z, slope);
-                    if (a.residual) {
-                        const float2 f = unpack_pair<T>(word(r[h], j));
-                        z = add2(z, pair(f.x, f.y));
-                    }
+                    const float2 f = a.residual ? unpack_pair<T>(word(r[h], j)) : make_float2(0.0f, 0.0f);
+                    Pair slope, z = activate<ACT, true>(pair(d[j][2 * h], d[j][2 * h + 1]), slope, pair(f.x, f.y));
                     y[j] = pack_pair<T>(both(z).x, both(z).y);
-                    codes[j] = slope_codes(slope);
+                    if (a.slope) codes[j] = slope_codes(slope);
                 }
                 const long long row = r0 + g + 8 * h;
                 if (row < u.to && inside) {
@@ -222,7 +171,7 @@ __global__ void __launch_bounds__(THREADS, KB * NB == 4 ? 2 : 3) thin_backward_k
     __shared__ float sums[NB * 32][KB * 32 + 1];
     __shared__ float bias_sums[NB * 32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
-    const Unit u = unit_at<true>(a, blockIdx.x);
+    const Unit u = unit_at<true>(a.offsets, a.groups, a.rows, a.chunk, blockIdx.x);
     if (u.g < 0) return;
     if (u.g == a.groups) {  // rows of no group
         for (long long row = u.from + warp * 8 + g; row < u.to; row += WARPS * 8) {
@@ -434,8 +383,12 @@ void launch_thin_forward(const ThinArgs& a, cudaStream_t stream) {
     with_blocks(a.inputs, a.outputs, [&](auto kb, auto nb) {
         constexpr int KB = decltype(kb)::value, NB = decltype(nb)::value;
         constexpr int BYTES = WARPS * FORWARD_STAGES * (KB * 2 + NB * 2) * 512;
-        ODIE_CUDA(cudaFuncSetAttribute(thin_forward_kernel<T, KB, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES));
-        thin_forward_kernel<T, KB, NB><<<unsigned(thin_units(a.rows, a.groups, a.chunk)), THREADS, BYTES, stream>>>(a);
+        const auto kernel = a.activation == ACT_RELU   ? thin_forward_kernel<T, KB, NB, ACT_RELU>
+                            : a.activation == ACT_SILU ? thin_forward_kernel<T, KB, NB, ACT_SILU>
+                            : a.activation == ACT_GELU ? thin_forward_kernel<T, KB, NB, ACT_GELU>
+                                                       : thin_forward_kernel<T, KB, NB, ACT_NONE>;
+        ODIE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES));
+        kernel<<<unsigned(thin_units(a.rows, a.groups, a.chunk)), THREADS, BYTES, stream>>>(a);
     });
     ODIE_CUDA(cudaGetLastError());
     note_launch();
