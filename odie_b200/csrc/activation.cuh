@@ -95,15 +95,14 @@ __device__ __forceinline__ Pair activate(Pair z, Pair& slope, Pair added = Pair{
     if (ACT == ACT_GELU) {
         const float2 x = both(mul2(mul2(z, z), same(-0.5f * LOG2E)));
         const Pair e = pair(exp2_approx(x.x), exp2_approx(x.y));
-        const float2 d = both(fma2(pair(fabsf(s.x), fabsf(s.y)), same(0.3275911f * 0.70710678118654752f), same(1.0f)));
-        const Pair t = pair(inverse_approx(d.x), inverse_approx(d.y));
-        Pair q = fma2(t, same(0.5f * 1.061405429f), same(0.5f * -1.453152027f));
-        q = fma2(t, q, same(0.5f * 1.421413741f));
-        q = fma2(t, q, same(0.5f * -0.284496736f));
-        q = fma2(t, q, same(0.5f * 0.254829592f));
-        q = mul2(mul2(q, t), e);  // P(-|z|)
-        const float2 below = both(q), above = both(fma2(q, same(-1.0f), same(1.0f)));
-        const Pair p = pair(s.x < 0.0f ? below.x : above.x, s.y < 0.0f ? below.y : above.y);
+        constexpr float U = 0.3275911f * 0.70710678118654752f;
+        const Pair t = pair(inverse_approx(fmaf(fabsf(s.x), U, 1.0f)), inverse_approx(fmaf(fabsf(s.y), U, 1.0f)));
+        Pair q = fma2(t, same(-0.5f * 1.061405429f), same(-0.5f * -1.453152027f));
+        q = fma2(t, q, same(-0.5f * 1.421413741f));
+        q = fma2(t, q, same(-0.5f * -0.284496736f));
+        q = fma2(t, q, same(-0.5f * 0.254829592f));
+        const float2 h = both(fma2(mul2(q, t), e, same(0.5f)));  // P(|z|) - 1/2
+        const Pair p = add2(pair(copysignf(h.x, s.x), copysignf(h.y, s.y)), same(0.5f));
         slope = fma2(mul2(z, same(0.39894228040143268f)), e, p);
         return ADD ? fma2(z, p, added) : mul2(z, p);
     }

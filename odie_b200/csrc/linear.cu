@@ -45,6 +45,14 @@ constexpr int EPILOGUE_WARP = 4;  // the first one
 constexpr uint32_t WAIT_LIMIT = 1u << 22;
 constexpr int STAGING = 2048;  // bytes per epilogue warp: 32 rows x 32 columns of 16 bits
 
+// n / d for 0 <= n < 2^31 by a multiplication: m = ceil(2^64 / d).
+struct Divide {
+    unsigned long long m;
+    uint32_t d;
+    static Divide by(int64_t d) { return {d > 1 ? ~0ull / uint64_t(d) + 1 : 0, uint32_t(d)}; }
+    __device__ __forceinline__ int operator()(int n) const { return d == 1 ? n : int(__umul64hi((unsigned long long)n, m)); }
+};
+
 struct GemmArgs {
     int groups;
     const int* offsets;  // null: one group of all rows
@@ -53,6 +61,8 @@ struct GemmArgs {
     int n;               // columns of C
     int k;               // FWD, DX: length of the sum
     int chunk;           // DW: rows per unit of work (a multiple of BK)
+    Divide by_bands;     // FWD, DX: tiles of a full band
+    Divide by_tiles, by_columns;  // DW: tiles of d W, and of one row of them
     void* out;
     const void* bias;
     const void* residual;
@@ -92,49 +102,64 @@ struct Tile {
     bool zero;           // nothing to sum: zeros are stored
 };
 
+constexpr int BAND = 16;  // row tiles walked together, so that a W tile serves them from L2
+
+// A role's walk over the tiles, in ascending order: the group is found by stepping on from the last one, and no integer
+// division is left (each of twenty warps walks; dividing, they spent four instructions per output element on it).
 template <int MODE, int CG, int BN>
-__device__ __forceinline__ Tile tile_at(const GemmArgs& p, const int* begin, const int* first, int t) {
-    constexpr int TM = 128 * CG;
-    constexpr int BAND = 16;  // row tiles walked together, so that a W tile serves them from L2
-    Tile tile;
-    const int nt = (p.n + BN - 1) / BN;
-    int key = t, inside = 0;
-    if (MODE == DW) {
-        const int per = nt * ((p.m + TM - 1) / TM);
-        key = t / per;
-        inside = t % per;
+struct Walk {
+    const GemmArgs& p;
+    const int* begin;
+    const int* first;
+    int g = 0;
+    __device__ __forceinline__ Walk(const GemmArgs& args, const int* b, const int* f) : p(args), begin(b), first(f) {}
+    __device__ __forceinline__ Tile at(int t) {
+        constexpr int TM = 128 * CG;
+        Tile tile;
+        int key = t, inside = 0;
+        if (MODE == DW) {
+            key = p.by_tiles(t);
+            inside = t - key * int(p.by_tiles.d);
+        }
+        while (g < p.groups && first[g + 1] <= key) ++g;
+        tile.g = g;
+        const int from = begin[g], to = g < p.groups ? begin[g + 1] : int(p.rows);
+        int local = key - first[g];
+        tile.unit = key;
+        if (MODE == DW) {
+            tile.k0 = from + local * p.chunk;
+            const int rows = max(0, min(to - tile.k0, p.chunk));
+            tile.k_blocks = (rows + BK - 1) / BK;
+            tile.zero = rows == 0;
+            const int m = p.by_columns(inside);
+            tile.n0 = (inside - m * int(p.by_columns.d)) * BN;
+            tile.m0 = m * TM;
+            tile.m_end = p.m;
+        } else {
+            const int band = p.by_bands(local), left = (to - from + TM - 1) / TM - band * BAND;
+            local -= band * int(p.by_bands.d);
+            int n = local / BAND, m = local % BAND;
+            if (left < BAND) {  // local < 2^18: the quotient is off by one at most
+                n = int((float(local) + 0.5f) * inverse_approx(float(left)));
+                m = local - n * left;
+                if (m < 0) {
+                    --n;
+                    m += left;
+                } else if (m >= left) {
+                    ++n;
+                    m -= left;
+                }
+            }
+            tile.m0 = from + (band * BAND + m) * TM;
+            tile.n0 = n * BN;
+            tile.m_end = to;
+            tile.k0 = 0;
+            tile.k_blocks = (p.k + BK - 1) / BK;
+            tile.zero = g == p.groups;
+        }
+        return tile;
     }
-    int lo = 0, hi = p.groups;  // first[lo] <= key < first[hi + 1]
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (first[mid] <= key) lo = mid;
-        else hi = mid - 1;
-    }
-    tile.g = lo;
-    const int from = begin[lo], to = lo < p.groups ? begin[lo + 1] : int(p.rows);
-    int local = key - first[lo];
-    tile.unit = key;
-    if (MODE == DW) {
-        tile.k0 = from + local * p.chunk;
-        const int rows = max(0, min(to - tile.k0, p.chunk));
-        tile.k_blocks = (rows + BK - 1) / BK;
-        tile.zero = rows == 0;
-        tile.n0 = (inside % nt) * BN;
-        tile.m0 = (inside / nt) * TM;
-        tile.m_end = p.m;
-    } else {
-        const int mt = (to - from + TM - 1) / TM;
-        const int band = local / (BAND * nt), height = min(BAND, mt - band * BAND);
-        local -= band * BAND * nt;
-        tile.m0 = from + (band * BAND + local % height) * TM;
-        tile.n0 = (local / height) * BN;
-        tile.m_end = to;
-        tile.k0 = 0;
-        tile.k_blocks = (p.k + BK - 1) / BK;
-        tile.zero = lo == p.groups;
-    }
-    return tile;
-}
+};
 
 // The staging tile of an epilogue warp: 32 rows of 64 bytes, the 16-byte units of a row permuted so that both a
 // thread per row and four threads per row meet no bank twice.
@@ -153,10 +178,14 @@ struct Window {
 __device__ __forceinline__ void window_load(const uint16_t* at, const Window& w, int lane, uint4 (&v)[4]) {
     const int r = lane / 4, c = (lane & 3) * 8;
     const uint16_t* from = at + (long long)r * w.ld + c;
-    if (c + 8 <= w.columns) {  // wide rows: columns are a multiple of 8
+    const long long step = 8ll * w.ld;
+    if (w.rows == 32 && w.columns >= 32) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            v[i] = r + 8 * i < w.rows ? __ldg(reinterpret_cast<const uint4*>(from + (long long)(8 * i) * w.ld)) : make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < 4; ++i, from += step) v[i] = __ldg(reinterpret_cast<const uint4*>(from));
+    } else if (c + 8 <= w.columns) {  // wide rows: columns are a multiple of 8
+#pragma unroll
+        for (int i = 0; i < 4; ++i, from += step)
+            v[i] = r + 8 * i < w.rows ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0, 0, 0, 0);
     }
 }
 __device__ __forceinline__ uint16_t* staged_element(char* base, int row, int c) {
@@ -172,10 +201,16 @@ __device__ __forceinline__ void window_store(uint16_t* at, const Window& w, int 
     if (w.wide) {
         const int r = lane / 4, c = (lane & 3) * 8;
         uint16_t* to = at + (long long)r * w.ld + c;
-        if (c + 8 <= w.columns) {
+        const long long step = 8ll * w.ld;
+        // rows r + 8 i share the permutation of row r: 512 bytes apart
+        const uint4* from = staged(staging, r, lane & 3);
+        if (w.rows == 32 && w.columns >= 32) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (r + 8 * i < w.rows) *reinterpret_cast<uint4*>(to + (long long)(8 * i) * w.ld) = *staged(staging, r + 8 * i, lane & 3);
+            for (int i = 0; i < 4; ++i, to += step) *reinterpret_cast<uint4*>(to) = from[i * 32];
+        } else if (c + 8 <= w.columns) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i, to += step)
+                if (r + 8 * i < w.rows) *reinterpret_cast<uint4*>(to) = from[i * 32];
         }
     } else if (lane < w.columns) {
 #pragma unroll 8
@@ -272,12 +307,13 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
     const int tiles = MODE == DW ? units * nt * ((p.m + S::TM - 1) / S::TM) : units;
     const int start = int(blockIdx.x) / CG, step = int(gridDim.x) / CG;
     bool fine = true;
+    Walk<MODE, CG, BN> walk(p, begin, first);
 
     if (warp == 0) {
         if (lane == 0) {
             uint32_t issued = 0;
             for (int t = start; t < tiles && fine; t += step) {
-                const Tile tile = tile_at<MODE, CG, BN>(p, begin, first, t);
+                const Tile tile = walk.at(t);
                 if (tile.zero) continue;
                 const void* ma = &map_a;
                 const void* mb = &map_b;
@@ -330,7 +366,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
             constexpr uint64_t A_STEP = (A_MN ? 2048 : 32) >> 4, B_STEP = (B_MN ? 2048 : 32) >> 4;
             uint32_t used = 0, summed = 0;
             for (int t = start; t < tiles && fine; t += step) {
-                const Tile tile = tile_at<MODE, CG, BN>(p, begin, first, t);
+                const Tile tile = walk.at(t);
                 const int acc = summed % S::ACCUMULATORS;
                 fine = tc::bar_wait_cluster(drained + acc, ((summed / S::ACCUMULATORS) & 1) ^ 1, WAIT_LIMIT);
                 if (!fine) break;
@@ -370,7 +406,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
         int bias_g = -1, bias_n0 = -1;  // whose bias is held
         uint32_t summed = set;
         for (int t = start + set * step; t < tiles && fine; t += S::SETS * step, summed += S::SETS) {
-            const Tile tile = tile_at<MODE, CG, BN>(p, begin, first, t);
+            const Tile tile = walk.at(t);
             const int acc = summed % S::ACCUMULATORS;
             const int row = tile.m0 + int(rank) * 128 + quadrant * 32, column0 = tile.n0 + group * 32;
             const long long at = (MODE == DW ? (long long)tile.g * p.m * p.n : 0) + (long long)row * p.n + column0;
@@ -818,8 +854,12 @@ void with_config(Config c, F&& f) {
 }
 
 template <typename T, int MODE, int CG, int BN>
-void launch_gemm(const CUtensorMap& a, const CUtensorMap& b, const GemmArgs& p, int64_t tiles, cudaStream_t stream) {
+void launch_gemm(const CUtensorMap& a, const CUtensorMap& b, GemmArgs p, int64_t tiles, cudaStream_t stream) {
     ODIE_REQUIRE(tiles < (int64_t(1) << 30), "too many rows and columns for one launch");
+    const int64_t nt = ceil_div(p.n, BN);
+    p.by_bands = Divide::by(BAND * nt);
+    p.by_columns = Divide::by(nt);
+    p.by_tiles = Divide::by(nt * ceil_div(std::max(1, p.m), 128 * CG));
     using S = Shape<CG, BN>;
     const auto kernel = gemm_kernel<T, MODE, CG, BN>;
     ODIE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes(1024)));
