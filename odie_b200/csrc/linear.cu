@@ -78,7 +78,7 @@ struct Shape {
     static constexpr int TM = 128 * CG;
     static constexpr int B_ROWS = BN / CG;  // per CTA
     static constexpr int A_BYTES = 128 * 128, B_BYTES = B_ROWS * 128, STAGE = A_BYTES + B_BYTES;
-    static constexpr int STAGES = BN == 64 ? 6 : 5;
+    static constexpr int STAGES = STAGE < 32768 ? 6 : 5;
     // Sixteen epilogue warps, four per set of 32 TMEM columns (GROUPS) of a tile; the short tiles of 64 columns are
     // handed out to four such sets in turn (SETS), each with an accumulator of its own.
     static constexpr int EPILOGUE_WARPS = 16, THREADS = (EPILOGUE_WARP + EPILOGUE_WARPS) * 32;
@@ -104,6 +104,9 @@ struct Tile {
 
 constexpr int BAND = 16;  // row tiles walked together, so that a W tile serves them from L2
 
+// The same value in every lane, as the compiler sees too.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+
 // A role's walk over the tiles, in ascending order: the group is found by stepping on from the last one, and no integer
 // division is left (each of twenty warps walks; dividing, they spent four instructions per output element on it).
 template <int MODE, int CG, int BN>
@@ -121,10 +124,10 @@ struct Walk {
             key = p.by_tiles(t);
             inside = t - key * int(p.by_tiles.d);
         }
-        while (g < p.groups && first[g + 1] <= key) ++g;
+        while (g < p.groups && uniform(first[g + 1]) <= key) ++g;
         tile.g = g;
-        const int from = begin[g], to = g < p.groups ? begin[g + 1] : int(p.rows);
-        int local = key - first[g];
+        const int from = uniform(begin[g]), to = g < p.groups ? uniform(begin[g + 1]) : int(p.rows);
+        int local = key - uniform(first[g]);
         tile.unit = key;
         if (MODE == DW) {
             tile.k0 = from + local * p.chunk;
@@ -252,8 +255,8 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
     int* begin = reinterpret_cast<int*>(reinterpret_cast<char*>(full) + S::HEAD);  // [groups + 2] first row of each group
     int* first = begin + p.groups + 2;                                            // [groups + 2] first unit
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = CG == 2 ? tc::cluster_rank() : 0;
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int rank = CG == 2 ? uniform(tc::cluster_rank()) : 0;
     const int nt = (p.n + BN - 1) / BN;
 
     if (warp == 0 && lane == 0) {
@@ -302,36 +305,41 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
     __syncthreads();
     if (CG == 2) tc::cluster_sync();
     tc::fence_after_sync();
-    const uint32_t tmem = *tmem_at;
-    const int units = first[p.groups + 1];
+    const uint32_t tmem = uniform(*tmem_at);
+    const uint32_t full_leader = CG == 2 ? uniform(tc::leader_address(full)) : 0;
+    const int units = uniform(first[p.groups + 1]);
     const int tiles = MODE == DW ? units * nt * ((p.m + S::TM - 1) / S::TM) : units;
     const int start = int(blockIdx.x) / CG, step = int(gridDim.x) / CG;
     bool fine = true;
     Walk<MODE, CG, BN> walk(p, begin, first);
 
+    // The loading and the multiplying warp walk their loops with all lanes and values that are the same in every lane,
+    // and one lane issues: the operands of these instructions live in uniform registers.  (With one lane in the loops,
+    // each of them was moved there first: 575 cycles a block, more than the products take.)
     if (warp == 0) {
-        if (lane == 0) {
-            uint32_t issued = 0;
-            for (int t = start; t < tiles && fine; t += step) {
-                const Tile tile = walk.at(t);
-                if (tile.zero) continue;
-                const void* ma = &map_a;
-                const void* mb = &map_b;
-                if (MODE == DW && p.group_maps) {
-                    ma = p.group_maps + 2 * tile.g;
-                    mb = p.group_maps + 2 * tile.g + 1;
-                    asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(ma) : "memory");
-                    asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(mb) : "memory");
-                }
-                for (int kb = 0; kb < tile.k_blocks; ++kb, ++issued) {
-                    const int s = issued % STAGES;
-                    fine = tc::bar_wait_cluster(empty + s, ((issued / STAGES) & 1) ^ 1, WAIT_LIMIT);
-                    if (!fine) break;
-                    const uint32_t bar = CG == 2 ? tc::leader_address(full + s) : tc::smem_u32(full + s);
+        const bool issuer = tc::elect_one();
+        int s = 0, phase = 1, issued = 0;
+        for (int t = start; t < tiles && fine; t += step) {
+            const Tile tile = walk.at(t);
+            if (tile.zero) continue;
+            const void* ma = &map_a;
+            const void* mb = &map_b;
+            if (MODE == DW && p.group_maps) {
+                ma = p.group_maps + 2 * tile.g;
+                mb = p.group_maps + 2 * tile.g + 1;
+                asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(ma) : "memory");
+                asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;" ::"l"(mb) : "memory");
+            }
+            const int m = tile.m0 + rank * 128, n = tile.n0 + rank * S::B_ROWS;
+            for (int kb = 0; kb < tile.k_blocks; ++kb) {
+                fine = __all_sync(0xffffffffu, tc::bar_wait(empty + s, phase, WAIT_LIMIT));
+                if (!fine) break;
+                if (issuer) {
+                    const uint32_t bar = CG == 2 ? full_leader + s * 8 : tc::smem_u32(full + s);
                     if (rank == 0) tc::bar_expect(full + s, S::STAGE * CG);
                     char* a = stages + s * S::STAGE;
                     char* b = a + S::A_BYTES;
-                    const int k = kb * BK, m = tile.m0 + int(rank) * 128, n = tile.n0 + int(rank) * S::B_ROWS;
+                    const int k = kb * BK;
                     if (MODE == DW) {
 #pragma unroll
                         for (int i = 0; i < 2; ++i) tc::tma_load_2d<CG>(a + i * 8192, ma, m + 64 * i, tile.k0 + k, bar);
@@ -349,48 +357,68 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
                         }
                     }
                 }
+                __syncwarp();
+                ++issued;
+                if (++s == STAGES) {
+                    s = 0;
+                    phase ^= 1;
+                }
             }
-            // every stage read out: no arrival is on its way when the CTA ends, and no copy (had a wait run out,
-            // the leader waits for its pair's copies here, with a limit)
-            for (uint32_t i = 0; i < STAGES && i < issued; ++i) {
-                const uint32_t last = issued - 1 - i;
-                if (fine) fine = tc::bar_wait_cluster(empty + last % STAGES, (last / STAGES) & 1, WAIT_LIMIT);
-                else if (rank == 0) tc::bar_wait(full + last % STAGES, (last / STAGES) & 1, WAIT_LIMIT);
-            }
-            if (!fine) atomicExch(p.error, 2);
         }
+        // every stage read out: no arrival is on its way when the CTA ends, and no copy (had a wait run out, the
+        // leader waits for its pair's copies here, with a limit)
+        for (int i = 0; i < STAGES && i < issued; ++i) {
+            const int last = issued - 1 - i;
+            if (fine) fine = __all_sync(0xffffffffu, tc::bar_wait(empty + last % STAGES, (last / STAGES) & 1, WAIT_LIMIT));
+            else if (rank == 0) tc::bar_wait(full + last % STAGES, (last / STAGES) & 1, WAIT_LIMIT);
+        }
+        if (!fine && lane == 0) atomicExch(p.error, 2);
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
+        if (rank == 0) {
             constexpr int A_MN = MODE == DW, B_MN = MODE != FWD;
             constexpr uint32_t ID = std::is_same<T, __half>::value ? tc::idesc(S::TM, BN, A_MN, B_MN) : tc::idesc_bf16(S::TM, BN, A_MN, B_MN);
             constexpr uint64_t A_STEP = (A_MN ? 2048 : 32) >> 4, B_STEP = (B_MN ? 2048 : 32) >> 4;
-            uint32_t used = 0, summed = 0;
+            const bool issuer = tc::elect_one();
+            const uint32_t a0 = tc::smem_u32(stages);
+            const uint64_t da = tc::sdesc_swizzled(a0, A_MN ? 8192 : 16), db = tc::sdesc_swizzled(a0 + S::A_BYTES, B_MN ? 8192 : 16);
+            int s = 0, phase = 0, acc = 0, acc_phase = 1;
             for (int t = start; t < tiles && fine; t += step) {
                 const Tile tile = walk.at(t);
-                const int acc = summed % S::ACCUMULATORS;
-                fine = tc::bar_wait_cluster(drained + acc, ((summed / S::ACCUMULATORS) & 1) ^ 1, WAIT_LIMIT);
+                const int blocks = tile.zero ? 0 : tile.k_blocks;
+                fine = __all_sync(0xffffffffu, tc::bar_wait(drained + acc, acc_phase, WAIT_LIMIT));
                 if (!fine) break;
                 tc::fence_after_sync();
-                for (int kb = 0; kb < tile.k_blocks && !tile.zero; ++kb, ++used) {
-                    const int s = used % STAGES;
-                    fine = tc::bar_wait_cluster(full + s, (used / STAGES) & 1, WAIT_LIMIT);
+                for (int kb = 0; kb < blocks; ++kb) {
+                    fine = __all_sync(0xffffffffu, tc::bar_wait(full + s, phase, WAIT_LIMIT));
                     if (!fine) break;
                     tc::fence_after_sync();
-                    const uint32_t a = tc::smem_u32(stages + s * S::STAGE);
-                    const uint64_t da = tc::sdesc_swizzled(a, A_MN ? 8192 : 16);
-                    const uint64_t db = tc::sdesc_swizzled(a + S::A_BYTES, B_MN ? 8192 : 16);
+                    if (issuer) {
+                        const uint64_t at = uint64_t(s * (S::STAGE >> 4));
 #pragma unroll
-                    for (int i = 0; i < BK / 16; ++i)
-                        tc::mma_group<CG>(tmem + acc * BN, da + i * A_STEP, db + i * B_STEP, ID, kb > 0 || i > 0);
-                    tc::commit_group<CG>(empty + s);
+                        for (int i = 0; i < BK / 16; ++i)
+                            tc::mma_group<CG>(tmem + acc * BN, da + at + i * A_STEP, db + at + i * B_STEP, ID, kb > 0 || i > 0);
+                        tc::commit_group<CG>(empty + s);
+                    }
+                    __syncwarp();
+                    if (++s == STAGES) {
+                        s = 0;
+                        phase ^= 1;
+                    }
                 }
                 if (!fine) break;
-                tc::commit_group<CG>(done + acc);
-                ++summed;
+                if (issuer) tc::commit_group<CG>(done + acc);
+                __syncwarp();
+                if (++acc == S::ACCUMULATORS) {
+                    acc = 0;
+                    acc_phase ^= 1;
+                }
             }
             if (!fine) {
-                atomicExch(p.error, 2);
-                tc::commit_group<CG>(drain);
+                if (issuer) {
+                    atomicExch(p.error, 2);
+                    tc::commit_group<CG>(drain);
+                }
+                __syncwarp();
                 tc::bar_wait(drain, 0, WAIT_LIMIT);
             }
         }
@@ -408,7 +436,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
         for (int t = start + set * step; t < tiles && fine; t += S::SETS * step, summed += S::SETS) {
             const Tile tile = walk.at(t);
             const int acc = summed % S::ACCUMULATORS;
-            const int row = tile.m0 + int(rank) * 128 + quadrant * 32, column0 = tile.n0 + group * 32;
+            const int row = tile.m0 + rank * 128 + quadrant * 32, column0 = tile.n0 + group * 32;
             const long long at = (MODE == DW ? (long long)tile.g * p.m * p.n : 0) + (long long)row * p.n + column0;
             const uint16_t* residual = MODE == FWD && p.residual && !tile.zero ? static_cast<const uint16_t*>(p.residual) + at : nullptr;
             Window w{p.n, min(32, tile.m_end - row), p.n - column0, wide};
@@ -427,7 +455,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
                     __syncwarp();
                 }
             }
-            fine = __all_sync(0xffffffffu, tc::bar_wait_cluster(done + acc, (summed / S::ACCUMULATORS) & 1, WAIT_LIMIT));
+            fine = __all_sync(0xffffffffu, tc::bar_wait(done + acc, (summed / S::ACCUMULATORS) & 1, WAIT_LIMIT));
             if (!fine) break;
             tc::fence_after_sync();
 #pragma unroll 1
@@ -837,14 +865,28 @@ void with_linear_type(int dtype, F&& f) {
 
 constexpr int SMS = 148;  // of a B200: the sizes of scratch must not depend on the device that asks
 
-// Tiles of 256 x 256 by SM pairs where they fill the machine, else 128 x 128, or 128 x 64 for 64 columns or fewer.
+// The tile shape: the one whose waves over the SMs (or SM pairs) take the least time, in columns of 128 rows per CTA.
+// The factors are what narrower tiles cost more per column: all are fed from L2 at its rate, about 11 TB/s, and the
+// smaller the tile the less arithmetic there is per byte (input gradient of 16384 x 2048 -> 8192 bf16: 256 x 256 by
+// pairs 1530 TFLOP/s, 128 x 128 890, 128 x 64 450; 256 x 128 by pairs no better than 128 x 128).
 struct Config {
     int cg, bn;
 };
-Config tile_config(int64_t m, int n, int64_t others) {
+Config tile_config(int64_t m, int n, int64_t groups, bool groups_share_m) {
     if (n <= 64) return {1, 64};
-    if (ceil_div(m, 256) * ceil_div(n, 256) * others >= SMS / 2) return {2, 256};
-    return {1, 128};
+    Config best{};
+    double least = 0;
+    for (const auto& [config, factor] : {std::pair<Config, double>{{2, 256}, 1.0}, {{1, 128}, 1.72}, {{1, 64}, 3.4}}) {
+        const int rows = 128 * config.cg;
+        // several groups in m rows: each leaves half a tile on average
+        const int64_t row_tiles = groups_share_m && groups > 1 ? m / rows + (groups + 1) / 2 : ceil_div(m, rows) * (groups_share_m ? 1 : groups);
+        const double cost = double(ceil_div(std::max<int64_t>(1, row_tiles) * ceil_div(n, config.bn), SMS / config.cg)) * config.bn * factor;
+        if (!best.cg || cost < least) {
+            best = config;
+            least = cost;
+        }
+    }
+    return best;
 }
 template <typename F>
 void with_config(Config c, F&& f) {
@@ -953,7 +995,7 @@ struct WeightUnits {
     int64_t chunk, units;
     bool split;
     WeightUnits(int64_t rows, int inputs, int outputs, int groups) {
-        config = tile_config(outputs, inputs, groups);
+        config = tile_config(outputs, inputs, groups, false);
         tiles = ceil_div(outputs, 128 * config.cg) * ceil_div(inputs, config.bn);
         const int64_t wanted = 2 * SMS / config.cg, have = tiles * groups;
         chunk = std::max<int64_t>(BK, ceil_div(rows, BK) * BK);
@@ -1078,7 +1120,7 @@ extern "C" int odie_linear(const void* x, const void* weight, const void* bias, 
         p.error = error_word();
         const bool bf16 = dtype == ROW_BF16;
         with_linear_type(dtype, [&](auto type) {
-            with_config(tile_config(ceil_div(rows, groups), outputs, groups), [&](auto cg, auto bn) {
+            with_config(tile_config(rows, outputs, groups, true), [&](auto cg, auto bn) {
                 constexpr int CG = decltype(cg)::value, BN = decltype(bn)::value;
                 launch_gemm<decltype(type), FWD, CG, BN>(tensor_map(x, bf16, inputs, rows, 0, ld, 128),
                                                          tensor_map(weight, bf16, inputs, outputs, groups, ld, BN / CG), p,
@@ -1171,7 +1213,7 @@ extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, cons
             if (d_x) {
                 p.k = outputs;
                 p.out = d_x;
-                with_config(tile_config(ceil_div(rows, groups), inputs, groups), [&](auto cg, auto bn) {
+                with_config(tile_config(rows, inputs, groups, true), [&](auto cg, auto bn) {
                     constexpr int CG = decltype(cg)::value, BN = decltype(bn)::value;
                     launch_gemm<T, DX, CG, BN>(tensor_map(dz, bf16, outputs, rows, 0, ld_z, 128),
                                                tensor_map(s.weight ? s.weight : weight, bf16, inputs, outputs, groups, ld_x, 64), p,

@@ -108,22 +108,6 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, uint32_
     return false;
 }
 
-// The same, also ordered after what other CTAs of the cluster did before they arrived.
-__device__ __forceinline__ bool bar_wait_cluster(uint64_t* bar, uint32_t parity, uint32_t limit) {
-    const uint32_t address = smem_u32(bar);
-    for (uint32_t i = 0; i < limit; ++i) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, "
-            "p;\n\t}\n"
-            : "=r"(done)
-            : "r"(address), "r"(parity)
-            : "memory");
-        if (done) return true;
-    }
-    return false;
-}
-
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory"); }
 __device__ __forceinline__ void fence_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
 __device__ __forceinline__ void fence_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
@@ -170,6 +154,13 @@ __device__ __forceinline__ void tmem_dealloc_group(uint32_t base, uint32_t colum
         asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(base), "r"(columns) : "memory");
     else
         tmem_dealloc(base, columns);
+}
+
+// One lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}\n" : "=r"(one));
+    return one != 0;
 }
 
 // Cluster helpers: this CTA's rank, the shared::cluster address of CTA 0's copy of a shared variable, and the
