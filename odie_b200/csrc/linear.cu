@@ -60,15 +60,16 @@ struct GemmArgs {
     int m;               // DW: outputs (rows of d W)
     int n;               // columns of C
     int k;               // FWD, DX: length of the sum
-    int chunk;           // DW: rows per unit of work (a multiple of BK)
+    int chunk;           // DW: rows per unit of work (a multiple of BK); FWD, DX: blocks of K per split
+    int splits;          // FWD, DX without offsets: the sum over K cut among this many tiles, joined by finish_kernel
     Divide by_bands;     // FWD, DX: tiles of a full band
-    Divide by_tiles, by_columns;  // DW: tiles of d W, and of one row of them
+    Divide by_tiles, by_columns;  // tiles of d W (DW) or of C (splits), and of one row of them
     void* out;
     const void* bias;
     const void* residual;
     uint16_t* slope;
     int activation;
-    float* partial;      // DW with several units per tile: [unit][m][n] sums, joined by join_kernel
+    float* partial;      // with several units per tile: [unit][m][n] sums, joined by join_kernel or finish_kernel (m: rows)
     const CUtensorMap* group_maps;  // DW with offsets: [groups][2]
     int* error;
 };
@@ -97,8 +98,8 @@ struct Tile {
     int g;
     int m0, n0;          // first row (FWD, DX: global row; DW: output) of the tile and first column
     int m_end;           // rows from here on are not stored
-    int k0, k_blocks;    // DW: first row of the sum; blocks of 64
-    int unit;            // DW: index of the partial sum
+    int k0, k_blocks;    // first value of K of the sum (DW: row); blocks of 64
+    int unit;            // index of the partial sum
     bool zero;           // nothing to sum: zeros are stored
 };
 
@@ -119,16 +120,20 @@ struct Walk {
     __device__ __forceinline__ Tile at(int t) {
         constexpr int TM = 128 * CG;
         Tile tile;
-        int key = t, inside = 0;
-        if (MODE == DW) {
+        int key = t, inside = 0, split = 0;
+        if (MODE == DW || p.splits > 1) {
             key = p.by_tiles(t);
             inside = t - key * int(p.by_tiles.d);
+            if (MODE != DW) {
+                split = key;
+                key = inside;
+            }
         }
         while (g < p.groups && uniform(first[g + 1]) <= key) ++g;
         tile.g = g;
         const int from = uniform(begin[g]), to = g < p.groups ? uniform(begin[g + 1]) : int(p.rows);
         int local = key - uniform(first[g]);
-        tile.unit = key;
+        tile.unit = MODE == DW ? key : split;
         if (MODE == DW) {
             tile.k0 = from + local * p.chunk;
             const int rows = max(0, min(to - tile.k0, p.chunk));
@@ -156,8 +161,8 @@ struct Walk {
             tile.m0 = from + (band * BAND + m) * TM;
             tile.n0 = n * BN;
             tile.m_end = to;
-            tile.k0 = 0;
-            tile.k_blocks = (p.k + BK - 1) / BK;
+            tile.k0 = split * p.chunk * BK;
+            tile.k_blocks = min((p.k + BK - 1) / BK - split * p.chunk, p.chunk);
             tile.zero = g == p.groups;
         }
         return tile;
@@ -308,7 +313,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
     const uint32_t tmem = uniform(*tmem_at);
     const uint32_t full_leader = CG == 2 ? uniform(tc::leader_address(full)) : 0;
     const int units = uniform(first[p.groups + 1]);
-    const int tiles = MODE == DW ? units * nt * ((p.m + S::TM - 1) / S::TM) : units;
+    const int tiles = MODE == DW ? units * nt * ((p.m + S::TM - 1) / S::TM) : units * p.splits;
     const int start = int(blockIdx.x) / CG, step = int(gridDim.x) / CG;
     bool fine = true;
     Walk<MODE, CG, BN> walk(p, begin, first);
@@ -339,13 +344,13 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
                     if (rank == 0) tc::bar_expect(full + s, S::STAGE * CG);
                     char* a = stages + s * S::STAGE;
                     char* b = a + S::A_BYTES;
-                    const int k = kb * BK;
+                    const int k = tile.k0 + kb * BK;
                     if (MODE == DW) {
 #pragma unroll
-                        for (int i = 0; i < 2; ++i) tc::tma_load_2d<CG>(a + i * 8192, ma, m + 64 * i, tile.k0 + k, bar);
+                        for (int i = 0; i < 2; ++i) tc::tma_load_2d<CG>(a + i * 8192, ma, m + 64 * i, k, bar);
 #pragma unroll
                         for (int i = 0; i < S::B_ROWS / 64; ++i)
-                            tc::tma_load_2d<CG>(b + i * 8192, mb, n + 64 * i, tile.k0 + k, bar);
+                            tc::tma_load_2d<CG>(b + i * 8192, mb, n + 64 * i, k, bar);
                     } else {
                         tc::tma_load_2d<CG>(a, ma, k, m, bar);
                         if (MODE == FWD) {
@@ -438,11 +443,11 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
             const int acc = summed % S::ACCUMULATORS;
             const int row = tile.m0 + rank * 128 + quadrant * 32, column0 = tile.n0 + group * 32;
             const long long at = (MODE == DW ? (long long)tile.g * p.m * p.n : 0) + (long long)row * p.n + column0;
-            const uint16_t* residual = MODE == FWD && p.residual && !tile.zero ? static_cast<const uint16_t*>(p.residual) + at : nullptr;
+            const uint16_t* residual = MODE == FWD && p.residual && !tile.zero && !p.partial ? static_cast<const uint16_t*>(p.residual) + at : nullptr;
             Window w{p.n, min(32, tile.m_end - row), p.n - column0, wide};
             Window wr{p.n, w.rows, w.columns, wide_residual};
             uint4 r[4];
-            if (MODE == FWD && !tile.zero) {  // what does not need the sum is read while it is awaited
+            if (MODE == FWD && !tile.zero && !p.partial) {  // what does not need the sum is read while it is awaited
                 if (residual && wr.wide) window_load(residual, wr, lane, r);
                 if (tile.g != bias_g || tile.n0 != bias_n0) {
                     bias_g = tile.g;
@@ -477,7 +482,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
                     __syncwarp();
                     if (lane == 0) tc::bar_arrive_cluster(CG == 2 ? tc::leader_address(drained + acc) : tc::smem_u32(drained + acc));
                 }
-                if (MODE == DW && p.partial) {
+                if (p.partial) {
                     if (lane < w.rows) {
                         float* to = p.partial + ((long long)tile.unit * p.m + row + lane) * p.n + column0 + j * STRIDE;
                         if (p.n % 4 == 0) {
@@ -611,6 +616,61 @@ __global__ void __launch_bounds__(256) join_kernel(const float* partial, T* d_we
         }
         __syncthreads();
     }
+}
+
+// The sums over parts of K, in order, with the epilogue of the products (DX: neither bias, residual nor activation).
+struct FinishArgs {
+    const float* partial;  // [splits][rows][n]
+    int splits;
+    long long count;       // rows * n
+    int n;
+    const void* bias;
+    const void* residual;
+    void* out;
+    uint16_t* slope;
+    int activation;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) finish_kernel(FinishArgs a) {
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < a.count; i += (long long)gridDim.x * 256) {
+        float sum = 0.0f;
+#pragma unroll 8
+        for (int s = 0; s < a.splits; ++s) sum += a.partial[s * a.count + i];
+        if (a.bias) sum += to_float(static_cast<const T*>(a.bias)[i % a.n]);
+        const Pair z = same(sum), added = same(a.residual ? to_float(static_cast<const T*>(a.residual)[i]) : 0.0f);
+        Pair slope, y;
+        if (a.activation == ACT_RELU) y = activate<ACT_RELU, true>(z, slope, added);
+        else if (a.activation == ACT_SILU) y = activate<ACT_SILU, true>(z, slope, added);
+        else if (a.activation == ACT_GELU) y = activate<ACT_GELU, true>(z, slope, added);
+        else y = activate<ACT_NONE, true>(z, slope, added);
+        static_cast<T*>(a.out)[i] = from_float<T>(both(y).x);
+        if (a.slope) a.slope[i] = uint16_t(slope_codes(slope));
+    }
+}
+
+// d W from few units: a thread per four elements.
+template <typename T>
+__global__ void __launch_bounds__(256) join_few_kernel(const float* partial, T* d_weight, const int* offsets, long long rows, int chunk,
+                                                       long long size) {
+    const int g = blockIdx.y, lane = threadIdx.x & 31;
+    long long begin, end;
+    int before = 0;
+    for (int i = lane; i < g; i += 32) {
+        group_rows(offsets, i, rows, begin, end);
+        before += int(max(1ll, (end - begin + chunk - 1) / chunk));
+    }
+    const long long unit = __reduce_add_sync(0xffffffffu, before);
+    group_rows(offsets, g, rows, begin, end);
+    const int count = int(max(1ll, (end - begin + chunk - 1) / chunk));
+    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
+    if (i >= size) return;
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int u = 0; u < count; ++u) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(partial + (unit + u) * size + i));
+        sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
+    }
+    *reinterpret_cast<uint2*>(d_weight + g * size + i) = make_uint2(pack_pair<T>(sum.x, sum.y), pack_pair<T>(sum.z, sum.w));
 }
 
 // ---------------------------------------------------------------- dz and the bias gradient
@@ -866,9 +926,9 @@ void with_linear_type(int dtype, F&& f) {
 constexpr int SMS = 148;  // of a B200: the sizes of scratch must not depend on the device that asks
 
 // The tile shape: the one whose waves over the SMs (or SM pairs) take the least time, in columns of 128 rows per CTA.
-// The factors are what narrower tiles cost more per column: all are fed from L2 at its rate, about 11 TB/s, and the
-// smaller the tile the less arithmetic there is per byte (input gradient of 16384 x 2048 -> 8192 bf16: 256 x 256 by
-// pairs 1530 TFLOP/s, 128 x 128 890, 128 x 64 450; 256 x 128 by pairs no better than 128 x 128).
+// The factors are what narrower tiles cost more per column, with less arithmetic per byte from L2 (input gradient of
+// 16384 x 2048 -> 8192 bf16: 256 x 256 by pairs 1491 TFLOP/s, 128 x 128 1082, 128 x 64 699; weight gradient 1335, 1105,
+// 694; 256 x 128 by pairs took a fifth longer than 256 x 256 and saved no wave there).
 struct Config {
     int cg, bn;
 };
@@ -876,7 +936,7 @@ Config tile_config(int64_t m, int n, int64_t groups, bool groups_share_m) {
     if (n <= 64) return {1, 64};
     Config best{};
     double least = 0;
-    for (const auto& [config, factor] : {std::pair<Config, double>{{2, 256}, 1.0}, {{1, 128}, 1.72}, {{1, 64}, 3.4}}) {
+    for (const auto& [config, factor] : {std::pair<Config, double>{{2, 256}, 1.0}, {{1, 128}, 1.35}, {{1, 64}, 2.0}}) {
         const int rows = 128 * config.cg;
         // several groups in m rows: each leaves half a tile on average
         const int64_t row_tiles = groups_share_m && groups > 1 ? m / rows + (groups + 1) / 2 : ceil_div(m, rows) * (groups_share_m ? 1 : groups);
@@ -901,7 +961,11 @@ void launch_gemm(const CUtensorMap& a, const CUtensorMap& b, GemmArgs p, int64_t
     const int64_t nt = ceil_div(p.n, BN);
     p.by_bands = Divide::by(BAND * nt);
     p.by_columns = Divide::by(nt);
-    p.by_tiles = Divide::by(nt * ceil_div(std::max(1, p.m), 128 * CG));
+    p.by_tiles = Divide::by(nt * ceil_div(MODE == DW ? p.m : p.rows, 128 * CG));
+    if (MODE != DW && p.splits <= 1) {
+        p.splits = 1;
+        p.chunk = int(ceil_div(p.k, BK));
+    }
     using S = Shape<CG, BN>;
     const auto kernel = gemm_kernel<T, MODE, CG, BN>;
     ODIE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes(1024)));
@@ -951,6 +1015,14 @@ void launch_few_rows(const FewArgs& a, cudaStream_t stream) {
 template <typename T>
 void launch_join(const float* partial, void* d_weight, void* d_bias, const int* offsets, int groups, int64_t rows, int64_t chunk,
                  int64_t size, int bias, cudaStream_t stream) {
+    // many elements and few units: 1024 x 1024 of 8 units took 45 us with a warp's share of units per element
+    if (bias == 0 && size % 4 == 0 && uintptr_t(d_weight) % 8 == 0 && size >= 16 * ceil_div(rows, chunk) * 256) {
+        join_few_kernel<T><<<dim3(unsigned(ceil_div(size, 1024)), unsigned(groups)), 256, 0, stream>>>(
+            partial, static_cast<T*>(d_weight), offsets, rows, int(chunk), size);
+        ODIE_CUDA(cudaGetLastError());
+        note_launch();
+        return;
+    }
     join_kernel<T><<<dim3(unsigned(std::min<int64_t>(ceil_div(size + bias, 32), 4096)), unsigned(groups)), 256, 0, stream>>>(
         partial, static_cast<T*>(d_weight), static_cast<T*>(d_bias), offsets, rows, int(chunk), size, bias);
     ODIE_CUDA(cudaGetLastError());
@@ -974,15 +1046,56 @@ bool on_16_bytes(std::initializer_list<const void*> pointers) {
     return bits % 16 == 0;
 }
 
+// FWD, DX of one group without offsets: where the tiles leave SMs idle, the sum over K is cut into as many parts as
+// there are SMs for (64 rows of 4096 -> 4096 bf16: 24 us in 64 tiles).
+struct Splits {
+    int parts, blocks;  // blocks of K per part
+    Splits(int64_t rows, int n, int k, int groups, bool offsets) : parts(1), blocks(int(ceil_div(k, BK))) {
+        if (rows == 0 || offsets) return;
+        const Config c = tile_config(rows, n, groups, true);
+        const int64_t tiles = ceil_div(rows, 128 * c.cg) * ceil_div(n, c.bn), wanted = std::min<int64_t>(SMS / c.cg / tiles, blocks / 8);
+        if (wanted < 2) return;
+        blocks = int(ceil_div(blocks, wanted));
+        parts = int(ceil_div(ceil_div(k, BK), blocks));
+    }
+    int64_t bytes(int64_t rows, int n) const { return parts > 1 ? parts * rows * n * 4 : 0; }
+};
+
+template <typename T, int MODE>
+void launch_product(const void* a, const void* b, int64_t ld_a, int64_t ld_b, int outputs, int inputs, GemmArgs p, const Splits& split,
+                    float* partial, cudaStream_t stream) {
+    const bool bf16 = std::is_same<T, __nv_bfloat16>::value;
+    if (split.parts > 1) {
+        p.splits = split.parts;
+        p.chunk = split.blocks;
+        p.partial = partial;
+        p.m = int(p.rows);
+    }
+    with_config(tile_config(p.rows, p.n, p.groups, true), [&](auto cg, auto bn) {
+        constexpr int CG = decltype(cg)::value, BN = decltype(bn)::value;
+        launch_gemm<T, MODE, CG, BN>(tensor_map(a, bf16, p.k, p.rows, 0, ld_a, 128),
+                                     tensor_map(b, bf16, inputs, outputs, p.groups, ld_b, MODE == FWD ? BN / CG : 64), p,
+                                     (ceil_div(p.rows, 128 * CG) + p.groups + 1) * ceil_div(p.n, BN) * split.parts, stream);
+    });
+    if (split.parts > 1) {
+        const FinishArgs f{partial, split.parts, p.rows * p.n, p.n, p.bias, p.residual, p.out, p.slope, p.activation};
+        finish_kernel<T><<<unsigned(std::min<int64_t>(ceil_div(f.count, 256), 16 * SMS)), 256, 0, stream>>>(f);
+        ODIE_CUDA(cudaGetLastError());
+        note_launch();
+    }
+}
+
 // ---- the pieces of scratch, in order; the size functions walk the same list
 struct ForwardScratch {
     void *x, *weight;
+    float* partial;
     int64_t bytes;
     ForwardScratch(void* base, int64_t rows, int inputs, int outputs, int groups) {
         Scratch s{static_cast<char*>(base)};
         const bool pad = inputs % 8 != 0;
         x = pad ? s.take(rows * round8(inputs) * 2) : nullptr;
         weight = pad ? s.take(int64_t(groups) * outputs * round8(inputs) * 2) : nullptr;
+        partial = static_cast<float*>(s.take(Splits(rows, outputs, inputs, groups, groups > 1).bytes(rows, outputs)));
         bytes = s.used;
     }
 };
@@ -1033,7 +1146,7 @@ void launch_dz(const DzArgs& a, cudaStream_t stream) {
 
 struct BackwardScratch {
     void *dz, *x, *weight, *maps;
-    float *bias, *partial, *thin;
+    float *bias, *partial, *split, *thin;
     int64_t bytes;
     BackwardScratch(void* base, int64_t rows, int inputs, int outputs, int groups) {
         Scratch s{static_cast<char*>(base)};
@@ -1045,6 +1158,7 @@ struct BackwardScratch {
         bias = static_cast<float*>(s.take(dz_units(rows, groups) * outputs * 4));
         const WeightUnits u(rows, inputs, outputs, groups);
         partial = static_cast<float*>(u.split ? s.take(u.units * outputs * int64_t(inputs) * 4) : nullptr);
+        split = static_cast<float*>(s.take(Splits(rows, inputs, outputs, groups, groups > 1).bytes(rows, inputs)));
         bytes = s.used;
         thin = static_cast<float*>(base);  // thin layers need nothing else
         if (thin_sizes(inputs, outputs))
@@ -1118,14 +1232,9 @@ extern "C" int odie_linear(const void* x, const void* weight, const void* bias, 
         p.slope = slope;
         p.activation = activation;
         p.error = error_word();
-        const bool bf16 = dtype == ROW_BF16;
         with_linear_type(dtype, [&](auto type) {
-            with_config(tile_config(rows, outputs, groups, true), [&](auto cg, auto bn) {
-                constexpr int CG = decltype(cg)::value, BN = decltype(bn)::value;
-                launch_gemm<decltype(type), FWD, CG, BN>(tensor_map(x, bf16, inputs, rows, 0, ld, 128),
-                                                         tensor_map(weight, bf16, inputs, outputs, groups, ld, BN / CG), p,
-                                                         (ceil_div(rows, 128 * CG) + groups + 1) * ceil_div(outputs, BN), stream);
-            });
+            launch_product<decltype(type), FWD>(x, weight, ld, ld, outputs, inputs, p, Splits(rows, outputs, inputs, groups, offsets), s.partial,
+                                                stream);
         });
     });
 }
@@ -1213,12 +1322,8 @@ extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, cons
             if (d_x) {
                 p.k = outputs;
                 p.out = d_x;
-                with_config(tile_config(rows, inputs, groups, true), [&](auto cg, auto bn) {
-                    constexpr int CG = decltype(cg)::value, BN = decltype(bn)::value;
-                    launch_gemm<T, DX, CG, BN>(tensor_map(dz, bf16, outputs, rows, 0, ld_z, 128),
-                                               tensor_map(s.weight ? s.weight : weight, bf16, inputs, outputs, groups, ld_x, 64), p,
-                                               (ceil_div(rows, 128 * CG) + groups + 1) * ceil_div(inputs, BN), stream);
-                });
+                launch_product<T, DX>(dz, s.weight ? s.weight : weight, ld_z, ld_x, outputs, inputs, p,
+                                      Splits(rows, inputs, outputs, groups, offsets), s.split, stream);
             }
             if (d_weight) {
                 const WeightUnits u(rows, inputs, outputs, groups);
