@@ -32,7 +32,7 @@ namespace {
 //   DX   A = dz [rows][outputs] (K-major), B = W_g read along its columns (MN-major), K = outputs
 //   DW   A = dz, B = x read along their columns (both MN-major), K = the group's rows; C = d W_g
 //
-// One warp loads (TMA, 128-byte swizzle, STAGES blocks in flight), one thread multiplies into one of two (or four) TMEM
+// One warp loads (TMA, 128-byte swizzle, STAGES blocks in flight), one thread multiplies into one of two TMEM
 // accumulators, sixteen warps take the other one to global memory with bias, activation, residual and slope, so
 // that the epilogue of one tile runs beside the products of the next.  Persistent: CTA (pair) i takes tiles i,
 // i + grid, ...  Rows of other groups that a tile loads are never stored (FWD, DX); for DW, whose sum runs over
@@ -80,12 +80,12 @@ struct Shape {
     static constexpr int B_ROWS = BN / CG;  // per CTA
     static constexpr int A_BYTES = 128 * 128, B_BYTES = B_ROWS * 128, STAGE = A_BYTES + B_BYTES;
     static constexpr int STAGES = STAGE < 32768 ? 6 : 5;
-    // Sixteen epilogue warps, four per set of 32 TMEM columns (GROUPS) of a tile; the short tiles of 64 columns are
-    // handed out to four such sets in turn (SETS), each with an accumulator of its own.
+    // Sixteen epilogue warps, four per set of 32 TMEM columns (GROUPS) of a tile; tiles of 64 columns are handed out to
+    // two such sets in turn (SETS), each with an accumulator of its own.
     static constexpr int EPILOGUE_WARPS = 16, THREADS = (EPILOGUE_WARP + EPILOGUE_WARPS) * 32;
-    static constexpr int SETS = BN == 64 ? 4 : 1, GROUPS = EPILOGUE_WARPS / 4 / SETS;
+    static constexpr int SETS = BN == 64 ? 2 : 1, GROUPS = EPILOGUE_WARPS / 4 / SETS;
     static constexpr int WINDOWS = BN / 32 / GROUPS;            // per warp and tile: columns 32 (group + GROUPS j)
-    static constexpr int ACCUMULATORS = SETS == 1 ? 2 : SETS;
+    static constexpr int ACCUMULATORS = 2;
     static constexpr int WARP_BYTES = STAGING + WINDOWS * 128;  // staging tile and bias of an epilogue warp
     static constexpr int COLUMNS = ACCUMULATORS * BN;  // of TMEM
     static constexpr int HEAD = 1024;       // barriers, TMEM address
@@ -448,7 +448,10 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
             Window wr{p.n, w.rows, w.columns, wide_residual};
             uint4 r[4];
             if (MODE == FWD && !tile.zero && !p.partial) {  // what does not need the sum is read while it is awaited
-                if (residual && wr.wide) window_load(residual, wr, lane, r);
+                if (residual) {
+                    if (wr.wide) window_load(residual, wr, lane, r);
+                    else window_fetch(residual, wr, lane, stage);
+                }
                 if (tile.g != bias_g || tile.n0 != bias_n0) {
                     bias_g = tile.g;
                     bias_n0 = tile.n0;
@@ -506,7 +509,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
                             wr.columns -= STRIDE;
                             if (j + 1 < WINDOWS && wr.columns > 0) window_load(residual + (j + 1) * STRIDE, wr, lane, r);
                         } else {
-                            window_fetch(residual + j * STRIDE, wr, lane, stage);
+                            if (j > 0) window_fetch(residual + j * STRIDE, wr, lane, stage);
                             wr.columns -= STRIDE;
                         }
                         __syncwarp();
@@ -794,9 +797,11 @@ __global__ void __launch_bounds__(256) pad_kernel(const uint16_t* from0, uint16_
 }
 
 // ---------------------------------------------------------------- a few rows
-// Up to eight rows: y is bound by the bytes of W, which every warp reads straight into registers, one row of W (one
-// output) per warp and U vectors in flight per lane; x comes through shared memory meanwhile.  (The tensor-core tiles, 128 rows each, took
-// 26 us for one row of 4096 x 4096 bf16: 32 CTAs cannot draw the memory's rate.)
+// One or two rows: y is bound by the bytes of W, which every warp reads straight into registers, 16 vectors in flight
+// per lane: one row of W (one output) of up to 16 x 32 vectors, or four short ones.  x comes through shared memory
+// meanwhile.  (The tensor-core tiles, 128 rows each, take 11.5 us for 4096 x 4096 bf16 however few the rows, this 6.7
+// for one and 9.3 for two.  Widening x to fp32 first, or cutting K among a block's warps, left fewer vectors in flight
+// and took 10 to 12 us.)
 struct FewArgs {
     const void* x;
     const void* weight;
@@ -804,70 +809,79 @@ struct FewArgs {
     const void* residual;
     void* y;
     uint16_t* slope;
-    int rows, inputs, outputs;
+    int rows, inputs, outputs;  // rows: M
     int activation;
 };
 
-constexpr int FEW_ROWS = 8, FEW_THREADS = 128;
+constexpr int FEW_ROWS = 2, FEW_THREADS = 128, FEW_VECTORS = 16;
 
-template <typename T, int BYTES, int M>
+// M: rows; V: vectors per lane of one row of W at a time.
+template <typename T, int BYTES, int M, int V>
 __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(FewArgs a) {
     using P = Pack<T, BYTES>;
-    constexpr int U = M <= 2 ? 16 : 8, CHUNK = 32 * P::N * U;  // values of K at a time
+    constexpr int COLUMNS = FEW_VECTORS / V, CHUNK = 32 * P::N * V;  // CHUNK: values of K at a time
     __shared__ alignas(16) T xs[M][CHUNK];
-    const int lane = threadIdx.x & 31, n = blockIdx.x * (FEW_THREADS / 32) + (threadIdx.x >> 5);
-    const T* w = static_cast<const T*>(a.weight) + (long long)min(n, a.outputs - 1) * a.inputs;
+    const int lane = threadIdx.x & 31, n0 = (blockIdx.x * (FEW_THREADS / 32) + (threadIdx.x >> 5)) * COLUMNS;
+    const T* w = static_cast<const T*>(a.weight);
     const T* x = static_cast<const T*>(a.x);
-    float sum[M];
+    float sum[COLUMNS][M];
 #pragma unroll
-    for (int m = 0; m < M; ++m) sum[m] = 0.0f;
-    for (int c0 = 0; c0 < a.inputs; c0 += CHUNK) {
-        P v[U];
+    for (int c = 0; c < COLUMNS; ++c)
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int k = c0 + (u * 32 + lane) * P::N;
-            v[u] = k < a.inputs ? P::load_once(w + k) : P::zero();
-        }
-        const int count = min(CHUNK, a.inputs - c0) / P::N;
-        if (c0 > 0) __syncthreads();
+        for (int m = 0; m < M; ++m) sum[c][m] = 0.0f;
+    for (int k0 = 0; k0 < a.inputs; k0 += CHUNK) {
+        P v[COLUMNS][V];
+#pragma unroll
+        for (int c = 0; c < COLUMNS; ++c)
+#pragma unroll
+            for (int u = 0; u < V; ++u) {
+                const int k = k0 + (u * 32 + lane) * P::N;
+                v[c][u] = k < a.inputs ? P::load_once(w + (long long)min(n0 + c, a.outputs - 1) * a.inputs + k) : P::zero();
+            }
+        const int count = min(CHUNK, a.inputs - k0) / P::N;
+        if (k0 > 0) __syncthreads();
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll 4
             for (int i = threadIdx.x; i < CHUNK / P::N; i += FEW_THREADS) {
-                const P q = i < count ? P::load(x + (long long)min(m, a.rows - 1) * a.inputs + c0 + i * P::N) : P::zero();
+                const P q = i < count ? P::load(x + (long long)m * a.inputs + k0 + i * P::N) : P::zero();
                 q.store(&xs[m][i * P::N]);
             }
         __syncthreads();
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < V; ++u)
 #pragma unroll
             for (int m = 0; m < M; ++m) {
                 P q;
                 *reinterpret_cast<typename Raw<BYTES>::type*>(&q) = *reinterpret_cast<const typename Raw<BYTES>::type*>(&xs[m][(u * 32 + lane) * P::N]);
 #pragma unroll
-                for (int e = 0; e < P::N; ++e) sum[m] = fmaf(to_float(v[u].v[e]), to_float(q.v[e]), sum[m]);
+                for (int c = 0; c < COLUMNS; ++c)
+#pragma unroll
+                    for (int e = 0; e < P::N; ++e) sum[c][m] = fmaf(to_float(v[c][u].v[e]), to_float(q.v[e]), sum[c][m]);
             }
     }
-    if (n >= a.outputs) return;
-    float mine = 0.0f;
 #pragma unroll
-    for (int m = 0; m < M; ++m) {
+    for (int c = 0; c < COLUMNS; ++c) {
+        const int n = n0 + c;
+        float mine = 0.0f;
 #pragma unroll
-        for (int d = 16; d > 0; d /= 2) sum[m] += __shfl_xor_sync(0xffffffffu, sum[m], d);
-        if (lane == m) mine = sum[m];
+        for (int m = 0; m < M; ++m) {
+#pragma unroll
+            for (int d = 16; d > 0; d /= 2) sum[c][m] += __shfl_xor_sync(0xffffffffu, sum[c][m], d);
+            if (lane == m) mine = sum[c][m];
+        }
+        if (lane >= M || n >= a.outputs) continue;
+        const long long at = (long long)lane * a.outputs + n;
+        if (a.bias) mine += to_float(static_cast<const T*>(a.bias)[n]);
+        const Pair z = same(mine), added = same(a.residual ? to_float(static_cast<const T*>(a.residual)[at]) : 0.0f);
+        Pair slope, y;
+        if (a.activation == ACT_RELU) y = activate<ACT_RELU, true>(z, slope, added);
+        else if (a.activation == ACT_SILU) y = activate<ACT_SILU, true>(z, slope, added);
+        else if (a.activation == ACT_GELU) y = activate<ACT_GELU, true>(z, slope, added);
+        else y = activate<ACT_NONE, true>(z, slope, added);
+        static_cast<T*>(a.y)[at] = from_float<T>(both(y).x);
+        if (a.slope) a.slope[at] = uint16_t(slope_codes(slope));
     }
-    if (lane >= min(M, a.rows)) return;
-    const long long at = (long long)lane * a.outputs + n;
-    if (a.bias) mine += to_float(static_cast<const T*>(a.bias)[n]);
-    const Pair z = same(mine), added = same(a.residual ? to_float(static_cast<const T*>(a.residual)[at]) : 0.0f);
-    Pair slope, y;
-    if (a.activation == ACT_RELU) y = activate<ACT_RELU, true>(z, slope, added);
-    else if (a.activation == ACT_SILU) y = activate<ACT_SILU, true>(z, slope, added);
-    else if (a.activation == ACT_GELU) y = activate<ACT_GELU, true>(z, slope, added);
-    else y = activate<ACT_NONE, true>(z, slope, added);
-    const float v = both(y).x;
-    static_cast<T*>(a.y)[at] = from_float<T>(v);
-    if (a.slope) a.slope[at] = uint16_t(slope_codes(slope));
 }
 
 // ---------------------------------------------------------------- host
@@ -996,18 +1010,20 @@ void launch_pad(const void* from0, void* to0, int64_t rows0, const void* from1, 
 
 template <typename T>
 void launch_few_rows(const FewArgs& a, cudaStream_t stream) {
-    const unsigned blocks = unsigned(ceil_div(a.outputs, FEW_THREADS / 32));
     const int vector = row_vector(a.inputs, ROW_F16, a.x, a.weight);
-    auto go = [&](auto bytes) {
-        constexpr int B = decltype(bytes)::value;
-        if (a.rows == 1) few_rows_kernel<T, B, 1><<<blocks, FEW_THREADS, 0, stream>>>(a);
-        else if (a.rows == 2) few_rows_kernel<T, B, 2><<<blocks, FEW_THREADS, 0, stream>>>(a);
-        else if (a.rows <= 4) few_rows_kernel<T, B, 4><<<blocks, FEW_THREADS, 0, stream>>>(a);
-        else few_rows_kernel<T, B, 8><<<blocks, FEW_THREADS, 0, stream>>>(a);
+    auto go = [&](auto bytes, auto rows) {
+        constexpr int B = decltype(bytes)::value, M = decltype(rows)::value, WARPS = FEW_THREADS / 32;
+        constexpr int SHORT = 4 * 32 * (B / 2);  // values of four vectors per lane
+        if (a.inputs <= SHORT) few_rows_kernel<T, B, M, 4><<<unsigned(ceil_div(a.outputs, WARPS * 4)), FEW_THREADS, 0, stream>>>(a);
+        else few_rows_kernel<T, B, M, FEW_VECTORS><<<unsigned(ceil_div(a.outputs, WARPS)), FEW_THREADS, 0, stream>>>(a);
     };
-    if (vector == 16) go(std::integral_constant<int, 16>{});
-    else if (vector == 4) go(std::integral_constant<int, 4>{});
-    else go(std::integral_constant<int, 2>{});
+    auto with_rows = [&](auto bytes) {
+        if (a.rows == 1) go(bytes, std::integral_constant<int, 1>{});
+        else go(bytes, std::integral_constant<int, 2>{});
+    };
+    if (vector == 16) with_rows(std::integral_constant<int, 16>{});
+    else if (vector == 4) with_rows(std::integral_constant<int, 4>{});
+    else with_rows(std::integral_constant<int, 2>{});
     ODIE_CUDA(cudaGetLastError());
     note_launch();
 }

@@ -143,7 +143,7 @@ def test_unaligned_and_strided_rows(cuda):
 
 
 # ---------------------------------------------------------------- linear
-LINEARS = [(1, 1, 1), (16, 4096, 72), (100, 3000, 200), (40, 1100, 515), (1, 64, 128), (2, 7, 3), (3, 256, 260), (8, 136, 24), (17, 40, 1000), (5, 333, 515), (127, 64, 64),
+LINEARS = [(1, 1, 1), (1, 9000, 40), (2, 1024, 33), (4, 2050, 64), (3, 5001, 10), (16, 4096, 72), (100, 3000, 200), (40, 1100, 515), (1, 64, 128), (2, 7, 3), (3, 256, 260), (8, 136, 24), (17, 40, 1000), (5, 333, 515), (127, 64, 64),
            (128, 32, 64), (129, 256, 256), (300, 1000, 72), (1000, 72, 264), (257, 2048, 128), (640, 520, 776), (5000, 200, 48), (2500, 1030, 31),
            # up to 64 inputs and outputs: the layers that stay in registers
            (9, 8, 8), (200, 24, 32), (333, 64, 40), (3000, 40, 64), (5000, 64, 64), (1111, 32, 8)]
