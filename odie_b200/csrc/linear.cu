@@ -60,6 +60,7 @@ struct GemmArgs {
     int m;               // DW: outputs (rows of d W)
     int n;               // columns of C
     int k;               // FWD, DX: length of the sum
+    int a_rows;          // FWD, DX: rows of A's boxes, 128 or, for fewer rows in all, those (rounded up to 8)
     int chunk;           // DW: rows per unit of work (a multiple of BK); FWD, DX: blocks of K per split
     int splits;          // FWD, DX without offsets: the sum over K cut among this many tiles, joined by finish_kernel
     Divide by_bands;     // FWD, DX: tiles of a full band
@@ -323,6 +324,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
     // each of them was moved there first: 575 cycles a block, more than the products take.)
     if (warp == 0) {
         const bool issuer = tc::elect_one();
+        const uint32_t stage_bytes = (MODE == DW ? S::STAGE : p.a_rows * 128 + S::B_BYTES) * CG;
         int s = 0, phase = 1, issued = 0;
         for (int t = start; t < tiles && fine; t += step) {
             const Tile tile = walk.at(t);
@@ -341,7 +343,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
                 if (!fine) break;
                 if (issuer) {
                     const uint32_t bar = CG == 2 ? full_leader + s * 8 : tc::smem_u32(full + s);
-                    if (rank == 0) tc::bar_expect(full + s, S::STAGE * CG);
+                    if (rank == 0) tc::bar_expect(full + s, stage_bytes);
                     char* a = stages + s * S::STAGE;
                     char* b = a + S::A_BYTES;
                     const int k = tile.k0 + kb * BK;
@@ -1087,9 +1089,12 @@ void launch_product(const void* a, const void* b, int64_t ld_a, int64_t ld_b, in
         p.partial = partial;
         p.m = int(p.rows);
     }
+    // (boxes of 128 rows over a matrix of fewer than 16 were twice as slow: 16 us against 9 for 15 and 16 rows of
+    // 4096 -> 4096; what the rest of the tile holds only reaches rows that are not stored)
+    p.a_rows = int(std::min<int64_t>(128, round8(p.rows)));
     with_config(tile_config(p.rows, p.n, p.groups, true), [&](auto cg, auto bn) {
         constexpr int CG = decltype(cg)::value, BN = decltype(bn)::value;
-        launch_gemm<T, MODE, CG, BN>(tensor_map(a, bf16, p.k, p.rows, 0, ld_a, 128),
+        launch_gemm<T, MODE, CG, BN>(tensor_map(a, bf16, p.k, p.rows, 0, ld_a, p.a_rows),
                                      tensor_map(b, bf16, inputs, outputs, p.groups, ld_b, MODE == FWD ? BN / CG : 64), p,
                                      (ceil_div(p.rows, 128 * CG) + p.groups + 1) * ceil_div(p.n, BN) * split.parts, stream);
     });
