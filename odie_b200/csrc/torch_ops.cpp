@@ -46,13 +46,19 @@ void check_device(const Tensor& t, const Tensor& as, const char* name) {
     TORCH_CHECK_VALUE(t.device() == as.device(), name, " is on ", t.device(), ", not ", as.device());
 }
 
-// What a backward pass returns.  Asked for a graph of it (create_graph), it may not be differentiated again.
-variable_list once(variable_list gradients) {
+// What a backward pass returns.  Asked for a graph of it (create_graph), it hangs from the tensors it came from by a
+// node that refuses to be differentiated.
+variable_list once(variable_list gradients, const variable_list& from) {
     if (!at::GradMode::is_enabled()) return gradients;
-    for (Tensor& g : gradients)
-        if (g.defined())
-            g = (*std::make_shared<torch::autograd::DelayedError>("the row operators of odie_b200 are differentiable once", 1))(
-                variable_list{g.detach().requires_grad_()})[0];
+    for (Tensor& g : gradients) {
+        if (!g.defined()) continue;
+        variable_list all{g.detach().requires_grad_()};
+        for (const Tensor& t : from)
+            if (t.defined() && t.requires_grad()) all.push_back(t);
+        const auto refuse = std::make_shared<torch::autograd::DelayedError>("the row operators of odie_b200 are differentiable once",
+                                                                            int64_t(all.size()));
+        g = (*refuse)(std::move(all))[0];
+    }
     return gradients;
 }
 
@@ -138,7 +144,7 @@ struct Dispatch : torch::autograd::Function<Dispatch> {
         if (need & 1) d_x = combined(d_rows, o, saved[1]);
         // d weights[t, j] = <x[t], d rows[slot]>: the same product as combine's, the rows' roles exchanged
         if (need & 2) d_weights = combine_gradients(saved[0], d_rows, o, Tensor(), false, true).second;
-        return once({d_x, d_weights, Tensor(), Tensor(), Tensor(), Tensor()});
+        return once({d_x, d_weights, Tensor(), Tensor(), Tensor(), Tensor()}, {gradients[0], saved[0], saved[1]});
     }
 };
 
@@ -155,7 +161,7 @@ struct Combine : torch::autograd::Function<Combine> {
         const int64_t need = ctx->saved_data["need"].toInt();
         const auto [d_rows, d_weights] =
             combine_gradients(gradients[0].contiguous(), saved[0], {saved[2], saved[3]}, saved[1], need & 1, need & 2);
-        return once({d_rows, d_weights, Tensor(), Tensor(), Tensor(), Tensor()});
+        return once({d_rows, d_weights, Tensor(), Tensor(), Tensor(), Tensor()}, {gradients[0], saved[0], saved[1]});
     }
 };
 
@@ -253,7 +259,7 @@ struct Linear : torch::autograd::Function<Linear> {
                                       stream_of(d_y)),
                  "odie_linear_backward");
         }
-        return once({d_x, d_weight, d_bias, d_residual, Tensor(), Tensor(), Tensor()});
+        return once({d_x, d_weight, d_bias, d_residual, Tensor(), Tensor(), Tensor()}, {gradients[0], x, weight, relu_y});
     }
 };
 
@@ -325,7 +331,7 @@ struct Embed : torch::autograd::Function<Embed> {
         done(odie_embed_backward(data(ids), int(ids.element_size()), ids.numel(), data(d_out), rows, width, row_type(d_out),
                                  float(ctx->saved_data["scale"].toDouble()), data(d_table), data(work), stream_of(d_out)),
              "odie_embed_backward");
-        return once({Tensor(), d_table, Tensor()});
+        return once({Tensor(), d_table, Tensor()}, {gradients[0]});
     }
 };
 

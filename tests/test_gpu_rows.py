@@ -425,6 +425,50 @@ def test_embed_shapes_and_empty(cuda):
             embed(**{**dict(ids=ids, table=table), **bad})
 
 
+def test_no_rows(cuda):
+    from odie_b200.experts import combine, dispatch, sort_rows
+    order = sort_rows(torch.empty((0, 2), dtype=torch.int32, device=cuda), 4)
+    x = torch.empty((0, 8), device=cuda, requires_grad=True)
+    weights = torch.empty((0, 2), device=cuda, requires_grad=True)
+    sent = dispatch(x, order, weights)
+    out = combine(sent, order, weights)
+    assert sent.shape == (0, 8) and out.shape == (0, 8)
+    d = torch.autograd.grad(out, [x, weights], torch.empty_like(out))
+    assert d[0].shape == (0, 8) and d[1].shape == (0, 2)
+
+
+def test_gradients_are_differentiable_once(cuda):
+    """create_graph gives the same gradients; differentiating them again is an error, not a silent zero."""
+    from odie_b200.experts import combine, dispatch, embed, linear, sort_rows
+    g = generator(1)
+    x, w = normal(g, 30, 16).half().requires_grad_(), normal(g, 16, 16).half().requires_grad_()
+    table = normal(g, 5, 16).requires_grad_()
+    order = sort_rows(torch.randint(0, 3, (30,), generator=g, device=cuda), 3)
+    ids = torch.randint(0, 5, (30,), generator=g, device=cuda)
+    for f, leaf in ((lambda: linear(x, w, activation='silu'), x), (lambda: dispatch(x, order), x),
+                    (lambda: combine(x, order), x), (lambda: embed(ids, table), table)):
+        y = f()
+        d = torch.ones_like(y, requires_grad=True)
+        (plain,) = torch.autograd.grad(y, leaf, torch.ones_like(y), retain_graph=True)
+        (graph,) = torch.autograd.grad(y, leaf, d, create_graph=True)
+        assert torch.equal(plain, graph)
+        with pytest.raises(RuntimeError, match='once'):
+            torch.autograd.grad(graph.sum(), d)
+
+
+def test_leaves_of_modules_accumulate(cuda):
+    """backward() twice accumulates into .grad, also through shared weights."""
+    from odie_b200.experts import linear
+    g = generator(4)
+    x, w = normal(g, 20, 32).half(), normal(g, 32, 32, std=0.1).half().requires_grad_()
+    y = linear(linear(x, w, activation='gelu'), w)
+    d = normal(g, 20, 32).half()
+    (once,) = torch.autograd.grad(y, w, d, retain_graph=True)
+    y.backward(d, retain_graph=True)
+    y.backward(d)
+    assert torch.equal(w.grad, once + once)
+
+
 def test_order_refusals(cuda):
     from odie_b200.experts import combine, dispatch, sort_rows
     ids = torch.zeros(6, 2, dtype=torch.int32, device=cuda)
