@@ -111,7 +111,7 @@ __device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, 
 
 // A role's walk over the tiles, in ascending order: the group is found by stepping on from the last one, and no integer
 // division is left (each of twenty warps walks; dividing, they spent four instructions per output element on it).
-template <int MODE, int CG, int BN>
+template <int MODE, int CG, int BN, bool PARTIAL>
 struct Walk {
     const GemmArgs& p;
     const int* begin;
@@ -122,7 +122,7 @@ struct Walk {
         constexpr int TM = 128 * CG;
         Tile tile;
         int key = t, inside = 0, split = 0;
-        if (MODE == DW || p.splits > 1) {
+        if (MODE == DW || PARTIAL) {
             key = p.by_tiles(t);
             inside = t - key * int(p.by_tiles.d);
             if (MODE != DW) {
@@ -162,8 +162,9 @@ struct Walk {
             tile.m0 = from + (band * BAND + m) * TM;
             tile.n0 = n * BN;
             tile.m_end = to;
-            tile.k0 = split * p.chunk * BK;
-            tile.k_blocks = min((p.k + BK - 1) / BK - split * p.chunk, p.chunk);
+            tile.k0 = PARTIAL ? split * p.chunk * BK : 0;
+            tile.k_blocks = (p.k + BK - 1) / BK;
+            if (PARTIAL) tile.k_blocks = min(tile.k_blocks - split * p.chunk, p.chunk);
             tile.zero = g == p.groups;
         }
         return tile;
@@ -243,7 +244,8 @@ __device__ __forceinline__ void finish(float (&v)[32], uint32_t (&codes)[16], co
     }
 }
 
-template <typename T, int MODE, int CG, int BN>
+// PARTIAL: the sums go to p.partial as they are, joined by another kernel.
+template <typename T, int MODE, int CG, int BN, bool PARTIAL>
 __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
     gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GemmArgs p) {
     using S = Shape<CG, BN>;
@@ -314,10 +316,10 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
     const uint32_t tmem = uniform(*tmem_at);
     const uint32_t full_leader = CG == 2 ? uniform(tc::leader_address(full)) : 0;
     const int units = uniform(first[p.groups + 1]);
-    const int tiles = MODE == DW ? units * nt * ((p.m + S::TM - 1) / S::TM) : units * p.splits;
+    const int tiles = MODE == DW ? units * nt * ((p.m + S::TM - 1) / S::TM) : PARTIAL ? units * p.splits : units;
     const int start = int(blockIdx.x) / CG, step = int(gridDim.x) / CG;
     bool fine = true;
-    Walk<MODE, CG, BN> walk(p, begin, first);
+    Walk<MODE, CG, BN, PARTIAL> walk(p, begin, first);
 
     // The loading and the multiplying warp walk their loops with all lanes and values that are the same in every lane,
     // and one lane issues: the operands of these instructions live in uniform registers.  (With one lane in the loops,
@@ -445,11 +447,11 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
             const int acc = summed % S::ACCUMULATORS;
             const int row = tile.m0 + rank * 128 + quadrant * 32, column0 = tile.n0 + group * 32;
             const long long at = (MODE == DW ? (long long)tile.g * p.m * p.n : 0) + (long long)row * p.n + column0;
-            const uint16_t* residual = MODE == FWD && p.residual && !tile.zero && !p.partial ? static_cast<const uint16_t*>(p.residual) + at : nullptr;
+            const uint16_t* residual = MODE == FWD && !PARTIAL && p.residual && !tile.zero ? static_cast<const uint16_t*>(p.residual) + at : nullptr;
             Window w{p.n, min(32, tile.m_end - row), p.n - column0, wide};
             Window wr{p.n, w.rows, w.columns, wide_residual};
             uint4 r[4];
-            if (MODE == FWD && !tile.zero && !p.partial) {  // what does not need the sum is read while it is awaited
+            if (MODE == FWD && !PARTIAL && !tile.zero) {  // what does not need the sum is read while it is awaited
                 if (residual) {
                     if (wr.wide) window_load(residual, wr, lane, r);
                     else window_fetch(residual, wr, lane, stage);
@@ -487,7 +489,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
                     __syncwarp();
                     if (lane == 0) tc::bar_arrive_cluster(CG == 2 ? tc::leader_address(drained + acc) : tc::smem_u32(drained + acc));
                 }
-                if (p.partial) {
+                if (PARTIAL) {
                     if (lane < w.rows) {
                         float* to = p.partial + ((long long)tile.unit * p.m + row + lane) * p.n + column0 + j * STRIDE;
                         if (p.n % 4 == 0) {
@@ -585,12 +587,13 @@ __global__ void __launch_bounds__(32) group_maps_kernel(const __grid_constant__ 
                  : "memory");
 }
 
-// d W from the units' sums: a block per 32 elements, each warp over its share of the units, the shares in order.
-// A unit holds `size` sums of d W and `bias` sums of d b (either may be unwanted: null).
-template <typename T>
+// d W from the units' sums: a block per 32 x WIDTH elements (WIDTH 4 where sizes and pointers allow), each warp over its
+// share of the units, the shares in order.  A unit holds `size` sums of d W and `bias` sums of d b (either may be
+// unwanted: null).
+template <typename T, int WIDTH>
 __global__ void __launch_bounds__(256) join_kernel(const float* partial, T* d_weight, T* d_bias, const int* offsets, long long rows,
                                                    int chunk, long long size, int bias) {
-    __shared__ float part[8][33];
+    __shared__ float part[8][32 * WIDTH + 1];
     const int g = blockIdx.y, lane = threadIdx.x & 31, line = threadIdx.x >> 5;
     long long begin, end;
     int before = 0;  // units of earlier groups
@@ -603,21 +606,37 @@ __global__ void __launch_bounds__(256) join_kernel(const float* partial, T* d_we
     const int count = int(max(1ll, (end - begin + chunk - 1) / chunk)), share = (count + 7) / 8;
     const int from = min(count, line * share), last = min(count, from + share);
     const long long all = size + bias;
-    for (long long i0 = (long long)blockIdx.x * 32; i0 < all; i0 += (long long)gridDim.x * 32) {
-        const long long i = i0 + lane;
+    for (long long i0 = (long long)blockIdx.x * (32 * WIDTH); i0 < all; i0 += (long long)gridDim.x * (32 * WIDTH)) {
+        const long long i = i0 + lane * WIDTH;
         T* to = i < size ? (d_weight ? d_weight + g * size + i : nullptr) : i < all && d_bias ? d_bias + (long long)g * bias + (i - size) : nullptr;
-        float sum = 0.0f;
+        float sum[WIDTH];
+#pragma unroll
+        for (int e = 0; e < WIDTH; ++e) sum[e] = 0.0f;
         if (to) {
+            const float* at = partial + (unit + from) * all + i;
 #pragma unroll 8
-            for (int u = from; u < last; ++u) sum += partial[(unit + u) * all + i];
+            for (int u = from; u < last; ++u, at += all) {
+                if constexpr (WIDTH == 4) {
+                    const float4 v = __ldg(reinterpret_cast<const float4*>(at));
+                    sum[0] += v.x;
+                    sum[1] += v.y;
+                    sum[2] += v.z;
+                    sum[3] += v.w;
+                } else {
+                    sum[0] += __ldg(at);
+                }
+            }
         }
-        part[line][lane] = sum;
+#pragma unroll
+        for (int e = 0; e < WIDTH; ++e) part[line][lane * WIDTH + e] = sum[e];
         __syncthreads();
         if (line == 0 && to) {
-            sum = part[0][lane];
 #pragma unroll
-            for (int w = 1; w < 8; ++w) sum += part[w][lane];
-            *to = from_float<T>(sum);
+            for (int w = 1; w < 8; ++w)
+#pragma unroll
+                for (int e = 0; e < WIDTH; ++e) sum[e] += part[w][lane * WIDTH + e];
+            if constexpr (WIDTH == 4) *reinterpret_cast<uint2*>(to) = make_uint2(pack_pair<T>(sum[0], sum[1]), pack_pair<T>(sum[2], sum[3]));
+            else *to = from_float<T>(sum[0]);
         }
         __syncthreads();
     }
@@ -651,31 +670,6 @@ __global__ void __launch_bounds__(256) finish_kernel(FinishArgs a) {
         static_cast<T*>(a.out)[i] = from_float<T>(both(y).x);
         if (a.slope) a.slope[i] = uint16_t(slope_codes(slope));
     }
-}
-
-// d W from few units: a thread per four elements.
-template <typename T>
-__global__ void __launch_bounds__(256) join_few_kernel(const float* partial, T* d_weight, const int* offsets, long long rows, int chunk,
-                                                       long long size) {
-    const int g = blockIdx.y, lane = threadIdx.x & 31;
-    long long begin, end;
-    int before = 0;
-    for (int i = lane; i < g; i += 32) {
-        group_rows(offsets, i, rows, begin, end);
-        before += int(max(1ll, (end - begin + chunk - 1) / chunk));
-    }
-    const long long unit = __reduce_add_sync(0xffffffffu, before);
-    group_rows(offsets, g, rows, begin, end);
-    const int count = int(max(1ll, (end - begin + chunk - 1) / chunk));
-    const long long i = ((long long)blockIdx.x * 256 + threadIdx.x) * 4;
-    if (i >= size) return;
-    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int u = 0; u < count; ++u) {
-        const float4 v = __ldg(reinterpret_cast<const float4*>(partial + (unit + u) * size + i));
-        sum = make_float4(sum.x + v.x, sum.y + v.y, sum.z + v.z, sum.w + v.w);
-    }
-    *reinterpret_cast<uint2*>(d_weight + g * size + i) = make_uint2(pack_pair<T>(sum.x, sum.y), pack_pair<T>(sum.z, sum.w));
 }
 
 // ---------------------------------------------------------------- dz and the bias gradient
@@ -726,7 +720,7 @@ __global__ void __launch_bounds__(THREADS) dz_kernel(DzArgs a, int lanes_log2) {
 #pragma unroll
     for (int i = 0; i < COLUMNS; ++i) sum[i] = 0.0f;
     if (column < a.n) {
-#pragma unroll 4
+#pragma unroll COLUMNS == 8 ? 4 : 8
         for (long long row = u.from + line; row < u.to; row += lines) {
             const long long at = row * a.n + column;
             if constexpr (COLUMNS == 8) {
@@ -971,19 +965,16 @@ void with_config(Config c, F&& f) {
     else f(std::integral_constant<int, 1>{}, std::integral_constant<int, 64>{});
 }
 
-template <typename T, int MODE, int CG, int BN>
+template <typename T, int MODE, int CG, int BN, bool PARTIAL>
 void launch_gemm(const CUtensorMap& a, const CUtensorMap& b, GemmArgs p, int64_t tiles, cudaStream_t stream) {
     ODIE_REQUIRE(tiles < (int64_t(1) << 30), "too many rows and columns for one launch");
     const int64_t nt = ceil_div(p.n, BN);
     p.by_bands = Divide::by(BAND * nt);
     p.by_columns = Divide::by(nt);
     p.by_tiles = Divide::by(nt * ceil_div(MODE == DW ? p.m : p.rows, 128 * CG));
-    if (MODE != DW && p.splits <= 1) {
-        p.splits = 1;
-        p.chunk = int(ceil_div(p.k, BK));
-    }
+
     using S = Shape<CG, BN>;
-    const auto kernel = gemm_kernel<T, MODE, CG, BN>;
+    const auto kernel = gemm_kernel<T, MODE, CG, BN, PARTIAL>;
     ODIE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes(1024)));
     const int pairs = int(std::min<int64_t>(tiles, sm_count() / CG));
     cudaLaunchConfig_t config{};
@@ -1033,16 +1024,13 @@ void launch_few_rows(const FewArgs& a, cudaStream_t stream) {
 template <typename T>
 void launch_join(const float* partial, void* d_weight, void* d_bias, const int* offsets, int groups, int64_t rows, int64_t chunk,
                  int64_t size, int bias, cudaStream_t stream) {
-    // many elements and few units: 1024 x 1024 of 8 units took 45 us with a warp's share of units per element
-    if (bias == 0 && size % 4 == 0 && uintptr_t(d_weight) % 8 == 0 && size >= 16 * ceil_div(rows, chunk) * 256) {
-        join_few_kernel<T><<<dim3(unsigned(ceil_div(size, 1024)), unsigned(groups)), 256, 0, stream>>>(
-            partial, static_cast<T*>(d_weight), offsets, rows, int(chunk), size);
-        ODIE_CUDA(cudaGetLastError());
-        note_launch();
-        return;
-    }
-    join_kernel<T><<<dim3(unsigned(std::min<int64_t>(ceil_div(size + bias, 32), 4096)), unsigned(groups)), 256, 0, stream>>>(
-        partial, static_cast<T*>(d_weight), static_cast<T*>(d_bias), offsets, rows, int(chunk), size, bias);
+    const bool wide = size % 4 == 0 && bias % 4 == 0 && (uintptr_t(d_weight) | uintptr_t(d_bias)) % 8 == 0;
+    const dim3 grid(unsigned(std::min<int64_t>(ceil_div(size + bias, wide ? 128 : 32), 16384)), unsigned(groups));
+    auto go = [&](auto kernel) {
+        kernel<<<grid, 256, 0, stream>>>(partial, static_cast<T*>(d_weight), static_cast<T*>(d_bias), offsets, rows, int(chunk), size, bias);
+    };
+    if (wide) go(join_kernel<T, 4>);
+    else go(join_kernel<T, 1>);
     ODIE_CUDA(cudaGetLastError());
     note_launch();
 }
@@ -1071,7 +1059,8 @@ struct Splits {
     Splits(int64_t rows, int n, int k, int groups, bool offsets) : parts(1), blocks(int(ceil_div(k, BK))) {
         if (rows == 0 || offsets) return;
         const Config c = tile_config(rows, n, groups, true);
-        const int64_t tiles = ceil_div(rows, 128 * c.cg) * ceil_div(n, c.bn), wanted = std::min<int64_t>(SMS / c.cg / tiles, blocks / 8);
+        if (c.cg != 1) return;
+        const int64_t tiles = ceil_div(rows, 128) * ceil_div(n, c.bn), wanted = std::min<int64_t>(SMS / tiles, blocks / 8);
         if (wanted < 2) return;
         blocks = int(ceil_div(blocks, wanted));
         parts = int(ceil_div(ceil_div(k, BK), blocks));
@@ -1094,9 +1083,13 @@ void launch_product(const void* a, const void* b, int64_t ld_a, int64_t ld_b, in
     p.a_rows = int(std::min<int64_t>(128, round8(p.rows)));
     with_config(tile_config(p.rows, p.n, p.groups, true), [&](auto cg, auto bn) {
         constexpr int CG = decltype(cg)::value, BN = decltype(bn)::value;
-        launch_gemm<T, MODE, CG, BN>(tensor_map(a, bf16, p.k, p.rows, 0, ld_a, p.a_rows),
-                                     tensor_map(b, bf16, inputs, outputs, p.groups, ld_b, MODE == FWD ? BN / CG : 64), p,
-                                     (ceil_div(p.rows, 128 * CG) + p.groups + 1) * ceil_div(p.n, BN) * split.parts, stream);
+        const CUtensorMap map_a = tensor_map(a, bf16, p.k, p.rows, 0, ld_a, p.a_rows);
+        const CUtensorMap map_b = tensor_map(b, bf16, inputs, outputs, p.groups, ld_b, MODE == FWD ? BN / CG : 64);
+        const int64_t tiles = (ceil_div(p.rows, 128 * CG) + p.groups + 1) * ceil_div(p.n, BN) * split.parts;
+        if constexpr (CG == 1) {
+            if (split.parts > 1) return launch_gemm<T, MODE, CG, BN, true>(map_a, map_b, p, tiles, stream);
+        }
+        launch_gemm<T, MODE, CG, BN, false>(map_a, map_b, p, tiles, stream);
     });
     if (split.parts > 1) {
         const FinishArgs f{partial, split.parts, p.rows * p.n, p.n, p.bias, p.residual, p.out, p.slope, p.activation};
@@ -1183,7 +1176,7 @@ struct BackwardScratch {
         bytes = s.used;
         thin = static_cast<float*>(base);  // thin layers need nothing else
         if (thin_sizes(inputs, outputs))
-            bytes = std::max(bytes, aligned(thin_units(rows, groups, thin_chunk(rows, true)) * (int64_t(outputs) * inputs + outputs) * 4));
+            bytes = std::max(bytes, aligned(thin_units(rows, groups, thin_chunk(rows, inputs, outputs, true)) * (int64_t(outputs) * inputs + outputs) * 4));
     }
 };
 
@@ -1222,7 +1215,7 @@ extern "C" int odie_linear(const void* x, const void* weight, const void* bias, 
             a.outputs = outputs;
             a.groups = groups;
             a.offsets = offsets;
-            a.chunk = thin_chunk(rows, false);
+            a.chunk = thin_chunk(rows, inputs, outputs, false);
             a.x = x;
             a.weight = weight;
             a.bias = bias;
@@ -1286,7 +1279,7 @@ extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, cons
             a.outputs = outputs;
             a.groups = groups;
             a.offsets = offsets;
-            a.chunk = thin_chunk(rows, true);
+            a.chunk = thin_chunk(rows, inputs, outputs, true);
             a.x = x;
             a.weight = weight;
             a.d_y = d_y;
@@ -1361,7 +1354,9 @@ extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, cons
                     p.group_maps = static_cast<const CUtensorMap*>(s.maps);
                 }
                 with_config(u.config, [&](auto cg, auto bn) {
-                    launch_gemm<T, DW, decltype(cg)::value, decltype(bn)::value>(a, b, p, u.units * u.tiles, stream);
+                    constexpr int CG = decltype(cg)::value, BN = decltype(bn)::value;
+                    if (u.split) launch_gemm<T, DW, CG, BN, true>(a, b, p, u.units * u.tiles, stream);
+                    else launch_gemm<T, DW, CG, BN, false>(a, b, p, u.units * u.tiles, stream);
                 });
                 if (u.split) {
                     const int64_t size = int64_t(outputs) * inputs;

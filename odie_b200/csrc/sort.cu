@@ -3,7 +3,6 @@
 // every run.
 #include "rows.cuh"
 #include "odie_b200.h"
-#include <type_traits>
 
 namespace odie {
 namespace {
@@ -11,9 +10,11 @@ namespace {
 // A tile of pairs per block of 256 threads.  Warp w holds the tile's pairs [w * 32 R, (w + 1) * 32 R) in R
 // rounds of 32, lane order within a round, so that (warp, round, lane) is the input order.
 constexpr int THREADS = 256, WARPS = THREADS / 32;
-constexpr int ROUNDS = 8, TILE = THREADS * ROUNDS;
-// One block orders up to 4096 pairs by itself, one of 1024 threads up to 16384 (15009 pairs of 37 experts: one launch
-// instead of three); more are cut into tiles of 2048.
+// Up to 128 tiles, every block sums the counts of the tiles before its own itself (32 tiles: 6.5 us with that, 8.8 in
+// two kernels; 512 tiles take the kernel between).
+constexpr int ROUNDS = 8, TILE = THREADS * ROUNDS, FOLD = 128;
+// One block orders up to 4096 pairs by itself, one of 1024 threads up to 16384: one launch
+// instead of two; more are cut into tiles of 2048.
 constexpr int ONE_ROUNDS = 16, ONE_THREADS = 1024, ONE_TILE = ONE_THREADS * ONE_ROUNDS;
 // Digits of up to 10 bits: two passes order 2^20 keys, one pass 1023 experts, and the eight warps' counts fit
 // in 32 KB of shared memory.
@@ -255,10 +256,11 @@ __global__ void __launch_bounds__(1024) tile_starts_kernel(Pass p, int tiles) {
     }
 }
 
+// tiles: their count where the blocks sum the counts of earlier tiles, 0 where tile_starts_kernel did.
 // The tile's pairs are put in digit order in shared memory first, so that neighbouring threads write neighbouring
 // places (2^20 pairs of 16384 ids: 15 us a pass written straight to their places).
 template <int SOURCE>
-__global__ void __launch_bounds__(THREADS) tile_place_kernel(SortArgs a, Pass p) {
+__global__ void __launch_bounds__(THREADS) tile_place_kernel(SortArgs a, Pass p, int tiles) {
     extern __shared__ uint32_t shared[];
     const int digits = 1 << p.bits;
     uint32_t* counts = shared;                  // [WARPS][digits]
@@ -282,16 +284,27 @@ __global__ void __launch_bounds__(THREADS) tile_place_kernel(SortArgs a, Pass p)
     uint32_t running = 0, running_local = 0;
     for (int base = 0; base < digits; base += THREADS) {
         const int d = base + threadIdx.x;
-        uint32_t total, tile_total, c = 0;
+        uint32_t total, tile_total, c = 0, all = 0, earlier = 0;
         if (d < digits) {
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) c += counts[w * digits + d];
+            if (tiles) {
+#pragma unroll 16
+                for (int t = 0; t < tiles; ++t) {
+                    const uint32_t other = p.tiles[(long long)t * digits + d];
+                    all += other;
+                    earlier += t < int(blockIdx.x) ? other : 0;
+                }
+            } else {
+                all = p.totals[d];
+                earlier = p.tiles[(long long)blockIdx.x * digits + d];
+            }
         }
-        const uint32_t before = block_exclusive<WARPS>(d < digits ? p.totals[d] : 0, scan, total);
+        const uint32_t before = block_exclusive<WARPS>(all, scan, total);
         const uint32_t before_local = block_exclusive<WARPS>(c, scan, tile_total);
         if (d < digits) {
             local[d] = running_local + before_local;
-            shift_to[d] = running + before + p.tiles[(long long)blockIdx.x * digits + d] - local[d];
+            shift_to[d] = running + before + earlier - local[d];
             // one pass: the digit is the key
             if (!p.keys_out && SOURCE && a.offsets && blockIdx.x == 0 && d <= a.bins) a.offsets[d] = int(running + before);
         }
@@ -415,13 +428,16 @@ void launch_sort(const SortArgs& a, cudaStream_t stream) {
         const auto counts = i > 0 ? tile_counts_kernel<0> : wide ? tile_counts_kernel<8> : tile_counts_kernel<4>;
         const auto place = i > 0 ? tile_place_kernel<0> : wide ? tile_place_kernel<8> : tile_place_kernel<4>;
         counts<<<tiles, THREADS, size_t(digits) * 4, stream>>>(last, p);
-        tile_starts_kernel<<<(digits + 31) / 32, 1024, 0, stream>>>(p, tiles);
+        if (tiles > FOLD) {
+            tile_starts_kernel<<<(digits + 31) / 32, 1024, 0, stream>>>(p, tiles);
+            note_launch();
+        }
         const size_t bytes = (size_t(WARPS + 2) * digits + 2 * TILE) * 4;
         if (bytes > 48 * 1024)
             ODIE_CUDA(cudaFuncSetAttribute(place, cudaFuncAttributeMaxDynamicSharedMemorySize, ((WARPS + 2) * (1 << MAX_DIGIT_BITS) + 2 * TILE) * 4));
-        place<<<tiles, THREADS, bytes, stream>>>(last, p);
+        place<<<tiles, THREADS, bytes, stream>>>(last, p, tiles > FOLD ? 0 : tiles);
         ODIE_CUDA(cudaGetLastError());
-        note_launch(3);
+        note_launch(2);
     }
     if (passes > 1 && a.offsets) {
         key_offsets_kernel<<<blocks_for(a.bins + 1, THREADS), THREADS, 0, stream>>>(last.sorted, a.n, a.bins, a.offsets);

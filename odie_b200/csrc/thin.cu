@@ -19,7 +19,11 @@ namespace odie {
 namespace {
 
 constexpr int THREADS = 128, WARPS = 4;
-constexpr int FORWARD_STAGES = 4, BACKWARD_STAGES = 3;  // steps of 16 rows per warp, one in work, the others on their way
+// Steps of 16 rows per warp, one in work, the others on their way; two blocks share an SM in the backward pass (three
+// with three stages each took 4 % longer).
+constexpr int FORWARD_STAGES = 4;
+template <int KB, int NB>
+constexpr int STAGES_BACK = KB * NB == 4 ? 3 : 5;
 
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -57,7 +61,7 @@ __device__ __forceinline__ uint4 load_row(const void* base, long long row, int w
 
 // KB, NB: blocks of 32 inputs and outputs.
 template <typename T, int KB, int NB, int ACT>
-__global__ void __launch_bounds__(THREADS, 4) thin_forward_kernel(ThinArgs a) {
+__global__ void __launch_bounds__(THREADS, KB * NB == 4 ? 3 : 4) thin_forward_kernel(ThinArgs a) {
     constexpr int VECTORS = KB * 2 + NB * 2;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
     const Unit u = unit_at<false>(a.offsets, a.groups, a.rows, a.chunk, blockIdx.x);
@@ -163,7 +167,8 @@ __global__ void __launch_bounds__(THREADS, 4) thin_forward_kernel(ThinArgs a) {
 }
 
 template <typename T, int KB, int NB>
-__global__ void __launch_bounds__(THREADS, KB * NB == 4 ? 2 : 3) thin_backward_kernel(ThinArgs a) {
+__global__ void __launch_bounds__(THREADS, 2) thin_backward_kernel(ThinArgs a) {
+    constexpr int BACKWARD_STAGES = STAGES_BACK<KB, NB>;
     constexpr int VECTORS = NB * 4 + KB * 2;
     extern __shared__ uint4 slots[];
     // W by its rows' order for d x: [K-step of 16 outputs][8-column tile of inputs][lane]
@@ -398,7 +403,7 @@ template <typename T>
 void launch_thin_backward(const ThinArgs& a, cudaStream_t stream) {
     with_blocks(a.inputs, a.outputs, [&](auto kb, auto nb) {
         constexpr int KB = decltype(kb)::value, NB = decltype(nb)::value;
-        constexpr int BYTES = WARPS * BACKWARD_STAGES * (NB * 4 + KB * 2) * 512;
+        constexpr int BYTES = WARPS * STAGES_BACK<KB, NB> * (NB * 4 + KB * 2) * 512;
         ODIE_CUDA(cudaFuncSetAttribute(thin_backward_kernel<T, KB, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES));
         thin_backward_kernel<T, KB, NB><<<unsigned(thin_units(a.rows, a.groups, a.chunk)), THREADS, BYTES, stream>>>(a);
     });

@@ -30,10 +30,11 @@ struct ThinArgs {
 };
 
 inline bool thin_sizes(int inputs, int outputs) { return inputs <= 64 && outputs <= 64 && inputs % 8 == 0 && outputs % 8 == 0; }
-// Rows per block: as many blocks as fit the SMs at once (four or three per SM), so that W is read and sums are
-// written as seldom as that allows.
-inline int thin_chunk(int64_t rows, bool backward) {
-    const int64_t blocks = 148 * (backward ? 3 : 4), share = (rows + blocks - 1) / blocks;
+// Rows per block: as many blocks as fit the SMs at once (two per SM backward, four forward, three for more than 32
+// inputs and outputs), so that W is read and sums are written as seldom as that allows.
+inline int thin_blocks(int inputs, int outputs, bool backward) { return backward ? 2 : inputs > 32 && outputs > 32 ? 3 : 4; }
+inline int thin_chunk(int64_t rows, int inputs, int outputs, bool backward) {
+    const int64_t blocks = 148 * thin_blocks(inputs, outputs, backward), share = (rows + blocks - 1) / blocks;
     return int(std::max<int64_t>(64, (share + 63) / 64 * 64));
 }
 // Units of work (blocks) at most: every group has at least one, and rows of no group their own.

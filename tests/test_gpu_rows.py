@@ -21,7 +21,8 @@ def normal(g, *shape, dtype=torch.float32, std=1.0):
 # ---------------------------------------------------------------- order
 SORTS = [(0, 1, 4), (1, 1, 1), (31, 1, 3), (4096, 1, 5), (4097, 1, 5), (257, 3, 64), (1000, 8, 1023), (3000, 2, 1024),
          (20000, 1, 1), (12345, 2, 200), (9000, 1, 70000), (5, 1, 70000), (50000, 1, (1 << 20) + 3),
-         (16384, 1, 511), (16385, 1, 512), (8192, 2, 1 << 19), (4096, 1, 300), (70000, 1, 5)]
+         (16384, 1, 511), (16385, 1, 512), (8192, 2, 1 << 19), (4096, 1, 300), (70000, 1, 5), (262144, 1, 700),
+         (262145, 1, 40), (300001, 1, 1500), (1100000, 1, 16)]
 
 
 @pytest.mark.parametrize('rows, choices, bins', SORTS)
