@@ -4,6 +4,7 @@ The library is the product's compute path: every CUDA kernel plus the C-ABI
 declared in include/odie_b200.h.  It is built next to this file so that it
 travels with the repository snapshot; nothing is installed elsewhere.
 """
+from concurrent.futures import ThreadPoolExecutor
 import os
 import subprocess
 import sys
@@ -70,15 +71,17 @@ def build(force=False, verbose=False):
 def build_library(verbose=False):
     build_dir = PACKAGE / '_build'
     build_dir.mkdir(exist_ok=True)
-    objects = []
     include = ['-I', str(PACKAGE / 'csrc'), '-I', str(ROOT / 'include')]
-    for source in SOURCES:
+
+    def compile_source(source):
         obj = build_dir / (Path(source).stem + '.o')
         command = [nvcc(), *FLAGS, *ARCH, *include, '-c', str(PACKAGE / 'csrc' / source), '-o', str(obj)]
         if verbose:
             print(' '.join(command), file=sys.stderr)
         subprocess.run(command, check=True)
-        objects.append(str(obj))
+        return str(obj)
+    with ThreadPoolExecutor(min(8, os.cpu_count() or 1)) as pool:  # each source is an nvcc of its own
+        objects = list(pool.map(compile_source, SOURCES))
     tmp = LIBRARY.with_suffix('.so.tmp')
     subprocess.run([nvcc(), '-shared', *ARCH, *objects, '-o', str(tmp), '-lcudart'], check=True)
     os.replace(tmp, LIBRARY)

@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(ROW_THREADS) combine_backward_kernel(RowArgs a
 
 // The same for wide rows with several choices, walking the unsorted rows: d out is read once for up to four choices.
 template <typename T, int BYTES>
-__global__ void __launch_bounds__(ROW_THREADS) combine_backward_rows_kernel(RowArgs a, const T* __restrict__ d_out,
+__global__ void __launch_bounds__(ROW_THREADS, 3) combine_backward_rows_kernel(RowArgs a, const T* __restrict__ d_out,
                                                                             const T* __restrict__ sorted, T* __restrict__ d_sorted,
                                                                             float* __restrict__ d_weights) {
     using P = Pack<T, BYTES>;
@@ -308,9 +308,9 @@ void check_rows(int64_t n, int choices, int64_t width, int dtype, const int32_t*
 RowArgs sorted_args(int64_t n, int choices, int64_t width, int dtype, int vector, const int32_t* order, const int32_t* slot,
                     const float* weights) {
     const int64_t vectors = width * row_type_size(dtype) / vector;
-    RowArgs a{row_shape(n * choices, vectors), n * choices, choices, width, order, nullptr, weights};
+    RowArgs a{row_shape(n * choices, vectors, vector), n * choices, choices, width, order, nullptr, weights};
     if (!a.shape.narrow && choices > 1) {
-        a.shape = row_shape(n, vectors);
+        a.shape = row_shape(n, vectors, vector);
         a.order = nullptr;
         a.slot = slot;
     }
@@ -365,7 +365,7 @@ extern "C" int odie_combine(const void* sorted, int64_t n, int choices, int64_t 
         if (n == 0) return;
         ODIE_REQUIRE(sorted && out, "sorted and out are required");
         const int vector = row_vector(width, dtype, sorted, out);
-        const RowArgs a{row_shape(n, width * row_type_size(dtype) / vector), n * choices, choices, width, nullptr, slot, weights};
+        const RowArgs a{row_shape(n, width * row_type_size(dtype) / vector, vector), n * choices, choices, width, nullptr, slot, weights};
         with_rows(dtype, vector, a.shape.narrow, [&](auto type, auto bytes, auto narrow) {
             using T = decltype(type);
             auto go = [&](auto batch) {

@@ -212,7 +212,7 @@ extern "C" int odie_embed(const void* ids, int id_bytes, int64_t n, const void* 
         if (n == 0) return;
         ODIE_REQUIRE(ids && table && out, "ids, table and out are required");
         const int vector = row_vector(width, dtype, table, out);
-        const EmbedArgs a{row_shape(n, width * row_type_size(dtype) / vector), ids, id_bytes, rows, width, scale};
+        const EmbedArgs a{row_shape(n, width * row_type_size(dtype) / vector, vector), ids, id_bytes, rows, width, scale};
         with_row_type(dtype, vector, [&](auto type, auto bytes) {
             using T = decltype(type);
             constexpr int B = decltype(bytes)::value;

@@ -96,13 +96,14 @@ struct RowShape {
     int lanes_log2;
     bool narrow;
 };
-inline RowShape row_shape(int64_t rows, int64_t vectors) {
+inline RowShape row_shape(int64_t rows, int64_t vectors, int bytes) {
+    const int most = bytes == 16 ? 4 : 16;  // vectors per thread of a wide row: 64 bytes
     RowShape s{rows, vectors, 0, vectors <= 32};
     if (s.narrow) {
         while ((1 << s.lanes_log2) < vectors) ++s.lanes_log2;
     } else {
         s.lanes_log2 = 5;
-        while (s.lanes_log2 < 8 && (int64_t(4) << s.lanes_log2) < vectors) ++s.lanes_log2;
+        while (s.lanes_log2 < 8 && (int64_t(most) << s.lanes_log2) < vectors) ++s.lanes_log2;
     }
     return s;
 }
