@@ -408,7 +408,9 @@ ODIE_API int odie_combine_backward(const void* d_out, const void* sorted, int64_
  * the rows' type for the products: d_x = dz W, d_weight = dz^T x, d_bias =
  * sum of the unrounded dz over the group's rows and d_residual = d_y (each may
  * be NULL); zero for rows behind the last group and for empty groups.
- * x, weight, d_y and scratch start on 16-byte boundaries.
+ * x, weight and d_y start on 16-byte boundaries, scratch on a 256-byte one.
+ * Offsets that run backwards or out of range are cut to the rows: nothing out
+ * of bounds is read or written, and the results are not defined.
  * ------------------------------------------------------------------------ */
 ODIE_API int64_t odie_linear_scratch(int64_t rows, int inputs, int outputs, int groups);
 ODIE_API int odie_linear(const void* x, const void* weight, const void* bias, const void* residual, int64_t rows, int inputs,

@@ -62,6 +62,7 @@ struct GemmArgs {
     int k;               // FWD, DX: length of the sum
     int a_rows;          // FWD, DX: rows of A's boxes, 128 or, for fewer rows in all, those (rounded up to 8)
     int chunk;           // DW: rows per unit of work (a multiple of BK); FWD, DX: blocks of K per split
+    int units;           // DW: partial sums there is room for (offsets that run backwards would make more)
     int splits;          // FWD, DX without offsets: the sum over K cut among this many tiles, joined by finish_kernel
     Divide by_bands;     // FWD, DX: tiles of a full band
     Divide by_tiles, by_columns;  // tiles of d W (DW) or of C (splits), and of one row of them
@@ -490,7 +491,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
                     if (lane == 0) tc::bar_arrive_cluster(CG == 2 ? tc::leader_address(drained + acc) : tc::smem_u32(drained + acc));
                 }
                 if (PARTIAL) {
-                    if (lane < w.rows) {
+                    if (lane < w.rows && (MODE != DW || tile.unit < p.units)) {
                         float* to = p.partial + ((long long)tile.unit * p.m + row + lane) * p.n + column0 + j * STRIDE;
                         if (p.n % 4 == 0) {
 #pragma unroll
@@ -592,7 +593,7 @@ __global__ void __launch_bounds__(32) group_maps_kernel(const __grid_constant__ 
 // unwanted: null).
 template <typename T, int WIDTH>
 __global__ void __launch_bounds__(256) join_kernel(const float* partial, T* d_weight, T* d_bias, const int* offsets, long long rows,
-                                                   int chunk, long long size, int bias) {
+                                                   int chunk, long long units, long long size, int bias) {
     __shared__ float part[8][32 * WIDTH + 1];
     const int g = blockIdx.y, lane = threadIdx.x & 31, line = threadIdx.x >> 5;
     long long begin, end;
@@ -603,7 +604,8 @@ __global__ void __launch_bounds__(256) join_kernel(const float* partial, T* d_we
     }
     const long long unit = __reduce_add_sync(0xffffffffu, before);
     group_rows(offsets, g, rows, begin, end);
-    const int count = int(max(1ll, (end - begin + chunk - 1) / chunk)), share = (count + 7) / 8;
+    // no more than were written: offsets that run backwards would make more
+    const int count = int(max(0ll, min(units - unit, max(1ll, (end - begin + chunk - 1) / chunk)))), share = (count + 7) / 8;
     const int from = min(count, line * share), last = min(count, from + share);
     const long long all = size + bias;
     for (long long i0 = (long long)blockIdx.x * (32 * WIDTH); i0 < all; i0 += (long long)gridDim.x * (32 * WIDTH)) {
@@ -1023,11 +1025,11 @@ void launch_few_rows(const FewArgs& a, cudaStream_t stream) {
 
 template <typename T>
 void launch_join(const float* partial, void* d_weight, void* d_bias, const int* offsets, int groups, int64_t rows, int64_t chunk,
-                 int64_t size, int bias, cudaStream_t stream) {
+                 int64_t units, int64_t size, int bias, cudaStream_t stream) {
     const bool wide = size % 4 == 0 && bias % 4 == 0 && (uintptr_t(d_weight) | uintptr_t(d_bias)) % 8 == 0;
     const dim3 grid(unsigned(std::min<int64_t>(ceil_div(size + bias, wide ? 128 : 32), 16384)), unsigned(groups));
     auto go = [&](auto kernel) {
-        kernel<<<grid, 256, 0, stream>>>(partial, static_cast<T*>(d_weight), static_cast<T*>(d_bias), offsets, rows, int(chunk), size, bias);
+        kernel<<<grid, 256, 0, stream>>>(partial, static_cast<T*>(d_weight), static_cast<T*>(d_bias), offsets, rows, int(chunk), units, size, bias);
     };
     if (wide) go(join_kernel<T, 4>);
     else go(join_kernel<T, 1>);
@@ -1128,6 +1130,11 @@ struct WeightUnits {
         chunk = std::max<int64_t>(BK, ceil_div(rows, BK) * BK);
         split = have < wanted / 2 && rows > 32 * BK;  // a second kernel joins the sums: 2048 rows are walked sooner
         if (split) chunk = std::max<int64_t>(8 * BK, ceil_div(ceil_div(rows * tiles, wanted), BK) * BK);
+        // a unit is at most 2^20 rows: its sum (7 ms) ends well before the epilogue's wait for it would give up
+        if (rows > (1 << 20)) {
+            split = true;
+            chunk = std::min<int64_t>(chunk, 1 << 20);
+        }
         units = split ? ceil_div(rows, chunk) + groups : groups;  // at most
     }
 };
@@ -1227,7 +1234,7 @@ extern "C" int odie_linear(const void* x, const void* weight, const void* bias, 
             return;
         }
         const ForwardScratch s(scratch, rows, inputs, outputs, groups);
-        ODIE_REQUIRE(scratch || s.bytes == 0, "scratch is required");
+        ODIE_REQUIRE(s.bytes == 0 || (scratch && uintptr_t(scratch) % 256 == 0), "scratch is required, on a 256-byte boundary");
         const int64_t ld = round8(inputs);
         if (s.x) {
             launch_pad(x, s.x, rows, weight, s.weight, int64_t(groups) * outputs, inputs, stream);
@@ -1270,6 +1277,7 @@ extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, cons
             return;
         }
         ODIE_REQUIRE(d_y && (x || !d_weight) && (weight || !d_x) && scratch, "d_y, x, weight and scratch are required");
+        ODIE_REQUIRE(uintptr_t(scratch) % 256 == 0, "scratch must start on a 256-byte boundary");
         ODIE_REQUIRE(!slope || !relu_y, "slope and relu_y exclude each other");
         const BackwardScratch s(scratch, rows, inputs, outputs, groups);
         if (thin_sizes(inputs, outputs) && on_16_bytes({d_y, slope, relu_y, x, weight, d_x, d_residual})) {
@@ -1295,7 +1303,8 @@ extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, cons
                 using T = decltype(type);
                 launch_thin_backward<T>(a, stream);
                 if (join)
-                    launch_join<T>(s.thin, d_weight, d_bias, offsets, groups, rows, a.chunk, int64_t(outputs) * inputs, outputs, stream);
+                    launch_join<T>(s.thin, d_weight, d_bias, offsets, groups, rows, a.chunk, thin_units(rows, groups, a.chunk),
+                                   int64_t(outputs) * inputs, outputs, stream);
             });
             return;
         }
@@ -1323,7 +1332,7 @@ extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, cons
                 a.groups = groups;
                 a.offsets = offsets;
                 launch_dz<T>(a, stream);
-                if (join) launch_join<T>(s.bias, nullptr, d_bias, offsets, groups, rows, a.chunk, 0, outputs, stream);
+                if (join) launch_join<T>(s.bias, nullptr, d_bias, offsets, groups, rows, a.chunk, dz_units(rows, groups), 0, outputs, stream);
             }
             if (s.x && products)
                 launch_pad(x, s.x, d_weight ? rows : 0, weight, s.weight, d_x ? int64_t(groups) * outputs : 0, inputs, stream);
@@ -1345,6 +1354,7 @@ extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, cons
                 const CUtensorMap b = tensor_map(s.x ? s.x : x, bf16, inputs, rows, 0, ld_x, 64);
                 p.m = outputs;
                 p.chunk = int(u.chunk);
+                p.units = int(u.units);
                 p.out = d_weight;
                 p.partial = u.split ? s.partial : nullptr;
                 if (offsets) {
@@ -1360,7 +1370,7 @@ extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, cons
                 });
                 if (u.split) {
                     const int64_t size = int64_t(outputs) * inputs;
-                    launch_join<T>(s.partial, d_weight, nullptr, offsets, groups, rows, u.chunk, int64_t(outputs) * inputs, 0, stream);
+                    launch_join<T>(s.partial, d_weight, nullptr, offsets, groups, rows, u.chunk, u.units, int64_t(outputs) * inputs, 0, stream);
                 }
             }
         });

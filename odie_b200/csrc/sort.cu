@@ -13,20 +13,20 @@ constexpr int THREADS = 256, WARPS = THREADS / 32;
 // Up to 128 tiles, every block sums the counts of the tiles before its own itself (32 tiles: 6.5 us with that, 8.8 in
 // two kernels; 512 tiles take the kernel between).
 constexpr int ROUNDS = 8, TILE = THREADS * ROUNDS, FOLD = 128;
-// One block orders up to 4096 pairs by itself, one of 1024 threads up to 16384: one launch
-// instead of two; more are cut into tiles of 2048.
-constexpr int ONE_ROUNDS = 16, ONE_THREADS = 1024, ONE_TILE = ONE_THREADS * ONE_ROUNDS;
+// One block orders up to 4096 pairs by itself; more are cut into tiles of 2048.  (A block of 1024 threads for up to 16384
+// saved a launch and took 19 us where two kernels take 9.)
+constexpr int ONE_ROUNDS = 16, ONE_TILE = THREADS * ONE_ROUNDS;
 // Digits of up to 10 bits: two passes order 2^20 keys, one pass 1023 experts, and the eight warps' counts fit
 // in 32 KB of shared memory.
-constexpr int MAX_DIGIT_BITS = 10, ONE_DIGIT_BITS = 9;  // 32 warps' counts beside 16384 pairs: 9 bits
+constexpr int MAX_DIGIT_BITS = 10;
 
 int key_bits(int bins) {  // keys 0..bins
     int bits = 1;
     while ((int64_t(1) << bits) <= bins) ++bits;
     return bits;
 }
-int pass_count(int bins, int most) { return (key_bits(bins) + most - 1) / most; }
-int digit_bits(int bins, int most) { return (key_bits(bins) + pass_count(bins, most) - 1) / pass_count(bins, most); }
+int pass_count(int bins) { return (key_bits(bins) + MAX_DIGIT_BITS - 1) / MAX_DIGIT_BITS; }
+int digit_bits(int bins) { return (key_bits(bins) + pass_count(bins) - 1) / pass_count(bins); }
 
 // SOURCE: where a pass finds its pairs: 4 or 8, the caller's int32 or int64 keys, or 0, the pairs of the pass before.
 template <int SOURCE>
@@ -43,7 +43,6 @@ __device__ __forceinline__ uint32_t read_key(const void* keys, long long i, uint
 }
 
 // Exclusive sum over the block's threads; total gets the sum of all.  scratch: WARPS words of shared memory.
-template <int WARPS>
 __device__ __forceinline__ uint32_t block_exclusive(uint32_t v, uint32_t* scratch, uint32_t& total) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     uint32_t sum = v;
@@ -79,11 +78,11 @@ __device__ __forceinline__ uint32_t digit_peers(uint32_t d, bool on, int bits) {
 
 // Ranks of the tile's pairs among those with the same digit in their own warp, in input order; the warps' digit
 // counts are left in counts[warp][digits].
-template <int WARPS, int R>
+template <int R>
 __device__ __forceinline__ void warp_ranks(const uint32_t (&key)[R], int rounds, int live, int shift, int bits, uint32_t* counts,
                                            uint32_t (&rank)[R]) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, digits = 1 << bits;
-    for (int i = threadIdx.x; i < WARPS * digits; i += WARPS * 32) counts[i] = 0;
+    for (int i = threadIdx.x; i < WARPS * digits; i += THREADS) counts[i] = 0;
     __syncthreads();
     uint32_t* mine = counts + warp * digits;
 #pragma unroll
@@ -102,9 +101,8 @@ __device__ __forceinline__ void warp_ranks(const uint32_t (&key)[R], int rounds,
 }
 
 // counts[warp][digit] becomes first[digit] + the pairs of that digit in earlier warps.
-template <int WARPS>
 __device__ __forceinline__ void warp_starts(uint32_t* counts, int digits, const uint32_t* first) {
-    for (int d = threadIdx.x; d < digits; d += WARPS * 32) {
+    for (int d = threadIdx.x; d < digits; d += THREADS) {
         uint32_t at = first[d];
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
@@ -117,15 +115,14 @@ __device__ __forceinline__ void warp_starts(uint32_t* counts, int digits, const 
 }
 
 // All of it in one block, for at most one tile: a step's few rows cost one launch.
-template <int SOURCE, int THREADS>
+template <int SOURCE>
 __global__ void __launch_bounds__(THREADS) sort_tile_kernel(SortArgs a, int passes, int bits) {
-    constexpr int WARPS = THREADS / 32, TILE = THREADS * ONE_ROUNDS;
     extern __shared__ uint32_t shared[];
     const int digits = 1 << bits, n = int(a.n);
     uint32_t* counts = shared;                    // [WARPS][digits]
     uint32_t* first = counts + WARPS * digits;    // [digits]
-    uint32_t* index = first + digits;             // [TILE]
-    uint32_t* keys = index + TILE;                // [TILE], of several passes or where they are wanted
+    uint32_t* index = first + digits;             // [ONE_TILE]
+    uint32_t* keys = index + ONE_TILE;            // [ONE_TILE], of several passes or where they are wanted
     const bool keep_keys = passes > 1 || a.sorted;
     __shared__ uint32_t scan[WARPS];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -138,21 +135,21 @@ __global__ void __launch_bounds__(THREADS) sort_tile_kernel(SortArgs a, int pass
         id[r] = uint32_t(i);
     }
     for (int p = 0; p < passes; ++p) {
-        warp_ranks<WARPS>(key, rounds, n, p * bits, bits, counts, rank);
+        warp_ranks(key, rounds, n, p * bits, bits, counts, rank);
         uint32_t running = 0;
         for (int base = 0; base < digits; base += THREADS) {
             const int d = base + threadIdx.x;
             uint32_t c = 0, total;
             if (d < digits)
                 for (int w = 0; w < WARPS; ++w) c += counts[w * digits + d];
-            const uint32_t before = block_exclusive<WARPS>(c, scan, total);
+            const uint32_t before = block_exclusive(c, scan, total);
             if (d < digits) first[d] = running + before;
             running += total;
         }
         __syncthreads();
         if (passes == 1 && a.offsets)
             for (int d = threadIdx.x; d <= a.bins; d += THREADS) a.offsets[d] = int(first[d]);
-        warp_starts<WARPS>(counts, digits, first);
+        warp_starts(counts, digits, first);
         const bool last = p + 1 == passes;
 #pragma unroll
         for (int r = 0; r < ONE_ROUNDS; ++r) {
@@ -177,7 +174,7 @@ __global__ void __launch_bounds__(THREADS) sort_tile_kernel(SortArgs a, int pass
         }
         __syncthreads();
     }
-    // out through shared memory: written at their places, they took 16 of 21 us for 15009 pairs
+    // out through shared memory, in order
     for (int i = threadIdx.x; i < n; i += THREADS) {
         a.order[i] = int(index[i]);
         if (a.sorted) a.sorted[i] = keys[i];
@@ -280,7 +277,7 @@ __global__ void __launch_bounds__(THREADS) tile_place_kernel(SortArgs a, Pass p,
         key[r] = read_key<SOURCE>(p.keys, at, uint32_t(a.bins));
         id[r] = SOURCE ? uint32_t(at) : __ldg(p.index + at);
     }
-    warp_ranks<WARPS>(key, ROUNDS, live, p.shift, p.bits, counts, rank);
+    warp_ranks(key, ROUNDS, live, p.shift, p.bits, counts, rank);
     uint32_t running = 0, running_local = 0;
     for (int base = 0; base < digits; base += THREADS) {
         const int d = base + threadIdx.x;
@@ -300,8 +297,8 @@ __global__ void __launch_bounds__(THREADS) tile_place_kernel(SortArgs a, Pass p,
                 earlier = p.tiles[(long long)blockIdx.x * digits + d];
             }
         }
-        const uint32_t before = block_exclusive<WARPS>(all, scan, total);
-        const uint32_t before_local = block_exclusive<WARPS>(c, scan, tile_total);
+        const uint32_t before = block_exclusive(all, scan, total);
+        const uint32_t before_local = block_exclusive(c, scan, tile_total);
         if (d < digits) {
             local[d] = running_local + before_local;
             shift_to[d] = running + before + earlier - local[d];
@@ -312,7 +309,7 @@ __global__ void __launch_bounds__(THREADS) tile_place_kernel(SortArgs a, Pass p,
         running_local += tile_total;
     }
     __syncthreads();
-    warp_starts<WARPS>(counts, digits, local);
+    warp_starts(counts, digits, local);
     const bool last = !p.keys_out;
 #pragma unroll
     for (int r = 0; r < ROUNDS; ++r) {
@@ -366,8 +363,8 @@ int64_t padded(int64_t words) { return (words + 63) / 64 * 64; }
 
 int64_t sort_scratch_bytes(int64_t n, int bins) {
     if (n <= ONE_TILE) return 0;
-    const int64_t digits = int64_t(1) << digit_bits(bins, MAX_DIGIT_BITS), tiles = (n + TILE - 1) / TILE;
-    const int passes = pass_count(bins, MAX_DIGIT_BITS);
+    const int64_t digits = int64_t(1) << digit_bits(bins), tiles = (n + TILE - 1) / TILE;
+    const int passes = pass_count(bins);
     // tile counts, totals, and for more than one pass two pair buffers and the sorted keys
     int64_t words = padded(tiles * digits) + padded(digits);
     if (passes > 1) words += (passes > 2 ? 4 : 2) * padded(n) + padded(n);
@@ -386,23 +383,19 @@ void launch_sort(const SortArgs& a, cudaStream_t stream) {
         }
         return;
     }
+    const int passes = pass_count(a.bins), bits = digit_bits(a.bins), digits = 1 << bits;
+    const bool wide = a.key_bytes == 8;
     if (a.n <= ONE_TILE) {
-        const int passes = pass_count(a.bins, ONE_DIGIT_BITS), bits = digit_bits(a.bins, ONE_DIGIT_BITS);
-        const bool small = a.n <= THREADS * ONE_ROUNDS;
-        const int threads = small ? THREADS : ONE_THREADS;
-        const size_t bytes = (size_t(threads / 32 + 1) * (size_t(1) << bits) + (passes > 1 || a.sorted ? 2 : 1) * threads * ONE_ROUNDS) * 4;
-        const bool wide = a.key_bytes == 8;
-        const auto kernel = small ? (wide ? sort_tile_kernel<8, THREADS> : sort_tile_kernel<4, THREADS>)
-                                  : (wide ? sort_tile_kernel<8, ONE_THREADS> : sort_tile_kernel<4, ONE_THREADS>);
+        const size_t bytes = (size_t(WARPS + 1) * digits + (passes > 1 || a.sorted ? 2 : 1) * ONE_TILE) * 4;
+        const auto kernel = wide ? sort_tile_kernel<8> : sort_tile_kernel<4>;
         if (bytes > 48 * 1024)
             ODIE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           ((threads / 32 + 1) * (1 << ONE_DIGIT_BITS) + 2 * threads * ONE_ROUNDS) * 4));
-        kernel<<<1, threads, bytes, stream>>>(a, passes, bits);
+                                           ((WARPS + 1) * (1 << MAX_DIGIT_BITS) + 2 * ONE_TILE) * 4));
+        kernel<<<1, THREADS, bytes, stream>>>(a, passes, bits);
         ODIE_CUDA(cudaGetLastError());
         note_launch();
         return;
     }
-    const int passes = pass_count(a.bins, MAX_DIGIT_BITS), bits = digit_bits(a.bins, MAX_DIGIT_BITS), digits = 1 << bits;
     ODIE_REQUIRE(a.scratch, "scratch is missing");
     const int tiles = int((a.n + TILE - 1) / TILE);
     uint32_t* at = static_cast<uint32_t*>(a.scratch);
@@ -424,7 +417,6 @@ void launch_sort(const SortArgs& a, cudaStream_t stream) {
         p.keys_out = i + 1 < passes ? buffers[i % 2][0] : nullptr;
         p.index_out = i + 1 < passes ? buffers[i % 2][1] : nullptr;
         p.shift = i * bits;
-        const bool wide = a.key_bytes == 8;
         const auto counts = i > 0 ? tile_counts_kernel<0> : wide ? tile_counts_kernel<8> : tile_counts_kernel<4>;
         const auto place = i > 0 ? tile_place_kernel<0> : wide ? tile_place_kernel<8> : tile_place_kernel<4>;
         counts<<<tiles, THREADS, size_t(digits) * 4, stream>>>(last, p);

@@ -68,7 +68,7 @@ std::tuple<Tensor, Tensor, Tensor> sort_rows(const Tensor& expert, int64_t bins)
     TORCH_CHECK_VALUE(expert.dim() == 1 || (expert.dim() == 2 && expert.size(1) > 0), "expert must have the shape [rows] or [rows, choices]");
     TORCH_CHECK_VALUE(bins >= 1 && bins < (int64_t(1) << 30), "bins must be 1 to 2^30 - 1");
     const int64_t rows = expert.size(0), choices = expert.dim() == 1 ? 1 : expert.size(1), n = rows * choices;
-    TORCH_CHECK_VALUE(n < (int64_t(1) << 31) - (1 << 14), "too many (row, choice) pairs");
+    TORCH_CHECK_VALUE(n < (int64_t(1) << 31) - 4096, "too many (row, choice) pairs");
     const c10::cuda::CUDAGuard guard(expert.device());
     const Tensor keys = expert.contiguous();
     const auto options = expert.options().dtype(at::kInt);
@@ -339,7 +339,7 @@ Tensor embed(const Tensor& ids, const Tensor& table, double scale) {
     check_ids(ids, "ids");
     check_rows(table, "table");
     TORCH_CHECK_VALUE(table.size(0) >= 1 && table.size(0) < (int64_t(1) << 30), "the table must have 1 to 2^30 - 1 rows");
-    TORCH_CHECK_VALUE(ids.numel() < (int64_t(1) << 31) - (1 << 14), "too many ids");
+    TORCH_CHECK_VALUE(ids.numel() < (int64_t(1) << 31) - 4096, "too many ids");
     check_device(ids, table, "ids");
     const Tensor flat = ids.contiguous(), rows = table.contiguous();
     const Tensor out = at::GradMode::is_enabled() && wants(rows) ? Embed::apply(flat, rows, scale) : embedded(flat, rows, scale);

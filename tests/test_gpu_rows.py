@@ -207,14 +207,15 @@ def test_linear_groups(cuda, sizes, inputs, outputs, dtype, activation, tail):
     check_linear(case, activation, edges, offsets)
 
 
+@pytest.mark.parametrize('inputs, outputs', [(72, 136), (32, 64), (33, 70)])
 @pytest.mark.parametrize('poison', [float('nan'), float('inf')])
-def test_linear_groups_keep_apart(cuda, poison):
+def test_linear_groups_keep_apart(cuda, poison, inputs, outputs):
     """NaN or infinity in one group's rows and weights, or behind the last group, reaches nothing of the others."""
     from odie_b200.experts import linear
     g = generator(5)
     sizes = [70, 50, 0, 90]
     offsets = torch.tensor([0] + sizes, device=cuda).cumsum(0).to(torch.int32)
-    rows, inputs, outputs = sum(sizes) + 11, 72, 136
+    rows = sum(sizes) + 11
     x, w, b = normal(g, rows, inputs).half(), normal(g, 4, outputs, inputs, std=0.1).half(), normal(g, 4, outputs).half()
     d_y = normal(g, rows, outputs).half()
     clean = [t.clone() for t in (x, w, b, d_y)]
@@ -357,6 +358,26 @@ def test_linear_offsets_out_of_range_stay_inside(cuda):
     assert torch.equal(got, linear(x, w, offsets=torch.tensor([0, 60, 100], dtype=torch.int32, device=cuda)))
     got = linear(x, w, offsets=torch.tensor([-5, -3, 40], dtype=torch.int32, device=cuda))
     assert torch.equal(got, linear(x, w, offsets=torch.tensor([0, 0, 40], dtype=torch.int32, device=cuda)))
+
+
+@pytest.mark.parametrize('inputs, outputs', [(64, 64), (136, 72)])
+def test_linear_offsets_running_backwards_stay_inside(cuda, inputs, outputs):
+    """Offsets that run backwards make groups overlap, and more units of work than there is room for: what the results
+    are is open, but the gradients' neighbours in memory keep their values and later calls work."""
+    from odie_b200.experts import linear
+    g = generator(6)
+    rows = 6000
+    x, w, b = (normal(g, *s).half().requires_grad_() for s in ((rows, inputs), (6, outputs, inputs), (6, outputs)))
+    d = normal(g, rows, outputs).half()
+    good = torch.arange(0, 7, dtype=torch.int32, device=cuda) * 1000
+    bad = torch.tensor([0, 6000, 0, 6000, 10, 5990, 0], dtype=torch.int32, device=cuda)
+    want = torch.autograd.grad(linear(x, w, b, activation='silu', offsets=good), [x, w, b], d)
+    guards = [torch.full((1 << 20,), 7.0, device=cuda) for _ in range(8)]
+    torch.autograd.grad(linear(x, w, b, activation='silu', offsets=bad), [x, w, b], d)
+    torch.cuda.synchronize()
+    assert all((t == 7.0).all() for t in guards)
+    again = torch.autograd.grad(linear(x, w, b, activation='silu', offsets=good), [x, w, b], d)
+    assert all(torch.equal(a, e) for a, e in zip(want, again))
 
 
 # ---------------------------------------------------------------- embed

@@ -30,7 +30,7 @@ def test_cpu_tensors_are_refused():
 
 
 # Non-null pointers that nothing reads: every call below fails its checks before it touches them.
-SOME = ctypes.c_void_p(16)
+SOME = ctypes.c_void_p(256)
 
 
 @pytest.mark.parametrize('change, message', [
@@ -85,7 +85,8 @@ def test_linear_refuses(lib, change, message):
     assert message in _lib.error()
 
 
-@pytest.mark.parametrize('change, message', LINEAR + [(dict(d_y=None), 'required'), (dict(slope=SOME, relu_y=SOME), 'exclude')])
+@pytest.mark.parametrize('change, message', LINEAR + [(dict(d_y=None), 'required'), (dict(slope=SOME, relu_y=SOME), 'exclude'),
+                                                      (dict(scratch=ctypes.c_void_p(16)), '256-byte')])
 def test_linear_backward_refuses(lib, change, message):
     a = dict(d_y=SOME, slope=None, relu_y=None, x=SOME, weight=SOME, rows=8, inputs=8, outputs=8, groups=1, offsets=None, dtype=0,
              d_x=SOME, d_weight=SOME, d_bias=None, d_residual=None, scratch=SOME, stream=0)
@@ -118,7 +119,7 @@ def test_embed_backward_refuses(lib, change, message):
 
 
 def test_scratch_sizes_are_bounded_and_grow(lib):
-    assert lib.odie_sort_rows_scratch(16384, 1 << 20) == 0  # one block
-    assert 0 < lib.odie_sort_rows_scratch(16385, 16) < lib.odie_sort_rows_scratch(1 << 20, 16) <= 4 * (1 << 20)
+    assert lib.odie_sort_rows_scratch(4096, 1 << 20) == 0  # one block
+    assert 0 < lib.odie_sort_rows_scratch(4097, 16) < lib.odie_sort_rows_scratch(1 << 20, 16) <= 4 * (1 << 20)
     assert lib.odie_sort_rows_scratch(1 << 20, 1 << 16) >= 3 * 4 * (1 << 20)  # a pair buffer and the sorted keys
     assert lib.odie_embed_backward_scratch(1 << 16, 1 << 16, 1024) > lib.odie_embed_backward_scratch(1 << 16, 1 << 16, 32)
