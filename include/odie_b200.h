@@ -401,10 +401,12 @@ ODIE_API int odie_combine_backward(const void* d_out, const void* sorted, int64_
  * the device (NULL for one group of all rows; offsets[0] is taken as 0):
  * group g is rows [offsets[g], offsets[g + 1]); rows behind the last group
  * give zero rows.  activation: 0 none, 1 ReLU, 2 SiLU, 3 GELU (erf).  slope
- * (may be NULL) u16[rows][outputs]: act'(x W^T + b) for the backward pass, as
+ * (may be NULL): act'(x W^T + b) for the backward pass; ReLU: one bit per
+ * output, u8[rows][ceil(outputs / 8)], bit c % 8 of byte c / 8 for column c,
+ * set unless the fp32 sum is <= 0; SiLU and GELU: u16[rows][outputs],
  * round(2^15 (act' + 1/4)), 65535 for NaN.
- * odie_linear_backward: with dz = d_y act' (slope NULL: act' = 1; or, for a
- * ReLU without residual, relu_y = its y, whose sign is act'), rounded to
+ * odie_linear_backward: with dz = d_y act' (slope as odie_linear wrote it for
+ * the same activation; not read for activation 0), rounded to
  * the rows' type for the products: d_x = dz W, d_weight = dz^T x, d_bias =
  * sum of the unrounded dz over the group's rows and d_residual = d_y (each may
  * be NULL); zero for rows behind the last group and for empty groups.
@@ -414,10 +416,10 @@ ODIE_API int odie_combine_backward(const void* d_out, const void* sorted, int64_
  * ------------------------------------------------------------------------ */
 ODIE_API int64_t odie_linear_scratch(int64_t rows, int inputs, int outputs, int groups);
 ODIE_API int odie_linear(const void* x, const void* weight, const void* bias, const void* residual, int64_t rows, int inputs,
-                   int outputs, int groups, const int32_t* offsets, int dtype, int activation, void* y, uint16_t* slope,
+                   int outputs, int groups, const int32_t* offsets, int dtype, int activation, void* y, void* slope,
                    void* scratch, uint64_t stream);
 ODIE_API int64_t odie_linear_backward_scratch(int64_t rows, int inputs, int outputs, int groups);
-ODIE_API int odie_linear_backward(const void* d_y, const uint16_t* slope, const void* relu_y, const void* x, const void* weight,
+ODIE_API int odie_linear_backward(const void* d_y, const void* slope, int activation, const void* x, const void* weight,
                    int64_t rows, int inputs, int outputs, int groups, const int32_t* offsets, int dtype, void* d_x, void* d_weight,
                    void* d_bias, void* d_residual, void* scratch, uint64_t stream);
 /* *status (device int32) = 0, or 2 once a bounded wait of the linear kernels on this

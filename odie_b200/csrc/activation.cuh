@@ -7,6 +7,12 @@ namespace odie {
 
 enum Activation : int { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3 };
 
+// How training keeps act'(z): a ReLU's as one bit per output, rows of ceil(outputs / 8) bytes, bit c % 8 of byte c / 8
+// for column c,
+// set unless z <= 0; the smooth ones' as a 16-bit code per output.
+enum SlopeKind : int { SLOPE_ONE = 0, SLOPE_CODES = 1, SLOPE_MASK = 2 };
+inline int slope_kind(int activation, const void* kept) { return !kept || activation == ACT_NONE ? SLOPE_ONE : activation == ACT_RELU ? SLOPE_MASK : SLOPE_CODES; }
+
 // Pairs of fp32 values: sm_100 multiplies and adds two per instruction.
 struct Pair {
     unsigned long long v;
@@ -64,8 +70,12 @@ __device__ __forceinline__ float slope_value(uint32_t c) {  // c: 16 bits
     return c == 0xffffu ? __int_as_float(0x7fffffff) : d;
 }
 
-// The slope of a ReLU by its output (NaN where that is NaN).
-__device__ __forceinline__ float sign_slope(float y) { return y > 0.0f ? 1.0f : y; }
+// bits, with (first <= 0, second <= 0) below them: where a ReLU is off.  They are the signs of z - 2^-149, the least
+// fp32, negative for z <= 0 alone (a NaN that arithmetic returns is positive: its gradient passes).
+__device__ __forceinline__ uint32_t off_bits(uint32_t bits, float first, float second) {
+    const float2 below = both(add2(pair(first, second), same(-0x1p-149f)));
+    return __funnelshift_l(__float_as_uint(below.x), __funnelshift_l(__float_as_uint(below.y), bits, 1), 1);
+}
 
 // act(z) (with ADD: added + act(z), its last product and the sum one fused step, so that kernels that do and do not
 // keep the slope give the same bits), with act'(z) in slope, of two values.

@@ -6,7 +6,7 @@
 // Rows of no group (behind the last offset) give zero rows of y and d x and add to no gradient.  Training keeps
 // act'(z) as a 16-bit fixed-point code (15 fraction bits above -1/4): act' lies in (-0.13, 1.13) for every
 // activation here, so the code is within 2^-16 of it, closer than a 16-bit float of it or of z would be.  A ReLU
-// without residual keeps nothing: its output's sign is its slope.
+// keeps one bit.
 //
 // The three products are one tensor-core kernel (gemm_kernel) with another operand order each; see there.  dz is
 // rounded to the rows' type, because the tensor cores take 16-bit operands; the bias gradient sums it unrounded.
@@ -69,7 +69,7 @@ struct GemmArgs {
     void* out;
     const void* bias;
     const void* residual;
-    uint16_t* slope;
+    void* slope;         // null: not kept
     int activation;
     float* partial;      // with several units per tile: [unit][m][n] sums, joined by join_kernel or finish_kernel (m: rows)
     const CUtensorMap* group_maps;  // DW with offsets: [groups][2]
@@ -242,6 +242,31 @@ __device__ __forceinline__ void finish(float (&v)[32], uint32_t (&codes)[16], co
             v[i + j + 1] = y.y;
             codes[(i + j) / 2] = slope_codes(slope);
         }
+    }
+}
+// ReLU: gives a mask, a bit where it is on.
+__device__ __forceinline__ uint32_t finish_relu(float (&v)[32], const float* bias) {
+    uint32_t off = 0;
+#pragma unroll
+    for (int i = 30; i >= 0; i -= 2) {
+        const float2 z = both(add2(pair(v[i], v[i + 1]), pair(bias[i], bias[i + 1])));
+        off = off_bits(off, z.x, z.y);
+        v[i] = max_nan(z.x, 0.0f);
+        v[i + 1] = max_nan(z.y, 0.0f);
+    }
+    return ~off;
+}
+
+// A row's bits of 32 columns, per lane (rows: of the window inside the matrix, columns: from `column` on).
+__device__ __forceinline__ void mask_store(const GemmArgs& p, int row, int column, int rows, int columns, int lane, uint32_t mask) {
+    uint8_t* to = static_cast<uint8_t*>(p.slope) + (long long)(row + lane) * ((p.n + 7) / 8) + column / 8;
+    if (lane >= rows) return;
+    if (columns >= 32 && reinterpret_cast<uintptr_t>(to) % 4 == 0) {
+        *reinterpret_cast<uint32_t*>(to) = mask;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; i += 8)
+            if (i < columns) to[i / 8] = uint8_t(mask >> i & (columns - i < 8 ? (1u << (columns - i)) - 1 : 0xffu));
     }
 }
 
@@ -439,7 +464,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
         char* stage = staging + (warp - EPILOGUE_WARP) * STAGING;
         float* bias = reinterpret_cast<float*>(staging + S::EPILOGUE_WARPS * STAGING) + (warp - EPILOGUE_WARP) * WINDOWS * 32;
         const uint32_t lanes = tmem + (uint32_t(quadrant * 32) << 16);
-        const bool wide = p.n % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) | reinterpret_cast<uintptr_t>(p.slope)) % 16 == 0;
+        const bool wide = p.n % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) | (p.activation == ACT_RELU ? 0 : reinterpret_cast<uintptr_t>(p.slope))) % 16 == 0;
         const bool wide_residual = p.n % 8 == 0 && reinterpret_cast<uintptr_t>(p.residual) % 16 == 0;
         int bias_g = -1, bias_n0 = -1;  // whose bias is held
         uint32_t summed = set;
@@ -506,6 +531,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
                     w.columns -= STRIDE;
                     continue;
                 }
+                if (MODE == FWD && tile.zero && p.slope && p.activation == ACT_RELU) mask_store(p, row, column0 + j * STRIDE, w.rows, w.columns, lane, 0);
                 if (MODE == FWD && !tile.zero) {
                     if (residual) {
                         if (wr.wide) {
@@ -519,8 +545,10 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
                         }
                         __syncwarp();
                     }
-                    if (p.activation == ACT_RELU) finish<ACT_RELU>(v, codes, bias + j * 32);
-                    else if (p.activation == ACT_SILU) finish<ACT_SILU>(v, codes, bias + j * 32);
+                    if (p.activation == ACT_RELU) {
+                        const uint32_t mask = finish_relu(v, bias + j * 32);
+                        if (p.slope) mask_store(p, row, column0 + j * STRIDE, w.rows, w.columns, lane, mask);
+                    } else if (p.activation == ACT_SILU) finish<ACT_SILU>(v, codes, bias + j * 32);
                     else if (p.activation == ACT_GELU) finish<ACT_GELU>(v, codes, bias + j * 32);
                     else finish<ACT_NONE>(v, codes, bias + j * 32);
                     if (residual) {
@@ -545,12 +573,12 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
                 __syncwarp();
                 window_store(static_cast<uint16_t*>(p.out) + at + j * STRIDE, w, lane, stage);
                 __syncwarp();
-                if (MODE == FWD && p.slope) {
+                if (MODE == FWD && p.slope && p.activation != ACT_RELU) {
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
                         *staged(stage, lane, u) = make_uint4(codes[u * 4], codes[u * 4 + 1], codes[u * 4 + 2], codes[u * 4 + 3]);
                     __syncwarp();
-                    window_store(p.slope + at + j * STRIDE, w, lane, stage);
+                    window_store(static_cast<uint16_t*>(p.slope) + at + j * STRIDE, w, lane, stage);
                     __syncwarp();
                 }
                 w.columns -= STRIDE;
@@ -645,40 +673,51 @@ __global__ void __launch_bounds__(256) join_kernel(const float* partial, T* d_we
 }
 
 // The sums over parts of K, in order, with the epilogue of the products (DX: neither bias, residual nor activation).
+// Rows of threads are padded to eight columns.
 struct FinishArgs {
     const float* partial;  // [splits][rows][n]
     int splits;
-    long long count;       // rows * n
+    long long rows;
     int n;
     const void* bias;
     const void* residual;
     void* out;
-    uint16_t* slope;
+    void* slope;
     int activation;
 };
 template <typename T>
 __global__ void __launch_bounds__(256) finish_kernel(FinishArgs a) {
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < a.count; i += (long long)gridDim.x * 256) {
-        float sum = 0.0f;
+    const int pitch = (a.n + 7) / 8;
+    // (K is cut only where there are fewer tiles than SMs, so that 32 bits hold the padded count)
+    const unsigned unit = blockIdx.x * 256 + threadIdx.x, line = unit / unsigned(pitch * 8);
+    const int column = int(unit - line * unsigned(pitch * 8));
+    const long long row = line;
+    const bool inside = row < a.rows && column < a.n;
+    const long long at = row * a.n + column;
+    float z = 0.0f;
+    if (inside) {
 #pragma unroll 8
-        for (int s = 0; s < a.splits; ++s) sum += a.partial[s * a.count + i];
-        if (a.bias) sum += to_float(static_cast<const T*>(a.bias)[i % a.n]);
-        const Pair z = same(sum), added = same(a.residual ? to_float(static_cast<const T*>(a.residual)[i]) : 0.0f);
+        for (int s = 0; s < a.splits; ++s) z += __ldg(a.partial + s * a.rows * a.n + at);
+        if (a.bias) z += to_float(static_cast<const T*>(a.bias)[column]);
+        const Pair added = same(a.residual ? to_float(static_cast<const T*>(a.residual)[at]) : 0.0f);
         Pair slope, y;
-        if (a.activation == ACT_RELU) y = activate<ACT_RELU, true>(z, slope, added);
-        else if (a.activation == ACT_SILU) y = activate<ACT_SILU, true>(z, slope, added);
-        else if (a.activation == ACT_GELU) y = activate<ACT_GELU, true>(z, slope, added);
-        else y = activate<ACT_NONE, true>(z, slope, added);
-        static_cast<T*>(a.out)[i] = from_float<T>(both(y).x);
-        if (a.slope) a.slope[i] = uint16_t(slope_codes(slope));
+        if (a.activation == ACT_RELU) y = activate<ACT_RELU, true>(same(z), slope, added);
+        else if (a.activation == ACT_SILU) y = activate<ACT_SILU, true>(same(z), slope, added);
+        else if (a.activation == ACT_GELU) y = activate<ACT_GELU, true>(same(z), slope, added);
+        else y = activate<ACT_NONE, true>(same(z), slope, added);
+        static_cast<T*>(a.out)[at] = from_float<T>(both(y).x);
+        if (a.slope && a.activation != ACT_RELU) static_cast<uint16_t*>(a.slope)[at] = uint16_t(slope_codes(slope));
+    }
+    if (a.slope && a.activation == ACT_RELU) {  // eight lanes have a byte
+        const uint32_t on = __ballot_sync(0xffffffffu, inside && !(z <= 0.0f));
+        if (inside && column % 8 == 0) static_cast<uint8_t*>(a.slope)[row * pitch + column / 8] = uint8_t(on >> (threadIdx.x & 24));
     }
 }
 
 // ---------------------------------------------------------------- dz and the bias gradient
 struct DzArgs {
     const void* d_y;
-    const uint16_t* slope;  // codes; null: 1
-    const void* y;          // instead of codes: the output of a ReLU, whose slope is its sign
+    const void* kept;       // the slope that forward kept
     void* dz;               // null: not wanted
     void* d_residual;       // null: not wanted
     void* d_bias;           // null: not wanted
@@ -691,25 +730,11 @@ struct DzArgs {
     const int* offsets;
 };
 
-template <typename T>
-__device__ __forceinline__ float2 dz_pair(const DzArgs& a, uint32_t d_y, uint32_t kept) {
-    float2 f = unpack_pair<T>(d_y);
-    if (a.slope) {
-        f.x *= slope_value(kept & 0xffffu);
-        f.y *= slope_value(kept >> 16);
-    } else if (a.y) {
-        const float2 o = unpack_pair<T>(kept);
-        f.x *= sign_slope(o.x);
-        f.y *= sign_slope(o.y);
-    }
-    return f;
-}
-
 // A block: one unit of rows (of one group, or of none) x COLUMNS columns per thread of `lanes` threads: eight, or one
 // where rows do not start on 16-byte boundaries.  Column sums: each thread over its rows, the lanes of a warp in a
 // tree, the warps in order.
-template <typename T, int COLUMNS, int THREADS>
-__global__ void __launch_bounds__(THREADS) dz_kernel(DzArgs a, int lanes_log2) {
+template <typename T, int COLUMNS, int THREADS, int KIND>
+__global__ void __launch_bounds__(THREADS, THREADS == 256 ? 5 : 1) dz_kernel(DzArgs a, int lanes_log2) {
     constexpr int WARPS = THREADS / 32;
     __shared__ float sums[WARPS][32 * COLUMNS];
     const Unit u = unit_at<true>(a.offsets, a.groups, a.rows, a.chunk, blockIdx.x);
@@ -717,7 +742,7 @@ __global__ void __launch_bounds__(THREADS) dz_kernel(DzArgs a, int lanes_log2) {
     const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1), line = threadIdx.x >> lanes_log2, lines = THREADS >> lanes_log2;
     const int column = (blockIdx.y * lanes + lane) * COLUMNS;
     const bool live = u.g < a.groups;
-    const void* kept = a.slope ? static_cast<const void*>(a.slope) : a.y;
+    const int mask_pitch = (a.n + 7) / 8;
     float sum[COLUMNS];
 #pragma unroll
     for (int i = 0; i < COLUMNS; ++i) sum[i] = 0.0f;
@@ -727,12 +752,21 @@ __global__ void __launch_bounds__(THREADS) dz_kernel(DzArgs a, int lanes_log2) {
             const long long at = row * a.n + column;
             if constexpr (COLUMNS == 8) {
                 const uint4 d = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.d_y) + at));
-                const uint4 k = kept ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(kept) + at)) : make_uint4(0, 0, 0, 0);
+                uint4 k = make_uint4(0, 0, 0, 0);
+                if (KIND == SLOPE_CODES) k = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.kept) + at));
+                if (KIND == SLOPE_MASK) k.x = __ldg(static_cast<const uint8_t*>(a.kept) + row * mask_pitch + column / 8);
                 const uint32_t ds[4] = {d.x, d.y, d.z, d.w}, ks[4] = {k.x, k.y, k.z, k.w};
                 uint32_t z[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float2 f = dz_pair<T>(a, ds[i], ks[i]);
+                    float2 f = unpack_pair<T>(ds[i]);
+                    if (KIND == SLOPE_CODES) {
+                        f.x *= slope_value(ks[i] & 0xffffu);
+                        f.y *= slope_value(ks[i] >> 16);
+                    } else if (KIND == SLOPE_MASK) {
+                        f.x = k.x >> (2 * i) & 1 ? f.x : 0.0f;
+                        f.y = k.x >> (2 * i + 1) & 1 ? f.y : 0.0f;
+                    }
                     z[i] = pack_pair<T>(f.x, f.y);
                     sum[2 * i] += f.x;
                     sum[2 * i + 1] += f.y;
@@ -742,7 +776,9 @@ __global__ void __launch_bounds__(THREADS) dz_kernel(DzArgs a, int lanes_log2) {
                     *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.d_residual) + at) = live ? d : make_uint4(0, 0, 0, 0);
             } else {
                 const uint16_t d = static_cast<const uint16_t*>(a.d_y)[at];
-                const float f = dz_pair<T>(a, d, kept ? static_cast<const uint16_t*>(kept)[at] : 0).x;
+                float f = unpack_pair<T>(d).x;
+                if (KIND == SLOPE_CODES) f *= slope_value(static_cast<const uint16_t*>(a.kept)[at]);
+                if (KIND == SLOPE_MASK) f = static_cast<const uint8_t*>(a.kept)[row * mask_pitch + column / 8] >> (column & 7) & 1 ? f : 0.0f;
                 if (a.dz) static_cast<T*>(a.dz)[row * a.ld + column] = from_float<T>(f);
                 if (a.d_residual) static_cast<uint16_t*>(a.d_residual)[at] = live ? d : uint16_t(0);
                 sum[0] += f;
@@ -806,20 +842,23 @@ struct FewArgs {
     const void* bias;
     const void* residual;
     void* y;
-    uint16_t* slope;
+    void* slope;
     int rows, inputs, outputs;  // rows: M
     int activation;
 };
 
-constexpr int FEW_ROWS = 2, FEW_THREADS = 128, FEW_VECTORS = 16;
+constexpr int FEW_ROWS = 2, FEW_VECTORS = 16;
 
-// M: rows; V: vectors per lane of one row of W at a time.
-template <typename T, int BYTES, int M, int V>
-__global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(FewArgs a) {
+// M: rows; V: vectors per lane of one row of W at a time; MASK: a ReLU's bits are kept (the block has whole bytes).
+template <typename T, int BYTES, int M, int V, int THREADS, bool MASK>
+__global__ void __launch_bounds__(THREADS) few_rows_kernel(FewArgs a) {
     using P = Pack<T, BYTES>;
     constexpr int COLUMNS = FEW_VECTORS / V, CHUNK = 32 * P::N * V;  // CHUNK: values of K at a time
+    constexpr int BLOCK = THREADS / 32 * COLUMNS;  // columns of the block
+    static_assert(!MASK || BLOCK % 8 == 0, "whole bytes");
     __shared__ alignas(16) T xs[M][CHUNK];
-    const int lane = threadIdx.x & 31, n0 = (blockIdx.x * (FEW_THREADS / 32) + (threadIdx.x >> 5)) * COLUMNS;
+    __shared__ bool on[M][BLOCK];
+    const int lane = threadIdx.x & 31, n0 = blockIdx.x * BLOCK + (threadIdx.x >> 5) * COLUMNS;
     const T* w = static_cast<const T*>(a.weight);
     const T* x = static_cast<const T*>(a.x);
     float sum[COLUMNS][M];
@@ -841,7 +880,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(FewArgs a) {
 #pragma unroll
         for (int m = 0; m < M; ++m)
 #pragma unroll 4
-            for (int i = threadIdx.x; i < CHUNK / P::N; i += FEW_THREADS) {
+            for (int i = threadIdx.x; i < CHUNK / P::N; i += THREADS) {
                 const P q = i < count ? P::load(x + (long long)m * a.inputs + k0 + i * P::N) : P::zero();
                 q.store(&xs[m][i * P::N]);
             }
@@ -868,6 +907,7 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(FewArgs a) {
             for (int d = 16; d > 0; d /= 2) sum[c][m] += __shfl_xor_sync(0xffffffffu, sum[c][m], d);
             if (lane == m) mine = sum[c][m];
         }
+        if (MASK && lane < M) on[lane][n - blockIdx.x * BLOCK] = false;
         if (lane >= M || n >= a.outputs) continue;
         const long long at = (long long)lane * a.outputs + n;
         if (a.bias) mine += to_float(static_cast<const T*>(a.bias)[n]);
@@ -878,7 +918,18 @@ __global__ void __launch_bounds__(FEW_THREADS) few_rows_kernel(FewArgs a) {
         else if (a.activation == ACT_GELU) y = activate<ACT_GELU, true>(z, slope, added);
         else y = activate<ACT_NONE, true>(z, slope, added);
         static_cast<T*>(a.y)[at] = from_float<T>(both(y).x);
-        if (a.slope) a.slope[at] = uint16_t(slope_codes(slope));
+        if (MASK) on[lane][n - blockIdx.x * BLOCK] = !(mine <= 0.0f);
+        else if (a.slope) static_cast<uint16_t*>(a.slope)[at] = uint16_t(slope_codes(slope));
+    }
+    if constexpr (MASK) {
+        __syncthreads();
+        const int pitch = (a.outputs + 7) / 8, m = threadIdx.x / (BLOCK / 8), b = threadIdx.x % (BLOCK / 8), at = blockIdx.x * (BLOCK / 8) + b;
+        if (m < M && at < pitch) {
+            uint32_t bits = 0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) bits |= on[m][b * 8 + e] ? 1u << e : 0u;
+            static_cast<uint8_t*>(a.slope)[m * pitch + at] = uint8_t(bits);
+        }
     }
 }
 
@@ -1007,10 +1058,18 @@ template <typename T>
 void launch_few_rows(const FewArgs& a, cudaStream_t stream) {
     const int vector = row_vector(a.inputs, ROW_F16, a.x, a.weight);
     auto go = [&](auto bytes, auto rows) {
-        constexpr int B = decltype(bytes)::value, M = decltype(rows)::value, WARPS = FEW_THREADS / 32;
+        constexpr int B = decltype(bytes)::value, M = decltype(rows)::value;
         constexpr int SHORT = 4 * 32 * (B / 2);  // values of four vectors per lane
-        if (a.inputs <= SHORT) few_rows_kernel<T, B, M, 4><<<unsigned(ceil_div(a.outputs, WARPS * 4)), FEW_THREADS, 0, stream>>>(a);
-        else few_rows_kernel<T, B, M, FEW_VECTORS><<<unsigned(ceil_div(a.outputs, WARPS)), FEW_THREADS, 0, stream>>>(a);
+        auto launch = [&](auto v, auto threads, auto mask) {
+            constexpr int V = decltype(v)::value, THREADS = decltype(threads)::value, BLOCK = THREADS / 32 * (FEW_VECTORS / V);
+            few_rows_kernel<T, B, M, V, THREADS, decltype(mask)::value><<<unsigned(ceil_div(a.outputs, BLOCK)), THREADS, 0, stream>>>(a);
+        };
+        using std::integral_constant;
+        const bool mask = a.slope && a.activation == ACT_RELU;
+        if (a.inputs <= SHORT && mask) launch(integral_constant<int, 4>{}, integral_constant<int, 128>{}, std::true_type{});
+        else if (a.inputs <= SHORT) launch(integral_constant<int, 4>{}, integral_constant<int, 128>{}, std::false_type{});
+        else if (mask) launch(integral_constant<int, FEW_VECTORS>{}, integral_constant<int, 256>{}, std::true_type{});
+        else launch(integral_constant<int, FEW_VECTORS>{}, integral_constant<int, 128>{}, std::false_type{});
     };
     auto with_rows = [&](auto bytes) {
         if (a.rows == 1) go(bytes, std::integral_constant<int, 1>{});
@@ -1094,8 +1153,8 @@ void launch_product(const void* a, const void* b, int64_t ld_a, int64_t ld_b, in
         launch_gemm<T, MODE, CG, BN, false>(map_a, map_b, p, tiles, stream);
     });
     if (split.parts > 1) {
-        const FinishArgs f{partial, split.parts, p.rows * p.n, p.n, p.bias, p.residual, p.out, p.slope, p.activation};
-        finish_kernel<T><<<unsigned(std::min<int64_t>(ceil_div(f.count, 256), 16 * SMS)), 256, 0, stream>>>(f);
+        const FinishArgs f{partial, split.parts, p.rows, p.n, p.bias, p.residual, p.out, p.slope, p.activation};
+        finish_kernel<T><<<unsigned(ceil_div(p.rows * ceil_div(p.n, 8) * 8, 256)), 256, 0, stream>>>(f);
         ODIE_CUDA(cudaGetLastError());
         note_launch();
     }
@@ -1149,18 +1208,24 @@ int64_t dz_chunk(int64_t rows, int groups) {
 int64_t dz_units(int64_t rows, int groups) { return ceil_div(rows, dz_chunk(rows, groups)) + groups + 1; }
 
 template <typename T>
-void launch_dz(const DzArgs& a, cudaStream_t stream) {
-    const bool wide = a.n % 8 == 0 && (uintptr_t(a.d_y) | uintptr_t(a.slope) | uintptr_t(a.y) | uintptr_t(a.d_residual)) % 16 == 0;
+void launch_dz(const DzArgs& a, int kind, cudaStream_t stream) {
+    const bool wide = a.n % 8 == 0 && (uintptr_t(a.d_y) | (kind == SLOPE_CODES ? uintptr_t(a.kept) : 0) | uintptr_t(a.d_residual)) % 16 == 0;
     const bool single = dz_single(a.rows, a.groups);
     const int columns = wide ? 8 : 1;
     int log2 = 0;
     while (log2 < (single && wide ? 1 : 5) && (columns << log2) < a.n) ++log2;
     const dim3 grid(unsigned(dz_units(a.rows, a.groups)), unsigned(ceil_div(a.n, columns << log2)));
     ODIE_REQUIRE(grid.y <= 65535, "too many outputs for one launch");
-    if (single && wide) dz_kernel<T, 8, 1024><<<grid, 1024, 0, stream>>>(a, log2);
-    else if (single) dz_kernel<T, 1, 1024><<<grid, 1024, 0, stream>>>(a, log2);
-    else if (wide) dz_kernel<T, 8, 256><<<grid, 256, 0, stream>>>(a, log2);
-    else dz_kernel<T, 1, 256><<<grid, 256, 0, stream>>>(a, log2);
+    auto go = [&](auto k) {
+        constexpr int KIND = decltype(k)::value;
+        if (single && wide) dz_kernel<T, 8, 1024, KIND><<<grid, 1024, 0, stream>>>(a, log2);
+        else if (single) dz_kernel<T, 1, 1024, KIND><<<grid, 1024, 0, stream>>>(a, log2);
+        else if (wide) dz_kernel<T, 8, 256, KIND><<<grid, 256, 0, stream>>>(a, log2);
+        else dz_kernel<T, 1, 256, KIND><<<grid, 256, 0, stream>>>(a, log2);
+    };
+    if (kind == SLOPE_MASK) go(std::integral_constant<int, SLOPE_MASK>{});
+    else if (kind == SLOPE_CODES) go(std::integral_constant<int, SLOPE_CODES>{});
+    else go(std::integral_constant<int, SLOPE_ONE>{});
     ODIE_CUDA(cudaGetLastError());
     note_launch();
 }
@@ -1204,7 +1269,7 @@ extern "C" int64_t odie_linear_scratch(int64_t rows, int inputs, int outputs, in
 
 extern "C" int odie_linear(const void* x, const void* weight, const void* bias, const void* residual, int64_t rows, int inputs,
                            int outputs, int groups, const int32_t* offsets, int dtype, int activation, void* y,
-                           uint16_t* slope, void* scratch, uint64_t stream_handle) {
+                           void* slope, void* scratch, uint64_t stream_handle) {
     return guarded([&] {
         check_linear(rows, inputs, outputs, groups, offsets, dtype, activation);
         if (rows == 0) return;
@@ -1215,7 +1280,7 @@ extern "C" int odie_linear(const void* x, const void* weight, const void* bias, 
             with_linear_type(dtype, [&](auto type) { launch_few_rows<decltype(type)>(a, stream); });
             return;
         }
-        if (thin_sizes(inputs, outputs) && on_16_bytes({x, weight, residual, y, slope})) {
+        if (thin_sizes(inputs, outputs) && on_16_bytes({x, weight, residual, y, activation == ACT_RELU ? nullptr : slope})) {
             ThinArgs a{};
             a.rows = rows;
             a.inputs = inputs;
@@ -1265,11 +1330,11 @@ extern "C" int64_t odie_linear_backward_scratch(int64_t rows, int inputs, int ou
     return BackwardScratch(nullptr, rows, inputs, outputs, groups).bytes;
 }
 
-extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, const void* relu_y, const void* x, const void* weight, int64_t rows,
+extern "C" int odie_linear_backward(const void* d_y, const void* slope, int activation, const void* x, const void* weight, int64_t rows,
                                     int inputs, int outputs, int groups, const int32_t* offsets, int dtype, void* d_x,
                                     void* d_weight, void* d_bias, void* d_residual, void* scratch, uint64_t stream_handle) {
     return guarded([&] {
-        check_linear(rows, inputs, outputs, groups, offsets, dtype, ACT_NONE);
+        check_linear(rows, inputs, outputs, groups, offsets, dtype, activation);
         const cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_handle);
         if (rows == 0) {
             if (d_weight) ODIE_CUDA(cudaMemsetAsync(d_weight, 0, size_t(groups) * outputs * inputs * 2, stream));
@@ -1278,9 +1343,10 @@ extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, cons
         }
         ODIE_REQUIRE(d_y && (x || !d_weight) && (weight || !d_x) && scratch, "d_y, x, weight and scratch are required");
         ODIE_REQUIRE(uintptr_t(scratch) % 256 == 0, "scratch must start on a 256-byte boundary");
-        ODIE_REQUIRE(!slope || !relu_y, "slope and relu_y exclude each other");
+        ODIE_REQUIRE(slope || activation == ACT_NONE, "slope is required with an activation");
+        const int kind = slope_kind(activation, slope);
         const BackwardScratch s(scratch, rows, inputs, outputs, groups);
-        if (thin_sizes(inputs, outputs) && on_16_bytes({d_y, slope, relu_y, x, weight, d_x, d_residual})) {
+        if (thin_sizes(inputs, outputs) && on_16_bytes({d_y, kind == SLOPE_CODES ? slope : nullptr, x, weight, d_x, d_residual})) {
             ThinArgs a{};
             a.rows = rows;
             a.inputs = inputs;
@@ -1291,8 +1357,8 @@ extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, cons
             a.x = x;
             a.weight = weight;
             a.d_y = d_y;
-            a.code = slope;
-            a.relu_y = relu_y;
+            a.kept = slope;
+            a.activation = activation;
             a.d_x = d_x;
             a.d_weight = d_weight;
             a.d_bias = d_bias;
@@ -1311,15 +1377,14 @@ extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, cons
         const bool bf16 = dtype == ROW_BF16;
         const int64_t ld_x = round8(inputs), ld_z = round8(outputs);
         const bool products = d_x || d_weight;
-        const bool as_is = !slope && !relu_y && outputs % 8 == 0;  // dz is d_y
+        const bool as_is = kind == SLOPE_ONE && outputs % 8 == 0;  // dz is d_y
         const void* dz = as_is ? d_y : s.dz;
         with_linear_type(dtype, [&](auto type) {
             using T = decltype(type);
             if ((products && !as_is) || d_bias || d_residual) {
                 DzArgs a{};
                 a.d_y = d_y;
-                a.slope = slope;
-                a.y = relu_y;
+                a.kept = slope;
                 a.dz = products && !as_is ? s.dz : nullptr;
                 a.d_residual = d_residual;
                 const bool join = d_bias && rows > dz_chunk(rows, groups);
@@ -1331,7 +1396,7 @@ extern "C" int odie_linear_backward(const void* d_y, const uint16_t* slope, cons
                 a.chunk = int(dz_chunk(rows, groups));
                 a.groups = groups;
                 a.offsets = offsets;
-                launch_dz<T>(a, stream);
+                launch_dz<T>(a, kind, stream);
                 if (join) launch_join<T>(s.bias, nullptr, d_bias, offsets, groups, rows, a.chunk, dz_units(rows, groups), 0, outputs, stream);
             }
             if (s.x && products)

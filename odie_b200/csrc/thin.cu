@@ -11,6 +11,11 @@
 // W is read in the same order.  Column n' of output tile j stands for column 8 (n' / 2) + 2 j + n' % 2, so a lane
 // ends with the 8 columns 8 c .. 8 c + 7 of the result.  d W = dz^T x needs dz and x by columns: movmatrix turns
 // each 8 x 8 tile, in the same order of columns.
+//
+// A ReLU's corner: where the tensor cores' sum is within its own error of zero, the fp32 chain of fused multiply-adds
+// in ascending order of the inputs decides (the convention of this library's router), so that a unit is on or off as
+// in any fp32 evaluation of the layer; at these sizes one unit is a large part of a row's gradient.  About one step of
+// 16 rows in forty looks at a chain.
 #include "thin.cuh"
 #include "odie_b200.h"
 #include <algorithm>
@@ -59,6 +64,37 @@ __device__ __forceinline__ uint4 load_row(const void* base, long long row, int w
     return on ? __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + row * width + column)) : make_uint4(0, 0, 0, 0);
 }
 
+// The larger magnitudes, pairwise, of two pairs of 16-bit elements; the signs are off.
+template <typename T>
+__device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
+    return __vmaxu2(a & 0x7fff7fffu, b & 0x7fff7fffu);  // magnitudes order as their bits do
+}
+template <typename T>
+__device__ __forceinline__ uint32_t larger(uint32_t a, const uint4& v) {
+    return larger<T>(larger<T>(larger<T>(a, v.x), larger<T>(v.y, v.z)), v.w);
+}
+template <typename T>
+__device__ __forceinline__ float larger_of(uint32_t pair) {
+    const float2 f = unpack_pair<T>(pair);
+    return fmaxf(f.x, f.y);
+}
+
+// x . w as the chain in ascending order; count is a multiple of 8.
+template <typename T>
+__device__ __forceinline__ float chain(const void* x, const void* w, int count) {
+    float sum = 0.0f;
+#pragma unroll 4
+    for (int k = 0; k < count / 8; ++k) {
+        const uint4 a = __ldg(static_cast<const uint4*>(x) + k), b = __ldg(static_cast<const uint4*>(w) + k);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = unpack_pair<T>(word(a, i)), g = unpack_pair<T>(word(b, i));
+            sum = fmaf(f.y, g.y, fmaf(f.x, g.x, sum));
+        }
+    }
+    return sum;
+}
+
 // KB, NB: blocks of 32 inputs and outputs.
 template <typename T, int KB, int NB, int ACT>
 __global__ void __launch_bounds__(THREADS, KB * NB == 4 ? 3 : 4) thin_forward_kernel(ThinArgs a) {
@@ -72,7 +108,8 @@ __global__ void __launch_bounds__(THREADS, KB * NB == 4 ? 3 : 4) thin_forward_ke
                 const int column = nb * 32 + c * 8;
                 if (column >= a.outputs) continue;
                 *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.y) + row * a.outputs + column) = make_uint4(0, 0, 0, 0);
-                if (a.slope) *reinterpret_cast<uint4*>(a.slope + row * a.outputs + column) = make_uint4(0, 0, 0, 0);
+                if (ACT == ACT_RELU && a.slope) static_cast<uint8_t*>(a.slope)[(row * a.outputs + column) / 8] = 0;
+                else if (a.slope) *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.slope) + row * a.outputs + column) = make_uint4(0, 0, 0, 0);
             }
         }
         return;
@@ -94,6 +131,28 @@ __global__ void __launch_bounds__(THREADS, KB * NB == 4 ? 3 : 4) thin_forward_ke
             const int n = nb * 32 + c * 8 + e;
             bias[nb][e] = a.bias && n < a.outputs ? to_float(static_cast<const T*>(a.bias)[(long long)u.g * a.outputs + n]) : 0.0f;
         }
+    }
+    float bias_corner = 0.0f, corner = 0.0f;  // corner: times a row's largest input: what the tensor cores' sum may be off by
+    if (ACT == ACT_RELU) {
+        uint32_t largest = 0;
+        float most_bias = 0.0f;
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int kb = 0; kb < KB; ++kb) largest = larger<T>(largest, w[nb][j][kb]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most_bias = fmaxf(most_bias, fabsf(bias[nb][e]));
+        }
+        float most = larger_of<T>(largest);
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) {
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, d));
+            most_bias = fmaxf(most_bias, __shfl_xor_sync(0xffffffffu, most_bias, d));
+        }
+        corner = most * float(a.inputs) * 0x1p-20f;
+        bias_corner = most_bias * 0x1p-21f;
     }
     extern __shared__ uint4 slots[];
     uint4* mine = slots + warp * (FORWARD_STAGES * VECTORS * 32) + lane;
@@ -125,6 +184,14 @@ __global__ void __launch_bounds__(THREADS, KB * NB == 4 ? 3 : 4) thin_forward_ke
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) x[kb][h] = now[(kb * 2 + h) * 32];
+        float near = 0.0f;  // for both rows of the lane
+        if (ACT == ACT_RELU) {
+            uint32_t largest = larger<T>(larger<T>(0, x[0][0]), x[0][1]);
+            if (KB == 2) largest = larger<T>(larger<T>(largest, x[KB - 1][0]), x[KB - 1][1]);
+            largest = larger<T>(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+            largest = larger<T>(largest, __shfl_xor_sync(0xffffffffu, largest, 2));
+            near = larger_of<T>(largest) * corner + bias_corner;
+        }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
             const int column = nb * 32 + c * 8;
@@ -146,30 +213,54 @@ __global__ void __launch_bounds__(THREADS, KB * NB == 4 ? 3 : 4) thin_forward_ke
                         mma16816<T>(d[j], word(x[kb][0], 2 * s), word(x[kb][1], 2 * s), word(x[kb][0], 2 * s + 1), word(x[kb][1], 2 * s + 1),
                                     word(w[nb][j][kb], 2 * s), word(w[nb][j][kb], 2 * s + 1));
             }
+            if (ACT == ACT_RELU) {
+                float least = fabsf(d[0][0]);
+#pragma unroll
+                for (int e = 1; e < 16; ++e) least = fminf(least, fabsf(d[e / 4][e % 4]));
+                if (least < near) {
+                    uint32_t which = 0;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e)
+                        which |= fabsf(d[e / 4][e % 4]) < near && inside && r0 + g + (e % 4 / 2) * 8 < u.to ? 1u << e : 0u;
+#pragma unroll 1
+                    for (; which; which &= which - 1) {
+                        const int at = __ffs(which) - 1, n = column + at / 4 * 2 + at % 2;
+                        const long long row = r0 + g + (at % 4 / 2) * 8;
+                        const float z = chain<T>(static_cast<const uint16_t*>(a.x) + row * a.inputs, weight + n * a.inputs, a.inputs) +
+                                        (a.bias ? to_float(static_cast<const T*>(a.bias)[(long long)u.g * a.outputs + n]) : 0.0f);
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) d[e / 4][e % 4] = at == e ? z : d[e / 4][e % 4];
+                    }
+                }
+            }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                uint32_t y[4], codes[4];
+                const long long row = r0 + g + 8 * h;
+                uint32_t y[4], codes[4], off = 0;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const float2 f = a.residual ? unpack_pair<T>(word(r[h], j)) : make_float2(0.0f, 0.0f);
                     Pair slope, z = activate<ACT, true>(pair(d[j][2 * h], d[j][2 * h + 1]), slope, pair(f.x, f.y));
                     y[j] = pack_pair<T>(both(z).x, both(z).y);
-                    if (a.slope) codes[j] = slope_codes(slope);
+                    if (ACT == ACT_RELU) off = off_bits(off, d[3 - j][2 * h], d[3 - j][2 * h + 1]);
+                    else if (a.slope) codes[j] = slope_codes(slope);
                 }
-                const long long row = r0 + g + 8 * h;
                 if (row < u.to && inside) {
                     *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.y) + row * a.outputs + column) = make_uint4(y[0], y[1], y[2], y[3]);
-                    if (a.slope) *reinterpret_cast<uint4*>(a.slope + row * a.outputs + column) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+                    if (ACT == ACT_RELU && a.slope)
+                        static_cast<uint8_t*>(a.slope)[(row * a.outputs + column) / 8] = uint8_t(~off);
+                    else if (a.slope)
+                        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.slope) + row * a.outputs + column) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
                 }
             }
         }
     }
 }
 
-template <typename T, int KB, int NB>
+template <typename T, int KB, int NB, int KIND>
 __global__ void __launch_bounds__(THREADS, 2) thin_backward_kernel(ThinArgs a) {
     constexpr int BACKWARD_STAGES = STAGES_BACK<KB, NB>;
-    constexpr int VECTORS = NB * 4 + KB * 2;
+    constexpr int AT_X = NB * (KIND == SLOPE_CODES ? 4 : 2), VECTORS = AT_X + KB * 2;
     extern __shared__ uint4 slots[];
     // W by its rows' order for d x: [K-step of 16 outputs][8-column tile of inputs][lane]
     __shared__ uint2 turned_w[NB * 2][KB * 4][32];
@@ -215,7 +306,6 @@ __global__ void __launch_bounds__(THREADS, 2) thin_backward_kernel(ThinArgs a) {
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int e = 0; e < 8; ++e) db[nb][e] = 0.0f;
-    const void* kept = a.code ? static_cast<const void*>(a.code) : a.relu_y;
     uint4* mine = slots + warp * (BACKWARD_STAGES * VECTORS * 32) + lane;
     auto ahead = [&](int step) {
         const long long r0 = u.from + warp * 16 + (long long)step * WARPS * 16;
@@ -228,19 +318,40 @@ __global__ void __launch_bounds__(THREADS, 2) thin_backward_kernel(ThinArgs a) {
             for (int nb = 0; nb < NB; ++nb) {
                 const int column = nb * 32 + c * 8;
                 copy_ahead(to + (nb * 2 + h) * 32, a.d_y, row, a.outputs, column, on && column < a.outputs);
-                if (kept) copy_ahead(to + (NB * 2 + nb * 2 + h) * 32, kept, row, a.outputs, column, on && column < a.outputs);
+                if (KIND == SLOPE_CODES) copy_ahead(to + (NB * 2 + nb * 2 + h) * 32, a.kept, row, a.outputs, column, on && column < a.outputs);
             }
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
                 const int column = kb * 32 + c * 8;
-                if (a.d_weight) copy_ahead(to + (NB * 4 + kb * 2 + h) * 32, a.x, row, a.inputs, column, on && column < a.inputs);
+                if (a.d_weight) copy_ahead(to + (AT_X + kb * 2 + h) * 32, a.x, row, a.inputs, column, on && column < a.inputs);
             }
         }
         copies_end();
     };
     for (int s = 0; s < BACKWARD_STAGES - 1; ++s) ahead(s);
+    // the mask's bytes, a step ahead
+    uint32_t next[NB][2];
+    auto masks = [&](long long r0) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const long long row = r0 + g + 8 * h;
+                const int column = nb * 32 + c * 8;
+                next[nb][h] = row < u.to && column < a.outputs ? __ldg(static_cast<const uint8_t*>(a.kept) + (row * a.outputs + column) / 8) : 0;
+            }
+    };
+    if (KIND == SLOPE_MASK) masks(u.from + warp * 16);
     int step = 0;
     for (long long r0 = u.from + warp * 16; r0 < u.to; r0 += WARPS * 16, ++step) {
+        uint32_t bits[NB][2];
+        if (KIND == SLOPE_MASK) {
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) bits[nb][h] = next[nb][h];
+            masks(r0 + WARPS * 16);
+        }
         ahead(step + BACKWARD_STAGES - 1);
         copies_wait<BACKWARD_STAGES - 1>();
         const uint4* now = mine + step % BACKWARD_STAGES * (VECTORS * 32);
@@ -250,10 +361,10 @@ __global__ void __launch_bounds__(THREADS, 2) thin_backward_kernel(ThinArgs a) {
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 z[nb][h] = now[(nb * 2 + h) * 32];
-                s[nb][h] = kept ? now[(NB * 2 + nb * 2 + h) * 32] : make_uint4(0, 0, 0, 0);
+                if (KIND == SLOPE_CODES) s[nb][h] = now[(NB * 2 + nb * 2 + h) * 32];
             }
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb) x[kb][h] = a.d_weight ? now[(NB * 4 + kb * 2 + h) * 32] : make_uint4(0, 0, 0, 0);
+            for (int kb = 0; kb < KB; ++kb) x[kb][h] = a.d_weight ? now[(AT_X + kb * 2 + h) * 32] : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
@@ -266,14 +377,13 @@ __global__ void __launch_bounds__(THREADS, 2) thin_backward_kernel(ThinArgs a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     float2 f = unpack_pair<T>(word(z[nb][h], i));
-                    const uint32_t k = word(s[nb][h], i);
-                    if (a.code) {
+                    if (KIND == SLOPE_CODES) {
+                        const uint32_t k = word(s[nb][h], i);
                         f.x *= slope_value(k & 0xffffu);
                         f.y *= slope_value(k >> 16);
-                    } else if (a.relu_y) {
-                        const float2 o = unpack_pair<T>(k);
-                        f.x *= sign_slope(o.x);
-                        f.y *= sign_slope(o.y);
+                    } else if (KIND == SLOPE_MASK) {
+                        f.x = bits[nb][h] >> (2 * i) & 1 ? f.x : 0.0f;
+                        f.y = bits[nb][h] >> (2 * i + 1) & 1 ? f.y : 0.0f;
                     }
                     db[nb][2 * i] += f.x;
                     db[nb][2 * i + 1] += f.y;
@@ -403,9 +513,17 @@ template <typename T>
 void launch_thin_backward(const ThinArgs& a, cudaStream_t stream) {
     with_blocks(a.inputs, a.outputs, [&](auto kb, auto nb) {
         constexpr int KB = decltype(kb)::value, NB = decltype(nb)::value;
-        constexpr int BYTES = WARPS * STAGES_BACK<KB, NB> * (NB * 4 + KB * 2) * 512;
-        ODIE_CUDA(cudaFuncSetAttribute(thin_backward_kernel<T, KB, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES));
-        thin_backward_kernel<T, KB, NB><<<unsigned(thin_units(a.rows, a.groups, a.chunk)), THREADS, BYTES, stream>>>(a);
+        auto go = [&](auto kind) {
+            constexpr int KIND = decltype(kind)::value;
+            constexpr int BYTES = WARPS * STAGES_BACK<KB, NB> * (NB * (KIND == SLOPE_CODES ? 4 : 2) + KB * 2) * 512;
+            const auto kernel = thin_backward_kernel<T, KB, NB, KIND>;
+            ODIE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES));
+            kernel<<<unsigned(thin_units(a.rows, a.groups, a.chunk)), THREADS, BYTES, stream>>>(a);
+        };
+        const int kind = slope_kind(a.activation, a.kept);
+        if (kind == SLOPE_MASK) go(std::integral_constant<int, SLOPE_MASK>{});
+        else if (kind == SLOPE_CODES) go(std::integral_constant<int, SLOPE_CODES>{});
+        else go(std::integral_constant<int, SLOPE_ONE>{});
     });
     ODIE_CUDA(cudaGetLastError());
     note_launch();

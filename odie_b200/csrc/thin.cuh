@@ -16,12 +16,11 @@ struct ThinArgs {
     const void* bias;
     const void* residual;
     void* y;
-    uint16_t* slope;
+    void* slope;            // null: not kept
     int activation;
     // backward
     const void* d_y;
-    const uint16_t* code;   // of the slope, or
-    const void* relu_y;     // a ReLU's output, or neither
+    const void* kept;       // the slope that forward kept; null: 1
     void* d_x;              // each null where not wanted
     void* d_weight;
     void* d_bias;

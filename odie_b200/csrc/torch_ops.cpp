@@ -212,11 +212,12 @@ Tensor linear_forward(const Tensor& x, const Tensor& weight, const Tensor& bias,
     const c10::cuda::CUDAGuard guard(x.device());
     const Sizes s(x, weight);
     Tensor y = rows_like(x, {s.rows, s.outputs});
-    if (keep_slope) slope = at::empty({s.rows, s.outputs}, x.options().dtype(at::kShort).requires_grad(false));
+    if (keep_slope)  // a ReLU's as bits
+        slope = activation == 1 ? at::empty({s.rows, (s.outputs + 7) / 8}, x.options().dtype(at::kByte).requires_grad(false))
+                                : at::empty({s.rows, s.outputs}, x.options().dtype(at::kShort).requires_grad(false));
     const Tensor work = scratch(x, odie_linear_scratch(s.rows, int(s.inputs), int(s.outputs), int(s.groups)));
     done(odie_linear(data(x), data(weight), data(bias), data(residual), s.rows, int(s.inputs), int(s.outputs), int(s.groups),
-                     static_cast<const int32_t*>(data(offsets)), row_type(x), int(activation), data(y), static_cast<uint16_t*>(data(slope)),
-                     data(work), stream_of(x)),
+                     static_cast<const int32_t*>(data(offsets)), row_type(x), int(activation), data(y), data(slope), data(work), stream_of(x)),
          "odie_linear");
     return y;
 }
@@ -226,20 +227,20 @@ struct Linear : torch::autograd::Function<Linear> {
     static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const Maybe& maybe_bias, const Maybe& maybe_residual,
                           const Maybe& maybe_offsets, int64_t activation, int64_t need) {
         const Tensor bias = present(maybe_bias), residual = present(maybe_residual), offsets = present(maybe_offsets);
-        const bool sums = need & 7;
-        // a ReLU's slope is the sign of its output, unless a residual hides it
-        const bool sign = activation == 1 && !residual.defined() && sums;
         Tensor slope;
-        Tensor y = linear_forward(x, weight, bias, residual, offsets, activation, sums && activation != 0 && !sign, slope);
-        ctx->save_for_backward({need & 2 ? x : Tensor(), need & 1 ? weight : Tensor(), slope, sign ? y : Tensor(), offsets});
+        Tensor y = linear_forward(x, weight, bias, residual, offsets, activation, (need & 7) && activation != 0, slope);
+        ctx->save_for_backward({need & 2 ? x : Tensor(), need & 1 ? weight : Tensor(), slope, offsets});
         ctx->saved_data["need"] = need;
+        ctx->saved_data["activation"] = activation;
         ctx->saved_data["inputs"] = x.size(1);
         ctx->saved_data["weight"] = weight.sizes().vec();
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list gradients) {
         const auto saved = ctx->get_saved_variables();
-        const Tensor &x = saved[0], &weight = saved[1], &slope = saved[2], &relu_y = saved[3], &offsets = saved[4];
+        const Tensor &x = saved[0], &weight = saved[1], &slope = saved[2], &offsets = saved[3];
+        // without a slope (only the residual's gradient is wanted) there is no activation to undo
+        const int64_t activation = slope.defined() ? ctx->saved_data["activation"].toInt() : 0;
         const int64_t need = ctx->saved_data["need"].toInt(), inputs = ctx->saved_data["inputs"].toInt();
         const auto shape = ctx->saved_data["weight"].toIntVector();
         const int64_t groups = shape.size() == 3 ? shape[0] : 1, outputs = shape[shape.size() - 2];
@@ -253,13 +254,13 @@ struct Linear : torch::autograd::Function<Linear> {
         if (need & 8) d_residual = offsets.defined() ? rows_like(d_y, {rows, outputs}) : d_y;  // every row is a group's row
         if ((need & 7) || (need & 8 && offsets.defined())) {
             const Tensor work = scratch(d_y, odie_linear_backward_scratch(rows, int(inputs), int(outputs), int(groups)));
-            done(odie_linear_backward(data(d_y), static_cast<const uint16_t*>(data(slope)), data(relu_y), data(x), data(weight), rows,
+            done(odie_linear_backward(data(d_y), data(slope), int(activation), data(x), data(weight), rows,
                                       int(inputs), int(outputs), int(groups), static_cast<const int32_t*>(data(offsets)), row_type(d_y),
                                       data(d_x), data(d_weight), data(d_bias), offsets.defined() ? data(d_residual) : nullptr, data(work),
                                       stream_of(d_y)),
                  "odie_linear_backward");
         }
-        return once({d_x, d_weight, d_bias, d_residual, Tensor(), Tensor(), Tensor()}, {gradients[0], x, weight, relu_y});
+        return once({d_x, d_weight, d_bias, d_residual, Tensor(), Tensor(), Tensor()}, {gradients[0], x, weight});
     }
 };
 

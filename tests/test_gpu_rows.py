@@ -252,6 +252,64 @@ def test_linear_infinities_and_nan_pass_through(cuda):
     assert d.isnan().all()  # the kept slope holds NaN
 
 
+def passing(x, weight, **kwargs):
+    """[rows, outputs] bool: where linear's ReLU passes a gradient, one output at a time: d x is then a row of W or 0."""
+    from odie_b200.experts import linear
+    x = x.clone().requires_grad_()
+    y = linear(x, weight, activation='relu', **kwargs)
+    found = torch.empty(y.shape, dtype=torch.bool, device=y.device)
+    for n in range(y.shape[1]):
+        d_y = torch.zeros_like(y)
+        d_y[:, n] = 1
+        (d_x,) = torch.autograd.grad(y, x, d_y, retain_graph=True)
+        found[:, n] = (d_x != 0).any(1)
+    return found
+
+
+@pytest.mark.parametrize('rows, inputs, outputs', [(1, 64, 128), (2, 5000, 33), (2, 40, 21), (17, 40, 72), (5, 333, 35), (40, 2048, 24), (300, 72, 264),
+                                                   (3, 24, 32), (333, 64, 40), (200, 24, 8)])
+@pytest.mark.parametrize('residual', [False, True])
+def test_linear_relu_of_sums_too_small_for_y(cuda, rows, inputs, outputs, residual):
+    """A ReLU is on where its fp32 sum is above zero, also where y holds 0 for it, or a residual hides it."""
+    g = generator(rows + inputs + outputs)
+    signs = torch.randint(-1, 2, (outputs, inputs), generator=g, device=cuda)
+    signs[:, 0] += signs[:, 0] == 0  # (no row of W is zero)
+    at = torch.randint(inputs, (rows,), generator=g, device=cuda)
+    x = torch.zeros(rows, inputs, device=cuda, dtype=torch.float16)
+    x[torch.arange(rows, device=cuda), at] = 2 ** -13
+    r = normal(g, rows, outputs).half() if residual else None
+    found = passing(x, signs * torch.tensor(2 ** -13, device=cuda, dtype=torch.float16), residual=r)  # sums of 2^-26, 0 and -2^-26
+    assert torch.equal(found, signs.t()[at] > 0)
+
+
+@pytest.mark.parametrize('rows, inputs, outputs', [(2000, 32, 64), (333, 64, 40), (500, 24, 8), (1, 32, 16), (900, 64, 64)])
+@pytest.mark.parametrize('dtype', HALVES)
+def test_thin_relu_at_its_corner(cuda, rows, inputs, outputs, dtype):
+    """Sums that cancel to the last bits: a layer of up to 64 inputs and outputs is on where the fp32 chain in ascending
+    order of the inputs is above zero.  (The products of 16-bit values are exact in fp32, so a rounded product and sum
+    are the fused step.)"""
+    g = generator(rows + inputs)
+    x, w = normal(g, rows, inputs, dtype=dtype), normal(g, outputs, inputs, std=0.3, dtype=dtype)
+    for level in range(3):  # the last inputs cancel the sum of output 0 to 2^-24 of it
+        k = inputs - 3 + level
+        w[0, k] = 2.0 ** (-8 * level)
+        x[:, k] = (-(x[:, :k].double() @ w[0, :k].double()) * 2.0 ** (8 * level)).to(dtype)
+    chain = torch.zeros(rows, outputs, device=cuda)
+    for k in range(inputs):
+        chain = chain + x[:, k:k + 1].float() * w[:, k].float()
+    assert torch.equal(passing(x, w), chain > 0)
+
+
+@pytest.mark.parametrize('rows, inputs, outputs', [(1, 64, 16), (20, 72, 16), (20, 32, 16)])
+def test_linear_relu_passes_gradients_of_nan(cuda, rows, inputs, outputs):
+    """A NaN sum is not <= 0: its gradient passes, as torch.relu's does."""
+    g = generator(rows)
+    x, w = normal(g, rows, inputs).half(), normal(g, outputs, inputs).half()
+    x[0, 3] = float('nan')
+    found = passing(x, w)
+    assert found[0].all() and torch.equal(found[1:], x[1:].double() @ w.double().t() > 0)
+
+
 def test_linear_shapes_and_strides(cuda):
     """Leading dimensions, no rows, transposed and misaligned operands, broadcast residual, expanded gradients."""
     from odie_b200.experts import linear

@@ -85,10 +85,10 @@ def test_linear_refuses(lib, change, message):
     assert message in _lib.error()
 
 
-@pytest.mark.parametrize('change, message', LINEAR + [(dict(d_y=None), 'required'), (dict(slope=SOME, relu_y=SOME), 'exclude'),
+@pytest.mark.parametrize('change, message', LINEAR + [(dict(d_y=None), 'required'), (dict(activation=1), 'slope'), (dict(activation=5), 'activation'),
                                                       (dict(scratch=ctypes.c_void_p(16)), '256-byte')])
 def test_linear_backward_refuses(lib, change, message):
-    a = dict(d_y=SOME, slope=None, relu_y=None, x=SOME, weight=SOME, rows=8, inputs=8, outputs=8, groups=1, offsets=None, dtype=0,
+    a = dict(d_y=SOME, slope=None, activation=0, x=SOME, weight=SOME, rows=8, inputs=8, outputs=8, groups=1, offsets=None, dtype=0,
              d_x=SOME, d_weight=SOME, d_bias=None, d_residual=None, scratch=SOME, stream=0)
     a.update(change)
     assert lib.odie_linear_backward(*a.values()) == -1
