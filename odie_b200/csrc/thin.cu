@@ -23,7 +23,7 @@
 namespace odie {
 namespace {
 
-constexpr int THREADS = 128, WARPS = 4;
+constexpr int THREADS = 128, WARPS = 4, STEP = WARPS * 16;
 // Steps of 16 rows per warp, one in work, the others on their way; two blocks share an SM in the backward pass (three
 // with three stages each took 4 % longer).
 constexpr int FORWARD_STAGES = 4;
@@ -46,13 +46,20 @@ __device__ __forceinline__ uint32_t turned(uint32_t v) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
+// Byte 0's sign over the lower half, byte 2's over the upper.
+__device__ __forceinline__ uint32_t signs_of_bytes_0_2(uint32_t v) {
+    uint32_t r;
+    asm("prmt.b32 %0, %1, 0, 0xaa88;" : "=r"(r) : "r"(v));
+    return r;
+}
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
 // Copies ahead: a lane's own 16-byte words, in shared memory slots that only it reads, so that rows are on their way
 // without holding registers.  A copy that is off writes zeros.
-__device__ __forceinline__ void copy_ahead(uint4* slot, const void* base, long long row, int width, int column, bool on) {
-    const uint16_t* from = static_cast<const uint16_t*>(base) + (on ? row * width + column : 0);
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(uint32_t(__cvta_generic_to_shared(slot))), "l"(from), "r"(on ? 16 : 0) : "memory");
+__device__ __forceinline__ void copy_ahead(uint4* slot, const uint16_t* from, bool on, const void* base) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(uint32_t(__cvta_generic_to_shared(slot))),
+                 "l"(on ? static_cast<const void*>(from) : base), "r"(on ? 16 : 0)
+                 : "memory");
 }
 __device__ __forceinline__ void copies_end() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int LEFT>
@@ -93,6 +100,29 @@ __device__ __forceinline__ float chain(const void* x, const void* w, int count) 
         }
     }
     return sum;
+}
+
+// A ReLU's bits in memory: lane (g, c) holds a byte per (h, nb), columns 32 nb + 8 c .. of row g + 8 h, as byte h NB + nb
+// of a word; turned among the row's four lanes, lane c has the four bytes of the c-th (h, nb), one word of the mask.
+__device__ __forceinline__ uint32_t turned_bytes(uint32_t v, int c) {
+    uint32_t other = __shfl_xor_sync(0xffffffffu, v, 1);
+    v = c & 1 ? __byte_perm(other, v, 0x7351) : __byte_perm(v, other, 0x6240);  // bytes (mine, theirs) of even or odd places
+    other = __shfl_xor_sync(0xffffffffu, v, 2);
+    return c & 2 ? __byte_perm(other, v, 0x7632) : __byte_perm(v, other, 0x5410);
+}
+
+// max(v, 0) of two packed values, NaN for NaN, +0 for -0.
+template <typename T>
+__device__ __forceinline__ uint32_t above_zero(uint32_t v) {
+    uint32_t r;
+    if constexpr (std::is_same<T, __half>::value) asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(0));
+    else asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(v), "r"(0));
+    return r;
+}
+__device__ __forceinline__ float least_magnitude(float a, float b, float c) {
+    float r;
+    asm("min.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
 }
 
 // KB, NB: blocks of 32 inputs and outputs.
@@ -156,34 +186,45 @@ __global__ void __launch_bounds__(THREADS, KB * NB == 4 ? 3 : 4) thin_forward_ke
     }
     extern __shared__ uint4 slots[];
     uint4* mine = slots + warp * (FORWARD_STAGES * VECTORS * 32) + lane;
-    auto ahead = [&](int step) {
-        const long long r0 = u.from + warp * 16 + (long long)step * WARPS * 16;
-        uint4* to = mine + step % FORWARD_STAGES * (VECTORS * 32);
+    const long long row0 = u.from + warp * 16 + g;
+    int left = int(u.to - row0);     // rows from the lane's first row of this step on: row 8 h is there if left > 8 h
+    int left_ahead = left, fill = 0;  // of the step that is fetched, its slot
+    const uint16_t* x_ahead = static_cast<const uint16_t*>(a.x) + row0 * a.inputs + c * 8;
+    uint16_t* y = static_cast<uint16_t*>(a.y) + row0 * a.outputs + c * 8;
+    auto ahead = [&]() {
+        uint4* to = mine + fill * (VECTORS * 32);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const long long row = r0 + g + 8 * h;
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
-                copy_ahead(to + (kb * 2 + h) * 32, a.x, row, a.inputs, kb * 32 + c * 8, row < u.to && kb * 32 + c * 8 < a.inputs);
+                copy_ahead(to + (kb * 2 + h) * 32, x_ahead + 8 * h * a.inputs + kb * 32, left_ahead > 8 * h && kb * 32 + c * 8 < a.inputs, a.x);
+            if (a.residual) {
+                const uint16_t* residual_ahead = static_cast<const uint16_t*>(a.residual) + (u.to - left_ahead) * a.outputs + c * 8;
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb)
-                if (a.residual)
-                    copy_ahead(to + (KB * 2 + nb * 2 + h) * 32, a.residual, row, a.outputs, nb * 32 + c * 8,
-                               row < u.to && nb * 32 + c * 8 < a.outputs);
+                for (int nb = 0; nb < NB; ++nb)
+                    copy_ahead(to + (KB * 2 + nb * 2 + h) * 32, residual_ahead + 8 * h * a.outputs + nb * 32,
+                               left_ahead > 8 * h && nb * 32 + c * 8 < a.outputs, a.residual);
+            }
         }
         copies_end();
+        x_ahead += STEP * a.inputs;
+        left_ahead -= STEP;
+        fill = fill + 1 == FORWARD_STAGES ? 0 : fill + 1;
     };
-    for (int s = 0; s < FORWARD_STAGES - 1; ++s) ahead(s);
-    int step = 0;
-    for (long long r0 = u.from + warp * 16; r0 < u.to; r0 += WARPS * 16, ++step) {
-        ahead(step + FORWARD_STAGES - 1);
+    for (int s = 0; s < FORWARD_STAGES - 1; ++s) ahead();
+    const bool words = reinterpret_cast<uintptr_t>(a.slope) % 4 == 0;
+    int use = 0;
+    for (int from = warp * 16; from < u.to - u.from; from += STEP, left -= STEP, y += STEP * a.outputs) {
+        ahead();
         copies_wait<FORWARD_STAGES - 1>();
-        const uint4* now = mine + step % FORWARD_STAGES * (VECTORS * 32);
+        const uint4* now = mine + use * (VECTORS * 32);
+        use = use + 1 == FORWARD_STAGES ? 0 : use + 1;
         uint4 x[KB][2];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) x[kb][h] = now[(kb * 2 + h) * 32];
+        uint32_t on = 0;    // ReLU: a byte per (h, nb)
         float near = 0.0f;  // for both rows of the lane
         if (ACT == ACT_RELU) {
             uint32_t largest = larger<T>(larger<T>(0, x[0][0]), x[0][1]);
@@ -216,41 +257,71 @@ __global__ void __launch_bounds__(THREADS, KB * NB == 4 ? 3 : 4) thin_forward_ke
             if (ACT == ACT_RELU) {
                 float least = fabsf(d[0][0]);
 #pragma unroll
-                for (int e = 1; e < 16; ++e) least = fminf(least, fabsf(d[e / 4][e % 4]));
-                if (least < near) {
+                for (int e = 2; e < 16; e += 2) least = least_magnitude(least, d[e / 4][e % 4], d[e / 4][e % 4 + 1]);
+                least = fminf(least, fabsf(d[0][1]));
+                if (least <= near) {
                     uint32_t which = 0;
 #pragma unroll
-                    for (int e = 0; e < 16; ++e)
-                        which |= fabsf(d[e / 4][e % 4]) < near && inside && r0 + g + (e % 4 / 2) * 8 < u.to ? 1u << e : 0u;
+                    for (int e = 0; e < 16; ++e) which |= fabsf(d[e / 4][e % 4]) < near && inside && left > (e % 4 / 2) * 8 ? 1u << e : 0u;
 #pragma unroll 1
                     for (; which; which &= which - 1) {
                         const int at = __ffs(which) - 1, n = column + at / 4 * 2 + at % 2;
-                        const long long row = r0 + g + (at % 4 / 2) * 8;
+                        const long long row = u.from + from + g + (at % 4 / 2) * 8;
                         const float z = chain<T>(static_cast<const uint16_t*>(a.x) + row * a.inputs, weight + n * a.inputs, a.inputs) +
                                         (a.bias ? to_float(static_cast<const T*>(a.bias)[(long long)u.g * a.outputs + n]) : 0.0f);
 #pragma unroll
                         for (int e = 0; e < 16; ++e) d[e / 4][e % 4] = at == e ? z : d[e / 4][e % 4];
                     }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) d[e / 4][e % 4] = d[e / 4][e % 4] == 0.0f ? -0x1p-149f : d[e / 4][e % 4];
                 }
             }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const long long row = r0 + g + 8 * h;
-                uint32_t y[4], codes[4], off = 0;
+                const bool there = left > 8 * h && inside;
+                const int at = 8 * h * a.outputs + nb * 32;
+                uint32_t out[4], codes[4], off = 0;
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float2 f = a.residual ? unpack_pair<T>(word(r[h], j)) : make_float2(0.0f, 0.0f);
-                    Pair slope, z = activate<ACT, true>(pair(d[j][2 * h], d[j][2 * h + 1]), slope, pair(f.x, f.y));
-                    y[j] = pack_pair<T>(both(z).x, both(z).y);
-                    if (ACT == ACT_RELU) off = off_bits(off, d[3 - j][2 * h], d[3 - j][2 * h + 1]);
-                    else if (a.slope) codes[j] = slope_codes(slope);
+                    if (ACT == ACT_RELU) {  // the packed sums' signs say where it is off (a zero is negative by now)
+                        const uint32_t z = pack_pair<T>(d[j][2 * h], d[j][2 * h + 1]);
+                        off |= z >> (15 - 2 * j) & (0x10001u << (2 * j));
+                        out[j] = above_zero<T>(z);
+                    } else {
+                        const float2 f = a.residual ? unpack_pair<T>(word(r[h], j)) : make_float2(0.0f, 0.0f);
+                        Pair slope;
+                        const float2 v = both(activate<ACT, true>(pair(d[j][2 * h], d[j][2 * h + 1]), slope, pair(f.x, f.y)));
+                        out[j] = pack_pair<T>(v.x, v.y);
+                        if (a.slope) codes[j] = slope_codes(slope);
+                    }
                 }
-                if (row < u.to && inside) {
-                    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.y) + row * a.outputs + column) = make_uint4(y[0], y[1], y[2], y[3]);
-                    if (ACT == ACT_RELU && a.slope)
-                        static_cast<uint8_t*>(a.slope)[(row * a.outputs + column) / 8] = uint8_t(~off);
-                    else if (a.slope)
-                        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.slope) + row * a.outputs + column) = make_uint4(codes[0], codes[1], codes[2], codes[3]);
+                if (ACT == ACT_RELU && a.residual) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 f = unpack_pair<T>(word(r[h], j));
+                        out[j] = pack_pair<T>(max_nan(d[j][2 * h], 0.0f) + f.x, max_nan(d[j][2 * h + 1], 0.0f) + f.y);
+                    }
+                }
+                if (ACT == ACT_RELU) on |= (~(off | off >> 15) & 0xffu) << ((h * NB + nb) * 8);
+                if (there) {
+                    *reinterpret_cast<uint4*>(y + at) = make_uint4(out[0], out[1], out[2], out[3]);
+                    if (ACT != ACT_RELU && a.slope)
+                        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.slope) + (y + at - static_cast<uint16_t*>(a.y))) =
+                            make_uint4(codes[0], codes[1], codes[2], codes[3]);
+                }
+            }
+        }
+        if (ACT == ACT_RELU && a.slope) {
+            on = turned_bytes(on, c);
+            const int h = c / NB, nb = c % NB, pitch = a.outputs / 8;
+            if (h < 2 && left > 8 * h) {
+                uint8_t* to = static_cast<uint8_t*>(a.slope) + (u.to - left + 8 * h) * pitch + nb * 4;
+                if (pitch % 4 == 0 && words) {
+                    *reinterpret_cast<uint32_t*>(to) = on;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (nb * 4 + i < pitch) to[i] = uint8_t(on >> (8 * i));
                 }
             }
         }
@@ -295,102 +366,125 @@ __global__ void __launch_bounds__(THREADS, 2) thin_backward_kernel(ThinArgs a) {
     for (int i = threadIdx.x; i < NB * 32 * (KB * 32 + 1); i += THREADS) (&sums[0][0])[i] = 0.0f;
     for (int i = threadIdx.x; i < NB * 32; i += THREADS) bias_sums[i] = 0.0f;
     __syncthreads();
-    float dw[NB * 2][KB * 4][4], db[NB][8];
+    // d b: with codes the lanes' sums of the unrounded dz (db); else dz is exact, and a product with ones sums it (ones)
+    constexpr bool BY_ONES = KIND != SLOPE_CODES;
+    constexpr uint32_t ONES = std::is_same<T, __half>::value ? 0x3c003c00u : 0x3f803f80u;
+    float dw[NB * 2][KB * 4][4], ones[NB * 2][4], db[NB][8];
 #pragma unroll
     for (int m = 0; m < NB * 2; ++m)
 #pragma unroll
-        for (int n = 0; n < KB * 4; ++n)
+        for (int i = 0; i < 4; ++i) {
+            ones[m][i] = 0.0f;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) dw[m][n][i] = 0.0f;
+            for (int n = 0; n < KB * 4; ++n) dw[m][n][i] = 0.0f;
+        }
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int e = 0; e < 8; ++e) db[nb][e] = 0.0f;
     uint4* mine = slots + warp * (BACKWARD_STAGES * VECTORS * 32) + lane;
-    auto ahead = [&](int step) {
-        const long long r0 = u.from + warp * 16 + (long long)step * WARPS * 16;
-        uint4* to = mine + step % BACKWARD_STAGES * (VECTORS * 32);
+    const long long row0 = u.from + warp * 16 + g;
+    int left = int(u.to - row0);      // row 8 h of this step is there if left > 8 h
+    int left_ahead = left, fill = 0;  // of the step that is fetched, its slot
+    const uint16_t* d_y_ahead = static_cast<const uint16_t*>(a.d_y) + row0 * a.outputs + c * 8;
+    const uint16_t* x_ahead = static_cast<const uint16_t*>(a.x) + row0 * a.inputs + c * 8;
+    const long long codes_from_d_y = static_cast<const uint16_t*>(a.kept) - static_cast<const uint16_t*>(a.d_y);
+    uint16_t* d_x = static_cast<uint16_t*>(a.d_x) + row0 * a.inputs + c * 8;
+    uint16_t* d_residual = static_cast<uint16_t*>(a.d_residual) + row0 * a.outputs + c * 8;
+    auto ahead = [&]() {
+        uint4* to = mine + fill * (VECTORS * 32);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const long long row = r0 + g + 8 * h;
-            const bool on = row < u.to;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-                const int column = nb * 32 + c * 8;
-                copy_ahead(to + (nb * 2 + h) * 32, a.d_y, row, a.outputs, column, on && column < a.outputs);
-                if (KIND == SLOPE_CODES) copy_ahead(to + (NB * 2 + nb * 2 + h) * 32, a.kept, row, a.outputs, column, on && column < a.outputs);
+                const bool on = left_ahead > 8 * h && nb * 32 + c * 8 < a.outputs;
+                const uint16_t* from = d_y_ahead + 8 * h * a.outputs + nb * 32;
+                copy_ahead(to + (nb * 2 + h) * 32, from, on, a.d_y);
+                if (KIND == SLOPE_CODES) copy_ahead(to + (NB * 2 + nb * 2 + h) * 32, from + codes_from_d_y, on, a.kept);
             }
+            if (a.d_weight) {
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-                const int column = kb * 32 + c * 8;
-                if (a.d_weight) copy_ahead(to + (AT_X + kb * 2 + h) * 32, a.x, row, a.inputs, column, on && column < a.inputs);
+                for (int kb = 0; kb < KB; ++kb)
+                    copy_ahead(to + (AT_X + kb * 2 + h) * 32, x_ahead + 8 * h * a.inputs + kb * 32, left_ahead > 8 * h && kb * 32 + c * 8 < a.inputs, a.x);
             }
         }
         copies_end();
+        d_y_ahead += STEP * a.outputs;
+        x_ahead += STEP * a.inputs;
+        left_ahead -= STEP;
+        fill = fill + 1 == BACKWARD_STAGES ? 0 : fill + 1;
     };
-    for (int s = 0; s < BACKWARD_STAGES - 1; ++s) ahead(s);
+    for (int s = 0; s < BACKWARD_STAGES - 1; ++s) ahead();
     // the mask's bytes, a step ahead
-    uint32_t next[NB][2];
-    auto masks = [&](long long r0) {
+    uint32_t next = 0;
+    const bool words = reinterpret_cast<uintptr_t>(a.kept) % 4 == 0;
+    auto masks = [&](int left) {
+        const int h = c / NB, nb = c % NB, pitch = a.outputs / 8;
+        next = 0;
+        if (h < 2 && left > 8 * h) {
+            const uint8_t* from = static_cast<const uint8_t*>(a.kept) + (u.to - left + 8 * h) * pitch + nb * 4;
+            if (pitch % 4 == 0 && words) {
+                next = __ldg(reinterpret_cast<const uint32_t*>(from));
+            } else {
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const long long row = r0 + g + 8 * h;
-                const int column = nb * 32 + c * 8;
-                next[nb][h] = row < u.to && column < a.outputs ? __ldg(static_cast<const uint8_t*>(a.kept) + (row * a.outputs + column) / 8) : 0;
+                for (int i = 0; i < 4; ++i)
+                    if (nb * 4 + i < pitch) next |= uint32_t(__ldg(from + i)) << (8 * i);
             }
+        }
     };
-    if (KIND == SLOPE_MASK) masks(u.from + warp * 16);
-    int step = 0;
-    for (long long r0 = u.from + warp * 16; r0 < u.to; r0 += WARPS * 16, ++step) {
+    if (KIND == SLOPE_MASK) masks(left);
+    int use = 0;
+    for (int from = warp * 16; from < u.to - u.from; from += STEP, left -= STEP) {
         uint32_t bits[NB][2];
         if (KIND == SLOPE_MASK) {
+            const uint32_t on = turned_bytes(next, c);
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-                for (int h = 0; h < 2; ++h) bits[nb][h] = next[nb][h];
-            masks(r0 + WARPS * 16);
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t byte = on >> ((h * NB + nb) * 8) & 0xffu;
+                    bits[nb][h] = byte | byte << 15;
+                }
+            masks(left - STEP);
         }
-        ahead(step + BACKWARD_STAGES - 1);
+        ahead();
         copies_wait<BACKWARD_STAGES - 1>();
-        const uint4* now = mine + step % BACKWARD_STAGES * (VECTORS * 32);
-        uint4 z[NB][2], s[NB][2], x[KB][2];
+        const uint4* now = mine + use * (VECTORS * 32);
+        use = use + 1 == BACKWARD_STAGES ? 0 : use + 1;
+        uint4 z[NB][2], x[KB][2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                z[nb][h] = now[(nb * 2 + h) * 32];
-                if (KIND == SLOPE_CODES) s[nb][h] = now[(NB * 2 + nb * 2 + h) * 32];
-            }
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) x[kb][h] = a.d_weight ? now[(AT_X + kb * 2 + h) * 32] : make_uint4(0, 0, 0, 0);
-        }
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const long long row = r0 + g + 8 * h;
-                if (a.d_residual && row < u.to && nb * 32 + c * 8 < a.outputs)
-                    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.d_residual) + row * a.outputs + nb * 32 + c * 8) = z[nb][h];
+                z[nb][h] = now[(nb * 2 + h) * 32];
+                if (a.d_residual && left > 8 * h && nb * 32 + c * 8 < a.outputs)
+                    *reinterpret_cast<uint4*>(d_residual + 8 * h * a.outputs + nb * 32) = z[nb][h];
                 uint32_t q[4];
+                if (KIND == SLOPE_CODES) {
+                    const uint4 s = now[(NB * 2 + nb * 2 + h) * 32];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float2 f = unpack_pair<T>(word(z[nb][h], i));
-                    if (KIND == SLOPE_CODES) {
-                        const uint32_t k = word(s[nb][h], i);
-                        f.x *= slope_value(k & 0xffffu);
-                        f.y *= slope_value(k >> 16);
-                    } else if (KIND == SLOPE_MASK) {
-                        f.x = bits[nb][h] >> (2 * i) & 1 ? f.x : 0.0f;
-                        f.y = bits[nb][h] >> (2 * i + 1) & 1 ? f.y : 0.0f;
+                    for (int i = 0; i < 4; ++i) {
+                        float2 f = unpack_pair<T>(word(z[nb][h], i));
+                        f.x *= slope_value(word(s, i) & 0xffffu);
+                        f.y *= slope_value(word(s, i) >> 16);
+                        db[nb][2 * i] += f.x;
+                        db[nb][2 * i + 1] += f.y;
+                        q[i] = pack_pair<T>(f.x, f.y);
                     }
-                    db[nb][2 * i] += f.x;
-                    db[nb][2 * i + 1] += f.y;
-                    q[i] = pack_pair<T>(f.x, f.y);
+                    z[nb][h] = make_uint4(q[0], q[1], q[2], q[3]);
+                } else if (KIND == SLOPE_MASK) {
+                    // bit 2 i to the sign of byte 0, bit 2 i + 1 (its copy 15 above) to that of byte 2, and over their halves
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        q[i] = word(z[nb][h], i) & signs_of_bytes_0_2(bits[nb][h] << (7 - 2 * i));
+                    z[nb][h] = make_uint4(q[0], q[1], q[2], q[3]);
                 }
-                z[nb][h] = make_uint4(q[0], q[1], q[2], q[3]);
             }
+        d_residual += STEP * a.outputs;
         if (a.d_x) {
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) {
@@ -410,16 +504,15 @@ __global__ void __launch_bounds__(THREADS, 2) thin_backward_kernel(ThinArgs a) {
                 }
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const long long row = r0 + g + 8 * h;
-                    const int column = kb * 32 + c * 8;
-                    if (row < u.to && column < a.inputs)
-                        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.d_x) + row * a.inputs + column) =
+                    if (left > 8 * h && kb * 32 + c * 8 < a.inputs)
+                        *reinterpret_cast<uint4*>(d_x + 8 * h * a.inputs + kb * 32) =
                             make_uint4(pack_pair<T>(d[0][2 * h], d[0][2 * h + 1]), pack_pair<T>(d[1][2 * h], d[1][2 * h + 1]),
                                        pack_pair<T>(d[2][2 * h], d[2][2 * h + 1]), pack_pair<T>(d[3][2 * h], d[3][2 * h + 1]));
                 }
             }
         }
-        if (a.d_weight) {
+        d_x += STEP * a.inputs;
+        if (a.d_weight || (BY_ONES && a.d_bias)) {
             uint32_t xt[KB][4][2];
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
@@ -434,6 +527,7 @@ __global__ void __launch_bounds__(THREADS, 2) thin_backward_kernel(ThinArgs a) {
                 const uint32_t a2 = turned(word(z[nb][1], 2 * p)), a3 = turned(word(z[nb][1], 2 * p + 1));
 #pragma unroll
                 for (int n = 0; n < KB * 4; ++n) mma16816<T>(dw[m][n], a0, a1, a2, a3, xt[n / 4][n % 4][0], xt[n / 4][n % 4][1]);
+                if (BY_ONES) mma16816<T>(ones[m], a0, a1, a2, a3, ONES, ONES);
             }
         }
     }
@@ -456,7 +550,13 @@ __global__ void __launch_bounds__(THREADS, 2) thin_backward_kernel(ThinArgs a) {
                         const int out = (m / 2) * 32 + (g >> 1) * 8 + (2 * (m % 2) + (i >> 1)) * 2 + (g & 1);
                         sums[out][(n / 4) * 32 + c * 8 + (n % 4) * 2 + (i & 1)] += dw[m][n][i];
                     }
-            if (g == 0) {
+            if (BY_ONES && c == 0) {
+#pragma unroll
+                for (int m = 0; m < NB * 2; ++m)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) bias_sums[(m / 2) * 32 + (g >> 1) * 8 + (2 * (m % 2) + i) * 2 + (g & 1)] += ones[m][2 * i];
+            }
+            if (!BY_ONES && g == 0) {
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
