@@ -1248,7 +1248,7 @@ struct BackwardScratch {
         bytes = s.used;
         thin = static_cast<float*>(base);  // thin layers need nothing else
         if (thin_sizes(inputs, outputs))
-            bytes = std::max(bytes, aligned(thin_units(rows, groups, thin_chunk(rows, inputs, outputs, true)) * (int64_t(outputs) * inputs + outputs) * 4));
+            bytes = std::max(bytes, aligned(thin_units(rows, groups, thin_chunk(rows, inputs, outputs, ACT_NONE, true)) * (int64_t(outputs) * inputs + outputs) * 4));
     }
 };
 
@@ -1287,7 +1287,7 @@ extern "C" int odie_linear(const void* x, const void* weight, const void* bias, 
             a.outputs = outputs;
             a.groups = groups;
             a.offsets = offsets;
-            a.chunk = thin_chunk(rows, inputs, outputs, false);
+            a.chunk = thin_chunk(rows, inputs, outputs, activation, false);
             a.x = x;
             a.weight = weight;
             a.bias = bias;
@@ -1353,7 +1353,7 @@ extern "C" int odie_linear_backward(const void* d_y, const void* slope, int acti
             a.outputs = outputs;
             a.groups = groups;
             a.offsets = offsets;
-            a.chunk = thin_chunk(rows, inputs, outputs, true);
+            a.chunk = thin_chunk(rows, inputs, outputs, ACT_NONE, true);
             a.x = x;
             a.weight = weight;
             a.d_y = d_y;

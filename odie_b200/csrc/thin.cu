@@ -127,7 +127,7 @@ __device__ __forceinline__ float least_magnitude(float a, float b, float c) {
 
 // KB, NB: blocks of 32 inputs and outputs.
 template <typename T, int KB, int NB, int ACT>
-__global__ void __launch_bounds__(THREADS, KB * NB == 4 ? 3 : 4) thin_forward_kernel(ThinArgs a) {
+__global__ void __launch_bounds__(THREADS, thin_blocks(KB * 32, NB * 32, ACT, false)) thin_forward_kernel(ThinArgs a) {
     constexpr int VECTORS = KB * 2 + NB * 2;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
     const Unit u = unit_at<false>(a.offsets, a.groups, a.rows, a.chunk, blockIdx.x);

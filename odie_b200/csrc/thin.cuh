@@ -29,11 +29,14 @@ struct ThinArgs {
 };
 
 inline bool thin_sizes(int inputs, int outputs) { return inputs <= 64 && outputs <= 64 && inputs % 8 == 0 && outputs % 8 == 0; }
-// Rows per block: as many blocks as fit the SMs at once (two per SM backward, four forward, three for more than 32
-// inputs and outputs), so that W is read and sums are written as seldom as that allows.
-inline int thin_blocks(int inputs, int outputs, bool backward) { return backward ? 2 : inputs > 32 && outputs > 32 ? 3 : 4; }
-inline int thin_chunk(int64_t rows, int inputs, int outputs, bool backward) {
-    const int64_t blocks = 148 * thin_blocks(inputs, outputs, backward), share = (rows + blocks - 1) / blocks;
+// Blocks that share an SM: as many as their registers allow without spilling (a ReLU's corner takes some: at 2^20 rows of
+// 32 -> 64 fp16 four blocks took 60 us, three 50).
+constexpr int thin_blocks(int inputs, int outputs, int activation, bool backward) {
+    return backward ? 2 : 4 - (inputs > 32 || outputs > 32) * (activation == ACT_RELU) - (inputs > 32 && outputs > 32);
+}
+// Rows per block: as many blocks as fit the SMs at once, so that W is read and sums are written as seldom as that allows.
+inline int thin_chunk(int64_t rows, int inputs, int outputs, int activation, bool backward) {
+    const int64_t blocks = 148 * thin_blocks(inputs, outputs, activation, backward), share = (rows + blocks - 1) / blocks;
     return int(std::max<int64_t>(64, (share + 63) / 64 * 64));
 }
 // Units of work (blocks) at most: every group has at least one, and rows of no group their own.
