@@ -1353,7 +1353,7 @@ extern "C" int odie_linear_backward(const void* d_y, const void* slope, int acti
             a.outputs = outputs;
             a.groups = groups;
             a.offsets = offsets;
-            a.chunk = thin_chunk(rows, inputs, outputs, ACT_NONE, true);
+            a.chunk = thin_chunk(rows, inputs, outputs, kind == SLOPE_ONE ? ACT_NONE : activation, true);
             a.x = x;
             a.weight = weight;
             a.d_y = d_y;

@@ -3,7 +3,9 @@
 // Bound by the bytes of the rows (64 to 128 bytes each), not by arithmetic: 2^20 rows of 32 -> 64 fp16 are 192 MB
 // forward against 4.3 GFLOP.  So a warp keeps its 16 rows in registers from the 16-byte loads to the 16-byte stores
 // and multiplies them with mma.sync fragments.  (The tensor-core tiles of linear.cu, whose rows pass through shared
-// memory, TMEM and a staging tile, took 102 us forward and 205 us in four kernels backward.)
+// memory, TMEM and a staging tile, took 102 us forward and 205 us in four kernels backward; these take 45 and 57 with
+// ReLU, 4.4 and 4.7 TB/s.  What is left is the issue of about 400 instructions per warp and 16 rows, at 12 to 16 warps
+// per SM.)
 //
 // The fragments' order of columns is chosen so that no data is exchanged.  Lane (g, c) = (lane / 4, lane % 4) loads
 // the 8 columns 8 c .. 8 c + 7 of rows g and g + 8 for each 32-column block: word i (columns 8 c + 2 i, + 1) is what
@@ -24,11 +26,10 @@ namespace odie {
 namespace {
 
 constexpr int THREADS = 128, WARPS = 4, STEP = WARPS * 16;
-// Steps of 16 rows per warp, one in work, the others on their way; two blocks share an SM in the backward pass (three
-// with three stages each took 4 % longer).
+// Steps of 16 rows per warp, one in work, the others on their way.
 constexpr int FORWARD_STAGES = 4;
-template <int KB, int NB>
-constexpr int STAGES_BACK = KB * NB == 4 ? 3 : 5;
+template <int KB, int NB, int KIND>
+constexpr int STAGES_BACK = KB * NB == 4 ? 3 : KIND == SLOPE_CODES ? 5 : 4;
 
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -329,8 +330,8 @@ __global__ void __launch_bounds__(THREADS, thin_blocks(KB * 32, NB * 32, ACT, fa
 }
 
 template <typename T, int KB, int NB, int KIND>
-__global__ void __launch_bounds__(THREADS, 2) thin_backward_kernel(ThinArgs a) {
-    constexpr int BACKWARD_STAGES = STAGES_BACK<KB, NB>;
+__global__ void __launch_bounds__(THREADS, thin_blocks(KB * 32, NB * 32, KIND == SLOPE_CODES ? ACT_GELU : ACT_NONE, true)) thin_backward_kernel(ThinArgs a) {
+    constexpr int BACKWARD_STAGES = STAGES_BACK<KB, NB, KIND>;
     constexpr int AT_X = NB * (KIND == SLOPE_CODES ? 4 : 2), VECTORS = AT_X + KB * 2;
     extern __shared__ uint4 slots[];
     // W by its rows' order for d x: [K-step of 16 outputs][8-column tile of inputs][lane]
@@ -615,7 +616,7 @@ void launch_thin_backward(const ThinArgs& a, cudaStream_t stream) {
         constexpr int KB = decltype(kb)::value, NB = decltype(nb)::value;
         auto go = [&](auto kind) {
             constexpr int KIND = decltype(kind)::value;
-            constexpr int BYTES = WARPS * STAGES_BACK<KB, NB> * (NB * (KIND == SLOPE_CODES ? 4 : 2) + KB * 2) * 512;
+            constexpr int BYTES = WARPS * STAGES_BACK<KB, NB, KIND> * (NB * (KIND == SLOPE_CODES ? 4 : 2) + KB * 2) * 512;
             const auto kernel = thin_backward_kernel<T, KB, NB, KIND>;
             ODIE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, BYTES));
             kernel<<<unsigned(thin_units(a.rows, a.groups, a.chunk)), THREADS, BYTES, stream>>>(a);

@@ -30,9 +30,12 @@ struct ThinArgs {
 
 inline bool thin_sizes(int inputs, int outputs) { return inputs <= 64 && outputs <= 64 && inputs % 8 == 0 && outputs % 8 == 0; }
 // Blocks that share an SM: as many as their registers allow without spilling (a ReLU's corner takes some: at 2^20 rows of
-// 32 -> 64 fp16 four blocks took 60 us, three 50).
+// 32 -> 64 fp16 four blocks took 60 us, three 50) and, backward, the rows on their way in shared memory.  Backward with
+// codes: two, with more stages each.
 constexpr int thin_blocks(int inputs, int outputs, int activation, bool backward) {
-    return backward ? 2 : 4 - (inputs > 32 || outputs > 32) * (activation == ACT_RELU) - (inputs > 32 && outputs > 32);
+    const int wide = (inputs > 32) + (outputs > 32);
+    if (backward) return activation == ACT_SILU || activation == ACT_GELU ? 2 : 4 - wide;
+    return activation == ACT_RELU ? 4 - wide : wide == 2 ? 3 : 4;
 }
 // Rows per block: as many blocks as fit the SMs at once, so that W is read and sums are written as seldom as that allows.
 inline int thin_chunk(int64_t rows, int inputs, int outputs, int activation, bool backward) {
