@@ -404,7 +404,7 @@ ODIE_API int odie_combine_backward(const void* d_out, const void* sorted, int64_
  * (may be NULL): act'(x W^T + b) for the backward pass; ReLU: one bit per
  * output, u8[rows][ceil(outputs / 8)], bit c % 8 of byte c / 8 for column c,
  * set unless the fp32 sum is <= 0; SiLU and GELU: u16[rows][outputs],
- * round(2^15 (act' + 1/4)), 65535 for NaN.
+ * round(2^15 (act' + 1/4)), 65535 for NaN; not written for activation 0.
  * odie_linear_backward: with dz = d_y act' (slope as odie_linear wrote it for
  * the same activation; not read for activation 0), rounded to
  * the rows' type for the products: d_x = dz W, d_weight = dz^T x, d_bias =

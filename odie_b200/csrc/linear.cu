@@ -1274,6 +1274,7 @@ extern "C" int odie_linear(const void* x, const void* weight, const void* bias, 
         check_linear(rows, inputs, outputs, groups, offsets, dtype, activation);
         if (rows == 0) return;
         ODIE_REQUIRE(x && weight && y, "x, weight and y are required");
+        if (activation == ACT_NONE) slope = nullptr;  // 1 everywhere
         const cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_handle);
         if (rows <= FEW_ROWS && !offsets) {
             const FewArgs a{x, weight, bias, residual, y, slope, int(rows), inputs, outputs, activation};
