@@ -25,11 +25,16 @@ struct RowArgs {
     const float* weights;
 };
 
+// Rows that a thread takes of narrow ones, or vectors of a wide one.  (2^20 rows of 32 fp16: 51 us with one row, 35 with
+// two, 41 with four, whose registers leave half the blocks; 4-byte vectors, rows of 20 fp16: 85 with two, 72 with four.)
+template <int BYTES, bool NARROW>
+constexpr int DISPATCH_ITEMS = NARROW && BYTES == 16 ? 2 : 4;
+
 // Walks the sorted rows: they are written in order, and row order[p] / choices is fetched for each.
 template <typename T, int BYTES, bool NARROW>
 __global__ void __launch_bounds__(ROW_THREADS) dispatch_kernel(RowArgs a, const T* __restrict__ rows, T* __restrict__ sorted) {
     using P = Pack<T, BYTES>;
-    constexpr int ITEMS = 4;
+    constexpr int ITEMS = DISPATCH_ITEMS<BYTES, NARROW>;
     const RowWalk<NARROW, ITEMS> walk(a.shape);
     long long row[ITEMS];
     float w[ITEMS];
@@ -58,9 +63,9 @@ __global__ void __launch_bounds__(ROW_THREADS) dispatch_kernel(RowArgs a, const 
     }
 }
 
-// Vectors of a row that a thread takes together where they are 16 bytes (1) or fewer (4: as many bytes in flight).
-template <int BYTES>
-constexpr int SCALE = BYTES == 16 ? 1 : 4;
+// Vectors of a wide row that a thread takes together where they are 16 bytes (1) or fewer (4: as many bytes in flight).
+template <int BYTES, bool NARROW = false>
+constexpr int SCALE = NARROW || BYTES == 16 ? 1 : 4;
 
 // Wide rows with several choices: walks the unsorted rows, so that each is read once however many choices it has.
 // (Walking the sorted side, rows were evicted from L2 between their choices: 16384 rows of 4 KB, four choices each,
@@ -99,7 +104,7 @@ __global__ void __launch_bounds__(ROW_THREADS) dispatch_rows_kernel(RowArgs a, c
 template <typename T, int BYTES, bool NARROW, int BATCH>
 __global__ void __launch_bounds__(ROW_THREADS) combine_kernel(RowArgs a, const T* __restrict__ sorted, T* __restrict__ out) {
     using P = Pack<T, BYTES>;
-    constexpr int ITEMS = 4 / BATCH * SCALE<BYTES>, ROWS = NARROW ? ITEMS : 1;
+    constexpr int ITEMS = 4 / BATCH * SCALE<BYTES, NARROW>, ROWS = NARROW ? ITEMS : 1;
     const RowWalk<NARROW, ITEMS> walk(a.shape);
     for (long long c = walk.lane; c < walk.vectors; c += walk.stride()) {
         float sum[ITEMS][P::N];
@@ -150,9 +155,10 @@ __global__ void __launch_bounds__(ROW_THREADS) combine_kernel(RowArgs a, const T
     }
 }
 
-// Walks the sorted rows.  The dot product's partial sums are joined in a fixed tree.
+// Walks the sorted rows.  The dot product's partial sums are joined in a fixed tree.  (2^20 rows of 32 fp16: 57 us at the
+// four blocks per SM that the compiler's registers leave, 53 at six.)
 template <typename T, int BYTES, bool NARROW>
-__global__ void __launch_bounds__(ROW_THREADS) combine_backward_kernel(RowArgs a, const T* __restrict__ d_out,
+__global__ void __launch_bounds__(ROW_THREADS, NARROW && BYTES == 16 ? 6 : 0) combine_backward_kernel(RowArgs a, const T* __restrict__ d_out,
                                                                        const T* __restrict__ sorted, T* __restrict__ d_sorted,
                                                                        float* __restrict__ d_weights) {
     using P = Pack<T, BYTES>;
@@ -303,14 +309,32 @@ void check_rows(int64_t n, int choices, int64_t width, int dtype, const int32_t*
     ODIE_REQUIRE(n == 0 || order, std::string(name) + " is required");
 }
 
+// Which rows are narrow: up to 32 vectors always; more where there are many rows and few choices, whose rows one thread
+// then reads side by side.  Measured at 2^26 halves in all, dispatch / combine / its gradient in us, narrow against wide:
+//   16 bytes  one choice, 64 vectors 49 / 55 / 74 against 78 / 100 / 90, 256: 51 / 57 / 76 against 53 / 64 / 78, 512:
+//             53 / 68 / 92 against 53 / 61 / 78; two, 64: 45 / 47 / 70 against 45 / 47 / 86; four, 64: 39 / 41 / 68
+//             against 35 / 41 / 61
+//   4 bytes   one choice, 150: 84 / 100 / 121 against 137 / 274 / 143, 501: 80 / 100 / 109 against 78 / 104 / 107; two,
+//             115: 82 / 92 / 125 against 84 / 94 / 143, 150: 78 / 92 / 117 against 100 / 78 / 150; four, 50: 104 / 80 /
+//             168 against 121 / 119 / 152, 115: 74 / 70 / 121 against 59 / 74 / 90
+bool narrow_rows(int64_t n, int64_t vectors, int bytes, int choices) {
+    int most = 32;
+    if (n * choices >= MANY_ROWS) {
+        if (bytes == 16) most = choices <= 2 ? 256 : 32;
+        else most = choices == 1 ? 256 : choices == 2 ? 128 : 64;
+    }
+    return vectors <= most;
+}
+
 // The walk of a kernel that writes the sorted side: by rows (slot) for wide rows with several choices, by places
 // (order) for the others.
 RowArgs sorted_args(int64_t n, int choices, int64_t width, int dtype, int vector, const int32_t* order, const int32_t* slot,
                     const float* weights) {
     const int64_t vectors = width * row_type_size(dtype) / vector;
-    RowArgs a{row_shape(n * choices, vectors, vector), n * choices, choices, width, order, nullptr, weights};
+    const bool narrow = narrow_rows(n, vectors, vector, choices);
+    RowArgs a{row_shape(n * choices, vectors, vector, narrow), n * choices, choices, width, order, nullptr, weights};
     if (!a.shape.narrow && choices > 1) {
-        a.shape = row_shape(n, vectors, vector);
+        a.shape = row_shape(n, vectors, vector, narrow);
         a.order = nullptr;
         a.slot = slot;
     }
@@ -350,7 +374,7 @@ extern "C" int odie_dispatch(const void* rows, int64_t n, int choices, int64_t w
         } else with_rows(dtype, vector, a.shape.narrow, [&](auto type, auto bytes, auto narrow) {
             using T = decltype(type);
             dispatch_kernel<T, decltype(bytes)::value, decltype(narrow)::value>
-                <<<row_blocks(a.shape, 4), ROW_THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+                <<<row_blocks(a.shape, (DISPATCH_ITEMS<decltype(bytes)::value, decltype(narrow)::value>)), ROW_THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
                     a, static_cast<const T*>(rows), static_cast<T*>(sorted));
         });
         ODIE_CUDA(cudaGetLastError());
@@ -365,12 +389,13 @@ extern "C" int odie_combine(const void* sorted, int64_t n, int choices, int64_t 
         if (n == 0) return;
         ODIE_REQUIRE(sorted && out, "sorted and out are required");
         const int vector = row_vector(width, dtype, sorted, out);
-        const RowArgs a{row_shape(n, width * row_type_size(dtype) / vector, vector), n * choices, choices, width, nullptr, slot, weights};
+        const int64_t vectors = width * row_type_size(dtype) / vector;
+        const RowArgs a{row_shape(n, vectors, vector, narrow_rows(n, vectors, vector, choices)), n * choices, choices, width, nullptr, slot, weights};
         with_rows(dtype, vector, a.shape.narrow, [&](auto type, auto bytes, auto narrow) {
             using T = decltype(type);
             auto go = [&](auto batch) {
                 combine_kernel<T, decltype(bytes)::value, decltype(narrow)::value, decltype(batch)::value>
-                    <<<row_blocks(a.shape, 4 / decltype(batch)::value * SCALE<decltype(bytes)::value>), ROW_THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
+                    <<<row_blocks(a.shape, 4 / decltype(batch)::value * SCALE<decltype(bytes)::value, decltype(narrow)::value>), ROW_THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(
                         a, static_cast<const T*>(sorted), static_cast<T*>(out));
             };
             if (choices == 1) go(std::integral_constant<int, 1>{});

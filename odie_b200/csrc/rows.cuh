@@ -86,21 +86,23 @@ void with_row_type(int dtype, int vector, F&& f) {
 }
 
 // How the 256 threads of a block share rows of `vectors` vectors, so that each has several independent loads in
-// flight and neighbours read neighbouring vectors.  Narrow rows (at most 32 vectors): 2^lanes_log2 threads hold
-// one vector each of a row, and a thread takes ITEMS rows.  Wide rows: 32 to 256 threads walk a row together,
-// ITEMS vectors at a time.  item<ITEMS>(q, ..) is the thread's q-th (row, vector) of a step.
+// flight and neighbours read neighbouring vectors.  Narrow rows (as the caller says): 2^lanes_log2 threads, 32 at most,
+// take one vector each of a row at a time, and each of them ITEMS rows.  Wide rows: 32 to 256 threads walk a row
+// together, ITEMS vectors at a time.  item<ITEMS>(q, ..) is the thread's q-th (row, vector) of a step.
 constexpr int ROW_THREADS = 256;
+// Rows from which a warp or less for several of them fills the SMs.
+constexpr int64_t MANY_ROWS = 1 << 14;
 struct RowShape {
     long long rows;
     long long vectors;
     int lanes_log2;
     bool narrow;
 };
-inline RowShape row_shape(int64_t rows, int64_t vectors, int bytes) {
+inline RowShape row_shape(int64_t rows, int64_t vectors, int bytes, bool narrow) {
     const int most = bytes == 16 ? 4 : 16;  // vectors per thread of a wide row: 64 bytes
-    RowShape s{rows, vectors, 0, vectors <= 32};
+    RowShape s{rows, vectors, 0, narrow};
     if (s.narrow) {
-        while ((1 << s.lanes_log2) < vectors) ++s.lanes_log2;
+        while (s.lanes_log2 < 5 && (1 << s.lanes_log2) < vectors) ++s.lanes_log2;
     } else {
         s.lanes_log2 = 5;
         while (s.lanes_log2 < 8 && (int64_t(most) << s.lanes_log2) < vectors) ++s.lanes_log2;

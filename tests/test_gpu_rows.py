@@ -58,7 +58,9 @@ def test_sort_rows_all_dropped_and_all_equal(cuda):
 
 # ---------------------------------------------------------------- dispatch and combine
 ROWS = [(1, 1, 1, 1), (3, 2, 2, 7), (33, 1, 4, 32), (100, 3, 7, 33), (257, 2, 64, 128), (65, 4, 16, 1030), (7, 5, 9, 4104),
-        (2000, 8, 12, 24)]
+        (2000, 8, 12, 24),
+        # enough rows for a warp per several wide ones
+        (16500, 1, 16, 520), (8300, 2, 16, 300), (16400, 1, 5, 131), (5600, 3, 6, 35), (4100, 4, 9, 100), (16384, 1, 3, 2048)]
 
 
 @pytest.mark.parametrize('rows, choices, bins, width', ROWS)
@@ -440,7 +442,8 @@ def test_linear_offsets_running_backwards_stay_inside(cuda, inputs, outputs):
 
 # ---------------------------------------------------------------- embed
 EMBEDS = [(1, 1, 1), (5, 3, 7), (64, 1, 32), (300, 2, 33), (129, 1000, 128), (4096, 50, 24), (5000, 5000, 16), (70000, 3, 8),
-          (1000, 70000, 40), (200, 17, 2056), (20000, (1 << 20) + 5, 1)]
+          (1000, 70000, 40), (200, 17, 2056), (20000, (1 << 20) + 5, 1),
+          (16500, 3000, 130), (16384, 100, 520), (16384, 100, 257)]
 
 
 @pytest.mark.parametrize('count, rows, width', EMBEDS)
