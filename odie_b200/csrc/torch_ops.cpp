@@ -269,6 +269,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const Maybe& bias, const Ma
                       "x must be a CUDA fp16 or bf16 tensor with at least one column");
     TORCH_CHECK_VALUE(weight.dim() == (offsets ? 3 : 2) && weight.size(-1) == x.size(-1) && weight.numel() > 0, "weight must be [",
                       offsets ? "experts, " : "", "outputs, ", x.size(-1), "], not ", weight.sizes());
+    TORCH_CHECK_VALUE(weight.size(-1) <= (1 << 20) && weight.size(-2) <= (1 << 20), "at most 2^20 inputs and outputs");
     TORCH_CHECK_VALUE(!bias || bias->sizes() == weight.sizes().slice(0, weight.dim() - 1), "bias must be ",
                       weight.sizes().slice(0, weight.dim() - 1), ", not ", bias ? bias->sizes() : at::IntArrayRef());
     auto check = [&](const Tensor& t, const char* name) {

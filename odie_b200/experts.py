@@ -76,7 +76,8 @@ def linear(x, weight, bias=None, residual=None, activation='none', offsets=None)
     Without offsets: weight [outputs, inputs], bias [outputs].  With offsets (CUDA int32 [experts + 1], as of
     RowOrder; non-decreasing from 0): x [rows, inputs], weight [experts, outputs, inputs], bias [experts, outputs];
     rows [offsets[e], offsets[e + 1]) take expert e's layer, rows behind the last offset give zero rows (without
-    the residual).  residual: broadcastable to the result.  activation: 'none', 'relu', 'silu' or 'gelu' (erf)."""
+    the residual).  residual: broadcastable to the result.  activation: 'none', 'relu', 'silu' or 'gelu' (erf).  Up to
+    2^20 inputs and outputs, 1024 experts and 2^31 - 257 rows."""
     code = ACTIVATIONS.get(activation)
     if code is None:
         raise ValueError(f'activation must be one of {", ".join(ACTIVATIONS)}')

@@ -405,6 +405,10 @@ def test_linear_refusals(cuda):
                 dict(weight=w.cpu()), dict(x=x[None], weight=wg, offsets=off), dict(x=x[:, :0], weight=w[:, :0])):
         with pytest.raises(ValueError):
             linear(**{**dict(x=x, weight=w), **bad})
+    wide = x[:1, :1].expand(1, (1 << 32) + 8)  # 8 in 32 bits
+    for bad in (dict(x=wide, weight=wide), dict(weight=w[:1].expand((1 << 20) + 1, 8))):
+        with pytest.raises(ValueError, match='2\\^20'):
+            linear(**{**dict(x=x), **bad})
     with pytest.raises(RuntimeError):  # not broadcastable
         linear(x, w, residual=torch.zeros(3, 16, device=cuda).half())
 
