@@ -312,6 +312,38 @@ def test_linear_relu_passes_gradients_of_nan(cuda, rows, inputs, outputs):
     assert found[0].all() and torch.equal(found[1:], x[1:].double() @ w.double().t() > 0)
 
 
+@pytest.mark.parametrize('rows, inputs, outputs', [(2, 40, 21), (2, 5000, 9), (300, 72, 264), (130, 64, 67), (40, 2048, 35), (333, 64, 40), (333, 32, 64)])
+@pytest.mark.parametrize('shift', [0, 1])
+def test_linear_relu_bits(cuda, rows, inputs, outputs, shift):
+    """The C interface's slope of a ReLU: bit c % 8 of byte c / 8, at any address, read back by the gradient; nothing is
+    written around it, nor anything without an activation.  Whole numbers, so that every sum is exact."""
+    from odie_b200 import _lib
+    lib = _lib.library()
+    g = generator(rows + outputs)
+    x = torch.randint(-2, 3, (rows, inputs), generator=g, device=cuda).half()
+    w = torch.randint(-2, 3, (outputs, inputs), generator=g, device=cuda).half()
+    z = x.double() @ w.double().t()
+    pitch = (outputs + 7) // 8
+    buffer = torch.full((rows * pitch + 16,), 0xa5, dtype=torch.uint8, device=cuda)
+    y, d_x = torch.empty(rows, outputs, device=cuda).half(), torch.empty_like(x)
+    sizes = (rows, inputs, outputs, 1)
+    scratch = torch.empty(max(1, lib.odie_linear_scratch(*sizes), lib.odie_linear_backward_scratch(*sizes)), dtype=torch.uint8, device=cuda)
+    stream = torch.cuda.current_stream().cuda_stream
+    slope = buffer.data_ptr() + 8 + shift
+    for activation in (0, 1):
+        assert lib.odie_linear(x.data_ptr(), w.data_ptr(), None, None, *sizes, None, 0, activation, y.data_ptr(), slope, scratch.data_ptr(), stream) == 0
+        if activation == 0:
+            assert (buffer == 0xa5).all()
+    bits = buffer[8 + shift:8 + shift + rows * pitch].view(rows, pitch, 1) >> torch.arange(8, device=cuda, dtype=torch.uint8) & 1
+    assert torch.equal(bits.view(rows, pitch * 8)[:, :outputs].bool(), z > 0)
+    assert (buffer[:8 + shift] == 0xa5).all() and (buffer[8 + shift + rows * pitch:] == 0xa5).all()
+    d_y = torch.randint(-2, 3, (rows, outputs), generator=g, device=cuda).half()
+    assert lib.odie_linear_backward(d_y.data_ptr(), slope, 1, x.data_ptr(), w.data_ptr(), *sizes, None, 0, d_x.data_ptr(), None, None, None,
+                                    scratch.data_ptr(), stream) == 0
+    want = (d_y.double() * (z > 0)) @ w.double()
+    within(d_x, want, rounding(want, torch.float16), 'd_x')
+
+
 def test_linear_shapes_and_strides(cuda):
     """Leading dimensions, no rows, transposed and misaligned operands, broadcast residual, expanded gradients."""
     from odie_b200.experts import linear
