@@ -6,7 +6,7 @@
 //   backward   d sorted[slot] = w d out[t], d w[t, j] = <sorted[slot], d out[t]> in fp32
 // The gradient of dispatch is combine without weights.  All are bound by the bytes of the rows.  Kernels walk the
 // side that they write, so that writes are whole lines in order and only reads are scattered (writes of 64-byte rows
-// to their places took half as long again: 47 us against 31 for 2^20 rows of 32 fp16), but for wide rows with several
+// to their places took half as long again: 47 us against 27 for 2^20 rows of 32 fp16), but for wide rows with several
 // choices, whose places are whole lines anyway.
 #include "rows.cuh"
 #include "odie_b200.h"

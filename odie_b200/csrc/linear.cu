@@ -1276,12 +1276,13 @@ extern "C" int odie_linear(const void* x, const void* weight, const void* bias, 
         ODIE_REQUIRE(x && weight && y, "x, weight and y are required");
         if (activation == ACT_NONE) slope = nullptr;  // 1 everywhere
         const cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_handle);
-        if (rows <= FEW_ROWS && !offsets) {
+        const bool thin = thin_sizes(inputs, outputs) && on_16_bytes({x, weight, residual, y, activation == ACT_RELU ? nullptr : slope});
+        if (rows <= FEW_ROWS && !offsets && !(thin && activation == ACT_RELU)) {  // (thin layers decide a ReLU's corner)
             const FewArgs a{x, weight, bias, residual, y, slope, int(rows), inputs, outputs, activation};
             with_linear_type(dtype, [&](auto type) { launch_few_rows<decltype(type)>(a, stream); });
             return;
         }
-        if (thin_sizes(inputs, outputs) && on_16_bytes({x, weight, residual, y, activation == ACT_RELU ? nullptr : slope})) {
+        if (thin) {
             ThinArgs a{};
             a.rows = rows;
             a.inputs = inputs;

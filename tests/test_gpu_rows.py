@@ -284,7 +284,7 @@ def test_linear_relu_of_sums_too_small_for_y(cuda, rows, inputs, outputs, residu
     assert torch.equal(found, signs.t()[at] > 0)
 
 
-@pytest.mark.parametrize('rows, inputs, outputs', [(2000, 32, 64), (333, 64, 40), (500, 24, 8), (1, 32, 16), (900, 64, 64)])
+@pytest.mark.parametrize('rows, inputs, outputs', [(2000, 32, 64), (333, 64, 40), (500, 24, 8), (1, 32, 16), (900, 64, 64), (2, 64, 64)])
 @pytest.mark.parametrize('dtype', HALVES)
 def test_thin_relu_at_its_corner(cuda, rows, inputs, outputs, dtype):
     """Sums that cancel to the last bits: a layer of up to 64 inputs and outputs is on where the fp32 chain in ascending
