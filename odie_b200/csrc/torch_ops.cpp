@@ -6,6 +6,7 @@
 // its kernels.
 #include <torch/extension.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include "odie_b200.h"
@@ -44,6 +45,15 @@ void check_ids(const Tensor& t, const char* name) {
 }
 void check_device(const Tensor& t, const Tensor& as, const char* name) {
     TORCH_CHECK_VALUE(t.device() == as.device(), name, " is on ", t.device(), ", not ", as.device());
+}
+
+// Forward-mode derivatives are refused: the kernels' results would have no tangent, and the derivative be wrong.
+bool dual(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool dual(const Maybe& t) { return t && dual(*t); }
+template <typename... Tensors>
+void refuse_tangents(const Tensors&... tensors) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!(c10::AutogradState::get_tls_state().get_fw_grad_mode() && (dual(tensors) || ...)),
+                                "the row operators of odie_b200 have no forward-mode derivatives");
 }
 
 // What a backward pass returns.  Asked for a graph of it (create_graph), it hangs from the tensors it came from by a
@@ -136,6 +146,7 @@ struct Dispatch : torch::autograd::Function<Dispatch> {
         return dispatched(x, {order, slot}, weights);
     }
     static variable_list backward(AutogradContext* ctx, variable_list gradients) {
+        refuse_tangents(gradients[0]);
         const auto saved = ctx->get_saved_variables();
         const int64_t need = ctx->saved_data["need"].toInt();
         const Order o{saved[2], saved[3]};
@@ -157,6 +168,7 @@ struct Combine : torch::autograd::Function<Combine> {
         return combined(rows, {order, slot}, weights);
     }
     static variable_list backward(AutogradContext* ctx, variable_list gradients) {
+        refuse_tangents(gradients[0]);
         const auto saved = ctx->get_saved_variables();
         const int64_t need = ctx->saved_data["need"].toInt();
         const auto [d_rows, d_weights] =
@@ -177,6 +189,7 @@ Tensor check_weights(const Maybe& weights, const Order& o, const Tensor& x) {
 
 Tensor dispatch(const Tensor& x, const Tensor& order, const Tensor& slot, const Maybe& weights) {
     check_rows(x, "x");
+    refuse_tangents(x, weights);
     const Order o = check_order(order, slot);
     TORCH_CHECK_VALUE(x.size(0) == o.rows(), "x has ", x.size(0), " rows, the order ", o.rows());
     check_device(slot, x, "order");
@@ -187,6 +200,7 @@ Tensor dispatch(const Tensor& x, const Tensor& order, const Tensor& slot, const 
 
 Tensor combine(const Tensor& rows, const Tensor& order, const Tensor& slot, const Maybe& weights) {
     check_rows(rows, "rows");
+    refuse_tangents(rows, weights);
     const Order o = check_order(order, slot);
     TORCH_CHECK_VALUE(rows.size(0) == o.rows() * o.choices(), "rows has ", rows.size(0), " rows, the order ", o.rows(), " x ", o.choices());
     check_device(slot, rows, "order");
@@ -237,6 +251,7 @@ struct Linear : torch::autograd::Function<Linear> {
         return y;
     }
     static variable_list backward(AutogradContext* ctx, variable_list gradients) {
+        refuse_tangents(gradients[0]);
         const auto saved = ctx->get_saved_variables();
         const Tensor &x = saved[0], &weight = saved[1], &slope = saved[2], &offsets = saved[3];
         // without a slope (only the residual's gradient is wanted) there is no activation to undo
@@ -286,6 +301,7 @@ Tensor linear(const Tensor& x, const Tensor& weight, const Maybe& bias, const Ma
                           "offsets must be CUDA int32 [", weight.size(0) + 1, "]");
         check_device(*offsets, x, "offsets");
     }
+    refuse_tangents(x, weight, bias, residual);
     const int64_t outputs = weight.size(-2);
     std::vector<int64_t> shape = x.sizes().vec();
     shape.back() = outputs;
@@ -323,6 +339,7 @@ struct Embed : torch::autograd::Function<Embed> {
         return embedded(ids, table, scale);
     }
     static variable_list backward(AutogradContext* ctx, variable_list gradients) {
+        refuse_tangents(gradients[0]);
         const Tensor ids = ctx->get_saved_variables()[0];
         const int64_t rows = ctx->saved_data["rows"].toInt();
         const Tensor d_out = gradients[0].contiguous();
@@ -340,6 +357,7 @@ struct Embed : torch::autograd::Function<Embed> {
 Tensor embed(const Tensor& ids, const Tensor& table, double scale) {
     check_ids(ids, "ids");
     check_rows(table, "table");
+    refuse_tangents(table);
     TORCH_CHECK_VALUE(table.size(0) >= 1 && table.size(0) < (int64_t(1) << 30), "the table must have 1 to 2^30 - 1 rows");
     TORCH_CHECK_VALUE(ids.numel() < (int64_t(1) << 31) - 4096, "too many ids");
     check_device(ids, table, "ids");

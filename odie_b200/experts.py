@@ -5,7 +5,8 @@ The operators here give experts layers of their own: `sort_rows` orders the (row
 `dispatch` copies each row to its places, `linear` multiplies every group of consecutive rows by its expert's
 matrix with bias, activation and residual in the same kernel, `combine` brings the results back as weighted sums;
 `embed` looks rows of a learned table up by id.  All of them run the kernels of libodie_b200.so on the current
-stream of their tensors' device, are differentiable (once) and give the same bits in every run.  `ExpertHeads`
+stream of their tensors' device, are differentiable (once, backward; forward-mode derivatives and transforms of
+torch.func are refused) and give the same bits in every run.  `ExpertHeads`
 is the MLP of `model.Head` with one set of weights per expert, built from them.
 
 There is no CPU path: tensors that are not on a CUDA device are refused.

@@ -1,0 +1,66 @@
+"""The routed-expert row operators on the GPU (odie_b200.experts) at the ends of what they take: derivatives of other
+kinds, the widest rows, values that are no numbers, far tails, waits that run out.  Bounds as in rows_cases."""
+import pytest
+import torch
+
+from rows_cases import SUM, plain_linear, rounding, within
+
+pytestmark = pytest.mark.gpu
+
+HALVES = [torch.float16, torch.bfloat16]
+
+
+def generator(seed):
+    return torch.Generator(device='cuda').manual_seed(seed)
+
+
+def normal(g, *shape, dtype=torch.float32, std=1.0):
+    return (torch.randn(shape, generator=g, device='cuda') * std).to(dtype)
+
+
+# ---------------------------------------------------------------- derivatives of other kinds
+def differentiable_calls():
+    """{name: (call, its differentiable arguments)} of every operator."""
+    from odie_b200.experts import combine, dispatch, embed, linear, sort_rows
+    g = generator(1)
+    order = sort_rows(torch.randint(0, 3, (30, 2), generator=g, device='cuda'), 3)
+    ids = torch.randint(0, 5, (30,), generator=g, device='cuda')
+    weights = torch.rand((30, 2), generator=g, device='cuda')
+    half = [normal(g, *s, dtype=torch.float16) for s in ((30, 16), (24, 16), (24,), (30, 24))]
+    return {'linear': (lambda x, w, b, r: linear(x, w, b, r, 'silu'), half),
+            'linear x.T': (lambda x, w: linear(x.t(), w), [half[0].t().contiguous(), half[1]]),
+            'dispatch': (lambda x, p: dispatch(x, order, p), [normal(g, 30, 8), weights]),
+            'combine': (lambda y, p: combine(y, order, p), [normal(g, 60, 8), weights]),
+            'embed': (lambda table: embed(ids, table), [normal(g, 5, 16)])}
+
+
+@pytest.mark.parametrize('name', ['linear', 'linear x.T', 'dispatch', 'combine', 'embed'])
+@pytest.mark.parametrize('requires_grad', [False, True])
+def test_forward_mode_is_refused(cuda, name, requires_grad):
+    """A tangent is not dropped: of an argument, or of the gradient that a backward pass is given."""
+    from torch.autograd import forward_ad
+    call, arguments = differentiable_calls()[name]
+    with forward_ad.dual_level():
+        for i, t in enumerate(arguments):
+            dual = forward_ad.make_dual(t.detach().clone().requires_grad_(requires_grad), torch.ones_like(t))
+            for grad in (torch.enable_grad, torch.no_grad):
+                with grad(), pytest.raises(RuntimeError, match='forward-mode'):
+                    call(*arguments[:i], dual, *arguments[i + 1:])
+        leaves = [t.detach().clone().requires_grad_() for t in arguments]
+        y = call(*leaves)
+        d = torch.ones_like(y)
+        want = torch.autograd.grad(y, leaves, d, retain_graph=True)
+        with pytest.raises(RuntimeError, match='forward-mode'):
+            torch.autograd.grad(y, leaves, forward_ad.make_dual(d, torch.ones_like(d)), retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, leaves, d), want))
+
+
+@pytest.mark.parametrize('name', ['linear', 'dispatch', 'combine', 'embed'])
+def test_function_transforms_are_refused(cuda, name):
+    call, arguments = differentiable_calls()[name]
+    first, rest = arguments[0], arguments[1:]
+    for transformed in (lambda: torch.func.vmap(lambda t: call(t, *rest))(first[None]),
+                        lambda: torch.func.grad(lambda t: call(t, *rest).float().sum())(first),
+                        lambda: torch.func.jvp(lambda t: call(t, *rest), (first,), (first,))):
+        with pytest.raises(RuntimeError):
+            transformed()
