@@ -5,7 +5,9 @@
 // through autograd nodes written in Python (the engine's thread waits for the interpreter at every node), more than
 // its kernels.
 #include <torch/extension.h>
+#include <torch/csrc/autograd/engine.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -56,18 +58,22 @@ void refuse_tangents(const Tensors&... tensors) {
                                 "the row operators of odie_b200 have no forward-mode derivatives");
 }
 
-// What a backward pass returns.  Asked for a graph of it (create_graph), it hangs from the tensors it came from by a
-// node that refuses to be differentiated.
-variable_list once(variable_list gradients, const variable_list& from) {
+// What a backward pass returns.  Asked for a graph of it (create_graph), it hangs by a node that refuses to be
+// differentiated from the tensors that it depends on: `from`, and the first `arguments` of the forward pass (by the
+// running node's edges to them, so that none is kept for it).
+variable_list once(variable_list gradients, const variable_list& from, size_t arguments = 0) {
     if (!at::GradMode::is_enabled()) return gradients;
+    torch::autograd::edge_list edges = torch::autograd::collect_next_edges(from);
+    if (arguments) {
+        const auto node = torch::autograd::get_current_node();
+        TORCH_CHECK(node && node->num_outputs() >= arguments, "a backward pass outside of its node");
+        for (size_t i = 0; i < arguments; ++i) edges.push_back(node->next_edge(i));
+    }
     for (Tensor& g : gradients) {
         if (!g.defined()) continue;
-        variable_list all{g.detach().requires_grad_()};
-        for (const Tensor& t : from)
-            if (t.defined() && t.requires_grad()) all.push_back(t);
-        const auto refuse = std::make_shared<torch::autograd::DelayedError>("the row operators of odie_b200 are differentiable once",
-                                                                            int64_t(all.size()));
-        g = (*refuse)(std::move(all))[0];
+        g = g.detach();
+        torch::autograd::set_history(g, std::make_shared<torch::autograd::Error>("the row operators of odie_b200 are differentiable once",
+                                                                                 torch::autograd::edge_list(edges)));
     }
     return gradients;
 }
@@ -246,6 +252,7 @@ struct Linear : torch::autograd::Function<Linear> {
         ctx->save_for_backward({need & 2 ? x : Tensor(), need & 1 ? weight : Tensor(), slope, offsets});
         ctx->saved_data["need"] = need;
         ctx->saved_data["activation"] = activation;
+        ctx->saved_data["slope of"] = int64_t(bias.defined() ? 3 : 2);
         ctx->saved_data["inputs"] = x.size(1);
         ctx->saved_data["weight"] = weight.sizes().vec();
         return y;
@@ -275,7 +282,8 @@ struct Linear : torch::autograd::Function<Linear> {
                                       stream_of(d_y)),
                  "odie_linear_backward");
         }
-        return once({d_x, d_weight, d_bias, d_residual, Tensor(), Tensor(), Tensor()}, {gradients[0], x, weight});
+        return once({d_x, d_weight, d_bias, d_residual, Tensor(), Tensor(), Tensor()}, {gradients[0], x, weight},
+                    slope.defined() && activation != 1 ? ctx->saved_data["slope of"].toInt() : 0);
     }
 };
 

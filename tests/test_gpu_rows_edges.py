@@ -64,3 +64,33 @@ def test_function_transforms_are_refused(cuda, name):
                         lambda: torch.func.jvp(lambda t: call(t, *rest), (first,), (first,))):
         with pytest.raises(RuntimeError):
             transformed()
+
+
+@pytest.mark.parametrize('activation', ['relu', 'silu', 'gelu'])
+@pytest.mark.parametrize('inputs, outputs', [(16, 24), (80, 72)])
+def test_second_derivatives_of_linear_are_refused(cuda, activation, inputs, outputs):
+    """Also where the first derivative that is asked for keeps little: a smooth slope depends on x, weight and bias."""
+    from odie_b200.experts import linear
+    g = generator(1)
+    arguments = [normal(g, *s, dtype=torch.float16) for s in ((30, inputs), (outputs, inputs), (outputs,), (30, outputs))]
+    smooth = activation != 'relu'
+    for wanted in ([0], [1], [2], [0, 1, 2, 3]):
+        leaves = [t.detach().clone().requires_grad_(j in wanted) for j, t in enumerate(arguments)]
+        y = linear(*leaves, activation)
+        first = torch.autograd.grad(y, [leaves[i] for i in wanted], torch.ones_like(y), create_graph=True)
+        for i, a in zip(wanted, first):
+            for j in wanted:
+                if (smooth and i < 3 and j < 3) or (i, j) in ((0, 1), (1, 0)):
+                    with pytest.raises(RuntimeError, match='once'):
+                        torch.autograd.grad(a.float().square().sum(), leaves[j], retain_graph=True, allow_unused=True)
+
+
+@pytest.mark.parametrize('name', ['dispatch', 'combine'])
+def test_second_derivatives_between_rows_and_weights_are_refused(cuda, name):
+    call, arguments = differentiable_calls()[name]
+    leaves = [t.detach().clone().requires_grad_() for t in arguments]
+    y = call(*leaves)
+    first = torch.autograd.grad(y, leaves, torch.ones_like(y), create_graph=True)
+    for a, other in zip(first, leaves[::-1]):
+        with pytest.raises(RuntimeError, match='once'):
+            torch.autograd.grad(a.float().square().sum(), other, retain_graph=True, allow_unused=True)
