@@ -1214,8 +1214,8 @@ void launch_dz(const DzArgs& a, int kind, cudaStream_t stream) {
     const int columns = wide ? 8 : 1;
     int log2 = 0;
     while (log2 < (single && wide ? 1 : 5) && (columns << log2) < a.n) ++log2;
+    while (ceil_div(a.n, columns << log2) > 65535) ++log2;  // one unit of 2^20 outputs: four threads a row, not two
     const dim3 grid(unsigned(dz_units(a.rows, a.groups)), unsigned(ceil_div(a.n, columns << log2)));
-    ODIE_REQUIRE(grid.y <= 65535, "too many outputs for one launch");
     auto go = [&](auto k) {
         constexpr int KIND = decltype(k)::value;
         if (single && wide) dz_kernel<T, 8, 1024, KIND><<<grid, 1024, 0, stream>>>(a, log2);

@@ -94,3 +94,20 @@ def test_second_derivatives_between_rows_and_weights_are_refused(cuda, name):
     for a, other in zip(first, leaves[::-1]):
         with pytest.raises(RuntimeError, match='once'):
             torch.autograd.grad(a.float().square().sum(), other, retain_graph=True, allow_unused=True)
+
+
+# ---------------------------------------------------------------- the widest rows
+@pytest.mark.parametrize('rows, inputs, outputs', [(3, 8, 1 << 20), (5, 16, (1 << 20) - 8), (2, 8, 1 << 20), (3, 1 << 20, 8), (3, 4, (1 << 20) - 3)])
+def test_linear_of_the_most_inputs_and_outputs(cuda, rows, inputs, outputs):
+    """Up to 2^20 of either, with every gradient."""
+    from odie_b200.experts import linear
+    g = generator(rows + inputs)
+    case = [normal(g, *s, dtype=torch.bfloat16, std=std) for s, std in (((rows, inputs), 1), ((outputs, inputs), inputs ** -0.5), ((outputs,), 1),
+                                                                        ((rows, outputs), 1), ((rows, outputs), 1))]
+    leaves = [t.requires_grad_() for t in case[:4]]
+    y = linear(*leaves, 'silu')
+    grads = torch.autograd.grad(y, leaves, case[4])
+    plain = plain_linear(*(t.detach() for t in case[:4]), [(0, rows)], 'silu', case[4])
+    within(y.detach(), *plain['y'], 'y')
+    for name, got in zip(('x', 'weight', 'bias', 'residual'), grads):
+        within(got, *plain['d_' + name], 'd_' + name)
