@@ -62,6 +62,7 @@ __global__ void __launch_bounds__(THREADS) embed_kernel(EmbedArgs a, const T* __
 struct GradArgs {
     long long n, rows, width;
     int lanes_log2;
+    long long column0;       // first vector of the launch: a grid has at most 65535 blocks of columns
     float scale;
     const uint32_t* sorted;  // [n] ids in order; the table's row count for ids outside it
     const int* order;        // [n] position in d out
@@ -75,7 +76,7 @@ __global__ void __launch_bounds__(THREADS, 4) embed_chunk_kernel(GradArgs a, con
     using P = Pack<T, BYTES>;
     const int lanes = 1 << a.lanes_log2, lane = threadIdx.x & (lanes - 1);
     const long long chunk = ((long long)blockIdx.x * THREADS + threadIdx.x) >> a.lanes_log2;
-    const long long c = (long long)blockIdx.y * lanes + lane;
+    const long long c = a.column0 + (long long)blockIdx.y * lanes + lane;
     const long long begin = chunk * CHUNK;
     if (begin >= a.n || c * P::N >= a.width) return;
     const int count = int(min((long long)CHUNK, a.n - begin));
@@ -159,7 +160,7 @@ __global__ void __launch_bounds__(THREADS) embed_join_kernel(GradArgs a, T* __re
     if (threadIdx.x < count) runs[threadIdx.x] = a.runs[v0 + threadIdx.x];
     __syncthreads();
     const int lanes = 1 << a.lanes_log2, lane = threadIdx.x & (lanes - 1), step = THREADS >> a.lanes_log2;
-    const long long c = (long long)blockIdx.y * lanes + lane;
+    const long long c = a.column0 + (long long)blockIdx.y * lanes + lane;
     if (c * P::N >= a.width) return;
     for (int q = threadIdx.x >> a.lanes_log2; q < count; q += step) {
         const int2 run = runs[q];
@@ -280,17 +281,19 @@ extern "C" int odie_embed_backward(const void* ids, int id_bytes, int64_t n, con
         const int64_t chunk_blocks = ((chunks << g.lanes_log2) + THREADS - 1) / THREADS;
         const int64_t step = THREADS >> g.lanes_log2;
         const int64_t span = std::max<int64_t>(1, std::min<int64_t>({MAX_SPAN, 16 * step, rows / (148 * 8)})), join_blocks = (rows + span - 1) / span;
-        ODIE_REQUIRE(columns <= 65535 && chunk_blocks < (int64_t(1) << 31) && join_blocks < (int64_t(1) << 31),
-                     "too many rows or columns for one launch");
+        ODIE_REQUIRE(chunk_blocks < (int64_t(1) << 31) && join_blocks < (int64_t(1) << 31), "too many rows for one launch");
         with_row_type(dtype, vector, [&](auto type, auto bytes) {
             using T = decltype(type);
             constexpr int B = decltype(bytes)::value;
-            embed_chunk_kernel<T, B><<<dim3(unsigned(chunk_blocks), unsigned(columns)), THREADS, 0, stream>>>(
-                g, static_cast<const T*>(d_out), static_cast<T*>(d_table));
-            embed_join_kernel<T, B><<<dim3(unsigned(join_blocks), unsigned(columns)), THREADS, 0, stream>>>(
-                g, static_cast<T*>(d_table), int(span));
+            for (int64_t first = 0; first < columns; first += 65535) {
+                const unsigned count = unsigned(std::min<int64_t>(65535, columns - first));
+                g.column0 = first * lanes;
+                embed_chunk_kernel<T, B><<<dim3(unsigned(chunk_blocks), count), THREADS, 0, stream>>>(
+                    g, static_cast<const T*>(d_out), static_cast<T*>(d_table));
+                embed_join_kernel<T, B><<<dim3(unsigned(join_blocks), count), THREADS, 0, stream>>>(g, static_cast<T*>(d_table), int(span));
+                ODIE_CUDA(cudaGetLastError());
+                note_launch(2);
+            }
         });
-        ODIE_CUDA(cudaGetLastError());
-        note_launch(2);
     });
 }

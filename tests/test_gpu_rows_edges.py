@@ -111,3 +111,17 @@ def test_linear_of_the_most_inputs_and_outputs(cuda, rows, inputs, outputs):
     within(y.detach(), *plain['y'], 'y')
     for name, got in zip(('x', 'weight', 'bias', 'residual'), grads):
         within(got, *plain['d_' + name], 'd_' + name)
+
+
+@pytest.mark.parametrize('dtype, width', [(torch.float16, 65535 * 256 + 1), (torch.float32, 65535 * 256 + 3)])
+def test_embed_of_very_wide_rows(cuda, dtype, width):
+    """More columns than one launch's second grid dimension holds."""
+    from odie_b200.experts import embed
+    g = generator(3)
+    ids = torch.tensor([1, 0, 1, 5], device=cuda)
+    table, d_out = normal(g, 3, width, dtype=dtype).requires_grad_(), normal(g, 4, width, dtype=dtype)
+    out = embed(ids, table)
+    assert torch.equal(out[:3], table[ids[:3]]) and (out[3] == 0).all()
+    (grad,) = torch.autograd.grad(out, table, d_out)
+    assert torch.equal(grad[0], d_out[1]) and (grad[2] == 0).all()
+    assert torch.equal(grad[1], (d_out[0].float() + d_out[2].float()).to(dtype))  # one fp32 sum, rounded once
