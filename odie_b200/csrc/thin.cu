@@ -81,10 +81,16 @@ template <typename T>
 __device__ __forceinline__ uint32_t larger(uint32_t a, const uint4& v) {
     return larger<T>(larger<T>(larger<T>(a, v.x), larger<T>(v.y, v.z)), v.w);
 }
+// The larger of two magnitudes; infinity where either is NaN.
 template <typename T>
 __device__ __forceinline__ float larger_of(uint32_t pair) {
-    const float2 f = unpack_pair<T>(pair);
-    return fmaxf(f.x, f.y);
+    constexpr uint32_t INF = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    return unpack_pair<T>(min(max(pair & 0xffffu, pair >> 16), INF)).x;
+}
+// Two magnitudes, 0 in place of those that are not finite.
+template <typename T>
+__device__ __forceinline__ uint32_t finite(uint32_t pair) {
+    return pair & ~__vcmpgeu2(pair & 0x7fff7fffu, std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u);
 }
 
 // x . w as the chain in ascending order; count is a multiple of 8.
@@ -163,7 +169,9 @@ __global__ void __launch_bounds__(THREADS, thin_blocks(KB * 32, NB * 32, ACT, fa
             bias[nb][e] = a.bias && n < a.outputs ? to_float(static_cast<const T*>(a.bias)[(long long)u.g * a.outputs + n]) : 0.0f;
         }
     }
-    float bias_corner = 0.0f, corner = 0.0f;  // corner: times a row's largest input: what the tensor cores' sum may be off by
+    // corner: times a row's largest input: what the tensor cores' sum may be off by.  Of the finite weights and biases: a
+    // unit of others has no finite sum.
+    float bias_corner = 0.0f, corner = 0.0f;
     if (ACT == ACT_RELU) {
         uint32_t largest = 0;
         float most_bias = 0.0f;
@@ -172,9 +180,11 @@ __global__ void __launch_bounds__(THREADS, thin_blocks(KB * 32, NB * 32, ACT, fa
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int kb = 0; kb < KB; ++kb) largest = larger<T>(largest, w[nb][j][kb]);
+                for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int e = 0; e < 8; ++e) most_bias = fmaxf(most_bias, fabsf(bias[nb][e]));
+                    for (int i = 0; i < 4; ++i) largest = larger<T>(largest, finite<T>(word(w[nb][j][kb], i)));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) most_bias = fmaxf(most_bias, isfinite(bias[nb][e]) ? fabsf(bias[nb][e]) : 0.0f);
         }
         float most = larger_of<T>(largest);
 #pragma unroll
@@ -226,7 +236,7 @@ __global__ void __launch_bounds__(THREADS, thin_blocks(KB * 32, NB * 32, ACT, fa
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) x[kb][h] = now[(kb * 2 + h) * 32];
         uint32_t on = 0;    // ReLU: a byte per (h, nb)
-        float near = 0.0f;  // for both rows of the lane
+        float near = 0.0f;  // for both rows of the lane; infinite or NaN if either holds no numbers: every finite sum goes by its chain
         if (ACT == ACT_RELU) {
             uint32_t largest = larger<T>(larger<T>(0, x[0][0]), x[0][1]);
             if (KB == 2) largest = larger<T>(larger<T>(largest, x[KB - 1][0]), x[KB - 1][1]);
@@ -260,10 +270,13 @@ __global__ void __launch_bounds__(THREADS, thin_blocks(KB * 32, NB * 32, ACT, fa
 #pragma unroll
                 for (int e = 2; e < 16; e += 2) least = least_magnitude(least, d[e / 4][e % 4], d[e / 4][e % 4 + 1]);
                 least = fminf(least, fabsf(d[0][1]));
-                if (least <= near) {
+                if (!(least > near)) {
                     uint32_t which = 0;
 #pragma unroll
-                    for (int e = 0; e < 16; ++e) which |= fabsf(d[e / 4][e % 4]) < near && inside && left > (e % 4 / 2) * 8 ? 1u << e : 0u;
+                    for (int e = 0; e < 16; ++e) {
+                        const float z = fabsf(d[e / 4][e % 4]);
+                        which |= !(z >= near) && z < INFINITY && inside && left > (e % 4 / 2) * 8 ? 1u << e : 0u;
+                    }
 #pragma unroll 1
                     for (; which; which &= which - 1) {
                         const int at = __ffs(which) - 1, n = column + at / 4 * 2 + at % 2;

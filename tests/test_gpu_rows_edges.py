@@ -125,3 +125,80 @@ def test_embed_of_very_wide_rows(cuda, dtype, width):
     (grad,) = torch.autograd.grad(out, table, d_out)
     assert torch.equal(grad[0], d_out[1]) and (grad[2] == 0).all()
     assert torch.equal(grad[1], (d_out[0].float() + d_out[2].float()).to(dtype))  # one fp32 sum, rounded once
+
+
+# ---------------------------------------------------------------- what is no number, in other rows
+def passing(x, weight, **kwargs):
+    """[rows, outputs] bool: where linear's ReLU passes a gradient, one output at a time: d x is then a row of W or 0."""
+    from odie_b200.experts import linear
+    x = x.clone().requires_grad_()
+    y = linear(x, weight, activation='relu', **kwargs)
+    found = torch.empty(y.shape, dtype=torch.bool, device=y.device)
+    for n in range(y.shape[1]):
+        d_y = torch.zeros_like(y)
+        d_y[:, n] = 1
+        (d_x,) = torch.autograd.grad(y, x, d_y, retain_graph=True)
+        found[:, n] = (d_x != 0).any(1)
+    return found
+
+
+@pytest.mark.parametrize('poison', [float('nan'), float('inf'), float('-inf')])
+@pytest.mark.parametrize('inputs, outputs', [(32, 16), (64, 64), (24, 40)])
+@pytest.mark.parametrize('dtype', HALVES)
+def test_thin_relu_corner_beside_rows_of_no_numbers(cuda, poison, inputs, outputs, dtype):
+    """A row's units go by its own fp32 chain in ascending order of the inputs (a unit of sum zero is off), whatever stands
+    in the rows around it: sums that cancel to their last bits, with all their weight in even columns, and rows of zeros."""
+    g = generator(inputs)
+    rows = 4096
+    x, w = normal(g, rows, inputs, dtype=dtype), normal(g, outputs, inputs, std=0.3, dtype=dtype)
+    x[:, 1::2] = 0
+    for level in range(3):  # the last even inputs cancel the sum of output 0 to 2^-24 of it
+        k = inputs - 6 + 2 * level
+        w[0, k] = 2.0 ** (-8 * level)
+        x[:, k] = (-(x[:, :k].double() @ w[0, :k].double()) * 2.0 ** (8 * level)).to(dtype)
+    x[::5] = 0
+    hit = torch.rand(rows, generator=g, device=cuda) < 0.3
+    x[hit, torch.randint(inputs // 2, (rows,), generator=g, device=cuda)[hit] * 2] = poison
+    both = hit & (torch.rand(rows, generator=g, device=cuda) < 0.3)
+    x[both] = poison
+    chain = torch.zeros(rows, outputs, device=cuda)
+    for k in range(inputs):
+        chain = chain + x[:, k:k + 1].float() * w[:, k].float()
+    found = passing(x, w)
+    assert torch.equal(found[~hit], chain[~hit] > 0)
+
+
+def relu_bits(x, weight, bias):
+    """[rows, outputs] bool: the ReLU's bits that the C interface keeps for the gradient."""
+    from odie_b200 import _lib
+    (rows, inputs), outputs = x.shape, weight.shape[0]
+    y, bits = x.new_empty(rows, outputs), torch.empty((rows, (outputs + 7) // 8, 1), device=x.device, dtype=torch.uint8)
+    status = _lib.library().odie_linear(x.data_ptr(), weight.data_ptr(), bias.data_ptr(), None, rows, inputs, outputs, 1, None,
+                                        int(x.dtype == torch.bfloat16), 1, y.data_ptr(), bits.data_ptr(), None, _lib.stream_handle())
+    _lib.check(status, 'odie_linear')
+    return (bits >> torch.arange(8, device=x.device, dtype=torch.uint8) & 1).view(rows, -1)[:, :outputs].bool()
+
+
+@pytest.mark.parametrize('where', ['weight', 'bias'])
+@pytest.mark.parametrize('poison', [float('nan'), float('inf')])
+def test_thin_relu_corner_beside_units_of_no_numbers(cuda, where, poison):
+    """The same beside another output whose weights or bias are no numbers."""
+    g = generator(7)
+    rows, inputs, outputs = 2000, 32, 24
+    x, w, b = normal(g, rows, inputs).half(), normal(g, outputs, inputs, std=0.3).half(), torch.zeros(outputs, device=cuda).half()
+    w[:, 1::2] = 0
+    for level in range(3):
+        k = inputs - 6 + 2 * level
+        w[0, k] = 2.0 ** (-8 * level)
+        x[:, k] = (-(x[:, :k].double() @ w[0, :k].double()) * 2.0 ** (8 * level)).half()
+    x[::5], x[640:768] = 0, 0
+    chain = torch.zeros(rows, outputs, device=cuda)
+    for k in range(inputs):
+        chain = chain + x[:, k:k + 1].float() * w[:, k].float()
+    if where == 'weight':
+        w[5, 2] = poison
+    else:
+        b[5] = poison
+    found = relu_bits(x, w, b)  # (d x would hold 0 times the other unit's weight)
+    others = torch.arange(outputs, device=cuda) != 5
+    assert torch.equal(found[:, others], chain[:, others] > 0)
