@@ -202,3 +202,22 @@ def test_thin_relu_corner_beside_units_of_no_numbers(cuda, where, poison):
     found = relu_bits(x, w, b)  # (d x would hold 0 times the other unit's weight)
     others = torch.arange(outputs, device=cuda) != 5
     assert torch.equal(found[:, others], chain[:, others] > 0)
+
+
+# ---------------------------------------------------------------- far tails
+@pytest.mark.parametrize('rows, width', [(2000, 64), (2000, 72), (1, 64), (2, 72), (100, 1024)])
+@pytest.mark.parametrize('dtype', HALVES)
+def test_gelu_tails(cuda, rows, width, dtype):
+    """z P(z) to half a step of its own size and 2^-15 of it, from z = -9 to 9 (z: the elements of x, by a product with
+    the unit matrix, exact).
+
+    What the fp32 arithmetic is off by, relative to the result: P(-u) = t (polynomial in t) e^(-u^2/2) is a fit to
+    2^-14.5 = 4.3e-5 of P in the far tail; e^(-u^2/2) with u^2/2 log2 e <= 58.5
+    rounded twice, 2 x 58.5 x 2^-24 ln 2 = 4.8e-6; the approximate exponential and inverse and eight roundings,
+    12 x 2^-23 = 1.4e-6.  Together below 2^-14."""
+    from odie_b200.experts import linear
+    z = (torch.linspace(-9, 9, rows * width, device=cuda) if rows > 2 else torch.linspace(-9, -3, rows * width, device=cuda)).to(dtype).view(rows, width)
+    y = linear(z, torch.eye(width, device=cuda, dtype=dtype), activation='gelu')
+    want = z.double() * torch.special.erfc(z.double() * -(0.5 ** 0.5)) / 2  # (ndtr's tail has an absolute grain of 1e-16)
+    off = 2.0 ** -14 * want.abs()
+    within(y, want, off + rounding(want.abs() + off, dtype), 'gelu')
