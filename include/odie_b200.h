@@ -422,6 +422,9 @@ ODIE_API int64_t odie_linear_backward_scratch(int64_t rows, int inputs, int outp
 ODIE_API int odie_linear_backward(const void* d_y, const void* slope, int activation, const void* x, const void* weight,
                    int64_t rows, int inputs, int outputs, int groups, const int32_t* offsets, int dtype, void* d_x, void* d_weight,
                    void* d_bias, void* d_residual, void* scratch, uint64_t stream);
+/* Polls (up to 4 us each) after which a wait of the linear kernels that are launched from now on gives up: 0 to 2^22,
+ * -1 for the default, 2^22.  For tests of what follows. */
+ODIE_API int odie_linear_wait_limit(int64_t polls);
 /* *status (device int32) = 0, or 2 once a bounded wait of the linear kernels on this
  * device has run out (their results are then incomplete). */
 ODIE_API int odie_linear_status(int32_t* status, uint64_t stream);

@@ -16,6 +16,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <algorithm>
+#include <atomic>
 #include <initializer_list>
 #include <type_traits>
 
@@ -42,6 +43,8 @@ enum Mode : int { FWD = 0, DX = 1, DW = 2 };
 
 constexpr int BK = 64;
 constexpr int EPILOGUE_WARP = 4;  // the first one
+// Polls of a wait, up to 4 us each: some ten seconds.  Waits of the products have GemmArgs::limit, what gives up waits for
+// its own copies and products with this one.
 constexpr uint32_t WAIT_LIMIT = 1u << 22;
 constexpr int STAGING = 2048;  // bytes per epilogue warp: 32 rows x 32 columns of 16 bits
 
@@ -74,6 +77,7 @@ struct GemmArgs {
     float* partial;      // with several units per tile: [unit][m][n] sums, joined by join_kernel or finish_kernel (m: rows)
     const CUtensorMap* group_maps;  // DW with offsets: [groups][2]
     int* error;
+    uint32_t limit;      // polls of a wait
 };
 
 template <int CG, int BN>
@@ -286,6 +290,8 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
     uint64_t* drained = done + S::ACCUMULATORS;       // per accumulator: read out
     uint64_t* drain = drained + S::ACCUMULATORS;
     uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drain + 1);
+    uint32_t* gave_up = tmem_at + 1;                  // a wait of either CTA has run out
+    uint32_t* issued_by = gave_up + 1;                // [2], the leader's: blocks that each CTA has loaded
     int* begin = reinterpret_cast<int*>(reinterpret_cast<char*>(full) + S::HEAD);  // [groups + 2] first row of each group
     int* first = begin + p.groups + 2;                                            // [groups + 2] first unit
 
@@ -304,6 +310,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
         }
         tc::bar_init(drain, 1);
         tc::fence_bar_init();
+        *gave_up = issued_by[0] = issued_by[1] = 0;
     }
     if (warp == 2) tc::tmem_alloc_group<CG>(tmem_at, S::COLUMNS);
     if (warp == 3) {  // the groups' rows and units
@@ -367,7 +374,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
             }
             const int m = tile.m0 + rank * 128, n = tile.n0 + rank * S::B_ROWS;
             for (int kb = 0; kb < tile.k_blocks; ++kb) {
-                fine = __all_sync(0xffffffffu, tc::bar_wait(empty + s, phase, WAIT_LIMIT));
+                fine = __all_sync(0xffffffffu, tc::bar_wait(empty + s, phase, p.limit));
                 if (!fine) break;
                 if (issuer) {
                     const uint32_t bar = CG == 2 ? full_leader + s * 8 : tc::smem_u32(full + s);
@@ -400,14 +407,12 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
                 }
             }
         }
-        // every stage read out: no arrival is on its way when the CTA ends, and no copy (had a wait run out, the
-        // leader waits for its pair's copies here, with a limit)
-        for (int i = 0; i < STAGES && i < issued; ++i) {
+        // every stage read out: no arrival is on its way when the CTA ends, and no copy
+        for (int i = 0; i < STAGES && i < issued && fine; ++i) {
             const int last = issued - 1 - i;
-            if (fine) fine = __all_sync(0xffffffffu, tc::bar_wait(empty + last % STAGES, (last / STAGES) & 1, WAIT_LIMIT));
-            else if (rank == 0) tc::bar_wait(full + last % STAGES, (last / STAGES) & 1, WAIT_LIMIT);
+            fine = __all_sync(0xffffffffu, tc::bar_wait(empty + last % STAGES, (last / STAGES) & 1, p.limit));
         }
-        if (!fine && lane == 0) atomicExch(p.error, 2);
+        if (lane == 0) tc::store_leader<CG>(issued_by + rank, issued);
     } else if (warp == 1) {
         if (rank == 0) {
             constexpr int A_MN = MODE == DW, B_MN = MODE != FWD;
@@ -420,11 +425,11 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
             for (int t = start; t < tiles && fine; t += step) {
                 const Tile tile = walk.at(t);
                 const int blocks = tile.zero ? 0 : tile.k_blocks;
-                fine = __all_sync(0xffffffffu, tc::bar_wait(drained + acc, acc_phase, WAIT_LIMIT));
+                fine = __all_sync(0xffffffffu, tc::bar_wait(drained + acc, acc_phase, p.limit));
                 if (!fine) break;
                 tc::fence_after_sync();
                 for (int kb = 0; kb < blocks; ++kb) {
-                    fine = __all_sync(0xffffffffu, tc::bar_wait(full + s, phase, WAIT_LIMIT));
+                    fine = __all_sync(0xffffffffu, tc::bar_wait(full + s, phase, p.limit));
                     if (!fine) break;
                     tc::fence_after_sync();
                     if (issuer) {
@@ -447,14 +452,6 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
                     acc = 0;
                     acc_phase ^= 1;
                 }
-            }
-            if (!fine) {
-                if (issuer) {
-                    atomicExch(p.error, 2);
-                    tc::commit_group<CG>(drain);
-                }
-                __syncwarp();
-                tc::bar_wait(drain, 0, WAIT_LIMIT);
             }
         }
     } else if (warp >= EPILOGUE_WARP) {
@@ -493,7 +490,7 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
                     __syncwarp();
                 }
             }
-            fine = __all_sync(0xffffffffu, tc::bar_wait(done + acc, (summed / S::ACCUMULATORS) & 1, WAIT_LIMIT));
+            fine = __all_sync(0xffffffffu, tc::bar_wait(done + acc, (summed / S::ACCUMULATORS) & 1, p.limit));
             if (!fine) break;
             tc::fence_after_sync();
 #pragma unroll 1
@@ -584,13 +581,40 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
                 w.columns -= STRIDE;
             }
         }
-        if (!fine && lane == 0) atomicExch(p.error, 2);
+    }
+    if (!fine && lane == 0) {
+        atomicExch(p.error, 2);
+        tc::store_both<CG>(gave_up, 1);
     }
     __syncwarp();
     tc::fence_before_sync();
     __syncthreads();
     if (CG == 2) tc::cluster_sync();
     tc::fence_after_sync();
+    // Nothing is issued any more.  Had a wait run out, copies and products may still be on their way: they are awaited
+    // before the shared memory and the TMEM go.
+    if (tc::load_shared(gave_up)) {
+        if (warp == 0 && rank == 0) {
+            const int mine = int(tc::load_shared(issued_by)), other = CG == 2 ? int(tc::load_shared(issued_by + 1)) : mine;
+            const uint32_t share = MODE == DW ? S::STAGE : p.a_rows * 128 + S::B_BYTES;  // of one CTA in a block
+            for (int b = max(0, max(mine, other) - STAGES); b < max(mine, other); ++b) {
+                uint64_t* bar = full + b % STAGES;
+                if (lane == 0 && b >= mine) tc::bar_expect(bar, share);
+                if (lane == 0 && b >= other) tc::bar_unexpect(bar, share);
+                __syncwarp();
+                tc::bar_wait(bar, (b / STAGES) & 1, WAIT_LIMIT);
+            }
+        }
+        if (warp == 1) {
+            if (rank == 0 && tc::elect_one()) tc::commit_group<CG>(drain);
+            __syncwarp();
+            tc::bar_wait(drain, 0, WAIT_LIMIT);
+        }
+        tc::fence_before_sync();
+        __syncthreads();
+        if (CG == 2) tc::cluster_sync();
+        tc::fence_after_sync();
+    }
     if (warp == 2) tc::tmem_dealloc_group<CG>(tmem, S::COLUMNS);
 }
 
@@ -935,6 +959,7 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(FewArgs a) {
 
 // ---------------------------------------------------------------- host
 __device__ int linear_error;
+std::atomic<uint32_t> wait_limit{WAIT_LIMIT};
 
 int* error_word() {
     int* p;
@@ -1320,6 +1345,7 @@ extern "C" int odie_linear(const void* x, const void* weight, const void* bias, 
         p.slope = slope;
         p.activation = activation;
         p.error = error_word();
+        p.limit = wait_limit;
         with_linear_type(dtype, [&](auto type) {
             launch_product<decltype(type), FWD>(x, weight, ld, ld, outputs, inputs, p, Splits(rows, outputs, inputs, groups, offsets), s.partial,
                                                 stream);
@@ -1409,6 +1435,7 @@ extern "C" int odie_linear_backward(const void* d_y, const void* slope, int acti
             p.rows = rows;
             p.n = inputs;
             p.error = error_word();
+            p.limit = wait_limit;
             if (d_x) {
                 p.k = outputs;
                 p.out = d_x;
@@ -1441,6 +1468,13 @@ extern "C" int odie_linear_backward(const void* d_y, const void* slope, int acti
                 }
             }
         });
+    });
+}
+
+extern "C" int odie_linear_wait_limit(int64_t polls) {
+    return guarded([&] {
+        ODIE_REQUIRE(polls >= -1 && polls <= int64_t(WAIT_LIMIT), "polls must be 0 to 2^22, or -1");
+        wait_limit = polls < 0 ? WAIT_LIMIT : uint32_t(polls);
     });
 }
 

@@ -186,6 +186,33 @@ __device__ __forceinline__ void bar_expect(uint64_t* bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
 }
 
+// Takes bytes off the barrier's count as a copy would whose bytes were expected and that is not issued.
+__device__ __forceinline__ void bar_unexpect(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;\n" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
+// A word of both CTAs' copies of a shared variable, or of CTA 0's.
+template <int CG>
+__device__ __forceinline__ void store_both(uint32_t* p, uint32_t v) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "{\n\t.reg .u32 a;\n\tmapa.shared::cluster.u32 a, %0, 0;\n\tst.shared::cluster.u32 [a], %1;\n\t"
+            "mapa.shared::cluster.u32 a, %0, 1;\n\tst.shared::cluster.u32 [a], %1;\n\t}\n" ::"r"(smem_u32(p)),
+            "r"(v)
+            : "memory");
+    else
+        asm volatile("st.shared.u32 [%0], %1;\n" ::"r"(smem_u32(p)), "r"(v) : "memory");
+}
+template <int CG>
+__device__ __forceinline__ void store_leader(uint32_t* p, uint32_t v) {
+    if constexpr (CG == 2) asm volatile("st.shared::cluster.u32 [%0], %1;\n" ::"r"(leader_address(p)), "r"(v) : "memory");
+    else asm volatile("st.shared.u32 [%0], %1;\n" ::"r"(smem_u32(p)), "r"(v) : "memory");
+}
+__device__ __forceinline__ uint32_t load_shared(const uint32_t* p) {
+    uint32_t v;
+    asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(v) : "r"(smem_u32(p)) : "memory");
+    return v;
+}
+
 // TMA loads of one box into this CTA's shared memory, their bytes counted at `bar` (a shared::cluster address:
 // for a pair the leader's barrier).  No multicast.
 template <int CG>

@@ -221,3 +221,54 @@ def test_gelu_tails(cuda, rows, width, dtype):
     want = z.double() * torch.special.erfc(z.double() * -(0.5 ** 0.5)) / 2  # (ndtr's tail has an absolute grain of 1e-16)
     off = 2.0 ** -14 * want.abs()
     within(y, want, off + rounding(want.abs() + off, dtype), 'gelu')
+
+
+# ---------------------------------------------------------------- waits that run out
+@pytest.fixture
+def wait_limit(cuda):
+    from odie_b200 import _lib
+    yield lambda polls: _lib.check(_lib.library().odie_linear_wait_limit(polls), 'odie_linear_wait_limit')
+    torch.cuda.synchronize()
+    _lib.library().odie_linear_wait_limit(-1)
+
+
+def linear_status():
+    from odie_b200 import _lib
+    status = torch.full((1,), -1, dtype=torch.int32, device='cuda')
+    _lib.check(_lib.library().odie_linear_status(status.data_ptr(), _lib.stream_handle()), 'odie_linear_status')
+    return status.item()
+
+
+# single tiles, the sum over K cut, tiles of 64 and 128 columns, SM pairs, several experts, units of a long sum over rows
+WAITS = [(100, 72, 72, 0), (40, 2048, 200, 0), (3000, 200, 136, 0), (4096, 520, 2048, 0), (2000, 136, 264, 3), (20000, 256, 264, 0)]
+
+
+def waiting_pass(case):
+    from odie_b200.experts import linear
+    rows, inputs, outputs, groups = case
+    g = generator(rows)
+    lead = (groups,) if groups else ()
+    leaves = [normal(g, *s, dtype=torch.bfloat16).requires_grad_() for s in ((rows, inputs), (*lead, outputs, inputs), (*lead, outputs))]
+    offsets = torch.linspace(0, rows - 7, groups + 1, device='cuda').int() if groups else None
+    d = normal(g, rows, outputs, dtype=torch.bfloat16)
+
+    def run():
+        y = linear(*leaves, activation='silu', offsets=offsets)
+        return [y.detach(), *torch.autograd.grad(y, leaves, d)]
+    return run
+
+
+@pytest.mark.parametrize('case', WAITS)
+def test_linear_after_waits_that_ran_out(cuda, wait_limit, case):
+    """A kernel whose waits give up (at once, or while its copies and products are on their way) ends, says so, and
+    leaves the next one as it was."""
+    run = waiting_pass(case)
+    want = run()
+    for polls in (0, 1, 2, 3, 5):
+        wait_limit(polls)
+        run()
+        torch.cuda.synchronize()
+        if polls == 0:
+            assert linear_status() == 2
+        wait_limit(-1)
+        assert all(torch.equal(a, b) for a, b in zip(run(), want))
