@@ -425,8 +425,12 @@ ODIE_API int odie_linear_backward(const void* d_y, const void* slope, int activa
 /* Polls (up to 4 us each) after which a wait of the linear kernels that are launched from now on gives up: 0 to 2^22,
  * -1 for the default, 2^22.  For tests of what follows. */
 ODIE_API int odie_linear_wait_limit(int64_t polls);
-/* *status (device int32) = 0, or 2 once a bounded wait of the linear kernels on this
- * device has run out (their results are then incomplete). */
+/* A bounded wait of a linear kernel that runs out leaves its results incomplete.  The next call of odie_linear,
+ * odie_linear_backward or odie_linear_check on the device that finds this out gives -1, once; the first two then do
+ * nothing else.  odie_linear_check looks at what has happened so far and waits for nothing.
+ * odie_linear_status: *status (device int32) = 2 if a wait has run out and no call has said so yet, else 0, in stream
+ * order. */
+ODIE_API int odie_linear_check(void);
 ODIE_API int odie_linear_status(int32_t* status, uint64_t stream);
 
 /* ------------------------------------------------------------------------

@@ -76,7 +76,7 @@ struct GemmArgs {
     int activation;
     float* partial;      // with several units per tile: [unit][m][n] sums, joined by join_kernel or finish_kernel (m: rows)
     const CUtensorMap* group_maps;  // DW with offsets: [groups][2]
-    int* error;
+    int* error;          // on the host: 2 once a wait has run out
     uint32_t limit;      // polls of a wait
 };
 
@@ -583,7 +583,8 @@ __global__ void __launch_bounds__(Shape<CG, BN>::THREADS, 1)
         }
     }
     if (!fine && lane == 0) {
-        atomicExch(p.error, 2);
+        *static_cast<volatile int*>(p.error) = 2;
+        __threadfence_system();
         tc::store_both<CG>(gave_up, 1);
     }
     __syncwarp();
@@ -958,13 +959,35 @@ __global__ void __launch_bounds__(THREADS) few_rows_kernel(FewArgs a) {
 }
 
 // ---------------------------------------------------------------- host
-__device__ int linear_error;
 std::atomic<uint32_t> wait_limit{WAIT_LIMIT};
 
+// The word of the current device in which its kernels leave 2 when a wait has run out: pinned host memory, so that the
+// next call can look at it without waiting for the device.
+constexpr int MAX_DEVICES = 64;
 int* error_word() {
-    int* p;
-    ODIE_CUDA(cudaGetSymbolAddress(reinterpret_cast<void**>(&p), linear_error));
-    return p;
+    static int* const words = [] {
+        void* p = nullptr;
+        // (the first call may come while a graph is captured, which an allocation does not concern)
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        ODIE_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+        const cudaError_t status = cudaHostAlloc(&p, MAX_DEVICES * sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped);
+        cudaThreadExchangeStreamCaptureMode(&mode);
+        ODIE_CUDA(status);
+        std::fill_n(static_cast<int*>(p), MAX_DEVICES, 0);
+        return static_cast<int*>(p);
+    }();
+    int device = 0;
+    ODIE_CUDA(cudaGetDevice(&device));
+    ODIE_REQUIRE(device < MAX_DEVICES, "at most 64 devices");
+    return words + device;
+}
+
+// Refuses once after a wait has run out.
+int* checked_error_word() {
+    int* word = error_word();
+    if (__atomic_load_n(word, __ATOMIC_RELAXED) != 0 && __atomic_exchange_n(word, 0, __ATOMIC_RELAXED) != 0)
+        throw std::runtime_error("a wait of an earlier linear call on this device ran out: that call's results are incomplete");
+    return word;
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encoder() {
@@ -1299,6 +1322,7 @@ extern "C" int odie_linear(const void* x, const void* weight, const void* bias, 
         check_linear(rows, inputs, outputs, groups, offsets, dtype, activation);
         if (rows == 0) return;
         ODIE_REQUIRE(x && weight && y, "x, weight and y are required");
+        int* const error = checked_error_word();
         if (activation == ACT_NONE) slope = nullptr;  // 1 everywhere
         const cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_handle);
         const bool thin = thin_sizes(inputs, outputs) && on_16_bytes({x, weight, residual, y, activation == ACT_RELU ? nullptr : slope});
@@ -1344,7 +1368,7 @@ extern "C" int odie_linear(const void* x, const void* weight, const void* bias, 
         p.residual = residual;
         p.slope = slope;
         p.activation = activation;
-        p.error = error_word();
+        p.error = error;
         p.limit = wait_limit;
         with_linear_type(dtype, [&](auto type) {
             launch_product<decltype(type), FWD>(x, weight, ld, ld, outputs, inputs, p, Splits(rows, outputs, inputs, groups, offsets), s.partial,
@@ -1372,6 +1396,7 @@ extern "C" int odie_linear_backward(const void* d_y, const void* slope, int acti
         ODIE_REQUIRE(d_y && (x || !d_weight) && (weight || !d_x) && scratch, "d_y, x, weight and scratch are required");
         ODIE_REQUIRE(uintptr_t(scratch) % 256 == 0, "scratch must start on a 256-byte boundary");
         ODIE_REQUIRE(slope || activation == ACT_NONE, "slope is required with an activation");
+        int* const error = checked_error_word();
         const int kind = slope_kind(activation, slope);
         const BackwardScratch s(scratch, rows, inputs, outputs, groups);
         if (thin_sizes(inputs, outputs) && on_16_bytes({d_y, kind == SLOPE_CODES ? slope : nullptr, x, weight, d_x, d_residual})) {
@@ -1434,7 +1459,7 @@ extern "C" int odie_linear_backward(const void* d_y, const void* slope, int acti
             p.offsets = offsets;
             p.rows = rows;
             p.n = inputs;
-            p.error = error_word();
+            p.error = error;
             p.limit = wait_limit;
             if (d_x) {
                 p.k = outputs;
@@ -1481,6 +1506,10 @@ extern "C" int odie_linear_wait_limit(int64_t polls) {
 extern "C" int odie_linear_status(int32_t* status, uint64_t stream) {
     return guarded([&] {
         ODIE_REQUIRE(status, "status is required");
-        ODIE_CUDA(cudaMemcpyAsync(status, error_word(), sizeof(int), cudaMemcpyDeviceToDevice, reinterpret_cast<cudaStream_t>(stream)));
+        ODIE_CUDA(cudaMemcpyAsync(status, error_word(), sizeof(int), cudaMemcpyHostToDevice, reinterpret_cast<cudaStream_t>(stream)));
     });
+}
+
+extern "C" int odie_linear_check(void) {
+    return guarded([&] { checked_error_word(); });
 }

@@ -20,7 +20,7 @@ from torch import nn
 
 from . import _lib
 
-__all__ = ['RowOrder', 'sort_rows', 'dispatch', 'combine', 'linear', 'embed', 'ExpertHeads']
+__all__ = ['RowOrder', 'sort_rows', 'dispatch', 'combine', 'linear', 'embed', 'check', 'ExpertHeads']
 
 ACTIVATIONS = {'none': 0, 'relu': 1, 'silu': 2, 'gelu': 3}
 
@@ -78,7 +78,10 @@ def linear(x, weight, bias=None, residual=None, activation='none', offsets=None)
     RowOrder; non-decreasing from 0): x [rows, inputs], weight [experts, outputs, inputs], bias [experts, outputs];
     rows [offsets[e], offsets[e + 1]) take expert e's layer, rows behind the last offset give zero rows (without
     the residual).  residual: broadcastable to the result.  activation: 'none', 'relu', 'silu' or 'gelu' (erf).  Up to
-    2^20 inputs and outputs, 1024 experts and 2^31 - 257 rows."""
+    2^20 inputs and outputs, 1024 experts and 2^31 - 257 rows.
+
+    The kernels' waits are bounded (some ten seconds).  If one runs out, as on a device that has stopped answering, the
+    results are incomplete, and the next `linear` or gradient of it, or `check`, raises RuntimeError."""
     code = ACTIVATIONS.get(activation)
     if code is None:
         raise ValueError(f'activation must be one of {", ".join(ACTIVATIONS)}')
@@ -89,6 +92,14 @@ def embed(ids, table, scale=1.0):
     """scale * table[ids]: ids of any shape (CUDA int32 or int64), table [rows, width] CUDA fp16, bf16 or fp32, result
     [*ids.shape, width] of the table's type.  An id outside the table gives a zero row and takes no gradient."""
     return _ops().embed(ids, table, scale)
+
+
+def check(device=None):
+    """Wait for the device (the current one) and raise RuntimeError if a wait of `linear` has run out there that no call
+    has raised for yet: after the last step of a program, say, or after replaying a captured graph."""
+    with torch.cuda.device(device):
+        torch.cuda.synchronize()
+        _lib.check(_lib.library().odie_linear_check(), 'linear')
 
 
 # ---------------------------------------------------------------- a model of them

@@ -243,32 +243,93 @@ def linear_status():
 WAITS = [(100, 72, 72, 0), (40, 2048, 200, 0), (3000, 200, 136, 0), (4096, 520, 2048, 0), (2000, 136, 264, 3), (20000, 256, 264, 0)]
 
 
-def waiting_pass(case):
-    from odie_b200.experts import linear
-    rows, inputs, outputs, groups = case
-    g = generator(rows)
-    lead = (groups,) if groups else ()
-    leaves = [normal(g, *s, dtype=torch.bfloat16).requires_grad_() for s in ((rows, inputs), (*lead, outputs, inputs), (*lead, outputs))]
-    offsets = torch.linspace(0, rows - 7, groups + 1, device='cuda').int() if groups else None
-    d = normal(g, rows, outputs, dtype=torch.bfloat16)
-
-    def run():
-        y = linear(*leaves, activation='silu', offsets=offsets)
-        return [y.detach(), *torch.autograd.grad(y, leaves, d)]
-    return run
-
-
 @pytest.mark.parametrize('case', WAITS)
 def test_linear_after_waits_that_ran_out(cuda, wait_limit, case):
     """A kernel whose waits give up (at once, or while its copies and products are on their way) ends, says so, and
     leaves the next one as it was."""
-    run = waiting_pass(case)
-    want = run()
+    from odie_b200 import experts
+    rows, inputs, outputs, groups = case
+    g = generator(rows)
+    lead = (groups,) if groups else ()
+    leaves = [normal(g, *s, dtype=torch.bfloat16).requires_grad_() for s in ((rows, inputs), (*lead, outputs, inputs), (*lead, outputs))]
+    offsets = torch.linspace(0, rows - 7, groups + 1, device=cuda).int() if groups else None
+    d = normal(g, rows, outputs, dtype=torch.bfloat16)
+
+    def forward():
+        return experts.linear(*leaves, activation='silu', offsets=offsets)
+    y = forward()
+
+    def backward():
+        return torch.autograd.grad(y, leaves, d, retain_graph=True)
+    grads = backward()
     for polls in (0, 1, 2, 3, 5):
-        wait_limit(polls)
-        run()
+        for call in (forward, backward):
+            wait_limit(polls)
+            call()
+            torch.cuda.synchronize()
+            wait_limit(-1)
+            status = linear_status()
+            assert status in ((2,) if polls == 0 else (0, 2))
+            if status:
+                with pytest.raises(RuntimeError, match='incomplete'):
+                    experts.check()
+            assert torch.equal(forward(), y) and all(torch.equal(a, b) for a, b in zip(backward(), grads))
+
+
+@pytest.mark.parametrize('case', [(100, 72, 72, 0), (4096, 520, 2048, 0)])
+def test_linear_raises_after_a_wait_that_ran_out(cuda, wait_limit, case):
+    """Once, at the next forward or backward call or check, whichever comes first; also for a replayed graph."""
+    from odie_b200 import experts
+    g = generator(1)
+    rows, inputs, outputs, _ = case
+    x, w = normal(g, rows, inputs).half().requires_grad_(), normal(g, outputs, inputs).half().requires_grad_()
+    want = experts.linear(x, w, activation='relu')
+    d = torch.ones_like(want)
+    grads = torch.autograd.grad(want, [x, w], d, retain_graph=True)
+
+    def fails():
+        wait_limit(0)
+        experts.linear(x.detach(), w.detach())
         torch.cuda.synchronize()
-        if polls == 0:
-            assert linear_status() == 2
         wait_limit(-1)
-        assert all(torch.equal(a, b) for a, b in zip(run(), want))
+    for call in (lambda: experts.linear(x, w), lambda: torch.autograd.grad(want, [x, w], d, retain_graph=True), experts.check):
+        fails()
+        with pytest.raises(RuntimeError, match='incomplete'):
+            call()
+        call()
+        experts.check()
+    assert linear_status() == 0
+    assert torch.equal(experts.linear(x, w, activation='relu'), want)
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(want, [x, w], d), grads))
+    wait_limit(0)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        experts.linear(x.detach(), w.detach())
+    wait_limit(-1)
+    experts.check()
+    for _ in range(2):
+        graph.replay()
+        with pytest.raises(RuntimeError, match='incomplete'):
+            experts.check()
+    experts.check()
+
+
+def test_linear_captured_first(cuda):
+    """A graph may hold the process's first call."""
+    import subprocess
+    import sys
+    program = """
+import torch
+from odie_b200.experts import linear, check
+x, w = torch.randn(300, 80, device='cuda').half(), torch.randn(72, 80, device='cuda').half()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = linear(x, w)
+graph.replay()
+check()
+assert torch.equal(y, linear(x, w))
+print('the same')
+"""
+    from pathlib import Path
+    run = subprocess.run([sys.executable, '-c', program], capture_output=True, text=True, timeout=300, cwd=Path(__file__).resolve().parents[1])
+    assert run.returncode == 0 and 'the same' in run.stdout, run.stderr

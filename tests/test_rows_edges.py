@@ -16,3 +16,9 @@ def test_linear_wait_limit_refuses(lib):
         assert lib.odie_linear_wait_limit(polls) == -1
         assert 'polls' in _lib.error()
     assert lib.odie_linear_wait_limit(0) == 0 and lib.odie_linear_wait_limit(-1) == 0
+
+
+def test_linear_check_without_a_device(lib):
+    import torch
+    if not torch.cuda.is_available():  # an error, not an abort
+        assert lib.odie_linear_check() == -1 and _lib.error()
