@@ -2,12 +2,14 @@
 
 The library is the product's compute path: every CUDA kernel plus the C-ABI
 declared in include/odie_b200.h.  It is built next to this file so that it
-travels with the repository snapshot; nothing is installed elsewhere.
+travels with the repository snapshot; nothing is installed elsewhere.  The library needs no torch: where torch or its
+headers are missing, it alone is built.
 """
 from concurrent.futures import ThreadPoolExecutor
 import os
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PACKAGE = Path(__file__).resolve().parent
@@ -42,9 +44,18 @@ def torch_ops_stale():
                                                    Path(__file__)))
 
 
+def torch_headers():
+    """Whether this interpreter can compile extensions of its torch."""
+    try:
+        import torch
+    except ImportError:
+        return False
+    return ((Path(torch.__file__).parent / 'include' / 'torch' / 'extension.h').exists() and
+            (Path(sysconfig.get_paths()['include']) / 'Python.h').exists())
+
+
 def build_torch_ops():
     """g++ on csrc/torch_ops.cpp against this interpreter's torch; the library beside it is found by its folder."""
-    import sysconfig
     import torch
     from torch.utils import cpp_extension
     include = [*cpp_extension.include_paths(), sysconfig.get_paths()['include'],
@@ -64,7 +75,10 @@ def build(force=False, verbose=False):
     if force or stale():
         build_library(verbose)
     if force or torch_ops_stale():
-        build_torch_ops()
+        if torch_headers():
+            build_torch_ops()
+        else:
+            print(f'{TORCH_OPS.name} is not built: torch or its headers are missing', file=sys.stderr)
     return LIBRARY
 
 

@@ -32,7 +32,7 @@ def _ops():
     try:
         from . import _torch_ops
     except ImportError as e:
-        raise _lib.LibraryMissing(f'odie_b200/_torch_ops.so cannot be loaded ({e}): run odie_b200.build()') from e
+        raise _lib.LibraryMissing(f'odie_b200/_torch_ops.so cannot be loaded ({e}): run odie_b200.build() where torch has its headers') from e
     return _torch_ops
 
 

@@ -1,7 +1,13 @@
 """CPU: what the row operators refuse, and how they are built, beyond test_rows.py."""
+import subprocess
+import sys
+from pathlib import Path
+
 import pytest
 
 from odie_b200 import _lib
+
+ROOT = Path(__file__).resolve().parents[1]
 
 
 @pytest.fixture(scope='module')
@@ -22,3 +28,34 @@ def test_linear_check_without_a_device(lib):
     import torch
     if not torch.cuda.is_available():  # an error, not an abort
         assert lib.odie_linear_check() == -1 and _lib.error()
+
+
+WITHOUT_TORCH = """
+import sys
+class Hidden:
+    def find_spec(self, name, path=None, target=None):
+        if name.split('.')[0] == 'torch':
+            raise ModuleNotFoundError(name)
+sys.meta_path.insert(0, Hidden())
+import odie_b200
+from odie_b200 import builder
+from pathlib import Path
+builder.TORCH_OPS = Path(sys.argv[1]) / '_torch_ops.so'
+assert odie_b200.build() == builder.LIBRARY and builder.LIBRARY.exists() and not builder.TORCH_OPS.exists()
+odie_b200.library()
+"""
+
+
+def test_the_library_is_built_without_torch(lib, tmp_path):
+    run = subprocess.run([sys.executable, '-c', WITHOUT_TORCH, str(tmp_path)], capture_output=True, text=True, cwd=ROOT)
+    assert run.returncode == 0, run.stderr
+    assert 'not built' in run.stderr
+
+
+def test_the_library_is_built_without_torch_headers(lib, tmp_path, monkeypatch, capsys):
+    from odie_b200 import builder
+    assert builder.torch_headers()
+    monkeypatch.setattr(builder, 'TORCH_OPS', tmp_path / '_torch_ops.so')
+    monkeypatch.setattr(builder.sysconfig, 'get_paths', lambda: {'include': str(tmp_path)})
+    assert builder.build() == builder.LIBRARY and not builder.TORCH_OPS.exists()
+    assert 'not built' in capsys.readouterr().err
