@@ -6,6 +6,7 @@ travels with the repository snapshot; nothing is installed elsewhere.  The libra
 headers are missing, it alone is built.
 """
 from concurrent.futures import ThreadPoolExecutor
+import importlib.metadata
 import os
 import subprocess
 import sys
@@ -36,8 +37,22 @@ def stale():
     return any(p.stat().st_mtime > built for p in inputs)
 
 
+def torch_key():
+    """What _torch_ops.so is compiled against: the versions of this interpreter and of its torch (without importing it)."""
+    try:
+        torch = importlib.metadata.version('torch')
+    except importlib.metadata.PackageNotFoundError:
+        torch = 'unknown'
+    return f'{sys.implementation.cache_tag} torch {torch}'
+
+
+def torch_ops_key():
+    """The file that says what TORCH_OPS was compiled against."""
+    return PACKAGE / '_build' / (TORCH_OPS.stem + '.key')
+
+
 def torch_ops_stale():
-    if not TORCH_OPS.exists():
+    if not TORCH_OPS.exists() or not torch_ops_key().exists() or torch_ops_key().read_text() != torch_key():
         return True
     built = TORCH_OPS.stat().st_mtime
     return any(p.stat().st_mtime > built for p in (PACKAGE / 'csrc' / 'torch_ops.cpp', ROOT / 'include' / 'odie_b200.h',
@@ -68,7 +83,10 @@ def build_torch_ops():
                f'-L{libs}', '-lc10', '-lc10_cuda', '-ltorch', '-ltorch_cpu', '-ltorch_cuda', '-ltorch_python', f'-L{PACKAGE}',
                '-lodie_b200', '-Wl,-rpath,$ORIGIN', f'-Wl,-rpath,{libs}']
     subprocess.run(command, check=True)
+    torch_ops_key().parent.mkdir(exist_ok=True)
+    torch_ops_key().unlink(missing_ok=True)  # (none, rather than another file's, if this ends here)
     os.replace(tmp, TORCH_OPS)
+    torch_ops_key().write_text(torch_key())
 
 
 def build(force=False, verbose=False):

@@ -59,3 +59,18 @@ def test_the_library_is_built_without_torch_headers(lib, tmp_path, monkeypatch, 
     monkeypatch.setattr(builder.sysconfig, 'get_paths', lambda: {'include': str(tmp_path)})
     assert builder.build() == builder.LIBRARY and not builder.TORCH_OPS.exists()
     assert 'not built' in capsys.readouterr().err
+
+
+def test_torch_ops_of_another_torch_are_stale(lib, monkeypatch):
+    """The file is built again after torch has changed, whatever the files' times say."""
+    import importlib.metadata
+    from odie_b200 import builder
+    assert not builder.torch_ops_stale()
+    with monkeypatch.context() as m:
+        m.setattr(importlib.metadata, 'version', lambda name: '0.0.1')
+        assert builder.torch_ops_stale()
+        built = []
+        m.setattr(builder, 'build_torch_ops', lambda: built.append(True))
+        builder.build()
+        assert built
+    assert not builder.torch_ops_stale()
