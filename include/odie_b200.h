@@ -419,6 +419,11 @@ ODIE_API int odie_linear(const void* x, const void* weight, const void* bias, co
                    int outputs, int groups, const int32_t* offsets, int dtype, int activation, void* y, void* slope,
                    void* scratch, uint64_t stream);
 ODIE_API int64_t odie_linear_backward_scratch(int64_t rows, int inputs, int outputs, int groups);
+/* The scratch of calls of which more is known, at most the above: with offsets or without (offsets 0), and on_16 != 0
+ * where every pointer of rows, weight, slope and their gradients starts on a 16-byte boundary.  One or two rows without
+ * offsets need none; backward, up to 64 inputs and outputs, multiples of 8, on_16, need sums of the weights alone. */
+ODIE_API int64_t odie_linear_scratch_for(int64_t rows, int inputs, int outputs, int groups, int offsets, int on_16);
+ODIE_API int64_t odie_linear_backward_scratch_for(int64_t rows, int inputs, int outputs, int groups, int on_16);
 ODIE_API int odie_linear_backward(const void* d_y, const void* slope, int activation, const void* x, const void* weight,
                    int64_t rows, int inputs, int outputs, int groups, const int32_t* offsets, int dtype, void* d_x, void* d_weight,
                    void* d_bias, void* d_residual, void* scratch, uint64_t stream);

@@ -81,6 +81,8 @@ SIGNATURES = {
     'odie_linear': (I32, [P, P, P, P, I64, I32, I32, I32, P, I32, I32, P, P, P, U64]),
     'odie_linear_backward_scratch': (I64, [I64, I32, I32, I32]),
     'odie_linear_backward': (I32, [P, P, I32, P, P, I64, I32, I32, I32, P, I32, P, P, P, P, P, U64]),
+    'odie_linear_scratch_for': (I64, [I64, I32, I32, I32, I32, I32]),
+    'odie_linear_backward_scratch_for': (I64, [I64, I32, I32, I32, I32]),
     'odie_linear_wait_limit': (I32, [I64]),
     'odie_linear_check': (I32, []),
     'odie_linear_status': (I32, [P, U64]),

@@ -1295,10 +1295,22 @@ struct BackwardScratch {
         split = static_cast<float*>(s.take(Splits(rows, inputs, outputs, groups, groups > 1).bytes(rows, inputs)));
         bytes = s.used;
         thin = static_cast<float*>(base);  // thin layers need nothing else
-        if (thin_sizes(inputs, outputs))
-            bytes = std::max(bytes, aligned(thin_units(rows, groups, thin_chunk(rows, inputs, outputs, ACT_NONE, true)) * (int64_t(outputs) * inputs + outputs) * 4));
+    }
+    // (the activation whose units are most)
+    static int64_t thin_bytes(int64_t rows, int inputs, int outputs, int groups) {
+        return aligned(thin_units(rows, groups, thin_chunk(rows, inputs, outputs, ACT_NONE, true)) * (int64_t(outputs) * inputs + outputs) * 4);
     }
 };
+
+// The kernels that serve a forward pass (thin.cu decides a ReLU's corner, so one or two thin rows with a ReLU go there);
+// a backward pass takes THIN or TILES.
+enum class Path { FEW, THIN, TILES };
+Path forward_path(int64_t rows, int inputs, int outputs, bool offsets, int activation, bool on_16) {
+    const bool thin = thin_sizes(inputs, outputs) && on_16;
+    if (rows <= FEW_ROWS && !offsets && !(thin && activation == ACT_RELU)) return Path::FEW;
+    return thin ? Path::THIN : Path::TILES;
+}
+Path backward_path(int inputs, int outputs, bool on_16) { return thin_sizes(inputs, outputs) && on_16 ? Path::THIN : Path::TILES; }
 
 bool sizes_fit(int64_t rows, int inputs, int outputs, int groups) {
     return rows >= 0 && rows < (int64_t(1) << 31) && inputs >= 1 && outputs >= 1 && inputs <= (1 << 20) && outputs <= (1 << 20) &&
@@ -1310,9 +1322,13 @@ bool sizes_fit(int64_t rows, int inputs, int outputs, int groups) {
 
 using namespace odie;
 
-extern "C" int64_t odie_linear_scratch(int64_t rows, int inputs, int outputs, int groups) {
+extern "C" int64_t odie_linear_scratch_for(int64_t rows, int inputs, int outputs, int groups, int offsets, int on_16) {
     if (!sizes_fit(rows, inputs, outputs, groups)) return 0;
-    return ForwardScratch(nullptr, rows, inputs, outputs, groups).bytes;
+    return forward_path(rows, inputs, outputs, offsets, ACT_NONE, on_16) == Path::TILES ? ForwardScratch(nullptr, rows, inputs, outputs, groups).bytes : 0;
+}
+
+extern "C" int64_t odie_linear_scratch(int64_t rows, int inputs, int outputs, int groups) {
+    return odie_linear_scratch_for(rows, inputs, outputs, groups, 1, 0);
 }
 
 extern "C" int odie_linear(const void* x, const void* weight, const void* bias, const void* residual, int64_t rows, int inputs,
@@ -1325,13 +1341,14 @@ extern "C" int odie_linear(const void* x, const void* weight, const void* bias, 
         int* const error = checked_error_word();
         if (activation == ACT_NONE) slope = nullptr;  // 1 everywhere
         const cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_handle);
-        const bool thin = thin_sizes(inputs, outputs) && on_16_bytes({x, weight, residual, y, activation == ACT_RELU ? nullptr : slope});
-        if (rows <= FEW_ROWS && !offsets && !(thin && activation == ACT_RELU)) {  // (thin layers decide a ReLU's corner)
+        const Path path = forward_path(rows, inputs, outputs, offsets, activation,
+                                       on_16_bytes({x, weight, residual, y, activation == ACT_RELU ? nullptr : slope}));
+        if (path == Path::FEW) {
             const FewArgs a{x, weight, bias, residual, y, slope, int(rows), inputs, outputs, activation};
             with_linear_type(dtype, [&](auto type) { launch_few_rows<decltype(type)>(a, stream); });
             return;
         }
-        if (thin) {
+        if (path == Path::THIN) {
             ThinArgs a{};
             a.rows = rows;
             a.inputs = inputs;
@@ -1377,9 +1394,14 @@ extern "C" int odie_linear(const void* x, const void* weight, const void* bias, 
     });
 }
 
-extern "C" int64_t odie_linear_backward_scratch(int64_t rows, int inputs, int outputs, int groups) {
+extern "C" int64_t odie_linear_backward_scratch_for(int64_t rows, int inputs, int outputs, int groups, int on_16) {
     if (!sizes_fit(rows, inputs, outputs, groups)) return 0;
+    if (backward_path(inputs, outputs, on_16) == Path::THIN) return BackwardScratch::thin_bytes(rows, inputs, outputs, groups);
     return BackwardScratch(nullptr, rows, inputs, outputs, groups).bytes;
+}
+
+extern "C" int64_t odie_linear_backward_scratch(int64_t rows, int inputs, int outputs, int groups) {
+    return std::max(odie_linear_backward_scratch_for(rows, inputs, outputs, groups, 0), odie_linear_backward_scratch_for(rows, inputs, outputs, groups, 1));
 }
 
 extern "C" int odie_linear_backward(const void* d_y, const void* slope, int activation, const void* x, const void* weight, int64_t rows,
@@ -1399,7 +1421,7 @@ extern "C" int odie_linear_backward(const void* d_y, const void* slope, int acti
         int* const error = checked_error_word();
         const int kind = slope_kind(activation, slope);
         const BackwardScratch s(scratch, rows, inputs, outputs, groups);
-        if (thin_sizes(inputs, outputs) && on_16_bytes({d_y, kind == SLOPE_CODES ? slope : nullptr, x, weight, d_x, d_residual})) {
+        if (backward_path(inputs, outputs, on_16_bytes({d_y, kind == SLOPE_CODES ? slope : nullptr, x, weight, d_x, d_residual})) == Path::THIN) {
             ThinArgs a{};
             a.rows = rows;
             a.inputs = inputs;

@@ -216,10 +216,11 @@ Tensor combine(const Tensor& rows, const Tensor& order, const Tensor& slot, cons
 }
 
 // ---------------------------------------------------------------- linear
-// Contiguous, starting on a 16-byte boundary (a view of an odd offset is copied).
+bool on_16_bytes(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+// Contiguous, starting on a 16-byte boundary (a view of an odd offset is copied), as every new tensor does.
 Tensor aligned(const Tensor& t) {
     const Tensor c = t.contiguous();
-    return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 == 0 ? c : c.clone();
+    return on_16_bytes(c) ? c : c.clone();
 }
 struct Sizes {
     int64_t rows, inputs, outputs, groups;
@@ -235,7 +236,8 @@ Tensor linear_forward(const Tensor& x, const Tensor& weight, const Tensor& bias,
     if (keep_slope)  // a ReLU's as bits
         slope = activation == 1 ? at::empty({s.rows, (s.outputs + 7) / 8}, x.options().dtype(at::kByte).requires_grad(false))
                                 : at::empty({s.rows, s.outputs}, x.options().dtype(at::kShort).requires_grad(false));
-    const Tensor work = scratch(x, odie_linear_scratch(s.rows, int(s.inputs), int(s.outputs), int(s.groups)));
+    const bool on_16 = !residual.defined() || on_16_bytes(residual);  // the others are
+    const Tensor work = scratch(x, odie_linear_scratch_for(s.rows, int(s.inputs), int(s.outputs), int(s.groups), offsets.defined(), on_16));
     done(odie_linear(data(x), data(weight), data(bias), data(residual), s.rows, int(s.inputs), int(s.outputs), int(s.groups),
                      static_cast<const int32_t*>(data(offsets)), row_type(x), int(activation), data(y), data(slope), data(work), stream_of(x)),
          "odie_linear");
@@ -275,7 +277,7 @@ struct Linear : torch::autograd::Function<Linear> {
         if (need & 4) d_bias = rows_like(d_y, at::IntArrayRef(shape.data(), shape.size() - 1));
         if (need & 8) d_residual = offsets.defined() ? rows_like(d_y, {rows, outputs}) : d_y;  // every row is a group's row
         if ((need & 7) || (need & 8 && offsets.defined())) {
-            const Tensor work = scratch(d_y, odie_linear_backward_scratch(rows, int(inputs), int(outputs), int(groups)));
+            const Tensor work = scratch(d_y, odie_linear_backward_scratch_for(rows, int(inputs), int(outputs), int(groups), 1));  // (see aligned)
             done(odie_linear_backward(data(d_y), data(slope), int(activation), data(x), data(weight), rows,
                                       int(inputs), int(outputs), int(groups), static_cast<const int32_t*>(data(offsets)), row_type(d_y),
                                       data(d_x), data(d_weight), data(d_bias), offsets.defined() ? data(d_residual) : nullptr, data(work),

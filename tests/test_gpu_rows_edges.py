@@ -333,3 +333,45 @@ print('the same')
     from pathlib import Path
     run = subprocess.run([sys.executable, '-c', program], capture_output=True, text=True, timeout=300, cwd=Path(__file__).resolve().parents[1])
     assert run.returncode == 0 and 'the same' in run.stdout, run.stderr
+
+
+# ---------------------------------------------------------------- memory
+def peak(call):
+    """(bytes that call takes beside its results, its results)."""
+    call()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    results = call()
+    torch.cuda.synchronize()
+    return torch.cuda.max_memory_allocated() - torch.cuda.memory_allocated(), results
+
+
+@pytest.mark.parametrize('rows', [1, 2])
+def test_few_rows_take_no_scratch(cuda, rows):
+    """No padded copy of the weights, whose rows are no multiple of 16 bytes."""
+    from odie_b200.experts import linear
+    g = generator(rows)
+    x, w = normal(g, rows, 1025, dtype=torch.float16), normal(g, 2000, 1025, dtype=torch.float16)
+    taken, y = peak(lambda: linear(x, w))
+    assert taken == 0
+    want, off = x.double() @ w.double().t(), 1026 * SUM * (x.double().abs() @ w.double().abs().t())
+    within(y, want, off + rounding(want.abs() + off, torch.float16), 'y')
+
+
+@pytest.mark.parametrize('shift', [0, 1])
+def test_thin_gradients_take_the_sums_of_the_weights_alone(cuda, shift):
+    """Also where the residual starts on no 16-byte boundary and the forward pass leaves the thin kernel."""
+    from odie_b200.experts import linear
+    g = generator(9)
+    rows, inputs, outputs = 1 << 17, 32, 64
+    x, w, b = (normal(g, *s, dtype=torch.float16).requires_grad_() for s in ((rows, inputs), (outputs, inputs), (outputs,)))
+    residual = normal(g, rows * outputs + 8, dtype=torch.float16)[shift:shift + rows * outputs].view(rows, outputs)
+    y = linear(x, w, b, residual, 'silu')
+    d = normal(g, rows, outputs, dtype=torch.float16)
+    taken, grads = peak(lambda: torch.autograd.grad(y, [x, w, b], d, retain_graph=True))
+    assert taken <= 4 << 20  # 412 units of 33 x 64 fp32 sums: 3.5 MB; dz would be 17 MB
+    plain = plain_linear(x.detach(), w.detach(), b.detach(), residual, [(0, rows)], 'silu', d)
+    within(y.detach(), *plain['y'], 'y')
+    for name, got in zip(('x', 'weight', 'bias'), grads):
+        within(got, *plain['d_' + name], 'd_' + name)

@@ -74,3 +74,17 @@ def test_torch_ops_of_another_torch_are_stale(lib, monkeypatch):
         builder.build()
         assert built
     assert not builder.torch_ops_stale()
+
+
+def test_linear_scratch_is_what_the_call_uses(lib):
+    """Nothing for one or two rows without offsets, the weights' sums alone behind thin layers; at most the general size."""
+    for rows, inputs, outputs, groups in ((1, 4097, 8192, 1), (2, 333, 515, 1), (1 << 20, 32, 64, 1), (1 << 20, 64, 64, 16), (700, 333, 72, 5),
+                                          (64, 4096, 4096, 1)):
+        most, most_back = lib.odie_linear_scratch(rows, inputs, outputs, groups), lib.odie_linear_backward_scratch(rows, inputs, outputs, groups)
+        for offsets in (0, 1):
+            for on_16 in (0, 1):
+                size, back = lib.odie_linear_scratch_for(rows, inputs, outputs, groups, offsets, on_16), lib.odie_linear_backward_scratch_for(rows, inputs, outputs, groups, on_16)
+                thin = on_16 and inputs <= 64 and outputs <= 64
+                assert size == (0 if thin or (rows <= 2 and not offsets) else most)
+                assert 0 < back <= most_back and (not thin or back <= 4 * (148 * 4 + groups + 1) * (inputs + 1) * outputs + 256)
+    assert lib.odie_linear_scratch_for(8, 0, 8, 1, 0, 1) == 0 and lib.odie_linear_backward_scratch_for(8, 8, 8, 1025, 1) == 0
