@@ -155,10 +155,21 @@ __global__ void __launch_bounds__(ROW_THREADS) combine_kernel(RowArgs a, const T
     }
 }
 
-// Walks the sorted rows.  The dot product's partial sums are joined in a fixed tree.  (2^20 rows of 32 fp16: 57 us at the
-// four blocks per SM that the compiler's registers leave, 53 at six.)
+// Blocks per SM of the gradient kernels, more of them at the price of spilled registers.  Us at none asked for (as the
+// compiler's registers leave), four, five and six, 2^20 rows of 32 and of 64:
+//   fp16  59, 59, 55, 53;  98, 98, 92, 84       fp32  98, 100, 92, 86;  184, 186, 170, 158
+//   bf16  72, 64, 66, 70;  127, 109, 111, 115   (its product takes more registers; at six it spills 56 bytes)
+// Wide rows, several choices, at none, two, three and four: 16384 rows of 2048, four choices, fp16 107, 121, 104, 100; bf16
+// 123, 123, 111, 115; fp32 188, 221, 193, 189; two choices of 4096, 139, 176, 139, 123; 180, 180, 150, 148; 229, 315, 258,
+// 231; 4-byte vectors, four choices of 1026 fp16 102, 100, 82, 104; bf16 168, 168, 143, 145; of 1025 fp32 148, 180, 145, 184.
 template <typename T, int BYTES, bool NARROW>
-__global__ void __launch_bounds__(ROW_THREADS, NARROW && BYTES == 16 ? 6 : 0) combine_backward_kernel(RowArgs a, const T* __restrict__ d_out,
+constexpr int GRADIENT_BLOCKS = NARROW && BYTES == 16 ? (std::is_same<T, __nv_bfloat16>::value ? 4 : 6) : 0;
+template <typename T, int BYTES>
+constexpr int GRADIENT_ROWS_BLOCKS = BYTES == 16 && !std::is_same<T, __nv_bfloat16>::value ? 4 : 3;
+
+// Walks the sorted rows.  The dot product's partial sums are joined in a fixed tree.
+template <typename T, int BYTES, bool NARROW>
+__global__ void __launch_bounds__(ROW_THREADS, (GRADIENT_BLOCKS<T, BYTES, NARROW>)) combine_backward_kernel(RowArgs a, const T* __restrict__ d_out,
                                                                        const T* __restrict__ sorted, T* __restrict__ d_sorted,
                                                                        float* __restrict__ d_weights) {
     using P = Pack<T, BYTES>;
@@ -228,7 +239,7 @@ __global__ void __launch_bounds__(ROW_THREADS, NARROW && BYTES == 16 ? 6 : 0) co
 
 // The same for wide rows with several choices, walking the unsorted rows: d out is read once for up to four choices.
 template <typename T, int BYTES>
-__global__ void __launch_bounds__(ROW_THREADS, 3) combine_backward_rows_kernel(RowArgs a, const T* __restrict__ d_out,
+__global__ void __launch_bounds__(ROW_THREADS, (GRADIENT_ROWS_BLOCKS<T, BYTES>)) combine_backward_rows_kernel(RowArgs a, const T* __restrict__ d_out,
                                                                             const T* __restrict__ sorted, T* __restrict__ d_sorted,
                                                                             float* __restrict__ d_weights) {
     using P = Pack<T, BYTES>;
