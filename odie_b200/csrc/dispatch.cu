@@ -6,7 +6,7 @@
 //   backward   d sorted[slot] = w d out[t], d w[t, j] = <sorted[slot], d out[t]> in fp32
 // The gradient of dispatch is combine without weights.  All are bound by the bytes of the rows.  Kernels walk the
 // side that they write, so that writes are whole lines in order and only reads are scattered (writes of 64-byte rows
-// to their places took half as long again: 47 us against 27 for 2^20 rows of 32 fp16), but for wide rows with several
+// to their places took half as long again), but for wide rows with several
 // choices, whose places are whole lines anyway.
 #include "rows.cuh"
 #include "odie_b200.h"
@@ -26,7 +26,8 @@ struct RowArgs {
 };
 
 // Rows that a thread takes of narrow ones, or vectors of a wide one.  (2^20 rows of 32 fp16: 51 us with one row, 35 with
-// two, 41 with four, whose registers leave half the blocks; 4-byte vectors, rows of 20 fp16: 85 with two, 72 with four.)
+// two, 41 with four, whose registers leave half the blocks; 4-byte vectors, rows of 20 fp16: 84 with two, 72 with four; all
+// with L2 cold, one call at a time, ten in a row 44, 29, 33 and 75, 62.)
 template <int BYTES, bool NARROW>
 constexpr int DISPATCH_ITEMS = NARROW && BYTES == 16 ? 2 : 4;
 

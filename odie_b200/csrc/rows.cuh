@@ -1,4 +1,4 @@
-// Rows of any width and type, loaded and stored a vector at a time (rows.cu, embed.cu, linear.cu).
+// Rows of any width and type, loaded and stored a vector at a time (dispatch.cu, embed.cu, linear.cu).
 #pragma once
 #include <cuda_bf16.h>
 #include "common.cuh"

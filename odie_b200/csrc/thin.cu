@@ -3,9 +3,10 @@
 // Bound by the bytes of the rows (64 to 128 bytes each), not by arithmetic: 2^20 rows of 32 -> 64 fp16 are 192 MB
 // forward against 4.3 GFLOP.  So a warp keeps its 16 rows in registers from the 16-byte loads to the 16-byte stores
 // and multiplies them with mma.sync fragments.  (The tensor-core tiles of linear.cu, whose rows pass through shared
-// memory, TMEM and a staging tile, took 102 us forward and 205 us in four kernels backward; these take 45 and 57 with
-// ReLU, 4.4 and 4.7 TB/s.  What is left is the issue of about 400 instructions per warp and 16 rows, at 12 to 16 warps
-// per SM.)
+// memory, TMEM and a staging tile, took 102 us forward and 205 us in four kernels backward; these take 47 and 55 with
+// ReLU, 4.2 and 4.7 TB/s.  What is left is the wait of an instruction for the one before: registers leave room for 12
+// warps per SM, each issues every 4.9 cycles forward and every 6.7 backward, 1.2 and 2.3 of them such waits, backward 0.9
+// for memory; issue slots are 56 and 44 % busy.)
 //
 // The fragments' order of columns is chosen so that no data is exchanged.  Lane (g, c) = (lane / 4, lane % 4) loads
 // the 8 columns 8 c .. 8 c + 7 of rows g and g + 8 for each 32-column block: word i (columns 8 c + 2 i, + 1) is what
@@ -15,9 +16,9 @@
 // each 8 x 8 tile, in the same order of columns.
 //
 // A ReLU's corner: where the tensor cores' sum is within its own error of zero, the fp32 chain of fused multiply-adds
-// in ascending order of the inputs decides (the convention of this library's router), so that a unit is on or off as
-// in any fp32 evaluation of the layer; at these sizes one unit is a large part of a row's gradient.  About one step of
-// 16 rows in forty looks at a chain.
+// in ascending order of the inputs decides (the convention of this library's router), since at these sizes one unit is a
+// large part of a row's gradient.  (Its own error is an estimate: 2^-20 of inputs x the largest input x the largest weight.
+// An fp32 sum in another order may still differ in sign from the chain.)  About one step of 16 rows in forty looks at one.
 #include "thin.cuh"
 #include "odie_b200.h"
 #include <algorithm>

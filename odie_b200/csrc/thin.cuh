@@ -29,8 +29,8 @@ struct ThinArgs {
 };
 
 inline bool thin_sizes(int inputs, int outputs) { return inputs <= 64 && outputs <= 64 && inputs % 8 == 0 && outputs % 8 == 0; }
-// Blocks that share an SM: as many as their registers allow without spilling (a ReLU's corner takes some: at 2^20 rows of
-// 32 -> 64 fp16 four blocks took 60 us, three 50) and, backward, the rows on their way in shared memory.  Backward with
+// Blocks that share an SM: as many as their registers allow without spilling (a ReLU's corner takes some: 2^20 rows of
+// 32 -> 64, 64 -> 64 and 32 -> 32 fp16 take 61, 80 and 39 us at a block more, 47, 70 and 37 so) and, backward, the rows on their way in shared memory.  Backward with
 // codes: two, with more stages each.
 constexpr int thin_blocks(int inputs, int outputs, int activation, bool backward) {
     const int wide = (inputs > 32) + (outputs > 32);

@@ -104,9 +104,10 @@ def check(device=None):
 
 # ---------------------------------------------------------------- a model of them
 class ExpertHeads(nn.Module):
-    """The MLP of `model.Head` (ReLU hidden layers, linear output, fp16 activations, fp32 masters) with biases, one
+    """An MLP like `model.Head` (ReLU hidden layers, linear output, fp16 activations, fp32 masters) with biases, one
     set of weights per expert and, with codes > 0, a learned input code for each of that many ids (the tile of a
-    coordinate, say) added to the features."""
+    coordinate, say) added to the features.  Weights start uniform within sqrt(6 / (inputs + outputs)) of the layer's own
+    sizes (`Head` draws matrices padded to 16, so the same seed gives others there)."""
 
     def __init__(self, n_input, n_output, width, depth, experts, seed, codes=0, device='cuda'):
         super().__init__()
