@@ -451,6 +451,75 @@ ODIE_API int64_t odie_embed_backward_scratch(int64_t n, int64_t rows, int64_t wi
 ODIE_API int odie_embed_backward(const void* ids, int id_bytes, int64_t n, const void* d_out, int64_t rows, int64_t width,
                    int dtype, float scale, void* d_table, void* scratch, uint64_t stream);
 
+/* ------------------------------------------------------------------------
+ * The router of the experts (no reference counterpart): choices and weights
+ * from logits[rows][experts] (dtype as above; up to 1024 experts), and the
+ * load's balance.  mask (may be NULL): u8, expert e is open to row t where
+ * mask[t * mask_row_step + e * mask_expert_step] != 0 (steps may be 0).
+ * score: 0 softmax over the row's open experts, 1 sigmoid of each.
+ *
+ * odie_gate: expert i32[rows][choices], weights f32[rows][choices]: the open
+ * experts of the highest fp32(logit) + bias[e] (bias f32[experts], may be
+ * NULL; NaN above all, -inf is not taken), ties to the lowest; -1 with weight
+ * 0 where none is left.  weights: scale times the score (the bias is not in
+ * it), with normalize divided by the sum over the row's choices.  Up to 64
+ * choices, scale finite and not 0.
+ * odie_gate_backward: d_logits[rows][experts] for d_weights
+ * f32[rows][choices], from odie_gate's results and its logits and mask
+ * (neither is read for a normalised softmax, the mask for no sigmoid).
+ * odie_balance: *loss = experts * sum_e f_e P_e and *z = the mean square of
+ * log sum_e e^logit; P the mean over live rows (with an open expert of a logit
+ * above -inf) of the softmax (or the sigmoids divided by their sum), f_e =
+ * n_e / sum n, n the counts i32[experts] of the `pairs` choices in expert
+ * (int32 or int64: key_bytes; others than [0, experts) are dropped), or total
+ * i64[experts] (may be NULL) in their place.  0 without rows or choices.
+ * stats f32[experts + 1] is kept for odie_balance_backward: d_logits for
+ * *d_loss and *d_z (device, may be NULL: 0); f has no gradient.
+ * ------------------------------------------------------------------------ */
+ODIE_API int odie_gate(const void* logits, int64_t rows, int experts, int dtype, const float* bias, const uint8_t* mask,
+                   int64_t mask_row_step, int64_t mask_expert_step, int choices, int score, int normalize, float scale,
+                   int32_t* expert, float* weights, uint64_t stream);
+ODIE_API int odie_gate_backward(const float* d_weights, const void* logits, int64_t rows, int experts, int dtype,
+                   const uint8_t* mask, int64_t mask_row_step, int64_t mask_expert_step, const int32_t* expert,
+                   const float* weights, int choices, int score, int normalize, float scale, void* d_logits, uint64_t stream);
+ODIE_API int64_t odie_balance_scratch(int64_t rows, int experts);
+ODIE_API int odie_balance(const void* logits, int64_t rows, int experts, int dtype, const uint8_t* mask, int64_t mask_row_step,
+                   int64_t mask_expert_step, int score, const void* expert, int key_bytes, int64_t pairs, const int64_t* total,
+                   float* loss, float* z, int32_t* counts, float* stats, void* scratch, uint64_t stream);
+ODIE_API int odie_balance_backward(const float* d_loss, const float* d_z, const void* logits, int64_t rows, int experts,
+                   int dtype, const uint8_t* mask, int64_t mask_row_step, int64_t mask_expert_step, int score,
+                   const float* stats, void* d_logits, uint64_t stream);
+
+/* ------------------------------------------------------------------------
+ * Microscaled 4-bit rows (no reference counterpart): value = R s c, c in e2m1,
+ * s one scale per block of 16 values (e4m3) or 32 (e8m0, powers of two) of a
+ * row, R one fp32 power of two per row (1 with blocks of 32).
+ *   16: R = the least 2^k, k >= -126, with max |row| <= 2688 R (1 for zeros);
+ *       s = max |block| / (6 R); c = x / (R s), 0 where s is
+ *   32: s = the least 2^e, e >= -127, with max |block| <= 6 s; c = x / s
+ * rounded once each, to nearest even, saturating.  A row with an infinity or a
+ * NaN has R = NaN and codes 0.
+ * groups x rows x width values lie as codes u8[groups * rows][pitch], pitch =
+ * 16 ceil(width / 32), two to a byte, the even one low, zeros behind; scales
+ * u8[groups][ceil(rows / 128)][ceil(width / (4 block))][512]: row r, block b of
+ * a tile at byte 16 (r % 32) + 4 (r / 32) + b; row_scales f32[groups * rows].
+ * codes and scales start on 16-byte boundaries.
+ * odie_quantize: from x (dtype as above).  odie_dequantize: to out, rounded to
+ * its dtype.
+ * odie_linear4: odie_linear's y with W as such codes (groups x outputs x
+ * inputs) and x (fp16 or bf16) quantised in the same way, row by row, before
+ * the product; fp32 sums, one rounding.  No gradients.  scratch as sized for
+ * the same offsets (0: NULL) and block.  Its waits are those of odie_linear.
+ * ------------------------------------------------------------------------ */
+ODIE_API int odie_quantize(const void* x, int64_t groups, int64_t rows, int64_t width, int dtype, int block, uint8_t* codes,
+                   uint8_t* scales, float* row_scales, uint64_t stream);
+ODIE_API int odie_dequantize(const uint8_t* codes, const uint8_t* scales, const float* row_scales, int64_t groups, int64_t rows,
+                   int64_t width, int block, int dtype, void* out, uint64_t stream);
+ODIE_API int64_t odie_linear4_scratch(int64_t rows, int inputs, int outputs, int groups, int offsets, int block);
+ODIE_API int odie_linear4(const void* x, const uint8_t* codes, const uint8_t* scales, const float* row_scales, int block,
+                   const void* bias, const void* residual, int64_t rows, int inputs, int outputs, int groups,
+                   const int32_t* offsets, int dtype, int activation, void* y, void* scratch, uint64_t stream);
+
 #ifdef __cplusplus
 }
 #endif

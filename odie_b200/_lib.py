@@ -86,6 +86,15 @@ SIGNATURES = {
     'odie_linear_wait_limit': (I32, [I64]),
     'odie_linear_check': (I32, []),
     'odie_linear_status': (I32, [P, U64]),
+    'odie_gate': (I32, [P, I64, I32, I32, P, P, I64, I64, I32, I32, I32, F32, P, P, U64]),
+    'odie_gate_backward': (I32, [P, P, I64, I32, I32, P, I64, I64, P, P, I32, I32, I32, F32, P, U64]),
+    'odie_balance_scratch': (I64, [I64, I32]),
+    'odie_balance': (I32, [P, I64, I32, I32, P, I64, I64, I32, P, I32, I64, P, P, P, P, P, P, U64]),
+    'odie_balance_backward': (I32, [P, P, P, I64, I32, I32, P, I64, I64, I32, P, P, U64]),
+    'odie_quantize': (I32, [P, I64, I64, I64, I32, I32, P, P, P, U64]),
+    'odie_dequantize': (I32, [P, P, P, I64, I64, I64, I32, I32, P, U64]),
+    'odie_linear4_scratch': (I64, [I64, I32, I32, I32, I32, I32]),
+    'odie_linear4': (I32, [P, P, P, P, I32, P, P, I64, I32, I32, I32, P, I32, I32, P, P, U64]),
     'odie_embed': (I32, [P, I32, I64, P, I64, I64, I32, F32, P, U64]),
     'odie_embed_backward_scratch': (I64, [I64, I64, I64]),
     'odie_embed_backward': (I32, [P, I32, I64, P, I64, I64, I32, F32, P, P, U64]),

@@ -16,7 +16,8 @@ from pathlib import Path
 PACKAGE = Path(__file__).resolve().parent
 ROOT = PACKAGE.parent
 SOURCES = ['encode.cu', 'step.cu', 'mlp_tc.cu', 'router.cu', 'probe.cu', 'layout.cu', 'residual.cu', 'selection.cu',
-           'synth.cu', 'hashgrid32.cu', 'sort.cu', 'dispatch.cu', 'embed.cu', 'thin.cu', 'linear.cu',
+           'synth.cu', 'hashgrid32.cu', 'sort.cu', 'dispatch.cu', 'embed.cu', 'thin.cu', 'linear.cu', 'gate.cu', 'balance.cu',
+           'micro.cu', 'linear4.cu',
            'runtime.cu']
 LIBRARY = PACKAGE / 'libodie_b200.so'
 TORCH_OPS = PACKAGE / '_torch_ops.so'  # a Python extension module: odie_b200._torch_ops

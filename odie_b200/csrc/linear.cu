@@ -15,9 +15,7 @@
 // without (a ReLU's dz is exact).
 #include "thin.cuh"
 #include "odie_b200.h"
-#include "tc.cuh"
-#include <cuda.h>
-#include <cudaTypedefs.h>
+#include "product.cuh"
 #include <algorithm>
 #include <atomic>
 #include <initializer_list>
@@ -46,18 +44,6 @@ enum Mode : int { FWD = 0, DX = 1, DW = 2 };
 
 constexpr int BK = 64;
 constexpr int EPILOGUE_WARP = 4;  // the first one
-// Polls of a wait, up to 4 us each: some ten seconds.  Waits of the products have GemmArgs::limit, what gives up waits for
-// its own copies and products with this one.
-constexpr uint32_t WAIT_LIMIT = 1u << 22;
-constexpr int STAGING = 2048;  // bytes per epilogue warp: 32 rows x 32 columns of 16 bits
-
-// n / d for 0 <= n < 2^31 by a multiplication: m = ceil(2^64 / d).
-struct Divide {
-    unsigned long long m;
-    uint32_t d;
-    static Divide by(int64_t d) { return {d > 1 ? ~0ull / uint64_t(d) + 1 : 0, uint32_t(d)}; }
-    __device__ __forceinline__ int operator()(int n) const { return d == 1 ? n : int(__umul64hi((unsigned long long)n, m)); }
-};
 
 struct GemmArgs {
     int groups;
@@ -111,11 +97,6 @@ struct Tile {
     int unit;            // index of the partial sum
     bool zero;           // nothing to sum: zeros are stored
 };
-
-constexpr int BAND = 16;  // row tiles walked together, so that a W tile serves them from L2
-
-// The same value in every lane, as the compiler sees too.
-__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
 
 // A role's walk over the tiles, in ascending order: the group is found by stepping on from the last one, and no integer
 // division is left (each of twenty warps walks; dividing, they spent four instructions per output element on it).
@@ -178,91 +159,6 @@ struct Walk {
         return tile;
     }
 };
-
-// The staging tile of an epilogue warp: 32 rows of 64 bytes, the 16-byte units of a row permuted so that both a
-// thread per row and four threads per row meet no bank twice.
-__device__ __forceinline__ uint4* staged(char* base, int row, int unit) {
-    return reinterpret_cast<uint4*>(base + row * 64 + ((unit ^ ((row >> 1) & 3)) << 4));
-}
-
-// 32 rows x 32 columns of a row-major 16-bit matrix, moved between global memory and the staging tile.  Where every
-// row starts on a 16-byte boundary, thread (lane) moves the 16-byte unit lane % 4 of rows lane / 4 + 8 i, else the
-// element `lane` of every row.
-struct Window {
-    int ld;
-    int rows, columns;  // inside the matrix
-    bool wide;          // 16-byte accesses
-};
-__device__ __forceinline__ void window_load(const uint16_t* at, const Window& w, int lane, uint4 (&v)[4]) {
-    const int r = lane / 4, c = (lane & 3) * 8;
-    const uint16_t* from = at + (long long)r * w.ld + c;
-    const long long step = 8ll * w.ld;
-    if (w.rows == 32 && w.columns >= 32) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i, from += step) v[i] = __ldg(reinterpret_cast<const uint4*>(from));
-    } else if (c + 8 <= w.columns) {  // wide rows: columns are a multiple of 8
-#pragma unroll
-        for (int i = 0; i < 4; ++i, from += step)
-            v[i] = r + 8 * i < w.rows ? __ldg(reinterpret_cast<const uint4*>(from)) : make_uint4(0, 0, 0, 0);
-    }
-}
-__device__ __forceinline__ uint16_t* staged_element(char* base, int row, int c) {
-    return reinterpret_cast<uint16_t*>(staged(base, row, c >> 3)) + (c & 7);
-}
-__device__ __forceinline__ void window_fetch(const uint16_t* at, const Window& w, int lane, char* staging) {
-    if (lane < w.columns) {
-#pragma unroll 8
-        for (int r = 0; r < w.rows; ++r) *staged_element(staging, r, lane) = at[(long long)r * w.ld + lane];
-    }
-}
-__device__ __forceinline__ void window_store(uint16_t* at, const Window& w, int lane, char* staging) {
-    if (w.wide) {
-        const int r = lane / 4, c = (lane & 3) * 8;
-        uint16_t* to = at + (long long)r * w.ld + c;
-        const long long step = 8ll * w.ld;
-        // rows r + 8 i share the permutation of row r: 512 bytes apart
-        const uint4* from = staged(staging, r, lane & 3);
-        if (w.rows == 32 && w.columns >= 32) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i, to += step) *reinterpret_cast<uint4*>(to) = from[i * 32];
-        } else if (c + 8 <= w.columns) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i, to += step)
-                if (r + 8 * i < w.rows) *reinterpret_cast<uint4*>(to) = from[i * 32];
-        }
-    } else if (lane < w.columns) {
-#pragma unroll 8
-        for (int r = 0; r < w.rows; ++r) at[(long long)r * w.ld + lane] = *staged_element(staging, r, lane);
-    }
-}
-
-template <int ACT>
-__device__ __forceinline__ void finish(float (&v)[32], uint32_t (&codes)[16], const float* bias) {
-#pragma unroll
-    for (int i = 0; i < 32; i += 4) {
-        const float4 b = *reinterpret_cast<const float4*>(bias + i);
-#pragma unroll
-        for (int j = 0; j < 4; j += 2) {
-            Pair slope;
-            const float2 y = both(activate<ACT>(add2(pair(v[i + j], v[i + j + 1]), j ? pair(b.z, b.w) : pair(b.x, b.y)), slope));
-            v[i + j] = y.x;
-            v[i + j + 1] = y.y;
-            codes[(i + j) / 2] = slope_codes(slope);
-        }
-    }
-}
-// ReLU: gives a mask, a bit where it is on.
-__device__ __forceinline__ uint32_t finish_relu(float (&v)[32], const float* bias) {
-    uint32_t off = 0;
-#pragma unroll
-    for (int i = 30; i >= 0; i -= 2) {
-        const float2 z = both(add2(pair(v[i], v[i + 1]), pair(bias[i], bias[i + 1])));
-        off = off_bits(off, z.x, z.y);
-        v[i] = max_nan(z.x, 0.0f);
-        v[i + 1] = max_nan(z.y, 0.0f);
-    }
-    return ~off;
-}
 
 // A row's bits of 32 columns, per lane (rows: of the window inside the matrix, columns: from `column` on).
 __device__ __forceinline__ void mask_store(const GemmArgs& p, int row, int column, int rows, int columns, int lane, uint32_t mask) {
@@ -985,6 +881,8 @@ int* error_word() {
     return words + device;
 }
 
+}  // namespace
+
 // Refuses once after a wait has run out.
 int* checked_error_word() {
     int* word = error_word();
@@ -993,7 +891,9 @@ int* checked_error_word() {
     return word;
 }
 
-PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+uint32_t product_wait_limit() { return wait_limit; }
+
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
     static const PFN_cuTensorMapEncodeTiled_v12000 found = [] {
         void* f = nullptr;
         cudaDriverEntryPointQueryResult status;
@@ -1004,6 +904,8 @@ PFN_cuTensorMapEncodeTiled_v12000 encoder() {
     return found;
 }
 
+namespace {
+
 // A row-major [depth][rows][width] matrix of 16-bit elements with rows of ld elements; boxes of 64 columns x box_rows.
 CUtensorMap tensor_map(const void* base, bool bf16, int64_t width, int64_t rows, int64_t depth, int64_t ld, int box_rows) {
     CUtensorMap map;
@@ -1011,7 +913,7 @@ CUtensorMap tensor_map(const void* base, bool bf16, int64_t width, int64_t rows,
     const cuuint64_t strides[2] = {cuuint64_t(ld * 2), cuuint64_t(rows * ld * 2)};
     const cuuint32_t box[3] = {64, cuuint32_t(box_rows), 1}, unit[3] = {1, 1, 1};
     ODIE_REQUIRE(uintptr_t(base) % 16 == 0, "x, weight, d_y and scratch must start on 16-byte boundaries");
-    const CUresult status = encoder()(&map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, depth ? 3 : 2,
+    const CUresult status = tensor_map_encoder()(&map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, depth ? 3 : 2,
                                       const_cast<void*>(base), dims, strides, box, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
                                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     ODIE_REQUIRE(status == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with " + std::to_string(int(status)));

@@ -1,0 +1,707 @@
+// y = residual + act(q(x) W_g^T + b_g): rows and weights as microscaled 4-bit floats (micro.cuh), one weight matrix or
+// one per group of consecutive rows; fp32 sums, one rounding.  x is quantised first, in a kernel of its own, its scales
+// cut into tiles from each group's first row on, so that the products load them as they need them.
+//
+// Rows of no group (behind the last offset) give zero rows of y.
+#include "micro.cuh"
+#include "odie_b200.h"
+#include "product.cuh"
+#include <algorithm>
+#include <type_traits>
+
+namespace odie {
+namespace {
+
+// ---------------------------------------------------------------- the tensor-core product
+//
+// C = A B^T over tiles of 128 CG x BN, K in blocks of 256 values (128 bytes), by CG CTAs of an SM pair (CG = 2: 256 x
+// 256 tiles, each CTA holding its 128 rows of A and half of B's) or one (CG = 1: 128 x 128).
+// One warp loads codes (128-byte swizzle) and scales by TMA, STAGES blocks in flight; one thread copies the block's
+// scales to TMEM and multiplies (tcgen05 kind::mxf4nvf4, a K-step of 64) into one of two accumulators; sixteen warps
+// take the other one to global memory, with the rows' own scales, bias, activation and residual.  A CTA of a pair needs
+// the scales of its own rows of A and of all of B's.
+//
+// TMEM has 512 columns.  A pair's two accumulators of 256 overlap by half ([0, 256) and [128, 384)), which leaves 128
+// for two blocks' scales; the epilogue reads the shared half first, and the next tile's products wait for that alone.
+constexpr int BK = 256;
+constexpr int EPILOGUE_WARP = 4;  // the first one
+
+struct Gemm4Args {
+    int groups;
+    const int* offsets;  // null: one group of all rows
+    long long rows;
+    int n;               // outputs
+    int k;               // inputs
+    int a_rows;          // rows of A's boxes: 128 or, for fewer rows in all, those (rounded up to 8)
+    int a_tiles;         // tiles of A's scales that there are
+    int chunk, splits;   // without offsets: the sum over K cut among this many tiles of `chunk` blocks, joined by finish4_kernel
+    Divide by_bands;     // tiles of a full band
+    Divide by_tiles;     // splits: tiles of C
+    const float* row_scales;     // [rows]
+    const float* column_scales;  // [groups][n]
+    const void* bias;
+    const void* residual;
+    void* out;
+    int activation;
+    float* partial;      // splits: [split][rows][n] sums
+    int* error;          // on the host: 2 once a wait has run out
+    uint32_t limit;      // polls of a wait
+};
+
+template <int CG, int BN, int BLOCK>
+struct Shape4 {
+    static constexpr int TM = 128 * CG;
+    static constexpr int B_ROWS = BN / CG;  // per CTA
+    static constexpr int COLUMN_TILES = BK / (4 * BLOCK);  // tiles of scales in a block of K: 4 or 2
+    static constexpr int A_BYTES = 128 * 128, B_BYTES = B_ROWS * 128;
+    static constexpr int SA_BYTES = COLUMN_TILES * MICRO_TILE, SB_BYTES = BN / 128 * SA_BYTES;
+    static constexpr int STAGE = A_BYTES + B_BYTES + SA_BYTES + SB_BYTES;
+    static constexpr int STAGE_PITCH = (STAGE + 1023) / 1024 * 1024;
+    static constexpr int STAGES = 4;
+    static constexpr int EPILOGUE_WARPS = 16, THREADS = (EPILOGUE_WARP + EPILOGUE_WARPS) * 32;
+    static constexpr int GROUPS = EPILOGUE_WARPS / 4;   // epilogue warps per set of 32 TMEM lanes
+    static constexpr int WINDOWS = BN / 32 / GROUPS;    // per warp and tile: columns 32 (group + GROUPS j)
+    static constexpr bool OVERLAP = BN == 256;
+    static constexpr int SCALES_AT = OVERLAP ? 384 : 256;  // TMEM column of the scales, 64 per block
+    static constexpr int SB_AT = COLUMN_TILES * 4;         // B's behind A's
+    static constexpr int COLUMNS = 512;
+    static constexpr int WARP_BYTES = STAGING + WINDOWS * 256;  // staging tile, bias and column scales of an epilogue warp
+    static constexpr int HEAD = 1024;                           // barriers, TMEM address
+    static int bytes(int groups) { return 1024 + STAGES * STAGE_PITCH + EPILOGUE_WARPS * WARP_BYTES + HEAD + 3 * (groups + 2) * 4; }
+};
+
+struct Tile4 {
+    int g;
+    int m0, n0;    // first row and column
+    int m_end;     // rows from here on are not stored
+    int k0;        // first block of K
+    int k_blocks;
+    int split;
+    int scales;    // tile of A's scales of row m0
+    bool zero;     // nothing to sum: zeros are stored
+};
+
+// A role's walk over the tiles, in ascending order (as in linear.cu).
+template <int CG, int BN, bool PARTIAL>
+struct Walk4 {
+    const Gemm4Args& p;
+    const int* begin;
+    const int* first;
+    const int* scales;
+    int g = 0;
+    __device__ __forceinline__ Walk4(const Gemm4Args& args, const int* b, const int* f, const int* s) : p(args), begin(b), first(f), scales(s) {}
+    __device__ __forceinline__ Tile4 at(int t) {
+        constexpr int TM = 128 * CG;
+        Tile4 tile;
+        int key = t, split = 0;
+        if (PARTIAL) {
+            split = p.by_tiles(t);
+            key = t - split * int(p.by_tiles.d);
+        }
+        // (a CTA's tiles ascend in t but, with splits, not in `key`: there is one group then, or the rows of none)
+        if (PARTIAL) g = 0;
+        while (g < p.groups && uniform(first[g + 1]) <= key) ++g;
+        tile.g = g;
+        const int from = uniform(begin[g]), to = g < p.groups ? uniform(begin[g + 1]) : int(p.rows);
+        int local = key - uniform(first[g]);
+        const int band = p.by_bands(local), left = (to - from + TM - 1) / TM - band * BAND;
+        local -= band * int(p.by_bands.d);
+        int n = local / BAND, m = local % BAND;
+        if (left < BAND) {  // local < 2^18: the quotient is off by one at most
+            n = int((float(local) + 0.5f) * inverse_approx(float(left)));
+            m = local - n * left;
+            if (m < 0) {
+                --n;
+                m += left;
+            } else if (m >= left) {
+                ++n;
+                m -= left;
+            }
+        }
+        tile.m0 = from + (band * BAND + m) * TM;
+        tile.n0 = n * BN;
+        tile.m_end = to;
+        tile.split = split;
+        tile.k0 = PARTIAL ? split * p.chunk : 0;
+        tile.k_blocks = (p.k + BK - 1) / BK;
+        if (PARTIAL) tile.k_blocks = min(tile.k_blocks - tile.k0, p.chunk);
+        tile.scales = uniform(scales[g]) + (band * BAND + m) * CG;
+        tile.zero = g == p.groups;
+        return tile;
+    }
+};
+
+// PARTIAL: the sums go to p.partial as they are, joined by finish4_kernel.
+template <typename T, int CG, int BN, int BLOCK, bool PARTIAL>
+__global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
+    gemm4_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                 const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb, const Gemm4Args p) {
+    using S = Shape4<CG, BN, BLOCK>;
+    constexpr int STAGES = S::STAGES;
+    extern __shared__ char raw[];
+    char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) / 1024 * 1024);
+    char* stages = smem;
+    char* staging = stages + STAGES * S::STAGE_PITCH;
+    uint64_t* full = reinterpret_cast<uint64_t*>(staging + S::EPILOGUE_WARPS * S::WARP_BYTES);
+    uint64_t* empty = full + STAGES;
+    uint64_t* done = empty + STAGES;    // per accumulator: summed
+    uint64_t* drained = done + 2;       // per accumulator: read out (OVERLAP: what it shares with the other one)
+    uint64_t* drain = drained + 2;
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drain + 1);
+    uint32_t* gave_up = tmem_at + 1;    // a wait of either CTA has run out
+    uint32_t* issued_by = gave_up + 1;  // [2], the leader's: blocks that each CTA has loaded
+    int* begin = reinterpret_cast<int*>(reinterpret_cast<char*>(full) + S::HEAD);  // [groups + 2] first row of each group
+    int* first = begin + p.groups + 2;                                            // [groups + 2] first tile
+    int* scales = first + p.groups + 2;                                           // [groups + 2] first tile of A's scales
+
+    const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const int rank = CG == 2 ? uniform(tc::cluster_rank()) : 0;
+    const int nt = (p.n + BN - 1) / BN;
+
+    if (warp == 0 && lane == 0) {
+        for (int s = 0; s < STAGES; ++s) {
+            tc::bar_init(full + s, 1);
+            tc::bar_init(empty + s, 1);
+        }
+        for (int a = 0; a < 2; ++a) {
+            tc::bar_init(done + a, 1);
+            tc::bar_init(drained + a, S::EPILOGUE_WARPS * CG);
+        }
+        tc::bar_init(drain, 1);
+        tc::fence_bar_init();
+        *gave_up = issued_by[0] = issued_by[1] = 0;
+    }
+    if (warp == 2) tc::tmem_alloc_group<CG>(tmem_at, S::COLUMNS);
+    if (warp == 3) {  // the groups' rows, tiles and tiles of scales
+        int tiles = 0, units = 0;
+        for (int g0 = 0; g0 <= p.groups; g0 += 32) {
+            const int g = g0 + lane;
+            int count = 0, unit = 0;
+            if (g <= p.groups) {
+                long long from = 0, to = 0;
+                if (g < p.groups) {
+                    group_rows(p.offsets, g, p.rows, from, to);
+                } else {  // the rows of no group
+                    long long b;
+                    group_rows(p.offsets, p.groups - 1, p.rows, b, from);
+                    to = p.rows;
+                }
+                begin[g] = int(from);
+                count = int((to - from + S::TM - 1) / S::TM) * nt;
+                unit = int((to - from + MICRO_ROWS - 1) / MICRO_ROWS);
+            }
+            int sum = count, unit_sum = unit;
+#pragma unroll
+            for (int d = 1; d < 32; d *= 2) {
+                const int other = __shfl_up_sync(0xffffffffu, sum, d), other_unit = __shfl_up_sync(0xffffffffu, unit_sum, d);
+                if (lane >= d) {
+                    sum += other;
+                    unit_sum += other_unit;
+                }
+            }
+            if (g <= p.groups) {
+                first[g] = tiles + sum - count;
+                scales[g] = units + unit_sum - unit;
+            }
+            tiles += __shfl_sync(0xffffffffu, sum, 31);
+            units += __shfl_sync(0xffffffffu, unit_sum, 31);
+        }
+        if (lane == 0) first[p.groups + 1] = tiles;
+    }
+    tc::fence_before_sync();
+    __syncthreads();
+    if (CG == 2) tc::cluster_sync();
+    tc::fence_after_sync();
+    const uint32_t tmem = uniform(*tmem_at);
+    const uint32_t full_leader = CG == 2 ? uniform(tc::leader_address(full)) : 0;
+    const int units = uniform(first[p.groups + 1]);
+    const int tiles = PARTIAL ? units * p.splits : units;
+    const int start = int(blockIdx.x) / CG, step = int(gridDim.x) / CG;
+    bool fine = true;
+    Walk4<CG, BN, PARTIAL> walk(p, begin, first, scales);
+
+    // The loading and the multiplying warp walk their loops with all lanes, and one lane issues (see linear.cu).
+    if (warp == 0) {
+        const bool issuer = tc::elect_one();
+        const uint32_t stage_bytes = uint32_t(p.a_rows * 128 + S::B_BYTES + S::SA_BYTES + S::SB_BYTES) * CG;
+        int s = 0, phase = 1, issued = 0;
+        for (int t = start; t < tiles && fine; t += step) {
+            const Tile4 tile = walk.at(t);
+            if (tile.zero) continue;
+            const int m = tile.m0 + rank * 128, n = tile.n0 + rank * S::B_ROWS;
+            const int sa = min(tile.scales + rank, p.a_tiles - 1);  // (a pair's second half may have no rows)
+            for (int kb = 0; kb < tile.k_blocks; ++kb) {
+                fine = __all_sync(0xffffffffu, tc::bar_wait(empty + s, phase, p.limit));
+                if (!fine) break;
+                if (issuer) {
+                    const uint32_t bar = CG == 2 ? full_leader + s * 8 : tc::smem_u32(full + s);
+                    if (rank == 0) tc::bar_expect(full + s, stage_bytes);
+                    char* a = stages + s * S::STAGE_PITCH;
+                    char* b = a + S::A_BYTES;
+                    const int k = tile.k0 + kb;
+                    tc::tma_load_2d<CG>(a, &map_a, k * 128, m, bar);
+                    tc::tma_load_3d<CG>(b, &map_b, k * 128, n, tile.g, bar);
+                    tc::tma_load_3d<CG>(b + S::B_BYTES, &map_sa, 0, k * S::COLUMN_TILES, sa, bar);
+                    tc::tma_load_4d<CG>(b + S::B_BYTES + S::SA_BYTES, &map_sb, 0, k * S::COLUMN_TILES, tile.n0 / 128, tile.g, bar);
+                }
+                __syncwarp();
+                ++issued;
+                if (++s == STAGES) {
+                    s = 0;
+                    phase ^= 1;
+                }
+            }
+        }
+        // every stage read out: no arrival is on its way when the CTA ends, and no copy
+        for (int i = 0; i < STAGES && i < issued && fine; ++i) {
+            const int last = issued - 1 - i;
+            fine = __all_sync(0xffffffffu, tc::bar_wait(empty + last % STAGES, (last / STAGES) & 1, p.limit));
+        }
+        if (lane == 0) tc::store_leader<CG>(issued_by + rank, issued);
+    } else if (warp == 1) {
+        if (rank == 0) {
+            const bool issuer = tc::elect_one();
+            const uint32_t a0 = tc::smem_u32(stages);
+            const uint64_t da = tc::sdesc_swizzled(a0, 16), db = tc::sdesc_swizzled(a0 + S::A_BYTES, 16);
+            int s = 0, phase = 0, half = 0;  // half: of the TMEM columns for scales
+            uint32_t summed = 0;
+            for (int t = start; t < tiles && fine; t += step, ++summed) {
+                const Tile4 tile = walk.at(t);
+                const int blocks = tile.zero ? 0 : tile.k_blocks, acc = summed & 1;
+                // the accumulator is free, read out two tiles ago; with OVERLAP its half that the last tile had, too
+                if (S::OVERLAP) fine = summed == 0 || __all_sync(0xffffffffu, tc::bar_wait(drained + (acc ^ 1), ((summed - 1) >> 1) & 1, p.limit));
+                else fine = __all_sync(0xffffffffu, tc::bar_wait(drained + acc, ((summed >> 1) & 1) ^ 1, p.limit));
+                if (!fine) break;
+                tc::fence_after_sync();
+                const uint32_t to = tmem + acc * 128;
+                for (int kb = 0; kb < blocks; ++kb) {
+                    fine = __all_sync(0xffffffffu, tc::bar_wait(full + s, phase, p.limit));
+                    if (!fine) break;
+                    tc::fence_after_sync();
+                    if (issuer) {
+                        const uint32_t at = s * S::STAGE_PITCH, sa = a0 + at + S::A_BYTES + S::B_BYTES, sb = sa + S::SA_BYTES;
+                        const uint32_t scale = tmem + S::SCALES_AT + half * 64;
+                        const int left = p.k - (tile.k0 + kb) * BK, steps = min(BK / 64, (left + 63) / 64);
+#pragma unroll
+                        for (int i = 0; i < S::COLUMN_TILES; ++i) {
+                            tc::copy_scales<CG>(scale + i * 4, sa + i * MICRO_TILE);
+#pragma unroll
+                            for (int j = 0; j < BN / 128; ++j)
+                                tc::copy_scales<CG>(scale + S::SB_AT + i * (BN / 32) + j * 4, sb + (j * S::COLUMN_TILES + i) * MICRO_TILE);
+                        }
+#pragma unroll
+                        for (int i = 0; i < BK / 64; ++i) {
+                            constexpr int PER = 4 / S::COLUMN_TILES;  // K-steps of a tile of scales
+                            if (i < steps)
+                                tc::mma_scaled<CG, BLOCK>(to, da + uint64_t(at >> 4) + i * 2, db + uint64_t(at >> 4) + i * 2,
+                                                          tc::idesc_scaled<BLOCK>(S::TM, BN, i % PER), scale + i / PER * 4,
+                                                          scale + S::SB_AT + i / PER * (BN / 32), kb > 0 || i > 0);
+                        }
+                        tc::commit_group<CG>(empty + s);
+                    }
+                    __syncwarp();
+                    half ^= 1;
+                    if (++s == STAGES) {
+                        s = 0;
+                        phase ^= 1;
+                    }
+                }
+                if (!fine) break;
+                if (issuer) tc::commit_group<CG>(done + acc);
+                __syncwarp();
+            }
+        }
+    } else if (warp >= EPILOGUE_WARP) {
+        constexpr int WINDOWS = S::WINDOWS, STRIDE = 32 * S::GROUPS;
+        const int quadrant = warp & 3, group = (warp - EPILOGUE_WARP) >> 2;
+        char* stage = staging + (warp - EPILOGUE_WARP) * STAGING;
+        float* bias = reinterpret_cast<float*>(staging + S::EPILOGUE_WARPS * STAGING) + (warp - EPILOGUE_WARP) * WINDOWS * 64;
+        float* column_scale = bias + WINDOWS * 32;
+        const uint32_t lanes = tmem + (uint32_t(quadrant * 32) << 16);
+        const bool wide = p.n % 8 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
+        const bool wide_residual = p.n % 8 == 0 && reinterpret_cast<uintptr_t>(p.residual) % 16 == 0;
+        int held_g = -1, held_n0 = -1;  // whose bias and scales are held
+        uint32_t summed = 0;
+        for (int t = start; t < tiles && fine; t += step, ++summed) {
+            const Tile4 tile = walk.at(t);
+            const int acc = summed & 1;
+            const int row = tile.m0 + rank * 128 + quadrant * 32, column0 = tile.n0 + group * 32;
+            const int rows = min(32, tile.m_end - row), columns = p.n - column0;  // inside the matrix, from `column0` on
+            const long long at = (long long)row * p.n + column0;
+            const uint16_t* residual = !PARTIAL && p.residual && !tile.zero ? static_cast<const uint16_t*>(p.residual) + at : nullptr;
+            // with OVERLAP the window that both accumulators share comes first
+            const bool turned = S::OVERLAP && acc == 0;
+            uint4 r[4];
+            float row_scale = 1.0f;
+            if (!PARTIAL && !tile.zero) {  // what does not need the sum is read while it is awaited
+                const int j = turned ? WINDOWS - 1 : 0;
+                if (residual && columns > j * STRIDE) {
+                    const Window w{p.n, rows, columns - j * STRIDE, wide_residual};
+                    if (w.wide) window_load(residual + j * STRIDE, w, lane, r);
+                    else window_fetch(residual + j * STRIDE, w, lane, stage);
+                }
+                if (lane < rows) row_scale = __ldg(p.row_scales + row + lane);
+                if (tile.g != held_g || tile.n0 != held_n0) {
+                    held_g = tile.g;
+                    held_n0 = tile.n0;
+                    __syncwarp();
+#pragma unroll
+                    for (int j = 0; j < WINDOWS; ++j) {
+                        const bool on = j * STRIDE + lane < columns;
+                        const long long from = (long long)tile.g * p.n + column0 + j * STRIDE + lane;
+                        bias[j * 32 + lane] = on && p.bias ? to_float(static_cast<const T*>(p.bias)[from]) : 0.0f;
+                        column_scale[j * 32 + lane] = on ? __ldg(p.column_scales + from) : 0.0f;
+                    }
+                    __syncwarp();
+                }
+            }
+            fine = __all_sync(0xffffffffu, tc::bar_wait(done + acc, (summed >> 1) & 1, p.limit));
+            if (!fine) break;
+            tc::fence_after_sync();
+#pragma unroll 1
+            for (int i = 0; i < WINDOWS; ++i) {
+                const int j = turned ? WINDOWS - 1 - i : i;
+                const Window w{p.n, rows, columns - j * STRIDE, wide};
+                float v[32];
+                if (tile.zero) {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) v[e] = 0.0f;
+                } else if (w.columns > 0) {
+                    tc::tmem_ld32(lanes + acc * 128 + group * 32 + j * STRIDE, v);
+                }
+                if (i == (S::OVERLAP ? 0 : WINDOWS - 1)) {
+                    tc::fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) tc::bar_arrive_cluster(CG == 2 ? tc::leader_address(drained + acc) : tc::smem_u32(drained + acc));
+                }
+                if (w.columns <= 0) continue;
+                if (PARTIAL) {
+                    if (lane < rows) {
+                        float* to = p.partial + ((long long)tile.split * p.rows + row + lane) * p.n + column0 + j * STRIDE;
+                        if (p.n % 4 == 0) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 4)
+                                if (e < w.columns) *reinterpret_cast<float4*>(to + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                if (e < w.columns) to[e] = v[e];
+                        }
+                    }
+                    continue;
+                }
+                if (!tile.zero) {
+                    if (residual) {
+                        if (wide_residual) {
+                            if (i > 0) window_load(residual + j * STRIDE, Window{p.n, rows, w.columns, true}, lane, r);
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) *staged(stage, lane / 4 + 8 * u, lane & 3) = r[u];
+                        } else if (i > 0) {
+                            window_fetch(residual + j * STRIDE, Window{p.n, rows, w.columns, false}, lane, stage);
+                        }
+                        __syncwarp();
+                    }
+                    const Pair scale = same(row_scale);
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        const float2 c = *reinterpret_cast<const float2*>(column_scale + j * 32 + e);
+                        const float2 z = both(mul2(mul2(pair(v[e], v[e + 1]), scale), pair(c.x, c.y)));
+                        v[e] = z.x;
+                        v[e + 1] = z.y;
+                    }
+                    uint32_t codes[16];
+                    if (p.activation == ACT_RELU) finish_relu(v, bias + j * 32);
+                    else if (p.activation == ACT_SILU) finish<ACT_SILU>(v, codes, bias + j * 32);
+                    else if (p.activation == ACT_GELU) finish<ACT_GELU>(v, codes, bias + j * 32);
+                    else finish<ACT_NONE>(v, codes, bias + j * 32);
+                    if (residual) {
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            const uint4 q = *staged(stage, lane, u);
+                            const uint32_t e[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                            for (int h = 0; h < 4; ++h) {
+                                const float2 f = unpack_pair<T>(e[h]);
+                                v[u * 8 + h * 2] += f.x;
+                                v[u * 8 + h * 2 + 1] += f.y;
+                            }
+                        }
+                        __syncwarp();
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    *staged(stage, lane, u) = make_uint4(pack_pair<T>(v[u * 8], v[u * 8 + 1]), pack_pair<T>(v[u * 8 + 2], v[u * 8 + 3]),
+                                                         pack_pair<T>(v[u * 8 + 4], v[u * 8 + 5]), pack_pair<T>(v[u * 8 + 6], v[u * 8 + 7]));
+                __syncwarp();
+                window_store(static_cast<uint16_t*>(p.out) + at + j * STRIDE, w, lane, stage);
+                __syncwarp();
+            }
+        }
+    }
+    if (!fine && lane == 0) {
+        *static_cast<volatile int*>(p.error) = 2;
+        __threadfence_system();
+        tc::store_both<CG>(gave_up, 1);
+    }
+    __syncwarp();
+    tc::fence_before_sync();
+    __syncthreads();
+    if (CG == 2) tc::cluster_sync();
+    tc::fence_after_sync();
+    // Nothing is issued any more.  Had a wait run out, copies and products may still be on their way: they are awaited
+    // before the shared memory and the TMEM go.
+    if (tc::load_shared(gave_up)) {
+        if (warp == 0 && rank == 0) {
+            const int mine = int(tc::load_shared(issued_by)), other = CG == 2 ? int(tc::load_shared(issued_by + 1)) : mine;
+            const uint32_t share = uint32_t(p.a_rows * 128 + S::B_BYTES + S::SA_BYTES + S::SB_BYTES);  // of one CTA in a block
+            for (int b = max(0, max(mine, other) - STAGES); b < max(mine, other); ++b) {
+                uint64_t* bar = full + b % STAGES;
+                if (lane == 0 && b >= mine) tc::bar_expect(bar, share);
+                if (lane == 0 && b >= other) tc::bar_unexpect(bar, share);
+                __syncwarp();
+                tc::bar_wait(bar, (b / STAGES) & 1, WAIT_LIMIT);
+            }
+        }
+        if (warp == 1) {
+            if (rank == 0 && tc::elect_one()) tc::commit_group<CG>(drain);
+            __syncwarp();
+            tc::bar_wait(drain, 0, WAIT_LIMIT);
+        }
+        tc::fence_before_sync();
+        __syncthreads();
+        if (CG == 2) tc::cluster_sync();
+        tc::fence_after_sync();
+    }
+    if (warp == 2) tc::tmem_dealloc_group<CG>(tmem, S::COLUMNS);
+}
+
+// The sums over parts of K, in order, with the epilogue of the products.
+struct Finish4Args {
+    const float* partial;  // [splits][rows][n]
+    int splits;
+    long long rows;
+    int n;
+    const float* row_scales;
+    const float* column_scales;
+    const void* bias;
+    const void* residual;
+    void* out;
+    int activation;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) finish4_kernel(Finish4Args a) {
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= a.rows * a.n) return;
+    const long long row = i / a.n;
+    const int column = int(i - row * a.n);
+    float z = 0.0f;
+#pragma unroll 8
+    for (int s = 0; s < a.splits; ++s) z += __ldg(a.partial + s * a.rows * a.n + i);
+    z = z * a.row_scales[row] * a.column_scales[column];
+    if (a.bias) z += to_float(static_cast<const T*>(a.bias)[column]);
+    const Pair added = same(a.residual ? to_float(static_cast<const T*>(a.residual)[i]) : 0.0f);
+    Pair slope, y;
+    if (a.activation == ACT_RELU) y = activate<ACT_RELU, true>(same(z), slope, added);
+    else if (a.activation == ACT_SILU) y = activate<ACT_SILU, true>(same(z), slope, added);
+    else if (a.activation == ACT_GELU) y = activate<ACT_GELU, true>(same(z), slope, added);
+    else y = activate<ACT_NONE, true>(same(z), slope, added);
+    static_cast<T*>(a.out)[i] = from_float<T>(both(y).x);
+}
+
+// ---------------------------------------------------------------- host
+constexpr int SMS = 148;  // of a B200: the sizes of scratch must not depend on the device that asks
+
+int64_t aligned(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// 256 x 256 tiles by pairs, or 128 x 128 by one CTA where those leave SMs idle.
+bool pair_tiles(int64_t rows, int n, int groups) {
+    if (n <= 128) return false;
+    const int64_t pairs = (groups > 1 ? rows / 256 + (groups + 1) / 2 : ceil_div(rows, 256)) * ceil_div(n, 256);
+    const int64_t ones = (groups > 1 ? rows / 128 + (groups + 1) / 2 : ceil_div(rows, 128)) * ceil_div(n, 128);
+    return double(ceil_div(std::max<int64_t>(1, pairs), SMS / 2)) * 256 <= double(ceil_div(std::max<int64_t>(1, ones), SMS)) * 128 * 1.35;
+}
+
+// Without offsets, where 128 x 128 tiles leave SMs idle: the sum over K is cut into as many parts as there are SMs for.
+struct Splits4 {
+    int parts, blocks;  // blocks of K per part
+    Splits4(int64_t rows, int n, int k, int groups, bool offsets) : parts(1), blocks(int(ceil_div(k, BK))) {
+        if (rows == 0 || offsets || pair_tiles(rows, n, groups)) return;
+        const int64_t tiles = ceil_div(rows, 128) * ceil_div(n, 128), wanted = std::min<int64_t>(SMS / tiles, blocks / 2);
+        if (wanted < 2) return;
+        blocks = int(ceil_div(blocks, wanted));
+        parts = int(ceil_div(ceil_div(k, BK), blocks));
+    }
+    int64_t bytes(int64_t rows, int n) const { return parts > 1 ? parts * rows * n * 4 : 0; }
+};
+
+struct Scratch4 {
+    uint8_t *codes, *scales;
+    float *row_scales, *partial;
+    int64_t tiles, bytes = 0;
+    Scratch4(void* base, int64_t rows, int inputs, int outputs, int groups, bool offsets, int block) {
+        char* at = static_cast<char*>(base);
+        auto take = [&](int64_t size) {
+            char* p = at ? at + bytes : nullptr;
+            bytes += aligned(size);
+            return p;
+        };
+        tiles = offsets ? micro_tiles(rows, groups) : ceil_div(rows, MICRO_ROWS);
+        codes = reinterpret_cast<uint8_t*>(take(rows * micro_pitch(inputs)));
+        scales = reinterpret_cast<uint8_t*>(take(tiles * micro_columns(inputs, block) * MICRO_TILE));
+        row_scales = reinterpret_cast<float*>(take(rows * 4));
+        partial = reinterpret_cast<float*>(take(Splits4(rows, outputs, inputs, groups, offsets).bytes(rows, outputs)));
+    }
+};
+
+// A row-major array of bytes (4-byte units: words), the fastest dimension first, strides in bytes.
+CUtensorMap byte_map(const void* base, bool words, bool swizzled, int rank, const int64_t* dims, const int64_t* strides, const int* box) {
+    CUtensorMap map;
+    cuuint64_t d[4], s[3];
+    cuuint32_t b[4], unit[4] = {1, 1, 1, 1};
+    for (int i = 0; i < rank; ++i) {
+        d[i] = cuuint64_t(dims[i]);
+        b[i] = cuuint32_t(box[i]);
+        if (i > 0) s[i - 1] = cuuint64_t(strides[i - 1]);
+    }
+    ODIE_REQUIRE(uintptr_t(base) % 16 == 0, "codes, scales and scratch must start on 16-byte boundaries");
+    const CUresult status = tensor_map_encoder()(&map, words ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT8, cuuint32_t(rank),
+                                                 const_cast<void*>(base), d, s, b, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                                 swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    ODIE_REQUIRE(status == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with " + std::to_string(int(status)));
+    return map;
+}
+
+struct Product4 {
+    const uint8_t *a, *sa, *b, *sb;
+};
+
+template <typename T, int CG, int BN, int BLOCK, bool PARTIAL>
+void launch_gemm4(const Product4& x, Gemm4Args p, int64_t tiles, cudaStream_t stream) {
+    using S = Shape4<CG, BN, BLOCK>;
+    ODIE_REQUIRE(tiles < (int64_t(1) << 30), "too many rows and columns for one launch");
+    const int64_t nt = ceil_div(p.n, BN), pitch = micro_pitch(p.k), columns = micro_columns(p.k, BLOCK), row_tiles = ceil_div(p.n, MICRO_ROWS);
+    p.by_bands = Divide::by(BAND * nt);
+    p.by_tiles = Divide::by(nt * ceil_div(p.rows, 128 * CG));
+    const int64_t da[] = {pitch, p.rows}, ta[] = {pitch};
+    const int xa[] = {128, p.a_rows};
+    const CUtensorMap map_a = byte_map(x.a, false, true, 2, da, ta, xa);
+    const int64_t db[] = {pitch, p.n, p.groups}, tb[] = {pitch, pitch * p.n};
+    const int xb[] = {128, S::B_ROWS, 1};
+    const CUtensorMap map_b = byte_map(x.b, false, true, 3, db, tb, xb);
+    const int64_t dsa[] = {128, columns, p.a_tiles}, tsa[] = {MICRO_TILE, MICRO_TILE * columns};
+    const int xsa[] = {128, S::COLUMN_TILES, 1};
+    const CUtensorMap map_sa = byte_map(x.sa, true, false, 3, dsa, tsa, xsa);
+    const int64_t dsb[] = {128, columns, row_tiles, p.groups}, tsb[] = {MICRO_TILE, MICRO_TILE * columns, MICRO_TILE * columns * row_tiles};
+    const int xsb[] = {128, S::COLUMN_TILES, BN / 128, 1};
+    const CUtensorMap map_sb = byte_map(x.sb, true, false, 4, dsb, tsb, xsb);
+
+    const auto kernel = gemm4_kernel<T, CG, BN, BLOCK, PARTIAL>;
+    ODIE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes(1024)));
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(unsigned(std::min<int64_t>(tiles, sm_count() / CG) * CG));
+    config.blockDim = dim3(S::THREADS);
+    config.dynamicSmemBytes = size_t(S::bytes(p.groups));
+    config.stream = stream;
+    cudaLaunchAttribute cluster{};
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = CG;
+    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+    config.attrs = &cluster;
+    config.numAttrs = 1;
+    ODIE_CUDA(cudaLaunchKernelEx(&config, kernel, map_a, map_b, map_sa, map_sb, p));
+    note_launch();
+}
+
+template <typename T, int BLOCK>
+void launch_product4(const Product4& x, Gemm4Args p, const Splits4& split, float* partial, cudaStream_t stream) {
+    const bool pairs = pair_tiles(p.rows, p.n, p.groups);
+    p.a_rows = int(std::min<int64_t>(128, (p.rows + 7) / 8 * 8));
+    p.splits = 1;
+    const int64_t tiles = (ceil_div(p.rows, pairs ? 256 : 128) + p.groups + 1) * ceil_div(p.n, pairs ? 256 : 128);
+    if (pairs) {
+        launch_gemm4<T, 2, 256, BLOCK, false>(x, p, tiles, stream);
+    } else if (split.parts == 1) {
+        launch_gemm4<T, 1, 128, BLOCK, false>(x, p, tiles, stream);
+    } else {
+        p.splits = split.parts;
+        p.chunk = split.blocks;
+        p.partial = partial;
+        launch_gemm4<T, 1, 128, BLOCK, true>(x, p, tiles * split.parts, stream);
+        const Finish4Args f{partial, split.parts, p.rows, p.n, p.row_scales, p.column_scales, p.bias, p.residual, p.out, p.activation};
+        finish4_kernel<T><<<unsigned(ceil_div(p.rows * p.n, 256)), 256, 0, stream>>>(f);
+        ODIE_CUDA(cudaGetLastError());
+        note_launch();
+    }
+}
+
+bool sizes4_fit(int64_t rows, int64_t inputs, int64_t outputs, int64_t groups, int block) {
+    return rows >= 0 && rows < (int64_t(1) << 31) - 256 && inputs >= 1 && outputs >= 1 && inputs <= (1 << 20) && outputs <= (1 << 20) &&
+           groups >= 1 && groups <= 1024 && (block == 16 || block == 32);
+}
+
+}  // namespace
+}  // namespace odie
+
+using namespace odie;
+
+extern "C" int64_t odie_linear4_scratch(int64_t rows, int inputs, int outputs, int groups, int offsets, int block) {
+    if (!sizes4_fit(rows, inputs, outputs, groups, block)) return 0;
+    return Scratch4(nullptr, rows, inputs, outputs, groups, offsets, block).bytes;
+}
+
+extern "C" int odie_linear4(const void* x, const uint8_t* codes, const uint8_t* scales, const float* row_scales, int block, const void* bias,
+                            const void* residual, int64_t rows, int inputs, int outputs, int groups, const int32_t* offsets, int dtype,
+                            int activation, void* y, void* scratch, uint64_t stream_handle) {
+    return guarded([&] {
+        ODIE_REQUIRE(dtype == ROW_F16 || dtype == ROW_BF16, "linear4 takes fp16 (0) or bf16 (1)");
+        ODIE_REQUIRE(sizes4_fit(rows, inputs, outputs, groups, block),
+                     "0 to 2^31 - 257 rows, 1 to 2^20 inputs and outputs, 1 to 1024 groups, and blocks of 16 or 32");
+        ODIE_REQUIRE(offsets || groups == 1, "more than one group needs offsets");
+        ODIE_REQUIRE(activation >= ACT_NONE && activation <= ACT_GELU, "activation must be 0 (none), 1 (ReLU), 2 (SiLU) or 3 (GELU)");
+        if (rows == 0) return;
+        ODIE_REQUIRE(x && codes && scales && row_scales && y, "x, codes, scales, row_scales and y are required");
+        ODIE_REQUIRE((uintptr_t(codes) | uintptr_t(scales)) % 16 == 0, "codes and scales must start on 16-byte boundaries");
+        ODIE_REQUIRE(scratch && uintptr_t(scratch) % 256 == 0, "scratch is required, on a 256-byte boundary");
+        int* const error = checked_error_word();
+        const cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_handle);
+        const Scratch4 s(scratch, rows, inputs, outputs, groups, offsets, block);
+        MicroArgs q{};
+        q.x = x;
+        q.rows = q.group_rows = rows;
+        q.width = inputs;
+        q.groups = groups;
+        q.offsets = offsets;
+        q.codes = s.codes;
+        q.scales = s.scales;
+        q.row_scales = s.row_scales;
+        q.pitch = micro_pitch(inputs);
+        q.columns = micro_columns(inputs, block);
+        launch_quantize(q, dtype, block, stream);
+        Gemm4Args p{};
+        p.groups = groups;
+        p.offsets = offsets;
+        p.rows = rows;
+        p.n = outputs;
+        p.k = inputs;
+        p.a_tiles = int(s.tiles);
+        p.row_scales = s.row_scales;
+        p.column_scales = row_scales;
+        p.bias = bias;
+        p.residual = residual;
+        p.out = y;
+        p.activation = activation;
+        p.error = error;
+        p.limit = product_wait_limit();
+        const Product4 operands{s.codes, s.scales, codes, scales};
+        const Splits4 split(rows, outputs, inputs, groups, offsets);
+        auto go = [&](auto type) {
+            if (block == 16) launch_product4<decltype(type), 16>(operands, p, split, s.partial, stream);
+            else launch_product4<decltype(type), 32>(operands, p, split, s.partial, stream);
+        };
+        if (dtype == ROW_BF16) go(__nv_bfloat16{});
+        else go(__half{});
+    });
+}

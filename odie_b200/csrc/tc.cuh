@@ -73,6 +73,48 @@ __device__ __forceinline__ void mma_group(uint32_t d_tmem, uint64_t a, uint64_t 
             "l"(a), "l"(b), "r"(id), "r"(accumulate));
 }
 
+// Products of microscaled 4-bit rows (kind::mxf4nvf4): A and B hold e2m1 values, two to a byte, K-major, one scale for
+// each BLOCK of them: 16 (unsigned e4m3 scales, four to a K-step of 64) or 32 (powers of two, e8m0, two to a K-step).
+// The scales lie in TMEM, one byte each, the four of a row in a 32-bit column, rows 32 q + l of 128 in lane l (of every
+// quarter of the lanes) and column q; with BLOCK 32 a column serves two K-steps, `second` the later one.
+template <int BLOCK>
+__host__ __device__ constexpr uint32_t idesc_scaled(int M, int N, int second) {
+    return (uint32_t(second * 2) << 4) | (1u << 7) | (1u << 10) | (uint32_t(N >> 3) << 17) | (uint32_t(BLOCK == 32) << 23) |
+           (uint32_t(M >> 4) << 24) | (uint32_t(second * 2) << 29);
+}
+template <int CG, int BLOCK>
+__device__ __forceinline__ void mma_scaled(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t id, uint32_t scale_a, uint32_t scale_b,
+                                           uint32_t accumulate) {
+    if constexpr (CG == 2 && BLOCK == 16)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d_tmem),
+            "l"(a), "l"(b), "r"(id), "r"(scale_a), "r"(scale_b), "r"(accumulate));
+    else if constexpr (CG == 2)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::2.kind::mxf4nvf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d_tmem),
+            "l"(a), "l"(b), "r"(id), "r"(scale_a), "r"(scale_b), "r"(accumulate));
+    else if constexpr (BLOCK == 16)
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::4X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d_tmem),
+            "l"(a), "l"(b), "r"(id), "r"(scale_a), "r"(scale_b), "r"(accumulate));
+    else
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"
+            "tcgen05.mma.cta_group::1.kind::mxf4nvf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::"r"(d_tmem),
+            "l"(a), "l"(b), "r"(id), "r"(scale_a), "r"(scale_b), "r"(accumulate));
+}
+// 512 bytes of shared memory (of each CTA of the group its own), the scales of 128 rows, into four TMEM columns.  Runs
+// before the products that the same thread issues after it.
+template <int CG>
+__device__ __forceinline__ void copy_scales(uint32_t tmem, uint32_t address) {
+    const uint64_t from = sdesc(address, 128u, 128u);
+    if constexpr (CG == 2) asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n" ::"r"(tmem), "l"(from) : "memory");
+    else asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n" ::"r"(tmem), "l"(from) : "memory");
+}
+
 // D[tmem] (+)= A * B, issued by one thread.
 __device__ __forceinline__ void mma(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t id, uint32_t accumulate) {
     const uint32_t mask = 0;
@@ -243,6 +285,22 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const void* map, int x, i
             "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n" ::"r"(
                 smem_u32(dst)),
             "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+            : "memory");
+}
+
+template <int CG>
+__device__ __forceinline__ void tma_load_4d(void* dst, const void* map, int x, int y, int z, int w, uint32_t bar) {
+    if constexpr (CG == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(
+                smem_u32(dst)),
+            "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];\n" ::"r"(
+                smem_u32(dst)),
+            "l"(map), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar)
             : "memory");
 }
 

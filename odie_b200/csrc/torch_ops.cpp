@@ -12,6 +12,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include "odie_b200.h"
+#include <cmath>
 
 namespace {
 
@@ -379,6 +380,274 @@ Tensor embed(const Tensor& ids, const Tensor& table, double scale) {
     return out.view(shape);
 }
 
+// ---------------------------------------------------------------- the router
+struct OpenExperts {  // the mask, expanded to the logits' shape, as the kernels read it
+    Tensor mask;
+    const uint8_t* at = nullptr;
+    int64_t row_step = 0, expert_step = 0;
+    explicit OpenExperts(const Tensor& expanded) : mask(expanded) {
+        if (!mask.defined()) return;
+        at = static_cast<const uint8_t*>(mask.data_ptr());
+        row_step = mask.stride(0);
+        expert_step = mask.stride(1);
+    }
+};
+
+void check_logits(const Tensor& logits) {
+    check_rows(logits, "logits");
+    TORCH_CHECK_VALUE(logits.size(1) <= 1024, "at most 1024 experts");
+    TORCH_CHECK_VALUE(logits.size(0) < (int64_t(1) << 31), "too many rows");
+}
+Tensor check_mask(const Maybe& mask, const Tensor& logits) {
+    if (!mask) return Tensor();
+    TORCH_CHECK_VALUE(mask->is_cuda() && mask->scalar_type() == at::kBool, "mask must be a CUDA bool tensor");
+    check_device(*mask, logits, "mask");
+    const bool fits = mask->dim() <= 2 && (mask->dim() < 1 || mask->size(-1) == logits.size(1) || mask->size(-1) == 1) &&
+                      (mask->dim() < 2 || mask->size(0) == logits.size(0) || mask->size(0) == 1);
+    TORCH_CHECK_VALUE(fits, "mask ", mask->sizes(), " does not go with the logits ", logits.sizes());
+    return mask->expand(logits.sizes());
+}
+
+// (expert, weights)
+std::pair<Tensor, Tensor> gated(const Tensor& logits, const Tensor& bias, const Tensor& mask, int64_t choices, int64_t score, bool normalize,
+                                double scale) {
+    const c10::cuda::CUDAGuard guard(logits.device());
+    const OpenExperts open(mask);
+    const auto options = logits.options().requires_grad(false);
+    Tensor expert = at::empty({logits.size(0), choices}, options.dtype(at::kInt)), weights = at::empty({logits.size(0), choices}, options.dtype(at::kFloat));
+    done(odie_gate(data(logits), logits.size(0), int(logits.size(1)), row_type(logits), static_cast<const float*>(data(bias)), open.at, open.row_step,
+                   open.expert_step, int(choices), int(score), normalize, float(scale), static_cast<int32_t*>(data(expert)),
+                   static_cast<float*>(data(weights)), stream_of(logits)),
+         "odie_gate");
+    return {expert, weights};
+}
+
+struct Gate : torch::autograd::Function<Gate> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Maybe& bias, const Maybe& maybe_mask, int64_t choices,
+                                 int64_t score, bool normalize, double scale) {
+        const Tensor mask = present(maybe_mask);
+        const auto [expert, weights] = gated(logits, present(bias), mask, choices, score, normalize, scale);
+        ctx->mark_non_differentiable({expert});
+        // a normalised softmax's gradient needs the weights alone, a sigmoid's the chosen logits
+        const bool dense = score == 0 && !normalize, softmax = score == 0 && normalize;
+        ctx->save_for_backward({softmax ? Tensor() : logits, dense ? mask : Tensor(), expert, weights});
+        ctx->saved_data["experts"] = logits.size(1);
+        ctx->saved_data["type"] = logits.scalar_type();
+        ctx->saved_data["score"] = score;
+        ctx->saved_data["normalize"] = normalize;
+        ctx->saved_data["scale"] = scale;
+        return {expert, weights};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list gradients) {
+        refuse_tangents(gradients[1]);
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &logits = saved[0], &expert = saved[2], &weights = saved[3];
+        const int64_t experts = ctx->saved_data["experts"].toInt();
+        const OpenExperts open(saved[1]);
+        const Tensor d_weights = gradients[1].contiguous();
+        const c10::cuda::CUDAGuard guard(d_weights.device());
+        Tensor d_logits = at::empty({expert.size(0), experts}, weights.options().dtype(ctx->saved_data["type"].toScalarType()).requires_grad(false));
+        done(odie_gate_backward(static_cast<const float*>(data(d_weights)), data(logits), expert.size(0), int(experts), row_type(d_logits), open.at,
+                                open.row_step, open.expert_step, static_cast<const int32_t*>(data(expert)), static_cast<const float*>(data(weights)),
+                                int(expert.size(1)), int(ctx->saved_data["score"].toInt()), ctx->saved_data["normalize"].toBool(),
+                                float(ctx->saved_data["scale"].toDouble()), data(d_logits), stream_of(d_logits)),
+             "odie_gate_backward");
+        return once({d_logits, Tensor(), Tensor(), Tensor(), Tensor(), Tensor(), Tensor()}, {gradients[1]}, 1);
+    }
+};
+
+std::tuple<Tensor, Tensor> gate(const Tensor& logits, int64_t choices, const Maybe& bias, const Maybe& mask, int64_t score, bool normalize, double scale) {
+    check_logits(logits);
+    TORCH_CHECK_VALUE(choices >= 1 && choices <= 64 && choices <= logits.size(1), "choices must be 1 to 64 and no more than the experts");
+    TORCH_CHECK_VALUE(logits.size(0) * choices < (int64_t(1) << 31), "too many (row, choice) pairs");
+    TORCH_CHECK_VALUE(std::isfinite(float(scale)) && float(scale) != 0.0f, "scale must be finite and not 0");
+    refuse_tangents(logits);
+    Tensor shift;
+    if (bias) {
+        TORCH_CHECK_VALUE(bias->is_cuda() && bias->is_floating_point() && bias->dim() == 1 && bias->size(0) == logits.size(1),
+                          "bias must be a CUDA floating-point tensor [", logits.size(1), "]");
+        check_device(*bias, logits, "bias");
+        TORCH_CHECK_VALUE(!bias->requires_grad(), "bias has no gradient: pass bias.detach()");
+        shift = bias->to(at::kFloat).contiguous();
+    }
+    const Tensor in = logits.contiguous(), open = check_mask(mask, logits);
+    if (at::GradMode::is_enabled() && wants(in)) {
+        const variable_list out = Gate::apply(in, maybe(shift), maybe(open), choices, score, normalize, scale);
+        return {out[0], out[1]};
+    }
+    const auto [expert, weights] = gated(in, shift, open, choices, score, normalize, scale);
+    return {expert, weights};
+}
+
+// (loss, z, counts, stats)
+std::tuple<Tensor, Tensor, Tensor, Tensor> balanced(const Tensor& logits, const Tensor& expert, const Tensor& mask, int64_t score, const Tensor& total) {
+    const c10::cuda::CUDAGuard guard(logits.device());
+    const OpenExperts open(mask);
+    const int64_t experts = logits.size(1);
+    const auto options = logits.options().dtype(at::kFloat).requires_grad(false);
+    Tensor loss = at::empty({}, options), z = at::empty({}, options), counts = at::empty({experts}, options.dtype(at::kInt)), stats = at::empty({experts + 1}, options);
+    const Tensor work = scratch(logits, odie_balance_scratch(logits.size(0), int(experts)));
+    done(odie_balance(data(logits), logits.size(0), int(experts), row_type(logits), open.at, open.row_step, open.expert_step, int(score), data(expert),
+                      int(expert.element_size()), expert.numel(), static_cast<const int64_t*>(data(total)), static_cast<float*>(data(loss)),
+                      static_cast<float*>(data(z)), static_cast<int32_t*>(data(counts)), static_cast<float*>(data(stats)), data(work), stream_of(logits)),
+         "odie_balance");
+    return {loss, z, counts, stats};
+}
+
+struct Balance : torch::autograd::Function<Balance> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& logits, const Tensor& expert, const Maybe& maybe_mask, int64_t score,
+                                 const Maybe& total) {
+        ctx->set_materialize_grads(false);
+        const Tensor mask = present(maybe_mask);
+        const auto [loss, z, counts, stats] = balanced(logits, expert, mask, score, present(total));
+        ctx->mark_non_differentiable({counts});
+        ctx->save_for_backward({logits, mask, stats});
+        ctx->saved_data["score"] = score;
+        return {loss, z, counts};
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list gradients) {
+        const Tensor &d_loss = gradients[0], &d_z = gradients[1];
+        refuse_tangents(d_loss, d_z);
+        const auto saved = ctx->get_saved_variables();
+        const Tensor &logits = saved[0], &stats = saved[2];
+        if (!d_loss.defined() && !d_z.defined()) return {Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
+        const OpenExperts open(saved[1]);
+        const c10::cuda::CUDAGuard guard(logits.device());
+        Tensor d_logits = rows_like(logits, logits.sizes());
+        done(odie_balance_backward(static_cast<const float*>(data(d_loss)), static_cast<const float*>(data(d_z)), data(logits), logits.size(0),
+                                   int(logits.size(1)), row_type(logits), open.at, open.row_step, open.expert_step, int(ctx->saved_data["score"].toInt()),
+                                   static_cast<const float*>(data(stats)), data(d_logits), stream_of(logits)),
+             "odie_balance_backward");
+        return once({d_logits, Tensor(), Tensor(), Tensor(), Tensor()}, {d_loss, d_z, logits});
+    }
+};
+
+std::tuple<Tensor, Tensor, Tensor> balance(const Tensor& logits, const Tensor& expert, const Maybe& mask, int64_t score, const Maybe& total) {
+    check_logits(logits);
+    check_ids(expert, "expert");
+    TORCH_CHECK_VALUE((expert.dim() == 1 || expert.dim() == 2) && expert.size(0) == logits.size(0), "expert must have the shape [", logits.size(0),
+                      "] or [", logits.size(0), ", choices]");
+    TORCH_CHECK_VALUE(expert.numel() < (int64_t(1) << 31), "too many (row, choice) pairs");
+    check_device(expert, logits, "expert");
+    refuse_tangents(logits);
+    Tensor counted;
+    if (total) {
+        check_ids(*total, "total");
+        TORCH_CHECK_VALUE(total->dim() == 1 && total->size(0) == logits.size(1), "total must have the shape [", logits.size(1), "]");
+        check_device(*total, logits, "total");
+        counted = total->to(at::kLong).contiguous();
+    }
+    const Tensor in = logits.contiguous(), keys = expert.contiguous(), open = check_mask(mask, logits);
+    if (at::GradMode::is_enabled() && wants(in)) {
+        const variable_list out = Balance::apply(in, keys, maybe(open), score, maybe(counted));
+        return {out[0], out[1], out[2]};
+    }
+    const auto [loss, z, counts, stats] = balanced(in, keys, open, score, counted);
+    return {loss, z, counts};
+}
+
+// ---------------------------------------------------------------- microscaled 4-bit rows
+struct MicroSizes {
+    int64_t groups, rows, width, block;
+    int64_t pitch() const { return (width + 31) / 32 * 16; }
+    std::vector<int64_t> scales() const { return {groups, (rows + 127) / 128, (width + 4 * block - 1) / (4 * block), 512}; }
+};
+
+void check_block(int64_t block) { TORCH_CHECK_VALUE(block == 16 || block == 32, "block must be 16 or 32"); }
+
+std::tuple<Tensor, Tensor, Tensor> quantize(const Tensor& x, int64_t block) {
+    check_block(block);
+    TORCH_CHECK_VALUE(x.is_cuda() && row_type(x) >= 0 && (x.dim() == 2 || x.dim() == 3) && x.size(-1) > 0 && (x.dim() == 2 || x.size(0) > 0),
+                      "x must be a CUDA fp16, bf16 or fp32 tensor [rows, width] or [groups, rows, width] with at least one column and group");
+    TORCH_CHECK_VALUE(x.size(-1) <= (1 << 20), "at most 2^20 columns");
+    refuse_tangents(x);
+    const MicroSizes s{x.dim() == 3 ? x.size(0) : 1, x.size(-2), x.size(-1), block};
+    const c10::cuda::CUDAGuard guard(x.device());
+    const Tensor in = x.contiguous();
+    const auto options = x.options().dtype(at::kByte).requires_grad(false);
+    std::vector<int64_t> shape = x.sizes().vec();
+    Tensor row_scales = at::empty(at::IntArrayRef(shape.data(), shape.size() - 1), options.dtype(at::kFloat));
+    shape.back() = s.pitch();
+    Tensor codes = at::empty(shape, options), scales = at::empty(s.scales(), options);
+    done(odie_quantize(data(in), s.groups, s.rows, s.width, row_type(in), int(block), static_cast<uint8_t*>(data(codes)),
+                       static_cast<uint8_t*>(data(scales)), static_cast<float*>(data(row_scales)), stream_of(in)),
+         "odie_quantize");
+    return {codes, scales, row_scales};
+}
+
+MicroSizes check_micro(const Tensor& codes, const Tensor& scales, const Tensor& row_scales, int64_t width, int64_t block) {
+    check_block(block);
+    TORCH_CHECK_VALUE(width >= 1 && width <= (1 << 20), "at most 2^20 columns");
+    const bool typed = codes.is_cuda() && codes.scalar_type() == at::kByte && scales.scalar_type() == at::kByte && row_scales.scalar_type() == at::kFloat &&
+                       scales.device() == codes.device() && row_scales.device() == codes.device() && (codes.dim() == 2 || codes.dim() == 3);
+    TORCH_CHECK_VALUE(typed, "the microscaled rows must hold CUDA tensors of quantize");
+    const MicroSizes s{codes.dim() == 3 ? codes.size(0) : 1, codes.size(-2), width, block};
+    TORCH_CHECK_VALUE(s.groups >= 1 && codes.size(-1) == s.pitch() && scales.sizes() == at::IntArrayRef(s.scales()) &&
+                          row_scales.sizes() == codes.sizes().slice(0, codes.dim() - 1),
+                      "the microscaled rows' sizes do not belong together");
+    TORCH_CHECK_VALUE(codes.is_contiguous() && scales.is_contiguous() && row_scales.is_contiguous() && on_16_bytes(codes) && on_16_bytes(scales),
+                      "the microscaled rows must be contiguous, codes and scales on 16-byte boundaries");
+    return s;
+}
+
+Tensor dequantize(const Tensor& codes, const Tensor& scales, const Tensor& row_scales, int64_t width, int64_t block, at::ScalarType dtype) {
+    const MicroSizes s = check_micro(codes, scales, row_scales, width, block);
+    const c10::cuda::CUDAGuard guard(codes.device());
+    std::vector<int64_t> shape = codes.sizes().vec();
+    shape.back() = width;
+    Tensor out = at::empty(shape, codes.options().dtype(dtype));
+    TORCH_CHECK_VALUE(row_type(out) >= 0, "dtype must be torch.float16, bfloat16 or float32");
+    done(odie_dequantize(static_cast<const uint8_t*>(data(codes)), static_cast<const uint8_t*>(data(scales)), static_cast<const float*>(data(row_scales)),
+                         s.groups, s.rows, width, int(block), row_type(out), data(out), stream_of(codes)),
+         "odie_dequantize");
+    return out;
+}
+
+Tensor linear4(const Tensor& x, const Tensor& codes, const Tensor& scales, const Tensor& row_scales, int64_t width, int64_t block, const Maybe& bias,
+               const Maybe& residual, int64_t activation, const Maybe& offsets) {
+    TORCH_CHECK_VALUE(x.is_cuda() && (x.scalar_type() == at::kHalf || x.scalar_type() == at::kBFloat16) && x.dim() >= 1 && x.size(-1) > 0,
+                      "x must be a CUDA fp16 or bf16 tensor with at least one column");
+    const MicroSizes s = check_micro(codes, scales, row_scales, width, block);
+    check_device(codes, x, "weight");
+    TORCH_CHECK_VALUE(codes.dim() == (offsets ? 3 : 2) && width == x.size(-1) && s.rows >= 1, "weight must be [", offsets ? "experts, " : "",
+                      "outputs, ", x.size(-1), "]");
+    TORCH_CHECK_VALUE(s.rows <= (1 << 20), "at most 2^20 outputs");
+    std::vector<int64_t> bias_shape = codes.sizes().vec();
+    bias_shape.pop_back();
+    TORCH_CHECK_VALUE(!bias || bias->sizes() == at::IntArrayRef(bias_shape), "bias must be ", at::IntArrayRef(bias_shape));
+    auto check = [&](const Tensor& t, const char* name) {
+        TORCH_CHECK_VALUE(t.scalar_type() == x.scalar_type(), name, " must have the type of x, ", x.scalar_type());
+        check_device(t, x, name);
+    };
+    if (bias) check(*bias, "bias");
+    if (residual) check(*residual, "residual");
+    if (offsets) {
+        TORCH_CHECK_VALUE(x.dim() == 2, "x must be [rows, inputs] with offsets");
+        TORCH_CHECK_VALUE(s.groups <= 1024, "at most 1024 experts");
+        TORCH_CHECK_VALUE(offsets->is_cuda() && offsets->scalar_type() == at::kInt && offsets->dim() == 1 && offsets->size(0) == s.groups + 1,
+                          "offsets must be CUDA int32 [", s.groups + 1, "]");
+        check_device(*offsets, x, "offsets");
+    }
+    refuse_tangents(x, bias, residual);
+    TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && (wants(x) || (bias && wants(*bias)) || (residual && wants(*residual)))),
+                      "linear4 has no gradient: call it under torch.no_grad, or with detached tensors");
+    std::vector<int64_t> shape = x.sizes().vec();
+    shape.back() = s.rows;
+    int64_t rows = 1;
+    for (int64_t i = 0; i + 1 < x.dim(); ++i) rows *= x.size(i);
+    const Tensor in = x.reshape({rows, x.size(-1)}).contiguous(), b = bias ? bias->contiguous() : Tensor(), o = offsets ? offsets->contiguous() : Tensor();
+    Tensor r;
+    if (residual) r = residual->expand(shape).reshape({rows, s.rows}).contiguous();
+    const c10::cuda::CUDAGuard guard(x.device());
+    Tensor y = rows_like(x, {rows, s.rows});
+    const Tensor work = scratch(x, odie_linear4_scratch(rows, int(width), int(s.rows), int(s.groups), o.defined(), int(block)));
+    done(odie_linear4(data(in), static_cast<const uint8_t*>(data(codes)), static_cast<const uint8_t*>(data(scales)),
+                      static_cast<const float*>(data(row_scales)), int(block), data(b), data(r), rows, int(width), int(s.rows), int(s.groups),
+                      static_cast<const int32_t*>(data(o)), row_type(x), int(activation), data(y), data(work), stream_of(x)),
+         "odie_linear4");
+    return y.view(shape);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -387,4 +656,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("combine", &combine);
     m.def("linear", &linear);
     m.def("embed", &embed);
+    m.def("gate", &gate);
+    m.def("balance", &balance);
+    m.def("quantize", &quantize);
+    m.def("dequantize", [](const Tensor& codes, const Tensor& scales, const Tensor& row_scales, int64_t width, int64_t block, const py::object& dtype) {
+        return dequantize(codes, scales, row_scales, width, block, torch::python::detail::py_object_to_dtype(dtype));
+    });
+    m.def("linear4", &linear4);
 }

@@ -20,8 +20,10 @@ from torch import nn
 
 from . import _lib
 
-__all__ = ['RowOrder', 'sort_rows', 'dispatch', 'combine', 'linear', 'embed', 'check', 'ExpertHeads']
+__all__ = ['RowOrder', 'sort_rows', 'dispatch', 'combine', 'linear', 'embed', 'Gating', 'gate', 'Balance', 'balance', 'Micro', 'quantize',
+           'dequantize', 'linear4', 'check', 'ExpertHeads']
 
+SCORES = {'softmax': 0, 'sigmoid': 1}
 ACTIVATIONS = {'none': 0, 'relu': 1, 'silu': 2, 'gelu': 3}
 
 
@@ -92,6 +94,100 @@ def embed(ids, table, scale=1.0):
     """scale * table[ids]: ids of any shape (CUDA int32 or int64), table [rows, width] CUDA fp16, bf16 or fp32, result
     [*ids.shape, width] of the table's type.  An id outside the table gives a zero row and takes no gradient."""
     return _ops().embed(ids, table, scale)
+
+
+def _score(name):
+    code = SCORES.get(name)
+    if code is None:
+        raise ValueError(f'score must be one of {", ".join(SCORES)}')
+    return code
+
+
+class Gating(NamedTuple):
+    """The choices of rows (gate): expert int32 [rows, choices], -1 where none was left; weights fp32 [rows, choices]."""
+    expert: torch.Tensor
+    weights: torch.Tensor
+
+
+def gate(logits, choices, bias=None, mask=None, score='softmax', normalize=True, scale=1.0):
+    """The experts of each row, and their weights, from a router's logits [rows, experts] (CUDA fp16, bf16 or fp32).
+
+    A row takes its `choices` (up to 64) experts of the highest logit + bias (fp32; bias [experts], not differentiated),
+    ties to the lowest, among those whose mask (bool, broadcastable to the logits) is on and whose sum is not -inf; a
+    choice for which none is left is -1 with weight 0.  A NaN is taken first, and makes its row's weights NaN (a sigmoid
+    without normalize: its own).  weights: scale times the softmax over the row's open experts, or the sigmoid of the
+    logit, with `normalize` divided by its sum over the row's choices.  Differentiable in the logits through the weights.
+    For sort_rows, dispatch and combine.  Up to 1024 experts."""
+    return Gating(*_ops().gate(logits, choices, bias, mask, _score(score), normalize, scale))
+
+
+class Balance(NamedTuple):
+    """How evenly rows are spread over experts (balance): loss and z, fp32 scalars, and counts int32 [experts]."""
+    loss: torch.Tensor
+    z: torch.Tensor
+    counts: torch.Tensor
+
+
+def balance(logits, expert, mask=None, score='softmax', total=None):
+    """The balance loss of a router's logits [rows, experts] (CUDA fp16, bf16 or fp32) and choices `expert` (int32 or
+    int64, [rows] or [rows, choices]; values outside [0, experts) are dropped): experts * sum_e f_e P_e, which is 1 for
+    an even load.
+
+    f_e is expert e's share of the choices (without gradient), from `total` [experts], where given: counts summed over
+    several ranks, say.  P_e is the mean over live rows (those with an expert whose mask is on and whose logit is not -inf)
+    of the softmax over open experts, or with score 'sigmoid' of the sigmoids divided by their sum.  z: the mean over live
+    rows of the square of log sum exp of their logits.  counts: this call's choices of each expert.  Without rows or
+    choices the loss is 0.  Differentiable in the logits through loss and z."""
+    return Balance(*_ops().balance(logits, expert, mask, _score(score), total))
+
+
+class Micro(NamedTuple):
+    """Microscaled 4-bit rows (quantize): value = row scale x block scale x code.
+
+    codes uint8 [..., rows, 16 ceil(width / 32)]: e2m1, two to a byte, the even one low; scales uint8 [groups,
+    ceil(rows / 128), ceil(width / (4 block)), 512]: one for each block, e4m3 (block 16) or e8m0 (block 32), in tiles of
+    128 rows x 4 blocks: row r, block b at byte 16 (r % 32) + 4 (r // 32) + b; row_scales fp32 [..., rows]."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    row_scales: torch.Tensor
+    width: int
+    block: int
+
+    @property
+    def shape(self):
+        return torch.Size((*self.codes.shape[:-1], self.width))
+
+
+def quantize(x, block=16):
+    """x [rows, width] or [groups, rows, width] (CUDA fp16, bf16 or fp32, up to 2^20 columns) as microscaled 4-bit rows.
+
+    block 16: blocks of 16 values share an e4m3 scale, rows a power of two (so that the largest block's scale is near
+    e4m3's largest); block 32: blocks of 32 share a power of two, the least with which nothing saturates.  All roundings
+    to nearest even.  A row that holds an infinity or a NaN becomes NaN.  Not differentiable."""
+    return Micro(*_ops().quantize(x, block), x.shape[-1], block)
+
+
+def _micro(m):
+    if not isinstance(m, Micro):
+        raise ValueError('microscaled rows must be the Micro of quantize')
+    return m.codes, m.scales, m.row_scales, m.width, m.block
+
+
+def dequantize(micro, dtype=torch.float32):
+    """The values of microscaled rows, rounded to dtype (exact in fp32, and in bf16 for its normal numbers)."""
+    return _ops().dequantize(*_micro(micro), dtype)
+
+
+def linear4(x, weight, bias=None, residual=None, activation='none', offsets=None):
+    """`linear` in 4 bits, for decoding: residual + act(q(x) W^T + bias) with weight the Micro of quantize([outputs,
+    inputs]), or of [experts, outputs, inputs] with offsets, and q(x) the rows of x (CUDA fp16 or bf16) quantised in the
+    same format in the call; fp32 sums rounded once.  Everything else as for `linear`, but that there are no gradients: an
+    argument that wants one is refused.  A row's result does not depend on the rows beside it, but for the order of its
+    sum, which depends on how many there are."""
+    code = ACTIVATIONS.get(activation)
+    if code is None:
+        raise ValueError(f'activation must be one of {", ".join(ACTIVATIONS)}')
+    return _ops().linear4(x, *_micro(weight), bias, residual, code, offsets)
 
 
 def check(device=None):
