@@ -25,6 +25,7 @@ namespace {
 // for two blocks' scales; the epilogue reads the shared half first, and the next tile's products wait for that alone.
 constexpr int BK = 256;
 constexpr int EPILOGUE_WARP = 4;  // the first one
+constexpr int MAX_SHARED = 227 * 1024;
 
 struct Gemm4Args {
     int groups;
@@ -44,6 +45,9 @@ struct Gemm4Args {
     void* out;
     int activation;
     float* partial;      // splits: [split][rows][n] sums
+    bool boxes;          // TMA takes rows of out (every one starts on a 16-byte boundary); boxes_in: of the residual
+    bool boxes_in;
+    int stages;          // blocks in flight
     int* error;          // on the host: 2 once a wait has run out
     uint32_t limit;      // polls of a wait
 };
@@ -57,17 +61,21 @@ struct Shape4 {
     static constexpr int SA_BYTES = COLUMN_TILES * MICRO_TILE, SB_BYTES = BN / 128 * SA_BYTES;
     static constexpr int STAGE = A_BYTES + B_BYTES + SA_BYTES + SB_BYTES;
     static constexpr int STAGE_PITCH = (STAGE + 1023) / 1024 * 1024;
-    static constexpr int STAGES = 4;
+    static constexpr int STAGES = CG == 2 ? 4 : 5;  // at most: as many as there is room for beside the groups
     static constexpr int EPILOGUE_WARPS = 16, THREADS = (EPILOGUE_WARP + EPILOGUE_WARPS) * 32;
-    static constexpr int GROUPS = EPILOGUE_WARPS / 4;   // epilogue warps per set of 32 TMEM lanes
-    static constexpr int WINDOWS = BN / 32 / GROUPS;    // per warp and tile: columns 32 (group + GROUPS j)
+    static constexpr int COLS = BN / (EPILOGUE_WARPS / 4);  // columns of an epilogue warp's 32 rows: 64 or 32
+    static constexpr int BOX = 32 * COLS * 2;               // its rows in shared memory, in bytes, as TMA swizzles them
     static constexpr bool OVERLAP = BN == 256;
     static constexpr int SCALES_AT = OVERLAP ? 384 : 256;  // TMEM column of the scales, 64 per block
     static constexpr int SB_AT = COLUMN_TILES * 4;         // B's behind A's
     static constexpr int COLUMNS = 512;
-    static constexpr int WARP_BYTES = STAGING + WINDOWS * 256;  // staging tile, bias and column scales of an epilogue warp
-    static constexpr int HEAD = 1024;                           // barriers, TMEM address
-    static int bytes(int groups) { return 1024 + STAGES * STAGE_PITCH + EPILOGUE_WARPS * WARP_BYTES + HEAD + 3 * (groups + 2) * 4; }
+    // What the epilogue needs to know of a tile, written ahead by a warp of its own: the tile, its rows' scales, its
+    // columns' scales and bias (of two columns side by side).
+    static constexpr int SLOTS = 3, SLOT = 32 + 128 * 4 + BN * 8;
+    static constexpr int HEAD = 512;  // barriers, TMEM address
+    static int rest(int groups) { return 1024 + EPILOGUE_WARPS * BOX + SLOTS * SLOT + HEAD + 3 * (groups + 2) * 4; }
+    static int stages(int groups) { return std::min(STAGES, (MAX_SHARED - rest(groups)) / STAGE_PITCH); }
+    static int bytes(int groups) { return rest(groups) + stages(groups) * STAGE_PITCH; }
 };
 
 struct Tile4 {
@@ -131,23 +139,86 @@ struct Walk4 {
     }
 };
 
+// The 16-byte unit `unit` of a row of a box, as TMA's swizzle of its rows' length (128 or 64 bytes) places it.
+template <int COLS>
+__device__ __forceinline__ uint4* boxed(char* box, int row, int unit) {
+    return reinterpret_cast<uint4*>(box + row * (COLS * 2) + ((COLS == 64 ? unit ^ (row & 7) : unit ^ ((row >> 1) & 3)) << 4));
+}
+// The same rows moved by the warp itself: where some are outside the matrix, or do not start on 16-byte boundaries.
+template <int COLS, bool STORE>
+__device__ __forceinline__ void move_box(uint16_t* at, char* box, int ld, int rows, int columns, int lane) {
+    constexpr int UNITS = COLS / 8;
+    columns = min(columns, COLS);
+    if (ld % 8 == 0 && reinterpret_cast<uintptr_t>(at) % 16 == 0) {  // (columns are a multiple of 8 then)
+        for (int i = lane; i < rows * UNITS; i += 32) {
+            const int r = i / UNITS, u = i % UNITS;
+            if (u * 8 >= columns) continue;
+            uint4* out = reinterpret_cast<uint4*>(at + (long long)r * ld + u * 8);
+            if (STORE) *out = *boxed<COLS>(box, r, u);
+            else *boxed<COLS>(box, r, u) = *out;
+        }
+    } else {
+        for (int r = 0; r < rows; ++r)
+            for (int c = lane; c < columns; c += 32) {
+                uint16_t* in = reinterpret_cast<uint16_t*>(boxed<COLS>(box, r, c / 8)) + c % 8;
+                uint16_t* out = at + (long long)r * ld + c;
+                if (STORE) *out = *in;
+                else *in = *out;
+            }
+    }
+}
+
+// y = act((v r) c + b) (+ residual, in the box), rounded into the box.  A thread has the columns 8 u + 2 (lane % 4) + 0, 1 of
+// rows 8 j + lane / 4, as tcgen05.ld 16x256b and the 8 x 8 matrices of ldmatrix and stmatrix have them: c and b are read
+// once for four rows.  (With a row to a thread, every thread read every column's: the shared memory was busy with that for
+// longer than with the products.)  columns: c and b of two columns side by side.
+template <typename T, int ACT, int COLS, bool ADD>
+__device__ __forceinline__ void finish_box(const float (&v)[2][COLS / 2], const float (&row_scale)[4], const float* columns, char* box, int lane) {
+#pragma unroll
+    for (int u = 0; u < COLS / 8; ++u) {
+        const float4 cb = *reinterpret_cast<const float4*>(columns + (u * 4 + (lane & 3)) * 4);
+        const Pair c = pair(cb.x, cb.y), b = pair(cb.z, cb.w);
+        const uint32_t at = tc::smem_u32(boxed<COLS>(box, lane, u));
+        uint32_t out[4], in[4];
+        if (ADD) tc::load_matrices(at, in);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int e = u * 4 + j % 2 * 2;
+            const Pair z = fma2(mul2(pair(v[j / 2][e], v[j / 2][e + 1]), same(row_scale[j])), c, b);
+            Pair slope, added{};
+            if (ADD) {
+                const float2 f = unpack_pair<T>(in[j]);
+                added = pair(f.x, f.y);
+            }
+            const float2 y = both(activate<ACT, ADD>(z, slope, added));
+            out[j] = pack_pair<T>(y.x, y.y);
+        }
+        tc::store_matrices(at, out);
+    }
+}
+
 // PARTIAL: the sums go to p.partial as they are, joined by finish4_kernel.
 template <typename T, int CG, int BN, int BLOCK, bool PARTIAL>
 __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
     gemm4_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                 const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb, const Gemm4Args p) {
+                 const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb,
+                 const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_residual, const Gemm4Args p) {
     using S = Shape4<CG, BN, BLOCK>;
-    constexpr int STAGES = S::STAGES;
+    const int stage_count = p.stages;
     extern __shared__ char raw[];
     char* smem = reinterpret_cast<char*>((reinterpret_cast<uintptr_t>(raw) + 1023) / 1024 * 1024);
     char* stages = smem;
-    char* staging = stages + STAGES * S::STAGE_PITCH;
-    uint64_t* full = reinterpret_cast<uint64_t*>(staging + S::EPILOGUE_WARPS * S::WARP_BYTES);
-    uint64_t* empty = full + STAGES;
-    uint64_t* done = empty + STAGES;    // per accumulator: summed
+    char* boxes = stages + stage_count * S::STAGE_PITCH;
+    char* slots = boxes + S::EPILOGUE_WARPS * S::BOX;
+    uint64_t* full = reinterpret_cast<uint64_t*>(slots + S::SLOTS * S::SLOT);
+    uint64_t* empty = full + S::STAGES;
+    uint64_t* done = empty + S::STAGES; // per accumulator: summed
     uint64_t* drained = done + 2;       // per accumulator: read out (OVERLAP: what it shares with the other one)
     uint64_t* drain = drained + 2;
-    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(drain + 1);
+    uint64_t* arrived = drain + 1;      // per epilogue warp: its rows of the residual
+    uint64_t* told = arrived + S::EPILOGUE_WARPS;  // per slot: written
+    uint64_t* heard = told + S::SLOTS;             // per slot: read
+    uint32_t* tmem_at = reinterpret_cast<uint32_t*>(heard + S::SLOTS);
     uint32_t* gave_up = tmem_at + 1;    // a wait of either CTA has run out
     uint32_t* issued_by = gave_up + 1;  // [2], the leader's: blocks that each CTA has loaded
     int* begin = reinterpret_cast<int*>(reinterpret_cast<char*>(full) + S::HEAD);  // [groups + 2] first row of each group
@@ -159,13 +230,18 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
     const int nt = (p.n + BN - 1) / BN;
 
     if (warp == 0 && lane == 0) {
-        for (int s = 0; s < STAGES; ++s) {
+        for (int s = 0; s < stage_count; ++s) {
             tc::bar_init(full + s, 1);
             tc::bar_init(empty + s, 1);
         }
         for (int a = 0; a < 2; ++a) {
             tc::bar_init(done + a, 1);
-            tc::bar_init(drained + a, S::EPILOGUE_WARPS * CG);
+            tc::bar_init(drained + a, (S::OVERLAP ? S::EPILOGUE_WARPS / 2 : S::EPILOGUE_WARPS) * CG);
+        }
+        for (int w = 0; w < S::EPILOGUE_WARPS; ++w) tc::bar_init(arrived + w, 1);
+        for (int i = 0; i < S::SLOTS; ++i) {
+            tc::bar_init(told + i, 1);
+            tc::bar_init(heard + i, S::EPILOGUE_WARPS);
         }
         tc::bar_init(drain, 1);
         tc::fence_bar_init();
@@ -246,16 +322,16 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
                 }
                 __syncwarp();
                 ++issued;
-                if (++s == STAGES) {
+                if (++s == stage_count) {
                     s = 0;
                     phase ^= 1;
                 }
             }
         }
         // every stage read out: no arrival is on its way when the CTA ends, and no copy
-        for (int i = 0; i < STAGES && i < issued && fine; ++i) {
+        for (int i = 0; i < stage_count && i < issued && fine; ++i) {
             const int last = issued - 1 - i;
-            fine = __all_sync(0xffffffffu, tc::bar_wait(empty + last % STAGES, (last / STAGES) & 1, p.limit));
+            fine = __all_sync(0xffffffffu, tc::bar_wait(empty + last % stage_count, (last / stage_count) & 1, p.limit));
         }
         if (lane == 0) tc::store_leader<CG>(issued_by + rank, issued);
     } else if (warp == 1) {
@@ -301,7 +377,7 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
                     }
                     __syncwarp();
                     half ^= 1;
-                    if (++s == STAGES) {
+                    if (++s == stage_count) {
                         s = 0;
                         phase ^= 1;
                     }
@@ -311,46 +387,96 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
                 __syncwarp();
             }
         }
-    } else if (warp >= EPILOGUE_WARP) {
-        constexpr int WINDOWS = S::WINDOWS, STRIDE = 32 * S::GROUPS;
-        const int quadrant = warp & 3, group = (warp - EPILOGUE_WARP) >> 2;
-        char* stage = staging + (warp - EPILOGUE_WARP) * STAGING;
-        float* bias = reinterpret_cast<float*>(staging + S::EPILOGUE_WARPS * STAGING) + (warp - EPILOGUE_WARP) * WINDOWS * 64;
-        float* column_scale = bias + WINDOWS * 32;
-        const uint32_t lanes = tmem + (uint32_t(quadrant * 32) << 16);
-        const bool wide = p.n % 8 == 0 && reinterpret_cast<uintptr_t>(p.out) % 16 == 0;
-        const bool wide_residual = p.n % 8 == 0 && reinterpret_cast<uintptr_t>(p.residual) % 16 == 0;
-        int held_g = -1, held_n0 = -1;  // whose bias and scales are held
-        uint32_t summed = 0;
-        for (int t = start; t < tiles && fine; t += step, ++summed) {
+    } else if (warp == 3) {
+        // One tile ahead of the epilogue, whose warps would each wait for these loads, and walk, between two tiles (a third
+        // of its time).
+        int q = 0, phase = 1;
+        for (int t = start; t < tiles && fine; t += step) {
             const Tile4 tile = walk.at(t);
-            const int acc = summed & 1;
-            const int row = tile.m0 + rank * 128 + quadrant * 32, column0 = tile.n0 + group * 32;
-            const int rows = min(32, tile.m_end - row), columns = p.n - column0;  // inside the matrix, from `column0` on
-            const long long at = (long long)row * p.n + column0;
-            const uint16_t* residual = !PARTIAL && p.residual && !tile.zero ? static_cast<const uint16_t*>(p.residual) + at : nullptr;
-            // with OVERLAP the window that both accumulators share comes first
-            const bool turned = S::OVERLAP && acc == 0;
-            uint4 r[4];
-            float row_scale = 1.0f;
-            if (!PARTIAL && !tile.zero) {  // what does not need the sum is read while it is awaited
-                const int j = turned ? WINDOWS - 1 : 0;
-                if (residual && columns > j * STRIDE) {
-                    const Window w{p.n, rows, columns - j * STRIDE, wide_residual};
-                    if (w.wide) window_load(residual + j * STRIDE, w, lane, r);
-                    else window_fetch(residual + j * STRIDE, w, lane, stage);
-                }
-                if (lane < rows) row_scale = __ldg(p.row_scales + row + lane);
-                if (tile.g != held_g || tile.n0 != held_n0) {
-                    held_g = tile.g;
-                    held_n0 = tile.n0;
-                    __syncwarp();
+            float rows[4], columns[BN / 32], bias[BN / 32];
+            if (!PARTIAL && !tile.zero) {
 #pragma unroll
-                    for (int j = 0; j < WINDOWS; ++j) {
-                        const bool on = j * STRIDE + lane < columns;
-                        const long long from = (long long)tile.g * p.n + column0 + j * STRIDE + lane;
-                        bias[j * 32 + lane] = on && p.bias ? to_float(static_cast<const T*>(p.bias)[from]) : 0.0f;
-                        column_scale[j * 32 + lane] = on ? __ldg(p.column_scales + from) : 0.0f;
+                for (int i = 0; i < 4; ++i) {
+                    const int row = tile.m0 + rank * 128 + i * 32 + lane;
+                    rows[i] = row < tile.m_end ? __ldg(p.row_scales + row) : 0.0f;
+                }
+                const long long at = (long long)tile.g * p.n + tile.n0 + lane;
+#pragma unroll
+                for (int i = 0; i < BN / 32; ++i) columns[i] = tile.n0 + lane + i * 32 < p.n ? __ldg(p.column_scales + at + i * 32) : 0.0f;
+#pragma unroll
+                for (int i = 0; i < BN / 32; ++i)
+                    bias[i] = p.bias && tile.n0 + lane + i * 32 < p.n ? to_float(static_cast<const T*>(p.bias)[at + i * 32]) : 0.0f;
+            }
+            fine = __all_sync(0xffffffffu, tc::bar_wait(heard + q, phase, p.limit));
+            if (!fine) break;
+            int* slot = reinterpret_cast<int*>(slots + q * S::SLOT);
+            if (lane == 0) {
+                *reinterpret_cast<int4*>(slot) = make_int4(tile.g, tile.m0, tile.n0, tile.m_end);
+                *reinterpret_cast<int4*>(slot + 4) = make_int4(tile.split, tile.zero, 0, 0);
+            }
+            if (!PARTIAL && !tile.zero) {
+                float* to = reinterpret_cast<float*>(slot + 8);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) to[i * 32 + lane] = rows[i];
+                to += 128 + lane / 2 * 4 + lane % 2;
+#pragma unroll
+                for (int i = 0; i < BN / 32; ++i) {
+                    to[i * 64] = columns[i];
+                    to[i * 64 + 2] = bias[i];
+                }
+            }
+            __syncwarp();
+            if (lane == 0) tc::bar_arrive(told + q);
+            if (++q == S::SLOTS) {
+                q = 0;
+                phase ^= 1;
+            }
+        }
+    } else if (warp >= EPILOGUE_WARP) {
+        // Warp (group, quadrant) has rows 32 quadrant + lane and columns COLS group + 0 .. of a tile.  The residual is asked
+        // for as soon as the box is free; the box goes out by TMA.
+        constexpr int COLS = S::COLS;
+        const int index = warp - EPILOGUE_WARP, quadrant = warp & 3, group = index >> 2;
+        char* box = boxes + index * S::BOX;
+        const uint32_t lanes = tmem + (uint32_t(quadrant * 32) << 16) + group * COLS;
+        int q = 0, q_phase = 0;
+        uint32_t summed = 0, phase = 0;
+        bool asked = false;  // for rows of the residual that have not been awaited
+        for (int t = start; t < tiles; t += step, ++summed) {
+            fine = __all_sync(0xffffffffu, tc::bar_wait(told + q, q_phase, p.limit));
+            if (!fine) break;
+            const int* slot = reinterpret_cast<const int*>(slots + q * S::SLOT);
+            const int4 first_word = *reinterpret_cast<const int4*>(slot), second_word = *reinterpret_cast<const int4*>(slot + 4);
+            Tile4 tile;
+            tile.g = uniform(first_word.x);
+            tile.m0 = uniform(first_word.y);
+            tile.n0 = uniform(first_word.z);
+            tile.m_end = uniform(first_word.w);
+            tile.split = uniform(second_word.x);
+            tile.zero = uniform(second_word.y);
+            const float* column = reinterpret_cast<const float*>(slot + 8) + 128 + group * COLS * 2;
+            const int acc = summed & 1;
+            const int row = tile.m0 + rank * 128 + quadrant * 32, column0 = tile.n0 + group * COLS;
+            const int rows = min(32, tile.m_end - row), columns = p.n - column0;  // inside the matrix
+            const bool inside = rows > 0 && columns > 0, whole = rows == 32 && columns > 0;
+            const long long at = (long long)row * p.n + column0;
+            const bool residual = !PARTIAL && p.residual && !tile.zero && inside;
+            float row_scale[4];
+            if (!PARTIAL) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) row_scale[j] = reinterpret_cast<const float*>(slot + 8)[quadrant * 32 + j * 8 + lane / 4];
+                if (lane == 0) tc::stores_read();  // the box is free
+                __syncwarp();
+                if (residual) {
+                    if (whole && p.boxes_in) {
+                        if (lane == 0) {
+                            tc::fence_async_smem();
+                            tc::bar_expect(arrived + index, S::BOX);
+                            tc::tma_load_2d<1>(box, &map_residual, column0, row, tc::smem_u32(arrived + index));
+                        }
+                        asked = true;
+                    } else {
+                        move_box<COLS, false>(static_cast<uint16_t*>(const_cast<void*>(p.residual)) + at, box, p.n, rows, columns, lane);
                     }
                     __syncwarp();
                 }
@@ -358,86 +484,71 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
             fine = __all_sync(0xffffffffu, tc::bar_wait(done + acc, (summed >> 1) & 1, p.limit));
             if (!fine) break;
             tc::fence_after_sync();
-#pragma unroll 1
-            for (int i = 0; i < WINDOWS; ++i) {
-                const int j = turned ? WINDOWS - 1 - i : i;
-                const Window w{p.n, rows, columns - j * STRIDE, wide};
-                float v[32];
+            float v[2][COLS / 2];  // (of a tile of nothing: of no use)
+            tc::tmem_ld_rows<COLS>(lanes + acc * 128, v[0], v[1]);
+            if (!S::OVERLAP || (group >> 1) != acc) {  // with OVERLAP: the half that both accumulators have
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) tc::bar_arrive_cluster(CG == 2 ? tc::leader_address(drained + acc) : tc::smem_u32(drained + acc));
+            }
+            if (PARTIAL) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int r = j * 8 + lane / 4;
+                    float* to = p.partial + ((long long)tile.split * p.rows + row + r) * p.n + column0 + (lane & 3) * 2;
+                    if (r >= rows) continue;
+#pragma unroll
+                    for (int u = 0; u < COLS / 8; ++u) {
+                        const float x = v[j / 2][u * 4 + j % 2 * 2], y = v[j / 2][u * 4 + j % 2 * 2 + 1];
+                        const int left = columns - u * 8 - (lane & 3) * 2;
+                        if (p.n % 2 == 0) {
+                            if (left > 0) *reinterpret_cast<float2*>(to + u * 8) = make_float2(x, y);
+                        } else {
+                            if (left > 0) to[u * 8] = x;
+                            if (left > 1) to[u * 8 + 1] = y;
+                        }
+                    }
+                }
+            } else {
+                if (asked) {
+                    fine = __all_sync(0xffffffffu, tc::bar_wait(arrived + index, phase, p.limit));
+                    if (!fine) break;
+                    phase ^= 1;
+                    asked = false;
+                }
+                auto go = [&](auto act) {
+                    constexpr int ACT = decltype(act)::value;
+                    if (residual) finish_box<T, ACT, COLS, true>(v, row_scale, column, box, lane);
+                    else finish_box<T, ACT, COLS, false>(v, row_scale, column, box, lane);
+                };
                 if (tile.zero) {
 #pragma unroll
-                    for (int e = 0; e < 32; ++e) v[e] = 0.0f;
-                } else if (w.columns > 0) {
-                    tc::tmem_ld32(lanes + acc * 128 + group * 32 + j * STRIDE, v);
-                }
-                if (i == (S::OVERLAP ? 0 : WINDOWS - 1)) {
-                    tc::fence_before_sync();
+                    for (int u = 0; u < COLS / 8; ++u) *boxed<COLS>(box, lane, u) = make_uint4(0, 0, 0, 0);
+                } else if (p.activation == ACT_RELU) go(std::integral_constant<int, ACT_RELU>{});
+                else if (p.activation == ACT_SILU) go(std::integral_constant<int, ACT_SILU>{});
+                else if (p.activation == ACT_GELU) go(std::integral_constant<int, ACT_GELU>{});
+                else go(std::integral_constant<int, ACT_NONE>{});
+                __syncwarp();
+                if (lane == 0) tc::bar_arrive(heard + q);
+                if (whole && p.boxes) {
+                    tc::fence_async_smem();
                     __syncwarp();
-                    if (lane == 0) tc::bar_arrive_cluster(CG == 2 ? tc::leader_address(drained + acc) : tc::smem_u32(drained + acc));
+                    if (lane == 0) tc::tma_store_2d(&map_out, column0, row, box);
+                } else {
+                    __syncwarp();
+                    if (inside) move_box<COLS, true>(static_cast<uint16_t*>(p.out) + at, box, p.n, rows, columns, lane);
+                    __syncwarp();
                 }
-                if (w.columns <= 0) continue;
-                if (PARTIAL) {
-                    if (lane < rows) {
-                        float* to = p.partial + ((long long)tile.split * p.rows + row + lane) * p.n + column0 + j * STRIDE;
-                        if (p.n % 4 == 0) {
-#pragma unroll
-                            for (int e = 0; e < 32; e += 4)
-                                if (e < w.columns) *reinterpret_cast<float4*>(to + e) = make_float4(v[e], v[e + 1], v[e + 2], v[e + 3]);
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                if (e < w.columns) to[e] = v[e];
-                        }
-                    }
-                    continue;
-                }
-                if (!tile.zero) {
-                    if (residual) {
-                        if (wide_residual) {
-                            if (i > 0) window_load(residual + j * STRIDE, Window{p.n, rows, w.columns, true}, lane, r);
-#pragma unroll
-                            for (int u = 0; u < 4; ++u) *staged(stage, lane / 4 + 8 * u, lane & 3) = r[u];
-                        } else if (i > 0) {
-                            window_fetch(residual + j * STRIDE, Window{p.n, rows, w.columns, false}, lane, stage);
-                        }
-                        __syncwarp();
-                    }
-                    const Pair scale = same(row_scale);
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        const float2 c = *reinterpret_cast<const float2*>(column_scale + j * 32 + e);
-                        const float2 z = both(mul2(mul2(pair(v[e], v[e + 1]), scale), pair(c.x, c.y)));
-                        v[e] = z.x;
-                        v[e + 1] = z.y;
-                    }
-                    uint32_t codes[16];
-                    if (p.activation == ACT_RELU) finish_relu(v, bias + j * 32);
-                    else if (p.activation == ACT_SILU) finish<ACT_SILU>(v, codes, bias + j * 32);
-                    else if (p.activation == ACT_GELU) finish<ACT_GELU>(v, codes, bias + j * 32);
-                    else finish<ACT_NONE>(v, codes, bias + j * 32);
-                    if (residual) {
-#pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            const uint4 q = *staged(stage, lane, u);
-                            const uint32_t e[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                            for (int h = 0; h < 4; ++h) {
-                                const float2 f = unpack_pair<T>(e[h]);
-                                v[u * 8 + h * 2] += f.x;
-                                v[u * 8 + h * 2 + 1] += f.y;
-                            }
-                        }
-                        __syncwarp();
-                    }
-                }
-#pragma unroll
-                for (int u = 0; u < 4; ++u)
-                    *staged(stage, lane, u) = make_uint4(pack_pair<T>(v[u * 8], v[u * 8 + 1]), pack_pair<T>(v[u * 8 + 2], v[u * 8 + 3]),
-                                                         pack_pair<T>(v[u * 8 + 4], v[u * 8 + 5]), pack_pair<T>(v[u * 8 + 6], v[u * 8 + 7]));
-                __syncwarp();
-                window_store(static_cast<uint16_t*>(p.out) + at + j * STRIDE, w, lane, stage);
-                __syncwarp();
+            }
+            if (PARTIAL && lane == 0) tc::bar_arrive(heard + q);
+            if (++q == S::SLOTS) {
+                q = 0;
+                q_phase ^= 1;
             }
         }
+        if (asked) tc::bar_wait(arrived + index, phase, WAIT_LIMIT);  // (a wait has run out: no copy is left behind)
+        if (lane == 0) tc::stores_done();
+        __syncwarp();
     }
     if (!fine && lane == 0) {
         *static_cast<volatile int*>(p.error) = 2;
@@ -455,12 +566,12 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
         if (warp == 0 && rank == 0) {
             const int mine = int(tc::load_shared(issued_by)), other = CG == 2 ? int(tc::load_shared(issued_by + 1)) : mine;
             const uint32_t share = uint32_t(p.a_rows * 128 + S::B_BYTES + S::SA_BYTES + S::SB_BYTES);  // of one CTA in a block
-            for (int b = max(0, max(mine, other) - STAGES); b < max(mine, other); ++b) {
-                uint64_t* bar = full + b % STAGES;
+            for (int b = max(0, max(mine, other) - stage_count); b < max(mine, other); ++b) {
+                uint64_t* bar = full + b % stage_count;
                 if (lane == 0 && b >= mine) tc::bar_expect(bar, share);
                 if (lane == 0 && b >= other) tc::bar_unexpect(bar, share);
                 __syncwarp();
-                tc::bar_wait(bar, (b / STAGES) & 1, WAIT_LIMIT);
+                tc::bar_wait(bar, (b / stage_count) & 1, WAIT_LIMIT);
             }
         }
         if (warp == 1) {
@@ -555,8 +666,9 @@ struct Scratch4 {
     }
 };
 
-// A row-major array of bytes (4-byte units: words), the fastest dimension first, strides in bytes.
-CUtensorMap byte_map(const void* base, bool words, bool swizzled, int rank, const int64_t* dims, const int64_t* strides, const int* box) {
+// A row-major array, the fastest dimension first, strides in bytes.
+CUtensorMap tensor_map(const void* base, CUtensorMapDataType type, CUtensorMapSwizzle swizzle, int rank, const int64_t* dims, const int64_t* strides,
+                       const int* box) {
     CUtensorMap map;
     cuuint64_t d[4], s[3];
     cuuint32_t b[4], unit[4] = {1, 1, 1, 1};
@@ -566,9 +678,7 @@ CUtensorMap byte_map(const void* base, bool words, bool swizzled, int rank, cons
         if (i > 0) s[i - 1] = cuuint64_t(strides[i - 1]);
     }
     ODIE_REQUIRE(uintptr_t(base) % 16 == 0, "codes, scales and scratch must start on 16-byte boundaries");
-    const CUresult status = tensor_map_encoder()(&map, words ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT8, cuuint32_t(rank),
-                                                 const_cast<void*>(base), d, s, b, unit, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                                                 swizzled ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+    const CUresult status = tensor_map_encoder()(&map, type, cuuint32_t(rank), const_cast<void*>(base), d, s, b, unit, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     ODIE_REQUIRE(status == CUDA_SUCCESS, "cuTensorMapEncodeTiled failed with " + std::to_string(int(status)));
     return map;
@@ -587,19 +697,29 @@ void launch_gemm4(const Product4& x, Gemm4Args p, int64_t tiles, cudaStream_t st
     p.by_tiles = Divide::by(nt * ceil_div(p.rows, 128 * CG));
     const int64_t da[] = {pitch, p.rows}, ta[] = {pitch};
     const int xa[] = {128, p.a_rows};
-    const CUtensorMap map_a = byte_map(x.a, false, true, 2, da, ta, xa);
+    const CUtensorMap map_a = tensor_map(x.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, 2, da, ta, xa);
     const int64_t db[] = {pitch, p.n, p.groups}, tb[] = {pitch, pitch * p.n};
     const int xb[] = {128, S::B_ROWS, 1};
-    const CUtensorMap map_b = byte_map(x.b, false, true, 3, db, tb, xb);
+    const CUtensorMap map_b = tensor_map(x.b, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, 3, db, tb, xb);
     const int64_t dsa[] = {128, columns, p.a_tiles}, tsa[] = {MICRO_TILE, MICRO_TILE * columns};
     const int xsa[] = {128, S::COLUMN_TILES, 1};
-    const CUtensorMap map_sa = byte_map(x.sa, true, false, 3, dsa, tsa, xsa);
+    const CUtensorMap map_sa = tensor_map(x.sa, CU_TENSOR_MAP_DATA_TYPE_UINT32, CU_TENSOR_MAP_SWIZZLE_NONE, 3, dsa, tsa, xsa);
     const int64_t dsb[] = {128, columns, row_tiles, p.groups}, tsb[] = {MICRO_TILE, MICRO_TILE * columns, MICRO_TILE * columns * row_tiles};
     const int xsb[] = {128, S::COLUMN_TILES, BN / 128, 1};
-    const CUtensorMap map_sb = byte_map(x.sb, true, false, 4, dsb, tsb, xsb);
+    const CUtensorMap map_sb = tensor_map(x.sb, CU_TENSOR_MAP_DATA_TYPE_UINT32, CU_TENSOR_MAP_SWIZZLE_NONE, 4, dsb, tsb, xsb);
+
+    p.stages = S::stages(p.groups);
+    p.boxes = p.n % 8 == 0 && uintptr_t(p.out) % 16 == 0;
+    p.boxes_in = p.residual && p.n % 8 == 0 && uintptr_t(p.residual) % 16 == 0;
+    const int64_t dy[] = {p.n, p.rows}, ty[] = {int64_t(p.n) * 2};
+    const int xy[] = {S::COLS, 32};
+    const auto y_map = [&](bool on, const void* base) {
+        return on ? tensor_map(base, CU_TENSOR_MAP_DATA_TYPE_UINT16, S::COLS == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, 2, dy, ty, xy) : CUtensorMap{};
+    };
+    const CUtensorMap map_out = y_map(p.boxes, p.out), map_residual = y_map(p.boxes_in, p.residual);
 
     const auto kernel = gemm4_kernel<T, CG, BN, BLOCK, PARTIAL>;
-    ODIE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::bytes(1024)));
+    ODIE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SHARED));
     cudaLaunchConfig_t config{};
     config.gridDim = dim3(unsigned(std::min<int64_t>(tiles, sm_count() / CG) * CG));
     config.blockDim = dim3(S::THREADS);
@@ -611,7 +731,7 @@ void launch_gemm4(const Product4& x, Gemm4Args p, int64_t tiles, cudaStream_t st
     cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
     config.attrs = &cluster;
     config.numAttrs = 1;
-    ODIE_CUDA(cudaLaunchKernelEx(&config, kernel, map_a, map_b, map_sa, map_sb, p));
+    ODIE_CUDA(cudaLaunchKernelEx(&config, kernel, map_a, map_b, map_sa, map_sb, map_out, map_residual, p));
     note_launch();
 }
 
