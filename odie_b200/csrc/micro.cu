@@ -1,14 +1,18 @@
 // Rows as microscaled 4-bit floats and back (micro.cuh has the format).
 //
 // Bound by HBM.  A thread takes 16 values at a time, a row is 8 to 256 threads of a block, whose values stay in
-// registers between the row's maximum and the rounding (up to 64 per thread; longer rows are read again from L2).
+// registers between the row's maximum and the rounding (up to 64 per thread; longer rows are read again from L2).  Rows
+// that do not start on 16-byte boundaries are moved element by element, neighbours by neighbouring threads, through
+// shared memory.
 //
 // Roundings are exact: a quotient next to a border between two codes decides by a whole step.  x / R is exact.  For
-// 16-bit x, q = x / (R s) is x times the rounded inverse of s, within 2^-22 of the quotient; a quotient of an 11-bit x
-// that is not itself on a border (a number of three bits, times the four of s) is at least 2^-13 away from it, so that q
-// rounded to a multiple of 2^-17 is on the border where the quotient is, and on the quotient's side of it else.  fp32 x
-// and the scales take a division whose remainder, where it is not zero, goes into the last bit (rounding to odd:
-// Boldo and Melquiond, "Emulation of FMA and correctly rounded sums", 2008), which makes the second rounding right.
+// 16-bit x, q = x / (R s) is x times an approximate inverse of s, within 2^-22 of the quotient, rounded to a multiple of
+// 2^-17 (by adding 96 in the same fused step): a quotient of an 11-bit x that is not itself on a border (a number of
+// three bits, times the four of s) is at least 2^-13 away from it, so that the rounded q is on the border where the
+// quotient is, and on the quotient's side of it else.  Their scales likewise, rounded to 16 bits: a border of e4m3 is a
+// number of five bits, times 6.  fp32 x and its scales take a division whose remainder, where it is not zero, goes into the
+// last bit (rounding to odd: Boldo and Melquiond, "Emulation of FMA and correctly rounded sums", 2008), which makes the
+// second rounding right.
 #include "micro.cuh"
 #include "odie_b200.h"
 #include <algorithm>
@@ -33,7 +37,7 @@ __device__ __forceinline__ int least_power(uint32_t bits, uint32_t most_mantissa
     return max(least, e);  // (a subnormal v: far below any `least`)
 }
 // Eight values as codes, the first in the lowest four bits.
-__device__ __forceinline__ uint32_t codes_of(const float (&q)[8]) {
+__device__ __forceinline__ uint32_t codes_of(const float2 (&q)[4]) {
     uint32_t r;
     asm("{\n\t.reg .b8 a, b, c, d;\n\t"
         "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
@@ -42,90 +46,139 @@ __device__ __forceinline__ uint32_t codes_of(const float (&q)[8]) {
         "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
         "mov.b32 %0, {a, b, c, d};\n\t}"
         : "=r"(r)
-        : "f"(q[0]), "f"(q[1]), "f"(q[2]), "f"(q[3]), "f"(q[4]), "f"(q[5]), "f"(q[6]), "f"(q[7]));
+        : "f"(q[0].x), "f"(q[0].y), "f"(q[1].x), "f"(q[1].y), "f"(q[2].x), "f"(q[2].y), "f"(q[3].x), "f"(q[3].y));
     return r;
+}
+__device__ __forceinline__ float e4m3_value(uint32_t byte) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(uint8_t(byte), __NV_E4M3))); }
+
+// Where N values of each thread of a row are exchanged, one word per row of N beyond them: no two in one bank.  value(i): the
+// thread's i-th of its N neighbours' in a row; strided(i): the one that is i x lanes behind its lane's (lanes a multiple of N).
+template <int N>
+struct Exchange {
+    uint32_t *row, *at;
+    int step;
+    __device__ __forceinline__ Exchange(uint32_t* words, int lanes, int lane) {
+        words += (threadIdx.x - lane) * (N + 1);
+        row = words + lane * (N + 1);
+        at = words + lane + lane / N;
+        step = lanes + lanes / N;
+    }
+    __device__ __forceinline__ uint32_t& value(int i) const { return row[i]; }
+    __device__ __forceinline__ uint32_t& strided(int i) const { return at[i * step]; }
+};
+__device__ __forceinline__ void sync_row(int lanes) {  // the threads of a row
+    if (lanes > 32) __syncthreads();
+    else __syncwarp();
 }
 
 // 16 consecutive values of a row from column c on, zeros behind its end.
 template <typename T>
 struct Run {
-    uint32_t w[16 * sizeof(T) / 4];
-    template <bool WIDE>
-    __device__ __forceinline__ void load(const T* row, long long c, int width) {
+    static constexpr int WORDS = 16 * sizeof(T) / 4;
+    uint32_t w[WORDS];
+    __device__ __forceinline__ void load_wide(const T* row, long long c, int width) {  // width a multiple of PER
         constexpr int PER = 16 / int(sizeof(T));
-        if (WIDE) {  // width a multiple of PER
 #pragma unroll
-            for (int i = 0; i < int(sizeof(T)); ++i) {
-                const uint4 v = c + i * PER < width ? __ldg(reinterpret_cast<const uint4*>(row + c + i * PER)) : make_uint4(0, 0, 0, 0);
-                w[4 * i] = v.x;
-                w[4 * i + 1] = v.y;
-                w[4 * i + 2] = v.z;
-                w[4 * i + 3] = v.w;
-            }
-        } else if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) w[i] = c + i < width ? __float_as_uint(row[c + i]) : 0u;
-        } else {
-            const uint16_t* at = reinterpret_cast<const uint16_t*>(row);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                w[i] = (c + 2 * i < width ? at[c + 2 * i] : 0u) | uint32_t(c + 2 * i + 1 < width ? at[c + 2 * i + 1] : 0u) << 16;
+        for (int i = 0; i < int(sizeof(T)); ++i) {
+            const uint4 v = c + i * PER < width ? __ldg(reinterpret_cast<const uint4*>(row + c + i * PER)) : make_uint4(0, 0, 0, 0);
+            w[4 * i] = v.x;
+            w[4 * i + 1] = v.y;
+            w[4 * i + 2] = v.z;
+            w[4 * i + 3] = v.w;
         }
     }
-    __device__ __forceinline__ float value(int i) const {
-        if constexpr (sizeof(T) == 4) {
-            return __uint_as_float(w[i]);
-        } else {
-            const float2 f = unpack_pair<T>(w[i / 2]);
-            return i % 2 ? f.y : f.x;
+    // The row's `lanes` threads take its 16 lanes values from `from` on, `left` of them inside.
+    __device__ __forceinline__ void load(const T* from, int left, int lanes, int lane, const Exchange<16>& x) {
+        from += lane;
+        left -= lane;
+        uint32_t v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            if constexpr (sizeof(T) == 4) v[i] = i * lanes < left ? __float_as_uint(from[i * lanes]) : 0u;
+            else v[i] = i * lanes < left ? reinterpret_cast<const uint16_t*>(from)[i * lanes] : 0u;
         }
+        sync_row(lanes);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x.strided(i) = v[i];
+        sync_row(lanes);
+#pragma unroll
+        for (int i = 0; i < WORDS; ++i) {
+            if constexpr (sizeof(T) == 4) w[i] = x.value(i);
+            else w[i] = x.value(2 * i) | x.value(2 * i + 1) << 16;
+        }
+    }
+    __device__ __forceinline__ float2 pair_at(int i) const {  // values 2 i and 2 i + 1
+        if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+        else return unpack_pair<T>(w[i]);
     }
     // The bits of the largest magnitude as fp32: those of infinities and NaNs are the largest.
     __device__ __forceinline__ uint32_t largest() const {
         uint32_t m = 0;
+        if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) m = max(m, __float_as_uint(value(i)) & 0x7fffffffu);
-        return m;
+            for (int i = 0; i < 16; ++i) m = max(m, w[i] & 0x7fffffffu);
+            return m;
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
+            m = max(m & 0xffffu, m >> 16);
+            if constexpr (std::is_same<T, __nv_bfloat16>::value) return m << 16;
+            else return __float_as_uint(__half2float(__ushort_as_half(uint16_t(m))));
+        }
     }
 };
 
 // Sixteen codes and their scale's byte; largest: of the block.
 template <typename T, int BLOCK>
 __device__ __forceinline__ uint2 round_run(const Run<T>& x, uint32_t largest, float inverse_row, uint32_t& scale) {
-    float factor, divisor = 1.0f;
-    if (BLOCK == 16) {
-        scale = __nv_cvt_float_to_fp8(divide_odd(__uint_as_float(largest) * inverse_row, 6.0f), __NV_SATFINITE, __NV_E4M3);
-        divisor = __half2float(__half(__nv_cvt_fp8_to_halfraw(uint8_t(scale), __NV_E4M3)));
-        factor = scale ? __frcp_rn(divisor) : 0.0f;
-    } else {
+    float2 q[8];
+    if constexpr (BLOCK == 32) {
         const int e = least_power(largest, 0x400000u, 2, -127);
         scale = uint32_t(e + 127);
-        factor = power_of_two(-e);
-    }
-    uint32_t out[2];
+        const Pair factor = same(power_of_two(-e));
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        float q[8];
+        for (int i = 0; i < 8; ++i) q[i] = both(mul2(pair(x.pair_at(i).x, x.pair_at(i).y), factor));
+    } else if constexpr (sizeof(T) == 2) {
+        const float t = __uint_as_float(largest) * inverse_row * (1.0f / 6.0f), wide = t * 257.0f;
+        scale = __nv_cvt_float_to_fp8(__fsub_rn(wide, __fsub_rn(wide, t)), __NV_SATFINITE, __NV_E4M3);
+        const float factor = scale ? inverse_approx(e4m3_value(scale)) : 0.0f;
+        const Pair up = same(96.0f), down = same(-96.0f);
+        if (std::is_same<T, __half>::value || inverse_row < 0x1p100f) {
+            const Pair by = same(inverse_row * factor);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float v = x.value(h * 8 + i);
-            if (BLOCK == 32) {
-                q[i] = v * factor;
-            } else if (sizeof(T) == 2) {
-                q[i] = __fsub_rn(__fadd_rn(v * inverse_row * factor, 96.0f), 96.0f);
-            } else {
-                q[i] = scale ? copysignf(divide_odd(fabsf(v) * inverse_row, divisor), v) : 0.0f;
+            for (int i = 0; i < 8; ++i) {
+                const float2 v = x.pair_at(i);
+                q[i] = both(add2(fma2(pair(v.x, v.y), by, up), down));
+            }
+        } else {  // the factors' product may be infinite
+            const Pair first = same(inverse_row), second = same(factor);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float2 v = x.pair_at(i);
+                q[i] = both(add2(fma2(mul2(pair(v.x, v.y), first), second, up), down));
             }
         }
-        out[h] = codes_of(q);
+    } else {
+        scale = __nv_cvt_float_to_fp8(divide_odd(__uint_as_float(largest) * inverse_row, 6.0f), __NV_SATFINITE, __NV_E4M3);
+        const float divisor = scale ? e4m3_value(scale) : INFINITY;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float2 v = x.pair_at(i);
+            q[i].x = copysignf(divide_odd(fabsf(v.x) * inverse_row, divisor), v.x);
+            q[i].y = copysignf(divide_odd(fabsf(v.y) * inverse_row, divisor), v.y);
+        }
+        if (!scale) return make_uint2(0, 0);
     }
-    return make_uint2(out[0], out[1]);
+    const float2 low[4] = {q[0], q[1], q[2], q[3]}, high[4] = {q[4], q[5], q[6], q[7]};
+    return make_uint2(codes_of(low), codes_of(high));
 }
 
 template <typename T, int BLOCK, bool WIDE>
-__global__ void __launch_bounds__(MICRO_THREADS) quantize_kernel(MicroArgs a, int lanes_log2) {
+__global__ void __launch_bounds__(MICRO_THREADS, sizeof(T) == 2 ? 4 : 2) quantize_kernel(MicroArgs a, int lanes_log2) {
     __shared__ uint32_t tops[MICRO_THREADS / 32];
+    __shared__ uint32_t words[WIDE ? 1 : MICRO_THREADS * 17];
     const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1), line = threadIdx.x >> lanes_log2;
+    const Exchange<16> exchange(words, lanes, lane);
     // the tile of rows
     const int tile = blockIdx.x / a.first_blocks, part = blockIdx.x - tile * a.first_blocks;
     long long from, to;
@@ -143,23 +196,31 @@ __global__ void __launch_bounds__(MICRO_THREADS) quantize_kernel(MicroArgs a, in
     const long long row = from + inside;
     const bool live = row < to;
     const T* x = static_cast<const T*>(a.x) + row * a.width;
-    const int steps = int((a.columns * (4 * BLOCK) + 16 * lanes - 1) / (16 * lanes));
+    const int steps = int((uint32_t(a.columns) * (4 * BLOCK) + 16 * lanes - 1) >> (lanes_log2 + 4));
+    auto load = [&](Run<T>& run, int s) {
+        const int first = s * lanes * 16;
+        if constexpr (WIDE) {
+            if (live && first + lane * 16 < a.width) run.load_wide(x, first + lane * 16, a.width);
+        } else {
+            run.load(x + first, live ? a.width - first : 0, lanes, lane, exchange);
+        }
+    };
 
     Run<T> held[HELD];
-    uint32_t top = 0;
+    uint32_t largest[HELD], top = 0;
 #pragma unroll
     for (int s = 0; s < HELD; ++s) {
-        const long long c = ((long long)s * lanes + lane) * 16;
         held[s] = Run<T>{};
-        if (live && c < a.width) held[s].template load<WIDE>(x, c, a.width);
+        if (s < steps) load(held[s], s);
     }
 #pragma unroll
-    for (int s = 0; s < HELD; ++s) top = max(top, held[s].largest());
+    for (int s = 0; s < HELD; ++s) {
+        largest[s] = held[s].largest();
+        top = max(top, largest[s]);
+    }
     for (int s = HELD; s < steps; ++s) {
-        const long long c = ((long long)s * lanes + lane) * 16;
-        if (!live || c >= a.width) continue;
-        Run<T> run;
-        run.template load<WIDE>(x, c, a.width);
+        Run<T> run{};
+        load(run, s);
         top = max(top, run.largest());
     }
     for (int d = 1; d < min(32, lanes); d *= 2) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
@@ -170,15 +231,19 @@ __global__ void __launch_bounds__(MICRO_THREADS) quantize_kernel(MicroArgs a, in
         for (int w = 0; w < lanes / 32; ++w) top = max(top, tops[first + w]);
     }
     const bool finite = top < 0x7f800000u;
-    const int k = BLOCK == 16 && top ? least_power(top, 0x280000u, 11, -126) : 0;
+    const int k = BLOCK == 16 && top && finite ? least_power(top, 0x280000u, 11, -126) : 0;
     const float inverse_row = power_of_two(-k);
     if (live && lane == 0) a.row_scales[row] = finite ? power_of_two(k) : __int_as_float(0x7fffffff);
 
-    auto finish = [&](const Run<T>& run, int s) {
-        const long long unit = (long long)s * lanes + lane, c = unit * 16;
-        uint32_t largest = run.largest(), scale = 0;
-        if (BLOCK == 32) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
-        uint2 codes = round_run<T, BLOCK>(run, finite ? largest : 0u, inverse_row, scale);
+    constexpr uint32_t PER = BLOCK / 4;  // threads of four scales
+    const uint32_t columns = uint32_t(a.columns), pitch = uint32_t(a.pitch);
+    uint8_t* codes_at = a.codes + row * a.pitch + lane * 8;
+    uint8_t* scales_at = a.scales + ((long long)tile * a.columns + uint32_t(lane) / PER) * MICRO_TILE + micro_byte(inside);
+    auto finish = [&](const Run<T>& run, uint32_t most, int s) {
+        const uint32_t unit = uint32_t(s) * lanes + lane;
+        uint32_t scale = 0;
+        if (BLOCK == 32) most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+        uint2 codes = round_run<T, BLOCK>(run, finite ? most : 0u, inverse_row, scale);
         if (!finite || !live) {
             codes = make_uint2(0, 0);
             scale = 0;
@@ -191,19 +256,16 @@ __global__ void __launch_bounds__(MICRO_THREADS) quantize_kernel(MicroArgs a, in
             scale |= __shfl_xor_sync(0xffffffffu, scale, 2) << 8;
             scale |= __shfl_xor_sync(0xffffffffu, scale, 4) << 16;
         }
-        const int per = BLOCK / 4;  // threads of a word
-        if (lane % per == 0 && unit / per < a.columns)
-            *reinterpret_cast<uint32_t*>(a.scales + ((long long)tile * a.columns + unit / per) * MICRO_TILE + micro_byte(inside)) = scale;
-        if (live && c / 2 < a.pitch) *reinterpret_cast<uint2*>(a.codes + row * a.pitch + c / 2) = codes;
+        if (lane % PER == 0 && unit / PER < columns) *reinterpret_cast<uint32_t*>(scales_at + uint32_t(s) * (uint32_t(lanes) / PER) * MICRO_TILE) = scale;
+        if (live && unit * 8 < pitch) *reinterpret_cast<uint2*>(codes_at + uint32_t(s) * lanes * 8) = codes;
     };
 #pragma unroll
     for (int s = 0; s < HELD; ++s)
-        if (s < steps) finish(held[s], s);
+        if (s < steps) finish(held[s], largest[s], s);
     for (int s = HELD; s < steps; ++s) {
-        const long long c = ((long long)s * lanes + lane) * 16;
         Run<T> run{};
-        if (live && c < a.width) run.template load<WIDE>(x, c, a.width);
-        finish(run, s);
+        load(run, s);
+        finish(run, run.largest(), s);
     }
 }
 
@@ -213,49 +275,78 @@ struct ValuesArgs {
     const float* row_scales;
     long long rows;
     int width;
-    long long group_rows;
+    uint32_t group_rows;
     long long pitch, columns;
     void* out;
-    long long units;  // of 16 values, per row
 };
+constexpr int VALUES_RUNS = 4;  // of a thread, that finding its row's place is worth it
 
+// A row by 2^lanes_log2 threads, N values (16 bytes, or 8 values that leave one by one) of each at a time.
 template <typename T, int BLOCK, bool WIDE>
-__global__ void __launch_bounds__(256) values_kernel(ValuesArgs a) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    const long long row = i / a.units;
-    if (row >= a.rows) return;
-    const int c = int(i - row * a.units) * 16;
-    const long long g = row / a.group_rows, inside = row - g * a.group_rows, tiles = (a.group_rows + MICRO_ROWS - 1) / MICRO_ROWS;
-    const long long tile = g * tiles + inside / MICRO_ROWS;
-    const int block = c / BLOCK;
-    const uint32_t scale = a.scales[(tile * a.columns + block / 4) * MICRO_TILE + micro_byte(int(inside % MICRO_ROWS)) + block % 4];
-    const uint2 codes = *reinterpret_cast<const uint2*>(a.codes + row * a.pitch + c / 2);
-    const float s = BLOCK == 16 ? __half2float(__half(__nv_cvt_fp8_to_halfraw(uint8_t(scale), __NV_E4M3)))
-                                : scale ? __uint_as_float(scale << 23) : 0x1p-127f;
-    const float r = a.row_scales[row];
-    float v[16];
+__global__ void __launch_bounds__(MICRO_THREADS) values_kernel(ValuesArgs a, int lanes_log2) {
+    constexpr int N = WIDE ? 16 / int(sizeof(T)) : 8;
+    __shared__ uint32_t shared_words[WIDE ? 1 : MICRO_THREADS * (N + 1)];
+    const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1);
+    const Exchange<N> exchange(shared_words, lanes, lane);
+    const long long row = (long long)blockIdx.x * (MICRO_THREADS >> lanes_log2) + (threadIdx.x >> lanes_log2);
+    const bool live = row < a.rows;
+    const uint32_t g = live ? uint32_t(row) / a.group_rows : 0, inside = uint32_t(row) - g * a.group_rows;
+    const long long tile = (long long)g * ((a.group_rows + MICRO_ROWS - 1) / MICRO_ROWS) + inside / MICRO_ROWS;
+    const uint8_t* scales = a.scales + tile * a.columns * MICRO_TILE + micro_byte(inside % MICRO_ROWS);
+    const uint8_t* codes_at = a.codes + row * a.pitch;
+    T* out = static_cast<T*>(a.out) + row * a.width;
+    const float row_scale = live ? __ldg(a.row_scales + row) : 0.0f;
+    const uint32_t width = a.width;
+    const uint32_t steps = (width + N * lanes - 1) >> (lanes_log2 + (N == 8 ? 3 : 2));
+#pragma unroll VALUES_RUNS
+    for (uint32_t s = 0; s < steps; ++s) {
+        const uint32_t first = s * lanes * N, c = first + lane * N;
+        uint32_t words[N * sizeof(T) / 4];
+        if (live && c < width) {
+            const uint32_t block = c / BLOCK;
+            const uint32_t scale = __ldg(scales + block / 4 * MICRO_TILE + block % 4);  // (at most 2^16 x 512 bytes)
+            const uint32_t codes = N == 8 ? __ldg(reinterpret_cast<const uint32_t*>(codes_at + c / 2)) : uint32_t(__ldg(reinterpret_cast<const uint16_t*>(codes_at + c / 2)));
+            // both exact, and their product too: six bits
+            const Pair by = same((BLOCK == 16 ? e4m3_value(scale) : scale ? __uint_as_float(scale << 23) : 0x1p-127f) * row_scale);
 #pragma unroll
-    for (int e = 0; e < 16; ++e) {
-        // e2m1 as fp16, its exponent's bias 14 too small: exact, subnormals too
-        const uint32_t code = (e < 8 ? codes.x : codes.y) >> (e % 8 * 4);
-        const float m = __half2float(__ushort_as_half(uint16_t((code & 8) << 12 | (code & 7) << 9))) * 16384.0f;
-        v[e] = m * s * r;
-    }
-    T* out = static_cast<T*>(a.out) + row * a.width + c;
-    if (WIDE) {
-        constexpr int PER = 16 / int(sizeof(T));
-#pragma unroll
-        for (int p = 0; p < 16 / PER; ++p) {
-            Pack<T, 16> pack;
-#pragma unroll
-            for (int e = 0; e < PER; ++e) pack.v[e] = from_float<T>(v[p * PER + e]);
-            if (c + p * PER < a.width) pack.store(out + p * PER);
+            for (int e = 0; e < N / 2; ++e) {
+                uint32_t halves;
+                asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\t}" : "=r"(halves) : "r"(codes >> (e * 8)));
+                const float2 m = __half22float2(*reinterpret_cast<const __half2*>(&halves)), v = both(mul2(pair(m.x, m.y), by));
+                if constexpr (sizeof(T) == 4) {
+                    words[2 * e] = __float_as_uint(v.x);
+                    words[2 * e + 1] = __float_as_uint(v.y);
+                } else {
+                    words[e] = pack_pair<T>(v.x, v.y);
+                }
+            }
         }
-    } else {
+        if constexpr (WIDE) {
+            if (live && c < width) *reinterpret_cast<uint4*>(out + c) = make_uint4(words[0], words[1], words[2], words[3]);
+        } else {
+            sync_row(lanes);
 #pragma unroll
-        for (int e = 0; e < 16; ++e)
-            if (c + e < a.width) out[e] = from_float<T>(v[e]);
+            for (int e = 0; e < N; ++e) exchange.value(e) = sizeof(T) == 4 ? words[e * sizeof(T) / 4] : words[e * sizeof(T) / 4] >> (e % 2 * 16);
+            sync_row(lanes);
+            const int left = live ? int(width - first) - lane : 0;
+            T* to = out + first + lane;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                if (e * lanes >= left) continue;
+                if constexpr (sizeof(T) == 4) to[e * lanes] = __uint_as_float(exchange.strided(e));
+                else reinterpret_cast<uint16_t*>(to)[e * lanes] = uint16_t(exchange.strided(e));
+            }
+        }
     }
+}
+
+// The threads of a row, as a power of two of at least 2^least: as few as take it in `runs` runs of n values each; more, up
+// to one run each, where the rows leave threads idle (four blocks to an SM).
+int row_lanes(int64_t rows, int64_t width, int n, int runs, int least) {
+    int log2 = least;
+    while (log2 < 8 && (int64_t(n) * runs << log2) < width) ++log2;
+    while (log2 < 8 && (int64_t(n) << log2) < width && (rows << log2) < 148 * 4 * MICRO_THREADS) ++log2;
+    return log2;
 }
 
 bool wide_rows(const void* p, int64_t width, int dtype) { return (uintptr_t(p) | uintptr_t(width * row_type_size(dtype))) % 16 == 0; }
@@ -284,13 +375,12 @@ void check_micro(int64_t groups, int64_t rows, int64_t width, int dtype, int blo
 }  // namespace
 
 void launch_quantize(MicroArgs a, int dtype, int block, cudaStream_t stream) {
-    // as few threads to a row as hold it: more rows at a time
-    int log2 = 3;
-    while (log2 < 8 && (16 * HELD << log2) < a.width) ++log2;
+    const bool whole = wide_rows(a.x, a.width, dtype);
+    const int log2 = row_lanes(a.rows, a.width, 16, HELD, whole ? 3 : 4);
     a.first_blocks = MICRO_ROWS / (MICRO_THREADS >> log2);
     const int64_t tiles = a.offsets ? micro_tiles(a.rows, a.groups) : a.groups * ((a.group_rows + MICRO_ROWS - 1) / MICRO_ROWS);
     ODIE_REQUIRE(tiles * a.first_blocks < (int64_t(1) << 31), "too many rows for one launch");
-    with_micro(dtype, block, wide_rows(a.x, a.width, dtype), [&](auto type, auto b, auto wide) {
+    with_micro(dtype, block, whole, [&](auto type, auto b, auto wide) {
         quantize_kernel<decltype(type), decltype(b)::value, decltype(wide)::value>
             <<<unsigned(tiles * a.first_blocks), MICRO_THREADS, 0, stream>>>(a, log2);
     });
@@ -331,12 +421,14 @@ extern "C" int odie_dequantize(const uint8_t* codes, const uint8_t* scales, cons
         if (rows == 0) return;
         ODIE_REQUIRE(codes && scales && row_scales && out, "codes, scales, row_scales and out are required");
         ODIE_REQUIRE((uintptr_t(codes) | uintptr_t(scales)) % 16 == 0, "codes and scales must start on 16-byte boundaries");
-        const ValuesArgs a{codes, scales, row_scales, groups * rows, int(width), rows, micro_pitch(width), micro_columns(width, block), out, (width + 15) / 16};
-        const int64_t blocks = (a.rows * a.units + 255) / 256;
-        ODIE_REQUIRE(blocks < (int64_t(1) << 31), "too many rows and columns for one launch");
-        with_micro(dtype, block, wide_rows(out, width, dtype), [&](auto type, auto b, auto wide) {
+        const ValuesArgs a{codes, scales, row_scales, groups * rows, int(width), uint32_t(rows), micro_pitch(width), micro_columns(width, block), out};
+        const bool whole = wide_rows(out, width, dtype);
+        const int n = whole ? 16 / row_type_size(dtype) : 8;  // values_kernel's N
+        const int log2 = row_lanes(a.rows, width, n, VALUES_RUNS, whole ? 0 : 3);
+        const int64_t blocks = (a.rows + (MICRO_THREADS >> log2) - 1) / (MICRO_THREADS >> log2);
+        with_micro(dtype, block, whole, [&](auto type, auto b, auto wide) {
             values_kernel<decltype(type), decltype(b)::value, decltype(wide)::value>
-                <<<unsigned(blocks), 256, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a);
+                <<<unsigned(blocks), MICRO_THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a, log2);
         });
         ODIE_CUDA(cudaGetLastError());
         note_launch();
