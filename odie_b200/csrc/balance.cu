@@ -31,51 +31,49 @@ struct BalanceArgs {
 };
 
 // p of a row (unscaled: times `inverse` of it), the softmax's numerators where they differ, and lse.
-template <int V, bool SIGMOID>
+template <int V, int LANES, bool SIGMOID>
 struct Shares {
     float p[V];
     float soft[SIGMOID ? V : 1];
     float inverse, soft_inverse, lse;
     bool live;
-    __device__ __forceinline__ Shares(const float (&v)[V], int lanes_log2) {
-        float top = NOTHING, sum = 0.0f, soft_sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < V; ++i) top = v[i] > top || v[i] != v[i] ? v[i] : top;
-        top = group_max(top, lanes_log2);
+    __device__ __forceinline__ explicit Shares(const float (&v)[V]) {
+        const float top = group_max<LANES>(largest(v));
         live = top != NOTHING;
-        const float base = live ? top : 0.0f, low = fminf(base, 0.0f);
+        const float base = live ? top : 0.0f;
+        float sum;
+        if constexpr (SIGMOID) {
+            const float low = fminf(base, 0.0f);
+            float all = 0.0f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const float e = expf(v[i] - base);
-            if (SIGMOID) {
-                // divided by e^low, lest all of a row's sigmoids underflow
-                soft[i] = e;
-                const float t = expf(-fabsf(v[i]));
-                p[i] = (v[i] >= 0.0f ? 1.0f : low == 0.0f ? t : expf(v[i] - low)) / (1.0f + t);
-                soft_sum += e;
-            } else {
-                p[i] = e;
+            for (int i = 0; i < V; ++i) {
+                p[i] = sigmoid_over(v[i], low);
+                all += p[i];
+                soft[i] = v[i];
             }
-            sum += p[i];
+            // (every lane of the warp takes part in both sums, live or not)
+            sum = group_sum<LANES>(powers(soft, base));
+            all = group_sum<LANES>(all);
+            inverse = live ? inverse_approx(all) : 0.0f;
+            soft_inverse = live ? inverse_approx(sum) : 0.0f;
+        } else {
+#pragma unroll
+            for (int i = 0; i < V; ++i) p[i] = v[i];
+            sum = group_sum<LANES>(powers(p, base));
+            soft_inverse = inverse = live ? inverse_approx(sum) : 0.0f;
         }
-        sum = group_sum(sum, lanes_log2);
-        if (SIGMOID) soft_sum = group_sum(soft_sum, lanes_log2);
-        else soft_sum = sum;
-        inverse = live ? 1.0f / sum : 0.0f;
-        soft_inverse = live ? 1.0f / soft_sum : 0.0f;
-        lse = live ? base + logf(soft_sum) : 0.0f;
+        lse = live ? base + logf(sum) : 0.0f;
     }
 };
 
-template <typename T, int V, bool SIGMOID>
+template <typename T, int V, int LANES, bool SIGMOID>
 __global__ void __launch_bounds__(LOGIT_THREADS) balance_kernel(BalanceArgs a, LogitShape s) {
-    constexpr int WARPS = LOGIT_THREADS / 32;
+    constexpr int WARPS = LOGIT_THREADS / 32, PER_BLOCK = LOGIT_THREADS / LANES;
     __shared__ int hist[MAX_EXPERTS];
-    __shared__ float sums[WARPS][32 * V];
+    __shared__ float sums[WARPS][LANES * V];
     __shared__ float squares[WARPS];
     __shared__ int alive[WARPS];
-    const int lanes = 1 << s.lanes_log2, lane = threadIdx.x & (lanes - 1), warp = threadIdx.x >> 5;
-    const int per_block = LOGIT_THREADS >> s.lanes_log2;
+    const int lane = threadIdx.x & (LANES - 1), warp = threadIdx.x >> 5;
     for (int e = threadIdx.x; e < s.experts; e += LOGIT_THREADS) hist[e] = 0;
     __syncthreads();
 
@@ -99,29 +97,28 @@ __global__ void __launch_bounds__(LOGIT_THREADS) balance_kernel(BalanceArgs a, L
     int live = 0;
 #pragma unroll
     for (int i = 0; i < V; ++i) sum[i] = 0.0f;
-    for (long long row0 = (long long)blockIdx.x * per_block; row0 < s.rows; row0 += (long long)gridDim.x * per_block) {
-        const long long row = row0 + (threadIdx.x >> s.lanes_log2);
+    for (long long row0 = (long long)blockIdx.x * PER_BLOCK; row0 < s.rows; row0 += (long long)gridDim.x * PER_BLOCK) {
+        const long long row = row0 + threadIdx.x / LANES;
         float v[V];
+        load_logits<T, V, LANES>(static_cast<const T*>(a.logits), s, a.mask, row, row < s.rows, lane, v);
+        const Shares<V, LANES, SIGMOID> share(v);
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = NOTHING;
-        if (row < s.rows) load_logits<T, V>(static_cast<const T*>(a.logits), s, a.mask, row, lane, v);
-        const Shares<V, SIGMOID> share(v, s.lanes_log2);
-#pragma unroll
-        for (int i = 0; i < V; ++i) sum[i] += share.live ? share.p[i] * share.inverse : 0.0f;
+        for (int i = 0; i < V; ++i) sum[i] = fmaf(share.p[i], share.inverse, sum[i]);
         if (lane == 0) {
             square += share.lse * share.lse;
             live += share.live;
         }
     }
-    for (int d = lanes; d < 32; d *= 2) {
+#pragma unroll
+    for (int d = LANES; d < 32; d *= 2) {
 #pragma unroll
         for (int i = 0; i < V; ++i) sum[i] += __shfl_xor_sync(0xffffffffu, sum[i], d);
         square += __shfl_xor_sync(0xffffffffu, square, d);
         live += __shfl_xor_sync(0xffffffffu, live, d);
     }
-    if ((threadIdx.x & 31) < lanes) {
+    if ((threadIdx.x & 31) < LANES) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) sums[warp][(((i / 8) << s.lanes_log2) + lane) * 8 + i % 8] = sum[i];
+        for (int i = 0; i < V; ++i) sums[warp][run_at<LANES>(i / 8, lane) + i % 8] = sum[i];
         if (lane == 0) {
             squares[warp] = square;
             alive[warp] = live;
@@ -254,27 +251,25 @@ struct BalanceBackward {
     void* d_logits;
 };
 
-template <typename T, int V, bool SIGMOID>
+template <typename T, int V, int LANES, bool SIGMOID>
 __global__ void __launch_bounds__(LOGIT_THREADS) balance_backward_kernel(BalanceBackward a, LogitShape s) {
-    const int lanes = 1 << s.lanes_log2, lane = threadIdx.x & (lanes - 1);
-    const long long row = (long long)blockIdx.x * (LOGIT_THREADS >> s.lanes_log2) + (threadIdx.x >> s.lanes_log2);
+    const int lane = threadIdx.x & (LANES - 1);
+    const long long row = (long long)blockIdx.x * (LOGIT_THREADS / LANES) + threadIdx.x / LANES;
     const bool inside = row < s.rows;
     float v[V], f[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = NOTHING;
-    if (inside) load_logits<T, V>(static_cast<const T*>(a.logits), s, a.mask, row, lane, v);
+    load_logits<T, V, LANES>(static_cast<const T*>(a.logits), s, a.mask, row, inside, lane, v);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        const int e = (((i / 8) << s.lanes_log2) + lane) * 8 + i % 8;
+        const int e = run_at<LANES>(i / 8, lane) + i % 8;
         f[i] = e < s.experts ? __ldg(a.stats + e) : 0.0f;
     }
     const float per = __ldg(a.stats + s.experts);
     const float first = a.d_loss ? __ldg(a.d_loss) * float(s.experts) * per : 0.0f, second = a.d_z ? __ldg(a.d_z) * 2.0f * per : 0.0f;
-    const Shares<V, SIGMOID> share(v, s.lanes_log2);
+    const Shares<V, LANES, SIGMOID> share(v);
     float mean = 0.0f;
 #pragma unroll
     for (int i = 0; i < V; ++i) mean += f[i] * share.p[i];
-    mean = group_sum(mean, s.lanes_log2) * share.inverse;
+    mean = group_sum<LANES>(mean) * share.inverse;
     const float scale = first * share.inverse, pull = second * share.lse * share.soft_inverse;
 #pragma unroll
     for (int i = 0; i < V; ++i) {
@@ -283,21 +278,18 @@ __global__ void __launch_bounds__(LOGIT_THREADS) balance_backward_kernel(Balance
         else d += pull * share.p[i];
         v[i] = v[i] == NOTHING || !share.live ? 0.0f : d;
     }
-    if (inside) store_logits<T, V>(static_cast<T*>(a.d_logits), s, row, lane, v);
+    if (inside) store_logits<T, V, LANES>(static_cast<T*>(a.d_logits), s, row, lane, v);
 }
 
 constexpr int SMS = 148;  // of a B200: the sizes of scratch must not depend on the device that asks
 
-int64_t balance_blocks(int64_t rows, int experts) {
-    const LogitShape s = logit_shape(rows, experts, ROW_F32, {}, Mask{});
-    return std::min<int64_t>(logit_blocks(s), SMS * 4);
-}
+int64_t balance_blocks(int64_t rows, int experts) { return std::min<int64_t>(logit_blocks(rows, experts), SMS * 4); }
 
 template <typename F>
 void with_balance(int dtype, int experts, int score, F&& f) {
-    with_logits(dtype, experts, [&](auto type, auto v) {
-        if (score == SCORE_SIGMOID) f(type, v, std::true_type{});
-        else f(type, v, std::false_type{});
+    with_logits(dtype, experts, [&](auto type, auto v, auto lanes) {
+        if (score == SCORE_SIGMOID) f(type, v, lanes, std::true_type{});
+        else f(type, v, lanes, std::false_type{});
     });
 }
 
@@ -337,8 +329,8 @@ extern "C" int odie_balance(const void* logits, int64_t rows, int experts, int d
         a.live = reinterpret_cast<int*>(a.squares + blocks);
         if (blocks) {
             const LogitShape s = logit_shape(rows, experts, dtype, {logits}, a.mask);
-            with_balance(dtype, experts, score, [&](auto type, auto v, auto sigmoid) {
-                balance_kernel<decltype(type), decltype(v)::value, decltype(sigmoid)::value><<<unsigned(blocks), LOGIT_THREADS, 0, stream>>>(a, s);
+            with_balance(dtype, experts, score, [&](auto type, auto v, auto lanes, auto sigmoid) {
+                balance_kernel<decltype(type), decltype(v)::value, decltype(lanes)::value, decltype(sigmoid)::value><<<unsigned(blocks), LOGIT_THREADS, 0, stream>>>(a, s);
             });
             ODIE_CUDA(cudaGetLastError());
             note_launch();
@@ -359,9 +351,9 @@ extern "C" int odie_balance_backward(const float* d_loss, const float* d_z, cons
         ODIE_REQUIRE(logits && stats && d_logits, "logits, stats and d_logits are required");
         const BalanceBackward a{logits, {mask, mask_row_step, mask_expert_step}, stats, d_loss, d_z, d_logits};
         const LogitShape s = logit_shape(rows, experts, dtype, {logits, d_logits}, a.mask);
-        with_balance(dtype, experts, score, [&](auto type, auto v, auto sigmoid) {
-            balance_backward_kernel<decltype(type), decltype(v)::value, decltype(sigmoid)::value>
-                <<<unsigned(logit_blocks(s)), LOGIT_THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a, s);
+        with_balance(dtype, experts, score, [&](auto type, auto v, auto lanes, auto sigmoid) {
+            balance_backward_kernel<decltype(type), decltype(v)::value, decltype(lanes)::value, decltype(sigmoid)::value>
+                <<<unsigned(logit_blocks(rows, experts)), LOGIT_THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a, s);
         });
         ODIE_CUDA(cudaGetLastError());
         note_launch();

@@ -7,8 +7,7 @@
 //
 // The key has no transcendental function in it, so that which experts a row takes does not depend on how one is
 // rounded; the bias shifts choices and not weights, and has no gradient.  A softmax over the chosen logits is the
-// normalised softmax over all, so that nothing but the chosen is read for it; normalised sigmoids are taken by their
-// logarithms, which do not underflow.
+// normalised softmax over all, so that nothing but the chosen is read for it.
 //
 //   backward, with g = d weight, p = s (normalised: divided by the sum):
 //     softmax, normalised   d l_j = w_j (g_j - sum w g / scale)              at the chosen, 0 elsewhere
@@ -47,86 +46,161 @@ struct GateArgs {
     void* d_logits;
 };
 
-// The order of keys as unsigned numbers: 0 for what is not there, a NaN above all; -0 and 0 are one key.
+// The order of keys as unsigned numbers: a NaN (which an addition makes positive) above all, -0 and 0 one key.
 __device__ __forceinline__ uint32_t ordered(float v) {
     const uint32_t bits = __float_as_uint(v + 0.0f);
-    const uint32_t key = bits ^ (bits >> 31 ? 0xffffffffu : 0x80000000u);
-    return v != v ? 0xffffffffu : v == NOTHING ? 0u : key;
+    return bits ^ (uint32_t(int(bits) >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float unordered(uint32_t key) { return __uint_as_float(key >> 31 ? key ^ 0x80000000u : ~key); }
+constexpr uint32_t NO_KEY = 0x007fffffu;  // -inf, and what was taken (0)
+
+template <int LANES>
+__device__ __forceinline__ uint32_t group_highest(uint32_t v) {
+    if constexpr (LANES == 32) {
+        return __reduce_max_sync(0xffffffffu, v);
+    } else {
+#pragma unroll
+        for (int d = 1; d < LANES; d *= 2) v = max(v, __shfl_xor_sync(0xffffffffu, v, d));
+        return v;
+    }
+}
+template <int LANES>
+__device__ __forceinline__ int group_lowest(int v) {
+    if constexpr (LANES == 32) {
+        return __reduce_min_sync(0xffffffffu, v);
+    } else {
+#pragma unroll
+        for (int d = 1; d < LANES; d *= 2) v = min(v, __shfl_xor_sync(0xffffffffu, v, d));
+        return v;
+    }
 }
 
-template <typename T, int V>
-__global__ void __launch_bounds__(LOGIT_THREADS) gate_kernel(GateArgs a, LogitShape s) {
-    // Choice j is kept by lane j % lanes, in slot j / lanes: lanes x 8 cover the experts, so 8 slots cover the choices.
-    constexpr int SLOTS = 8;
-    const int lanes = 1 << s.lanes_log2, lane = threadIdx.x & (lanes - 1);
-    const long long row = (long long)blockIdx.x * (LOGIT_THREADS >> s.lanes_log2) + (threadIdx.x >> s.lanes_log2);
-    const bool inside = row < s.rows;
-    const T* logits = static_cast<const T*>(a.logits);
-    float v[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = NOTHING;
-    if (inside) load_logits<T, V>(logits, s, a.mask, row, lane, v);
-
-    uint32_t key[V];
-#pragma unroll
-    for (int c = 0; c < V / 8; ++c)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int e = ((c << s.lanes_log2) + lane) * 8 + i;
-            const float z = v[c * 8 + i];
-            key[c * 8 + i] = ordered(a.bias && e < s.experts && z != NOTHING ? z + __ldg(a.bias + e) : z);
-        }
-    int chosen[SLOTS];
-#pragma unroll
-    for (int q = 0; q < SLOTS; ++q) chosen[q] = -1;
+// The choices one after another: the highest key, the lowest expert that has it, which is taken out.  Choice j goes to lane
+// j % LANES, slot j / LANES.
+template <int V, int LANES, int SLOTS>
+__device__ __forceinline__ void choose(uint32_t (&key)[V], int choices, int lane, int (&chosen)[SLOTS], uint32_t& most) {
 #pragma unroll
     for (int q = 0; q < SLOTS; ++q) {
-        for (int t = 0; t < lanes && q * lanes + t < a.choices; ++t) {
-            uint32_t best = 0;
+        chosen[q] = -1;
+#pragma unroll 1
+        for (int t = 0; t < LANES && q * LANES + t < choices; ++t) {
+            uint32_t best = key[0];
 #pragma unroll
-            for (int i = 0; i < V; ++i) best = max(best, key[i]);
-            for (int d = 1; d < lanes; d *= 2) best = max(best, __shfl_xor_sync(0xffffffffu, best, d));
+            for (int i = 1; i < V; ++i) best = max(best, key[i]);
+            best = group_highest<LANES>(best);
+            if (q == 0 && t == 0) most = best;
             int at = MAX_EXPERTS;
 #pragma unroll
             for (int i = V - 1; i >= 0; --i)
-                if (key[i] == best) at = (((i / 8) << s.lanes_log2) + lane) * 8 + i % 8;
-            for (int d = 1; d < lanes; d *= 2) at = min(at, __shfl_xor_sync(0xffffffffu, at, d));
+                if (key[i] == best) at = run_at<LANES>(i / 8, lane) + i % 8;
+            at = group_lowest<LANES>(at);
+            if (t == lane && best > NO_KEY) chosen[q] = at;
+            if (q * LANES + t + 1 < choices) {
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                if ((((i / 8) << s.lanes_log2) + lane) * 8 + i % 8 == at) key[i] = 0;
-            if (t == lane && best) chosen[q] = at;
+                for (int i = 0; i < V; ++i)
+                    if (run_at<LANES>(i / 8, lane) + i % 8 == at) key[i] = 0;
+            }
         }
+    }
+}
+
+// The same for a warp to a row and 8 keys to a lane, for several choices: each lane sorts its keys first, so that a choice is
+// the highest of the lanes' first ones and the lane that had it moves up.  (65536 rows of 256 bf16, 8 choices: MEASURED.)
+// `at` is where a key was in its lane; the lower lane has the lower experts.
+__device__ __forceinline__ void exchange(uint32_t& a, uint32_t& b, int& at_a, int& at_b) {
+    const bool turn = b > a || (b == a && at_b < at_a);
+    const uint32_t high = turn ? b : a, low = turn ? a : b;
+    const int at_high = turn ? at_b : at_a, at_low = turn ? at_a : at_b;
+    a = high;
+    b = low;
+    at_a = at_high;
+    at_b = at_low;
+}
+template <int SLOTS>
+__device__ __forceinline__ void choose_sorted(uint32_t (&key)[8], int choices, int lane, int (&chosen)[SLOTS], uint32_t& most) {
+    int at[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) at[i] = i;
+    // Batcher's odd-even merge sort of eight
+    constexpr int PAIRS[19][2] = {{0, 1}, {2, 3}, {4, 5}, {6, 7}, {0, 2}, {1, 3}, {4, 6}, {5, 7}, {1, 2}, {5, 6},
+                                  {0, 4}, {1, 5}, {2, 6}, {3, 7}, {2, 4}, {3, 5}, {1, 2}, {3, 4}, {5, 6}};
+#pragma unroll
+    for (int i = 0; i < 19; ++i) exchange(key[PAIRS[i][0]], key[PAIRS[i][1]], at[PAIRS[i][0]], at[PAIRS[i][1]]);
+#pragma unroll
+    for (int q = 0; q < SLOTS; ++q) {
+        chosen[q] = -1;
+#pragma unroll 1
+        for (int t = 0; t < 32 && q * 32 + t < choices; ++t) {
+            const uint32_t best = __reduce_max_sync(0xffffffffu, key[0]);
+            if (q == 0 && t == 0) most = best;
+            const int winner = __ffs(__ballot_sync(0xffffffffu, key[0] == best)) - 1;
+            const int e = winner * 8 + __shfl_sync(0xffffffffu, at[0], winner);
+            if (t == lane && best > NO_KEY) chosen[q] = e;
+            if (lane == winner) {
+#pragma unroll
+                for (int i = 0; i < 7; ++i) {
+                    key[i] = key[i + 1];
+                    at[i] = at[i + 1];
+                }
+                key[7] = 0;
+            }
+        }
+    }
+}
+
+// As few slots as hold the choices are compiled for: LANES x 8 cover up to 256 experts, so 8 do always.
+template <typename T, int V, int LANES, int SLOTS>
+__global__ void __launch_bounds__(LOGIT_THREADS) gate_kernel(GateArgs a, LogitShape s) {
+    const int lane = threadIdx.x & (LANES - 1);
+    const long long row = (long long)blockIdx.x * (LOGIT_THREADS / LANES) + threadIdx.x / LANES;
+    const bool inside = row < s.rows;
+    const T* logits = static_cast<const T*>(a.logits);
+    float v[V];
+    load_logits<T, V, LANES>(logits, s, a.mask, row, inside, lane, v);
+
+    uint32_t key[V], most = 0;  // most: the highest key of all
+    if (a.bias) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int e = run_at<LANES>(i / 8, lane) + i % 8;
+            key[i] = ordered(e < s.experts && v[i] != NOTHING ? v[i] + __ldg(a.bias + e) : v[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) key[i] = ordered(v[i]);
+    }
+    int chosen[SLOTS];
+    if constexpr (LANES == 32 && V == 8) {
+        if (a.choices > 3) choose_sorted<SLOTS>(key, a.choices, lane, chosen, most);
+        else choose<V, LANES, SLOTS>(key, a.choices, lane, chosen, most);
+    } else {
+        choose<V, LANES, SLOTS>(key, a.choices, lane, chosen, most);
     }
 
     float l[SLOTS], w[SLOTS];
 #pragma unroll
     for (int q = 0; q < SLOTS; ++q) l[q] = chosen[q] >= 0 ? to_float(logits[row * s.experts + chosen[q]]) : NOTHING;
-    if (a.score == SCORE_SOFTMAX || a.normalize) {
-        // a softmax of the chosen logits, or of the logarithms of their sigmoids; without normalize of all logits
-        if (a.score == SCORE_SIGMOID) {
-#pragma unroll
-            for (int q = 0; q < SLOTS; ++q) l[q] = chosen[q] >= 0 ? log_sigmoid(l[q]) : NOTHING;
-        }
-        float top = NOTHING, sum = 0.0f;
-        if (a.normalize) {
-#pragma unroll
-            for (int q = 0; q < SLOTS; ++q) top = l[q] > top || l[q] != l[q] ? l[q] : top;
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) top = v[i] > top || v[i] != v[i] ? v[i] : top;
-        }
-        top = group_max(top, s.lanes_log2);
+    if (a.score == SCORE_SOFTMAX || a.normalize) {  // e^(l - top), or sigmoids over e^top, over their sum (without normalize: of all)
+        float top, sum = 0.0f;
+        if (a.normalize) top = group_max<LANES>(largest(l));
+        else if (!a.bias) top = unordered(most);
+        else top = group_max<LANES>(largest(v));
         if (top == NOTHING) top = 0.0f;
+        if (a.score == SCORE_SIGMOID) top = fminf(top, 0.0f);
+#pragma unroll
+        for (int q = 0; q < SLOTS; ++q) {
+            w[q] = a.score == SCORE_SIGMOID ? sigmoid_over(l[q], top) : power(l[q], top);
+            if (chosen[q] < 0) w[q] = 0.0f;
+        }
         if (a.normalize) {
 #pragma unroll
-            for (int q = 0; q < SLOTS; ++q) sum += chosen[q] >= 0 ? expf(l[q] - top) : 0.0f;
+            for (int q = 0; q < SLOTS; ++q) sum += w[q];
         } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) sum += expf(v[i] - top);
+            sum = powers(v, top);
         }
-        sum = group_sum(sum, s.lanes_log2);
+        const float scale = a.scale * inverse_approx(group_sum<LANES>(sum));
 #pragma unroll
-        for (int q = 0; q < SLOTS; ++q) w[q] = a.scale * (expf(l[q] - top) / sum);
+        for (int q = 0; q < SLOTS; ++q) w[q] *= scale;
     } else {
 #pragma unroll
         for (int q = 0; q < SLOTS; ++q) w[q] = a.scale * sigmoid_of(l[q]);
@@ -134,18 +208,19 @@ __global__ void __launch_bounds__(LOGIT_THREADS) gate_kernel(GateArgs a, LogitSh
     if (!inside) return;
 #pragma unroll
     for (int q = 0; q < SLOTS; ++q) {
-        const int j = q * lanes + lane;
+        const int j = q * LANES + lane;
         if (j >= a.choices) break;
         a.expert[row * a.choices + j] = chosen[q];
         a.weights[row * a.choices + j] = chosen[q] >= 0 ? w[q] : 0.0f;
     }
 }
 
-template <typename T, int V>
+template <typename T, int V, int LANES, int SLOTS>
 __global__ void __launch_bounds__(LOGIT_THREADS) gate_backward_kernel(GateArgs a, LogitShape s) {
-    constexpr int SLOTS = 8;
-    const int lanes = 1 << s.lanes_log2, lane = threadIdx.x & (lanes - 1);
-    const long long row = (long long)blockIdx.x * (LOGIT_THREADS >> s.lanes_log2) + (threadIdx.x >> s.lanes_log2);
+    // where the lanes that have a choice find the lane that has its expert
+    __shared__ alignas(16) float rows[LOGIT_THREADS / LANES][LANES * V];
+    const int lane = threadIdx.x & (LANES - 1);
+    const long long row = (long long)blockIdx.x * (LOGIT_THREADS / LANES) + threadIdx.x / LANES;
     const bool inside = row < s.rows;
     const T* logits = static_cast<const T*>(a.logits);
     const bool dense = a.score == SCORE_SOFTMAX && !a.normalize;
@@ -155,7 +230,7 @@ __global__ void __launch_bounds__(LOGIT_THREADS) gate_backward_kernel(GateArgs a
     float w[SLOTS], d[SLOTS], sum = 0.0f;
 #pragma unroll
     for (int q = 0; q < SLOTS; ++q) {
-        const int j = q * lanes + lane;
+        const int j = q * LANES + lane;
         chosen[q] = -1;
         w[q] = d[q] = 0.0f;
         if (!inside || j >= a.choices) continue;
@@ -167,49 +242,51 @@ __global__ void __launch_bounds__(LOGIT_THREADS) gate_backward_kernel(GateArgs a
         d[q] = a.d_weights[at];
         sum += w[q] * d[q];
     }
-    sum = group_sum(sum, s.lanes_log2);
-    const float mean = a.normalize || dense ? sum / a.scale : 0.0f;
+    float* mine = rows[threadIdx.x / LANES];
+#pragma unroll
+    for (int c = 0; c < V / 4; ++c) *reinterpret_cast<float4*>(mine + run_at<LANES>(c / 2, lane) + c % 2 * 4) = make_float4(0, 0, 0, 0);
+    if (a.normalize || dense) sum = group_sum<LANES>(sum);
+    const float mean = a.normalize ? sum * (1.0f / a.scale) : 0.0f;
+    __syncwarp();
 #pragma unroll
     for (int q = 0; q < SLOTS; ++q) {
         if (chosen[q] < 0) continue;
-        d[q] = w[q] * (dense ? d[q] : d[q] - mean);
+        d[q] = w[q] * (d[q] - mean);
         if (a.score == SCORE_SIGMOID) d[q] *= sigmoid_of(-to_float(logits[row * s.experts + chosen[q]]));
+        mine[chosen[q]] = d[q];
     }
 
     float v[V];
     if (dense) {  // - scale p_e sum p g
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = NOTHING;
-        if (inside) load_logits<T, V>(logits, s, a.mask, row, lane, v);
-        float top = NOTHING, total = 0.0f;
-#pragma unroll
-        for (int i = 0; i < V; ++i) top = v[i] > top || v[i] != v[i] ? v[i] : top;
-        top = group_max(top, s.lanes_log2);
+        load_logits<T, V, LANES>(logits, s, a.mask, row, inside, lane, v);
+        float top = group_max<LANES>(largest(v));
         if (top == NOTHING) top = 0.0f;
+        const float total = group_sum<LANES>(powers(v, top)), share = total > 0.0f || total != total ? -sum * inverse_approx(total) : 0.0f;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            v[i] = expf(v[i] - top);
-            total += v[i];
-        }
-        total = group_sum(total, s.lanes_log2);
-        const float share = total > 0.0f || total != total ? sum / total : 0.0f;
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] *= -share;
+        for (int i = 0; i < V; ++i) v[i] *= share;
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = 0.0f;
     }
+    __syncwarp();
 #pragma unroll
-    for (int q = 0; q < SLOTS; ++q) {
-        for (int t = 0; t < lanes && q * lanes + t < a.choices; ++t) {
-            const int e = __shfl_sync(0xffffffffu, chosen[q], t, lanes);
-            const float add = __shfl_sync(0xffffffffu, d[q], t, lanes);
-#pragma unroll
-            for (int i = 0; i < V; ++i)
-                if ((((i / 8) << s.lanes_log2) + lane) * 8 + i % 8 == e) v[i] += add;
-        }
+    for (int c = 0; c < V / 4; ++c) {
+        const float4 add = *reinterpret_cast<const float4*>(mine + run_at<LANES>(c / 2, lane) + c % 2 * 4);
+        v[c * 4] += add.x;
+        v[c * 4 + 1] += add.y;
+        v[c * 4 + 2] += add.z;
+        v[c * 4 + 3] += add.w;
     }
-    if (inside) store_logits<T, V>(static_cast<T*>(a.d_logits), s, row, lane, v);
+    if (inside) store_logits<T, V, LANES>(static_cast<T*>(a.d_logits), s, row, lane, v);
+}
+
+template <typename F>
+void with_gate(int dtype, int experts, int choices, F&& f) {
+    with_logits(dtype, experts, [&](auto type, auto v, auto lanes) {
+        constexpr int LANES = decltype(lanes)::value;
+        if (choices <= LANES) f(type, v, lanes, std::integral_constant<int, 1>{});
+        else f(type, v, lanes, std::integral_constant<int, LANES == 32 ? 2 : LANES == 16 ? 4 : 8>{});
+    });
 }
 
 void check_gate(int64_t rows, int experts, int choices, int dtype, int score, float scale) {
@@ -242,9 +319,9 @@ extern "C" int odie_gate(const void* logits, int64_t rows, int experts, int dtyp
         a.expert = expert;
         a.weights = weights;
         const LogitShape s = logit_shape(rows, experts, dtype, {logits}, a.mask);
-        with_logits(dtype, experts, [&](auto type, auto v) {
-            gate_kernel<decltype(type), decltype(v)::value>
-                <<<unsigned(logit_blocks(s)), LOGIT_THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a, s);
+        with_gate(dtype, experts, choices, [&](auto type, auto v, auto lanes, auto slots) {
+            gate_kernel<decltype(type), decltype(v)::value, decltype(lanes)::value, decltype(slots)::value>
+                <<<unsigned(logit_blocks(rows, experts)), LOGIT_THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a, s);
         });
         ODIE_CUDA(cudaGetLastError());
         note_launch();
@@ -271,9 +348,9 @@ extern "C" int odie_gate_backward(const float* d_weights, const void* logits, in
         a.d_weights = d_weights;
         a.d_logits = d_logits;
         const LogitShape s = logit_shape(rows, experts, dtype, {logits, d_logits}, a.mask);
-        with_logits(dtype, experts, [&](auto type, auto v) {
-            gate_backward_kernel<decltype(type), decltype(v)::value>
-                <<<unsigned(logit_blocks(s)), LOGIT_THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a, s);
+        with_gate(dtype, experts, choices, [&](auto type, auto v, auto lanes, auto slots) {
+            gate_backward_kernel<decltype(type), decltype(v)::value, decltype(lanes)::value, decltype(slots)::value>
+                <<<unsigned(logit_blocks(rows, experts)), LOGIT_THREADS, 0, reinterpret_cast<cudaStream_t>(stream)>>>(a, s);
         });
         ODIE_CUDA(cudaGetLastError());
         note_launch();

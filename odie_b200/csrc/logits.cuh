@@ -1,6 +1,6 @@
 // Rows of a router's logits, held by groups of lanes (gate.cu, balance.cu).
 #pragma once
-#include "rows.cuh"
+#include "activation.cuh"
 #include <initializer_list>
 #include <type_traits>
 
@@ -17,74 +17,95 @@ struct Mask {
     long long row_step, expert_step;
 };
 
-// A row of E logits among 2^lanes_log2 lanes of a warp, V per lane in runs of 8: lane l has experts
-// (c * lanes + l) * 8 + i, c < V / 8, i < 8.  So neighbouring lanes read neighbouring 16 bytes, and up to 8 experts are
-// one thread's.
+// A row of E logits among LANES lanes of a warp, V per lane in runs of 8: lane l has experts (c * LANES + l) * 8 + i,
+// c < V / 8, i < 8.  So neighbouring lanes read neighbouring 16 bytes, and up to 8 experts are one thread's.  V is 8 but for
+// more than 256 experts.
 struct LogitShape {
     long long rows;
     int experts;
-    int lanes_log2;
     int wide;       // every row starts on a 16-byte boundary
     int mask_wide;  // every row of the mask on an 8-byte one, its experts side by side
 };
 inline LogitShape logit_shape(int64_t rows, int experts, int dtype, std::initializer_list<const void*> pointers, const Mask& mask) {
-    LogitShape s{rows, experts, 0, 0, 0};
-    while (s.lanes_log2 < 5 && (8 << s.lanes_log2) < experts) ++s.lanes_log2;
+    LogitShape s{rows, experts, 0, 0};
     uintptr_t bits = uintptr_t(experts) * row_type_size(dtype);
     for (const void* p : pointers) bits |= uintptr_t(p);
     s.wide = bits % 16 == 0 && experts % 8 == 0;
     s.mask_wide = mask.at && mask.expert_step == 1 && (uintptr_t(mask.at) | uintptr_t(mask.row_step) | uintptr_t(experts)) % 8 == 0;
     return s;
 }
-inline int64_t logit_blocks(const LogitShape& s) { return (s.rows + (LOGIT_THREADS >> s.lanes_log2) - 1) / (LOGIT_THREADS >> s.lanes_log2); }
+inline int logit_lanes(int experts) {
+    int lanes = 1;
+    while (lanes < 32 && lanes * 8 < experts) lanes *= 2;
+    return lanes;
+}
+inline int64_t logit_blocks(int64_t rows, int experts) {
+    const int per_block = LOGIT_THREADS / logit_lanes(experts);
+    return (rows + per_block - 1) / per_block;
+}
 
-// Calls f(T{}, std::integral_constant<int, V>{}) for the type and values per lane at run time.
+// Calls f(T{}, integral_constant<int, V>{}, integral_constant<int, LANES>{}) for the type and number of experts.
 template <typename F>
 void with_logits(int dtype, int experts, F&& f) {
-    auto typed = [&](auto v) {
-        if (dtype == ROW_F32) f(float{}, v);
-        else if (dtype == ROW_BF16) f(__nv_bfloat16{}, v);
-        else f(__half{}, v);
+    auto typed = [&](auto v, auto lanes) {
+        if (dtype == ROW_F32) f(float{}, v, lanes);
+        else if (dtype == ROW_BF16) f(__nv_bfloat16{}, v, lanes);
+        else f(__half{}, v, lanes);
     };
-    if (experts <= 256) typed(std::integral_constant<int, 8>{});
-    else if (experts <= 512) typed(std::integral_constant<int, 16>{});
-    else typed(std::integral_constant<int, 32>{});
+    using std::integral_constant;
+    const integral_constant<int, 8> eight{};
+    if (experts <= 8) typed(eight, integral_constant<int, 1>{});
+    else if (experts <= 16) typed(eight, integral_constant<int, 2>{});
+    else if (experts <= 32) typed(eight, integral_constant<int, 4>{});
+    else if (experts <= 64) typed(eight, integral_constant<int, 8>{});
+    else if (experts <= 128) typed(eight, integral_constant<int, 16>{});
+    else if (experts <= 256) typed(eight, integral_constant<int, 32>{});
+    else if (experts <= 512) typed(integral_constant<int, 16>{}, integral_constant<int, 32>{});
+    else typed(integral_constant<int, 32>{}, integral_constant<int, 32>{});
 }
 
 constexpr float NOTHING = -INFINITY;
 
-// The lane's logits of a row; NOTHING where the mask is off or no expert is.
-template <typename T, int V>
-__device__ __forceinline__ void load_logits(const T* logits, const LogitShape& s, const Mask& mask, long long row, int lane, float (&v)[V]) {
+// The first expert of a lane's c-th run.
+template <int LANES>
+__device__ __forceinline__ int run_at(int c, int lane) { return (c * LANES + lane) * 8; }
+
+// The lane's logits of a row; NOTHING where the mask is off or no expert is, and everywhere for a row that is not (`inside`).
+template <typename T, int V, int LANES>
+__device__ __forceinline__ void load_logits(const T* logits, const LogitShape& s, const Mask& mask, long long row, bool inside, int lane,
+                                            float (&v)[V]) {
     constexpr int PER = 16 / int(sizeof(T));
     const T* at = logits + row * s.experts;
 #pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = NOTHING;
+#pragma unroll
     for (int c = 0; c < V / 8; ++c) {
-        const int e0 = ((c << s.lanes_log2) + lane) * 8;
+        const int e0 = run_at<LANES>(c, lane);
+        if (!inside || e0 >= s.experts) continue;
         if (s.wide) {
 #pragma unroll
             for (int p = 0; p < 8 / PER; ++p) {
-                Pack<T, 16> x;
-                if (e0 < s.experts) x = Pack<T, 16>::load(at + e0 + p * PER);
+                const auto x = Pack<T, 16>::load(at + e0 + p * PER);
 #pragma unroll
-                for (int i = 0; i < PER; ++i) v[c * 8 + p * PER + i] = e0 < s.experts ? to_float(x.v[i]) : NOTHING;
+                for (int i = 0; i < PER; ++i) v[c * 8 + p * PER + i] = to_float(x.v[i]);
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[c * 8 + i] = e0 + i < s.experts ? to_float(at[e0 + i]) : NOTHING;
+            for (int i = 0; i < 8; ++i)
+                if (e0 + i < s.experts) v[c * 8 + i] = to_float(at[e0 + i]);
         }
         if (!mask.at) continue;
         const uint8_t* m = mask.at + row * mask.row_step;
         if (s.mask_wide) {
-            if (e0 >= s.experts) continue;
             const uint2 bytes = __ldg(reinterpret_cast<const uint2*>(m + e0));
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (((i < 4 ? bytes.x : bytes.y) >> (i % 4 * 8) & 0xff) == 0) v[c * 8 + i] = NOTHING;
         } else if (mask.expert_step == 0) {
-            if (*m == 0)
+            if (*m == 0) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) v[c * 8 + i] = NOTHING;
+            }
         } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -93,20 +114,25 @@ __device__ __forceinline__ void load_logits(const T* logits, const LogitShape& s
     }
 }
 
-template <typename T, int V>
+template <typename T, int V, int LANES>
 __device__ __forceinline__ void store_logits(T* to, const LogitShape& s, long long row, int lane, const float (&v)[V]) {
     constexpr int PER = 16 / int(sizeof(T));
     T* at = to + row * s.experts;
 #pragma unroll
     for (int c = 0; c < V / 8; ++c) {
-        const int e0 = ((c << s.lanes_log2) + lane) * 8;
+        const int e0 = run_at<LANES>(c, lane);
+        if (e0 >= s.experts) continue;
         if (s.wide) {
-            if (e0 >= s.experts) continue;
 #pragma unroll
             for (int p = 0; p < 8 / PER; ++p) {
                 Pack<T, 16> x;
+                if constexpr (sizeof(T) == 4) {
 #pragma unroll
-                for (int i = 0; i < PER; ++i) x.v[i] = from_float<T>(v[c * 8 + p * PER + i]);
+                    for (int i = 0; i < PER; ++i) x.v[i] = v[c * 8 + p * PER + i];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) reinterpret_cast<uint32_t*>(x.v)[i] = pack_pair<T>(v[c * 8 + 2 * i], v[c * 8 + 2 * i + 1]);
+                }
                 x.store(at + e0 + p * PER);
             }
         } else {
@@ -118,24 +144,55 @@ __device__ __forceinline__ void store_logits(T* to, const LogitShape& s, long lo
 }
 
 // Over the lanes of a row (all lanes of the warp take part).
-__device__ __forceinline__ float group_sum(float v, int lanes_log2) {
-    for (int d = 1; d < 1 << lanes_log2; d *= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
+template <int LANES>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+    for (int d = 1; d < LANES; d *= 2) v += __shfl_xor_sync(0xffffffffu, v, d);
     return v;
 }
-__device__ __forceinline__ float group_max(float v, int lanes_log2) {  // a NaN stays
-    for (int d = 1; d < 1 << lanes_log2; d *= 2) {
-        const float other = __shfl_xor_sync(0xffffffffu, v, d);
-        v = other > v || other != other ? other : v;
-    }
+template <int LANES>
+__device__ __forceinline__ float group_max(float v) {  // a NaN stays
+#pragma unroll
+    for (int d = 1; d < LANES; d *= 2) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, d));
     return v;
+}
+template <int V>
+__device__ __forceinline__ float largest(const float (&v)[V]) {
+    float top = v[0];
+#pragma unroll
+    for (int i = 1; i < V; ++i) top = max_nan(top, v[i]);
+    return top;
 }
 
-// e^-|v|, from which both sigmoid(v) and sigmoid(-v) come without cancellation.
-__device__ __forceinline__ float sigmoid_of(float v) {
-    const float e = expf(-fabsf(v));
-    return (v >= 0.0f ? 1.0f : e) / (1.0f + e);  // (NaN: e is)
+constexpr float LOG2E = 1.4426950408889634f;
+// e^(v - top), within 2^-22 of it and the rounding of its exponent.  (The difference first: a multiple of the lowest number
+// is -inf.)
+__device__ __forceinline__ float power(float v, float top) { return exp2_approx((v - top) * LOG2E); }
+// In place, with the sum.
+template <int V>
+__device__ __forceinline__ float powers(float (&v)[V], float top) {
+    Pair sum = same(0.0f);
+#pragma unroll
+    for (int i = 0; i < V; i += 2) {
+        const float2 x = both(mul2(add2(pair(v[i], v[i + 1]), same(-top)), same(LOG2E)));
+        v[i] = exp2_approx(x.x);
+        v[i + 1] = exp2_approx(x.y);
+        sum = add2(sum, pair(v[i], v[i + 1]));
+    }
+    const float2 s = both(sum);
+    return s.x + s.y;
 }
-__device__ __forceinline__ float log_sigmoid(float v) { return fminf(v, 0.0f) - log1pf(expf(-fabsf(v))) + (v != v ? v : 0.0f); }
+
+// sigmoid(v) from e^-|v|, which both sigmoid(v) and sigmoid(-v) come from without cancellation.
+__device__ __forceinline__ float sigmoid_of(float v) {
+    const float e = exp2_approx(-fabsf(v) * LOG2E);
+    return (v >= 0.0f ? 1.0f : e) * inverse_approx(1.0f + e);  // (NaN: e is)
+}
+// sigmoid(v) / e^low, low <= 0 the least of 0 and the row's largest logit: not all of a row's underflow.
+__device__ __forceinline__ float sigmoid_over(float v, float low) {
+    const float r = power(fminf(v, 0.0f), low) * inverse_approx(1.0f + exp2_approx(-fabsf(v) * LOG2E));
+    return v != v ? v : r;
+}
 
 void check_logits(int64_t rows, int experts, int dtype, int score);
 

@@ -2,11 +2,15 @@
 
 Choices, counts, codes and scales have to be equal.  A softmax's exponentials are off by their arguments' rounding,
 2^-24 of at most `depth` (the distance between a row's logits), and by the function's own 2^-22; a sum of n positive terms
-by n 2^-24 of it.
+by n 2^-24 of it.  The instruction for the exponential gives 0 below the least normal number, 2^-126 (TINY): what it is
+multiplied by is off by as much.
 """
 import torch
 
 from rows_cases import SUM, rounding  # noqa: F401
+
+
+TINY = 2.0 ** -126
 
 
 def masked(logits, mask):
@@ -50,9 +54,9 @@ def plain_gate(logits, choices, bias, mask, score, normalize, scale, d_weights):
         d, most = p * torch.sigmoid(-x) * g, p * torch.sigmoid(-x) * g.abs()
     d, most = scale * torch.where(torch.isneginf(x), 0.0, d), abs(scale) * torch.where(torch.isneginf(x), 0.0, most)
     weights = scale * torch.where(live, own.gather(1, order[:, :choices]), 0.0)
-    d_bound = most * (4 * error + (choices + 8) * SUM)
-    return (expert, (weights, weights.abs() * error + 2.0 ** -140),
-            (d, d_bound + rounding(d.abs() + d_bound, logits.dtype) + 2.0 ** -140))
+    d_bound = most * (4 * error + (choices + 8) * SUM) + abs(scale) * (g.abs() + size) * TINY
+    return (expert, (weights, weights.abs() * error + abs(scale) * TINY),
+            (d, d_bound + rounding(d.abs() + d_bound, logits.dtype) + TINY))
 
 
 def plain_balance(logits, expert, mask, score, total, d_loss, d_z):
@@ -85,7 +89,8 @@ def plain_balance(logits, expert, mask, score, total, d_loss, d_z):
     a, b = d_loss * experts * per * p * slope, d_z * 2 * per * lse[:, None] * soft
     d = a * (f - inner) + b
     bound = a.abs() * (f + inner) * (6 * error + (experts + 16) * SUM) + b.abs() * (6 * error + 16 * SUM) + abs(d_z) * 2 * per * soft * off[:, None]
-    return answer, counts, (d, bound + rounding(d.abs() + bound, logits.dtype) + 2.0 ** -140)
+    bound = bound + (abs(d_loss) * experts * (f + inner) + abs(d_z) * 2 * lse.abs()[:, None] + 1) * TINY
+    return answer, counts, (d, bound + rounding(d.abs() + bound, logits.dtype))
 
 
 CODES = [0, 0.5, 1, 1.5, 2, 3, 4, 6]
