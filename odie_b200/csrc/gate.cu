@@ -34,6 +34,7 @@ constexpr int MAX_CHOICES = 64;
 struct GateArgs {
     const void* logits;
     const float* bias;  // null: none
+    int bias_wide;      // on a 16-byte boundary
     Mask mask;
     int choices;
     int score;
@@ -78,10 +79,11 @@ __device__ __forceinline__ int group_lowest(int v) {
 // The choices one after another: the highest key, the lowest expert that has it, which is taken out.  Choice j goes to lane
 // j % LANES, slot j / LANES.
 template <int V, int LANES, int SLOTS>
-__device__ __forceinline__ void choose(uint32_t (&key)[V], int choices, int lane, int (&chosen)[SLOTS], uint32_t& most) {
+__device__ __forceinline__ void choose(uint32_t (&key)[V], int choices, int lane, int (&chosen)[SLOTS], uint32_t (&won)[SLOTS], uint32_t& most) {
 #pragma unroll
     for (int q = 0; q < SLOTS; ++q) {
         chosen[q] = -1;
+        won[q] = NO_KEY;
 #pragma unroll 1
         for (int t = 0; t < LANES && q * LANES + t < choices; ++t) {
             uint32_t best = key[0];
@@ -94,7 +96,10 @@ __device__ __forceinline__ void choose(uint32_t (&key)[V], int choices, int lane
             for (int i = V - 1; i >= 0; --i)
                 if (key[i] == best) at = run_at<LANES>(i / 8, lane) + i % 8;
             at = group_lowest<LANES>(at);
-            if (t == lane && best > NO_KEY) chosen[q] = at;
+            if (t == lane && best > NO_KEY) {
+                chosen[q] = at;
+                won[q] = best;
+            }
             if (q * LANES + t + 1 < choices) {
 #pragma unroll
                 for (int i = 0; i < V; ++i)
@@ -117,7 +122,7 @@ __device__ __forceinline__ void exchange(uint32_t& a, uint32_t& b, int& at_a, in
     at_b = at_low;
 }
 template <int SLOTS>
-__device__ __forceinline__ void choose_sorted(uint32_t (&key)[8], int choices, int lane, int (&chosen)[SLOTS], uint32_t& most) {
+__device__ __forceinline__ void choose_sorted(uint32_t (&key)[8], int choices, int lane, int (&chosen)[SLOTS], uint32_t (&won)[SLOTS], uint32_t& most) {
     int at[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) at[i] = i;
@@ -126,29 +131,34 @@ __device__ __forceinline__ void choose_sorted(uint32_t (&key)[8], int choices, i
                                   {0, 4}, {1, 5}, {2, 6}, {3, 7}, {2, 4}, {3, 5}, {1, 2}, {3, 4}, {5, 6}};
 #pragma unroll
     for (int i = 0; i < 19; ++i) exchange(key[PAIRS[i][0]], key[PAIRS[i][1]], at[PAIRS[i][0]], at[PAIRS[i][1]]);
+    uint32_t places = 0;  // four bits each, the first lowest
+#pragma unroll
+    for (int i = 0; i < 8; ++i) places |= uint32_t(at[i]) << (4 * i);
 #pragma unroll
     for (int q = 0; q < SLOTS; ++q) {
         chosen[q] = -1;
+        won[q] = NO_KEY;
 #pragma unroll 1
         for (int t = 0; t < 32 && q * 32 + t < choices; ++t) {
             const uint32_t best = __reduce_max_sync(0xffffffffu, key[0]);
             if (q == 0 && t == 0) most = best;
             const int winner = __ffs(__ballot_sync(0xffffffffu, key[0] == best)) - 1;
-            const int e = winner * 8 + __shfl_sync(0xffffffffu, at[0], winner);
-            if (t == lane && best > NO_KEY) chosen[q] = e;
+            const int e = winner * 8 + int(__shfl_sync(0xffffffffu, places, winner) & 15);
+            if (t == lane && best > NO_KEY) {
+                chosen[q] = e;
+                won[q] = best;
+            }
             if (lane == winner) {
 #pragma unroll
-                for (int i = 0; i < 7; ++i) {
-                    key[i] = key[i + 1];
-                    at[i] = at[i + 1];
-                }
+                for (int i = 0; i < 7; ++i) key[i] = key[i + 1];
                 key[7] = 0;
+                places >>= 4;
             }
         }
     }
 }
 
-// As few slots as hold the choices are compiled for: LANES x 8 cover up to 256 experts, so 8 do always.
+// As few slots as hold the choices are compiled for: never more than V, nor than hold 64.
 template <typename T, int V, int LANES, int SLOTS>
 __global__ void __launch_bounds__(LOGIT_THREADS) gate_kernel(GateArgs a, LogitShape s) {
     const int lane = threadIdx.x & (LANES - 1);
@@ -161,25 +171,37 @@ __global__ void __launch_bounds__(LOGIT_THREADS) gate_kernel(GateArgs a, LogitSh
     uint32_t key[V], most = 0;  // most: the highest key of all
     if (a.bias) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int e = run_at<LANES>(i / 8, lane) + i % 8;
-            key[i] = ordered(e < s.experts && v[i] != NOTHING ? v[i] + __ldg(a.bias + e) : v[i]);
+        for (int c = 0; c < V / 4; ++c) {
+            const int e = run_at<LANES>(c / 2, lane) + c % 2 * 4;
+            float4 b = make_float4(0, 0, 0, 0);
+            if (e + 4 <= s.experts && a.bias_wide) {
+                b = __ldg(reinterpret_cast<const float4*>(a.bias + e));
+            } else {
+                if (e < s.experts) b.x = __ldg(a.bias + e);
+                if (e + 1 < s.experts) b.y = __ldg(a.bias + e + 1);
+                if (e + 2 < s.experts) b.z = __ldg(a.bias + e + 2);
+                if (e + 3 < s.experts) b.w = __ldg(a.bias + e + 3);
+            }
+            const float add[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) key[c * 4 + i] = v[c * 4 + i] == NOTHING ? NO_KEY : ordered(v[c * 4 + i] + add[i]);  // (the bias may be infinite)
         }
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) key[i] = ordered(v[i]);
     }
     int chosen[SLOTS];
+    uint32_t won[SLOTS];  // their keys
     if constexpr (LANES == 32 && V == 8) {
-        if (a.choices > 3) choose_sorted<SLOTS>(key, a.choices, lane, chosen, most);
-        else choose<V, LANES, SLOTS>(key, a.choices, lane, chosen, most);
+        if (a.choices > 3) choose_sorted<SLOTS>(key, a.choices, lane, chosen, won, most);
+        else choose<V, LANES, SLOTS>(key, a.choices, lane, chosen, won, most);
     } else {
-        choose<V, LANES, SLOTS>(key, a.choices, lane, chosen, most);
+        choose<V, LANES, SLOTS>(key, a.choices, lane, chosen, won, most);
     }
 
     float l[SLOTS], w[SLOTS];
 #pragma unroll
-    for (int q = 0; q < SLOTS; ++q) l[q] = chosen[q] >= 0 ? to_float(logits[row * s.experts + chosen[q]]) : NOTHING;
+    for (int q = 0; q < SLOTS; ++q) l[q] = a.bias && chosen[q] >= 0 ? to_float(logits[row * s.experts + chosen[q]]) : unordered(won[q]);
     if (a.score == SCORE_SOFTMAX || a.normalize) {  // e^(l - top), or sigmoids over e^top, over their sum (without normalize: of all)
         float top, sum = 0.0f;
         if (a.normalize) top = group_max<LANES>(largest(l));
@@ -215,16 +237,21 @@ __global__ void __launch_bounds__(LOGIT_THREADS) gate_kernel(GateArgs a, LogitSh
     }
 }
 
+// Word i of the rows in shared memory: their 16-byte units permuted so that lanes that read V words each meet no bank twice.
+__device__ __forceinline__ int spread(int i) { return i ^ (i >> 3 & 12); }
+
 template <typename T, int V, int LANES, int SLOTS>
 __global__ void __launch_bounds__(LOGIT_THREADS) gate_backward_kernel(GateArgs a, LogitShape s) {
     // where the lanes that have a choice find the lane that has its expert
-    __shared__ alignas(16) float rows[LOGIT_THREADS / LANES][LANES * V];
+    __shared__ alignas(16) float rows[LOGIT_THREADS * V];
     const int lane = threadIdx.x & (LANES - 1);
     const long long row = (long long)blockIdx.x * (LOGIT_THREADS / LANES) + threadIdx.x / LANES;
     const bool inside = row < s.rows;
     const T* logits = static_cast<const T*>(a.logits);
     const bool dense = a.score == SCORE_SOFTMAX && !a.normalize;
 
+    float v[V];
+    if (dense) load_logits<T, V, LANES>(logits, s, a.mask, row, inside, lane, v);
     // d l at the chosen experts, but for what all experts share
     int chosen[SLOTS];
     float w[SLOTS], d[SLOTS], sum = 0.0f;
@@ -242,9 +269,9 @@ __global__ void __launch_bounds__(LOGIT_THREADS) gate_backward_kernel(GateArgs a
         d[q] = a.d_weights[at];
         sum += w[q] * d[q];
     }
-    float* mine = rows[threadIdx.x / LANES];
+    const int mine = threadIdx.x / LANES * (LANES * V);
 #pragma unroll
-    for (int c = 0; c < V / 4; ++c) *reinterpret_cast<float4*>(mine + run_at<LANES>(c / 2, lane) + c % 2 * 4) = make_float4(0, 0, 0, 0);
+    for (int c = 0; c < V / 4; ++c) *reinterpret_cast<float4*>(rows + spread(mine + run_at<LANES>(c / 2, lane) + c % 2 * 4)) = make_float4(0, 0, 0, 0);
     if (a.normalize || dense) sum = group_sum<LANES>(sum);
     const float mean = a.normalize ? sum * (1.0f / a.scale) : 0.0f;
     __syncwarp();
@@ -253,12 +280,10 @@ __global__ void __launch_bounds__(LOGIT_THREADS) gate_backward_kernel(GateArgs a
         if (chosen[q] < 0) continue;
         d[q] = w[q] * (d[q] - mean);
         if (a.score == SCORE_SIGMOID) d[q] *= sigmoid_of(-to_float(logits[row * s.experts + chosen[q]]));
-        mine[chosen[q]] = d[q];
+        rows[spread(mine + chosen[q])] = d[q];
     }
 
-    float v[V];
     if (dense) {  // - scale p_e sum p g
-        load_logits<T, V, LANES>(logits, s, a.mask, row, inside, lane, v);
         float top = group_max<LANES>(largest(v));
         if (top == NOTHING) top = 0.0f;
         const float total = group_sum<LANES>(powers(v, top)), share = total > 0.0f || total != total ? -sum * inverse_approx(total) : 0.0f;
@@ -271,7 +296,7 @@ __global__ void __launch_bounds__(LOGIT_THREADS) gate_backward_kernel(GateArgs a
     __syncwarp();
 #pragma unroll
     for (int c = 0; c < V / 4; ++c) {
-        const float4 add = *reinterpret_cast<const float4*>(mine + run_at<LANES>(c / 2, lane) + c % 2 * 4);
+        const float4 add = *reinterpret_cast<const float4*>(rows + spread(mine + run_at<LANES>(c / 2, lane) + c % 2 * 4));
         v[c * 4] += add.x;
         v[c * 4 + 1] += add.y;
         v[c * 4 + 2] += add.z;
@@ -284,8 +309,10 @@ template <typename F>
 void with_gate(int dtype, int experts, int choices, F&& f) {
     with_logits(dtype, experts, [&](auto type, auto v, auto lanes) {
         constexpr int LANES = decltype(lanes)::value;
+        constexpr int V = decltype(v)::value, MOST = V < MAX_CHOICES / LANES ? V : MAX_CHOICES / LANES;
         if (choices <= LANES) f(type, v, lanes, std::integral_constant<int, 1>{});
-        else f(type, v, lanes, std::integral_constant<int, LANES == 32 ? 2 : LANES == 16 ? 4 : 8>{});
+        else if (choices <= 2 * LANES) f(type, v, lanes, std::integral_constant<int, 2>{});
+        else if constexpr (MOST > 2) f(type, v, lanes, std::integral_constant<int, MOST>{});
     });
 }
 
@@ -311,6 +338,7 @@ extern "C" int odie_gate(const void* logits, int64_t rows, int experts, int dtyp
         GateArgs a{};
         a.logits = logits;
         a.bias = bias;
+        a.bias_wide = uintptr_t(bias) % 16 == 0;
         a.mask = {mask, mask_row_step, mask_expert_step};
         a.choices = choices;
         a.score = score;

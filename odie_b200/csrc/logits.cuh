@@ -18,8 +18,9 @@ struct Mask {
 };
 
 // A row of E logits among LANES lanes of a warp, V per lane in runs of 8: lane l has experts (c * LANES + l) * 8 + i,
-// c < V / 8, i < 8.  So neighbouring lanes read neighbouring 16 bytes, and up to 8 experts are one thread's.  V is 8 but for
-// more than 256 experts.
+// c < V / 8, i < 8.  So neighbouring lanes read neighbouring 16 bytes.  The kernels are bound by their instructions, of
+// which a good part is per lane and row: 16 values to a lane rather than 8 where that does not leave lanes idle (2^20 rows of
+// 16 fp16, gate forward and backward: MEASURED).
 struct LogitShape {
     long long rows;
     int experts;
@@ -34,13 +35,16 @@ inline LogitShape logit_shape(int64_t rows, int experts, int dtype, std::initial
     s.mask_wide = mask.at && mask.expert_step == 1 && (uintptr_t(mask.at) | uintptr_t(mask.row_step) | uintptr_t(experts)) % 8 == 0;
     return s;
 }
-inline int logit_lanes(int experts) {
-    int lanes = 1;
-    while (lanes < 32 && lanes * 8 < experts) lanes *= 2;
-    return lanes;
+struct LogitLanes {
+    int lanes, values;
+};
+inline LogitLanes logit_lanes(int experts) {
+    if (experts <= 8) return {1, 8};
+    if (experts <= 128) return {experts <= 16 ? 1 : experts <= 32 ? 2 : experts <= 64 ? 4 : 8, 16};
+    return {32, experts <= 256 ? 8 : experts <= 512 ? 16 : 32};
 }
 inline int64_t logit_blocks(int64_t rows, int experts) {
-    const int per_block = LOGIT_THREADS / logit_lanes(experts);
+    const int per_block = LOGIT_THREADS / logit_lanes(experts).lanes;
     return (rows + per_block - 1) / per_block;
 }
 
@@ -53,15 +57,16 @@ void with_logits(int dtype, int experts, F&& f) {
         else f(__half{}, v, lanes);
     };
     using std::integral_constant;
-    const integral_constant<int, 8> eight{};
-    if (experts <= 8) typed(eight, integral_constant<int, 1>{});
-    else if (experts <= 16) typed(eight, integral_constant<int, 2>{});
-    else if (experts <= 32) typed(eight, integral_constant<int, 4>{});
-    else if (experts <= 64) typed(eight, integral_constant<int, 8>{});
-    else if (experts <= 128) typed(eight, integral_constant<int, 16>{});
-    else if (experts <= 256) typed(eight, integral_constant<int, 32>{});
-    else if (experts <= 512) typed(integral_constant<int, 16>{}, integral_constant<int, 32>{});
-    else typed(integral_constant<int, 32>{}, integral_constant<int, 32>{});
+    const LogitLanes l = logit_lanes(experts);
+    const integral_constant<int, 8> v8{};
+    const integral_constant<int, 16> v16{};
+    if (l.values == 32) typed(integral_constant<int, 32>{}, integral_constant<int, 32>{});
+    else if (l.values == 8) l.lanes == 1 ? typed(v8, integral_constant<int, 1>{}) : typed(v8, integral_constant<int, 32>{});
+    else if (l.lanes == 1) typed(v16, integral_constant<int, 1>{});
+    else if (l.lanes == 2) typed(v16, integral_constant<int, 2>{});
+    else if (l.lanes == 4) typed(v16, integral_constant<int, 4>{});
+    else if (l.lanes == 8) typed(v16, integral_constant<int, 8>{});
+    else typed(v16, integral_constant<int, 32>{});
 }
 
 constexpr float NOTHING = -INFINITY;
