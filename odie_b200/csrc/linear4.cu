@@ -600,6 +600,14 @@ struct Finish4Args {
     void* out;
     int activation;
 };
+__device__ __forceinline__ float activated(int activation, float z, Pair added) {
+    Pair slope, y;
+    if (activation == ACT_RELU) y = activate<ACT_RELU, true>(same(z), slope, added);
+    else if (activation == ACT_SILU) y = activate<ACT_SILU, true>(same(z), slope, added);
+    else if (activation == ACT_GELU) y = activate<ACT_GELU, true>(same(z), slope, added);
+    else y = activate<ACT_NONE, true>(same(z), slope, added);
+    return both(y).x;
+}
 template <typename T>
 __global__ void __launch_bounds__(256) finish4_kernel(Finish4Args a) {
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
@@ -612,12 +620,200 @@ __global__ void __launch_bounds__(256) finish4_kernel(Finish4Args a) {
     z = z * a.row_scales[row] * a.column_scales[column];
     if (a.bias) z += to_float(static_cast<const T*>(a.bias)[column]);
     const Pair added = same(a.residual ? to_float(static_cast<const T*>(a.residual)[i]) : 0.0f);
-    Pair slope, y;
-    if (a.activation == ACT_RELU) y = activate<ACT_RELU, true>(same(z), slope, added);
-    else if (a.activation == ACT_SILU) y = activate<ACT_SILU, true>(same(z), slope, added);
-    else if (a.activation == ACT_GELU) y = activate<ACT_GELU, true>(same(z), slope, added);
-    else y = activate<ACT_NONE, true>(same(z), slope, added);
-    static_cast<T*>(a.out)[i] = from_float<T>(both(y).x);
+    static_cast<T*>(a.out)[i] = from_float<T>(activated(a.activation, z, added));
+}
+
+// ---------------------------------------------------------------- a few rows
+// One kernel for up to four rows: bound by the bytes of W and by what one launch takes.  A warp has the rows n, n + 32, n + 64
+// and n + 96 of a tile of W, whose scales lie side by side, and every `splits`-th 1024 values of K; the first of them are on
+// their way while the block quantises x into shared memory.  Products of codes are multiples of 1/4 of at most 36, and eight of
+// them add up exactly in fp16: a block of 16 takes eight packed products and one fp32 step with its scales.
+struct Few4Args {
+    const void* x;
+    const uint8_t* codes;
+    const uint8_t* scales;
+    const float* row_scales;
+    const void* bias;
+    const void* residual;
+    void* y;
+    int rows, inputs, outputs, activation;
+    uint32_t pitch, columns;  // of W's codes and scales
+    int splits, quads;        // warps that share a sum, and sums (of four rows of W) of a block
+    int wide;                 // x starts on a 16-byte boundary, and so do its rows
+};
+
+constexpr int FEW4_ROWS = 4, FEW4_VALUES = 1024, FEW4_SHARED = 96 * 1024;
+template <int M>
+constexpr int FEW4_THREADS = M <= 2 ? 1024 : 512;
+
+// Eight codes as four pairs of fp16.
+__device__ __forceinline__ void halves_of(uint32_t codes, __half2 (&h)[8], int first) {
+    uint32_t r[4];
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\tcvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+        : "r"(codes));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[first + i] = *reinterpret_cast<const __half2*>(&r[i]);
+}
+template <int BLOCK>
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+    return BLOCK == 16 ? e4m3_value(byte) : byte ? __uint_as_float(byte << 23) : 0x1p-127f;
+}
+
+template <typename T, int M, int BLOCK>
+__global__ void __launch_bounds__(FEW4_THREADS<M>) few4_kernel(Few4Args a) {
+    constexpr int WARPS = FEW4_THREADS<M> / 32;
+    extern __shared__ char raw[];
+    uint8_t* const shared = reinterpret_cast<uint8_t*>(raw);
+    __shared__ uint32_t tops[WARPS][M];
+    __shared__ float parts[WARPS][4 * M];
+    uint8_t* x_codes = shared;                                         // [M][pitch]
+    float* x_scales = reinterpret_cast<float*>(shared + M * a.pitch);  // [M][runs], one per block
+    const uint32_t runs = a.pitch / 8, per_row = BLOCK == 16 ? runs : runs / 2;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int split = warp % a.splits, quad = blockIdx.x * a.quads + warp / a.splits;
+    const int n0 = quad / 32 * MICRO_ROWS + quad % 32;  // the first of the four rows of W
+    const bool live = warp / a.splits < a.quads && n0 < a.outputs;
+    const uint32_t chunks = (runs * 16 + FEW4_VALUES - 1) / FEW4_VALUES;
+
+    uint4 w[4], s;
+    auto fetch = [&](uint32_t chunk) {
+        const uint32_t c = chunk * FEW4_VALUES + lane * 32;
+        if (!live || chunk >= chunks || c >= runs * 16) return;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            w[q] = n0 + q * 32 < a.outputs ? __ldg(reinterpret_cast<const uint4*>(a.codes + (long long)(n0 + q * 32) * a.pitch + c / 2)) : make_uint4(0, 0, 0, 0);
+        s = __ldg(reinterpret_cast<const uint4*>(a.scales + ((long long)(quad / 32) * a.columns + c / (4 * BLOCK)) * MICRO_TILE + quad % 32 * 16));
+    };
+    fetch(split);
+
+    // q(x)
+    Run<T> first[M];
+    uint32_t most[M];
+    auto load = [&](Run<T>& run, int m, uint32_t u) {
+        run = Run<T>{};
+        if (m >= a.rows || u >= runs) return;
+        const T* row = static_cast<const T*>(a.x) + (long long)m * a.inputs;
+        if (a.wide) {
+            run.load_wide(row, u * 16, a.inputs);
+        } else {
+            const uint16_t* at = reinterpret_cast<const uint16_t*>(row);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int c = int(u) * 16 + 2 * i;
+                run.w[i] = (c < a.inputs ? at[c] : 0u) | uint32_t(c + 1 < a.inputs ? at[c + 1] : 0u) << 16;
+            }
+        }
+    };
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+        load(first[m], m, threadIdx.x);
+        most[m] = first[m].largest();
+        uint32_t top = most[m];
+        for (uint32_t u = threadIdx.x + blockDim.x; u < runs; u += blockDim.x) {
+            Run<T> run;
+            load(run, m, u);
+            top = max(top, run.largest());
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (lane == 0) tops[warp][m] = top;
+    }
+    __syncthreads();
+    float row_scale[M];
+#pragma unroll
+    for (int m = 0; m < M; ++m) {
+        const uint32_t top = __reduce_max_sync(0xffffffffu, lane < int(blockDim.x >> 5) ? tops[lane][m] : 0u);
+        const bool finite = top < 0x7f800000u;
+        const int k = BLOCK == 16 && top && finite ? least_power(top, 0x280000u, 11, -126) : 0;
+        row_scale[m] = finite ? power_of_two(k) : __int_as_float(0x7fffffff);
+        for (uint32_t u0 = 0; u0 < runs; u0 += blockDim.x) {
+            const uint32_t u = u0 + threadIdx.x;
+            if (u0) {
+                load(first[m], m, u);
+                most[m] = first[m].largest();
+            }
+            uint32_t largest = most[m], scale = 0;
+            if (BLOCK == 32) largest = max(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
+            uint2 codes = round_run<T, BLOCK>(first[m], finite ? largest : 0u, power_of_two(-k), scale);
+            if (!finite) codes = make_uint2(0, 0);
+            if (u >= runs) continue;
+            *reinterpret_cast<uint2*>(x_codes + m * a.pitch + u * 8) = codes;
+            if (BLOCK == 16) x_scales[m * per_row + u] = scale_value<BLOCK>(scale);
+            else if (u % 2 == 0) x_scales[m * per_row + u / 2] = scale_value<BLOCK>(scale);
+        }
+    }
+    __syncthreads();
+
+    float sum[4][M];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int m = 0; m < M; ++m) sum[q][m] = 0.0f;
+    for (uint32_t chunk = split; chunk < chunks; chunk += a.splits) {
+        const uint32_t c = chunk * FEW4_VALUES + lane * 32;
+        const uint4 now[4] = {w[0], w[1], w[2], w[3]}, scales = s;
+        if (int(chunk + a.splits) < int(chunks)) fetch(chunk + a.splits);
+        if (!live || c >= runs * 16) continue;
+        const uint32_t words[4][4] = {{now[0].x, now[0].y, now[0].z, now[0].w},
+                                      {now[1].x, now[1].y, now[1].z, now[1].w},
+                                      {now[2].x, now[2].y, now[2].z, now[2].w},
+                                      {now[3].x, now[3].y, now[3].z, now[3].w}};
+        const uint32_t bytes[4] = {scales.x, scales.y, scales.z, scales.w};
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {  // 16 values each
+            __half2 x[M][8];
+            float by[M];
+#pragma unroll
+            for (int m = 0; m < M; ++m) {
+                const uint2 codes = *reinterpret_cast<const uint2*>(x_codes + m * a.pitch + c / 2 + b * 8);
+                halves_of(codes.x, x[m], 0);
+                halves_of(codes.y, x[m], 4);
+                by[m] = x_scales[m * per_row + (BLOCK == 16 ? c / 16 + b : c / 32)];
+            }
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                __half2 h[8];
+                halves_of(words[q][2 * b], h, 0);
+                halves_of(words[q][2 * b + 1], h, 4);
+                const uint32_t at = BLOCK == 16 ? (c / 16 + b) % 4 : c / 32 % 4;
+                const float scale = scale_value<BLOCK>(bytes[q] >> (at * 8) & 0xffu);
+#pragma unroll
+                for (int m = 0; m < M; ++m) {
+                    __half2 dot = __hmul2(h[0], x[m][0]);
+#pragma unroll
+                    for (int i = 1; i < 8; ++i) dot = __hfma2(h[i], x[m][i], dot);
+                    const float2 d = __half22float2(dot);
+                    sum[q][m] = fmaf(d.x + d.y, scale * by[m], sum[q][m]);
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+        for (int m = 0; m < M; ++m) {
+#pragma unroll
+            for (int d = 16; d > 0; d /= 2) sum[q][m] += __shfl_xor_sync(0xffffffffu, sum[q][m], d);
+            if (lane == 0) parts[warp][q * M + m] = sum[q][m];
+        }
+    __syncthreads();
+    for (int i = threadIdx.x; i < a.quads * 4 * M; i += blockDim.x) {
+        const int part = i / (4 * M), q = i / M % 4, m = i % M, of = blockIdx.x * a.quads + part;
+        const int n = of / 32 * MICRO_ROWS + of % 32 + q * 32;
+        if (n >= a.outputs || m >= a.rows) continue;
+        float z = 0.0f;
+        for (int t = 0; t < a.splits; ++t) z += parts[part * a.splits + t][q * M + m];
+        float scale = 0.0f;
+#pragma unroll
+        for (int r = 0; r < M; ++r)
+            if (r == m) scale = row_scale[r];
+        z = z * scale * __ldg(a.row_scales + n);
+        if (a.bias) z += to_float(static_cast<const T*>(a.bias)[n]);
+        const long long at = (long long)m * a.outputs + n;
+        const Pair added = same(a.residual ? to_float(static_cast<const T*>(a.residual)[at]) : 0.0f);
+        static_cast<T*>(a.y)[at] = from_float<T>(activated(a.activation, z, added));
+    }
 }
 
 // ---------------------------------------------------------------- host
@@ -757,6 +953,39 @@ void launch_product4(const Product4& x, Gemm4Args p, const Splits4& split, float
     }
 }
 
+// Whether few4_kernel takes the call: its rows of x have to fit the shared memory.
+int64_t few4_shared(int64_t rows, int64_t inputs, int block) {
+    const int64_t m = rows <= 1 ? 1 : rows <= 2 ? 2 : 4, pitch = micro_pitch(inputs);
+    return m * (pitch + pitch / 8 * (block == 16 ? 4 : 2));
+}
+bool few4(int64_t rows, int64_t inputs, bool offsets, int block) {
+    return rows <= FEW4_ROWS && !offsets && few4_shared(rows, inputs, block) <= FEW4_SHARED;
+}
+
+template <typename T, int BLOCK>
+void launch_few4(Few4Args a, cudaStream_t stream) {
+    a.pitch = uint32_t(micro_pitch(a.inputs));
+    a.columns = uint32_t(micro_columns(a.inputs, BLOCK));
+    a.wide = (uintptr_t(a.x) | uintptr_t(a.inputs * 2)) % 16 == 0;
+    const int shared = int(few4_shared(a.rows, a.inputs, BLOCK));
+    auto go = [&](auto rows) {
+        constexpr int M = decltype(rows)::value, WARPS = FEW4_THREADS<M> / 32;
+        const int64_t quads = ceil_div(a.outputs, MICRO_ROWS) * 32, chunks = ceil_div(a.inputs, FEW4_VALUES);
+        // as many warps to a sum as it has chunks, up to eight, and as many sums to a block as fill the SMs once
+        a.splits = int(std::min<int64_t>(chunks, 8));
+        a.quads = int(std::min<int64_t>(std::max<int64_t>(1, ceil_div(quads, SMS)), WARPS / a.splits));
+        const int threads = std::max(256, a.quads * a.splits * 32);
+        const auto kernel = few4_kernel<T, M, BLOCK>;
+        ODIE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW4_SHARED));
+        kernel<<<unsigned(ceil_div(quads, a.quads)), threads, shared, stream>>>(a);
+        ODIE_CUDA(cudaGetLastError());
+        note_launch();
+    };
+    if (a.rows == 1) go(std::integral_constant<int, 1>{});
+    else if (a.rows == 2) go(std::integral_constant<int, 2>{});
+    else go(std::integral_constant<int, 4>{});
+}
+
 bool sizes4_fit(int64_t rows, int64_t inputs, int64_t outputs, int64_t groups, int block) {
     return rows >= 0 && rows < (int64_t(1) << 31) - 256 && inputs >= 1 && outputs >= 1 && inputs <= (1 << 20) && outputs <= (1 << 20) &&
            groups >= 1 && groups <= 1024 && (block == 16 || block == 32);
@@ -769,7 +998,7 @@ using namespace odie;
 
 extern "C" int64_t odie_linear4_scratch(int64_t rows, int inputs, int outputs, int groups, int offsets, int block) {
     if (!sizes4_fit(rows, inputs, outputs, groups, block)) return 0;
-    return Scratch4(nullptr, rows, inputs, outputs, groups, offsets, block).bytes;
+    return few4(rows, inputs, offsets, block) ? 0 : Scratch4(nullptr, rows, inputs, outputs, groups, offsets, block).bytes;
 }
 
 extern "C" int odie_linear4(const void* x, const uint8_t* codes, const uint8_t* scales, const float* row_scales, int block, const void* bias,
@@ -784,9 +1013,16 @@ extern "C" int odie_linear4(const void* x, const uint8_t* codes, const uint8_t* 
         if (rows == 0) return;
         ODIE_REQUIRE(x && codes && scales && row_scales && y, "x, codes, scales, row_scales and y are required");
         ODIE_REQUIRE((uintptr_t(codes) | uintptr_t(scales)) % 16 == 0, "codes and scales must start on 16-byte boundaries");
-        ODIE_REQUIRE(scratch && uintptr_t(scratch) % 256 == 0, "scratch is required, on a 256-byte boundary");
+        const bool few = few4(rows, inputs, offsets, block);
+        ODIE_REQUIRE(few || (scratch && uintptr_t(scratch) % 256 == 0), "scratch is required, on a 256-byte boundary");
         int* const error = checked_error_word();
         const cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_handle);
+        if (few) {
+            const Few4Args f{x, codes, scales, row_scales, bias, residual, y, int(rows), inputs, outputs, activation};
+            if (dtype == ROW_BF16) block == 16 ? launch_few4<__nv_bfloat16, 16>(f, stream) : launch_few4<__nv_bfloat16, 32>(f, stream);
+            else block == 16 ? launch_few4<__half, 16>(f, stream) : launch_few4<__half, 32>(f, stream);
+            return;
+        }
         const Scratch4 s(scratch, rows, inputs, outputs, groups, offsets, block);
         MicroArgs q{};
         q.x = x;

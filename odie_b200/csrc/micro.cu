@@ -23,156 +23,6 @@ namespace {
 constexpr int MICRO_THREADS = 256;
 constexpr int HELD = 4;  // runs of 16 values per thread that stay in registers
 
-// a / b, a >= 0, b > 0, cut to 24 bits with the last one set where the quotient is not exact.
-__device__ __forceinline__ float divide_odd(float a, float b) {
-    const float q = __fdiv_rn(a, b), r = fmaf(-q, b, a);
-    uint32_t bits = __float_as_uint(q);
-    if (r < 0.0f) --bits;
-    return __uint_as_float(r != 0.0f ? bits | 1u : bits);
-}
-__device__ __forceinline__ float power_of_two(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }  // -126 <= e <= 127
-// The least e >= least with v <= most 2^e; most = mantissa(of 1.m) 2^shift, v >= 0 as its bits.
-__device__ __forceinline__ int least_power(uint32_t bits, uint32_t most_mantissa, int shift, int least) {
-    const int e = int(bits >> 23) - 127 - shift + ((bits & 0x7fffffu) > most_mantissa);
-    return max(least, e);  // (a subnormal v: far below any `least`)
-}
-// Eight values as codes, the first in the lowest four bits.
-__device__ __forceinline__ uint32_t codes_of(const float2 (&q)[4]) {
-    uint32_t r;
-    asm("{\n\t.reg .b8 a, b, c, d;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
-        "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
-        "mov.b32 %0, {a, b, c, d};\n\t}"
-        : "=r"(r)
-        : "f"(q[0].x), "f"(q[0].y), "f"(q[1].x), "f"(q[1].y), "f"(q[2].x), "f"(q[2].y), "f"(q[3].x), "f"(q[3].y));
-    return r;
-}
-__device__ __forceinline__ float e4m3_value(uint32_t byte) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(uint8_t(byte), __NV_E4M3))); }
-
-// Where N values of each thread of a row are exchanged, one word per row of N beyond them: no two in one bank.  value(i): the
-// thread's i-th of its N neighbours' in a row; strided(i): the one that is i x lanes behind its lane's (lanes a multiple of N).
-template <int N>
-struct Exchange {
-    uint32_t *row, *at;
-    int step;
-    __device__ __forceinline__ Exchange(uint32_t* words, int lanes, int lane) {
-        words += (threadIdx.x - lane) * (N + 1);
-        row = words + lane * (N + 1);
-        at = words + lane + lane / N;
-        step = lanes + lanes / N;
-    }
-    __device__ __forceinline__ uint32_t& value(int i) const { return row[i]; }
-    __device__ __forceinline__ uint32_t& strided(int i) const { return at[i * step]; }
-};
-__device__ __forceinline__ void sync_row(int lanes) {  // the threads of a row
-    if (lanes > 32) __syncthreads();
-    else __syncwarp();
-}
-
-// 16 consecutive values of a row from column c on, zeros behind its end.
-template <typename T>
-struct Run {
-    static constexpr int WORDS = 16 * sizeof(T) / 4;
-    uint32_t w[WORDS];
-    __device__ __forceinline__ void load_wide(const T* row, long long c, int width) {  // width a multiple of PER
-        constexpr int PER = 16 / int(sizeof(T));
-#pragma unroll
-        for (int i = 0; i < int(sizeof(T)); ++i) {
-            const uint4 v = c + i * PER < width ? __ldg(reinterpret_cast<const uint4*>(row + c + i * PER)) : make_uint4(0, 0, 0, 0);
-            w[4 * i] = v.x;
-            w[4 * i + 1] = v.y;
-            w[4 * i + 2] = v.z;
-            w[4 * i + 3] = v.w;
-        }
-    }
-    // The row's `lanes` threads take its 16 lanes values from `from` on, `left` of them inside.
-    __device__ __forceinline__ void load(const T* from, int left, int lanes, int lane, const Exchange<16>& x) {
-        from += lane;
-        left -= lane;
-        uint32_t v[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            if constexpr (sizeof(T) == 4) v[i] = i * lanes < left ? __float_as_uint(from[i * lanes]) : 0u;
-            else v[i] = i * lanes < left ? reinterpret_cast<const uint16_t*>(from)[i * lanes] : 0u;
-        }
-        sync_row(lanes);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x.strided(i) = v[i];
-        sync_row(lanes);
-#pragma unroll
-        for (int i = 0; i < WORDS; ++i) {
-            if constexpr (sizeof(T) == 4) w[i] = x.value(i);
-            else w[i] = x.value(2 * i) | x.value(2 * i + 1) << 16;
-        }
-    }
-    __device__ __forceinline__ float2 pair_at(int i) const {  // values 2 i and 2 i + 1
-        if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
-        else return unpack_pair<T>(w[i]);
-    }
-    // The bits of the largest magnitude as fp32: those of infinities and NaNs are the largest.
-    __device__ __forceinline__ uint32_t largest() const {
-        uint32_t m = 0;
-        if constexpr (sizeof(T) == 4) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) m = max(m, w[i] & 0x7fffffffu);
-            return m;
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) m = __vmaxu2(m, w[i] & 0x7fff7fffu);
-            m = max(m & 0xffffu, m >> 16);
-            if constexpr (std::is_same<T, __nv_bfloat16>::value) return m << 16;
-            else return __float_as_uint(__half2float(__ushort_as_half(uint16_t(m))));
-        }
-    }
-};
-
-// Sixteen codes and their scale's byte; largest: of the block.
-template <typename T, int BLOCK>
-__device__ __forceinline__ uint2 round_run(const Run<T>& x, uint32_t largest, float inverse_row, uint32_t& scale) {
-    float2 q[8];
-    if constexpr (BLOCK == 32) {
-        const int e = least_power(largest, 0x400000u, 2, -127);
-        scale = uint32_t(e + 127);
-        const Pair factor = same(power_of_two(-e));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] = both(mul2(pair(x.pair_at(i).x, x.pair_at(i).y), factor));
-    } else if constexpr (sizeof(T) == 2) {
-        const float t = __uint_as_float(largest) * inverse_row * (1.0f / 6.0f), wide = t * 257.0f;
-        scale = __nv_cvt_float_to_fp8(__fsub_rn(wide, __fsub_rn(wide, t)), __NV_SATFINITE, __NV_E4M3);
-        const float factor = scale ? inverse_approx(e4m3_value(scale)) : 0.0f;
-        const Pair up = same(96.0f), down = same(-96.0f);
-        if (std::is_same<T, __half>::value || inverse_row < 0x1p100f) {
-            const Pair by = same(inverse_row * factor);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float2 v = x.pair_at(i);
-                q[i] = both(add2(fma2(pair(v.x, v.y), by, up), down));
-            }
-        } else {  // the factors' product may be infinite
-            const Pair first = same(inverse_row), second = same(factor);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float2 v = x.pair_at(i);
-                q[i] = both(add2(fma2(mul2(pair(v.x, v.y), first), second, up), down));
-            }
-        }
-    } else {
-        scale = __nv_cvt_float_to_fp8(divide_odd(__uint_as_float(largest) * inverse_row, 6.0f), __NV_SATFINITE, __NV_E4M3);
-        const float divisor = scale ? e4m3_value(scale) : INFINITY;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float2 v = x.pair_at(i);
-            q[i].x = copysignf(divide_odd(fabsf(v.x) * inverse_row, divisor), v.x);
-            q[i].y = copysignf(divide_odd(fabsf(v.y) * inverse_row, divisor), v.y);
-        }
-        if (!scale) return make_uint2(0, 0);
-    }
-    const float2 low[4] = {q[0], q[1], q[2], q[3]}, high[4] = {q[4], q[5], q[6], q[7]};
-    return make_uint2(codes_of(low), codes_of(high));
-}
-
 template <typename T, int BLOCK, bool WIDE>
 __global__ void __launch_bounds__(MICRO_THREADS, sizeof(T) == 2 ? 4 : 2) quantize_kernel(MicroArgs a, int lanes_log2) {
     __shared__ uint32_t tops[MICRO_THREADS / 32];
