@@ -35,16 +35,14 @@ struct Gemm4Args {
     int k;               // inputs
     int a_rows;          // rows of A's boxes: 128 or, for fewer rows in all, those (rounded up to 8)
     int a_tiles;         // tiles of A's scales that there are
-    int chunk, splits;   // without offsets: the sum over K cut among this many tiles of `chunk` blocks, joined by finish4_kernel
+    int chunk, splits;   // without offsets: the sum over K cut among the CTAs of a cluster, `chunk` blocks each
     Divide by_bands;     // tiles of a full band
-    Divide by_tiles;     // splits: tiles of C
     const float* row_scales;     // [rows]
     const float* column_scales;  // [groups][n]
     const void* bias;
     const void* residual;
     void* out;
     int activation;
-    float* partial;      // splits: [split][rows][n] sums
     bool boxes;          // TMA takes rows of out (every one starts on a 16-byte boundary); boxes_in: of the residual
     bool boxes_in;
     int stages;          // blocks in flight
@@ -84,7 +82,6 @@ struct Tile4 {
     int m_end;     // rows from here on are not stored
     int k0;        // first block of K
     int k_blocks;
-    int split;
     int scales;    // tile of A's scales of row m0
     bool zero;     // nothing to sum: zeros are stored
 };
@@ -96,22 +93,17 @@ struct Walk4 {
     const int* begin;
     const int* first;
     const int* scales;
+    int split;  // PARTIAL: the part of K
     int g = 0;
-    __device__ __forceinline__ Walk4(const Gemm4Args& args, const int* b, const int* f, const int* s) : p(args), begin(b), first(f), scales(s) {}
+    __device__ __forceinline__ Walk4(const Gemm4Args& args, const int* b, const int* f, const int* s, int part)
+        : p(args), begin(b), first(f), scales(s), split(part) {}
     __device__ __forceinline__ Tile4 at(int t) {
         constexpr int TM = 128 * CG;
         Tile4 tile;
-        int key = t, split = 0;
-        if (PARTIAL) {
-            split = p.by_tiles(t);
-            key = t - split * int(p.by_tiles.d);
-        }
-        // (a CTA's tiles ascend in t but, with splits, not in `key`: there is one group then, or the rows of none)
-        if (PARTIAL) g = 0;
-        while (g < p.groups && uniform(first[g + 1]) <= key) ++g;
+        while (g < p.groups && uniform(first[g + 1]) <= t) ++g;
         tile.g = g;
         const int from = uniform(begin[g]), to = g < p.groups ? uniform(begin[g + 1]) : int(p.rows);
-        int local = key - uniform(first[g]);
+        int local = t - uniform(first[g]);
         const int band = p.by_bands(local), left = (to - from + TM - 1) / TM - band * BAND;
         local -= band * int(p.by_bands.d);
         int n = local / BAND, m = local % BAND;
@@ -129,7 +121,6 @@ struct Walk4 {
         tile.m0 = from + (band * BAND + m) * TM;
         tile.n0 = n * BN;
         tile.m_end = to;
-        tile.split = split;
         tile.k0 = PARTIAL ? split * p.chunk : 0;
         tile.k_blocks = (p.k + BK - 1) / BK;
         if (PARTIAL) tile.k_blocks = min(tile.k_blocks - tile.k0, p.chunk);
@@ -158,13 +149,18 @@ __device__ __forceinline__ void move_box(uint16_t* at, char* box, int ld, int ro
             else *boxed<COLS>(box, r, u) = *out;
         }
     } else {
-        for (int r = 0; r < rows; ++r)
-            for (int c = lane; c < columns; c += 32) {
+#pragma unroll
+        for (int c = lane; c < COLS; c += 32) {
+            if (c >= columns) continue;
+#pragma unroll 16
+            for (int r = 0; r < 32; ++r) {
+                if (r >= rows) continue;
                 uint16_t* in = reinterpret_cast<uint16_t*>(boxed<COLS>(box, r, c / 8)) + c % 8;
                 uint16_t* out = at + (long long)r * ld + c;
                 if (STORE) *out = *in;
                 else *in = *out;
             }
+        }
     }
 }
 
@@ -197,7 +193,53 @@ __device__ __forceinline__ void finish_box(const float (&v)[2][COLS / 2], const 
     }
 }
 
-// PARTIAL: the sums go to p.partial as they are, joined by finish4_kernel.
+__device__ __forceinline__ float activated(int activation, float z, Pair added) {
+    Pair slope, y;
+    if (activation == ACT_RELU) y = activate<ACT_RELU, true>(same(z), slope, added);
+    else if (activation == ACT_SILU) y = activate<ACT_SILU, true>(same(z), slope, added);
+    else if (activation == ACT_GELU) y = activate<ACT_GELU, true>(same(z), slope, added);
+    else y = activate<ACT_NONE, true>(same(z), slope, added);
+    return both(y).x;
+}
+
+// A part's sums in shared memory, where its blocks of K were: rows of BN + 4.
+template <int BN>
+__device__ __forceinline__ float* part_at(char* base, int row, int column) {
+    return reinterpret_cast<float*>(base) + row * (BN + 4) + column;
+}
+// The cluster's parts of a tile to y: a CTA takes every splits-th row.
+template <typename T, int BN>
+__device__ __forceinline__ void join_parts(const Gemm4Args& p, const Tile4& tile, char* base) {
+    const int rank = int(tc::cluster_rank()), rows = min(128, tile.m_end - tile.m0), columns = min(BN, p.n - tile.n0);
+    for (int i = threadIdx.x; i < (rows - rank + p.splits - 1) / p.splits * (BN / 4); i += blockDim.x) {
+        const int r = rank + i / (BN / 4) * p.splits, c = i % (BN / 4) * 4;
+        if (c >= columns) continue;
+        float4 z = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        const uint32_t from = tc::smem_u32(part_at<BN>(base, r, c));
+#pragma unroll 8
+        for (int part = 0; part < p.splits; ++part) {
+            const float4 v = tc::load_cluster(from, part);
+            z.x += v.x;
+            z.y += v.y;
+            z.z += v.z;
+            z.w += v.w;
+        }
+        const float by = __ldg(p.row_scales + tile.m0 + r), zs[4] = {z.x, z.y, z.z, z.w};
+        const long long at = (long long)(tile.m0 + r) * p.n + tile.n0 + c;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (c + e >= columns) continue;
+            const int n = tile.n0 + c + e;
+            float y = zs[e] * by * __ldg(p.column_scales + n);
+            if (p.bias) y += to_float(static_cast<const T*>(p.bias)[n]);
+            const Pair added = same(p.residual ? to_float(static_cast<const T*>(p.residual)[at + e]) : 0.0f);
+            static_cast<T*>(p.out)[at + e] = from_float<T>(activated(p.activation, y, added));
+        }
+    }
+}
+
+// PARTIAL: one tile for each cluster, whose CTAs have a part of K each; they lay their sums into shared memory, and each
+// finishes a share of the rows from all parts, in their order.
 template <typename T, int CG, int BN, int BLOCK, bool PARTIAL>
 __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
     gemm4_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
@@ -291,11 +333,12 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
     const uint32_t tmem = uniform(*tmem_at);
     const uint32_t full_leader = CG == 2 ? uniform(tc::leader_address(full)) : 0;
     const int units = uniform(first[p.groups + 1]);
-    const int tiles = PARTIAL ? units * p.splits : units;
-    const int start = int(blockIdx.x) / CG, step = int(gridDim.x) / CG;
+    const int tiles = units;
+    const int start = PARTIAL ? int(blockIdx.x) / p.splits : int(blockIdx.x) / CG, step = PARTIAL ? units : int(gridDim.x) / CG;
     bool fine = true;
-    Walk4<CG, BN, PARTIAL> walk(p, begin, first, scales);
+    Walk4<CG, BN, PARTIAL> walk(p, begin, first, scales, PARTIAL ? uniform(tc::cluster_rank()) : 0);
 
+    dependencies_done();  // (all of the above runs beside the end of the kernel that quantises x)
     // The loading and the multiplying warp walk their loops with all lanes, and one lane issues (see linear.cu).
     if (warp == 0) {
         const bool issuer = tc::elect_one();
@@ -412,7 +455,7 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
             int* slot = reinterpret_cast<int*>(slots + q * S::SLOT);
             if (lane == 0) {
                 *reinterpret_cast<int4*>(slot) = make_int4(tile.g, tile.m0, tile.n0, tile.m_end);
-                *reinterpret_cast<int4*>(slot + 4) = make_int4(tile.split, tile.zero, 0, 0);
+                *reinterpret_cast<int4*>(slot + 4) = make_int4(tile.zero, 0, 0, 0);
             }
             if (!PARTIAL && !tile.zero) {
                 float* to = reinterpret_cast<float*>(slot + 8);
@@ -452,35 +495,34 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
             tile.m0 = uniform(first_word.y);
             tile.n0 = uniform(first_word.z);
             tile.m_end = uniform(first_word.w);
-            tile.split = uniform(second_word.x);
-            tile.zero = uniform(second_word.y);
+            tile.zero = uniform(second_word.x);
             const float* column = reinterpret_cast<const float*>(slot + 8) + 128 + group * COLS * 2;
             const int acc = summed & 1;
             const int row = tile.m0 + rank * 128 + quadrant * 32, column0 = tile.n0 + group * COLS;
             const int rows = min(32, tile.m_end - row), columns = p.n - column0;  // inside the matrix
             const bool inside = rows > 0 && columns > 0, whole = rows == 32 && columns > 0;
             const long long at = (long long)row * p.n + column0;
-            const bool residual = !PARTIAL && p.residual && !tile.zero && inside;
+            const bool residual = p.residual && !tile.zero && inside;
             float row_scale[4];
-            if (!PARTIAL) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) row_scale[j] = reinterpret_cast<const float*>(slot + 8)[quadrant * 32 + j * 8 + lane / 4];
-                if (lane == 0) tc::stores_read();  // the box is free
+            for (int j = 0; j < 4; ++j) row_scale[j] = reinterpret_cast<const float*>(slot + 8)[quadrant * 32 + j * 8 + lane / 4];
+            auto ask = [&] {  // for the residual, into the box
+                if (lane == 0) tc::stores_read();  // it is free
                 __syncwarp();
-                if (residual) {
-                    if (whole && p.boxes_in) {
-                        if (lane == 0) {
-                            tc::fence_async_smem();
-                            tc::bar_expect(arrived + index, S::BOX);
-                            tc::tma_load_2d<1>(box, &map_residual, column0, row, tc::smem_u32(arrived + index));
-                        }
-                        asked = true;
-                    } else {
-                        move_box<COLS, false>(static_cast<uint16_t*>(const_cast<void*>(p.residual)) + at, box, p.n, rows, columns, lane);
+                if (!residual) return;
+                if (whole && p.boxes_in) {
+                    if (lane == 0) {
+                        tc::fence_async_smem();
+                        tc::bar_expect(arrived + index, S::BOX);
+                        tc::tma_load_2d<1>(box, &map_residual, column0, row, tc::smem_u32(arrived + index));
                     }
-                    __syncwarp();
+                    asked = true;
+                } else {
+                    move_box<COLS, false>(static_cast<uint16_t*>(const_cast<void*>(p.residual)) + at, box, p.n, rows, columns, lane);
                 }
-            }
+                __syncwarp();
+            };
+            if (!PARTIAL) ask();
             fine = __all_sync(0xffffffffu, tc::bar_wait(done + acc, (summed >> 1) & 1, p.limit));
             if (!fine) break;
             tc::fence_after_sync();
@@ -493,22 +535,11 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
             }
             if (PARTIAL) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int r = j * 8 + lane / 4;
-                    float* to = p.partial + ((long long)tile.split * p.rows + row + r) * p.n + column0 + (lane & 3) * 2;
-                    if (r >= rows) continue;
+                for (int j = 0; j < 4; ++j)
 #pragma unroll
-                    for (int u = 0; u < COLS / 8; ++u) {
-                        const float x = v[j / 2][u * 4 + j % 2 * 2], y = v[j / 2][u * 4 + j % 2 * 2 + 1];
-                        const int left = columns - u * 8 - (lane & 3) * 2;
-                        if (p.n % 2 == 0) {
-                            if (left > 0) *reinterpret_cast<float2*>(to + u * 8) = make_float2(x, y);
-                        } else {
-                            if (left > 0) to[u * 8] = x;
-                            if (left > 1) to[u * 8 + 1] = y;
-                        }
-                    }
-                }
+                    for (int u = 0; u < COLS / 8; ++u)
+                        *reinterpret_cast<float2*>(part_at<BN>(stages, quadrant * 32 + j * 8 + lane / 4, group * COLS + u * 8 + (lane & 3) * 2)) =
+                            make_float2(v[j / 2][u * 4 + j % 2 * 2], v[j / 2][u * 4 + j % 2 * 2 + 1]);
             } else {
                 if (asked) {
                     fine = __all_sync(0xffffffffu, tc::bar_wait(arrived + index, phase, p.limit));
@@ -528,8 +559,6 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
                 else if (p.activation == ACT_SILU) go(std::integral_constant<int, ACT_SILU>{});
                 else if (p.activation == ACT_GELU) go(std::integral_constant<int, ACT_GELU>{});
                 else go(std::integral_constant<int, ACT_NONE>{});
-                __syncwarp();
-                if (lane == 0) tc::bar_arrive(heard + q);
                 if (whole && p.boxes) {
                     tc::fence_async_smem();
                     __syncwarp();
@@ -540,7 +569,8 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
                     __syncwarp();
                 }
             }
-            if (PARTIAL && lane == 0) tc::bar_arrive(heard + q);
+            __syncwarp();
+            if (lane == 0) tc::bar_arrive(heard + q);
             if (++q == S::SLOTS) {
                 q = 0;
                 q_phase ^= 1;
@@ -584,43 +614,13 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
         if (CG == 2) tc::cluster_sync();
         tc::fence_after_sync();
     }
+    if constexpr (PARTIAL) {
+        tc::cluster_sync();  // all parts are there
+        const Tile4 tile = walk.at(start);
+        join_parts<T, BN>(p, tile, stages);
+        tc::cluster_sync();  // and are not read any more
+    }
     if (warp == 2) tc::tmem_dealloc_group<CG>(tmem, S::COLUMNS);
-}
-
-// The sums over parts of K, in order, with the epilogue of the products.
-struct Finish4Args {
-    const float* partial;  // [splits][rows][n]
-    int splits;
-    long long rows;
-    int n;
-    const float* row_scales;
-    const float* column_scales;
-    const void* bias;
-    const void* residual;
-    void* out;
-    int activation;
-};
-__device__ __forceinline__ float activated(int activation, float z, Pair added) {
-    Pair slope, y;
-    if (activation == ACT_RELU) y = activate<ACT_RELU, true>(same(z), slope, added);
-    else if (activation == ACT_SILU) y = activate<ACT_SILU, true>(same(z), slope, added);
-    else if (activation == ACT_GELU) y = activate<ACT_GELU, true>(same(z), slope, added);
-    else y = activate<ACT_NONE, true>(same(z), slope, added);
-    return both(y).x;
-}
-template <typename T>
-__global__ void __launch_bounds__(256) finish4_kernel(Finish4Args a) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= a.rows * a.n) return;
-    const long long row = i / a.n;
-    const int column = int(i - row * a.n);
-    float z = 0.0f;
-#pragma unroll 8
-    for (int s = 0; s < a.splits; ++s) z += __ldg(a.partial + s * a.rows * a.n + i);
-    z = z * a.row_scales[row] * a.column_scales[column];
-    if (a.bias) z += to_float(static_cast<const T*>(a.bias)[column]);
-    const Pair added = same(a.residual ? to_float(static_cast<const T*>(a.residual)[i]) : 0.0f);
-    static_cast<T*>(a.out)[i] = from_float<T>(activated(a.activation, z, added));
 }
 
 // ---------------------------------------------------------------- a few rows
@@ -729,6 +729,7 @@ __global__ void __launch_bounds__(FEW4_THREADS<M>) few4_kernel(Few4Args a) {
         row_scale[m] = finite ? power_of_two(k) : __int_as_float(0x7fffffff);
         for (uint32_t u0 = 0; u0 < runs; u0 += blockDim.x) {
             const uint32_t u = u0 + threadIdx.x;
+            if (u0 + warp * 32 >= runs) break;  // nothing for the whole warp
             if (u0) {
                 load(first[m], m, u);
                 most[m] = first[m].largest();
@@ -835,19 +836,18 @@ struct Splits4 {
     int parts, blocks;  // blocks of K per part
     Splits4(int64_t rows, int n, int k, int groups, bool offsets) : parts(1), blocks(int(ceil_div(k, BK))) {
         if (rows == 0 || offsets || pair_tiles(rows, n, groups)) return;
-        const int64_t tiles = ceil_div(rows, 128) * ceil_div(n, 128), wanted = std::min<int64_t>(SMS / tiles, blocks / 2);
+        const int64_t tiles = ceil_div(rows, 128) * ceil_div(n, 128), wanted = std::min<int64_t>({128 / tiles, blocks / 2, 8});  // (clusters of 8 CTAs do not fill every SM)
         if (wanted < 2) return;
         blocks = int(ceil_div(blocks, wanted));
         parts = int(ceil_div(ceil_div(k, BK), blocks));
     }
-    int64_t bytes(int64_t rows, int n) const { return parts > 1 ? parts * rows * n * 4 : 0; }
 };
 
 struct Scratch4 {
     uint8_t *codes, *scales;
-    float *row_scales, *partial;
+    float* row_scales;
     int64_t tiles, bytes = 0;
-    Scratch4(void* base, int64_t rows, int inputs, int outputs, int groups, bool offsets, int block) {
+    Scratch4(void* base, int64_t rows, int inputs, int groups, bool offsets, int block) {
         char* at = static_cast<char*>(base);
         auto take = [&](int64_t size) {
             char* p = at ? at + bytes : nullptr;
@@ -858,7 +858,6 @@ struct Scratch4 {
         codes = reinterpret_cast<uint8_t*>(take(rows * micro_pitch(inputs)));
         scales = reinterpret_cast<uint8_t*>(take(tiles * micro_columns(inputs, block) * MICRO_TILE));
         row_scales = reinterpret_cast<float*>(take(rows * 4));
-        partial = reinterpret_cast<float*>(take(Splits4(rows, outputs, inputs, groups, offsets).bytes(rows, outputs)));
     }
 };
 
@@ -890,7 +889,6 @@ void launch_gemm4(const Product4& x, Gemm4Args p, int64_t tiles, cudaStream_t st
     ODIE_REQUIRE(tiles < (int64_t(1) << 30), "too many rows and columns for one launch");
     const int64_t nt = ceil_div(p.n, BN), pitch = micro_pitch(p.k), columns = micro_columns(p.k, BLOCK), row_tiles = ceil_div(p.n, MICRO_ROWS);
     p.by_bands = Divide::by(BAND * nt);
-    p.by_tiles = Divide::by(nt * ceil_div(p.rows, 128 * CG));
     const int64_t da[] = {pitch, p.rows}, ta[] = {pitch};
     const int xa[] = {128, p.a_rows};
     const CUtensorMap map_a = tensor_map(x.a, CU_TENSOR_MAP_DATA_TYPE_UINT8, CU_TENSOR_MAP_SWIZZLE_128B, 2, da, ta, xa);
@@ -917,26 +915,29 @@ void launch_gemm4(const Product4& x, Gemm4Args p, int64_t tiles, cudaStream_t st
     const auto kernel = gemm4_kernel<T, CG, BN, BLOCK, PARTIAL>;
     ODIE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SHARED));
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(unsigned(std::min<int64_t>(tiles, sm_count() / CG) * CG));
+    const unsigned cluster = PARTIAL ? unsigned(p.splits) : CG;
+    config.gridDim = dim3(unsigned(PARTIAL ? tiles : std::min<int64_t>(tiles, sm_count() / CG)) * cluster);
     config.blockDim = dim3(S::THREADS);
     config.dynamicSmemBytes = size_t(S::bytes(p.groups));
     config.stream = stream;
-    cudaLaunchAttribute cluster{};
-    cluster.id = cudaLaunchAttributeClusterDimension;
-    cluster.val.clusterDim.x = CG;
-    cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
-    config.attrs = &cluster;
-    config.numAttrs = 1;
+    cudaLaunchAttribute attributes[2]{};
+    attributes[0].id = cudaLaunchAttributeClusterDimension;
+    attributes[0].val.clusterDim.x = cluster;
+    attributes[0].val.clusterDim.y = attributes[0].val.clusterDim.z = 1;
+    attributes[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[1].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attributes;
+    config.numAttrs = 2;
     ODIE_CUDA(cudaLaunchKernelEx(&config, kernel, map_a, map_b, map_sa, map_sb, map_out, map_residual, p));
     note_launch();
 }
 
 template <typename T, int BLOCK>
-void launch_product4(const Product4& x, Gemm4Args p, const Splits4& split, float* partial, cudaStream_t stream) {
+void launch_product4(const Product4& x, Gemm4Args p, const Splits4& split, cudaStream_t stream) {
     const bool pairs = pair_tiles(p.rows, p.n, p.groups);
     p.a_rows = int(std::min<int64_t>(128, (p.rows + 7) / 8 * 8));
     p.splits = 1;
-    const int64_t tiles = (ceil_div(p.rows, pairs ? 256 : 128) + p.groups + 1) * ceil_div(p.n, pairs ? 256 : 128);
+    const int64_t side = pairs ? 256 : 128, tiles = (ceil_div(p.rows, side) + (p.offsets ? p.groups + 1 : 0)) * ceil_div(p.n, side);  // at most
     if (pairs) {
         launch_gemm4<T, 2, 256, BLOCK, false>(x, p, tiles, stream);
     } else if (split.parts == 1) {
@@ -944,12 +945,7 @@ void launch_product4(const Product4& x, Gemm4Args p, const Splits4& split, float
     } else {
         p.splits = split.parts;
         p.chunk = split.blocks;
-        p.partial = partial;
-        launch_gemm4<T, 1, 128, BLOCK, true>(x, p, tiles * split.parts, stream);
-        const Finish4Args f{partial, split.parts, p.rows, p.n, p.row_scales, p.column_scales, p.bias, p.residual, p.out, p.activation};
-        finish4_kernel<T><<<unsigned(ceil_div(p.rows * p.n, 256)), 256, 0, stream>>>(f);
-        ODIE_CUDA(cudaGetLastError());
-        note_launch();
+        launch_gemm4<T, 1, 128, BLOCK, true>(x, p, tiles, stream);
     }
 }
 
@@ -998,7 +994,7 @@ using namespace odie;
 
 extern "C" int64_t odie_linear4_scratch(int64_t rows, int inputs, int outputs, int groups, int offsets, int block) {
     if (!sizes4_fit(rows, inputs, outputs, groups, block)) return 0;
-    return few4(rows, inputs, offsets, block) ? 0 : Scratch4(nullptr, rows, inputs, outputs, groups, offsets, block).bytes;
+    return few4(rows, inputs, offsets, block) ? 0 : Scratch4(nullptr, rows, inputs, groups, offsets, block).bytes;
 }
 
 extern "C" int odie_linear4(const void* x, const uint8_t* codes, const uint8_t* scales, const float* row_scales, int block, const void* bias,
@@ -1023,7 +1019,7 @@ extern "C" int odie_linear4(const void* x, const uint8_t* codes, const uint8_t* 
             else block == 16 ? launch_few4<__half, 16>(f, stream) : launch_few4<__half, 32>(f, stream);
             return;
         }
-        const Scratch4 s(scratch, rows, inputs, outputs, groups, offsets, block);
+        const Scratch4 s(scratch, rows, inputs, groups, offsets, block);
         MicroArgs q{};
         q.x = x;
         q.rows = q.group_rows = rows;
@@ -1054,8 +1050,8 @@ extern "C" int odie_linear4(const void* x, const uint8_t* codes, const uint8_t* 
         const Product4 operands{s.codes, s.scales, codes, scales};
         const Splits4 split(rows, outputs, inputs, groups, offsets);
         auto go = [&](auto type) {
-            if (block == 16) launch_product4<decltype(type), 16>(operands, p, split, s.partial, stream);
-            else launch_product4<decltype(type), 32>(operands, p, split, s.partial, stream);
+            if (block == 16) launch_product4<decltype(type), 16>(operands, p, split, stream);
+            else launch_product4<decltype(type), 32>(operands, p, split, stream);
         };
         if (dtype == ROW_BF16) go(__nv_bfloat16{});
         else go(__half{});

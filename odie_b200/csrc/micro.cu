@@ -29,6 +29,7 @@ __global__ void __launch_bounds__(MICRO_THREADS, sizeof(T) == 2 ? 4 : 2) quantiz
     __shared__ uint32_t words[WIDE ? 1 : MICRO_THREADS * 17];
     const int lanes = 1 << lanes_log2, lane = threadIdx.x & (lanes - 1), line = threadIdx.x >> lanes_log2;
     const Exchange<16> exchange(words, lanes, lane);
+    dependents_may_start();
     // the tile of rows
     const int tile = blockIdx.x / a.first_blocks, part = blockIdx.x - tile * a.first_blocks;
     long long from, to;

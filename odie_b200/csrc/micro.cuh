@@ -40,6 +40,10 @@ struct MicroArgs {
     long long pitch, columns;  // of codes in bytes, of scales in tiles
     int first_blocks;          // blocks of threads per tile of rows
 };
+// A kernel may start while the one before it on its stream ends, if that says so and the launch of the other allows it; it
+// then waits for all of it, and for what it wrote, before it reads that.
+__device__ __forceinline__ void dependents_may_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void dependencies_done() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Tiles of rows that `rows` rows in `groups` groups may need: those of no group (behind the last offset) have some too.
 inline int64_t micro_tiles(int64_t rows, int64_t groups) { return (rows + MICRO_ROWS - 1) / MICRO_ROWS + groups + 1; }
 

@@ -247,3 +247,26 @@ def test_linear4_is_captured_and_replayed(cuda):
         for graph in graphs:
             graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(results, want[turn]))
+
+
+def test_linear4_wait_that_runs_out(cuda):
+    """A product whose waits may not poll at all ends, and the next call says so, once; then all is as before."""
+    from odie_b200 import _lib
+    from odie_b200.experts import check, linear4, quantize
+    lib = _lib.library()
+    g = generator(11)
+    for rows, inputs, outputs in ((64, 4096, 256), (700, 544, 2000), (4000, 512, 2048)):
+        x = torch.randn((rows, inputs), generator=g, device='cuda').bfloat16()
+        micro = quantize(torch.randn((outputs, inputs), generator=g, device='cuda'))
+        want = linear4(x, micro)
+        torch.cuda.synchronize()
+        assert lib.odie_linear_wait_limit(0) == 0
+        try:
+            linear4(x, micro)
+            torch.cuda.synchronize()
+        finally:
+            assert lib.odie_linear_wait_limit(-1) == 0
+        with pytest.raises(RuntimeError, match='ran out'):
+            linear4(x, micro)
+        check()
+        assert torch.equal(linear4(x, micro), want)
