@@ -26,6 +26,7 @@ namespace {
 constexpr int BK = 256;
 constexpr int EPILOGUE_WARP = 4;  // the first one
 constexpr int MAX_SHARED = 227 * 1024;
+constexpr int AHEAD = 64;         // columns of the residual that are brought to L2 at a time
 
 struct Gemm4Args {
     int groups;
@@ -244,7 +245,8 @@ template <typename T, int CG, int BN, int BLOCK, bool PARTIAL>
 __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
     gemm4_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                  const __grid_constant__ CUtensorMap map_sa, const __grid_constant__ CUtensorMap map_sb,
-                 const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_residual, const Gemm4Args p) {
+                 const __grid_constant__ CUtensorMap map_out, const __grid_constant__ CUtensorMap map_residual,
+                 const __grid_constant__ CUtensorMap map_ahead, const Gemm4Args p) {
     using S = Shape4<CG, BN, BLOCK>;
     const int stage_count = p.stages;
     extern __shared__ char raw[];
@@ -431,8 +433,8 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
             }
         }
     } else if (warp == 3) {
-        // One tile ahead of the epilogue, whose warps would each wait for these loads, and walk, between two tiles (a third
-        // of its time).
+        // Ahead of the epilogue, whose warps would each wait for these loads, and walk, between two tiles (a third of its
+        // time).  The residual is on its way from HBM to L2 meanwhile.
         int q = 0, phase = 1;
         for (int t = start; t < tiles && fine; t += step) {
             const Tile4 tile = walk.at(t);
@@ -452,6 +454,8 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
             }
             fine = __all_sync(0xffffffffu, tc::bar_wait(heard + q, phase, p.limit));
             if (!fine) break;
+            if (!PARTIAL && p.boxes_in && !tile.zero && lane < BN / AHEAD && tile.n0 + lane * AHEAD < p.n)
+                tc::tma_prefetch_2d(&map_ahead, tile.n0 + lane * AHEAD, tile.m0 + rank * 128);
             int* slot = reinterpret_cast<int*>(slots + q * S::SLOT);
             if (lane == 0) {
                 *reinterpret_cast<int4*>(slot) = make_int4(tile.g, tile.m0, tile.n0, tile.m_end);
@@ -911,6 +915,8 @@ void launch_gemm4(const Product4& x, Gemm4Args p, int64_t tiles, cudaStream_t st
         return on ? tensor_map(base, CU_TENSOR_MAP_DATA_TYPE_UINT16, S::COLS == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, 2, dy, ty, xy) : CUtensorMap{};
     };
     const CUtensorMap map_out = y_map(p.boxes, p.out), map_residual = y_map(p.boxes_in, p.residual);
+    const int xahead[] = {AHEAD, 128};
+    const CUtensorMap map_ahead = p.boxes_in ? tensor_map(p.residual, CU_TENSOR_MAP_DATA_TYPE_UINT16, CU_TENSOR_MAP_SWIZZLE_NONE, 2, dy, ty, xahead) : CUtensorMap{};
 
     const auto kernel = gemm4_kernel<T, CG, BN, BLOCK, PARTIAL>;
     ODIE_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SHARED));
@@ -928,7 +934,7 @@ void launch_gemm4(const Product4& x, Gemm4Args p, int64_t tiles, cudaStream_t st
     attributes[1].val.programmaticStreamSerializationAllowed = 1;
     config.attrs = attributes;
     config.numAttrs = 2;
-    ODIE_CUDA(cudaLaunchKernelEx(&config, kernel, map_a, map_b, map_sa, map_sb, map_out, map_residual, p));
+    ODIE_CUDA(cudaLaunchKernelEx(&config, kernel, map_a, map_b, map_sa, map_sb, map_out, map_residual, map_ahead, p));
     note_launch();
 }
 

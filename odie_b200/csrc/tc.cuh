@@ -316,6 +316,9 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const void* map, int x, i
             : "memory");
 }
 
+__device__ __forceinline__ void tma_prefetch_2d(const void* map, int x, int y) {  // to L2
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global.tile [%0, {%1, %2}];\n" ::"l"(map), "r"(x), "r"(y) : "memory");
+}
 // A TMA store of one box from shared memory, as a group of this thread's bulk copies; stores_read: their shared memory is
 // free again; stores_done: they are through.
 __device__ __forceinline__ void tma_store_2d(const void* map, int x, int y, const void* src) {
