@@ -556,7 +556,9 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
                     if (residual) finish_box<T, ACT, COLS, true>(v, row_scale, column, box, lane);
                     else finish_box<T, ACT, COLS, false>(v, row_scale, column, box, lane);
                 };
-                if (tile.zero) {
+                if (!inside) {
+                    // (a tile's rows behind its group, or columns behind the last)
+                } else if (tile.zero) {
 #pragma unroll
                     for (int u = 0; u < COLS / 8; ++u) *boxed<COLS>(box, lane, u) = make_uint4(0, 0, 0, 0);
                 } else if (p.activation == ACT_RELU) go(std::integral_constant<int, ACT_RELU>{});

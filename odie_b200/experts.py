@@ -1,13 +1,15 @@
-"""Rows of routed experts: sorted by expert and back, the experts' own linear layers, learned codes by id.
+"""Rows of routed experts: chosen, sorted by expert and back, the experts' own linear layers, learned codes by id.
 
 The routed models choose an expert for each row (`model.route`) and read that expert's table (`ExpertHashQuery`).
 The operators here give experts layers of their own: `sort_rows` orders the (row, choice) pairs by expert,
 `dispatch` copies each row to its places, `linear` multiplies every group of consecutive rows by its expert's
 matrix with bias, activation and residual in the same kernel, `combine` brings the results back as weighted sums;
-`embed` looks rows of a learned table up by id.  All of them run the kernels of libodie_b200.so on the current
+`embed` looks rows of a learned table up by id.  `gate` chooses the experts of rows from a learned router's logits, and
+`balance` says how evenly; `linear4` is `linear` for decoding, with weights that `quantize` has put into 4 bits.  All of them
+run the kernels of libodie_b200.so on the current
 stream of their tensors' device, are differentiable (once, backward; forward-mode derivatives and transforms of
-torch.func are refused) and give the same bits in every run.  `ExpertHeads`
-is the MLP of `model.Head` with one set of weights per expert, built from them.
+torch.func are refused; the 4-bit ones not at all) and give the same bits in every run.  `ExpertHeads`
+is the MLP of `model.Head` with one set of weights per expert, built from them, `ExpertRouter` a router to train with it.
 
 There is no CPU path: tensors that are not on a CUDA device are refused.
 """
@@ -21,7 +23,7 @@ from torch import nn
 from . import _lib
 
 __all__ = ['RowOrder', 'sort_rows', 'dispatch', 'combine', 'linear', 'embed', 'Gating', 'gate', 'Balance', 'balance', 'Micro', 'quantize',
-           'dequantize', 'linear4', 'check', 'ExpertHeads']
+           'dequantize', 'linear4', 'check', 'ExpertHeads', 'MicroHeads', 'ExpertRouter']
 
 SCORES = {'softmax': 0, 'sigmoid': 1}
 ACTIVATIONS = {'none': 0, 'relu': 1, 'silu': 2, 'gelu': 3}
@@ -234,3 +236,56 @@ class ExpertHeads(nn.Module):
             h = linear(h, w.to(torch.float16), b.to(torch.float16), offsets=order.offsets,
                        activation='relu' if i + 1 < len(self.weights) else 'none')
         return combine(h, order, weights)
+
+    def microscaled(self, block=16):
+        """These heads for decoding, weights in 4 bits (see quantize)."""
+        return MicroHeads(self, block)
+
+
+class MicroHeads(nn.Module):
+    """The heads of an ExpertHeads with weights in 4 bits, as they are now: `linear4` in the place of `linear`, without
+    gradients; called like ExpertHeads."""
+
+    def __init__(self, heads, block=16):
+        super().__init__()
+        with torch.no_grad():
+            self.experts = heads.experts
+            self.weights = [quantize(w, block=block) for w in heads.weights]
+            self.biases = [b.to(torch.float16) for b in heads.biases]
+            self.codes = None if heads.codes is None else heads.codes.to(torch.float16)
+
+    @torch.no_grad()
+    def forward(self, features, expert, weights=None, ids=None):
+        if (ids is None) != (self.codes is None):
+            raise ValueError('ids go with codes')
+        h = features.to(torch.float16)
+        if ids is not None:
+            h = h + embed(ids, self.codes)
+        order = sort_rows(expert, self.experts)
+        h = dispatch(h, order)
+        for i, (w, b) in enumerate(zip(self.weights, self.biases)):
+            h = linear4(h, w, b, offsets=order.offsets, activation='relu' if i + 1 < len(self.weights) else 'none')
+        return combine(h, order, weights)
+
+
+class ExpertRouter(nn.Module):
+    """A learned choice of `choices` of `experts` for each row, for ExpertHeads: bf16 logits of one linear layer (fp16
+    would lose the gradient of a mean over many rows), `gate` and `balance`.  `shift` [experts] is added to the logits for
+    the choice alone; it has no gradient, and a program may move it against the load."""
+
+    def __init__(self, n_input, experts, choices, seed, score='softmax', normalize=True, device='cuda'):
+        super().__init__()
+        if not 1 <= choices <= experts:
+            raise ValueError('choices must be 1 to experts')
+        _score(score)
+        self.choices, self.score, self.normalize = int(choices), score, bool(normalize)
+        bound = math.sqrt(6.0 / (n_input + experts))
+        weight = (torch.rand((experts, n_input), generator=torch.Generator().manual_seed(int(seed))) * 2 - 1) * bound
+        self.weight = nn.Parameter(weight.to(device))
+        self.register_buffer('shift', torch.zeros(experts, device=device))
+
+    def forward(self, features, mask=None):
+        """(Gating, Balance) of features [rows, n_input]; mask as for gate."""
+        logits = linear(features.to(torch.bfloat16), self.weight.to(torch.bfloat16))
+        routing = gate(logits, self.choices, bias=self.shift, mask=mask, score=self.score, normalize=self.normalize)
+        return routing, balance(logits, routing.expert, mask=mask, score=self.score)
