@@ -158,6 +158,52 @@ __device__ __forceinline__ void choose_sorted(uint32_t (&key)[8], int choices, i
     }
 }
 
+// And for 4 to FILTERED choices: the k-th highest of the lanes' highest keys is a bound that at least k keys reach, and few
+// more; these are gathered, and each counts those before it.  false: more than 32 reach it (many ties), choose_sorted takes
+// the row.  found: [64] of the warp.
+constexpr int FILTERED = 16;
+template <int SLOTS>
+__device__ __forceinline__ bool choose_filtered(const uint32_t (&key)[8], int choices, int lane, int (&chosen)[SLOTS], uint32_t (&won)[SLOTS],
+                                                uint32_t& most, uint2* found) {
+    uint32_t high = key[0], bound = 0;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) high = max(high, key[i]);
+    for (int t = 0; t < choices; ++t) {  // lanes with one and the same key leave together: the bound is lower then
+        bound = __reduce_max_sync(0xffffffffu, high);
+        if (t == 0) most = bound;
+        if (high == bound) high = 0;
+    }
+    bound = max(bound, NO_KEY + 1);
+    const uint32_t before = (1u << lane) - 1;
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t reach = __ballot_sync(0xffffffffu, key[i] >= bound);
+        const int at = count + __popc(reach & before);
+        if (key[i] >= bound && at < 32) found[at] = make_uint2(key[i], lane * 8 + i);
+        count += __popc(reach);
+    }
+    if (count > 32) return false;
+    __syncwarp();
+    const uint2 mine = lane < count ? found[lane] : make_uint2(0, 0);
+    int rank = 0;
+    for (int i = 0; i < count; ++i) {
+        const uint2 other = found[i];
+        rank += other.x > mine.x || (other.x == mine.x && other.y < mine.y);
+    }
+    if (lane < count && rank < choices) found[32 + rank] = mine;
+    __syncwarp();
+    chosen[0] = -1;
+    won[0] = NO_KEY;
+    if (lane < min(count, choices)) {
+        const uint2 taken = found[32 + lane];
+        chosen[0] = int(taken.y);
+        won[0] = taken.x;
+    }
+    __syncwarp();  // found is free again
+    return true;
+}
+
 // As few slots as hold the choices are compiled for: never more than V, nor than hold 64.
 template <typename T, int V, int LANES, int SLOTS>
 __global__ void __launch_bounds__(LOGIT_THREADS) gate_kernel(GateArgs a, LogitShape s) {
@@ -193,7 +239,10 @@ __global__ void __launch_bounds__(LOGIT_THREADS) gate_kernel(GateArgs a, LogitSh
     int chosen[SLOTS];
     uint32_t won[SLOTS];  // their keys
     if constexpr (LANES == 32 && V == 8) {
-        if (a.choices > 3) choose_sorted<SLOTS>(key, a.choices, lane, chosen, won, most);
+        __shared__ uint2 found[LOGIT_THREADS / 32][64];
+        if (SLOTS == 1 && a.choices > 3 && a.choices <= FILTERED &&
+            choose_filtered<SLOTS>(key, a.choices, lane, chosen, won, most, found[threadIdx.x / 32])) {
+        } else if (a.choices > 3) choose_sorted<SLOTS>(key, a.choices, lane, chosen, won, most);
         else choose<V, LANES, SLOTS>(key, a.choices, lane, chosen, won, most);
     } else {
         choose<V, LANES, SLOTS>(key, a.choices, lane, chosen, won, most);

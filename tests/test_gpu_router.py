@@ -8,7 +8,7 @@ from rows_cases import TYPES, within
 pytestmark = pytest.mark.gpu
 
 # rows, experts, choices
-SIZES = [(1, 1, 1), (1, 64, 2), (3, 7, 7), (33, 8, 3), (257, 9, 2), (1000, 16, 1), (130, 37, 5), (65, 64, 64), (129, 100, 8), (77, 256, 8),
+SIZES = [(1, 1, 1), (1, 64, 2), (3, 7, 7), (33, 8, 3), (257, 9, 2), (1000, 16, 1), (130, 37, 5), (65, 64, 64), (129, 100, 8), (77, 256, 8), (500, 200, 16), (300, 256, 4), (64, 130, 5),
          (50, 257, 4), (31, 512, 64), (9, 1000, 10), (17, 1024, 64), (5003, 16, 4)]
 
 
