@@ -652,21 +652,6 @@ constexpr int FEW4_ROWS = 4, FEW4_VALUES = 1024, FEW4_SHARED = 96 * 1024;
 template <int M>
 constexpr int FEW4_THREADS = M <= 2 ? 1024 : 512;
 
-// Eight codes as four pairs of fp16.
-__device__ __forceinline__ void halves_of(uint32_t codes, __half2 (&h)[8], int first) {
-    uint32_t r[4];
-    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
-        "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\tcvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-        : "r"(codes));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) h[first + i] = *reinterpret_cast<const __half2*>(&r[i]);
-}
-template <int BLOCK>
-__device__ __forceinline__ float scale_value(uint32_t byte) {
-    return BLOCK == 16 ? e4m3_value(byte) : byte ? __uint_as_float(byte << 23) : 0x1p-127f;
-}
-
 template <typename T, int M, int BLOCK>
 __global__ void __launch_bounds__(FEW4_THREADS<M>) few4_kernel(Few4Args a) {
     constexpr int WARPS = FEW4_THREADS<M> / 32;
@@ -774,15 +759,15 @@ __global__ void __launch_bounds__(FEW4_THREADS<M>) few4_kernel(Few4Args a) {
 #pragma unroll
             for (int m = 0; m < M; ++m) {
                 const uint2 codes = *reinterpret_cast<const uint2*>(x_codes + m * a.pitch + c / 2 + b * 8);
-                halves_of(codes.x, x[m], 0);
-                halves_of(codes.y, x[m], 4);
+                halves_of(codes.x, x[m]);
+                halves_of(codes.y, x[m] + 4);
                 by[m] = x_scales[m * per_row + (BLOCK == 16 ? c / 16 + b : c / 32)];
             }
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 __half2 h[8];
-                halves_of(words[q][2 * b], h, 0);
-                halves_of(words[q][2 * b + 1], h, 4);
+                halves_of(words[q][2 * b], h);
+                halves_of(words[q][2 * b + 1], h + 4);
                 const uint32_t at = BLOCK == 16 ? (c / 16 + b) % 4 : c / 32 % 4;
                 const float scale = scale_value<BLOCK>(bytes[q] >> (at * 8) & 0xffu);
 #pragma unroll

@@ -157,13 +157,17 @@ __global__ void __launch_bounds__(MICRO_THREADS) values_kernel(ValuesArgs a, int
             const uint32_t block = c / BLOCK;
             const uint32_t scale = __ldg(scales + block / 4 * MICRO_TILE + block % 4);  // (at most 2^16 x 512 bytes)
             const uint32_t codes = N == 8 ? __ldg(reinterpret_cast<const uint32_t*>(codes_at + c / 2)) : uint32_t(__ldg(reinterpret_cast<const uint16_t*>(codes_at + c / 2)));
-            // both exact, and their product too: six bits
-            const Pair by = same((BLOCK == 16 ? e4m3_value(scale) : scale ? __uint_as_float(scale << 23) : 0x1p-127f) * row_scale);
+            const Pair by = same(scale_value<BLOCK>(scale) * row_scale);  // exact, and so are the values: six bits
+            __half2 halves[4];
+            if constexpr (N == 8) {
+                halves_of(codes, halves);
+            } else {
+                halves[0] = halves_of(codes);
+                halves[1] = halves_of(codes >> 8);
+            }
 #pragma unroll
             for (int e = 0; e < N / 2; ++e) {
-                uint32_t halves;
-                asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\t}" : "=r"(halves) : "r"(codes >> (e * 8)));
-                const float2 m = __half22float2(*reinterpret_cast<const __half2*>(&halves)), v = both(mul2(pair(m.x, m.y), by));
+                const float2 m = __half22float2(halves[e]), v = both(mul2(pair(m.x, m.y), by));
                 if constexpr (sizeof(T) == 4) {
                     words[2 * e] = __float_as_uint(v.x);
                     words[2 * e + 1] = __float_as_uint(v.y);

@@ -76,6 +76,27 @@ __device__ __forceinline__ uint32_t codes_of(const float2 (&q)[4]) {
 }
 __device__ __forceinline__ float e4m3_value(uint32_t byte) { return __half2float(__half(__nv_cvt_fp8_to_halfraw(uint8_t(byte), __NV_E4M3))); }
 
+// Two codes, in the lowest byte, as a pair of fp16; eight as four pairs.  (Not for words whose upper half the compiler knows to
+// be zero: nvcc 12.9 made all four pairs zero then.)
+__device__ __forceinline__ __half2 halves_of(uint32_t codes) {
+    uint32_t r;
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %1;\n\tcvt.rn.f16x2.e2m1x2 %0, a;\n\t}" : "=r"(r) : "r"(codes));
+    return *reinterpret_cast<const __half2*>(&r);
+}
+__device__ __forceinline__ void halves_of(uint32_t codes, __half2* h) {
+    uint32_t r[4];
+    asm("{\n\t.reg .b8 a, b, c, d;\n\tmov.b32 {a, b, c, d}, %4;\n\t"
+        "cvt.rn.f16x2.e2m1x2 %0, a;\n\tcvt.rn.f16x2.e2m1x2 %1, b;\n\tcvt.rn.f16x2.e2m1x2 %2, c;\n\tcvt.rn.f16x2.e2m1x2 %3, d;\n\t}"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+        : "r"(codes));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = *reinterpret_cast<const __half2*>(&r[i]);
+}
+template <int BLOCK>
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+    return BLOCK == 16 ? e4m3_value(byte) : byte ? __uint_as_float(byte << 23) : 0x1p-127f;
+}
+
 // Where N values of each thread of a row are exchanged, one word per row of N beyond them: no two in one bank.  value(i): the
 // thread's i-th of its N neighbours' in a row; strided(i): the one that is i x lanes behind its lane's (lanes a multiple of N).
 template <int N>
