@@ -283,7 +283,11 @@ __global__ void __launch_bounds__(LOGIT_THREADS) balance_backward_kernel(Balance
 
 constexpr int SMS = 148;  // of a B200: the sizes of scratch must not depend on the device that asks
 
-int64_t balance_blocks(int64_t rows, int experts) { return std::min<int64_t>(logit_blocks(rows, experts), SMS * 4); }
+// Four blocks to an SM, and no more than 256 rows to a thread: its fp32 sums stay within 2^-16 of themselves.
+int64_t balance_blocks(int64_t rows, int experts) {
+    const int64_t blocks = logit_blocks(rows, experts);
+    return std::min(blocks, std::max<int64_t>(SMS * 4, (blocks + 255) / 256));
+}
 
 template <typename F>
 void with_balance(int dtype, int experts, int score, F&& f) {

@@ -126,7 +126,7 @@ def test_linear4_refuses(lib, change, message):
 
 def test_scratch_sizes(lib):
     assert lib.odie_balance_scratch(0, 8) == 0 and lib.odie_balance_scratch(-1, 8) == 0 and lib.odie_balance_scratch(8, 1025) == 0
-    assert 0 < lib.odie_balance_scratch(1, 8) <= lib.odie_balance_scratch(1 << 20, 8) == lib.odie_balance_scratch(2 ** 31 - 1, 8)
+    assert 0 < lib.odie_balance_scratch(1, 8) <= lib.odie_balance_scratch(1 << 20, 8) <= lib.odie_balance_scratch(2 ** 31 - 1, 8) < 1 << 22
     for block in (16, 32):
         for offsets in (0, 1):  # codes, scales and row scales of the rows, at least
             for rows, inputs in ((1, 1), (129, 333), (4096, 1024)):
