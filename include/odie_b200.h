@@ -463,7 +463,7 @@ ODIE_API int odie_embed_backward(const void* ids, int id_bytes, int64_t n, const
  * NULL; NaN above all, -inf is not taken), ties to the lowest; -1 with weight
  * 0 where none is left.  weights: scale times the score (the bias is not in
  * it), with normalize divided by the sum over the row's choices.  Up to 64
- * choices, scale finite and not 0.
+ * choices, scale a normal fp32 number.
  * odie_gate_backward: d_logits[rows][experts] for d_weights
  * f32[rows][choices], from odie_gate's results and its logits and mask
  * (neither is read for a normalised softmax, the mask for no sigmoid).

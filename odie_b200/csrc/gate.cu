@@ -371,7 +371,7 @@ void check_gate(int64_t rows, int experts, int choices, int dtype, int score, fl
     check_logits(rows, experts, dtype, score);
     ODIE_REQUIRE(choices >= 1 && choices <= experts && choices <= MAX_CHOICES, "1 to 64 choices, no more than experts");
     ODIE_REQUIRE(rows * choices < (int64_t(1) << 31), "too many (row, choice) pairs");
-    ODIE_REQUIRE(std::isfinite(scale) && scale != 0.0f, "scale must be finite and not 0");
+    ODIE_REQUIRE(std::isnormal(scale), "scale must be finite and not 0");  // (nor below the least normal number: its inverse is used)
 }
 
 }  // namespace

@@ -165,7 +165,8 @@ __device__ __forceinline__ void move_box(uint16_t* at, char* box, int ld, int ro
     }
 }
 
-// y = act((v r) c + b) (+ residual, in the box), rounded into the box.  A thread has the columns 8 u + 2 (lane % 4) + 0, 1 of
+// y = act(v (r c) + b) (+ residual, in the box), rounded into the box; r c is a power of two, exact unless it leaves fp32's range,
+// which v r alone may do where the result does not.  A thread has the columns 8 u + 2 (lane % 4) + 0, 1 of
 // rows 8 j + lane / 4, as tcgen05.ld 16x256b and the 8 x 8 matrices of ldmatrix and stmatrix have them: c and b are read
 // once for four rows.  (With a row to a thread, every thread read every column's: the shared memory was busy with that for
 // longer than with the products.)  columns: c and b of two columns side by side.
@@ -231,7 +232,7 @@ __device__ __forceinline__ void join_parts(const Gemm4Args& p, const Tile4& tile
         for (int e = 0; e < 4; ++e) {
             if (c + e >= columns) continue;
             const int n = tile.n0 + c + e;
-            float y = zs[e] * by * __ldg(p.column_scales + n);
+            float y = zs[e] * (by * __ldg(p.column_scales + n));
             if (p.bias) y += to_float(static_cast<const T*>(p.bias)[n]);
             const Pair added = same(p.residual ? to_float(static_cast<const T*>(p.residual)[at + e]) : 0.0f);
             static_cast<T*>(p.out)[at + e] = from_float<T>(activated(p.activation, y, added));
@@ -800,7 +801,7 @@ __global__ void __launch_bounds__(FEW4_THREADS<M>) few4_kernel(Few4Args a) {
 #pragma unroll
         for (int r = 0; r < M; ++r)
             if (r == m) scale = row_scale[r];
-        z = z * scale * __ldg(a.row_scales + n);
+        z = z * (scale * __ldg(a.row_scales + n));
         if (a.bias) z += to_float(static_cast<const T*>(a.bias)[n]);
         const long long at = (long long)m * a.outputs + n;
         const Pair added = same(a.residual ? to_float(static_cast<const T*>(a.residual)[at]) : 0.0f);

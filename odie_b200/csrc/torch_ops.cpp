@@ -460,7 +460,7 @@ std::tuple<Tensor, Tensor> gate(const Tensor& logits, int64_t choices, const May
     check_logits(logits);
     TORCH_CHECK_VALUE(choices >= 1 && choices <= 64 && choices <= logits.size(1), "choices must be 1 to 64 and no more than the experts");
     TORCH_CHECK_VALUE(logits.size(0) * choices < (int64_t(1) << 31), "too many (row, choice) pairs");
-    TORCH_CHECK_VALUE(std::isfinite(float(scale)) && float(scale) != 0.0f, "scale must be finite and not 0");
+    TORCH_CHECK_VALUE(std::isnormal(float(scale)), "scale must be finite and not 0");
     refuse_tangents(logits);
     Tensor shift;
     if (bias) {

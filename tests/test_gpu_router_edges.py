@@ -240,3 +240,19 @@ def test_quantize_the_longest_rows(cuda, dtype, block):
     for width in (1 << 20, (1 << 20) - 5):
         x = torch.randn((3, width), generator=generator(5), device='cuda').to(dtype)
         assert torch.equal(dequantize(quantize(x, block=block)).double(), plain_micro(x, block)[0])
+
+
+@pytest.mark.parametrize('up, down', [(100, -100), (-60, -50), (60, -110), (-110, 100), (110, -125)])
+@pytest.mark.parametrize('rows, inputs, outputs', [(1, 300, 40), (3, 64, 200), (50, 2048, 130), (300, 256, 700)])
+@pytest.mark.parametrize('block', [16, 32])
+def test_linear4_of_far_rows_and_weights(cuda, up, down, rows, inputs, outputs, block):
+    """Rows and weights of sizes whose product is far from either: no step on the way leaves the range that the result is in."""
+    from odie_b200.experts import linear4, quantize
+    g = generator(rows)
+    x, weight = torch.randn((rows, inputs), generator=g, device='cuda'), torch.randn((outputs, inputs), generator=g, device='cuda')
+    x, weight = (x.double() * 2.0 ** up).bfloat16(), (weight.double() * 2.0 ** down).bfloat16()
+    y = linear4(x, quantize(weight, block=block))
+    q, w = plain_micro(x, block)[0], plain_micro(weight, block)[0]
+    want = q @ w.t()
+    bound = (inputs + 1) * 2.0 ** -23 * (q.abs() @ w.abs().t()) + 3 * 2.0 ** -24 * want.abs()
+    within(y, want, bound + 2.0 ** -8 * (want.abs() + bound) + 2.0 ** -134, 'y')

@@ -44,7 +44,7 @@ NAN, INF = float('nan'), float('inf')
 LOGITS = [(dict(rows=-1), 'rows'), (dict(rows=2 ** 31), 'rows'), (dict(experts=0), 'experts'), (dict(experts=1025), 'experts'),
           (dict(dtype=3), 'element type'), (dict(score=2), 'score'), (dict(score=-1), 'score')]
 GATE = LOGITS + [(dict(choices=0), 'choices'), (dict(choices=9), 'choices'), (dict(experts=100, choices=65), 'choices'),
-                 (dict(rows=2 ** 30, choices=2), 'pairs'), (dict(scale=0.0), 'scale'), (dict(scale=NAN), 'scale'), (dict(scale=INF), 'scale'),
+                 (dict(rows=2 ** 30, choices=2), 'pairs'), (dict(scale=0.0), 'scale'), (dict(scale=NAN), 'scale'), (dict(scale=INF), 'scale'), (dict(scale=1e-40), 'scale'),
                  (dict(expert=None), 'required'), (dict(weights=None), 'required')]
 
 
