@@ -631,10 +631,11 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
 }
 
 // ---------------------------------------------------------------- a few rows
-// One kernel for up to four rows: bound by the bytes of W and by what one launch takes.  A warp has the rows n, n + 32, n + 64
-// and n + 96 of a tile of W, whose scales lie side by side, and every `splits`-th 1024 values of K; the first of them are on
-// their way while the block quantises x into shared memory.  Products of codes are multiples of 1/4 of at most 36, and eight of
-// them add up exactly in fp16: a block of 16 takes eight packed products and one fp32 step with its scales.
+// One kernel for one or two rows (four rows of 4096 -> 4096 took it 14.5 us, the tiles 9.8; two 8.5): bound by the bytes of W
+// and by what one launch takes.  A warp has the rows n, n + 32, n + 64 and n + 96 of a tile of W, whose scales lie side by
+// side, and every `splits`-th 1024 values of K; the first of them are on their way while the block quantises x into shared
+// memory.  Products of codes are multiples of 1/4 of at most 36, and eight of them add up exactly in fp16: a block of 16 takes
+// eight packed products and one fp32 step with its scales.
 struct Few4Args {
     const void* x;
     const uint8_t* codes;
@@ -649,13 +650,12 @@ struct Few4Args {
     int wide;                 // x starts on a 16-byte boundary, and so do its rows
 };
 
-constexpr int FEW4_ROWS = 4, FEW4_VALUES = 1024, FEW4_SHARED = 96 * 1024;
-template <int M>
-constexpr int FEW4_THREADS = M <= 2 ? 1024 : 512;
+constexpr int FEW4_ROWS = 2, FEW4_VALUES = 1024, FEW4_SHARED = 96 * 1024;
+constexpr int FEW4_THREADS = 1024;
 
 template <typename T, int M, int BLOCK>
-__global__ void __launch_bounds__(FEW4_THREADS<M>) few4_kernel(Few4Args a) {
-    constexpr int WARPS = FEW4_THREADS<M> / 32;
+__global__ void __launch_bounds__(FEW4_THREADS) few4_kernel(Few4Args a) {
+    constexpr int WARPS = FEW4_THREADS / 32;
     extern __shared__ char raw[];
     uint8_t* const shared = reinterpret_cast<uint8_t*>(raw);
     __shared__ uint32_t tops[WARPS][M];
@@ -823,14 +823,15 @@ bool pair_tiles(int64_t rows, int n, int groups) {
     return double(ceil_div(std::max<int64_t>(1, pairs), SMS / 2)) * 256 <= double(ceil_div(std::max<int64_t>(1, ones), SMS)) * 128 * 1.35;
 }
 
-// Without offsets, where 128 x 128 tiles leave SMs idle: the sum over K is cut into as many parts as there are SMs for.
+// Without offsets, where 128 x 128 tiles leave SMs idle: the sum over K is cut into 2, 4 or 8 parts of at least four blocks.
 struct Splits4 {
     int parts, blocks;  // blocks of K per part
     Splits4(int64_t rows, int n, int k, int groups, bool offsets) : parts(1), blocks(int(ceil_div(k, BK))) {
         if (rows == 0 || offsets || pair_tiles(rows, n, groups)) return;
-        const int64_t tiles = ceil_div(rows, 128) * ceil_div(n, 128), wanted = std::min<int64_t>({128 / tiles, blocks / 2, 8});  // (clusters of 8 CTAs do not fill every SM)
-        if (wanted < 2) return;
-        blocks = int(ceil_div(blocks, wanted));
+        const int64_t tiles = ceil_div(rows, 128) * ceil_div(n, 128), most = std::min<int64_t>(tiles <= 8 ? 8 : tiles <= 32 ? 4 : tiles <= 64 ? 2 : 1, blocks / 4);
+        if (most < 2) return;
+        parts = most >= 8 ? 8 : most >= 4 ? 4 : 2;
+        blocks = int(ceil_div(blocks, parts));
         parts = int(ceil_div(ceil_div(k, BK), blocks));
     }
 };
@@ -945,8 +946,8 @@ void launch_product4(const Product4& x, Gemm4Args p, const Splits4& split, cudaS
 
 // Whether few4_kernel takes the call: its rows of x have to fit the shared memory.
 int64_t few4_shared(int64_t rows, int64_t inputs, int block) {
-    const int64_t m = rows <= 1 ? 1 : rows <= 2 ? 2 : 4, pitch = micro_pitch(inputs);
-    return m * (pitch + pitch / 8 * (block == 16 ? 4 : 2));
+    const int64_t pitch = micro_pitch(inputs);
+    return std::max<int64_t>(1, rows) * (pitch + pitch / 8 * (block == 16 ? 4 : 2));
 }
 bool few4(int64_t rows, int64_t inputs, bool offsets, int block) {
     return rows <= FEW4_ROWS && !offsets && few4_shared(rows, inputs, block) <= FEW4_SHARED;
@@ -959,7 +960,7 @@ void launch_few4(Few4Args a, cudaStream_t stream) {
     a.wide = (uintptr_t(a.x) | uintptr_t(a.inputs * 2)) % 16 == 0;
     const int shared = int(few4_shared(a.rows, a.inputs, BLOCK));
     auto go = [&](auto rows) {
-        constexpr int M = decltype(rows)::value, WARPS = FEW4_THREADS<M> / 32;
+        constexpr int M = decltype(rows)::value, WARPS = FEW4_THREADS / 32;
         const int64_t quads = ceil_div(a.outputs, MICRO_ROWS) * 32, chunks = ceil_div(a.inputs, FEW4_VALUES);
         // as many warps to a sum as it has chunks, up to eight, and as many sums to a block as fill the SMs once
         a.splits = int(std::min<int64_t>(chunks, 8));
@@ -972,8 +973,7 @@ void launch_few4(Few4Args a, cudaStream_t stream) {
         note_launch();
     };
     if (a.rows == 1) go(std::integral_constant<int, 1>{});
-    else if (a.rows == 2) go(std::integral_constant<int, 2>{});
-    else go(std::integral_constant<int, 4>{});
+    else go(std::integral_constant<int, 2>{});
 }
 
 bool sizes4_fit(int64_t rows, int64_t inputs, int64_t outputs, int64_t groups, int block) {
