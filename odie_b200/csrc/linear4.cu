@@ -815,15 +815,20 @@ constexpr int SMS = 148;  // of a B200: the sizes of scratch must not depend on 
 int64_t aligned(int64_t bytes) { return (bytes + 255) / 256 * 256; }
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// 256 x 256 tiles by pairs, or 128 x 128 by one CTA where those leave SMs idle.
+// 256 x 256 tiles by pairs, or 128 x 128 by one CTA where those leave SMs idle: by the waves either takes, in columns, a
+// column of the smaller ones for 1.35.  (8192 rows of 4096 -> 4096: 74 us by pairs, 91 by ones; 1024 of 1024 -> 1024: 9.6 and
+// 7.9.  Over 128 to 8192 rows, 512 to 8192 outputs, 1024 and 4096 inputs the choice is within 8 % of the better one.  512 rows
+// in 32 groups, 1024 -> 2048: 20 us by pairs, 17 by ones.)
 bool pair_tiles(int64_t rows, int n, int groups) {
-    if (n <= 128) return false;
+    if (n <= 128 || (groups > 1 && rows < groups * int64_t(128))) return false;
     const int64_t pairs = (groups > 1 ? rows / 256 + (groups + 1) / 2 : ceil_div(rows, 256)) * ceil_div(n, 256);
     const int64_t ones = (groups > 1 ? rows / 128 + (groups + 1) / 2 : ceil_div(rows, 128)) * ceil_div(n, 128);
     return double(ceil_div(std::max<int64_t>(1, pairs), SMS / 2)) * 256 <= double(ceil_div(std::max<int64_t>(1, ones), SMS)) * 128 * 1.35;
 }
 
 // Without offsets, where 128 x 128 tiles leave SMs idle: the sum over K is cut into 2, 4 or 8 parts of at least four blocks.
+// (512 rows of 1024 -> 2048 in two parts of two blocks: 11.7 us, whole 7.7.  256 rows of 8192 -> 1024 in eight parts, for all
+// of whose clusters there is not room at a time: 20.5 us, in four 13.5.  64 rows of 4096 -> 4096: 10.6 us in four parts.)
 struct Splits4 {
     int parts, blocks;  // blocks of K per part
     Splits4(int64_t rows, int n, int k, int groups, bool offsets) : parts(1), blocks(int(ceil_div(k, BK))) {

@@ -1,18 +1,19 @@
 // Rows as microscaled 4-bit floats and back (micro.cuh has the format).
 //
-// Bound by HBM.  A thread takes 16 values at a time, a row is 8 to 256 threads of a block, whose values stay in
-// registers between the row's maximum and the rounding (up to 64 per thread; longer rows are read again from L2).  Rows
-// that do not start on 16-byte boundaries are moved element by element, neighbours by neighbouring threads, through
-// shared memory.
+// Bound by its instructions, 9 to 12 to a value, next to HBM (16384 x 2048 bf16: 18.5 us to 4 bits, 4.6 TB/s, and 16.5 back,
+// 5.1 TB/s).  A thread takes 16 values at a time, a row is 4 to 256 threads of a block, whose values stay in registers
+// between the row's maximum and the rounding (up to 64 per thread; longer rows are read again from L2).  Rows that do not
+// start on 16-byte boundaries are moved element by element, neighbours by neighbouring threads, through shared memory.
 //
 // Roundings are exact: a quotient next to a border between two codes decides by a whole step.  x / R is exact.  For
 // 16-bit x, q = x / (R s) is x times an approximate inverse of s, within 2^-22 of the quotient, rounded to a multiple of
 // 2^-17 (by adding 96 in the same fused step): a quotient of an 11-bit x that is not itself on a border (a number of
 // three bits, times the four of s) is at least 2^-13 away from it, so that the rounded q is on the border where the
 // quotient is, and on the quotient's side of it else.  Their scales likewise, rounded to 16 bits: a border of e4m3 is a
-// number of five bits, times 6.  fp32 x and its scales take a division whose remainder, where it is not zero, goes into the
-// last bit (rounding to odd: Boldo and Melquiond, "Emulation of FMA and correctly rounded sums", 2008), which makes the
-// second rounding right.
+// number of five bits, times 6.  fp32 x may be closer to a border: q is as above, and 2^-18 to the side that the sign of
+// x / R - q s, one fused step, says, so that it is on the border for a quotient that is.  The scales of fp32 rows take a division
+// whose remainder, where it is not zero, goes into the last bit (rounding to odd: Boldo and Melquiond, "Emulation of FMA and
+// correctly rounded sums", 2008), which makes the second rounding right.
 #include "micro.cuh"
 #include "odie_b200.h"
 #include <algorithm>
@@ -196,7 +197,8 @@ __global__ void __launch_bounds__(MICRO_THREADS) values_kernel(ValuesArgs a, int
 }
 
 // The threads of a row, as a power of two of at least 2^least: as few as take it in `runs` runs of n values each; more, up
-// to one run each, where the rows leave threads idle (four blocks to an SM).
+// to one run each, where the rows leave threads idle (four blocks to an SM; 64 x 4096 bf16 to 4 bits:
+// 2.5 us, with the fewest threads 3.2).
 int row_lanes(int64_t rows, int64_t width, int n, int runs, int least) {
     int log2 = least;
     while (log2 < 8 && (int64_t(n) * runs << log2) < width) ++log2;
@@ -231,7 +233,7 @@ void check_micro(int64_t groups, int64_t rows, int64_t width, int dtype, int blo
 
 void launch_quantize(MicroArgs a, int dtype, int block, cudaStream_t stream) {
     const bool whole = wide_rows(a.x, a.width, dtype);
-    const int log2 = row_lanes(a.rows, a.width, 16, HELD, whole ? 3 : 4);
+    const int log2 = row_lanes(a.rows, a.width, 16, HELD, whole ? (block == 16 ? 2 : 3) : 4);  // (at least the threads of four scales)
     a.first_blocks = MICRO_ROWS / (MICRO_THREADS >> log2);
     const int64_t tiles = a.offsets ? micro_tiles(a.rows, a.groups) : a.groups * ((a.group_rows + MICRO_ROWS - 1) / MICRO_ROWS);
     ODIE_REQUIRE(tiles * a.first_blocks < (int64_t(1) << 31), "too many rows for one launch");

@@ -206,14 +206,16 @@ __device__ __forceinline__ uint2 round_run(const Run<T>& x, uint32_t largest, fl
         }
     } else {
         scale = __nv_cvt_float_to_fp8(divide_odd(__uint_as_float(largest) * inverse_row, 6.0f), __NV_SATFINITE, __NV_E4M3);
-        const float divisor = scale ? e4m3_value(scale) : INFINITY;
+        const float divisor = e4m3_value(scale);
+        const Pair by = same(scale ? inverse_approx(divisor) : 0.0f), first = same(inverse_row), up = same(96.0f), down = same(-96.0f);
+        auto side = [](float rest) { return fminf(fmaxf(rest * 0x1p100f, -0x1p-18f), 0x1p-18f); };
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float2 v = x.pair_at(i);
-            q[i].x = copysignf(divide_odd(fabsf(v.x) * inverse_row, divisor), v.x);
-            q[i].y = copysignf(divide_odd(fabsf(v.y) * inverse_row, divisor), v.y);
+            const Pair y = mul2(pair(v.x, v.y), first), near = add2(fma2(y, by, up), down);
+            const float2 rest = both(fma2(mul2(near, same(-1.0f)), same(divisor), y));
+            q[i] = both(add2(near, pair(side(rest.x), side(rest.y))));
         }
-        if (!scale) return make_uint2(0, 0);
     }
     const float2 low[4] = {q[0], q[1], q[2], q[3]}, high[4] = {q[4], q[5], q[6], q[7]};
     return make_uint2(codes_of(low), codes_of(high));
