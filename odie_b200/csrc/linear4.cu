@@ -36,6 +36,7 @@ struct Gemm4Args {
     int k;               // inputs
     int a_rows;          // rows of A's boxes: 128 or, for fewer rows in all, those (rounded up to 8)
     int a_tiles;         // tiles of A's scales that there are
+    int most_tiles;      // of the result, with offsets in order: less than 2^30
     int chunk, splits;   // without offsets: the sum over K cut among the CTAs of a cluster, `chunk` blocks each
     Divide by_bands;     // tiles of a full band
     const float* row_scales;     // [rows]
@@ -294,10 +295,13 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
     }
     if (warp == 2) tc::tmem_alloc_group<CG>(tmem_at, S::COLUMNS);
     if (warp == 3) {  // the groups' rows, tiles and tiles of scales
+        // The sums stop at what offsets in order can come to: others (overlapping groups) would pass 32 bits, and a tile's first
+        // row would be negative.
         int tiles = 0, units = 0;
+        const int most_units = p.a_tiles;
         for (int g0 = 0; g0 <= p.groups; g0 += 32) {
             const int g = g0 + lane;
-            int count = 0, unit = 0;
+            int sum = 0, unit_sum = 0;
             if (g <= p.groups) {
                 long long from = 0, to = 0;
                 if (g < p.groups) {
@@ -308,24 +312,25 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
                     to = p.rows;
                 }
                 begin[g] = int(from);
-                count = int((to - from + S::TM - 1) / S::TM) * nt;
-                unit = int((to - from + MICRO_ROWS - 1) / MICRO_ROWS);
+                sum = int((to - from + S::TM - 1) / S::TM) * nt;
+                unit_sum = int((to - from + MICRO_ROWS - 1) / MICRO_ROWS);
             }
-            int sum = count, unit_sum = unit;
 #pragma unroll
             for (int d = 1; d < 32; d *= 2) {
                 const int other = __shfl_up_sync(0xffffffffu, sum, d), other_unit = __shfl_up_sync(0xffffffffu, unit_sum, d);
                 if (lane >= d) {
-                    sum += other;
-                    unit_sum += other_unit;
+                    sum = min(sum + other, p.most_tiles);
+                    unit_sum = min(unit_sum + other_unit, most_units);
                 }
             }
+            int before = __shfl_up_sync(0xffffffffu, sum, 1), unit_before = __shfl_up_sync(0xffffffffu, unit_sum, 1);
+            if (lane == 0) before = unit_before = 0;
             if (g <= p.groups) {
-                first[g] = tiles + sum - count;
-                scales[g] = units + unit_sum - unit;
+                first[g] = min(tiles + before, p.most_tiles);
+                scales[g] = min(units + unit_before, most_units);
             }
-            tiles += __shfl_sync(0xffffffffu, sum, 31);
-            units += __shfl_sync(0xffffffffu, unit_sum, 31);
+            tiles = min(tiles + __shfl_sync(0xffffffffu, sum, 31), p.most_tiles);
+            units = min(units + __shfl_sync(0xffffffffu, unit_sum, 31), most_units);
         }
         if (lane == 0) first[p.groups + 1] = tiles;
     }
@@ -901,6 +906,7 @@ void launch_gemm4(const Product4& x, Gemm4Args p, int64_t tiles, cudaStream_t st
     const CUtensorMap map_sb = tensor_map(x.sb, CU_TENSOR_MAP_DATA_TYPE_UINT32, CU_TENSOR_MAP_SWIZZLE_NONE, 4, dsb, tsb, xsb);
 
     p.stages = S::stages(p.groups);
+    p.most_tiles = int(tiles);
     p.boxes = p.n % 8 == 0 && uintptr_t(p.out) % 16 == 0;
     p.boxes_in = p.residual && p.n % 8 == 0 && uintptr_t(p.residual) % 16 == 0;
     const int64_t dy[] = {p.n, p.rows}, ty[] = {int64_t(p.n) * 2};

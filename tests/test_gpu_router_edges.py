@@ -256,3 +256,15 @@ def test_linear4_of_far_rows_and_weights(cuda, up, down, rows, inputs, outputs, 
     want = q @ w.t()
     bound = (inputs + 1) * 2.0 ** -23 * (q.abs() @ w.abs().t()) + 3 * 2.0 ** -24 * want.abs()
     within(y, want, bound + 2.0 ** -8 * (want.abs() + bound) + 2.0 ** -134, 'y')
+
+
+@pytest.mark.parametrize('groups', [256, 1024])
+def test_linear4_of_many_groups_with_offsets_out_of_order(cuda, groups):
+    from odie_b200.experts import linear4, quantize
+    x = torch.randn((700, 48), device='cuda').half()
+    weight = quantize(torch.randn((groups, 24, 48), device='cuda'))
+    for step in (1, 2, 3):
+        bad = torch.arange(groups + 1, dtype=torch.int32).remainder(step + 1).mul(900).sub(100).cuda()
+        assert linear4(x, weight, offsets=bad).shape == (700, 24)
+    y = linear4(x, weight, offsets=torch.full((groups + 1,), 700, dtype=torch.int32, device='cuda').mul_(torch.arange(groups + 1, device='cuda') > 0))
+    assert torch.isfinite(y).all()
