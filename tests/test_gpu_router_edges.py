@@ -258,6 +258,33 @@ def test_linear4_of_far_rows_and_weights(cuda, up, down, rows, inputs, outputs, 
     within(y, want, bound + 2.0 ** -8 * (want.abs() + bound) + 2.0 ** -134, 'y')
 
 
+@pytest.mark.parametrize('groups', [31, 32, 255, 256, 257, 1023, 1024])
+@pytest.mark.parametrize('spread', ['some empty', 'last only', 'none', 'one row each'])
+def test_linear4_of_many_groups(cuda, groups, spread):
+    """Each way of finding a tile's rows from the offsets, with rows of more than one tile and rows of no group."""
+    from odie_b200.experts import linear4, quantize
+    from test_gpu_micro import plain_linear4
+    g = generator(groups)
+    sizes = [0] * groups
+    if spread == 'some empty':
+        for i, n in ((0, 129), (groups // 3, 300), (groups - 2, 128), (groups - 1, 5)):
+            sizes[i] = n
+    elif spread == 'last only':
+        sizes[-1] = 400
+    elif spread == 'one row each':
+        sizes = [1] * groups
+    edges = [0]
+    for n in sizes:
+        edges.append(edges[-1] + n)
+    rows = edges[-1] + 140
+    x = torch.randn((rows, 48), generator=g, device='cuda').bfloat16()
+    weight = (torch.randn((groups, 24, 48), generator=g, device='cuda') / 7).bfloat16()
+    y = linear4(x, quantize(weight), offsets=torch.tensor(edges, dtype=torch.int32, device='cuda'))
+    value, bound = plain_linear4(x, weight, None, None, list(zip(edges, edges[1:])), 'none', 16)
+    within(y, value, bound, 'many groups')
+    assert (y[edges[-1]:] == 0).all()
+
+
 @pytest.mark.parametrize('groups', [256, 1024])
 def test_linear4_of_many_groups_with_offsets_out_of_order(cuda, groups):
     from odie_b200.experts import linear4, quantize
