@@ -69,8 +69,9 @@ struct Shape4 {
     static constexpr int SCALES_AT = OVERLAP ? 384 : 256;  // TMEM column of the scales, 64 per block
     static constexpr int SB_AT = COLUMN_TILES * 4;         // B's behind A's
     static constexpr int COLUMNS = 512;
-    // What the epilogue needs to know of a tile, written ahead by a warp of its own: the tile, its rows' scales, its
-    // columns' scales and bias (of two columns side by side).
+    // What the epilogue needs to know of a tile, written ahead by a warp of its own: the tile, whether it is one of zeros and
+    // whether a scale is far from 1, its rows' scales, its columns' scales (1 if one is far) and bias (of two columns side by
+    // side).
     static constexpr int SLOTS = 3, SLOT = 32 + 128 * 4 + BN * 8;
     static constexpr int HEAD = 512;  // barriers, TMEM address
     static int rest(int groups) { return 1024 + EPILOGUE_WARPS * BOX + SLOTS * SLOT + HEAD + 3 * (groups + 2) * 4; }
@@ -166,8 +167,24 @@ __device__ __forceinline__ void move_box(uint16_t* at, char* box, int ld, int ro
     }
 }
 
-// y = act(v (r c) + b) (+ residual, in the box), rounded into the box; r c is a power of two, exact unless it leaves fp32's range,
-// which v r alone may do where the result does not.  A thread has the columns 8 u + 2 (lane % 4) + 0, 1 of
+// Of a row's or column's scale (a power of two, or NaN): first second = scale, both near its root.  v r c is taken as
+// v (r1 c1) (r2 c2): sums are 0 or between 2^-20 (the least product of codes and e4m3 scales) and 2^42 (2^20 inputs), so that
+// no step leaves fp32's range but where the result does.  (v r and r c do: rows of 2^118 by weights of 2^-118, both of 2^-66.)
+struct Halves {
+    float first, second;
+};
+__device__ __forceinline__ Halves halves_of_scale(float scale) {
+    const int half = (int(__float_as_uint(scale) >> 23 & 255) - 127) >> 1;
+    return {power_of_two(half), scale * power_of_two(-half)};
+}
+// Within 2^-63 .. 2^63, or NaN.  Tiles of such rows and columns, all but strange ones, take v r c as (v r) c, which is in range
+// then, in the fused step of the bias.
+__device__ __forceinline__ bool is_near(float scale) {
+    const uint32_t e = __float_as_uint(scale) >> 23 & 255;
+    return e - 64u <= 126u || e == 255u;
+}
+
+// y = act(v r c + b) (+ residual, in the box), rounded into the box.  A thread has the columns 8 u + 2 (lane % 4) + 0, 1 of
 // rows 8 j + lane / 4, as tcgen05.ld 16x256b and the 8 x 8 matrices of ldmatrix and stmatrix have them: c and b are read
 // once for four rows.  (With a row to a thread, every thread read every column's: the shared memory was busy with that for
 // longer than with the products.)  columns: c and b of two columns side by side.
@@ -445,19 +462,25 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
         for (int t = start; t < tiles && fine; t += step) {
             const Tile4 tile = walk.at(t);
             float rows[4], columns[BN / 32], bias[BN / 32];
+            bool far = false;
             if (!PARTIAL && !tile.zero) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int row = tile.m0 + rank * 128 + i * 32 + lane;
-                    rows[i] = row < tile.m_end ? __ldg(p.row_scales + row) : 0.0f;
+                    rows[i] = row < tile.m_end ? __ldg(p.row_scales + row) : 1.0f;
+                    far |= !is_near(rows[i]);
                 }
                 const long long at = (long long)tile.g * p.n + tile.n0 + lane;
 #pragma unroll
-                for (int i = 0; i < BN / 32; ++i) columns[i] = tile.n0 + lane + i * 32 < p.n ? __ldg(p.column_scales + at + i * 32) : 0.0f;
+                for (int i = 0; i < BN / 32; ++i) {
+                    columns[i] = tile.n0 + lane + i * 32 < p.n ? __ldg(p.column_scales + at + i * 32) : 1.0f;
+                    far |= !is_near(columns[i]);
+                }
 #pragma unroll
                 for (int i = 0; i < BN / 32; ++i)
                     bias[i] = p.bias && tile.n0 + lane + i * 32 < p.n ? to_float(static_cast<const T*>(p.bias)[at + i * 32]) : 0.0f;
             }
+            far = BLOCK == 16 && __any_sync(0xffffffffu, far);  // (blocks of 32: rows and columns have 1)
             fine = __all_sync(0xffffffffu, tc::bar_wait(heard + q, phase, p.limit));
             if (!fine) break;
             if (!PARTIAL && p.boxes_in && !tile.zero && lane < BN / AHEAD && tile.n0 + lane * AHEAD < p.n)
@@ -465,7 +488,7 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
             int* slot = reinterpret_cast<int*>(slots + q * S::SLOT);
             if (lane == 0) {
                 *reinterpret_cast<int4*>(slot) = make_int4(tile.g, tile.m0, tile.n0, tile.m_end);
-                *reinterpret_cast<int4*>(slot + 4) = make_int4(tile.zero, 0, 0, 0);
+                *reinterpret_cast<int4*>(slot + 4) = make_int4(tile.zero, far, 0, 0);
             }
             if (!PARTIAL && !tile.zero) {
                 float* to = reinterpret_cast<float*>(slot + 8);
@@ -474,7 +497,7 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
                 to += 128 + lane / 2 * 4 + lane % 2;
 #pragma unroll
                 for (int i = 0; i < BN / 32; ++i) {
-                    to[i * 64] = columns[i];
+                    to[i * 64] = far ? 1.0f : columns[i];
                     to[i * 64 + 2] = bias[i];
                 }
             }
@@ -556,6 +579,23 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
                     if (!fine) break;
                     phase ^= 1;
                     asked = false;
+                }
+                if (BLOCK == 16 && uniform(second_word.y)) {  // far scales: the slot's columns have 1; a lane holds that of every 32nd
+                    float by[COLS / 32];
+#pragma unroll
+                    for (int i = 0; i < COLS / 32; ++i)
+                        by[i] = i * 32 + lane < columns ? __ldg(p.column_scales + (long long)tile.g * p.n + column0 + i * 32 + lane) : 1.0f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const Halves r = halves_of_scale(row_scale[j]);
+#pragma unroll
+                        for (int i = 0; i < COLS / 4; ++i) {
+                            const Halves c = halves_of_scale(__shfl_sync(0xffffffffu, by[i / 8], i / 2 % 4 * 8 + (lane & 3) * 2 + i % 2));
+                            float& z = v[j / 2][i / 2 * 4 + j % 2 * 2 + i % 2];
+                            z = z * (r.first * c.first) * (r.second * c.second);
+                        }
+                        row_scale[j] = 1.0f;
+                    }
                 }
                 auto go = [&](auto act) {
                     constexpr int ACT = decltype(act)::value;
