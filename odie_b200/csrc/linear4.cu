@@ -177,6 +177,10 @@ __device__ __forceinline__ Halves halves_of_scale(float scale) {
     const int half = (int(__float_as_uint(scale) >> 23 & 255) - 127) >> 1;
     return {power_of_two(half), scale * power_of_two(-half)};
 }
+__device__ __forceinline__ float scaled(float v, float r, float c) {
+    const Halves row = halves_of_scale(r), column = halves_of_scale(c);
+    return v * (row.first * column.first) * (row.second * column.second);
+}
 // Within 2^-63 .. 2^63, or NaN.  Tiles of such rows and columns, all but strange ones, take v r c as (v r) c, which is in range
 // then, in the fused step of the bias.
 __device__ __forceinline__ bool is_near(float scale) {
@@ -250,7 +254,7 @@ __device__ __forceinline__ void join_parts(const Gemm4Args& p, const Tile4& tile
         for (int e = 0; e < 4; ++e) {
             if (c + e >= columns) continue;
             const int n = tile.n0 + c + e;
-            float y = zs[e] * (by * __ldg(p.column_scales + n));
+            float y = scaled(zs[e], by, __ldg(p.column_scales + n));
             if (p.bias) y += to_float(static_cast<const T*>(p.bias)[n]);
             const Pair added = same(p.residual ? to_float(static_cast<const T*>(p.residual)[at + e]) : 0.0f);
             static_cast<T*>(p.out)[at + e] = from_float<T>(activated(p.activation, y, added));
@@ -846,7 +850,7 @@ __global__ void __launch_bounds__(FEW4_THREADS) few4_kernel(Few4Args a) {
 #pragma unroll
         for (int r = 0; r < M; ++r)
             if (r == m) scale = row_scale[r];
-        z = z * (scale * __ldg(a.row_scales + n));
+        z = scaled(z, scale, __ldg(a.row_scales + n));
         if (a.bias) z += to_float(static_cast<const T*>(a.bias)[n]);
         const long long at = (long long)m * a.outputs + n;
         const Pair added = same(a.residual ? to_float(static_cast<const T*>(a.residual)[at]) : 0.0f);
