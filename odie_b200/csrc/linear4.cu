@@ -684,7 +684,9 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
 // and by what one launch takes.  A warp has the rows n, n + 32, n + 64 and n + 96 of a tile of W, whose scales lie side by
 // side, and every `splits`-th 1024 values of K; the first of them are on their way while the block quantises x into shared
 // memory.  Products of codes are multiples of 1/4 of at most 36, and eight of them add up exactly in fp16: a block of 16 takes
-// eight packed products and one fp32 step with its scales.
+// eight packed products and one fp32 step with its scales.  The scales of blocks of 32 may leave fp32's range multiplied, where
+// a sum times them does not: their exponents are added and cut into halves, half an exponent a step (kept one bit below its
+// place in a float, the sum's upper bits are the half's).
 struct Few4Args {
     const void* x;
     const uint8_t* codes;
@@ -782,7 +784,7 @@ __global__ void __launch_bounds__(FEW4_THREADS) few4_kernel(Few4Args a) {
             if (u >= runs) continue;
             *reinterpret_cast<uint2*>(x_codes + m * a.pitch + u * 8) = codes;
             if (BLOCK == 16) x_scales[m * per_row + u] = scale_value<BLOCK>(scale);
-            else if (u % 2 == 0) x_scales[m * per_row + u / 2] = scale_value<BLOCK>(scale);
+            else if (u % 2 == 0) x_scales[m * per_row + u / 2] = __uint_as_float(scale << 22);
         }
     }
     __syncthreads();
@@ -819,14 +821,21 @@ __global__ void __launch_bounds__(FEW4_THREADS) few4_kernel(Few4Args a) {
                 halves_of(words[q][2 * b], h);
                 halves_of(words[q][2 * b + 1], h + 4);
                 const uint32_t at = BLOCK == 16 ? (c / 16 + b) % 4 : c / 32 % 4;
-                const float scale = scale_value<BLOCK>(bytes[q] >> (at * 8) & 0xffu);
+                const uint32_t byte = bytes[q] >> (at * 8) & 0xffu;
+                const float scale = BLOCK == 16 ? scale_value<BLOCK>(byte) : 0.0f;
 #pragma unroll
                 for (int m = 0; m < M; ++m) {
                     __half2 dot = __hmul2(h[0], x[m][0]);
 #pragma unroll
                     for (int i = 1; i < 8; ++i) dot = __hfma2(h[i], x[m][i], dot);
                     const float2 d = __half22float2(dot);
-                    sum[q][m] = fmaf(d.x + d.y, scale * by[m], sum[q][m]);
+                    if constexpr (BLOCK == 16) {
+                        sum[q][m] = fmaf(d.x + d.y, scale * by[m], sum[q][m]);
+                    } else {
+                        const uint32_t both_scales = (byte << 22) + __float_as_uint(by[m]);
+                        const float half = __uint_as_float(both_scales & 0x7f800000u), other = __uint_as_float((both_scales + 0x400000u) & 0x7f800000u);
+                        sum[q][m] = fmaf((d.x + d.y) * half, other, sum[q][m]);
+                    }
                 }
             }
         }

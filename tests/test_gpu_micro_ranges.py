@@ -84,7 +84,22 @@ def test_nothing_of_far_scales_is_nothing(cuda, rows, inputs, outputs, sizes):
     x, weight, _, _, offsets = made(rows, inputs, outputs, sizes, 120, 30, rows)
     x[:, 1::2] = 0
     weight[..., ::2] = 0
-    for block in (16,) if rows <= 2 else (16, 32):
+    for block in (16, 32):
         y = linear4(x, quantize(weight if sizes else weight[0], block=block), offsets=offsets)
         assert (y == 0).all(), (block, y.isnan().sum().item())
 
+
+@pytest.mark.parametrize('rows', [1, 2, 3, 300])
+@pytest.mark.parametrize('inputs, at', [(32, 5), (2100, 2077)])
+def test_scales_of_blocks(cuda, rows, inputs, at):
+    """Blocks of 32: the scales of a row's block and a weight's are 2^124 and 2^4 (their largest values meet zeros), the one
+    product 2^126; and with 2^-124 and 2^-4, 2^-130."""
+    from odie_b200.experts import linear4, quantize
+    block = at // 32 * 32
+    for sign in (1, -1):
+        x, w = (torch.zeros((n, inputs), dtype=torch.float64, device='cuda') for n in (rows, 40))
+        x[:, block], x[:, at] = 2.0 ** (126 if sign > 0 else -122), 2.0 ** (123 if sign > 0 else -125)
+        w[:, block + 1], w[:, at] = 2.0 ** (6 if sign > 0 else -2), 2.0 ** (3 if sign > 0 else -5)
+        micro = quantize(w.bfloat16(), block=32)
+        y = linear4(x.bfloat16(), micro)
+        assert (y.double() == 2.0 ** (126 if sign > 0 else -130)).all(), y
