@@ -245,15 +245,32 @@ class ExpertHeads(nn.Module):
 
 class MicroHeads(nn.Module):
     """The heads of an ExpertHeads with weights in 4 bits, as they are now: `linear4` in the place of `linear`, without
-    gradients; called like ExpertHeads."""
+    gradients; called like ExpertHeads.  Its buffers are all that it needs: a state dict of it is loaded into the
+    4-bit form, of the same block, of any heads of the same sizes.  Casts leave weights and their scales as they are."""
 
     def __init__(self, heads, block=16):
         super().__init__()
+        self.experts, self.block = heads.experts, int(block)
+        self.widths = [w.shape[-1] for w in heads.weights]
         with torch.no_grad():
-            self.experts = heads.experts
-            self.weights = [quantize(w, block=block) for w in heads.weights]
-            self.biases = [b.to(torch.float16) for b in heads.biases]
-            self.codes = None if heads.codes is None else heads.codes.to(torch.float16)
+            for i, (w, b) in enumerate(zip(heads.weights, heads.biases)):
+                micro = quantize(w, block=block)
+                self.register_buffer(f'weight{i}', micro.codes)
+                self.register_buffer(f'scales{i}_{block}', micro.scales)  # named by the block: those of another do not fit
+                self.register_buffer(f'row_scales{i}', micro.row_scales.view(torch.int32))  # as bits: a module's casts are for floats
+                self.register_buffer(f'bias{i}', b.to(torch.float16))
+            self.register_buffer('codes', None if heads.codes is None else heads.codes.to(torch.float16))
+
+    @property
+    def weights(self):
+        """The layers' weights, a Micro each."""
+        b = self._buffers
+        return [Micro(b[f'weight{i}'], b[f'scales{i}_{self.block}'], b[f'row_scales{i}'].view(torch.float32), width, self.block)
+                for i, width in enumerate(self.widths)]
+
+    @property
+    def biases(self):
+        return [self._buffers[f'bias{i}'].to(torch.float16) for i in range(len(self.widths))]
 
     @torch.no_grad()
     def forward(self, features, expert, weights=None, ids=None):
@@ -261,11 +278,11 @@ class MicroHeads(nn.Module):
             raise ValueError('ids go with codes')
         h = features.to(torch.float16)
         if ids is not None:
-            h = h + embed(ids, self.codes)
+            h = h + embed(ids, self.codes).to(torch.float16)
         order = sort_rows(expert, self.experts)
         h = dispatch(h, order)
         for i, (w, b) in enumerate(zip(self.weights, self.biases)):
-            h = linear4(h, w, b, offsets=order.offsets, activation='relu' if i + 1 < len(self.weights) else 'none')
+            h = linear4(h, w, b, offsets=order.offsets, activation='relu' if i + 1 < len(self.widths) else 'none')
         return combine(h, order, weights)
 
 
