@@ -245,7 +245,7 @@ class ExpertHeads(nn.Module):
 
 class MicroHeads(nn.Module):
     """The heads of an ExpertHeads with weights in 4 bits, as they are now: `linear4` in the place of `linear`, without
-    gradients; called like ExpertHeads.  Its buffers are all that it needs: a state dict of it is loaded into the
+    gradients; called like ExpertHeads.  Its buffers are copies, and all that it needs: a state dict of it is loaded into the
     4-bit form, of the same block, of any heads of the same sizes.  Casts leave weights and their scales as they are."""
 
     def __init__(self, heads, block=16):
@@ -258,8 +258,8 @@ class MicroHeads(nn.Module):
                 self.register_buffer(f'weight{i}', micro.codes)
                 self.register_buffer(f'scales{i}_{block}', micro.scales)  # named by the block: those of another do not fit
                 self.register_buffer(f'row_scales{i}', micro.row_scales.view(torch.int32))  # as bits: a module's casts are for floats
-                self.register_buffer(f'bias{i}', b.to(torch.float16))
-            self.register_buffer('codes', None if heads.codes is None else heads.codes.to(torch.float16))
+                self.register_buffer(f'bias{i}', b.to(torch.float16, copy=True))
+            self.register_buffer('codes', None if heads.codes is None else heads.codes.to(torch.float16, copy=True))
 
     @property
     def weights(self):

@@ -1,4 +1,4 @@
-"""MicroHeads as a module: what it holds is saved, loaded, moved and copied."""
+"""MicroHeads as a module: what it holds is saved, loaded, moved and copied, and is its own."""
 import copy
 import io
 
@@ -62,3 +62,18 @@ def test_moved_and_copied(cuda):
     for cast in (lambda m: m.half(), lambda m: m.float()):  # fp16 is what it has; the scales of 4-bit rows are no numbers to cast
         assert torch.equal(cast(micro)(*a), want)
     assert not list(micro.parameters()) and not micro(*a).requires_grad
+
+
+@pytest.mark.parametrize('half', [False, True])
+def test_what_it_holds_is_its_own(cuda, half):
+    """Heads that change afterwards, also fp16 ones, do not change their 4-bit form."""
+    a = arguments()
+    heads = made(4)
+    if half:
+        heads.half()
+    micro = heads.microscaled()
+    want = micro(*a)
+    with torch.no_grad():
+        for p in heads.parameters():
+            p.mul_(3)
+    assert torch.equal(micro(*a), want)
