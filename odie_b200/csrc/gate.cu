@@ -334,12 +334,14 @@ __global__ void __launch_bounds__(LOGIT_THREADS) gate_backward_kernel(GateArgs a
         rows[spread(mine + chosen[q])] = d[q];
     }
 
+    bool finite = true;
     if (dense) {  // - scale p_e sum p g
         float top = group_max<LANES>(largest(v));
         if (top == NOTHING) top = 0.0f;
         const float total = group_sum<LANES>(powers(v, top)), share = total > 0.0f || total != total ? -sum * inverse_approx(total) : 0.0f;
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] *= share;
+        finite = fabsf(share) < INFINITY;
     } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) v[i] = 0.0f;
@@ -353,7 +355,19 @@ __global__ void __launch_bounds__(LOGIT_THREADS) gate_backward_kernel(GateArgs a
         v[c * 4 + 2] += add.z;
         v[c * 4 + 3] += add.w;
     }
-    if (inside) store_logits<T, V, LANES>(static_cast<T*>(a.d_logits), s, row, lane, v);
+    if (!inside) return;
+    store_logits<T, V, LANES>(static_cast<T*>(a.d_logits), s, row, lane, v);
+    if (finite) return;
+    // A row with an open NaN or infinity, or such a gradient: experts that are closed to it have none all the same.  (Here, with
+    // nothing in registers, it costs the other rows none of theirs.)
+#pragma unroll 1
+    for (int i = 0; i < V; ++i) {
+        const int e = run_at<LANES>(i / 8, lane) + i % 8;
+        if (e >= s.experts) continue;
+        const long long at = row * s.experts + e;
+        if (to_float(logits[at]) == NOTHING || (a.mask.at && a.mask.at[row * a.mask.row_step + e * a.mask.expert_step] == 0))
+            static_cast<T*>(a.d_logits)[at] = from_float<T>(0.0f);
+    }
 }
 
 template <typename F>
