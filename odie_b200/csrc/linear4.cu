@@ -884,7 +884,8 @@ bool pair_tiles(int64_t rows, int n, int groups) {
     return double(ceil_div(std::max<int64_t>(1, pairs), SMS / 2)) * 256 <= double(ceil_div(std::max<int64_t>(1, ones), SMS)) * 128 * 1.35;
 }
 
-// Without offsets, where 128 x 128 tiles leave SMs idle: the sum over K is cut into 2, 4 or 8 parts of at least four blocks.
+// Without offsets, where 128 x 128 tiles leave SMs idle: the sum over K is cut into up to 2, 4 or 8 parts, for which it has four
+// blocks each; all but the last are of the same, rounded up, number (17 blocks in four: 5, 5, 5, 2; 33 in eight: six of 5, one of 3).
 // (512 rows of 1024 -> 2048 in two parts of two blocks: 11.7 us, whole 7.7.  256 rows of 8192 -> 1024 in eight parts, for all
 // of whose clusters there is not room at a time: 20.5 us, in four 13.5.  64 rows of 4096 -> 4096: 10.6 us in four parts.)
 struct Splits4 {
