@@ -887,7 +887,7 @@ int* error_word() {
 int* checked_error_word() {
     int* word = error_word();
     if (__atomic_load_n(word, __ATOMIC_RELAXED) != 0 && __atomic_exchange_n(word, 0, __ATOMIC_RELAXED) != 0)
-        throw std::runtime_error("a wait of an earlier linear call on this device ran out: that call's results are incomplete");
+        throw std::runtime_error("a wait of an earlier linear or linear4 call on this device ran out: that call's results are incomplete");
     return word;
 }
 

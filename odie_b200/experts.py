@@ -85,7 +85,7 @@ def linear(x, weight, bias=None, residual=None, activation='none', offsets=None)
     2^20 inputs and outputs, 1024 experts and 2^31 - 257 rows.
 
     The kernels' waits are bounded (some ten seconds).  If one runs out, as on a device that has stopped answering, the
-    results are incomplete, and the next `linear` or gradient of it, or `check`, raises RuntimeError."""
+    results are incomplete, and the next `linear`, gradient of it or `linear4`, or `check`, raises RuntimeError."""
     code = ACTIVATIONS.get(activation)
     if code is None:
         raise ValueError(f'activation must be one of {", ".join(ACTIVATIONS)}')
@@ -194,11 +194,11 @@ def linear4(x, weight, bias=None, residual=None, activation='none', offsets=None
 
 
 def check(device=None):
-    """Wait for the device (the current one) and raise RuntimeError if a wait of `linear` has run out there that no call
+    """Wait for the device (the current one) and raise RuntimeError if a wait of `linear` or `linear4` has run out there that no call
     has raised for yet: after the last step of a program, say, or after replaying a captured graph."""
     with torch.cuda.device(device):
         torch.cuda.synchronize()
-        _lib.check(_lib.library().odie_linear_check(), 'linear')
+        _lib.check(_lib.library().odie_linear_check(), 'linear or linear4')
 
 
 # ---------------------------------------------------------------- a model of them

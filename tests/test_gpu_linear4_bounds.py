@@ -1,5 +1,5 @@
 """linear4 writes its results and its scratch and nothing beside them, whatever the offsets; sums over K in parts of unequal
-length; rows that are no numbers among rows of far scales."""
+length; rows that are no numbers among rows of far scales; what a wait that ran out is called."""
 import pytest
 import torch
 
@@ -83,3 +83,25 @@ def test_no_numbers_among_far_scales(cuda, rows, inputs, outputs):
     if rows > 1:
         want[5] = True
     assert torch.equal(bad, want)
+
+
+def test_a_wait_that_ran_out_is_named(cuda):
+    """What `linear` or `check` raise after a product in 4 bits does not send its reader to `linear` alone."""
+    from odie_b200 import _lib
+    from odie_b200.experts import check, linear, linear4, quantize
+    lib = _lib.library()
+    x = torch.randn((300, 512), device='cuda').half()
+    micro = quantize(torch.randn((600, 512), device='cuda'))
+    want = linear4(x, micro)
+    for call in (check, lambda: linear(x, x[:8])):
+        torch.cuda.synchronize()
+        assert lib.odie_linear_wait_limit(0) == 0
+        try:
+            linear4(x, micro)
+            torch.cuda.synchronize()
+        finally:
+            assert lib.odie_linear_wait_limit(-1) == 0
+        with pytest.raises(RuntimeError, match='linear4'):
+            call()
+        call()
+    assert torch.equal(linear4(x, micro), want)
