@@ -460,8 +460,9 @@ ODIE_API int odie_embed_backward(const void* ids, int id_bytes, int64_t n, const
  *
  * odie_gate: expert i32[rows][choices], weights f32[rows][choices]: the open
  * experts of the highest fp32(logit) + bias[e] (bias f32[experts], may be
- * NULL; NaN above all, -inf is not taken), ties to the lowest; -1 with weight
- * 0 where none is left.  weights: scale times the score (the bias is not in
+ * NULL; with either score it is added to the logit; NaN above all, a logit or
+ * sum of -inf is not taken), ties to the lowest; -1 with weight 0 where none
+ * is left.  weights: scale times the score (the bias is not in
  * it), with normalize divided by the sum over the row's choices.  Up to 64
  * choices, scale a normal fp32 number.
  * odie_gate_backward: d_logits[rows][experts] for d_weights

@@ -1,6 +1,6 @@
 // The experts of each row and their weights from a router's logits, and the weights' gradient.
 //
-//   key_e    = fp32(logit_e) + bias_e, for experts whose mask is on and whose key is not -inf
+//   key_e    = fp32(logit_e) + bias_e, for experts whose mask is on and of which neither logit nor key is -inf
 //   choices  = the k highest keys, ties to the lowest expert; -1 where none is left
 //   s_e      = softmax over the row (mask on), or sigmoid(logit_e)
 //   weight_j = scale s_j, or scale s_j / (sum of the chosen s)

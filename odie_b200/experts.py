@@ -115,8 +115,9 @@ def gate(logits, choices, bias=None, mask=None, score='softmax', normalize=True,
     """The experts of each row, and their weights, from a router's logits [rows, experts] (CUDA fp16, bf16 or fp32).
 
     A row takes its `choices` (up to 64) experts of the highest logit + bias (fp32; bias [experts], not differentiated),
-    ties to the lowest, among those whose mask (bool, broadcastable to the logits) is on and whose sum is not -inf; a
-    choice for which none is left is -1 with weight 0.  A NaN is taken first, and makes its row's weights NaN (a sigmoid
+    ties to the lowest, among those whose mask (bool, broadcastable to the logits) is on and of which neither logit nor sum is
+    -inf; a choice for which none is left is -1 with weight 0.  The bias is added to the logit, also with score 'sigmoid': a
+    router that was trained with a bias on its scores, sigmoid(logit) + bias, takes other experts here.  A NaN is taken first, and makes its row's weights NaN (a sigmoid
     without normalize: its own).  weights: scale times the softmax over the row's open experts, or the sigmoid of the
     logit, with `normalize` divided by its sum over the row's choices.  Differentiable in the logits through the weights.
     For sort_rows, dispatch and combine.  Up to 1024 experts."""
@@ -288,7 +289,8 @@ class MicroHeads(nn.Module):
 
 class ExpertRouter(nn.Module):
     """A learned choice of `choices` of `experts` for each row, for ExpertHeads: bf16 logits of one linear layer (fp16
-    would lose the gradient of a mean over many rows), `gate` and `balance`.  `shift` [experts] is added to the logits for
+    would lose the gradient of a mean over many rows; logits that round to one number are a tie, which goes to the lower
+    expert), `gate` and `balance`.  `shift` [experts] is added to the logits for
     the choice alone; it has no gradient, and a program may move it against the load."""
 
     def __init__(self, n_input, experts, choices, seed, score='softmax', normalize=True, device='cuda'):
