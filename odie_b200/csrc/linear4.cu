@@ -316,8 +316,7 @@ __global__ void __launch_bounds__(Shape4<CG, BN, BLOCK>::THREADS, 1)
     }
     if (warp == 2) tc::tmem_alloc_group<CG>(tmem_at, S::COLUMNS);
     if (warp == 3) {  // the groups' rows, tiles and tiles of scales
-        // The sums stop at what offsets in order can come to: others (overlapping groups) would pass 32 bits, and a tile's first
-        // row would be negative.
+        // The sums stop at what offsets in order can come to: others (overlapping groups) have more, up to what passes 32 bits.
         int tiles = 0, units = 0;
         const int most_units = p.a_tiles;
         for (int g0 = 0; g0 <= p.groups; g0 += 32) {
